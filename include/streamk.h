@@ -395,6 +395,86 @@ int sk_q4_quantize_host(const uint16_t *W, int64_t N, int64_t K, int64_t ldw, in
 int sk_q4_quantize(const void *W, int64_t N, int64_t K, int64_t ldw, int group, int zero, void *Wq,
                    void *scales, void *stream);
 
+/*
+ * int8 products with scales, and their quantiser.  No counterpart in the reference.
+ *
+ * sk_gemm_i8_scaled: C[m][n] = activation(a[m] * b[n] * sum_k A[m][k] B[n][k] + bias[n]) for int8 A [M,K] and B [N,K], one fp32
+ * scale for each row of A (token) and of B (output channel), C fp16 or bfloat16 (ldc in its elements).  The sums are exact int32;
+ * each becomes fp32 (rounded beyond 24 bits), is multiplied by a[m], then by b[n], and rounded once to C's type behind bias (C's
+ * type) and activation.  The plan is made with dtype SK_I8 as for sk_gemm_i8; SK_ERR_CONFIG for plans of kernels that have no form
+ * with scales (the general small-M kernels: a plan of up to 64 rows is made with reserved[0] = 9 or 12).  Every schedule and
+ * fix-up gives the same bits.  Alignment as for sk_gemm_i8; C 2-byte, the scales 4-byte aligned.
+ *
+ * sk_quantize_i8: rows of X (SK_F16 or SK_BF16, row pitch ldx elements, M x K) to int8 Q (pitch ldq) and one fp32 scale a row:
+ * scale = max |x| / 127, q = x / scale to the nearest integer (ties to even), at most 127 in magnitude.  A row of zeros has scale 0;
+ * one with an infinity or a NaN has scale NaN and q = 0, so that its products are NaN.  Any alignment and K; whole 16-byte pieces
+ * are the fast path.
+ */
+typedef struct sk_scales {
+  const void *a, *b;   /* fp32, M and N values */
+  int32_t out_dtype;   /* SK_F16 or SK_BF16 */
+  int32_t reserved;    /* 0 */
+} sk_scales;
+int sk_gemm_i8_scaled(const void *A, const void *B, void *C, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t ldc,
+                      const sk_scales *scales, const sk_plan *plan, void *ws, size_t ws_bytes, void *stream, const sk_epilogue *epi);
+int sk_quantize_i8(const void *X, int dtype, int64_t M, int64_t K, int64_t ldx, void *Q, int64_t ldq, void *scales, void *stream);
+
+/*
+ * Products grouped by expert.  No counterpart in the reference.
+ *
+ * sk_gemm_grouped: for offsets[e] <= r < offsets[e + 1]
+ *   C[r] = activation(A[r] * op(B[e]) + bias[e])          SK_F16, SK_BF16
+ *   C[r] = activation(scale_a[r] * scale_b[e][n] * (A[r] * B[e]^T)[n] + bias[e][n])      SK_I8, C in out_dtype
+ * offsets: E + 1 int32 in device memory, ascending from 0 to at most R (the host does not read them); groups of any size, zero
+ * included.  Rows that no group holds are set to zero.  Offsets are clamped to 0 .. R and to ascending order before they are used, so
+ * no content of theirs leads outside the operands.  B: E matrices, expert_b elements apart, each [N, K] (SK_LAYOUT_NT, pitch ldb) or
+ * [K, N] (SK_LAYOUT_NN, 16-bit types).  bias: [E, N] in C's type, contiguous, or null.  lda, ldb and expert_b multiples of 8 (int8:
+ * 16), SK_LAYOUT_NT: K too; SK_LAYOUT_NN: N too, and where K is none, A has zeros in its columns from K to the next; A and B 16-byte, C and bias 2-byte, scales 4-byte aligned.  The same bits on every launch.
+ *
+ * sk_grouped_wgrad: C[e] = sum over the rows r of group e of A[r]^T B[r] with A [R, M] and B [R, N] in SK_F16 or SK_BF16, C [E, M, N]
+ * contiguous in that type, sums in fp32; a group without rows gives zeros.  With A the gradient of a grouped product's result and B
+ * its rows this is the gradient of its weights; the gradient of its rows is sk_gemm_grouped with the other layout.  lda, ldb and N
+ * multiples of 8, M rounded up to one at most lda (A's padding columns are read, and not used); A and B 16-byte aligned.
+ */
+typedef struct sk_grouped {
+  int32_t dtype, layout, out_dtype, activation;   /* sk_dtype, sk_layout, sk_dtype (that of the operands but for SK_I8), sk_activation */
+  int64_t E, R, N, K;
+  const void *A, *B, *offsets;
+  void *C;
+  int64_t lda, ldb, ldc, expert_b;
+  const void *bias, *scale_a, *scale_b;
+  int64_t reserved[2];                            /* 0 */
+} sk_grouped;
+int sk_gemm_grouped(const sk_grouped *g, void *stream);
+int sk_grouped_wgrad(const void *A, const void *B, const void *offsets, void *C, int dtype, int64_t E, int64_t R, int64_t M, int64_t N,
+                     int64_t lda, int64_t ldb, void *stream);
+
+/*
+ * Routing of tokens to experts.  No counterpart in the reference.
+ *
+ * sk_route_experts: logits [T, E] (fp32, fp16 or bfloat16, pitch ld); E up to 1024, k up to 64.  For each token its k largest logits,
+ * the largest first, equal ones by number; -infinity and NaN are never chosen, and a token with fewer than k others has -1 as its last
+ * experts, with weight 0.  weights [T, k] fp32 = exp(z - max) / sum over the chosen.  Slot t * k + j is token t's j-th expert:
+ *   offsets [E + 1]  where each expert's rows begin when the slots are sorted by expert (stably); offsets[E]: how many have one
+ *   order [T * k]    the slot of each sorted row, -1 from offsets[E] on
+ *   place [T, k]     the sorted row of each slot, -1 without an expert
+ * (all int32).  ws: sk_route_workspace_bytes(T, E, k) of scratch (0 is possible), no initialisation needed.
+ * sk_route_backward: dlogits [T, E] (dtype, contiguous) of the weights' gradient dweights [T, k] fp32.
+ * sk_dispatch_rows: rows[p] = row order[p] / k of x, any type by bytes; zeros where order[p] is negative.
+ * sk_combine_rows: out[t] = sum over j of weights[t][j] * y[place[t][j]] (weights null: 1), SK_F16 or SK_BF16, [T * k, H] to [T, H],
+ * added in fp32 in the order of j.  With weights null it is the gradient of sk_dispatch_rows.
+ * sk_combine_backward: dy [T * k, H] (zeros for rows without a slot) and dweights [T, k] of sk_combine_rows.
+ */
+size_t sk_route_workspace_bytes(int64_t T, int64_t E, int64_t k);
+int sk_route_experts(const void *logits, int dtype, int64_t T, int64_t E, int64_t k, int64_t ld, void *weights, void *experts, void *offsets,
+                     void *order, void *place, void *ws, size_t ws_bytes, void *stream);
+int sk_route_backward(const void *weights, const void *experts, const void *dweights, int64_t T, int64_t E, int64_t k, int dtype,
+                      void *dlogits, void *stream);
+int sk_dispatch_rows(const void *x, int64_t row_bytes, int64_t x_pitch, const void *order, int64_t T, int64_t k, void *rows, void *stream);
+int sk_combine_rows(const void *y, int dtype, const void *place, const void *weights, int64_t T, int64_t k, int64_t H, void *out, void *stream);
+int sk_combine_backward(const void *d_out, const void *y, int dtype, const void *order, const void *place, const void *weights, int64_t T,
+                        int64_t k, int64_t H, void *dy, void *dweights, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

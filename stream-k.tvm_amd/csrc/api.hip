@@ -6,6 +6,7 @@
 
 #include "launch.h"
 #include "q4_dequant.h"
+#include "scaled_launch.h"
 #include "streamk.h"
 
 using namespace sk;
@@ -247,14 +248,15 @@ int make_dev_plan(const sk_plan *plan, const KernelInfo *k, void *ws, size_t ws_
   return SK_OK;
 }
 
-// family: 0 tile kernels, 1 small-M kernels, 2 fp32 kernels
+// family: 0 tile kernels, 1 small-M kernels, 2 fp32 kernels, 3 int8 kernels with scales (under the int8 kernels' ids)
 int cached_occupancy(int id, int family) {
-  static int cache[1024];
-  static bool have[1024];
-  const int slot = id & 1023;  // kernel ids stay below 1024
+  static int cache[2048];
+  static bool have[2048];
+  const int slot = (id & 1023) + (family == 3 ? 1024 : 0);  // kernel ids stay below 1024
   std::lock_guard<std::mutex> lock(g_mutex);
   if (!have[slot]) {
-    cache[slot] = family == 1 ? occupancy_skinny(id) : (family == 2 ? occupancy_f32(id) : occupancy_tile(id));
+    cache[slot] = family == 1 ? occupancy_skinny(id)
+                  : (family == 2 ? occupancy_f32(id) : (family == 3 ? occupancy_scaled_i8(id) : occupancy_tile(id)));
     have[slot] = true;
   }
   return cache[slot];
@@ -480,6 +482,34 @@ extern "C" int sk_gemm_i8(const void *A, const void *B, void *C, int64_t M, int6
                           int64_t lda, int64_t ldb, int64_t ldc, const sk_plan *plan, void *ws,
                           size_t ws_bytes, void *stream) {
   return gemm_8bit(SK_I8, A, B, C, M, N, K, lda, ldb, ldc, 1.f, plan, ws, ws_bytes, stream);
+}
+
+extern "C" int sk_gemm_i8_scaled(const void *A, const void *B, void *C, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb,
+                                 int64_t ldc, const sk_scales *scales, const sk_plan *plan, void *ws, size_t ws_bytes, void *stream,
+                                 const sk_epilogue *epi) {
+  const void *bias = nullptr;
+  if (int rc = epilogue_word(epi, &bias)) return rc;
+  if (!A || !B || !C || !scales || !scales->a || !scales->b) return SK_ERR_NULL;
+  if ((scales->out_dtype != SK_F16 && scales->out_dtype != SK_BF16) || scales->reserved) return SK_ERR_CONFIG;
+  int rc = check_plan(plan, M, N, K, SK_I8, SK_LAYOUT_NT);
+  if (rc) return rc;
+  if (lda < K || ldb < K || ldc < N) return SK_ERR_SHAPE;
+  if ((K % 16) || (lda % 16) || (ldb % 16)) return SK_ERR_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(A) & 15) || (reinterpret_cast<uintptr_t>(B) & 15) || (reinterpret_cast<uintptr_t>(C) & 1) ||
+      (reinterpret_cast<uintptr_t>(scales->a) & 3) || (reinterpret_cast<uintptr_t>(scales->b) & 3))
+    return SK_ERR_ALIGN;
+  const KernelInfo *k = kernel_by_id(plan->kernel_id);
+  if (!k || k->dtype != SK_I8) return SK_ERR_CONFIG;
+  if (lda * k->bm >= (int64_t)1 << 31 || ldb * k->bn >= (int64_t)1 << 31) return SK_ERR_SHAPE;
+  const int occupancy = cached_occupancy(k->id, 3);
+  if (occupancy <= 0) return SK_ERR_CONFIG;   // (an int8 kernel without an instance with scales)
+  DevPlan dp;
+  Workspace w;
+  rc = make_dev_plan(plan, k, ws, ws_bytes, occupancy, (hipStream_t)stream, &dp, &w);
+  if (rc) return rc;
+  GemmArgs a{(const half_t *)A, (const half_t *)B, (half_t *)C, (int)M, (int)N, (int)(K / 2), lda / 2, ldb / 2, ldc, 1.f};
+  const Scales sc{(const float *)scales->a, (const float *)scales->b, scales->out_dtype == SK_BF16};
+  return launch_scaled_i8(k->id, a, sc, dp, w, (hipStream_t)stream, bias) == 0 ? SK_OK : SK_ERR_LAUNCH;
 }
 
 extern "C" int sk_gemm_f32(const void *A, const void *B, void *C, int64_t M, int64_t N, int64_t K,

@@ -1,0 +1,35 @@
+// Between the C ABI and the units that hold the grouped kernels.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include "grouped.h"
+
+namespace sk {
+
+enum GroupedType { GT_F16 = 0, GT_BF16 = 1, GT_I8 = 2 };
+struct GroupedShape {
+  int type;      // GroupedType
+  bool nn;       // weights [E, K, N]
+  int64_t E, R, N, K;   // (K in elements)
+  int cus;
+};
+// the most row tiles that R rows in E groups (and the two of rows without an expert) can make: every group has one tile that is not
+// full, and no tile is without a row
+static inline int64_t grouped_tiles(const GroupedShape &h, int bm) {
+  const int64_t by_size = h.R / bm + h.E + 2;
+  return by_size < h.R ? by_size : h.R;
+}
+// hipError_t as int
+int launch_grouped(const GroupedArgs &g, const GroupedShape &h, hipStream_t s);
+
+struct WgradArgs {
+  const half_t *dC, *A;   // [R, N] (width readable columns), [R, K]
+  half_t *dW;             // [E, N, K]
+  const int *offsets;
+  int64_t lddc, lda;
+  int E, R, N, K, width;
+  int tiles_m, tiles_n, grid;
+};
+int launch_wgrad(const WgradArgs &g, bool bf16, int cus, hipStream_t s);
+
+}  // namespace sk

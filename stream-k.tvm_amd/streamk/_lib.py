@@ -45,6 +45,20 @@ class SkEpilogue(ctypes.Structure):
     _fields_ = [("bias", ctypes.c_void_p), ("activation", ctypes.c_int64), ("reserved", ctypes.c_int64 * 2)]
 
 
+class SkScales(ctypes.Structure):
+    """sk_scales: the scales of an int8 product and its result's type."""
+    _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("out_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class SkGrouped(ctypes.Structure):
+    """sk_grouped: a product grouped by expert."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "layout", "out_dtype", "activation")] + [
+        (n, ctypes.c_int64) for n in ("E", "R", "N", "K")] + [
+        (n, ctypes.c_void_p) for n in ("A", "B", "offsets", "C")] + [
+        (n, ctypes.c_int64) for n in ("lda", "ldb", "ldc", "expert_b")] + [
+        (n, ctypes.c_void_p) for n in ("bias", "scale_a", "scale_b")] + [("reserved", ctypes.c_int64 * 2)]
+
+
 class StreamKError(RuntimeError):
     def __init__(self, status, where):
         self.status = status
@@ -122,6 +136,20 @@ def lib():
     L.sk_q4_tile.argtypes = [vp, i64, i64, vp, vp]
     for f in ("sk_q4_pack_host", "sk_q4_unpack_host", "sk_q4_quantize_host", "sk_q4_quantize", "sk_q4_tile_host",
               "sk_q4_untile_host", "sk_q4_tile"):
+        getattr(L, f).restype = ci
+    L.sk_gemm_i8_scaled.argtypes = [vp, vp, vp, i64, i64, i64, i64, i64, i64, P(SkScales), P(SkPlan), vp, sz, vp, P(SkEpilogue)]
+    L.sk_quantize_i8.argtypes = [vp, ci, i64, i64, i64, vp, i64, vp, vp]
+    L.sk_gemm_grouped.argtypes = [P(SkGrouped), vp]
+    L.sk_grouped_wgrad.argtypes = [vp, vp, vp, vp, ci, i64, i64, i64, i64, i64, i64, vp]
+    L.sk_route_workspace_bytes.argtypes = [i64, i64, i64]
+    L.sk_route_workspace_bytes.restype = sz
+    L.sk_route_experts.argtypes = [vp, ci, i64, i64, i64, i64, vp, vp, vp, vp, vp, vp, sz, vp]
+    L.sk_route_backward.argtypes = [vp, vp, vp, i64, i64, i64, ci, vp, vp]
+    L.sk_dispatch_rows.argtypes = [vp, i64, i64, vp, i64, i64, vp, vp]
+    L.sk_combine_rows.argtypes = [vp, ci, vp, vp, i64, i64, i64, vp, vp]
+    L.sk_combine_backward.argtypes = [vp, vp, ci, vp, vp, vp, i64, i64, i64, vp, vp, vp]
+    for f in ("sk_gemm_i8_scaled", "sk_quantize_i8", "sk_gemm_grouped", "sk_grouped_wgrad", "sk_route_experts", "sk_route_backward",
+              "sk_dispatch_rows", "sk_combine_rows", "sk_combine_backward"):
         getattr(L, f).restype = ci
     for f in ("sk_device_info", "sk_make_plan", "sk_plan_cta_range", "sk_plan_tile_coords",
               "sk_workspace_init", "sk_workspace_status", "sk_gemm_f16", "sk_gemm_f32",

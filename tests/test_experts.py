@@ -1,0 +1,468 @@
+"""The operators of a mixture of experts against 64-bit arithmetic: grouped products and their gradients, routing, dispatch, combination.
+
+Tolerances of products: fp32 sums of n terms, in any order, are within 2 n 2^-24 of the sum of the terms' magnitudes (an MFMA may cut
+instead of rounding: hence the 2), plus one rounding to the result's type (2^-8 of bfloat16, 2^-11 of fp16, 2^-24 absolute below
+fp16's normal numbers); bias and activation as in the int8 tests: 4e-6 of the value in front of the activation and of one."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+TYPES = {"float16": torch.float16, "bfloat16": torch.bfloat16}
+ROUNDING = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+
+
+@pytest.fixture(scope="module")
+def sk():
+    import streamk
+    streamk.lib()
+    return streamk
+
+
+def activate(x, name):
+    return {None: lambda v: v, "relu": torch.relu, "silu": lambda v: v * torch.sigmoid(v),
+            "gelu_tanh": lambda v: 0.5 * v * (1 + torch.tanh(math.sqrt(2 / math.pi) * (v + 0.044715 * v ** 3)))}[name](x)
+
+
+def assert_near(C, want, terms, magnitudes, pre=None):
+    tol = ROUNDING[C.dtype] * want.abs() * 1.001 + 1.2 * 2 * terms * 2.0 ** -24 * magnitudes + 2.0 ** -24
+    if pre is not None:
+        tol = tol + 4e-6 * (pre.abs() + 1)
+    off = (C.double() - want).abs()
+    assert torch.isfinite(C).all()
+    assert (off <= tol).all(), f"largest excess {(off - tol).max().item():.3g} of {int((off > tol).sum())} values"
+
+
+def offsets_of(sizes):
+    return torch.tensor([0] + torch.tensor(sizes).cumsum(0).tolist(), dtype=torch.int32, device="cuda")
+
+
+def groups(sizes):
+    start = 0
+    for e, n in enumerate(sizes):
+        yield e, slice(start, start + n)
+        start += n
+
+
+def rand(shape, dtype, seed, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * std).to(dtype).cuda()
+
+
+def plain(A, B, sizes, layout="nt"):
+    """(product, sums of magnitudes) in 64 bits; zeros for rows behind the last group"""
+    a, b = A.double(), B.double() if layout == "nt" else B.double().transpose(1, 2)
+    y = torch.zeros(A.shape[0], b.shape[1], dtype=torch.float64, device="cuda")
+    m = torch.zeros_like(y)
+    for e, at in groups(sizes):
+        y[at], m[at] = a[at] @ b[e].T, a[at].abs() @ b[e].abs().T
+    return y, m
+
+
+SIZES = {"one": [1], "empty": [0, 0, 0], "single rows": [1, 0, 1, 1], "ragged": [3, 0, 17, 129, 1, 64], "one expert has all": [0, 300, 0, 0],
+         "whole tiles": [128, 256, 128], "seventy experts": [(7 * i) % 11 for i in range(70)], "large": [700, 513, 1, 900]}
+
+
+# ---- the grouped product ----
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("layout", ["nt", "nn"])
+@pytest.mark.parametrize("sizes", sorted(SIZES))
+@pytest.mark.parametrize("N,K", [(136, 72), (8, 8), (520, 256), (256, 512)])
+def test_grouped_product(sk, dtype, layout, sizes, N, K):
+    sizes = SIZES[sizes]
+    R, E = sum(sizes) + 5, len(sizes)   # (five rows that no expert owns)
+    A, B = rand((R, K), TYPES[dtype], R), rand((E, N, K) if layout == "nt" else (E, K, N), TYPES[dtype], N, 1 / math.sqrt(K))
+    C = sk.streamk_grouped(A, B, offsets_of(sizes), layout=layout)
+    want, magnitudes = plain(A, B, sizes, layout)
+    assert_near(C, want, K, magnitudes)
+    assert not C[R - 5:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K", [(1, 8), (77, 64), (131, 1032), (2049, 192)])
+def test_grouped_product_of_odd_widths(sk, N, K):
+    sizes = [5, 0, 40, 200]
+    A, B = rand((245, K), torch.float16, 1), rand((4, N, K), torch.float16, 2, 1 / math.sqrt(K))
+    want, magnitudes = plain(A, B, sizes)
+    assert_near(sk.streamk_grouped(A, B, offsets_of(sizes)), want, K, magnitudes)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("activation", [None, "relu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("rows", [6, 90, 2000])
+def test_grouped_epilogue(sk, rows, activation):
+    sizes = [rows // 2, 0, rows - rows // 2]
+    A, B, bias = rand((rows, 128), torch.bfloat16, 3), rand((3, 200, 128), torch.bfloat16, 4, 0.1), rand((3, 200), torch.bfloat16, 5)
+    C = sk.streamk_grouped(A, B, offsets_of(sizes), bias=bias, activation=activation)
+    pre, magnitudes = plain(A, B, sizes)
+    for e, at in groups(sizes):
+        pre[at] += bias[e].double()
+    assert_near(C, activate(pre, activation), 128, 1.2 * magnitudes, pre)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", sorted(TYPES))
+@pytest.mark.parametrize("sizes", sorted(SIZES))
+@pytest.mark.parametrize("N,K", [(136, 80), (515, 1040), (256, 256)])
+def test_grouped_int8(sk, out, sizes, N, K):
+    sizes = SIZES[sizes]
+    R, E = sum(sizes) + 3, len(sizes)
+    g = torch.Generator().manual_seed(R + N)
+    A = torch.randint(-127, 128, (R, K), generator=g, dtype=torch.int8).cuda()
+    B = torch.randint(-127, 128, (E, N, K), generator=g, dtype=torch.int8).cuda()
+    sa, sb = (torch.rand(R, generator=g) + 0.5).cuda() * 0.01, (torch.rand(E, N, generator=g) + 0.5).cuda() / (73 * math.sqrt(K))
+    bias = rand((E, N), TYPES[out], 7)
+    C = sk.streamk_grouped(A, B, offsets_of(sizes), scale_a=sa, scale_b=sb, out_dtype=TYPES[out], bias=bias, activation="silu")
+    pre, _ = plain(A, B, sizes)
+    pre *= sa.double()[:, None]
+    for e, at in groups(sizes):
+        pre[at] = pre[at] * sb[e].double() + bias[e].double()
+    assert_near(C, activate(pre, "silu"), 0, 0, pre)
+    assert not C[R - 3:].any()
+
+
+@pytest.mark.gpu
+def test_grouped_views_and_out(sk):
+    sizes = [30, 0, 41, 100]
+    A, B = rand((171, 96), torch.float16, 1), rand((4, 72, 96), torch.float16, 2, 0.1)
+    offsets = offsets_of(sizes)
+    want = sk.streamk_grouped(A, B, offsets)
+    wide_a = torch.zeros(171, 160, dtype=torch.float16, device="cuda")
+    wide_a[:, 16:112] = A
+    wide_b = torch.zeros(4, 80, 128, dtype=torch.float16, device="cuda")
+    wide_b[:, :72, :96] = B
+    assert torch.equal(sk.streamk_grouped(wide_a[:, 16:112], wide_b[:, :72, :96], offsets), want)
+    shifted = torch.zeros(171, 97, dtype=torch.float16, device="cuda")
+    shifted[:, 1:] = A
+    assert torch.equal(sk.streamk_grouped(shifted[:, 1:], B, offsets), want)
+    assert torch.equal(sk.streamk_grouped(A, B[:1].expand(4, 72, 96), offsets), sk.streamk_grouped(A, B[:1].repeat(4, 1, 1), offsets))
+    out = torch.full((171, 79), 7.0, dtype=torch.float16, device="cuda")
+    sk.streamk_grouped(A, B, offsets, out=out[:, 3:75])
+    assert torch.equal(out[:, 3:75], want) and (out[:, :3] == 7).all() and (out[:, 75:] == 7).all()
+    assert sk.streamk_grouped(A[:0], B, torch.zeros_like(offsets)).shape == (0, 72)
+    one = sk.streamk_grouped(A[:1], B, offsets_of([0, 1, 0, 0]))
+    assert_near(one, *[t for t in (plain(A[:1], B, [0, 1, 0, 0])[0], 96, plain(A[:1], B, [0, 1, 0, 0])[1])])
+
+
+@pytest.mark.gpu
+def test_values_of_other_experts_do_not_leak(sk):
+    """NaN and infinities in the rows and weights around a group leave its results alone."""
+    sizes = [20, 7, 40]
+    A, B = rand((67, 64), torch.bfloat16, 1), rand((3, 48, 64), torch.bfloat16, 2)
+    clean = sk.streamk_grouped(A, B, offsets_of(sizes))
+    A[:20], A[27:] = math.nan, math.inf
+    B[0], B[2] = math.inf, math.nan
+    dirty = sk.streamk_grouped(A, B, offsets_of(sizes))
+    assert torch.equal(dirty[20:27], clean[20:27]) and not torch.isfinite(dirty[:20]).any() and not torch.isfinite(dirty[27:]).any()
+
+
+@pytest.mark.gpu
+def test_grouped_on_another_stream_and_in_a_graph(sk):
+    A, B = rand((300, 256), torch.float16, 1), rand((5, 256, 256), torch.float16, 2, 0.1)
+    offsets = offsets_of([50, 0, 100, 150, 0])
+    want = sk.streamk_grouped(A, B, offsets)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        assert torch.equal(sk.streamk_grouped(A, B, offsets), want)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        C = sk.streamk_grouped(A, B, offsets)
+    for sizes in ([50, 0, 100, 150, 0], [0, 0, 0, 0, 300], [1, 2, 3, 4, 5], [60, 60, 60, 60, 60]):
+        offsets.copy_(offsets_of(sizes))   # other groups in the same graph: the host does not know the sizes
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(C, sk.streamk_grouped(A, B, offsets))
+
+
+# ---- its gradients ----
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("sizes", sorted(SIZES))
+@pytest.mark.parametrize("M,N", [(136, 72), (77, 8), (520, 264), (256, 256)])
+def test_weight_gradient(sk, dtype, sizes, M, N):
+    sizes = SIZES[sizes]
+    R, E = sum(sizes) + 4, len(sizes)
+    dC, A = rand((R, M), TYPES[dtype], R), rand((R, N), TYPES[dtype], N)
+    got = sk.streamk_grouped_wgrad(dC, A, offsets_of(sizes))
+    assert got.shape == (E, M, N) and got.dtype == TYPES[dtype]
+    for e, at in groups(sizes):
+        want = dC[at].double().T @ A[at].double()
+        assert_near(got[e], want, sizes[e], dC[at].double().abs().T @ A[at].double().abs())
+
+
+@pytest.mark.gpu
+def test_weight_gradient_ignores_other_groups_rows(sk):
+    sizes = [20, 7, 40]
+    dC, A = rand((67, 40), torch.float16, 1), rand((67, 64), torch.float16, 2)
+    clean = sk.streamk_grouped_wgrad(dC, A, offsets_of(sizes))
+    dC[:20], A[27:] = math.nan, math.inf
+    assert torch.equal(sk.streamk_grouped_wgrad(dC, A, offsets_of(sizes))[1], clean[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("layout,N,K", [("nt", 72, 136), ("nt", 77, 64), ("nn", 72, 136), ("nt", 264, 520)])
+def test_gradients_of_the_product(sk, dtype, layout, N, K):
+    """Against the formulas, and against differences: the product is linear in each operand, so that f(A + V) - f(A - V) is exactly
+    2 <dA, V> but for roundings (of f's values to 16 bits, of dA's)."""
+    sizes = [33, 0, 130, 5]
+    R, t = sum(sizes) + 2, TYPES[dtype]
+    A, B = rand((R, K), t, 1), rand((4, N, K) if layout == "nt" else (4, K, N), t, 2, 0.1)
+    dC = rand((R, N), t, 3)
+    offsets = offsets_of(sizes)
+    A.requires_grad_()
+    B.requires_grad_()
+    C = sk.streamk_grouped(A, B, offsets, layout=layout)
+    dA, dB = torch.autograd.grad(C, (A, B), dC)
+    A, B = A.detach(), B.detach()
+    b = B.double() if layout == "nt" else B.double().transpose(1, 2)
+    for e, at in groups(sizes):
+        assert_near(dA[at], dC[at].double() @ b[e], N, dC[at].double().abs() @ b[e].abs())
+        want, m = dC[at].double().T @ A[at].double(), dC[at].double().abs().T @ A[at].double().abs()
+        if layout == "nn":
+            want, m = want.T, m.T
+        assert_near(dB[e], want, sizes[e], m)
+    assert not dA[R - 2:].any()
+    V, W = rand(A.shape, t, 4), rand(B.shape, t, 5, 0.1)
+    value = lambda a, w: (sk.streamk_grouped(a, w, offsets, layout=layout).double() * dC.double()).sum()  # noqa: E731
+    u = ROUNDING[t]
+    for got, x, v, f in ((dA, A, V, lambda z: value(z, B)), (dB, B, W, lambda z: value(A, z))):
+        up, down = (x + v), (x - v)   # (rounded: the step is what they differ by)
+        step = up.double() - down.double()
+        terms = (sk.streamk_grouped(up if x is A else A, up if x is B else B, offsets, layout=layout).double().abs() * dC.double().abs()).sum()
+        # roundings are independent: 6 standard deviations of the sum, bounded by the root of the number of terms; u / sqrt 3 each
+        bound = 6 * u * terms * 2 / math.sqrt(R * N) + 6 * u * (got.double().abs() * step.abs()).sum() / math.sqrt(got.numel())
+        assert abs(f(up) - f(down) - (got.double() * step).sum()) <= bound
+
+
+@pytest.mark.gpu
+def test_only_the_gradient_that_is_asked_for(sk):
+    A, B, offsets = rand((20, 64), torch.float16, 1), rand((2, 32, 64), torch.float16, 2), offsets_of([12, 8])
+    B.requires_grad_()
+    C = sk.streamk_grouped(A, B, offsets)
+    C.sum().backward()
+    assert A.grad is None and B.grad.shape == B.shape     # (an expanded gradient too: sum's)
+    with pytest.raises(ValueError):
+        sk.streamk_grouped(A, B, offsets, activation="silu")
+    with torch.no_grad():
+        sk.streamk_grouped(A, B, offsets, activation="silu")
+
+
+# ---- routing ----
+def plain_route(logits, k):
+    """Token by token, in Python."""
+    T, E = logits.shape
+    weights, experts = torch.zeros(T, k, dtype=torch.float64), torch.full((T, k), -1, dtype=torch.int32)
+    rows = [[] for _ in range(E)]
+    for t, z in enumerate(logits.double().tolist()):
+        best = sorted((e for e in range(E) if z[e] > -math.inf), key=lambda e: (-z[e], e))[:k]
+        p = [math.exp(z[e] - z[best[0]]) for e in best]
+        for j, e in enumerate(best):
+            weights[t, j], experts[t, j] = p[j] / sum(p), e
+            rows[e].append(t * k + j)
+    order = [s for r in rows for s in r]
+    offsets = [0]
+    for r in rows:
+        offsets.append(offsets[-1] + len(r))
+    place = torch.full((T * k,), -1, dtype=torch.int32)
+    for p, s in enumerate(order):
+        place[s] = p
+    return weights, experts, offsets, order + [-1] * (T * k - len(order)), place.view(T, k)
+
+
+def assert_route(route, logits, k):
+    weights, experts, offsets, order, place = plain_route(logits.cpu(), k)
+    assert torch.equal(route.experts.cpu(), experts)
+    assert route.offsets.tolist() == offsets and route.order.tolist() == order
+    assert torch.equal(route.place.cpu(), place)
+    # exp and the sum of at most 64 terms in fp32: 64 half units and the exponential's two
+    assert ((route.weights.cpu().double() - weights).abs() <= 66 * 2.0 ** -24 * weights + 1e-38).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,E,k", [(1, 1, 1), (1, 8, 2), (5, 3, 3), (63, 64, 8), (64, 256, 8), (65, 65, 4), (64, 300, 2), (200, 1000, 64), (1000, 128, 6), (3001, 17, 5), (17, 1024, 10)])
+def test_route(sk, T, E, k):
+    g = torch.Generator().manual_seed(T * E + k)
+    logits = (torch.randn(T, E, generator=g) * 2).bfloat16().float()   # (coarse: equal ones)
+    assert_route(sk.route_experts(logits.cuda(), k), logits, k)
+    closed = torch.rand(T, E, generator=g) < 0.6
+    closed[::7] = True
+    masked = logits.masked_fill(closed, -math.inf)
+    assert_route(sk.route_experts(masked.cuda(), k), masked, k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_route_of_special_values(sk, dtype):
+    low = torch.finfo(dtype).min
+    z = torch.tensor([[0.0, -0.0, 0.0, -0.0], [low, low, low, low], [low, 1, low, 1], [math.nan, 2, math.nan, 3], [math.nan] * 4, [-math.inf] * 4,
+                      [-math.inf, low, -math.inf, 5], [7, 7, 7, 7], [-1e-30, 1e-30, 0, -1]], dtype=dtype)
+    assert_route(sk.route_experts(z.cuda(), 3), z, 3)
+    r = sk.route_experts(z.cuda(), 3)
+    assert r.weights[1].tolist() == pytest.approx([1 / 3] * 3) and r.weights[4].tolist() == [0, 0, 0] and r.experts[0].tolist() == [0, 1, 2]
+    wide = torch.zeros(9, 11, dtype=dtype, device="cuda")
+    wide[:, 3:7] = z
+    for v in (wide[:, 3:7], wide[:, 3:7].t().contiguous().t()):
+        for a, b in zip(sk.route_experts(v, 3), r):
+            assert torch.equal(a, b)
+    empty = sk.route_experts(z[:0].cuda(), 2)
+    assert empty.weights.shape == (0, 2) and empty.offsets.tolist() == [0] * 5 and empty.order.shape == (0,)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T,E,k", [(5, 4, 2), (70, 300, 7), (1, 64, 64)])
+def test_route_gradient(sk, dtype, T, E, k):
+    g = torch.Generator().manual_seed(T)
+    z = (torch.randn(T, E, generator=g) * 2).to(dtype)
+    z[0, E // 2:] = -math.inf
+    if T > 2:
+        z[2] = -math.inf
+    dw = torch.randn(T, k, generator=g)
+    leaf = z.cuda().requires_grad_()
+    r = sk.route_experts(leaf, k)
+    got, = torch.autograd.grad(r.weights, leaf, dw.cuda())
+    assert got.dtype == dtype and got.shape == z.shape
+    # the formula in 64 bits on the same choice
+    w, e = plain_route(z, k)[:2]
+    dl = w * (dw.double() - (w * dw.double()).sum(1, keepdim=True))
+    want = torch.zeros(T, E, dtype=torch.float64).scatter_add_(1, e.clamp(min=0).long(), dl)
+    tol = (ROUNDING.get(dtype, 0.0) * want.abs() * 1.001 + 200 * 2.0 ** -24 * dw.abs().double().amax(1, keepdim=True) + (2.0 ** -24 if dtype == torch.float16 else 1e-37))
+    assert ((got.cpu().double() - want).abs() <= tol).all()
+    # differences of the weights in 64 bits, the choice held
+    h, v = 1e-6, torch.randn(T, E, generator=g).double()
+
+    def loss(x):
+        c = torch.where(e >= 0, x.gather(1, e.clamp(min=0).long()), -math.inf)
+        p = torch.where(e >= 0, torch.exp(c - c.max(1, keepdim=True).values.clamp(min=-1e300)), 0)
+        return ((p / p.sum(1, keepdim=True).clamp(min=1e-300)) * dw.double()).sum()
+    finite = torch.where(z.double() > -math.inf, z.double(), -1e4)
+    slope = (loss(finite + h * v) - loss(finite - h * v)) / (2 * h)
+    assert abs(slope - (want * v).sum()) <= 1e-6 * (1 + abs(slope))
+
+
+# ---- dispatch and combination ----
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("T,E,k,H", [(1, 4, 2, 64), (33, 8, 2, 520), (7, 3, 3, 1), (50, 16, 5, 77), (300, 64, 8, 4096), (64, 8, 1, 1000)])
+def test_dispatch_and_combine(sk, dtype, T, E, k, H):
+    t = TYPES[dtype]
+    z = rand((T, E), torch.float32, T)
+    z[rand((T, E), torch.float32, E) > 0.8] = -math.inf
+    z[::5] = -math.inf
+    route = sk.route_experts(z, k)
+    x, y = rand((T, H), t, 1), rand((T * k, H), t, 2)
+    rows = sk.dispatch_rows(x, route)
+    order, place, weights = route.order.long(), route.place.long(), route.weights.double()
+    assert torch.equal(rows, torch.where((order >= 0)[:, None], x[order.clamp(min=0) // k], 0))
+    used = (place >= 0)[..., None]
+    picked = torch.where(used, y.double()[place.clamp(min=0)], 0)
+    out = sk.combine_rows(y, route)
+    assert_near(out, (picked * weights[..., None]).sum(1), k, (picked * weights[..., None]).abs().sum(1))
+    assert not out[::5].any()
+    # gradients: formulas
+    x.requires_grad_()
+    y.requires_grad_()
+    route.weights.requires_grad_()
+    rows, out = sk.dispatch_rows(x, route), sk.combine_rows(y, route)
+    d_rows, d_out = rand((T * k, H), t, 3), rand((T, H), t, 4)
+    dx, dy, dw = torch.autograd.grad((rows, out), (x, y, route.weights), (d_rows, d_out))
+    g = torch.where(used, d_rows.double()[place.clamp(min=0)], 0)
+    assert_near(dx, g.sum(1), k, g.abs().sum(1))
+    flat = weights.view(-1)[order.clamp(min=0)][:, None] * d_out.double()[order.clamp(min=0) // k]
+    flat = torch.where((order >= 0)[:, None], flat, 0)
+    assert_near(dy, flat, 1, flat.abs())
+    terms = picked * d_out.double()[:, None, :]
+    assert ((dw.double() - terms.sum(2)).abs() <= 2 * H * 2.0 ** -24 * terms.abs().sum(2) + 1e-37).all()
+    # differences: the combination is linear in the weights
+    wv = torch.rand(T, k, generator=torch.Generator().manual_seed(9)).cuda() * used[..., 0]
+    moved = sk.combine_rows(y.detach(), route._replace(weights=route.weights.detach() + wv)).double() - out.detach().double()
+    m = ((picked.abs() * (weights + wv.double())[..., None]).sum(1) * d_out.double().abs()).sum()
+    assert abs((moved * d_out.double()).sum() - (dw.double() * wv.double()).sum()) <= 6 * ROUNDING[t] * 2 * m / math.sqrt(T * H) + 1e-6 * m
+
+
+@pytest.mark.gpu
+def test_dispatch_moves_any_type(sk):
+    route = sk.route_experts(rand((20, 4), torch.float32, 1), 2)
+    for x in (torch.randint(-128, 128, (20, 48), dtype=torch.int8, device="cuda"), torch.randn(20, device="cuda"), torch.randn(20, 3, device="cuda"),
+              torch.randint(-128, 128, (20, 13), dtype=torch.int8, device="cuda"), torch.randn(20, 64, device="cuda").half()[:, 8:40], torch.randn(6, 20, device="cuda").t()):
+        assert torch.equal(sk.dispatch_rows(x, route), x[route.order.long() // 2])
+    assert sk.dispatch_rows(torch.empty(0, 8, device="cuda"), sk.route_experts(torch.empty(0, 4, device="cuda"), 2)).shape == (0, 8)
+
+
+# ---- refusals ----
+def test_calls_are_refused_with_codes(sk):
+    L, lib = sk.lib(), __import__("streamk._lib", fromlist=["x"])
+    p = 1 << 12   # (an aligned address; every call below is refused before it is used)
+
+    def grouped(**kw):
+        d = dict(dtype=lib.SK_F16, layout=0, out_dtype=lib.SK_F16, activation=0, E=2, R=10, N=64, K=64, A=p, B=p, offsets=p, C=p, lda=64, ldb=64, ldc=64, expert_b=4096)
+        return L.sk_gemm_grouped(ctypes.byref(lib.SkGrouped(**{**d, **kw})), None)
+    assert L.sk_gemm_grouped(None, None) == -1
+    assert grouped(A=None) == -1 and grouped(offsets=None) == -1 and grouped(dtype=lib.SK_I8, out_dtype=0) == -1
+    for bad in (dict(dtype=lib.SK_F32, out_dtype=lib.SK_F32), dict(out_dtype=lib.SK_BF16), dict(layout=2), dict(activation=4), dict(scale_a=p), dict(activation=-1),
+                dict(dtype=lib.SK_I8, scale_a=p, scale_b=p, layout=1), dict(dtype=lib.SK_I8, scale_a=p, scale_b=p, out_dtype=lib.SK_F32)):
+        assert grouped(**bad) == -4, bad
+    for bad in (dict(E=0), dict(R=0), dict(N=0), dict(K=-8), dict(lda=56), dict(ldb=56), dict(ldc=63), dict(expert_b=-8), dict(R=1 << 31), dict(lda=1 << 40),
+                dict(layout=1, K=65, lda=64)):
+        assert grouped(**bad) == -2, bad
+    for bad in (dict(K=60), dict(lda=68), dict(ldb=68), dict(expert_b=4100), dict(A=p + 8), dict(B=p + 2), dict(C=p + 1), dict(offsets=p + 2), dict(bias=p + 1),
+                dict(layout=1, N=60), dict(dtype=lib.SK_I8, scale_a=p, scale_b=p, K=56)):
+        assert grouped(**bad) == -3, bad
+    wgrad = lambda A=p, dtype=0, E=2, R=5, M=64, N=64, lda=64, ldb=64: L.sk_grouped_wgrad(A, p, p, p, dtype, E, R, M, N, lda, ldb, None)  # noqa: E731
+    assert wgrad(A=None) == -1 and wgrad(dtype=lib.SK_I8) == -4 and wgrad(E=0) == -2 and wgrad(M=65, lda=64) == -2 and wgrad(N=60) == -3 and wgrad(A=p + 4) == -3
+    route = lambda logits=p, dtype=1, T=100, E=8, k=2, ld=8, ws=p, n=1 << 20: L.sk_route_experts(logits, dtype, T, E, k, ld, p, p, p, p, p, ws, n, None)  # noqa: E731
+    assert route(logits=None) == -1 and route(dtype=lib.SK_I8) == -4 and route(k=9) == -2 and route(E=1025, ld=1025) == -2 and route(ld=7) == -2 and route(T=0) == -2
+    assert route(n=4) == -5 and route(ws=None) == -5 and route(ws=p + 2) == -3
+    assert L.sk_route_workspace_bytes(16, 64, 8) == 0 and L.sk_route_workspace_bytes(100, 8, 2) > 0 and L.sk_route_workspace_bytes(100, 8, 9) == 0
+    assert L.sk_route_backward(p, p, None, 4, 8, 2, 1, p, None) == -1 and L.sk_route_backward(p, p, p, 4, 8, 9, 1, p, None) == -2
+    assert L.sk_dispatch_rows(p, 16, 8, p, 4, 2, p, None) == -2 and L.sk_dispatch_rows(None, 16, 16, p, 4, 2, p, None) == -1
+    assert L.sk_combine_rows(p, lib.SK_F32, p, p, 4, 2, 8, p, None) == -4 and L.sk_combine_rows(p, 0, p, p, 4, 2, 0, p, None) == -2
+    assert L.sk_combine_backward(p, p, 0, p, p, None, 4, 2, 8, p, p, None) == -1
+
+
+def test_fake_implementations(sk):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        new = lambda *s, dtype=torch.float16: torch.empty(*s, dtype=dtype, device="cuda")  # noqa: E731
+        off = new(4, dtype=torch.int32)
+        assert torch.ops.streamk.gemm_grouped(new(10, 64), new(3, 32, 64), off).shape == (10, 32)
+        assert torch.ops.streamk.gemm_grouped(new(10, 64), new(3, 64, 32), off, "nn").shape == (10, 32)
+        assert torch.ops.streamk.gemm_grouped(new(10, 64, dtype=torch.int8), new(3, 32, 64, dtype=torch.int8), off, "nt", torch.bfloat16).dtype == torch.bfloat16
+        assert torch.ops.streamk.grouped_wgrad(new(10, 32), new(10, 64), off).shape == (3, 32, 64)
+        w, e, o, order, place = torch.ops.streamk.route_experts(new(6, 3), 2)
+        assert w.shape == e.shape == place.shape == (6, 2) and o.shape == (4,) and order.shape == (12,) and w.dtype == torch.float32 and e.dtype == torch.int32
+        assert torch.ops.streamk.dispatch_rows(new(6, 64), order, 2).shape == (12, 64)
+        assert torch.ops.streamk.combine_rows(new(12, 64), place, w).shape == (6, 64)
+
+
+@pytest.mark.gpu
+def test_wrong_operands_are_refused(sk):
+    A, B, offsets = rand((20, 64), torch.float16, 1), rand((2, 32, 64), torch.float16, 2), offsets_of([12, 8])
+    i8 = lambda t: (t * 10).to(torch.int8)  # noqa: E731
+    for args, kw, error in [((A, B.bfloat16(), offsets), {}, TypeError), ((A.float(), B.float(), offsets), {}, TypeError), ((A, B[0], offsets), {}, ValueError),
+                            ((A, B, offsets.long()), {}, TypeError), ((A, B, offsets[:2]), {}, ValueError), ((A, B, offsets.cpu()), {}, TypeError),
+                            ((A[:, :32], B, offsets), {}, ValueError), ((A, B, offsets), dict(layout="tn"), ValueError), ((A, B, offsets), dict(activation="tanh"), ValueError),
+                            ((A, B, offsets), dict(bias=torch.zeros(32, device="cuda").half()), ValueError), ((A, B, offsets), dict(out_dtype=torch.bfloat16), ValueError),
+                            ((i8(A), i8(B), offsets), {}, ValueError), ((A, B, offsets), dict(scale_a=torch.ones(20, device="cuda")), ValueError),
+                            ((A, B, offsets), dict(out=torch.empty(20, 31, device="cuda").half()), ValueError), ((A[:, :60], B[:, :, :60], offsets), {}, sk.StreamKError),
+                            ((A, B.transpose(1, 2), offsets), dict(layout="nn"), ValueError)]:
+        with pytest.raises(error):
+            sk.streamk_grouped(*args, **kw)
+    with pytest.raises(ValueError):
+        sk.streamk_grouped_wgrad(A, A[:10], offsets)
+    with pytest.raises(ValueError):
+        sk.streamk_grouped_wgrad(A, A[:, :60], offsets)
+    for z, k, error in [(torch.zeros(4, 8, device="cuda"), 9, ValueError), (torch.zeros(4, 8, device="cuda"), 0, ValueError), (torch.zeros(4, 1025, device="cuda"), 2, ValueError),
+                        (torch.zeros(4, 8, device="cuda").double(), 2, TypeError), (torch.zeros(8, device="cuda"), 2, ValueError)]:
+        with pytest.raises(error):
+            sk.route_experts(z, k)
+    route = sk.route_experts(torch.zeros(4, 8, device="cuda"), 2)
+    with pytest.raises(ValueError):
+        sk.dispatch_rows(torch.zeros(5, 8, device="cuda"), route)
+    with pytest.raises(ValueError):
+        sk.combine_rows(torch.zeros(7, 8, device="cuda").half(), route)
