@@ -434,7 +434,9 @@ int sk_quantize_i8(const void *X, int dtype, int64_t M, int64_t K, int64_t ldx, 
  * sk_grouped_wgrad: C[e] = sum over the rows r of group e of A[r]^T B[r] with A [R, M] and B [R, N] in SK_F16 or SK_BF16, C [E, M, N]
  * contiguous in that type, sums in fp32; a group without rows gives zeros.  With A the gradient of a grouped product's result and B
  * its rows this is the gradient of its weights; the gradient of its rows is sk_gemm_grouped with the other layout.  lda, ldb and N
- * multiples of 8, M rounded up to one at most lda (A's padding columns are read, and not used); A and B 16-byte aligned.
+ * multiples of 8, M rounded up to one at most lda (A's padding columns are read, and not used); A and B 16-byte aligned.  variant: 0 by
+ * size; 1: 128 x 128 tiles; 2: 256 x 256 ((R + 64) lda and (R + 64) ldb below 2^30).
+ * A variant that does not exist or does not take the problem is refused with SK_ERR_CONFIG.
  */
 typedef struct sk_grouped {
   int32_t dtype, layout, out_dtype, activation;   /* sk_dtype, sk_layout, sk_dtype (that of the operands but for SK_I8), sk_activation */
@@ -443,11 +445,12 @@ typedef struct sk_grouped {
   void *C;
   int64_t lda, ldb, ldc, expert_b;
   const void *bias, *scale_a, *scale_b;
-  int64_t reserved[2];                            /* 0 */
+  int64_t variant;                                /* the tiles: 0 by size; 1: 128 x 128; 2: 256 x 256 (K a multiple of 64, int8: 128) */
+  int64_t reserved;                               /* 0 */
 } sk_grouped;
 int sk_gemm_grouped(const sk_grouped *g, void *stream);
 int sk_grouped_wgrad(const void *A, const void *B, const void *offsets, void *C, int dtype, int64_t E, int64_t R, int64_t M, int64_t N,
-                     int64_t lda, int64_t ldb, void *stream);
+                     int64_t lda, int64_t ldb, int variant, void *stream);
 
 /*
  * Routing of tokens to experts.  No counterpart in the reference.

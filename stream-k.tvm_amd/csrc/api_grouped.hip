@@ -9,6 +9,8 @@ using namespace sk;
 namespace {
 bool misaligned(const void *p, uintptr_t mask) { return (reinterpret_cast<uintptr_t>(p) & mask) != 0; }
 constexpr int64_t MAX_INT = 0x7fffff00;
+// (a variant that does not exist or does not take the problem)
+int status_of(int herr) { return herr == 0 ? SK_OK : (herr == (int)hipErrorNotSupported ? SK_ERR_CONFIG : SK_ERR_LAUNCH); }
 }  // namespace
 
 extern "C" int sk_gemm_grouped(const sk_grouped *g, void *stream) {
@@ -17,7 +19,7 @@ extern "C" int sk_gemm_grouped(const sk_grouped *g, void *stream) {
   if (!i8 && g->dtype != SK_F16 && g->dtype != SK_BF16) return SK_ERR_CONFIG;
   if ((!nn && g->layout != SK_LAYOUT_NT) || (nn && i8)) return SK_ERR_CONFIG;
   if (i8 ? g->out_dtype != SK_F16 && g->out_dtype != SK_BF16 : g->out_dtype != g->dtype) return SK_ERR_CONFIG;
-  if (g->activation < SK_ACT_NONE || g->activation > SK_ACT_SILU || g->reserved[0] || g->reserved[1]) return SK_ERR_CONFIG;
+  if (g->activation < SK_ACT_NONE || g->activation > SK_ACT_SILU || g->variant < 0 || g->reserved) return SK_ERR_CONFIG;
   if (i8 ? !g->scale_a || !g->scale_b : g->scale_a || g->scale_b) return i8 ? SK_ERR_NULL : SK_ERR_CONFIG;
   if (g->E <= 0 || g->R <= 0 || g->N <= 0 || g->K <= 0 || g->E > (1 << 20) || g->R > MAX_INT || g->N > MAX_INT || g->K > MAX_INT) return SK_ERR_SHAPE;
   if (g->lda < (nn ? (g->K + 7) / 8 * 8 : g->K) || g->ldb < (nn ? g->N : g->K) || g->ldc < g->N || g->expert_b < 0) return SK_ERR_SHAPE;
@@ -27,7 +29,7 @@ extern "C" int sk_gemm_grouped(const sk_grouped *g, void *stream) {
       misaligned(g->scale_a, 3) || misaligned(g->scale_b, 3))
     return SK_ERR_ALIGN;
   if (reinterpret_cast<uintptr_t>(g->bias) >> EPI_ACT_SHIFT) return SK_ERR_CONFIG;   // not a device address
-  GroupedShape h{i8 ? GT_I8 : (g->dtype == SK_BF16 ? GT_BF16 : GT_F16), nn, g->E, g->R, g->N, g->K, 0};
+  GroupedShape h{i8 ? GT_I8 : (g->dtype == SK_BF16 ? GT_BF16 : GT_F16), nn, g->E, g->R, g->N, g->K, 0, (int)g->variant};
   // a tile's rows (NN: all K rows of an expert's weights) are addressed with 32-bit byte offsets
   const int64_t bytes = i8 ? 1 : 2;
   if (g->lda * bytes * 256 >= (int64_t)1 << 31 || g->ldb * bytes * (nn ? g->K + 64 : 256) >= (int64_t)1 << 31 || g->ldc * 2 * 256 >= (int64_t)1 << 31)
@@ -50,11 +52,12 @@ extern "C" int sk_gemm_grouped(const sk_grouped *g, void *stream) {
   a.N = (int)g->N;
   a.K = (int)(g->K / pairs);
   a.act = g->activation;
-  return launch_grouped(a, h, (hipStream_t)stream) == 0 ? SK_OK : SK_ERR_LAUNCH;
+  return status_of(launch_grouped(a, h, (hipStream_t)stream));
 }
 
 extern "C" int sk_grouped_wgrad(const void *A, const void *B, const void *offsets, void *C, int dtype, int64_t E, int64_t R, int64_t M,
-                                int64_t N, int64_t lda, int64_t ldb, void *stream) {
+                                int64_t N, int64_t lda, int64_t ldb, int variant, void *stream) {
+  if (variant < 0) return SK_ERR_CONFIG;
   if (dtype != SK_F16 && dtype != SK_BF16) return SK_ERR_CONFIG;
   if (!A || !B || !offsets || !C) return SK_ERR_NULL;
   if (E <= 0 || R <= 0 || M <= 0 || N <= 0 || E > (1 << 20) || R > MAX_INT || M > MAX_INT || N > MAX_INT) return SK_ERR_SHAPE;
@@ -78,5 +81,5 @@ extern "C" int sk_grouped_wgrad(const void *A, const void *B, const void *offset
   a.N = (int)M;
   a.K = (int)N;
   a.width = (int)width;
-  return launch_wgrad(a, dtype == SK_BF16, cus, (hipStream_t)stream) == 0 ? SK_OK : SK_ERR_LAUNCH;
+  return status_of(launch_wgrad(a, dtype == SK_BF16, cus, variant, (hipStream_t)stream));
 }

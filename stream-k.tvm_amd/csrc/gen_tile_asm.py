@@ -53,10 +53,15 @@ one of two global chunks: v121 for even x, v122 for odd x.  A 16-column block of
 8-byte reads per K-step (K-rows 8 g' .. + 3 and + 4 .. + 7 for lane group g'), from one address register per block
 (%[rbt0] .. %[rbt7]; the swizzle makes the blocks' addresses differ by an XOR, not a sum): K-step 1 is 32 rows =
 16384 bytes further.  Per iteration the global offset of B advances by %[kbs] = 64 rows.
+
+TN layout (A is [K, M], B is [K, N]; SK_TILE_ASM_*_TN): both halves of a stage are as the NN form's B, and A has its own address
+registers (%[rat0] .. %[rat7]), second lane offset (v123) and step (%[kas]).  Row groups 0-3 of an operand are the rows of K-step 0
+and groups 4-7 those of K-step 1, so here EARLY and LATE split a stage by K-step: the rows of K-step 0 are free once block 0 has read
+its late fragments, those of K-step 1 once block 1 has, and every block again carries eight loads.
 """
 
 A0, B0, A1, B1 = 128, 160, 192, 224     # first registers of the fragment buffers
-VOA, VOB, VOB1 = 120, 121, 122          # v120 / v121 (/ v122, NN: odd row groups of B): load offsets of this iteration
+VOA, VOB, VOB1, VOA1 = 120, 121, 122, 123   # v120 / v121 (/ v122, v123: odd row groups of B, of A, in the [K, ..] layouts): load offsets of this iteration
 S_IT, S_KA, S_KB, S_T, S_OOB, S_M0, S_LDS, S_T2 = 80, 81, 82, 83, 84, 85, 86, 87
 
 # Row groups of a wave's eight per operand (group x holds rows 8 (wave + 4 x) .. + 7 of the tile's 256): the EARLY ones
@@ -98,7 +103,7 @@ class LdsTracker:
         return f'"s_waitcnt lgkmcnt({min(allowed, 15)})'
 
 
-def load_parts(x, nn, voa, vob, vob1, lds, ka, kb, prev=None):
+def load_parts(x, nn, voa, vob, vob1, lds, ka, kb, prev=None, voa1=None):
     """load x of a stage: 0..7 row groups of A, 8..15 of B (a wave's groups are 4 KB apart in LDS).  Returns
     (instructions that go before the m0 write, the m0 write, the load); s[S_T] walks the global offsets of the
     groups -- `prev` is the group the walk comes from (None: x is the first of its operand in this sequence) --,
@@ -113,37 +118,41 @@ def load_parts(x, nn, voa, vob, vob1, lds, ka, kb, prev=None):
     lds_off = (x * 4096) if x < 8 else (32768 + (x - 8) * 4096)
     m0 = f'"s_add_u32 m0, {lds}, {lds_off}'
     if x < 8:
-        ld = f'"buffer_load_dwordx4 {voa}, %[rsa], s{S_T} offen lds'
+        ld = f'"buffer_load_dwordx4 {voa1 if (nn == "tn" and x % 2 == 1) else voa}, %[rsa], s{S_T} offen lds'
     else:
         ld = f'"buffer_load_dwordx4 {vob1 if (nn and x % 2 == 1) else vob}, %[rsb], s{S_T} offen lds'
     return pre, m0, ld
 
 
-def load_sequence(xs, nn, voa, vob, vob1, lds, ka, kb):
+def load_sequence(xs, nn, voa, vob, vob1, lds, ka, kb, voa1=None):
     """load_parts for the groups xs (ascending; A before B), with the walk chained through them"""
     out, prev = [], None
     for x in xs:
         if prev is not None and (prev < 8) != (x < 8):
             prev = None
-        out.append(load_parts(x, nn, voa, vob, vob1, lds, ka, kb, prev))
+        out.append(load_parts(x, nn, voa, vob, vob1, lds, ka, kb, prev, voa1))
         prev = x
     return out
 
 
 def early_groups(nn):
     """the loads that must have landed a block ahead of the others: rows of blocks 0-3 (NN: and all of B, whose loads
-    fill whole K-rows)"""
+    fill whole K-rows; TN: the rows of K-step 0)"""
+    if nn == "tn":
+        return [x for x in range(16) if x % 8 < 4]
     return list(EARLY_X) + ([8 + x for x in range(8)] if nn else [8 + x for x in EARLY_X])
 
 
 def late_groups(nn):
+    if nn == "tn":
+        return [x for x in range(16) if x % 8 >= 4]
     return list(LATE_X) + ([] if nn else [8 + x for x in LATE_X])
 
 
 def stage_loads_text(nn, xs):
     """the loads xs of one stage, back to back (operands: the stage's LDS address, global offsets and lane offsets)"""
     L = []
-    for pre, m0, ld in load_sequence(xs, nn, "%[voa]", "%[vob]", "%[vob1]", "%[lds]", "%[ga]", "%[gb]"):
+    for pre, m0, ld in load_sequence(xs, nn, "%[voa]", "%[vob]", "%[vob1]", "%[lds]", "%[ga]", "%[gb]", "%[voa1]"):
         L += pre + [m0, '"s_nop 0', ld]
     return L
 
@@ -154,6 +163,8 @@ def offsets_for(nn, ahead):
            f'"v_or_b32 v{VOA}, s{S_OOB}, %[voa]', f'"v_or_b32 v{VOB}, s{S_OOB}, %[vob]']
     if nn:
         out.append(f'"v_or_b32 v{VOB1}, s{S_OOB}, %[vob1]')
+    if nn == "tn":
+        out.append(f'"v_or_b32 v{VOA1}, s{S_OOB}, %[voa1]')
     return out
 
 
@@ -171,7 +182,7 @@ def spread(plan, groups, first, last):
 
 
 def loop_text(nn):
-    """The loop for the NT (nn = False) or the NN layout.  The two blocks of an iteration are built alike; block b
+    """The loop for the NT (nn = False), the NN (True) or the TN layout ("tn").  The two blocks of an iteration are built alike; block b
     (K-step b of iteration `it`, fragment set b, stage cur = it % 2, nxt the other one):
       top      reads of the LATE fragments (blocks 4-7 of A and B) of set b from cur -- their rows were the last to
                be loaded and are the last to be overwritten
@@ -183,6 +194,8 @@ def loop_text(nn):
     L = []
     e = L.append
     kb_step = "%[kbs]" if nn else "128"
+    tn = nn == "tn"
+    ka_step = "%[kas]" if tn else "128"
     order = mfma_order()
     n_early, n_late = len(early_groups(nn)), len(late_groups(nn))
 
@@ -192,6 +205,11 @@ def loop_text(nn):
 
     # fragment reads as (tags, texts); 16 rows of 128 bytes per block of A (NT: of B too)
     def read_a(i, kk):
+        if tn:
+            ab = A0 if kk == 0 else A1
+            return ([("A", kk, i)] * 2,
+                    [f'"ds_read_b64_tr_b16 v[{ab + 4 * i + 2 * h}:{ab + 4 * i + 2 * h + 1}], %[rat{i}] offset:{kk * 16384 + h * 2048}'
+                     for h in range(2)])
         ab, addr = (A0, "%[ra0]") if kk == 0 else (A1, "%[ra1]")
         return ([("A", kk, i)], [f'"ds_read_b128 v[{ab + 4 * i}:{ab + 4 * i + 3}], {addr} offset:{i * 2048}'])
 
@@ -214,7 +232,7 @@ def loop_text(nn):
     def load_groups(xs):
         """loads as rider groups: the scalar instructions of a load share a gap, the load has its own"""
         groups = []
-        for pre, m0, ld in load_sequence(xs, nn, f"v{VOA}", f"v{VOB}", f"v{VOB1}", f"s{S_LDS}", f"s{S_KA}", f"s{S_KB}"):
+        for pre, m0, ld in load_sequence(xs, nn, f"v{VOA}", f"v{VOB}", f"v{VOB1}", f"s{S_LDS}", f"s{S_KA}", f"s{S_KB}", f"v{VOA1}"):
             groups += [(None, pre + [m0]), (None, [ld])]
         return groups
 
@@ -237,7 +255,7 @@ def loop_text(nn):
     zero_accumulators(L)
     e(f'"s_mov_b32 s{S_IT}, 0')
     e(f'"s_xor_b32 s{S_LDS}, %[lds], 0x10000')
-    e(f'"s_add_u32 s{S_KA}, %[ga0], 128')
+    e(f'"s_add_u32 s{S_KA}, %[ga0], {ka_step}')
     e(f'"s_add_u32 s{S_KB}, %[gb0], {kb_step}')
     L.extend(offsets_for(nn, 1))
     # (the youngest vector memory operations are the early loads of the second stage; the first stage has landed)
@@ -261,7 +279,7 @@ def loop_text(nn):
         # the addresses of set 0 move to the other stage behind the reads at the top (block 1 reads the early fragments
         # of the next iteration with them); NN: one register per block of B serves both K-steps -- those of blocks 0-3
         # flip between the early reads of block 0 and of block 1, those of blocks 4-7 behind the top reads of block 1
-        spread(plan, [flip("%[ra0]")] + ([] if nn else [flip("%[rb0]")]), TOP, 63)
+        spread(plan, ([] if tn else [flip("%[ra0]")]) + ([] if nn else [flip("%[rb0]")]), TOP, 63)
         # both ways into the loop: the early fragments of set 0 may still be in flight
         block(0, LdsTracker(at_top), plan,
               [f'"s_waitcnt vmcnt({n_late}) lgkmcnt(0)', '"s_barrier'])       # (the early loads, issued a block ago, have landed)
@@ -270,19 +288,21 @@ def loop_text(nn):
         plan = {}
         for g, item in enumerate(late_reads(1)):
             plan[g] = item
-        state = [(None, [f'"s_add_u32 s{S_KA}, s{S_KA}, 128', f'"s_add_u32 s{S_KB}, s{S_KB}, {kb_step}']),
+        state = [(None, [f'"s_add_u32 s{S_KA}, s{S_KA}, {ka_step}', f'"s_add_u32 s{S_KB}, s{S_KB}, {kb_step}']),
                  (None, [f'"s_xor_b32 s{S_LDS}, s{S_LDS}, 0x10000', f'"s_add_u32 s{S_T2}, s{S_IT}, 2']),
                  (None, [f'"s_cmp_lt_u32 s{S_T2}, %[n]', f'"s_cselect_b32 s{S_OOB}, 0, 0x80000000'])]
         state += [(None, [t]) for t in offsets_for(nn, 2)[3:]]
         if nn:
             state += [flip(f"%[rbt{j}]") for j in range(4)]
+        if tn:
+            state += [flip(f"%[rat{i}]") for i in range(4)]
         for g, item in enumerate(state):
             plan[TOP + g] = item
         after_state = TOP + len(state)
         plan[63] = (None, [f'"s_add_u32 s{S_IT}, s{S_IT}, 1'])
         spread(plan, load_groups(early_groups(nn)), after_state, LD_LAST)
         spread(plan, early_reads(0), after_state, RD_LAST)
-        spread(plan, [flip("%[ra1]")] + ([flip(f"%[rbt{j}]") for j in range(4, 8)] if nn else [flip("%[rb1]")]), after_state, 62)
+        spread(plan, ([flip(f"%[rat{i}]") for i in range(4, 8)] if tn else [flip("%[ra1]")]) + ([flip(f"%[rbt{j}]") for j in range(4, 8)] if nn else [flip("%[rb1]")]), after_state, 62)
         block(1, LdsTracker(), plan,
               [f'"s_waitcnt vmcnt({n_early}) lgkmcnt(0)', '"s_barrier',           # (the late loads of iteration it + 1 have landed)
                f'"s_cmp_lt_u32 s{S_IT}, %[n]', '"s_cbranch_scc1 L_sk_loop%='])
@@ -472,16 +492,19 @@ def emit_macro(name, params, lines):
 
 def main():
     print("// Generated by gen_tile_asm.py -- do not edit; see that file for the register plan and the schedule.")
-    print("// SK_TILE_ASM_LOADS / _LOADS_NN: the 16 loads of one stage.  SK_TILE_ASM_LOOP(MF) / _LOOP_NN(MF): the loop for the")
-    print("// NT / NN layout, MF = the MFMA mnemonic as a string literal.  SK_TILE_ASM_LOOP_F8(MF, MOD): fp8 operands, MOD =")
+    print("// SK_TILE_ASM_LOADS / _LOADS_NN / _LOADS_TN: the 16 loads of one stage.  SK_TILE_ASM_LOOP(MF) / _LOOP_NN(MF) / _LOOP_TN(MF): the loop")
+    print("// for the NT / NN / TN layout, MF = the MFMA mnemonic as a string literal.  SK_TILE_ASM_LOOP_F8(MF, MOD): fp8 operands, MOD =")
     print("// the format modifiers of the MFMA (\"\" for e4m3).  SK_TILE_ASM_STORE_x(CVT): the epilogue that leaves the stages alone.")
     print("#pragma once")
     emit_macro("SK_TILE_ASM_LOADS", "", stage_loads_text(False, range(16)))
     emit_macro("SK_TILE_ASM_LOADS_NN", "", stage_loads_text(True, range(16)))
     emit_macro("SK_TILE_ASM_LOADS_EARLY", "", stage_loads_text(False, early_groups(False)))
     emit_macro("SK_TILE_ASM_LOADS_EARLY_NN", "", stage_loads_text(True, early_groups(True)))
+    emit_macro("SK_TILE_ASM_LOADS_TN", "", stage_loads_text("tn", range(16)))
+    emit_macro("SK_TILE_ASM_LOADS_EARLY_TN", "", stage_loads_text("tn", early_groups("tn")))
     emit_macro("SK_TILE_ASM_LOOP", "(MF)", loop_text(False))
     emit_macro("SK_TILE_ASM_LOOP_NN", "(MF)", loop_text(True))
+    emit_macro("SK_TILE_ASM_LOOP_TN", "(MF)", loop_text("tn"))
     emit_macro("SK_TILE_ASM_LOOP_F8", "(MF, MOD)", loop_text_f8())
     for name, (ii0, ii1) in (("ALL", (0, 8)), ("HALF0", (0, 4)), ("HALF1", (4, 8))):
         emit_macro(f"SK_TILE_ASM_STORE_{name}", "(CVT)", store_text(ii0, ii1, False))

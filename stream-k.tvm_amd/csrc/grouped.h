@@ -31,6 +31,20 @@ struct GroupTile {
   int group, lo, rows, pm, pn;   // (group: 0 and E + 1 are no expert's)
 };
 
+// tile number `local` of a group of tm x tn: eight tiles down, then one to the right, so that CTAs which run together share rows of A
+// and of the weights
+__device__ __forceinline__ void group_raster(int local, int tm, int tn, int &pm, int &pn) {
+  if (tm == 1) {
+    pm = 0;
+    pn = local;
+    return;
+  }
+  const int q = (int)((unsigned)local / (unsigned)(8 * tn)), r = local - q * 8 * tn;
+  const int high = min(8, tm - 8 * q), c = (int)((unsigned)r / (unsigned)high);
+  pm = 8 * q + r - c * high;
+  pn = c;
+}
+
 template <int BM>
 struct GroupWalk {
   const int *offsets;
@@ -70,17 +84,7 @@ struct GroupWalk {
     t.group = 64 * chunk + i;
     t.lo = __builtin_amdgcn_readlane(lo, i);
     t.rows = __builtin_amdgcn_readlane(rows, i);
-    // eight tiles down, then one to the right: CTAs that run together share rows of A and of the weights
-    const int local = n - first, tm = (int)((unsigned)(t.rows + BM - 1) / BM);
-    if (tm == 1) {
-      t.pm = 0;
-      t.pn = local;
-    } else {
-      const int q = (int)((unsigned)local / (unsigned)(8 * tiles_n)), r = local - q * 8 * tiles_n;
-      const int high = min(8, tm - 8 * q), c = (int)((unsigned)r / (unsigned)high);
-      t.pm = 8 * q + r - c * high;
-      t.pn = c;
-    }
+    group_raster(n - first, (int)((unsigned)(t.rows + BM - 1) / BM), tiles_n, t.pm, t.pn);
     return true;
   }
 };

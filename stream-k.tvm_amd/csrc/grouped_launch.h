@@ -12,7 +12,10 @@ struct GroupedShape {
   bool nn;       // weights [E, K, N]
   int64_t E, R, N, K;   // (K in elements)
   int cus;
+  int variant;   // GroupedVariant
 };
+// which tiles (0: by the rule in kernels_grouped.hip)
+enum GroupedVariant { GV_RULE = 0, GV_TILE128 = 1, GV_ASM256 = 2, GV_LAST = GV_ASM256 };
 // the most row tiles that R rows in E groups (and the two of rows without an expert) can make: every group has one tile that is not
 // full, and no tile is without a row
 static inline int64_t grouped_tiles(const GroupedShape &h, int bm) {
@@ -30,6 +33,12 @@ struct WgradArgs {
   int E, R, N, K, width;
   int tiles_m, tiles_n, grid;
 };
-int launch_wgrad(const WgradArgs &g, bool bf16, int cus, hipStream_t s);
+int launch_wgrad(const WgradArgs &g, bool bf16, int cus, int variant, hipStream_t s);
+
+// the 256 x 256 tiles (kernels_grouped_asm.hip), and what they take
+bool grouped_asm_takes(const GroupedShape &h);
+int launch_grouped_asm(const GroupedArgs &g, const GroupedShape &h, hipStream_t s);
+bool wgrad_asm_takes(const WgradArgs &g);
+int launch_wgrad_asm(const WgradArgs &g, bool bf16, int cus, hipStream_t s);
 
 }  // namespace sk

@@ -11,6 +11,9 @@ __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_grouped_kernel(Grou
   run_grouped<P>(g, ipt, smem);
 }
 
+// Whether 256 x 256 tiles are ahead of 128 x 128.
+static bool large_tiles(const GroupedShape &h) { return h.R >= 128 * h.E; }
+
 template <class P>
 static int launch_grouped_policy(GroupedArgs g, const GroupedShape &h, hipStream_t s) {
   g.tiles_n = (g.N + P::BN - 1) / P::BN;
@@ -22,6 +25,8 @@ static int launch_grouped_policy(GroupedArgs g, const GroupedShape &h, hipStream
 }
 
 int launch_grouped(const GroupedArgs &g, const GroupedShape &h, hipStream_t s) {
+  if (h.variant > GV_LAST || (h.variant == GV_ASM256 && !grouped_asm_takes(h))) return (int)hipErrorNotSupported;
+  if (h.variant == GV_ASM256 || (h.variant == GV_RULE && grouped_asm_takes(h) && large_tiles(h))) return launch_grouped_asm(g, h, s);
   if (h.type == GT_I8) return launch_grouped_policy<ScaledDma<TileF16NTDma<128, 128, 2, 2, false, 64, true, false, 3>>>(g, h, s);
   if (h.nn) {
     if (h.type == GT_BF16) return launch_grouped_policy<TileF16NTDma<128, 128, 2, 2, true, 64, true, true>>(g, h, s);
@@ -38,9 +43,10 @@ __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_grouped_wgrad_kerne
   typename P::Acc acc;
   const int per_expert = g.tiles_m * g.tiles_n, total = g.E * per_expert;
   for (int tile = grouped_pid(g.grid); tile < total; tile += g.grid) {
-    const int e = tile / per_expert, local = tile - e * per_expert;
+    const int e = tile / per_expert;
     const int lo = min(max(g.offsets[e], 0), g.R), rows = min(max(g.offsets[e + 1], lo), g.R) - lo;
-    const int pm = local % g.tiles_m, pn = local / g.tiles_m;
+    int pm, pn;
+    group_raster(tile - e * per_expert, g.tiles_m, g.tiles_n, pm, pn);
     typename P::Args a;
     a.A = g.dC + (int64_t)lo * g.lddc;
     a.B = g.A + (int64_t)lo * g.lda;
@@ -69,7 +75,9 @@ static int launch_wgrad_policy(WgradArgs g, int cus, hipStream_t s) {
   return (int)hipGetLastError();
 }
 
-int launch_wgrad(const WgradArgs &g, bool bf16, int cus, hipStream_t s) {
+int launch_wgrad(const WgradArgs &g, bool bf16, int cus, int variant, hipStream_t s) {
+  if (variant > GV_ASM256 || (variant == GV_ASM256 && !wgrad_asm_takes(g))) return (int)hipErrorNotSupported;
+  if (variant == GV_ASM256 || (variant == GV_RULE && wgrad_asm_takes(g) && g.R >= 64 * g.E)) return launch_wgrad_asm(g, bf16, cus, s);
   return bf16 ? launch_wgrad_policy<TileTN<128, 128, 2, 2, true>>(g, cus, s) : launch_wgrad_policy<TileTN<128, 128, 2, 2, false>>(g, cus, s);
 }
 

@@ -56,7 +56,7 @@ class SkGrouped(ctypes.Structure):
         (n, ctypes.c_int64) for n in ("E", "R", "N", "K")] + [
         (n, ctypes.c_void_p) for n in ("A", "B", "offsets", "C")] + [
         (n, ctypes.c_int64) for n in ("lda", "ldb", "ldc", "expert_b")] + [
-        (n, ctypes.c_void_p) for n in ("bias", "scale_a", "scale_b")] + [("reserved", ctypes.c_int64 * 2)]
+        (n, ctypes.c_void_p) for n in ("bias", "scale_a", "scale_b")] + [("variant", ctypes.c_int64), ("reserved", ctypes.c_int64)]
 
 
 class StreamKError(RuntimeError):
@@ -140,7 +140,7 @@ def lib():
     L.sk_gemm_i8_scaled.argtypes = [vp, vp, vp, i64, i64, i64, i64, i64, i64, P(SkScales), P(SkPlan), vp, sz, vp, P(SkEpilogue)]
     L.sk_quantize_i8.argtypes = [vp, ci, i64, i64, i64, vp, i64, vp, vp]
     L.sk_gemm_grouped.argtypes = [P(SkGrouped), vp]
-    L.sk_grouped_wgrad.argtypes = [vp, vp, vp, vp, ci, i64, i64, i64, i64, i64, i64, vp]
+    L.sk_grouped_wgrad.argtypes = [vp, vp, vp, vp, ci, i64, i64, i64, i64, i64, i64, ci, vp]
     L.sk_route_workspace_bytes.argtypes = [i64, i64, i64]
     L.sk_route_workspace_bytes.restype = sz
     L.sk_route_experts.argtypes = [vp, ci, i64, i64, i64, i64, vp, vp, vp, vp, vp, vp, sz, vp]

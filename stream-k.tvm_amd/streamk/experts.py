@@ -47,7 +47,7 @@ def _pitch(t):
 
 
 # ---- the grouped product ----
-def _grouped(A, B, offsets, layout="nt", out_dtype=None, scale_a=None, scale_b=None, bias=None, activation="none", out=None):
+def _grouped(A, B, offsets, layout="nt", out_dtype=None, scale_a=None, scale_b=None, bias=None, activation="none", variant=0, out=None):
     if layout not in ("nt", "nn"):
         raise ValueError("layout must be 'nt' (B is [E, N, K]) or 'nn' (B is [E, K, N])")
     int8 = isinstance(A, torch.Tensor) and A.dtype == torch.int8
@@ -96,12 +96,12 @@ def _grouped(A, B, offsets, layout="nt", out_dtype=None, scale_a=None, scale_b=N
                        activation=_lib.ACTIVATIONS[activation], E=E, R=R, N=N, K=K, A=A.data_ptr(), B=B.data_ptr(),
                        offsets=offsets.data_ptr(), C=C.data_ptr(), lda=_pitch(A), ldb=ldb, ldc=max(C.stride(0), N),
                        expert_b=B.stride(0) if E > 1 else 0, bias=bias.data_ptr() if bias is not None else None,
-                       scale_a=scale_a.data_ptr() if int8 else None, scale_b=scale_b.data_ptr() if int8 else None)
+                       scale_a=scale_a.data_ptr() if int8 else None, scale_b=scale_b.data_ptr() if int8 else None, variant=variant)
     _lib.check(_lib.lib().sk_gemm_grouped(ctypes.byref(g), ops._stream_ptr()), "sk_gemm_grouped")
     return C
 
 
-_GROUPED_TAIL = "str layout=\"nt\", ScalarType? out_dtype=None, Tensor? scale_a=None, Tensor? scale_b=None, Tensor? bias=None, str activation=\"none\""
+_GROUPED_TAIL = "str layout=\"nt\", ScalarType? out_dtype=None, Tensor? scale_a=None, Tensor? scale_b=None, Tensor? bias=None, str activation=\"none\", int variant=0"
 _define(f"gemm_grouped(Tensor A, Tensor B, Tensor offsets, {_GROUPED_TAIL}) -> Tensor")
 _define(f"gemm_grouped_out(Tensor A, Tensor B, Tensor offsets, Tensor(a!) out, {_GROUPED_TAIL}) -> ()")
 
@@ -110,8 +110,8 @@ def _grouped_fake(A, B, offsets, layout="nt", out_dtype=None, *rest):
     return A.new_empty((A.shape[0], B.shape[1 if layout == "nt" else 2]), dtype=out_dtype or (torch.float16 if A.dtype == torch.int8 else A.dtype))
 
 
-def _grouped_out(A, B, offsets, out, layout="nt", out_dtype=None, scale_a=None, scale_b=None, bias=None, activation="none"):
-    _grouped(A, B, offsets, layout, out.dtype if out_dtype is None else out_dtype, scale_a, scale_b, bias, activation, out)
+def _grouped_out(A, B, offsets, out, layout="nt", out_dtype=None, scale_a=None, scale_b=None, bias=None, activation="none", variant=0):
+    _grouped(A, B, offsets, layout, out.dtype if out_dtype is None else out_dtype, scale_a, scale_b, bias, activation, variant, out)
 
 
 _implement("gemm_grouped", _grouped, _grouped_fake)
@@ -126,7 +126,7 @@ def _padded(t):
     return ops._aligned_rows(t)
 
 
-def _wgrad(A, B, offsets):
+def _wgrad(A, B, offsets, variant=0):
     _on_device(A, "A", tuple(_TYPES), 2)
     _on_device(B, "B", (A.dtype,), 2)
     if A.shape[0] != B.shape[0] or A.device != B.device:
@@ -143,13 +143,13 @@ def _wgrad(A, B, offsets):
         return C.zero_()
     A, B = _padded(A), ops._aligned_rows(B)
     rc = _lib.lib().sk_grouped_wgrad(A.data_ptr(), B.data_ptr(), offsets.data_ptr(), C.data_ptr(), _TYPES[C.dtype], E, A.shape[0], M, N, _pitch(A),
-                                     _pitch(B), ops._stream_ptr())
+                                     _pitch(B), variant, ops._stream_ptr())
     _lib.check(rc, "sk_grouped_wgrad")
     return C
 
 
-_define("grouped_wgrad(Tensor A, Tensor B, Tensor offsets) -> Tensor")
-_implement("grouped_wgrad", _wgrad, lambda A, B, offsets: A.new_empty((offsets.shape[0] - 1, A.shape[1], B.shape[1])))
+_define("grouped_wgrad(Tensor A, Tensor B, Tensor offsets, int variant=0) -> Tensor")
+_implement("grouped_wgrad", _wgrad, lambda A, B, offsets, variant=0: A.new_empty((offsets.shape[0] - 1, A.shape[1], B.shape[1])))
 
 
 class _GroupedProduct(torch.autograd.Function):
@@ -182,12 +182,13 @@ def _grouped_rows_grad(dC, B, offsets):
     return _ops.gemm_grouped(_padded(dC)[:, :N], B, offsets, "nn")
 
 
-def streamk_grouped(A, B, offsets, *, layout="nt", scale_a=None, scale_b=None, out_dtype=None, out=None, bias=None, activation=None):
+def streamk_grouped(A, B, offsets, *, layout="nt", scale_a=None, scale_b=None, out_dtype=None, out=None, bias=None, activation=None, variant=0):
     """Rows offsets[e] <= r < offsets[e + 1] of A [R, K] times the weights of expert e: C[r] = activation(A[r] @ B[e].T + bias[e]) for B
     [E, N, K] (layout 'nt'), A[r] @ B[e] for B [E, K, N] ('nn'); float16, bfloat16, or int8 ('nt') with scale_a [R] and scale_b
     [E, N] (float32), whose result is `out_dtype` (float16 by default).  offsets: int32 [E + 1] on the device, ascending from 0;
     groups of any size; rows behind the last group come out as zeros.  bias: [E, N] in C's type.  Sums in fp32 (int8: exact), rounded
-    once.  Differentiable in A and B without bias, activation, scales and out."""
+    once.  Differentiable in A and B without bias, activation, scales and out.  variant: which tiles run (sk_grouped in streamk.h); 0
+    lets the sizes decide."""
     activation = activation or "none"
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (A, B, bias, scale_a, scale_b)):
         if bias is not None or activation != "none" or scale_a is not None or scale_b is not None or out is not None:
@@ -196,15 +197,15 @@ def streamk_grouped(A, B, offsets, *, layout="nt", scale_a=None, scale_b=None, o
             raise ValueError(f"the result of {A.dtype} operands is {A.dtype}")
         return _GroupedProduct.apply(A, B, offsets, layout)
     if out is None:
-        return _ops.gemm_grouped(A, B, offsets, layout, out_dtype, scale_a, scale_b, bias, activation)
-    _ops.gemm_grouped_out(A, B, offsets, out, layout, out_dtype, scale_a, scale_b, bias, activation)
+        return _ops.gemm_grouped(A, B, offsets, layout, out_dtype, scale_a, scale_b, bias, activation, variant)
+    _ops.gemm_grouped_out(A, B, offsets, out, layout, out_dtype, scale_a, scale_b, bias, activation, variant)
     return out
 
 
-def streamk_grouped_wgrad(dC, A, offsets):
+def streamk_grouped_wgrad(dC, A, offsets, *, variant=0):
     """dB[e] = sum over the rows r of group e of dC[r]^T A[r]: [E, N, K] for dC [R, N] and A [R, K] (K a multiple of 8), the gradient of
-    streamk_grouped's weights ('nt'); fp32 sums, a group without rows gives zeros."""
-    return _ops.grouped_wgrad(dC, A, offsets)
+    streamk_grouped's weights ('nt'); fp32 sums, a group without rows gives zeros.  variant: sk_grouped_wgrad in streamk.h."""
+    return _ops.grouped_wgrad(dC, A, offsets, variant)
 
 
 # ---- routing ----

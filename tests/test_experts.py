@@ -413,7 +413,7 @@ def test_calls_are_refused_with_codes(sk):
     for bad in (dict(K=60), dict(lda=68), dict(ldb=68), dict(expert_b=4100), dict(A=p + 8), dict(B=p + 2), dict(C=p + 1), dict(offsets=p + 2), dict(bias=p + 1),
                 dict(layout=1, N=60), dict(dtype=lib.SK_I8, scale_a=p, scale_b=p, K=56)):
         assert grouped(**bad) == -3, bad
-    wgrad = lambda A=p, dtype=0, E=2, R=5, M=64, N=64, lda=64, ldb=64: L.sk_grouped_wgrad(A, p, p, p, dtype, E, R, M, N, lda, ldb, None)  # noqa: E731
+    wgrad = lambda A=p, dtype=0, E=2, R=5, M=64, N=64, lda=64, ldb=64: L.sk_grouped_wgrad(A, p, p, p, dtype, E, R, M, N, lda, ldb, 0, None)  # noqa: E731
     assert wgrad(A=None) == -1 and wgrad(dtype=lib.SK_I8) == -4 and wgrad(E=0) == -2 and wgrad(M=65, lda=64) == -2 and wgrad(N=60) == -3 and wgrad(A=p + 4) == -3
     route = lambda logits=p, dtype=1, T=100, E=8, k=2, ld=8, ws=p, n=1 << 20: L.sk_route_experts(logits, dtype, T, E, k, ld, p, p, p, p, p, ws, n, None)  # noqa: E731
     assert route(logits=None) == -1 and route(dtype=lib.SK_I8) == -4 and route(k=9) == -2 and route(E=1025, ld=1025) == -2 and route(ld=7) == -2 and route(T=0) == -2
@@ -466,3 +466,72 @@ def test_wrong_operands_are_refused(sk):
         sk.dispatch_rows(torch.zeros(5, 8, device="cuda"), route)
     with pytest.raises(ValueError):
         sk.combine_rows(torch.zeros(7, 8, device="cuda").half(), route)
+
+
+# ---- every kind of tile on every kind of groups ----
+VARIANTS = [1, 2]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", VARIANTS)
+@pytest.mark.parametrize("kind", ["float16 nt", "bfloat16 nt", "float16 nn", "bfloat16 nn", "int8"])
+@pytest.mark.parametrize("sizes", sorted(SIZES))
+@pytest.mark.parametrize("N,K,padding", [(520, 256, 0), (264, 128, 24), (1032, 640, 0)])
+def test_grouped_variants(sk, variant, kind, sizes, N, K, padding):
+    sizes = SIZES[sizes]
+    R, E = sum(sizes) + 2, len(sizes)
+    offsets = offsets_of(sizes)
+    out = torch.full((R, N + padding), 7.0, dtype=torch.bfloat16 if kind == "int8" else TYPES[kind.split()[0]], device="cuda")
+    bias = rand((E, N), out.dtype, 5)
+    if kind == "int8":
+        g = torch.Generator().manual_seed(R + N)
+        A = torch.randint(-127, 128, (R, K), generator=g, dtype=torch.int8).cuda()
+        B = torch.randint(-127, 128, (E, N, K), generator=g, dtype=torch.int8).cuda()
+        sa, sb = (torch.rand(R, generator=g) + 0.5).cuda() * 0.01, (torch.rand(E, N, generator=g) + 0.5).cuda() / (73 * math.sqrt(K))
+        run = lambda **kw: sk.streamk_grouped(A, B, offsets, scale_a=sa, scale_b=sb, variant=variant, **kw)  # noqa: E731
+        pre, magnitudes = plain(A, B, sizes)
+        pre, magnitudes = pre * sa.double()[:, None], 0
+        for e, at in groups(sizes):
+            pre[at] *= sb[e].double()
+    else:
+        layout = kind.split()[1]
+        A, B = rand((R, K), out.dtype, R), rand((E, N, K) if layout == "nt" else (E, K, N), out.dtype, N, 1 / math.sqrt(K))
+        run = lambda **kw: sk.streamk_grouped(A, B, offsets, layout=layout, variant=variant, **kw)  # noqa: E731
+        pre, magnitudes = plain(A, B, sizes, layout)
+    C = run(out_dtype=out.dtype)
+    assert_near(C, pre, K, magnitudes, pre)
+    assert not C[R - 2:].any()
+    for e, at in groups(sizes):
+        pre[at] += bias[e].double()
+    run(out=out[:, :N], bias=bias, activation="gelu_tanh")
+    want = activate(pre, "gelu_tanh")
+    want[R - 2:] = 0
+    assert_near(out[:, :N], want, K, 1.2 * magnitudes, pre)
+    assert (out[:, N:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", VARIANTS)
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("sizes", sorted(SIZES))
+@pytest.mark.parametrize("M,N", [(513, 264), (256, 520), (64, 8)])
+def test_weight_gradient_variants(sk, variant, dtype, sizes, M, N):
+    sizes = SIZES[sizes]
+    R = sum(sizes) + 3
+    dC, A = rand((R, M), TYPES[dtype], R), rand((R, N), TYPES[dtype], N)
+    got = sk.streamk_grouped_wgrad(dC, A, offsets_of(sizes), variant=variant)
+    for e, at in groups(sizes):
+        assert_near(got[e], dC[at].double().T @ A[at].double(), sizes[e], dC[at].double().abs().T @ A[at].double().abs())
+
+
+@pytest.mark.gpu
+def test_variants_that_do_not_take_a_problem_are_refused(sk):
+    A, B, offsets = rand((20, 72), torch.float16, 1), rand((2, 32, 72), torch.float16, 2), offsets_of([12, 8])
+    for variant in (2, 99, -1):
+        with pytest.raises(sk.StreamKError) as e:
+            sk.streamk_grouped(A, B, offsets, variant=variant)
+        assert e.value.status == -4
+    for variant in (99, -1):
+        with pytest.raises(sk.StreamKError) as e:
+            sk.streamk_grouped_wgrad(A, A, offsets, variant=variant)
+        assert e.value.status == -4
