@@ -430,6 +430,7 @@ int sk_quantize_i8(const void *X, int dtype, int64_t M, int64_t K, int64_t ldx, 
  * no content of theirs leads outside the operands.  B: E matrices, expert_b elements apart, each [N, K] (SK_LAYOUT_NT, pitch ldb) or
  * [K, N] (SK_LAYOUT_NN, 16-bit types).  bias: [E, N] in C's type, contiguous, or null.  lda, ldb and expert_b multiples of 8 (int8:
  * 16), SK_LAYOUT_NT: K too; SK_LAYOUT_NN: N too, and where K is none, A has zeros in its columns from K to the next; A and B 16-byte, C and bias 2-byte, scales 4-byte aligned.  The same bits on every launch.
+ * ws: as for the other products (sk_workspace_init has run on it); no launch waits for part of itself.
  *
  * sk_grouped_wgrad: C[e] = sum over the rows r of group e of A[r]^T B[r] with A [R, M] and B [R, N] in SK_F16 or SK_BF16, C [E, M, N]
  * contiguous in that type, sums in fp32; a group without rows gives zeros.  With A the gradient of a grouped product's result and B
@@ -445,10 +446,13 @@ typedef struct sk_grouped {
   void *C;
   int64_t lda, ldb, ldc, expert_b;
   const void *bias, *scale_a, *scale_b;
-  int64_t variant;                                /* the tiles: 0 by size; 1: 128 x 128; 2: 256 x 256 (K a multiple of 64, int8: 128) */
+  int64_t variant;                                /* the kernel: 0 by size; 1: 128 x 128 tiles; 2: 256 x 256 tiles (K a
+                                                     multiple of 64, int8: 128); 3, 4, 5 (SK_LAYOUT_NT): the weights streamed past 16, 32, 64
+                                                     rows at a time */
   int64_t reserved;                               /* 0 */
 } sk_grouped;
-int sk_gemm_grouped(const sk_grouped *g, void *stream);
+size_t sk_grouped_workspace_bytes(const sk_grouped *g);   /* for this shape and variant, on the current device; 0 is possible */
+int sk_gemm_grouped(const sk_grouped *g, void *ws, size_t ws_bytes, void *stream);
 int sk_grouped_wgrad(const void *A, const void *B, const void *offsets, void *C, int dtype, int64_t E, int64_t R, int64_t M, int64_t N,
                      int64_t lda, int64_t ldb, int variant, void *stream);
 

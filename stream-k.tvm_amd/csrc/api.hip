@@ -264,6 +264,23 @@ int cached_occupancy(int id, int family) {
 
 }  // namespace
 
+int sk::take_workspace(void *ws, size_t ws_bytes, size_t need, Workspace *w) {
+  *w = Workspace{nullptr, nullptr, nullptr};
+  if (need == 0) return SK_OK;
+  if (!ws || ws_bytes < need) return SK_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(ws) & 255) return SK_ERR_ALIGN;
+  {
+    std::lock_guard<std::mutex> lock(g_mutex);
+    auto it = g_ws.find(ws);
+    if (it == g_ws.end() || it->second.bytes < ws_bytes) return SK_ERR_WORKSPACE;  // sk_workspace_init was never run on it
+    if (it->second.poisoned) return SK_ERR_TIMEOUT;
+    it->second.maybe_dirty = true;
+  }
+  char *base = static_cast<char *>(ws);
+  *w = Workspace{reinterpret_cast<int *>(base), reinterpret_cast<int *>(base + 256), reinterpret_cast<float *>(base + WS_PART_OFF)};
+  return SK_OK;
+}
+
 extern "C" int sk_version(void) { return SK_VERSION; }
 
 extern "C" const char *sk_kernel_name(int kernel_id) {

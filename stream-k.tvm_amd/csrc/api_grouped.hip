@@ -2,6 +2,7 @@
 #include <hip/hip_runtime.h>
 
 #include "grouped_launch.h"
+#include "launch.h"
 #include "streamk.h"
 
 using namespace sk;
@@ -13,28 +14,43 @@ constexpr int64_t MAX_INT = 0x7fffff00;
 int status_of(int herr) { return herr == 0 ? SK_OK : (herr == (int)hipErrorNotSupported ? SK_ERR_CONFIG : SK_ERR_LAUNCH); }
 }  // namespace
 
-extern "C" int sk_gemm_grouped(const sk_grouped *g, void *stream) {
-  if (!g || !g->A || !g->B || !g->C || !g->offsets) return SK_ERR_NULL;
+// everything but the operands' addresses; fills h
+static int check_shape(const sk_grouped *g, GroupedShape *h) {
   const bool i8 = g->dtype == SK_I8, nn = g->layout == SK_LAYOUT_NN;
   if (!i8 && g->dtype != SK_F16 && g->dtype != SK_BF16) return SK_ERR_CONFIG;
   if ((!nn && g->layout != SK_LAYOUT_NT) || (nn && i8)) return SK_ERR_CONFIG;
   if (i8 ? g->out_dtype != SK_F16 && g->out_dtype != SK_BF16 : g->out_dtype != g->dtype) return SK_ERR_CONFIG;
   if (g->activation < SK_ACT_NONE || g->activation > SK_ACT_SILU || g->variant < 0 || g->reserved) return SK_ERR_CONFIG;
-  if (i8 ? !g->scale_a || !g->scale_b : g->scale_a || g->scale_b) return i8 ? SK_ERR_NULL : SK_ERR_CONFIG;
   if (g->E <= 0 || g->R <= 0 || g->N <= 0 || g->K <= 0 || g->E > (1 << 20) || g->R > MAX_INT || g->N > MAX_INT || g->K > MAX_INT) return SK_ERR_SHAPE;
   if (g->lda < (nn ? (g->K + 7) / 8 * 8 : g->K) || g->ldb < (nn ? g->N : g->K) || g->ldc < g->N || g->expert_b < 0) return SK_ERR_SHAPE;
   const int64_t step = i8 ? 16 : 8;
   if ((!nn && (g->K % step)) || (g->lda % step) || (g->ldb % step) || (g->expert_b % step) || (nn && (g->N % 8))) return SK_ERR_ALIGN;
-  if (misaligned(g->A, 15) || misaligned(g->B, 15) || misaligned(g->C, 1) || misaligned(g->bias, 1) || misaligned(g->offsets, 3) ||
-      misaligned(g->scale_a, 3) || misaligned(g->scale_b, 3))
-    return SK_ERR_ALIGN;
-  if (reinterpret_cast<uintptr_t>(g->bias) >> EPI_ACT_SHIFT) return SK_ERR_CONFIG;   // not a device address
-  GroupedShape h{i8 ? GT_I8 : (g->dtype == SK_BF16 ? GT_BF16 : GT_F16), nn, g->E, g->R, g->N, g->K, 0, (int)g->variant};
+  *h = GroupedShape{i8 ? GT_I8 : (g->dtype == SK_BF16 ? GT_BF16 : GT_F16), nn, g->E, g->R, g->N, g->K, 0, (int)g->variant};
   // a tile's rows (NN: all K rows of an expert's weights) are addressed with 32-bit byte offsets
   const int64_t bytes = i8 ? 1 : 2;
   if (g->lda * bytes * 256 >= (int64_t)1 << 31 || g->ldb * bytes * (nn ? g->K + 64 : 256) >= (int64_t)1 << 31 || g->ldc * 2 * 256 >= (int64_t)1 << 31)
     return SK_ERR_SHAPE;
+  return SK_OK;
+}
+
+extern "C" size_t sk_grouped_workspace_bytes(const sk_grouped *g) {
+  GroupedShape h;
+  return g && check_shape(g, &h) == SK_OK && sk_device_info(&h.cus, nullptr, nullptr) == SK_OK ? grouped_workspace(h) : 0;
+}
+
+extern "C" int sk_gemm_grouped(const sk_grouped *g, void *ws, size_t ws_bytes, void *stream) {
+  if (!g || !g->A || !g->B || !g->C || !g->offsets) return SK_ERR_NULL;
+  const bool i8 = g->dtype == SK_I8;
+  if (i8 ? !g->scale_a || !g->scale_b : g->scale_a || g->scale_b) return i8 ? SK_ERR_NULL : SK_ERR_CONFIG;
+  GroupedShape h;
+  if (int rc = check_shape(g, &h)) return rc;
+  if (misaligned(g->A, 15) || misaligned(g->B, 15) || misaligned(g->C, 1) || misaligned(g->bias, 1) || misaligned(g->offsets, 3) ||
+      misaligned(g->scale_a, 3) || misaligned(g->scale_b, 3))
+    return SK_ERR_ALIGN;
+  if (reinterpret_cast<uintptr_t>(g->bias) >> EPI_ACT_SHIFT) return SK_ERR_CONFIG;   // not a device address
   if (sk_device_info(&h.cus, nullptr, nullptr) != SK_OK) return SK_ERR_DEVICE;
+  Workspace w;
+  if (int rc = take_workspace(ws, ws_bytes, grouped_workspace(h), &w)) return rc;
   const int64_t pairs = i8 ? 2 : 1;
   GroupedArgs a{};
   a.A = (const half_t *)g->A;
@@ -52,7 +68,7 @@ extern "C" int sk_gemm_grouped(const sk_grouped *g, void *stream) {
   a.N = (int)g->N;
   a.K = (int)(g->K / pairs);
   a.act = g->activation;
-  return status_of(launch_grouped(a, h, (hipStream_t)stream));
+  return status_of(launch_grouped(a, h, w, (hipStream_t)stream));
 }
 
 extern "C" int sk_grouped_wgrad(const void *A, const void *B, const void *offsets, void *C, int dtype, int64_t E, int64_t R, int64_t M,

@@ -45,7 +45,8 @@ __device__ __forceinline__ void group_raster(int local, int tm, int tn, int &pm,
   pn = c;
 }
 
-template <int BM>
+// UNOWNED: groups 0 and E + 1 have tiles too
+template <int BM, bool UNOWNED = true>
 struct GroupWalk {
   const int *offsets;
   int E, R, tiles_n;
@@ -60,6 +61,7 @@ struct GroupWalk {
     if (g <= E + 1) {
       lo = g == 0 ? 0 : min(max(offsets[g - 1], 0), R);
       rows = (g == E + 1 ? R : min(max(offsets[g], lo), R)) - lo;
+      if (!UNOWNED && (g == 0 || g == E + 1)) rows = 0;
     }
     int x = (int)((unsigned)(rows + BM - 1) / BM) * tiles_n;
 #pragma unroll
@@ -68,6 +70,17 @@ struct GroupWalk {
       if (lane >= d) x += y;
     }
     ends = x;
+  }
+  // tiles of all groups (before the first find)
+  __device__ __forceinline__ int total_tiles() {
+    int sum = __builtin_amdgcn_readlane(ends, 63);
+    if (E + 1 < 64) return sum;
+    for (int c = 1; 64 * c <= E + 1; ++c) {
+      load(c);
+      sum += __builtin_amdgcn_readlane(ends, 63);
+    }
+    load(0);
+    return sum;
   }
   // the tile of this number, or false past the last one; numbers are asked for in ascending order
   __device__ __forceinline__ bool find(int tile, GroupTile &t) {

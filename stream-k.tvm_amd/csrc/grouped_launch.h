@@ -15,15 +15,21 @@ struct GroupedShape {
   int variant;   // GroupedVariant
 };
 // which tiles (0: by the rule in kernels_grouped.hip)
-enum GroupedVariant { GV_RULE = 0, GV_TILE128 = 1, GV_ASM256 = 2, GV_LAST = GV_ASM256 };
+enum GroupedVariant { GV_RULE = 0, GV_TILE128 = 1, GV_ASM256 = 2, GV_STREAM16 = 3, GV_STREAM32 = 4, GV_STREAM64 = 5 };
+// the variant that a call takes (never GV_RULE; what a caller asked for, if anything), and the workspace it needs
+int grouped_variant(const GroupedShape &h);
+size_t grouped_workspace(const GroupedShape &h);
 // the most row tiles that R rows in E groups (and the two of rows without an expert) can make: every group has one tile that is not
 // full, and no tile is without a row
 static inline int64_t grouped_tiles(const GroupedShape &h, int bm) {
   const int64_t by_size = h.R / bm + h.E + 2;
   return by_size < h.R ? by_size : h.R;
 }
-// hipError_t as int
-int launch_grouped(const GroupedArgs &g, const GroupedShape &h, hipStream_t s);
+// hipError_t as int; hipErrorNotSupported: h.variant does not exist or does not take the problem
+int launch_grouped(const GroupedArgs &g, const GroupedShape &h, const Workspace &ws, hipStream_t s);
+// few rows to an expert (kernels_grouped_stream.hip)
+size_t grouped_stream_workspace(int variant, int cus);
+int launch_grouped_stream(const GroupedArgs &g, const GroupedShape &h, const Workspace &ws, hipStream_t s);
 
 struct WgradArgs {
   const half_t *dC, *A;   // [R, N] (width readable columns), [R, K]

@@ -16,6 +16,10 @@
 
 namespace sk {
 
+// A caller's workspace (sk_workspace_init has run on it) for a launch that leaves partial sums in it, laid out; sk_status.  need 0:
+// nothing is taken.
+int take_workspace(void *ws, size_t ws_bytes, size_t need, Workspace *w);
+
 int tile_kernel_infos(KernelInfo *out, int max);
 int skinny_kernel_infos(KernelInfo *out, int max);
 

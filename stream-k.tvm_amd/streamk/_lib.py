@@ -139,7 +139,9 @@ def lib():
         getattr(L, f).restype = ci
     L.sk_gemm_i8_scaled.argtypes = [vp, vp, vp, i64, i64, i64, i64, i64, i64, P(SkScales), P(SkPlan), vp, sz, vp, P(SkEpilogue)]
     L.sk_quantize_i8.argtypes = [vp, ci, i64, i64, i64, vp, i64, vp, vp]
-    L.sk_gemm_grouped.argtypes = [P(SkGrouped), vp]
+    L.sk_gemm_grouped.argtypes = [P(SkGrouped), vp, sz, vp]
+    L.sk_grouped_workspace_bytes.argtypes = [P(SkGrouped)]
+    L.sk_grouped_workspace_bytes.restype = sz
     L.sk_grouped_wgrad.argtypes = [vp, vp, vp, vp, ci, i64, i64, i64, i64, i64, i64, ci, vp]
     L.sk_route_workspace_bytes.argtypes = [i64, i64, i64]
     L.sk_route_workspace_bytes.restype = sz

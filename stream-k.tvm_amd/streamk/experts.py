@@ -97,7 +97,9 @@ def _grouped(A, B, offsets, layout="nt", out_dtype=None, scale_a=None, scale_b=N
                        offsets=offsets.data_ptr(), C=C.data_ptr(), lda=_pitch(A), ldb=ldb, ldc=max(C.stride(0), N),
                        expert_b=B.stride(0) if E > 1 else 0, bias=bias.data_ptr() if bias is not None else None,
                        scale_a=scale_a.data_ptr() if int8 else None, scale_b=scale_b.data_ptr() if int8 else None, variant=variant)
-    _lib.check(_lib.lib().sk_gemm_grouped(ctypes.byref(g), ops._stream_ptr()), "sk_gemm_grouped")
+    ws = ops._workspace(_lib.lib().sk_grouped_workspace_bytes(ctypes.byref(g)), A.device)
+    _lib.check(_lib.lib().sk_gemm_grouped(ctypes.byref(g), ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
+                                          ops._stream_ptr()), "sk_gemm_grouped")
     return C
 
 

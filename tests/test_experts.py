@@ -401,8 +401,8 @@ def test_calls_are_refused_with_codes(sk):
 
     def grouped(**kw):
         d = dict(dtype=lib.SK_F16, layout=0, out_dtype=lib.SK_F16, activation=0, E=2, R=10, N=64, K=64, A=p, B=p, offsets=p, C=p, lda=64, ldb=64, ldc=64, expert_b=4096)
-        return L.sk_gemm_grouped(ctypes.byref(lib.SkGrouped(**{**d, **kw})), None)
-    assert L.sk_gemm_grouped(None, None) == -1
+        return L.sk_gemm_grouped(ctypes.byref(lib.SkGrouped(**{**d, **kw})), None, 0, None)
+    assert L.sk_gemm_grouped(None, None, 0, None) == -1
     assert grouped(A=None) == -1 and grouped(offsets=None) == -1 and grouped(dtype=lib.SK_I8, out_dtype=0) == -1
     for bad in (dict(dtype=lib.SK_F32, out_dtype=lib.SK_F32), dict(out_dtype=lib.SK_BF16), dict(layout=2), dict(activation=4), dict(scale_a=p), dict(activation=-1),
                 dict(dtype=lib.SK_I8, scale_a=p, scale_b=p, layout=1), dict(dtype=lib.SK_I8, scale_a=p, scale_b=p, out_dtype=lib.SK_F32)):
@@ -469,7 +469,7 @@ def test_wrong_operands_are_refused(sk):
 
 
 # ---- every kind of tile on every kind of groups ----
-VARIANTS = [1, 2]
+VARIANTS = [1, 2, 3, 4, 5]
 
 
 @pytest.mark.gpu
@@ -483,6 +483,8 @@ def test_grouped_variants(sk, variant, kind, sizes, N, K, padding):
     offsets = offsets_of(sizes)
     out = torch.full((R, N + padding), 7.0, dtype=torch.bfloat16 if kind == "int8" else TYPES[kind.split()[0]], device="cuda")
     bias = rand((E, N), out.dtype, 5)
+    if kind.endswith("nn") and variant > 2:
+        return   # ([E, N, K] weights only)
     if kind == "int8":
         g = torch.Generator().manual_seed(R + N)
         A = torch.randint(-127, 128, (R, K), generator=g, dtype=torch.int8).cuda()
@@ -511,7 +513,7 @@ def test_grouped_variants(sk, variant, kind, sizes, N, K, padding):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("variant", VARIANTS)
+@pytest.mark.parametrize("variant", [1, 2])
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("sizes", sorted(SIZES))
 @pytest.mark.parametrize("M,N", [(513, 264), (256, 520), (64, 8)])
