@@ -12,6 +12,7 @@
 // The tiles themselves are those of the ordinary products, each with its arguments moved to the expert's operands.
 #pragma once
 #include "sk_device.h"
+#include "sk_persistent.h"
 #include "tile_scaled_i8.h"
 
 namespace sk {
@@ -169,8 +170,125 @@ __device__ __forceinline__ void run_grouped(const GroupedArgs &g, int ipt, char 
       continue;
     }
     const typename P::Args a = expert_args<P>(g, t);
+    const void *epi = expert_epilogue(g, t);
+    if constexpr (has_prefetch_bias<P>::value) {
+      if (epi != nullptr) P::prefetch_bias(a, acc, t.pn, epi);
+    }
     P::mac(a, acc, t.pm, t.pn, 0, ipt, smem);
-    P::store_c(a, acc, t.pm, t.pn, smem, expert_epilogue(g, t));
+    P::store_c(a, acc, t.pm, t.pn, smem, epi);
+  }
+}
+
+// ---- Stream-K over the groups ----
+// As long as there is a tile for every CTA each takes one -- neighbouring tiles at a time, which share rows and weights in the L2s --
+// and the iterations of the tiles that are left, fewer than CTAs, are numbered through and dealt out in equal runs.  A tile that lies in one run is stored as it is.  Of one that is cut, every CTA with a part leaves its sums in the workspace, two
+// slots to a CTA: slot 1 for the tile whose start it has, slot 0 for the one that it enters in the middle.  When its run is over a CTA
+// adds its iterations to the tile's counter (kept at the CTA that has the tile's start, and zero before and after); who completes the
+// count adds up the parts in the order of the CTAs, which is the same on every launch, and stores.  Nobody waits for another CTA.
+struct SkRuns {
+  int total, ctas, each, extra;   // iterations, CTAs that have some, of each CTA, CTAs with one more
+  // least: iterations of a run, that its fix-up is worth
+  __device__ __forceinline__ SkRuns(int total_, int grid, int least) : total(total_) {
+    ctas = min(grid, max(1, total / least));
+    each = (int)((unsigned)total / (unsigned)ctas);
+    extra = total - each * ctas;
+  }
+  __device__ __forceinline__ int start(int pid) const { return pid * each + min(pid, extra); }
+  __device__ __forceinline__ int length(int pid) const { return each + (pid < extra ? 1 : 0); }
+  __device__ __forceinline__ int cta_of(int at) const {
+    const int boundary = extra * (each + 1);
+    return at < boundary ? (int)((unsigned)at / (unsigned)(each + 1)) : extra + (int)((unsigned)(at - boundary) / (unsigned)each);
+  }
+};
+// rows without an expert become zeros, shared out over the grid
+__device__ __forceinline__ void zero_unowned(const GroupedArgs &g, int pid, int threads) {
+  const int front = min(max(g.offsets[0], 0), g.R), back = min(max(g.offsets[g.E], front), g.R);
+  const int rows = front + g.R - back;
+  for (int r = pid; r < rows; r += g.grid) {
+    half_t *C = g.C + (int64_t)(r < front ? r : back + r - front) * g.ldc;
+    for (int col = threadIdx.x; col < g.N; col += threads) C[col] = (half_t)0.f;
+  }
+}
+
+// P: a policy whose partial tiles are coherent (store_partial, add_partial) and whose LDS is dead between two calls of mac
+template <class P>
+__device__ __forceinline__ void run_grouped_sk(const GroupedArgs &g, int ipt, const Workspace &ws, char *smem) {
+  static_assert(P::COHERENT_PARTIALS && P::FIXUP_WORD_IN_LDS, "see above");
+  GroupWalk<P::BM, false> walk(g.offsets, g.E, g.R, g.tiles_n);
+  const int pid = grouped_pid(g.grid);
+  zero_unowned(g, pid, P::NT);
+  const int tiles = walk.total_tiles(), whole = tiles - (int)((unsigned)tiles % (unsigned)g.grid);
+  auto slot = [&](int p, int which) { return ws.partials + (size_t)(2 * p + which) * P::TILE_ELEMS; };
+  typename P::Acc acc;
+  GroupTile t;
+  for (int tile = pid; tile < whole; tile += g.grid) {
+    walk.find(tile, t);
+    const typename P::Args a = expert_args<P>(g, t);
+    const void *epi = expert_epilogue(g, t);
+    if constexpr (has_prefetch_bias<P>::value) {
+      if (epi != nullptr) P::prefetch_bias(a, acc, t.pn, epi);
+    }
+    P::mac(a, acc, t.pm, t.pn, 0, ipt, smem);
+    P::store_c(a, acc, t.pm, t.pn, smem, epi);
+  }
+  const SkRuns runs((tiles - whole) * ipt, g.grid, 4);   // (a cut costs about as much as two iterations)
+  if (pid >= runs.ctas || runs.total == 0) return;
+  int at = runs.start(pid), left = runs.length(pid);
+  int cut_tile[2] = {-1, -1}, cut_n[2];   // [0]: entered in the middle, [1]: its start is here
+  GroupTile cut[2];
+  while (left > 0) {
+    const int tile = (int)((unsigned)at / (unsigned)ipt), k0 = at - tile * ipt, n = min(ipt - k0, left);
+    walk.find(whole + tile, t);
+    const typename P::Args a = expert_args<P>(g, t);
+    const void *epi = expert_epilogue(g, t);
+    if constexpr (has_prefetch_bias<P>::value) {
+      if (epi != nullptr) P::prefetch_bias(a, acc, t.pn, epi);
+    }
+    P::mac(a, acc, t.pm, t.pn, k0, n, smem);
+    if (n == ipt) {
+      P::store_c(a, acc, t.pm, t.pn, smem, epi);
+    } else {
+      P::store_partial(acc, slot(pid, k0 == 0));
+      if (k0 == 0) {
+        cut_tile[1] = tile;
+        cut_n[1] = n;
+        cut[1] = t;
+      } else {
+        cut_tile[0] = tile;
+        cut_n[0] = n;
+        cut[0] = t;
+      }
+    }
+    at += n;
+    left -= n;
+  }
+  if (cut_tile[0] < 0 && cut_tile[1] < 0) return;
+  wait_own_memory_ops();
+  __syncthreads();
+  int *word = reinterpret_cast<int *>(smem);
+  if (threadIdx.x == 0)
+    __hip_atomic_fetch_max(ws.status + WS_DIRTY, (int)(((size_t)(2 * pid + 2) * P::TILE_ELEMS * 4 + 255) >> 8), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    if (cut_tile[c] < 0) continue;   // (uniform)
+    const int p0 = runs.cta_of(cut_tile[c] * ipt), p1 = runs.cta_of(cut_tile[c] * ipt + ipt - 1);
+    if (threadIdx.x == 0) {
+      const int have = __hip_atomic_fetch_add(ws.flags + p0, cut_n[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + cut_n[c];
+      if (have == ipt) __hip_atomic_store(ws.flags + p0, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      *word = have == ipt;
+    }
+    __syncthreads();
+    const bool complete = *word != 0;
+    __syncthreads();
+    if (!complete) continue;
+    const typename P::Args a = expert_args<P>(g, cut[c]);
+    const void *epi = expert_epilogue(g, cut[c]);
+    if constexpr (has_prefetch_bias<P>::value) {
+      if (epi != nullptr) P::prefetch_bias(a, acc, cut[c].pn, epi);
+    }
+    P::zero_sums(acc);
+    for (int p = p0; p <= p1; ++p) P::add_partial(acc, slot(p, p == p0));
+    P::store_c(a, acc, cut[c].pm, cut[c].pn, smem, epi);
   }
 }
 

@@ -15,7 +15,7 @@ struct GroupedShape {
   int variant;   // GroupedVariant
 };
 // which tiles (0: by the rule in kernels_grouped.hip)
-enum GroupedVariant { GV_RULE = 0, GV_TILE128 = 1, GV_ASM256 = 2, GV_STREAM16 = 3, GV_STREAM32 = 4, GV_STREAM64 = 5 };
+enum GroupedVariant { GV_RULE = 0, GV_TILE128 = 1, GV_ASM256 = 2, GV_WAVEK16 = 3, GV_WAVEK32 = 4, GV_WAVEK64 = 5, GV_WAVEK64W = 6 };
 // the variant that a call takes (never GV_RULE; what a caller asked for, if anything), and the workspace it needs
 int grouped_variant(const GroupedShape &h);
 size_t grouped_workspace(const GroupedShape &h);
@@ -27,9 +27,9 @@ static inline int64_t grouped_tiles(const GroupedShape &h, int bm) {
 }
 // hipError_t as int; hipErrorNotSupported: h.variant does not exist or does not take the problem
 int launch_grouped(const GroupedArgs &g, const GroupedShape &h, const Workspace &ws, hipStream_t s);
-// few rows to an expert (kernels_grouped_stream.hip)
-size_t grouped_stream_workspace(int variant, int cus);
-int launch_grouped_stream(const GroupedArgs &g, const GroupedShape &h, const Workspace &ws, hipStream_t s);
+// up to some dozen rows to an expert (kernels_grouped_wavek.hip)
+size_t grouped_wavek_workspace(int variant, int cus);
+int launch_grouped_wavek(const GroupedArgs &g, const GroupedShape &h, const Workspace &ws, hipStream_t s);
 
 struct WgradArgs {
   const half_t *dC, *A;   // [R, N] (width readable columns), [R, K]
@@ -43,7 +43,8 @@ int launch_wgrad(const WgradArgs &g, bool bf16, int cus, int variant, hipStream_
 
 // the 256 x 256 tiles (kernels_grouped_asm.hip), and what they take
 bool grouped_asm_takes(const GroupedShape &h);
-int launch_grouped_asm(const GroupedArgs &g, const GroupedShape &h, hipStream_t s);
+size_t grouped_asm_workspace(int cus);
+int launch_grouped_asm(const GroupedArgs &g, const GroupedShape &h, const Workspace &ws, hipStream_t s);
 bool wgrad_asm_takes(const WgradArgs &g);
 int launch_wgrad_asm(const WgradArgs &g, bool bf16, int cus, hipStream_t s);
 

@@ -14,12 +14,18 @@ __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_grouped_kernel(Grou
 int grouped_variant(const GroupedShape &h) {
   if (h.variant != GV_RULE) return h.variant;
   const int64_t experts = h.E < h.R ? h.E : h.R, rows = h.R / experts;   // of an expert that has any, about
-  if (!h.nn && rows <= 8) return GV_STREAM16;
-  if (!h.nn && rows <= 24) return GV_STREAM32;
-  if (!h.nn && rows <= 48) return GV_STREAM64;
+  if (!h.nn) {
+    if (rows <= 8) return GV_WAVEK16;
+    if (rows <= 20) return GV_WAVEK32;
+    if (rows <= 40) return GV_WAVEK64;
+    if (rows <= 80) return GV_WAVEK64W;
+  }
   return grouped_asm_takes(h) && rows >= 128 ? GV_ASM256 : GV_TILE128;
 }
-size_t grouped_workspace(const GroupedShape &h) { return grouped_stream_workspace(grouped_variant(h), h.cus); }
+size_t grouped_workspace(const GroupedShape &h) {
+  const int v = grouped_variant(h);
+  return v == GV_ASM256 ? grouped_asm_workspace(h.cus) : grouped_wavek_workspace(v, h.cus);
+}
 
 template <class P>
 static int launch_grouped_policy(GroupedArgs g, const GroupedShape &h, hipStream_t s) {
@@ -34,8 +40,8 @@ static int launch_grouped_policy(GroupedArgs g, const GroupedShape &h, hipStream
 int launch_grouped(const GroupedArgs &g, const GroupedShape &h, const Workspace &ws, hipStream_t s) {
   GroupedShape with = h;
   with.variant = grouped_variant(h);
-  if (with.variant >= GV_STREAM16) return h.nn ? (int)hipErrorNotSupported : launch_grouped_stream(g, with, ws, s);
-  if (with.variant == GV_ASM256) return grouped_asm_takes(h) ? launch_grouped_asm(g, h, s) : (int)hipErrorNotSupported;
+  if (with.variant >= GV_WAVEK16) return h.nn ? (int)hipErrorNotSupported : launch_grouped_wavek(g, with, ws, s);
+  if (with.variant == GV_ASM256) return grouped_asm_takes(h) ? launch_grouped_asm(g, h, ws, s) : (int)hipErrorNotSupported;
   if (h.type == GT_I8) return launch_grouped_policy<ScaledDma<TileF16NTDma<128, 128, 2, 2, false, 64, true, false, 3>>>(g, h, s);
   if (h.nn) {
     if (h.type == GT_BF16) return launch_grouped_policy<TileF16NTDma<128, 128, 2, 2, true, 64, true, true>>(g, h, s);

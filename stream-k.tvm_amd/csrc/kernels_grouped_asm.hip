@@ -2,53 +2,151 @@
 // gradient of the experts' weights.  The first loads of a CTA's next tile go out before this one is stored, across experts too.
 #include "grouped.h"
 #include "grouped_launch.h"
+#include "kernel_table.h"
 #include "tile_scaled_i8_asm.h"
 #include "tile_tn_asm.h"
 
 namespace sk {
 
+// How the tiles that are left when every CTA has had its whole rounds are cut: K in `parts` equal parts, one to a CTA.  (Aligned cuts: the
+// CTAs stay at the same K of their tiles and share rows and weights in the L2s.  Runs of equal length that begin anywhere, as for the
+// small tiles in grouped.h, write 90 MB of sums and cost 100 us here: 8 x 11008 x 4096, 3000 rows, bfloat16 307 us, whole tiles 284.)
+struct Cuts {
+  int whole, parts;
+  __device__ __forceinline__ Cuts(int tiles, int grid, int ipt) {
+    const int rest = (int)((unsigned)tiles % (unsigned)grid);
+    parts = ipt < CUT_LEAST || rest == 0 ? 1 : (rest * 4 <= grid ? 4 : (rest * 2 <= grid ? 2 : 1));
+    whole = parts > 1 ? tiles - rest : tiles;
+  }
+  static constexpr int CUT_LEAST = 32;   // iterations of a tile from which the exchange, some 20 us, pays
+};
+
+// The end of a part of a cut tile.  Each CTA of the tile takes a ticket; all but the last put their sums into the workspace and raise a
+// flag, the last one -- the others are past their loops by then and wait for nobody, so the wait is a short one whatever else the
+// device does -- adds them to its own in the order of the parts, which is the same on every launch.  True: acc has the tile's sums.
+// flags: [grid] of the CTAs, then a counter for each cut tile; all zero before and after.
 template <class P>
-__global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_grouped_asm_kernel(GroupedArgs g, int ipt) {
-  GroupWalk<P::BM> walk(g.offsets, g.E, g.R, g.tiles_n);
+__device__ __forceinline__ bool join_parts(typename P::Acc &acc, int tile, int part, int parts, int grid, const Workspace &ws) {
+  int *ticket = ws.flags + grid + tile, *flags = ws.flags + tile * parts, *word = reinterpret_cast<int *>(P::lds() + 2 * P::STAGE_BYTES);
+  auto slot = [&](int q) { return ws.partials + (size_t)(tile * parts + q) * P::TILE_ELEMS; };
+  if (threadIdx.x == 0) *word = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  const bool last = *word == parts - 1;
+  __syncthreads();
+  if (!last) {
+    P::store_partial(acc, slot(part));
+    signal_partial_ready<true>(flags + part, ws.status + WS_DIRTY, (int)(((size_t)(tile * parts + part + 1) * P::TILE_ELEMS * 4 + 255) >> 8));
+    return false;
+  }
+  bool ok = true;
+  if (threadIdx.x < 64) {
+    for (int q = 0; q < parts; ++q) {
+      if (q == part) continue;
+      int got = 0;
+      for (int spin = 0; spin < (1 << 22) && !got; ++spin) {
+        got = __hip_atomic_load(flags + q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (!got) __builtin_amdgcn_s_sleep(1);
+      }
+      ok = ok && got;
+    }
+    if (threadIdx.x == 0) *word = ok;
+  }
+  __syncthreads();
+  if (*word == 0 && threadIdx.x == 0) ws.status[WS_STATUS] = -8;   // SK_ERR_TIMEOUT
+  // eight groups at a time: the parts in front of this one, this one, the parts behind it
+  constexpr int BATCH = 8;
+  const uint32_t off = (uint32_t)pin_here((int)threadIdx.x) * 16;
+  static_for<0, P::NV4 / BATCH>([&](auto b) {
+    constexpr int base = decltype(b)::value * BATCH;
+    typedef typename std::conditional<P::I8, typename P::intx4, floatx4>::type Sum;
+    Sum sum[BATCH];
+    for (int q = 0; q < parts; ++q) {
+      const BufferRsrc r = make_rsrc(slot(q), P::TILE_ELEMS * 4);
+      Sum x[BATCH];
+      if (q == part) {
+        static_for<0, BATCH>([&](auto i) { x[decltype(i)::value] = __builtin_bit_cast(Sum, agpr_read4<(base + decltype(i)::value) * 4>()); });
+      } else {
+        static_for<0, BATCH>([&](auto i) {
+          x[decltype(i)::value] = __builtin_bit_cast(Sum, ld_coherent16(r, off, (uint32_t)(base + decltype(i)::value) * P::NT * 16));
+        });
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) sum[i] = q == 0 ? x[i] : sum[i] + x[i];
+    }
+    static_for<0, BATCH>([&](auto i) { agpr_write4<(base + decltype(i)::value) * 4>(__builtin_bit_cast(floatx4, sum[decltype(i)::value])); });
+  });
+  if (threadIdx.x < parts) __hip_atomic_store(flags + threadIdx.x, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (threadIdx.x == 0) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return true;
+}
+
+template <class P>
+__global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_grouped_asm_kernel(GroupedArgs g, int ipt, Workspace ws) {
+  GroupWalk<P::BM, false> walk(g.offsets, g.E, g.R, g.tiles_n);
+  const int pid = grouped_pid(g.grid);
+  zero_unowned(g, pid, P::NT);
+  const int tiles = walk.total_tiles();
+  const Cuts cuts(tiles, g.grid, ipt);
+  struct Segment {
+    GroupTile t;
+    int cut, part, k0, n;   // (cut: number among the cut tiles, or -1)
+  };
+  int dp_tile = pid;
+  bool part_left = pid < (tiles - cuts.whole) * cuts.parts;
+  auto next_segment = [&](Segment &s) {
+    if (dp_tile < cuts.whole) {
+      walk.find(dp_tile, s.t);
+      s.cut = -1;
+      s.k0 = 0;
+      s.n = ipt;
+      dp_tile += g.grid;
+      return true;
+    }
+    if (!part_left) return false;
+    part_left = false;
+    s.cut = cuts.parts == 4 ? pid >> 2 : pid >> 1;
+    s.part = pid - s.cut * cuts.parts;
+    s.k0 = s.part * ipt / cuts.parts;
+    s.n = (s.part + 1) * ipt / cuts.parts - s.k0;
+    walk.find(cuts.whole + s.cut, s.t);
+    return true;
+  };
   typename P::Acc acc;
-  GroupTile t, next;
-  int tile = grouped_pid(g.grid);
-  bool have = walk.find(tile, t), requested = false;
+  Segment s, next;
+  bool have = next_segment(s), requested = false;
   while (have) {
-    const bool owned = t.group != 0 && t.group != g.E + 1;
-    const typename P::Args a = expert_args<P>(g, t);
-    const void *epi = expert_epilogue(g, t);
-    if (owned) P::mac(a, acc, t.pm, t.pn, 0, ipt, nullptr, requested);
+    const typename P::Args a = expert_args<P>(g, s.t);
+    const void *epi = expert_epilogue(g, s.t);
+    P::mac(a, acc, s.t.pm, s.t.pn, s.k0, s.n, nullptr, requested);
     requested = false;
-    tile += g.grid;
-    have = walk.find(tile, next);
-    if (have && owned && next.group != 0 && next.group != g.E + 1 && P::epilogue_lds_free(a, t.pn, epi)) {
-      P::prefetch_first_stage(expert_args<P>(g, next), next.pm, next.pn, 0, ipt);
+    have = next_segment(next);   // (a part comes last)
+    if (have && P::epilogue_lds_free(a, s.t.pn, epi)) {
+      P::prefetch_first_stage(expert_args<P>(g, next.t), next.t.pm, next.t.pn, next.k0, next.n);
       requested = true;
     }
-    if (owned) P::store_c(a, acc, t.pm, t.pn, nullptr, epi);
-    else zero_tile<P>(g, t);
-    t = next;
+    if (s.cut < 0 || join_parts<P>(acc, s.cut, s.part, cuts.parts, g.grid, ws)) P::store_c(a, acc, s.t.pm, s.t.pn, nullptr, epi);
+    s = next;
   }
 }
 
 template <class P>
-static int launch_asm(GroupedArgs g, const GroupedShape &h, int ipt, hipStream_t s) {
+static int launch_asm(GroupedArgs g, const GroupedShape &h, int ipt, const Workspace &ws, hipStream_t s) {
   g.tiles_n = (g.N + P::BN - 1) / P::BN;
-  const int64_t most = grouped_tiles(h, P::BM) * g.tiles_n;
-  if (most > 0x7fffffff) return (int)hipErrorInvalidValue;
-  g.grid = (int)(most < h.cus ? most : h.cus);
-  hipLaunchKernelGGL((sk_grouped_asm_kernel<P>), dim3(g.grid), dim3(P::NT), 0, s, g, ipt);
+  if (grouped_tiles(h, P::BM) * g.tiles_n > 0x7fffffff) return (int)hipErrorNotSupported;
+  g.grid = h.cus;
+  hipLaunchKernelGGL((sk_grouped_asm_kernel<P>), dim3(g.grid), dim3(P::NT), 0, s, g, ipt, ws);
   return (int)hipGetLastError();
 }
 
+size_t grouped_asm_workspace(int cus) { return (size_t)WS_PART_OFF + (size_t)cus * ScaledAsm::TILE_ELEMS * 4; }
+
 bool grouped_asm_takes(const GroupedShape &h) { return h.K % (h.type == GT_I8 ? 128 : 64) == 0; }
 
-int launch_grouped_asm(const GroupedArgs &g, const GroupedShape &h, hipStream_t s) {
+int launch_grouped_asm(const GroupedArgs &g, const GroupedShape &h, const Workspace &ws, hipStream_t s) {
   const int ipt = (int)(h.K / (h.type == GT_I8 ? 128 : 64));
-  if (h.type == GT_I8) return launch_asm<ScaledAsm>(g, h, ipt, s);
-  if (h.nn) return h.type == GT_BF16 ? launch_asm<TileF16Asm<1, true>>(g, h, ipt, s) : launch_asm<TileF16Asm<0, true>>(g, h, ipt, s);
-  return h.type == GT_BF16 ? launch_asm<TileF16Asm<1, false>>(g, h, ipt, s) : launch_asm<TileF16Asm<0, false>>(g, h, ipt, s);
+  if (h.type == GT_I8) return launch_asm<ScaledAsm>(g, h, ipt, ws, s);
+  if (h.nn) return h.type == GT_BF16 ? launch_asm<TileF16Asm<1, true>>(g, h, ipt, ws, s) : launch_asm<TileF16Asm<0, true>>(g, h, ipt, ws, s);
+  return h.type == GT_BF16 ? launch_asm<TileF16Asm<1, false>>(g, h, ipt, ws, s) : launch_asm<TileF16Asm<0, false>>(g, h, ipt, ws, s);
 }
 
 // ---- dW[e] = dC[rows of e]^T A[rows of e] ----

@@ -5,18 +5,20 @@
 
 namespace sk {
 
-// four fp32 values, rounded once to bfloat16 or fp16 (uniform choice: C's type is an argument of these kernels)
-__device__ __forceinline__ half4v round4(floatx4 x, bool bf16) {
+// four fp32 values, rounded once to bfloat16 or fp16 (C and the patches carry 16-bit patterns)
+template <bool BF16>
+__device__ __forceinline__ half4v round4(floatx4 x) {
   half4v h;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const __bf16 b = (__bf16)x[e];
-    h[e] = bf16 ? __builtin_bit_cast(half_t, b) : (half_t)x[e];   // (patches and C carry 16-bit patterns)
+    if constexpr (BF16) {
+      const __bf16 b = (__bf16)x[e];
+      h[e] = __builtin_bit_cast(half_t, b);
+    } else {
+      h[e] = (half_t)x[e];
+    }
   }
   return h;
-}
-__device__ __forceinline__ floatx4 bias4_of(const half_t *bias, int col, int N, bool bf16) {
-  return bf16 ? bias4_at<true>(bias, col, N) : bias4_at<false>(bias, col, N);
 }
 
 // Stores FM x FN blocks of a wave, the first of which stands at (row0, col0) of C, through a patch of LDS of the wave's own

@@ -34,26 +34,46 @@ __device__ __forceinline__ floatx4 scale4_at(const float *s, int col, int N) {
     if (col + e < N) r[e] = s[col + e];
   return r;
 }
-__device__ __forceinline__ half4v scaled4(intx4_s x, float sa, floatx4 sb, floatx4 bias, int act, bool bf16) {
+// EPI: bias and activation.  The instances differ in C's type and in EPI, and the store code is compiled for each: chosen by element,
+// the 256 x 256 tiles' end took 30 us.
+template <bool BF16, bool EPI>
+__device__ __forceinline__ half4v scaled4(intx4_s x, float sa, floatx4 sb, floatx4 bias, int act) {
   floatx4 y;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) y[e] = activate((float)x[e] * sa * sb[e] + bias[e], act);
-  return round4(y, bf16);
+  for (int e = 0; e < 4; ++e) {
+    y[e] = (float)x[e] * sa * sb[e];
+    if constexpr (EPI) y[e] += bias[e];
+  }
+  if constexpr (EPI) {
+    if (act != 0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = activate(y[e], act);
+    }
+  }
+  return round4<BF16>(y);
+}
+// f(BF16, EPI) as constants
+template <class F>
+__device__ __forceinline__ void by_result(bool bf16, const void *epi, F &&f) {
+  if (epi == nullptr) {
+    if (bf16) f(std::true_type{}, std::false_type{});
+    else f(std::false_type{}, std::false_type{});
+  } else {
+    if (bf16) f(std::true_type{}, std::true_type{});
+    else f(std::false_type{}, std::true_type{});
+  }
 }
 
 // what the columns of a wave's FN blocks and the rows of its FM blocks bring along
-template <int FM, int FN>
+template <int FM, int FN, bool BF16, bool EPI>
 struct ScaleRegs {
-  floatx4 sb[FN], bias[FN];
+  floatx4 sb[FN], bias[EPI ? FN : 1];
   float sa[FM];
   int act;
-  bool bf16;
   template <class Args>
-  __device__ __forceinline__ void load(const Args &a, int row0, int col0, const void *epi) {
+  __device__ __forceinline__ ScaleRegs(const Args &a, int row0, int col0, const void *epi) {
     const int lane = pin_here((int)threadIdx.x) & 63;
-    const half_t *b = epi_bias(epi);
-    act = epi_act(epi);
-    bf16 = a.s.bf16 != 0;
+    act = EPI ? epi_act(epi) : 0;
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int row = row0 + 16 * i + (lane & 15);
@@ -63,8 +83,12 @@ struct ScaleRegs {
     for (int j = 0; j < FN; ++j) {
       const int col = col0 + 16 * j + 4 * (lane >> 4);
       sb[j] = scale4_at(a.s.b, col, a.N);
-      bias[j] = bias4_of(b, col, a.N, bf16);
+      if constexpr (EPI) bias[j] = bias4_at<BF16>(epi_bias(epi), col, a.N);
     }
+  }
+  template <int I, int J>
+  __device__ __forceinline__ half4v values(intx4_s x) const {
+    return scaled4<BF16, EPI>(x, sa[I], sb[J], bias[EPI ? J : 0], act);
   }
 };
 
@@ -80,10 +104,11 @@ struct ScaledDma : P {
   static __device__ __forceinline__ void store_rows(const Args &a, const Acc &acc, int pm, int pn, const void *epi) {
     const int wave = threadIdx.x >> 6, wm = wave / P::WN, wn = wave % P::WN;
     const int row0 = pm * P::BM + wm * P::WTM, col0 = pn * P::BN + wn * P::WTN;
-    ScaleRegs<P::FM, P::FN> r;
-    r.load(a, row0, col0, epi);
-    Patch::template store<I0, I1>(a.C, a.ldc, a.M, a.N, row0, col0, P::stage(0) + wave * Patch::BYTES, [&](auto i, auto j) {
-      return scaled4(acc.v[i][j], r.sa[i], r.sb[j], r.bias[j], r.act, r.bf16);
+    by_result(a.s.bf16 != 0, epi, [&](auto bf16, auto with_epi) {
+      const ScaleRegs<P::FM, P::FN, decltype(bf16)::value, decltype(with_epi)::value> r(a, row0, col0, epi);
+      Patch::template store<I0, I1>(a.C, a.ldc, a.M, a.N, row0, col0, P::stage(0) + wave * Patch::BYTES, [&](auto i, auto j) {
+        return r.template values<decltype(i)::value, decltype(j)::value>(acc.v[i][j]);
+      });
     });
     __syncthreads();   // the patches overlap the stages of the next tile
   }
@@ -102,23 +127,29 @@ struct ScaledWaveK : P {
   typedef ScaledArgs<WaveKArgs> Args;
   typedef typename P::Acc Acc;
   static __device__ __forceinline__ void store_c(const Args &a, const Acc &acc, int pm, int pn, char *, const void *epi) {
-    const int tid = pin_here((int)threadIdx.x), act = epi_act(epi);
-    const half_t *bias = epi_bias(epi);
-    const bool bf16 = a.s.bf16 != 0, vec_ok = (a.ldc & 3) == 0 && (reinterpret_cast<uintptr_t>(a.C) & 7) == 0;
-    floatx4 sb[P::PIECES], b4[P::PIECES];
+    by_result(a.s.bf16 != 0, epi, [&](auto bf16, auto with_epi) { store<decltype(bf16)::value, decltype(with_epi)::value>(a, acc, pm, pn, epi); });
+  }
+  template <bool BF16, bool EPI>
+  static __device__ __forceinline__ void store(const Args &a, const Acc &acc, int pm, int pn, const void *epi) {
+    const int tid = pin_here((int)threadIdx.x), act = EPI ? epi_act(epi) : 0;
+    const bool vec_ok = (a.ldc & 3) == 0 && (reinterpret_cast<uintptr_t>(a.C) & 7) == 0;
+    constexpr int COLS = P::ONE_COL ? 1 : P::PIECES;   // (pieces below each other share their columns' scales)
+    floatx4 sb[COLS], b4[COLS];
     float sa[P::PIECES];
 #pragma unroll
     for (int u = 0; u < P::PIECES; ++u) {   // all loads at once
       const int row = pm * P::BM + P::piece_row(u, tid), col = pn * P::BN + P::piece_col(u, tid) * 4;
       sa[u] = row < a.M ? a.s.a[row] : 0.f;
-      sb[u] = scale4_at(a.s.b, col, a.N);
-      b4[u] = bias4_of(bias, col, a.N, bf16);
+      if (u < COLS) {
+        sb[u] = scale4_at(a.s.b, col, a.N);
+        if constexpr (EPI) b4[u] = bias4_at<BF16>(epi_bias(epi), col, a.N);
+      }
     }
 #pragma unroll
     for (int u = 0; u < P::PIECES; ++u) {
       const int row = pm * P::BM + P::piece_row(u, tid), col = pn * P::BN + P::piece_col(u, tid) * 4;
       if (row >= a.M || col >= a.N) continue;
-      const half4v h = scaled4(acc.c[u], sa[u], sb[u], b4[u], act, bf16);
+      const half4v h = scaled4<BF16, EPI>(acc.c[u], sa[u], sb[u % COLS], b4[u % COLS], act);
       half_t *dst = a.C + (int64_t)row * a.ldc + col;
       if (vec_ok && col + 4 <= a.N) {
         *reinterpret_cast<half4v *>(dst) = h;
@@ -140,24 +171,23 @@ struct ScaledStream : P {
     const int wm = wave % P::WM, wn = wave / P::WM;
     const int row0 = pm * P::BM + wm * P::MB * 16, col0 = pn * P::BN + wn * P::NB * 16;
     const bool vec_ok = (a.ldc & 3) == 0 && (reinterpret_cast<uintptr_t>(a.C) & 7) == 0;
-    ScaleRegs<P::MB, P::NB> r;
-    r.load(a, row0, col0, epi);
-#pragma unroll
-    for (int i = 0; i < P::MB; ++i) {
-      const int row = row0 + 16 * i + (lane & 15);
-#pragma unroll
-      for (int j = 0; j < P::NB; ++j) {
-        const int col = col0 + 16 * j + 4 * (lane >> 4);
-        if (row >= a.M || col >= a.N) continue;
-        const half4v h = scaled4(acc.c[i][j], r.sa[i], r.sb[j], r.bias[j], r.act, r.bf16);
-        half_t *dst = a.C + (int64_t)row * a.ldc + col;
-        if (vec_ok && col + 4 <= a.N) {
-          *reinterpret_cast<half4v *>(dst) = h;
-        } else {
-          for (int e = 0; e < 4 && col + e < a.N; ++e) dst[e] = h[e];
-        }
-      }
-    }
+    by_result(a.s.bf16 != 0, epi, [&](auto bf16, auto with_epi) {
+      const ScaleRegs<P::MB, P::NB, decltype(bf16)::value, decltype(with_epi)::value> r(a, row0, col0, epi);
+      static_for<0, P::MB>([&](auto i) {
+        const int row = row0 + 16 * i + (lane & 15);
+        static_for<0, P::NB>([&](auto j) {
+          const int col = col0 + 16 * j + 4 * (lane >> 4);
+          if (row >= a.M || col >= a.N) return;
+          const half4v h = r.template values<decltype(i)::value, decltype(j)::value>(acc.c[i][j]);
+          half_t *dst = a.C + (int64_t)row * a.ldc + col;
+          if (vec_ok && col + 4 <= a.N) {
+            *reinterpret_cast<half4v *>(dst) = h;
+          } else {
+            for (int e = 0; e < 4 && col + e < a.N; ++e) dst[e] = h[e];
+          }
+        });
+      });
+    });
   }
 };
 

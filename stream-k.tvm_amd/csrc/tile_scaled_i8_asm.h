@@ -16,13 +16,15 @@ struct ScaledAsm : TileF16Asm<2, false> {
   static __device__ __forceinline__ void store_rows(const Args &a, int pm, int pn, const void *epi) {
     const int wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
     const int row0 = pm * P::BM + wm * P::WTM, col0 = pn * P::BN + wn * P::WTN;
-    static_for<0, 2>([&](auto half) {
-      constexpr int j0 = decltype(half)::value * HALF;
-      ScaleRegs<P::FM, HALF> r;
-      r.load(a, row0, col0 + 16 * j0, epi);
-      Patch::store<I0, I1>(a.C, a.ldc, a.M, a.N, row0, col0 + 16 * j0, P::lds() + 2 * P::STAGE_BYTES + wave * P::FAST_PATCH_BYTES, [&](auto i, auto j) {
-        const intx4_s x = __builtin_bit_cast(intx4_s, agpr_read4<(decltype(i)::value * P::FN + j0 + decltype(j)::value) * 4>());
-        return scaled4(x, r.sa[i], r.sb[j], r.bias[j], r.act, r.bf16);
+    by_result(a.s.bf16 != 0, epi, [&](auto bf16, auto with_epi) {
+      static_for<0, 2>([&](auto half) {
+        constexpr int j0 = decltype(half)::value * HALF;
+        const ScaleRegs<P::FM, HALF, decltype(bf16)::value, decltype(with_epi)::value> r(a, row0, col0 + 16 * j0, epi);
+        Patch::store<I0, I1>(a.C, a.ldc, a.M, a.N, row0, col0 + 16 * j0, P::lds() + 2 * P::STAGE_BYTES + wave * P::FAST_PATCH_BYTES,
+                             [&](auto i, auto j) {
+                               constexpr int ii = decltype(i)::value, jj = decltype(j)::value;
+                               return r.template values<ii, jj>(__builtin_bit_cast(intx4_s, agpr_read4<(ii * P::FN + j0 + jj) * 4>()));
+                             });
       });
     });
   }

@@ -128,7 +128,7 @@ struct TileTN {
   static __device__ __forceinline__ void store_c(const Args &a, const Acc &acc, int pm, int pn, char *smem, const void *) {
     const int wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
     Patch::template store<0, FM>(a.C, a.ldc, a.M, a.N, pm * BM + wm * WTM, pn * BN + wn * WTN, smem + wave * Patch::BYTES,
-                                 [&](auto i, auto j) { return round4(acc.v[i][j], BF16_); });
+                                 [&](auto i, auto j) { return round4<BF16_>(acc.v[i][j]); });
     __syncthreads();   // the patches overlap the stages of the next tile
   }
 };

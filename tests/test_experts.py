@@ -469,7 +469,7 @@ def test_wrong_operands_are_refused(sk):
 
 
 # ---- every kind of tile on every kind of groups ----
-VARIANTS = [1, 2, 3, 4, 5]
+VARIANTS = [1, 2, 3, 4, 5, 6]
 
 
 @pytest.mark.gpu
@@ -537,3 +537,35 @@ def test_variants_that_do_not_take_a_problem_are_refused(sk):
         with pytest.raises(sk.StreamKError) as e:
             sk.streamk_grouped_wgrad(A, A, offsets, variant=variant)
         assert e.value.status == -4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["float16 nt", "bfloat16 nn", "int8"])
+@pytest.mark.parametrize("variant,sizes,N,K", [(2, [300, 0, 200], 512, 4096), (2, [300, 0, 200], 512, 4224), (2, [2000], 2304, 4096), (2, [40, 4000], 4352, 4096),
+                                               (3, [3, 0, 9], 520, 4096), (4, [30, 100, 1], 264, 2176), (5, [70, 200], 1000, 2048), (6, [128, 64], 512, 8192)])
+def test_tiles_that_are_cut_along_k(sk, kind, variant, sizes, N, K):
+    """Tiles shared by several CTAs: right, and the same bits launch after launch, in whatever order the parts arrive."""
+    if kind.endswith("nn") and variant > 2:
+        return
+    R, E = sum(sizes), len(sizes)
+    offsets = offsets_of(sizes)
+    if kind == "int8":
+        g = torch.Generator().manual_seed(R)
+        A = torch.randint(-127, 128, (R, K), generator=g, dtype=torch.int8).cuda()
+        B = torch.randint(-127, 128, (E, N, K), generator=g, dtype=torch.int8).cuda()
+        sa, sb = (torch.rand(R, generator=g) + 0.5).cuda() * 0.01, (torch.rand(E, N, generator=g) + 0.5).cuda() / (73 * math.sqrt(K))
+        run = lambda: sk.streamk_grouped(A, B, offsets, scale_a=sa, scale_b=sb, variant=variant)  # noqa: E731
+        pre, magnitudes = plain(A, B, sizes)
+        pre, magnitudes = pre * sa.double()[:, None], 0
+        for e, at in groups(sizes):
+            pre[at] *= sb[e].double()
+    else:
+        dtype, layout = kind.split()
+        A, B = rand((R, K), TYPES[dtype], R), rand((E, N, K) if layout == "nt" else (E, K, N), TYPES[dtype], N, 1 / math.sqrt(K))
+        run = lambda: sk.streamk_grouped(A, B, offsets, layout=layout, variant=variant)  # noqa: E731
+        pre, magnitudes = plain(A, B, sizes, layout)
+    C = run()
+    assert_near(C, pre, K, magnitudes, pre)
+    for _ in range(5):
+        assert torch.equal(run(), C)
+    sk.workspace_status()
