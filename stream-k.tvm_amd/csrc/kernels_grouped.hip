@@ -11,16 +11,56 @@ __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_grouped_kernel(Grou
   run_grouped<P>(g, ipt, smem);
 }
 
+// The host knows the rows and the experts, not who has how many: an expert is taken to have R / E rows, spread by half a tile.
+//
+// Up to 8 and 20 rows the 16- and 32-row tiles, whose rings hold the most weights: us, 8 experts of 11008 x 4096 and 64 of 2048 x
+// 4096, fp16, 16- / 32- / 64-row tiles: 8 rows each 127 / 130 / 133 and 181 / 180 / 184, 16 rows 134 / 131 / 135, 32 rows 176 / 142 /
+// 140.  Above, the tile with the least estimated time: the rounds of the CUs that the tiles make, each of tau iterations of K (128 bytes
+// of a row) and o for a tile's beginning and end, against the weights' and rows' way from memory at the rate the tile reaches.
+// Estimated / measured us of 64 x 64, 64 x 128, 128 x 128, 256 x 256 tiles: 8 experts, 11008 x 4096, 48 rows each 166 / 145, 165 / 140,
+// 192 / 192, 209 / 196; 187 rows 306 / 297, 260 / 264, 240 / 240, 196 / 220; 1024 rows (bfloat16) the last 530 / 565; 64 experts,
+// 2048 x 4096, 64 rows 246 / 241, 244 / 232, 278 / 282, 304 / 262, 128 rows 352 / 347, 302 / 314, 282 / 271, 308 / 289.
+struct TileCost {
+  int variant, bm, bn, per_cu;
+  double tau, o, rate;   // us per 64 iterations of a CU's tiles, us, bytes per us
+};
+static const TileCost TILE_COSTS[] = {{GV_WAVEK64, 64, 64, 1, 13.0, 2.5, 5.2e6},
+                                      {GV_WAVEK64W, 64, 128, 1, 22.0, 3.5, 5.2e6},
+                                      {GV_TILE128, 128, 128, 2, 69.0, 3.0, 4.3e6},
+                                      {GV_ASM256, 256, 256, 1, 75.0, 7.0, 3.9e6}};
+static double estimate(const GroupedShape &h, const TileCost &c) {
+  const double experts = (double)(h.E < h.R ? h.E : h.R), rows = h.R / experts, bytes = h.type == GT_I8 ? 1.0 : 2.0;
+  const double high = h.E == 1 ? (double)((h.R + c.bm - 1) / c.bm) : rows / c.bm + 0.5;
+  const double tiles = experts * (high > 1.0 ? high : 1.0) * (double)((h.N + c.bn - 1) / c.bn);
+  const double iters = h.K * bytes / 8192.0, round = c.tau * iters + c.o, slots = (double)h.cus * c.per_cu;
+  const double whole = (double)(int64_t)(tiles / slots), rest = tiles / slots - whole;
+  double busy = whole * round;
+  if (c.variant == GV_WAVEK64 || c.variant == GV_WAVEK64W) {
+    busy += rest * round + (whole > 0 ? 5.0 : 10.0);            // (cut evenly)
+  } else if (rest > 0 && c.variant == GV_TILE128) {
+    busy += rest <= 0.5 ? 0.58 * c.tau * iters + c.o : round;   // (a tile that has its CU for itself)
+  } else if (rest > 0) {
+    const int parts = iters < 0.5 ? 1 : (rest <= 0.25 ? 4 : (rest <= 0.5 ? 2 : 1));
+    busy += parts == 1 ? round : c.tau * iters / parts + c.o + 20.0;
+  }
+  const double memory = (experts * h.N * h.K * bytes + h.R * (h.K * bytes + 2.0 * h.N)) / c.rate;
+  return busy > memory ? busy + 0.15 * memory : memory + 0.15 * busy;   // (they overlap but for a part)
+}
 int grouped_variant(const GroupedShape &h) {
   if (h.variant != GV_RULE) return h.variant;
-  const int64_t experts = h.E < h.R ? h.E : h.R, rows = h.R / experts;   // of an expert that has any, about
-  if (!h.nn) {
-    if (rows <= 8) return GV_WAVEK16;
-    if (rows <= 20) return GV_WAVEK32;
-    if (rows <= 40) return GV_WAVEK64;
-    if (rows <= 80) return GV_WAVEK64W;
+  const int64_t experts = h.E < h.R ? h.E : h.R, rows = h.R / experts;
+  if (!h.nn && rows <= 20) return rows <= 8 ? GV_WAVEK16 : GV_WAVEK32;
+  int best = GV_TILE128;
+  double least = 0;
+  for (const TileCost &c : TILE_COSTS) {
+    if ((h.nn && c.variant >= GV_WAVEK16) || (c.variant == GV_ASM256 && !grouped_asm_takes(h))) continue;
+    const double t = estimate(h, c);
+    if (least == 0 || t < least) {
+      least = t;
+      best = c.variant;
+    }
   }
-  return grouped_asm_takes(h) && rows >= 128 ? GV_ASM256 : GV_TILE128;
+  return best;
 }
 size_t grouped_workspace(const GroupedShape &h) {
   const int v = grouped_variant(h);
