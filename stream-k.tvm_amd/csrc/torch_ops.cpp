@@ -27,21 +27,27 @@
 #include <tuple>
 
 #include "streamk.h"
+#include "torch_ops.h"
+
+std::shared_mutex streamk_torch::g_mutex;
+static std::map<std::pair<int, void *>, streamk_torch::Buffer> g_workspaces;
+bool streamk_torch::find_workspace(int device, void *stream, size_t bytes, Buffer *ws) {
+  const auto w = g_workspaces.find({device, stream});
+  if (w == g_workspaces.end() || w->second.bytes < bytes) return false;
+  *ws = w->second;
+  return true;
+}
 
 namespace {
 
 using torch::jit::Stack;
+using streamk_torch::Buffer;
+using streamk_torch::g_mutex;
 
 // (M, N, K, dtype, layout, device)
 typedef std::tuple<int64_t, int64_t, int64_t, int, int, int> PlanKey;
 constexpr size_t MAX_PLANS = 4096;
-std::shared_mutex g_mutex;
-struct Buffer {
-  void *ptr = nullptr;
-  size_t bytes = 0;
-};
 std::map<PlanKey, sk_plan> g_plans;
-std::map<std::pair<int, void *>, Buffer> g_workspaces;
 
 // what a launch on the current stream takes beside the operands; the workspace is there as long as this is.  (Nothing but
 // the launch happens while it lives: an allocation could run a caller's code, which may call an operator itself.)
@@ -57,11 +63,7 @@ struct Launch {
     const auto it = g_plans.find(PlanKey(M, N, K, dtype, layout, device));
     if (it == g_plans.end()) return false;
     plan = it->second;
-    if (plan.workspace_bytes == 0) return true;
-    const auto w = g_workspaces.find({device, stream});
-    if (w == g_workspaces.end() || w->second.bytes < (size_t)plan.workspace_bytes) return false;
-    ws = w->second;
-    return true;
+    return plan.workspace_bytes == 0 || streamk_torch::find_workspace(device, stream, (size_t)plan.workspace_bytes, &ws);
   }
 };
 
@@ -173,6 +175,31 @@ at::Tensor gemm_i8(const at::Tensor &A, const at::Tensor &B, const at::Tensor *o
   return rc == SK_OK ? C : at::Tensor();
 }
 
+// operands A, B, scale_a, scale_b; (out_dtype, config, bias, activation)
+at::Tensor gemm_i8_scaled(const c10::IValue *operands, const at::Tensor *out, const c10::IValue *a) {
+  const at::Tensor &A = operands[0].toTensor(), &B = operands[1].toTensor(), &sa = operands[2].toTensor(), &sb = operands[3].toTensor();
+  const at::ScalarType type = a[0].toScalarType();
+  if ((type != at::kHalf && type != at::kBFloat16) || !a[1].toStringRef().empty()) return {};
+  if (!is_matrix(A, at::kChar) || !aligned_rows(A) || !is_matrix(B, at::kChar)) return {};
+  const int64_t M = A.size(0), K = A.size(1), N = B.size(0);
+  if (B.size(1) != K) return {};
+  const auto is_scale = [&](const at::Tensor &s, int64_t n) {
+    return s.scalar_type() == at::kFloat && s.dim() == 1 && s.size(0) == n && s.is_contiguous() && s.device() == A.device();
+  };
+  if (!is_scale(sa, M) || !is_scale(sb, N)) return {};
+  sk_epilogue epi;
+  bool used;
+  if (!epilogue(a[2], a[3], A, N, type, &epi, &used)) return {};
+  at::Tensor C = result(out, A, M, N, type);
+  if (!C.defined()) return {};
+  Launch l;
+  if (!l.find(M, N, K, SK_I8, SK_LAYOUT_NT)) return {};
+  const sk_scales scales{sa.data_ptr(), sb.data_ptr(), type == at::kBFloat16 ? SK_BF16 : SK_F16, 0};
+  const int rc = sk_gemm_i8_scaled(A.data_ptr(), B.data_ptr(), C.data_ptr(), M, N, K, A.stride(0), B.stride(0), C.stride(0), &scales, &l.plan,
+                                   l.ws.ptr, l.ws.bytes, l.stream, used ? &epi : nullptr);
+  return rc == SK_OK ? C : at::Tensor();
+}
+
 // operands A, Wq, scales, zeros; (zero, group, tiled, config, bias, activation).  One launch, row-major weights, as many rows as
 // the Q4 tile kernels serve -- a shape that the general implementation answers with several launches never has a plan here
 // under these types.
@@ -205,7 +232,7 @@ at::Tensor gemm_q4(const c10::IValue *operands, const at::Tensor *out, const c10
   return rc == SK_OK ? C : at::Tensor();
 }
 
-enum Op { F16, BF16, F32, F8, I8, Q4 };
+enum Op { F16, BF16, F32, F8, I8, Q4, I8_SCALED };
 
 // boxed implementation of streamk::gemm_* (OUT: its _out twin): the arguments stay on the stack until the call is answered
 template <Op OP, bool OUT>
@@ -213,7 +240,7 @@ void boxed(const c10::OperatorHandle &op, c10::DispatchKeySet, Stack *stack) {
   at::AutoDispatchBelowADInplaceOrView guard;   // (autograd is behind us, also for what is called from here)
   const size_t nargs = op.schema().arguments().size();
   const c10::IValue *args = stack->data() + (stack->size() - nargs);
-  constexpr int operands = OP == Q4 ? 4 : 2;
+  constexpr int operands = OP == Q4 || OP == I8_SCALED ? 4 : 2;
   const c10::IValue *rest = args + operands + (OUT ? 1 : 0);
   at::Tensor C;
   const at::Tensor *out = OUT ? &args[operands].toTensor() : nullptr;
@@ -223,6 +250,7 @@ void boxed(const c10::OperatorHandle &op, c10::DispatchKeySet, Stack *stack) {
   if constexpr (OP == F8) C = gemm_f8(args[0].toTensor(), args[1].toTensor(), out, rest);
   if constexpr (OP == I8) C = gemm_i8(args[0].toTensor(), args[1].toTensor(), out, rest);
   if constexpr (OP == Q4) C = gemm_q4(args, out, rest);
+  if constexpr (OP == I8_SCALED) C = gemm_i8_scaled(args, out, rest);
   if (!C.defined()) {
     static const c10::OperatorHandle general =
         c10::Dispatcher::singleton().findSchemaOrThrow((op.schema().name() + "_general").c_str(), "");
@@ -245,6 +273,7 @@ TORCH_LIBRARY_IMPL(streamk, CUDA, m) {
   IMPL(F8, "gemm_f8")
   IMPL(I8, "gemm_i8")
   IMPL(Q4, "gemm_q4")
+  IMPL(I8_SCALED, "gemm_i8_scaled")
 #undef IMPL
 }
 

@@ -6,7 +6,9 @@
     out = combine_rows(streamk_grouped(h, down, route.offsets), route)   # the weighted sum of each token's rows
 
 Every function is an operator of the `streamk` namespace and, under autograd, differentiable in its floating operands (the grouped
-product without bias and activation).  Sizes of groups stay on the device: no call waits for it.
+product without bias and activation).  Sizes of groups stay on the device: no call waits for it.  Ordinary calls run, and record their
+gradients, in native code (csrc/torch_ops_experts.cpp), which passes every other one on to the implementations here, registered as
+`<name>_general`; without the native library those and the autograd functions here stand in.
 """
 import ctypes
 from typing import NamedTuple
@@ -18,11 +20,15 @@ from . import _lib, ops
 _TYPES = {torch.float16: _lib.SK_F16, torch.bfloat16: _lib.SK_BF16}
 _MAX_EXPERTS, _MAX_CHOSEN = 1024, 64
 _ops = torch.ops.streamk
-_define = ops._LIBRARY.define
+_NATIVE = _lib.torch_lib() is not None
 
 
-def _implement(name, run, fake):
-    ops._LIBRARY.impl(name, run, "CUDA")
+def _operator(name, schema, run, fake):
+    """Defines streamk::<name> and <name>_general; run is the implementation of the latter, and of both without the native library."""
+    for suffix in ("", "_general"):
+        ops._LIBRARY.define(f"{name}{suffix}{schema}")
+        if suffix or not _NATIVE:
+            ops._LIBRARY.impl(name + suffix, run, "CUDA")
     torch.library.register_fake(f"streamk::{name}", fake, lib=ops._LIBRARY)
 
 
@@ -104,8 +110,6 @@ def _grouped(A, B, offsets, layout="nt", out_dtype=None, scale_a=None, scale_b=N
 
 
 _GROUPED_TAIL = "str layout=\"nt\", ScalarType? out_dtype=None, Tensor? scale_a=None, Tensor? scale_b=None, Tensor? bias=None, str activation=\"none\", int variant=0"
-_define(f"gemm_grouped(Tensor A, Tensor B, Tensor offsets, {_GROUPED_TAIL}) -> Tensor")
-_define(f"gemm_grouped_out(Tensor A, Tensor B, Tensor offsets, Tensor(a!) out, {_GROUPED_TAIL}) -> ()")
 
 
 def _grouped_fake(A, B, offsets, layout="nt", out_dtype=None, *rest):
@@ -116,8 +120,8 @@ def _grouped_out(A, B, offsets, out, layout="nt", out_dtype=None, scale_a=None, 
     _grouped(A, B, offsets, layout, out.dtype if out_dtype is None else out_dtype, scale_a, scale_b, bias, activation, variant, out)
 
 
-_implement("gemm_grouped", _grouped, _grouped_fake)
-_implement("gemm_grouped_out", _grouped_out, lambda *args: None)
+_operator("gemm_grouped", f"(Tensor A, Tensor B, Tensor offsets, {_GROUPED_TAIL}) -> Tensor", _grouped, _grouped_fake)
+_operator("gemm_grouped_out", f"(Tensor A, Tensor B, Tensor offsets, Tensor(a!) out, {_GROUPED_TAIL}) -> ()", _grouped_out, lambda *args: None)
 
 
 # ---- the gradient of its weights ----
@@ -150,16 +154,15 @@ def _wgrad(A, B, offsets, variant=0):
     return C
 
 
-_define("grouped_wgrad(Tensor A, Tensor B, Tensor offsets, int variant=0) -> Tensor")
-_implement("grouped_wgrad", _wgrad, lambda A, B, offsets, variant=0: A.new_empty((offsets.shape[0] - 1, A.shape[1], B.shape[1])))
+_operator("grouped_wgrad", "(Tensor A, Tensor B, Tensor offsets, int variant=0) -> Tensor", _wgrad, lambda A, B, offsets, variant=0: A.new_empty((offsets.shape[0] - 1, A.shape[1], B.shape[1])))
 
 
 class _GroupedProduct(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, A, B, offsets, layout):
+    def forward(ctx, A, B, offsets, layout, variant):
         ctx.save_for_backward(A, B, offsets)
         ctx.layout = layout
-        return _ops.gemm_grouped(A, B, offsets, layout)
+        return _ops.gemm_grouped(A, B, offsets, layout, variant=variant)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -173,7 +176,7 @@ class _GroupedProduct(torch.autograd.Function):
                 dA = _grouped_rows_grad(dC, B, offsets)
         if ctx.needs_input_grad[1]:
             dB = _ops.grouped_wgrad(dC, A, offsets) if ctx.layout == "nt" else _ops.grouped_wgrad(A, dC, offsets)
-        return dA, dB, None, None
+        return dA, dB, None, None, None
 
 
 def _grouped_rows_grad(dC, B, offsets):
@@ -197,7 +200,8 @@ def streamk_grouped(A, B, offsets, *, layout="nt", scale_a=None, scale_b=None, o
             raise ValueError("the grouped product has gradients only without bias, activation, scales and out")
         if out_dtype not in (None, A.dtype):
             raise ValueError(f"the result of {A.dtype} operands is {A.dtype}")
-        return _GroupedProduct.apply(A, B, offsets, layout)
+        if not _NATIVE:
+            return _GroupedProduct.apply(A, B, offsets, layout, variant)
     if out is None:
         return _ops.gemm_grouped(A, B, offsets, layout, out_dtype, scale_a, scale_b, bias, activation, variant)
     _ops.gemm_grouped_out(A, B, offsets, out, layout, out_dtype, scale_a, scale_b, bias, activation, variant)
@@ -260,10 +264,9 @@ def _route_backward(weights, experts, dweights, E, dtype):
     return dlogits
 
 
-_define("route_experts(Tensor logits, int k) -> (Tensor, Tensor, Tensor, Tensor, Tensor)")
-_implement("route_experts", _route, _route_fake)
-_define("route_backward(Tensor weights, Tensor experts, Tensor dweights, int E, ScalarType dtype) -> Tensor")
-_implement("route_backward", _route_backward, lambda weights, experts, dweights, E, dtype: weights.new_empty((weights.shape[0], E), dtype=dtype))
+_operator("route_experts", "(Tensor logits, int k) -> (Tensor, Tensor, Tensor, Tensor, Tensor)", _route, _route_fake)
+_operator("route_backward", "(Tensor weights, Tensor experts, Tensor dweights, int E, ScalarType dtype) -> Tensor", _route_backward,
+          lambda weights, experts, dweights, E, dtype: weights.new_empty((weights.shape[0], E), dtype=dtype))
 
 
 class _RouteExperts(torch.autograd.Function):
@@ -286,7 +289,7 @@ def route_experts(logits, k):
     """Route of the tokens whose router logits are [T, E] (float32, float16 or bfloat16): the k largest of each, the largest first, equal
     ones by number.  -inf and NaN are never chosen: a token with fewer others has -1 and weight 0 in its last places, and one with none
     goes to no expert.  Differentiable: weights to logits."""
-    if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
+    if not _NATIVE and torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
         return Route(*_RouteExperts.apply(logits, k))
     return Route(*_ops.route_experts(logits, k))
 
@@ -341,13 +344,17 @@ def _combine_backward(d_out, y, order, place, weights):
     return dy, dweights
 
 
-_define("dispatch_rows(Tensor x, Tensor order, int k) -> Tensor")
-_implement("dispatch_rows", _dispatch, lambda x, order, k: x.new_empty((order.shape[0], *x.shape[1:])))
-_define("combine_rows(Tensor y, Tensor place, Tensor? weights=None) -> Tensor")
-_implement("combine_rows", _combine, lambda y, place, weights=None: y.new_empty((place.shape[0], y.shape[1])))
-_define("combine_backward(Tensor d_out, Tensor y, Tensor order, Tensor place, Tensor weights) -> (Tensor, Tensor)")
-_implement("combine_backward", _combine_backward,
-           lambda d_out, y, order, place, weights: (y.new_empty(y.shape), weights.new_empty(weights.shape)))
+_dispatch_fake = lambda x, order, k: x.new_empty((order.shape[0], *x.shape[1:]))  # noqa: E731
+_combine_fake = lambda y, place, weights=None: y.new_empty((place.shape[0], y.shape[1]))  # noqa: E731
+_operator("dispatch_rows", "(Tensor x, Tensor order, int k) -> Tensor", _dispatch, _dispatch_fake)
+_operator("combine_rows", "(Tensor y, Tensor place, Tensor? weights=None) -> Tensor", _combine, _combine_fake)
+_operator("combine_backward", "(Tensor d_out, Tensor y, Tensor order, Tensor place, Tensor weights) -> (Tensor, Tensor)", _combine_backward,
+          lambda d_out, y, order, place, weights: (y.new_empty(y.shape), weights.new_empty(weights.shape)))
+# the same with all of a route that their gradients need
+_operator("dispatch_routed", "(Tensor x, Tensor order, Tensor place) -> Tensor", lambda x, order, place: _dispatch(x, order, place.shape[1]),
+          lambda x, order, place: _dispatch_fake(x, order, place.shape[1]))
+_operator("combine_routed", "(Tensor y, Tensor weights, Tensor order, Tensor place) -> Tensor",
+          lambda y, weights, order, place: _combine(y, place, weights), lambda y, weights, order, place: _combine_fake(y, place))
 
 
 class _DispatchRows(torch.autograd.Function):
@@ -381,13 +388,14 @@ def dispatch_rows(x, route):
     the rows behind route.offsets[E].  Differentiable in x (float16 or bfloat16, two dimensions)."""
     if torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad:
         _on_device(x, "x", tuple(_TYPES), 2)
-        return _DispatchRows.apply(x, route.order, route.place)
-    return _ops.dispatch_rows(x, route.order, route.place.shape[1])
+        if not _NATIVE:
+            return _DispatchRows.apply(x, route.order, route.place)
+    return _ops.dispatch_routed(x, route.order, route.place)
 
 
 def combine_rows(y, route):
     """out[t] = sum over its experts of their weight times their row of y: [T, H] for y [T k, H] (float16 or bfloat16) in the experts' order;
     added in fp32, rounded once; a token without experts gets zeros.  Differentiable in y and route.weights."""
-    if torch.is_grad_enabled() and isinstance(y, torch.Tensor) and (y.requires_grad or route.weights.requires_grad):
+    if not _NATIVE and torch.is_grad_enabled() and isinstance(y, torch.Tensor) and (y.requires_grad or route.weights.requires_grad):
         return _CombineRows.apply(y, route.weights, route.order, route.place)
-    return _ops.combine_rows(y, route.place, route.weights)
+    return _ops.combine_routed(y, route.weights, route.order, route.place)

@@ -44,9 +44,7 @@ def _run_i8_scaled(A, B, scale_a, scale_b, C, out_dtype, config="", bias=None, a
 
 
 ops._register("gemm_i8_scaled", "Tensor A, Tensor B, Tensor scale_a, Tensor scale_b", f"ScalarType out_dtype, str config=\"\", {ops._EPI}",
-              _run_i8_scaled, lambda A, B, sa, sb, out_dtype, *rest: ((A.shape[0], B.shape[0]), out_dtype), native=False)
-
-ops._LIBRARY.define("quantize_i8(Tensor x) -> (Tensor, Tensor)")
+              _run_i8_scaled, lambda A, B, sa, sb, out_dtype, *rest: ((A.shape[0], B.shape[0]), out_dtype))
 
 
 def _check_quantised(x):
@@ -76,7 +74,10 @@ def _quantize(x):
     return q, scale
 
 
-ops._LIBRARY.impl("quantize_i8", _quantize, "CUDA")
+for _suffix in ("", "_general"):   # (the native implementation passes what is not ordinary on)
+    ops._LIBRARY.define(f"quantize_i8{_suffix}(Tensor x) -> (Tensor, Tensor)")
+    if _suffix or _lib.torch_lib() is None:
+        ops._LIBRARY.impl("quantize_i8" + _suffix, _quantize, "CUDA")
 torch.library.register_fake("streamk::quantize_i8", lambda x: (x.new_empty(x.shape, dtype=torch.int8), x.new_empty(x.shape[:-1], dtype=torch.float32)),
                             lib=ops._LIBRARY)
 

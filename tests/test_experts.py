@@ -569,3 +569,58 @@ def test_tiles_that_are_cut_along_k(sk, kind, variant, sizes, N, K):
     for _ in range(5):
         assert torch.equal(run(), C)
     sk.workspace_status()
+
+
+@pytest.mark.gpu
+def test_operators_pass_opcheck(sk):
+    o, check = torch.ops.streamk, torch.library.opcheck
+    tests = ("test_schema", "test_faketensor", "test_aot_dispatch_dynamic")
+    A, B, offsets = rand((20, 64), torch.float16, 1), rand((2, 32, 64), torch.float16, 2), offsets_of([12, 8])
+    route = sk.route_experts(rand((10, 4), torch.float32, 3), 2)
+    check(o.gemm_grouped, (A, B, offsets), test_utils=tests)
+    check(o.gemm_grouped, (A.detach().requires_grad_(), B.detach().requires_grad_(), offsets), test_utils=tests)
+    check(o.grouped_wgrad, (A[:, :32].contiguous(), A, offsets), test_utils=tests)
+    check(o.route_experts, (rand((10, 4), torch.float32, 3), 2), test_utils=tests)
+    check(o.dispatch_routed, (rand((10, 64), torch.float16, 4), route.order, route.place), test_utils=tests)
+    check(o.combine_routed, (A, route.weights, route.order, route.place), test_utils=tests)
+    check(o.quantize_i8, (A,), test_utils=tests)
+    q, s = sk.quantize_int8(A)
+    check(o.gemm_i8_scaled, (q, q, s, s, torch.float16), test_utils=tests)
+
+
+@pytest.mark.gpu
+def test_native_operators_answer_like_the_general_ones(sk):
+    """The two implementations of every operator, on ordinary operands and on ones that the native one passes on."""
+    o = torch.ops.streamk
+    A, B, offsets = rand((20, 64), torch.float16, 1), rand((2, 32, 64), torch.float16, 2), offsets_of([12, 8])
+    wide = torch.zeros(20, 80, dtype=torch.float16, device="cuda")
+    wide[:, 1:65] = A
+    logits, place = rand((10, 4), torch.float32, 3), None
+    route = sk.route_experts(logits, 2)
+    q, s = sk.quantize_int8(A)
+    w, sw = sk.quantize_int8(B)
+    calls = [("gemm_grouped", (A, B, offsets)), ("gemm_grouped", (wide[:, 1:65], B, offsets)), ("gemm_grouped", (A[:1], B, offsets_of([1, 0]))), ("gemm_grouped", (A[:0], B, offsets_of([0, 0]))),
+             ("gemm_grouped", (A, B, offsets, "nt", None, None, None, rand((2, 32), torch.float16, 5), "silu")), ("gemm_grouped", (A, B[:, :1], offsets)),
+             ("gemm_grouped", (q, w, offsets, "nt", torch.bfloat16, s, sw)), ("gemm_grouped", (q, w, offsets, "nt", None, s, sw)), ("gemm_grouped", (A, rand((2, 64, 32), torch.float16, 6), offsets, "nn")),
+             ("grouped_wgrad", (A, A, offsets)), ("grouped_wgrad", (wide[:, :77], A, offsets)), ("route_experts", (logits, 2)), ("route_experts", (logits[:, 1:], 3)), ("route_experts", (logits.half(), 1)),
+             ("route_backward", (route.weights, route.experts, route.weights, 4, torch.float32)), ("dispatch_rows", (A[:10], route.order, 2)), ("dispatch_rows", (wide[:10, 1:65], route.order, 2)),
+             ("dispatch_rows", (s[:10].contiguous(), route.order, 2)), ("combine_rows", (A, route.place, route.weights)), ("combine_rows", (A, route.place)), ("combine_rows", (wide[:, 1:65], route.place)),
+             ("combine_backward", (A[:10], A, route.order, route.place, route.weights)), ("combine_backward", (A[:1].expand(10, 64), A, route.order, route.place, route.weights)),
+             ("quantize_i8", (A,)), ("quantize_i8", (wide[:, 1:65],)), ("quantize_i8", (B,))]
+    for name, args in calls:
+        got, want = getattr(o, name)(*args), getattr(o, name + "_general")(*args)
+        for a, b in zip(got if isinstance(got, (tuple, list)) else [got], want if isinstance(want, (tuple, list)) else [want]):
+            assert a.dtype == b.dtype and a.shape == b.shape and torch.equal(a, b), name
+    out, ref = torch.empty(20, 40, dtype=torch.float16, device="cuda"), torch.empty(20, 40, dtype=torch.float16, device="cuda")
+    o.gemm_grouped_out(A, B, offsets, out[:, :32])
+    o.gemm_grouped_out_general(A, B, offsets, ref[:, :32])
+    assert torch.equal(out[:, :32], ref[:, :32])
+
+
+@pytest.mark.gpu
+def test_gradients_of_gradients_are_refused(sk):
+    A, B, offsets = rand((20, 64), torch.float16, 1).requires_grad_(), rand((2, 32, 64), torch.float16, 2), offsets_of([12, 8])
+    C = sk.streamk_grouped(A, B, offsets)
+    with pytest.raises(RuntimeError):
+        g, = torch.autograd.grad(C.float().square().sum(), A, create_graph=True)
+        g.sum().backward()
