@@ -467,7 +467,8 @@ int sk_grouped_wgrad(const void *A, const void *B, const void *offsets, void *C,
  *   place [T, k]     the sorted row of each slot, -1 without an expert
  * (all int32).  ws: sk_route_workspace_bytes(T, E, k) of scratch (0 is possible), no initialisation needed.
  * sk_route_backward: dlogits [T, E] (dtype, contiguous) of the weights' gradient dweights [T, k] fp32.
- * sk_dispatch_rows: rows[p] = row order[p] / k of x, any type by bytes; zeros where order[p] is negative.
+ * sk_dispatch_rows: rows[p] = row order[p] / k of x, any type by bytes; zeros where order[p] is negative.  place: the route's, or null
+ * (with it many tokens are read once each).
  * sk_combine_rows: out[t] = sum over j of weights[t][j] * y[place[t][j]] (weights null: 1), SK_F16 or SK_BF16, [T * k, H] to [T, H],
  * added in fp32 in the order of j.  With weights null it is the gradient of sk_dispatch_rows.
  * sk_combine_backward: dy [T * k, H] (zeros for rows without a slot) and dweights [T, k] of sk_combine_rows.
@@ -477,7 +478,8 @@ int sk_route_experts(const void *logits, int dtype, int64_t T, int64_t E, int64_
                      void *order, void *place, void *ws, size_t ws_bytes, void *stream);
 int sk_route_backward(const void *weights, const void *experts, const void *dweights, int64_t T, int64_t E, int64_t k, int dtype,
                       void *dlogits, void *stream);
-int sk_dispatch_rows(const void *x, int64_t row_bytes, int64_t x_pitch, const void *order, int64_t T, int64_t k, void *rows, void *stream);
+int sk_dispatch_rows(const void *x, int64_t row_bytes, int64_t x_pitch, const void *order, const void *place, int64_t T, int64_t k, void *rows,
+                     void *stream);
 int sk_combine_rows(const void *y, int dtype, const void *place, const void *weights, int64_t T, int64_t k, int64_t H, void *out, void *stream);
 int sk_combine_backward(const void *d_out, const void *y, int dtype, const void *order, const void *place, const void *weights, int64_t T,
                         int64_t k, int64_t H, void *dy, void *dweights, void *stream);

@@ -37,18 +37,6 @@ __device__ __forceinline__ void store_el(void *p, int64_t i, float x) {
   }
 }
 
-// the largest value of a wave's lanes, in every lane
-__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-#define SK_MAX_STEP(CTRL, ROWS) x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false))
-  SK_MAX_STEP(0x111, 0xf);   // rows of 16 lanes: from 1, 2, 4, 8 lanes below; then the last lane of a row to the next row, and of
-  SK_MAX_STEP(0x112, 0xf);   // the lower half to the upper
-  SK_MAX_STEP(0x114, 0xf);
-  SK_MAX_STEP(0x118, 0xf);
-  SK_MAX_STEP(0x142, 0xa);
-  SK_MAX_STEP(0x143, 0xc);
-#undef SK_MAX_STEP
-  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
-}
 __device__ __forceinline__ float wave_sum(float x) {
 #pragma unroll
   for (int d = 32; d > 0; d /= 2) x += __shfl_xor(x, d, 64);
@@ -222,14 +210,16 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void route_few_kernel(RouteArgs a) 
   place_slots<FEW_WAVES>(a, experts, 0, n, have);
 }
 
-constexpr int WAVES = 4;
+// More tokens: choice and counts by blocks, then places.  8192 tokens, 8 of 64 experts: 4 and 9 us (four waves a block for the choice 28 us:
+// a token is a chain of k reductions).
+constexpr int WAVES = 4, CHOOSE_WAVES = 16;
 template <int EL, int S>
-__global__ __launch_bounds__(64 * WAVES) void route_choose_kernel(RouteArgs a) {
+__global__ __launch_bounds__(64 * CHOOSE_WAVES) void route_choose_kernel(RouteArgs a) {
   extern __shared__ int lds[];   // [E] counts of the block
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t0 = blockIdx.x * a.tokens, t1 = min(a.T, t0 + a.tokens);
-  for (int e = threadIdx.x; e < a.E; e += 64 * WAVES) lds[e] = 0;
+  for (int e = threadIdx.x; e < a.E; e += 64 * CHOOSE_WAVES) lds[e] = 0;
   __syncthreads();
-  for (int t = t0 + wave; t < t1; t += WAVES) {
+  for (int t = t0 + wave; t < t1; t += CHOOSE_WAVES) {
     int e;
     float w;
     choose<EL, S>(a.logits, a.ld, t, a.E, a.k, e, w);
@@ -240,7 +230,7 @@ __global__ __launch_bounds__(64 * WAVES) void route_choose_kernel(RouteArgs a) {
     }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < a.E; e += 64 * WAVES) a.counts[(int64_t)blockIdx.x * a.E + e] = lds[e];
+  for (int e = threadIdx.x; e < a.E; e += 64 * CHOOSE_WAVES) a.counts[(int64_t)blockIdx.x * a.E + e] = lds[e];
 }
 // every block adds up the counts of all blocks, and of those in front of it, by itself
 __global__ __launch_bounds__(64 * WAVES) void route_place_kernel(RouteArgs a) {
@@ -248,15 +238,25 @@ __global__ __launch_bounds__(64 * WAVES) void route_place_kernel(RouteArgs a) {
   int *have = lds, *total = have + WAVES * a.E, *front = total + a.E, *word = front + a.E;
   const int t0 = blockIdx.x * a.tokens, t1 = min(a.T, t0 + a.tokens), slot0 = t0 * a.k, n = (t1 - t0) * a.k;
   const int *experts = a.experts + slot0;
-  for (int e = threadIdx.x; e < a.E; e += 64 * WAVES) {
+  for (int e = threadIdx.x; e < a.E; e += 64 * WAVES) total[e] = front[e] = 0;
+  __syncthreads();
+  // (SHARE threads to an expert, eight counts in flight each)
+  constexpr int SHARE = 16;
+  for (int i = threadIdx.x; i < SHARE * a.E; i += 64 * WAVES) {
+    const int e = (int)((unsigned)i % (unsigned)a.E), share = (int)((unsigned)i / (unsigned)a.E), blocks = (int)gridDim.x;
     int sum = 0, before = 0;
-    for (int b = 0; b < (int)gridDim.x; ++b) {
-      const int c = a.counts[(int64_t)b * a.E + e];
-      before += b < (int)blockIdx.x ? c : 0;
-      sum += c;
+    for (int b0 = share; b0 < blocks; b0 += 8 * SHARE) {
+      int c[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c[j] = b0 + j * SHARE < blocks ? a.counts[(int64_t)(b0 + j * SHARE) * a.E + e] : 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        sum += c[j];
+        before += b0 + j * SHARE < (int)blockIdx.x ? c[j] : 0;
+      }
     }
-    total[e] = sum;
-    front[e] = before;
+    atomicAdd(&total[e], sum);
+    atomicAdd(&front[e], before);
   }
   __syncthreads();
   count_parts<WAVES>(experts, n, a.E, have);
@@ -276,7 +276,7 @@ __global__ __launch_bounds__(64 * WAVES) void route_place_kernel(RouteArgs a) {
   place_slots<WAVES>(a, experts, slot0, n, have);
 }
 
-constexpr int MOST_BLOCKS = 128;   // (each of which reads all blocks' counts)
+constexpr int MOST_BLOCKS = 256;   // (each of which reads all blocks' counts)
 int route_tokens(int64_t T) {
   int64_t tokens = (T + MOST_BLOCKS - 1) / MOST_BLOCKS;
   if (tokens < 16) tokens = 16;
@@ -293,7 +293,7 @@ int launch_route(const RouteArgs &a, int blocks, hipStream_t s) {
     hipLaunchKernelGGL((route_few_kernel<EL, S>), dim3(1), dim3(64 * FEW_WAVES), lds, s, a);
     return (int)hipGetLastError();
   }
-  hipLaunchKernelGGL((route_choose_kernel<EL, S>), dim3(blocks), dim3(64 * WAVES), sizeof(int) * a.E, s, a);
+  hipLaunchKernelGGL((route_choose_kernel<EL, S>), dim3(blocks), dim3(64 * CHOOSE_WAVES), sizeof(int) * a.E, s, a);
   if (hipGetLastError() != hipSuccess) return 1;
   hipLaunchKernelGGL(route_place_kernel, dim3(blocks), dim3(64 * WAVES), sizeof(int) * ((WAVES + 2) * a.E + 1), s, a);
   return (int)hipGetLastError();
@@ -354,6 +354,39 @@ __global__ __launch_bounds__(64 * WAVES) void dispatch_kernel(const Unit *x, int
   for (; i < units; i += 64) dst[i] = src[i];
 }
 
+// The same by tokens: one wave reads a token's row once and stores it to each of its places; the waves also clear the rows without a
+// slot.  8192 tokens of 4 KB to 65536 rows: 62 us, by rows 71.
+template <class Unit>
+__global__ __launch_bounds__(64 * WAVES) void dispatch_tokens_kernel(const Unit *x, int64_t ldx, const int *order, const int *place, int T, int k,
+                                                                     int units, Unit *out) {
+  const int lane = threadIdx.x & 63;
+  const int64_t t = (int64_t)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), rows = (int64_t)T * k;
+  if (t >= T) return;
+  const Unit *src = x + t * ldx;
+  const int mine = lane < k ? place[t * k + lane] : -1, at = lane < k ? order[t * k + lane] : 0;   // (k <= 64)
+  for (int i0 = 0; i0 < units; i0 += 256) {
+    Unit u[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (i0 + 64 * q + lane < units) u[q] = src[i0 + 64 * q + lane];
+    for (int j = 0; j < k; ++j) {
+      const int p = __builtin_amdgcn_readlane(mine, j);
+      if (p >= 0 && p < rows) {
+        Unit *dst = out + (int64_t)p * units + i0 + lane;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (i0 + 64 * q + lane < units) dst[64 * q] = u[q];
+      }
+      if (__builtin_amdgcn_readlane(at, j) < 0) {
+        Unit *dst = out + (t * k + j) * units + i0 + lane;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (i0 + 64 * q + lane < units) dst[64 * q] = Unit{};
+      }
+    }
+  }
+}
+
 typedef uint16_t ushort8v __attribute__((ext_vector_type(8)));
 template <bool BF16>
 __device__ __forceinline__ float widen(uint16_t bits) {
@@ -386,27 +419,40 @@ __device__ __forceinline__ void store8(uint16_t *row, int c, int H, ushort8v v) 
   }
 }
 
-// out[t] = sum_j w[t][j] y[place[t][j]] (weights null: 1), j ascending; a thread eight columns
+// out[t] = sum_j w[t][j] y[place[t][j]] (weights null: 1), j ascending; a wave takes 512 columns of a token, a thread eight.  8192 tokens,
+// 8 rows of 4 KB each: 57 us, 5.3 TB/s (rows in the tokens' order 54).
 template <bool BF16, bool VEC>
-__global__ __launch_bounds__(64) void combine_kernel(const uint16_t *y, const int *place, const float *weights, int k, int H, int64_t rows,
-                                                     uint16_t *out, int blocks_x) {
-  const int64_t t = blockIdx.x / blocks_x;
-  const int c = ((int)(blockIdx.x % blocks_x) * 64 + threadIdx.x) * 8;
-  if (c >= H) return;
-  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int j = 0; j < k; ++j) {
-    const int p = place[t * k + j];   // (uniform)
-    if (p < 0 || p >= rows) continue;
-    const float w = weights ? weights[t * k + j] : 1.f;
-    const ushort8v v = load8<VEC>(y + (int64_t)p * H, c, H);
+__global__ __launch_bounds__(64 * WAVES) void combine_kernel(const uint16_t *y, const int *place, const float *weights, int k, int H, int64_t T,
+                                                             uint16_t *out, int pieces) {
+  const int64_t item = (int64_t)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), t = item / pieces, rows = T * k;
+  if (t >= T) return;
+  const int c = ((int)(item - t * pieces) * 64 + (threadIdx.x & 63)) * 8;
+  if (c < H) {
+    float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    // eight rows in flight; a slot without an expert reads row 0, whose values are not used
+    for (int j0 = 0; j0 < k; j0 += 8) {
+      ushort8v v[8];
+      float w[8];
+      bool used[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum[e] = fmaf(w, widen<BF16>(v[e]), sum[e]);
+      for (int j = 0; j < 8; ++j) {
+        const int p = j0 + j < k ? place[t * k + j0 + j] : -1;   // (uniform)
+        used[j] = p >= 0 && p < rows;
+        w[j] = used[j] && weights ? weights[t * k + j0 + j] : 1.f;
+        if (j0 + j < k) v[j] = load8<VEC>(y + (int64_t)(used[j] ? p : 0) * H, c, H);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (used[j]) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum[e] = fmaf(w[j], widen<BF16>(v[j][e]), sum[e]);
+        }
+    }
+    ushort8v o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = narrow<BF16>(sum[e]);
+    store8<VEC>(out + t * H, c, H, o);
   }
-  ushort8v o;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) o[e] = narrow<BF16>(sum[e]);
-  store8<VEC>(out + t * H, c, H, o);
 }
 
 // dy[p] = w d_out[t], dw[slot] = <d_out[t], y[p]> for the slot of p; one wave per slot.  Row number `slot` without a slot: zeros.
@@ -488,18 +534,31 @@ extern "C" int sk_route_backward(const void *weights, const void *experts, const
   return launched();
 }
 
-extern "C" int sk_dispatch_rows(const void *x, int64_t row_bytes, int64_t x_pitch, const void *order, int64_t T, int64_t k, void *rows, void *stream) {
+extern "C" int sk_dispatch_rows(const void *x, int64_t row_bytes, int64_t x_pitch, const void *order, const void *place, int64_t T, int64_t k, void *rows,
+                                void *stream) {
   if (!x || !order || !rows) return SK_ERR_NULL;
   if (T <= 0 || k <= 0 || T * k > 0x7fffffff / 2 || row_bytes <= 0 || row_bytes > 0x7fffffff || x_pitch < row_bytes) return SK_ERR_SHAPE;
   const int64_t n = T * k;
   const dim3 grid((unsigned)((n + WAVES - 1) / WAVES)), block(64 * WAVES);
   const uint64_t all = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(rows) | (uint64_t)row_bytes | (uint64_t)x_pitch;
-#define SK_DISPATCH(UNIT)                                                                                                        \
-  hipLaunchKernelGGL((dispatch_kernel<UNIT>), grid, block, 0, (hipStream_t)stream, (const UNIT *)x, x_pitch / (int64_t)sizeof(UNIT), \
-                     (const int *)order, (int)T, (int)k, n, (int)(row_bytes / (int64_t)sizeof(UNIT)), (UNIT *)rows)
-  if (all % 16 == 0) SK_DISPATCH(uint4v);
-  else if (all % 4 == 0) SK_DISPATCH(uint32_t);
-  else SK_DISPATCH(uint8_t);
+  // (many tokens: fewer waves than rows fill the device)
+  const bool by_tokens = place && k <= MAX_CHOSEN && T >= 2048;
+  const dim3 tokens_grid((unsigned)((T + WAVES - 1) / WAVES));
+#define SK_DISPATCH(UNIT)                                                                                                            \
+  if (by_tokens)                                                                                                                     \
+    hipLaunchKernelGGL((dispatch_tokens_kernel<UNIT>), tokens_grid, block, 0, (hipStream_t)stream, (const UNIT *)x,                   \
+                       x_pitch / (int64_t)sizeof(UNIT), (const int *)order, (const int *)place, (int)T, (int)k,                       \
+                       (int)(row_bytes / (int64_t)sizeof(UNIT)), (UNIT *)rows);                                                       \
+  else                                                                                                                               \
+    hipLaunchKernelGGL((dispatch_kernel<UNIT>), grid, block, 0, (hipStream_t)stream, (const UNIT *)x, x_pitch / (int64_t)sizeof(UNIT), \
+                       (const int *)order, (int)T, (int)k, n, (int)(row_bytes / (int64_t)sizeof(UNIT)), (UNIT *)rows)
+  if (all % 16 == 0) {
+    SK_DISPATCH(uint4v);
+  } else if (all % 4 == 0) {
+    SK_DISPATCH(uint32_t);
+  } else {
+    SK_DISPATCH(uint8_t);
+  }
 #undef SK_DISPATCH
   return launched();
 }
@@ -509,12 +568,13 @@ extern "C" int sk_combine_rows(const void *y, int dtype, const void *place, cons
   if (dtype != SK_F16 && dtype != SK_BF16) return SK_ERR_CONFIG;
   if (!y || !place || !out) return SK_ERR_NULL;
   if (T <= 0 || k <= 0 || H <= 0 || T * k > 0x7fffffff / 2 || H > 0x7fffff00) return SK_ERR_SHAPE;
-  const int blocks_x = (int)((H + 511) / 512);
-  if (T * blocks_x > 0x7fffffff) return SK_ERR_SHAPE;
+  const int pieces = (int)((H + 511) / 512);
+  const int64_t blocks = (T * pieces + WAVES - 1) / WAVES;
+  if (blocks > 0x7fffffff) return SK_ERR_SHAPE;
   const bool vec = H % 8 == 0 && aligned16(y) && aligned16(out);
-#define SK_COMBINE(BF, VEC)                                                                                                           \
-  hipLaunchKernelGGL((combine_kernel<BF, VEC>), dim3((unsigned)(T * blocks_x)), dim3(64), 0, (hipStream_t)stream, (const uint16_t *)y, \
-                     (const int *)place, (const float *)weights, (int)k, (int)H, T * k, (uint16_t *)out, blocks_x)
+#define SK_COMBINE(BF, VEC)                                                                                                            \
+  hipLaunchKernelGGL((combine_kernel<BF, VEC>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, (hipStream_t)stream, (const uint16_t *)y,   \
+                     (const int *)place, (const float *)weights, (int)k, (int)H, T, (uint16_t *)out, pieces)
   if (dtype == SK_BF16) {
     if (vec) SK_COMBINE(true, true);
     else SK_COMBINE(true, false);

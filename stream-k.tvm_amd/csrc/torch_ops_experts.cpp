@@ -7,6 +7,7 @@
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/core/LegacyTypeDispatch.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -43,7 +44,11 @@ int64_t pitch(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1);
 bool is_ints(const Tensor &t, const Tensor &like, int64_t dim) {
   return t.scalar_type() == at::kInt && t.dim() == dim && t.is_contiguous() && t.device() == like.device();
 }
-Tensor ints(const Tensor &like, at::IntArrayRef shape) { return at::empty(shape, like.options().dtype(at::kInt)); }
+// a new tensor on the device of another one: the allocator's own entry, half a microsecond less than the dispatcher's
+Tensor fresh(const Tensor &like, at::IntArrayRef shape, at::ScalarType type) {
+  return Tensor(at::detail::empty_cuda(shape, type, like.device(), std::nullopt));
+}
+Tensor ints(const Tensor &like, at::IntArrayRef shape) { return fresh(like, shape, at::kInt); }
 
 template <class F>
 auto general(const char *name) {
@@ -64,7 +69,7 @@ std::tuple<Tensor, Tensor> quantize_i8(const Tensor &x) {
   at::AutoDispatchBelowADInplaceOrView guard;
   if (x.is_cuda() && is16(x) && x.dim() >= 1 && x.numel() > 0 && x.is_contiguous()) {
     const int64_t K = x.size(-1), M = x.numel() / K;
-    Tensor q = at::empty(x.sizes(), x.options().dtype(at::kChar)), scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+    Tensor q = fresh(x, x.sizes(), at::kChar), scale = fresh(x, x.sizes().slice(0, x.dim() - 1), at::kFloat);
     if (sk_quantize_i8(x.data_ptr(), dtype_of(x.scalar_type()), M, K, K, q.data_ptr(), K, scale.data_ptr(), current_stream()) == SK_OK) return {q, scale};
   }
   GENERAL("quantize_i8", decltype(quantize_i8), x);
@@ -96,7 +101,7 @@ bool grouped(const Tensor &A, const Tensor &B, const Tensor &offsets, std::strin
   if (C.defined()) {
     if (!C.is_cuda() || C.scalar_type() != out || C.dim() != 2 || C.size(0) != R || C.size(1) != N || C.stride(1) != 1 || (R > 1 && C.stride(0) < N) || C.device() != A.device()) return false;
   } else {
-    C = at::empty({R, N}, A.options().dtype(out));
+    C = fresh(A, {R, N}, out);
   }
   g.dtype = dtype_of(type);
   g.layout = nn ? SK_LAYOUT_NN : SK_LAYOUT_NT;
@@ -139,7 +144,7 @@ Tensor grouped_wgrad(const Tensor &A, const Tensor &B, const Tensor &offsets, in
   if (is16(A) && B.scalar_type() == A.scalar_type() && rows_in_place(A) && rows_in_place(B) && A.size(0) == B.size(0) && A.device() == B.device() &&
       A.size(1) % 8 == 0 && B.size(1) % 8 == 0 && A.size(1) > 0 && B.size(1) > 0 && is_ints(offsets, A, 1) && offsets.size(0) >= 2) {
     const int64_t E = offsets.size(0) - 1, M = A.size(1), N = B.size(1);
-    Tensor C = at::empty({E, M, N}, A.options());
+    Tensor C = fresh(A, {E, M, N}, A.scalar_type());
     if (sk_grouped_wgrad(A.data_ptr(), B.data_ptr(), offsets.data_ptr(), C.data_ptr(), dtype_of(A.scalar_type()), E, A.size(0), M, N, pitch(A), pitch(B),
                          (int)variant, current_stream()) == SK_OK)
       return C;
@@ -154,11 +159,11 @@ FiveTensors route_experts(const Tensor &logits, int64_t k) {
   const int dtype = dtype_of(logits.scalar_type());
   if (logits.is_cuda() && dtype >= 0 && dtype != SK_I8 && logits.dim() == 2 && logits.size(0) > 0 && logits.is_contiguous() && k >= 1 && k <= logits.size(1)) {
     const int64_t T = logits.size(0), E = logits.size(1);
-    Tensor weights = at::empty({T, k}, logits.options().dtype(at::kFloat)), experts = ints(logits, {T, k}), offsets = ints(logits, {E + 1}),
+    Tensor weights = fresh(logits, {T, k}, at::kFloat), experts = ints(logits, {T, k}), offsets = ints(logits, {E + 1}),
            order = ints(logits, {T * k}), place = ints(logits, {T, k});
     const size_t bytes = sk_route_workspace_bytes(T, E, k);
     Tensor ws;
-    if (bytes > 0) ws = at::empty({(int64_t)bytes}, logits.options().dtype(at::kByte));
+    if (bytes > 0) ws = fresh(logits, {(int64_t)bytes}, at::kByte);
     if (sk_route_experts(logits.data_ptr(), dtype, T, E, k, E, weights.data_ptr(), experts.data_ptr(), offsets.data_ptr(), order.data_ptr(), place.data_ptr(),
                          bytes > 0 ? ws.data_ptr() : nullptr, bytes, current_stream()) == SK_OK)
       return {weights, experts, offsets, order, place};
@@ -170,28 +175,40 @@ Tensor route_backward(const Tensor &weights, const Tensor &experts, const Tensor
   if (weights.is_cuda() && weights.scalar_type() == at::kFloat && weights.dim() == 2 && weights.size(0) > 0 && weights.is_contiguous() && is_ints(experts, weights, 2) &&
       experts.sizes() == weights.sizes() && dweights.scalar_type() == at::kFloat && dweights.sizes() == weights.sizes() && dweights.is_contiguous() &&
       dweights.device() == weights.device() && dtype_of(dtype) >= 0) {
-    Tensor dlogits = at::empty({weights.size(0), E}, weights.options().dtype(dtype));
+    Tensor dlogits = fresh(weights, {weights.size(0), E}, dtype);
     if (sk_route_backward(weights.data_ptr(), experts.data_ptr(), dweights.data_ptr(), weights.size(0), E, weights.size(1), dtype_of(dtype), dlogits.data_ptr(),
                           current_stream()) == SK_OK)
       return dlogits;
   }
   GENERAL("route_backward", decltype(route_backward), weights, experts, dweights, E, dtype);
 }
+// (place undefined: none) an undefined tensor: not the ordinary case
+Tensor dispatched(const Tensor &x, const Tensor &order, const Tensor &place, int64_t k) {
+  if (!x.is_cuda() || (x.dim() != 1 && x.dim() != 2) || x.numel() == 0 || !x.is_contiguous() || k < 1 || !is_ints(order, x, 1) || order.size(0) != x.size(0) * k) return {};
+  const int64_t T = x.size(0), width = x.dim() == 2 ? x.size(1) : 1, bytes = width * (int64_t)x.element_size();
+  if (place.defined() && (!is_ints(place, x, 2) || place.size(0) != T || place.size(1) != k)) return {};
+  Tensor rows = x.dim() == 2 ? fresh(x, {T * k, width}, x.scalar_type()) : fresh(x, {T * k}, x.scalar_type());
+  const int rc = sk_dispatch_rows(x.data_ptr(), bytes, bytes, order.data_ptr(), place.defined() ? place.data_ptr() : nullptr, T, k, rows.data_ptr(), current_stream());
+  return rc == SK_OK ? rows : Tensor();
+}
 Tensor dispatch_rows(const Tensor &x, const Tensor &order, int64_t k) {
   at::AutoDispatchBelowADInplaceOrView guard;
-  if (x.is_cuda() && (x.dim() == 1 || x.dim() == 2) && x.numel() > 0 && x.is_contiguous() && k >= 1 && is_ints(order, x, 1) && order.size(0) == x.size(0) * k) {
-    const int64_t T = x.size(0), width = x.dim() == 2 ? x.size(1) : 1, bytes = width * (int64_t)x.element_size();
-    Tensor rows = x.dim() == 2 ? at::empty({T * k, width}, x.options()) : at::empty({T * k}, x.options());
-    if (sk_dispatch_rows(x.data_ptr(), bytes, bytes, order.data_ptr(), T, k, rows.data_ptr(), current_stream()) == SK_OK) return rows;
-  }
+  const Tensor rows = dispatched(x, order, Tensor(), k);
+  if (rows.defined()) return rows;
   GENERAL("dispatch_rows", decltype(dispatch_rows), x, order, k);
+}
+Tensor dispatch_routed(const Tensor &x, const Tensor &order, const Tensor &place) {
+  at::AutoDispatchBelowADInplaceOrView guard;
+  const Tensor rows = place.dim() == 2 ? dispatched(x, order, place, place.size(1)) : Tensor();
+  if (rows.defined()) return rows;
+  GENERAL("dispatch_routed", decltype(dispatch_routed), x, order, place);
 }
 Tensor combine_rows(const Tensor &y, const Tensor &place, const MaybeTensor &weights) {
   at::AutoDispatchBelowADInplaceOrView guard;
   if (y.is_cuda() && is16(y) && y.dim() == 2 && y.numel() > 0 && y.is_contiguous() && is_ints(place, y, 2) && y.size(0) == place.numel() &&
       (!weights.has_value() || (weights->scalar_type() == at::kFloat && weights->sizes() == place.sizes() && weights->is_contiguous() && weights->device() == y.device()))) {
     const int64_t T = place.size(0), k = place.size(1), H = y.size(1);
-    Tensor out = at::empty({T, H}, y.options());
+    Tensor out = fresh(y, {T, H}, y.scalar_type());
     if (sk_combine_rows(y.data_ptr(), dtype_of(y.scalar_type()), place.data_ptr(), weights.has_value() ? weights->data_ptr() : nullptr, T, k, H, out.data_ptr(),
                         current_stream()) == SK_OK)
       return out;
@@ -204,7 +221,7 @@ std::tuple<Tensor, Tensor> combine_backward(const Tensor &d_out, const Tensor &y
       order.size(0) == y.size(0) && d_out.scalar_type() == y.scalar_type() && d_out.dim() == 2 && d_out.size(0) == place.size(0) && d_out.size(1) == y.size(1) &&
       d_out.is_contiguous() && d_out.device() == y.device() && weights.scalar_type() == at::kFloat && weights.sizes() == place.sizes() && weights.is_contiguous() &&
       weights.device() == y.device()) {
-    Tensor dy = at::empty(y.sizes(), y.options()), dw = at::empty(weights.sizes(), weights.options());
+    Tensor dy = fresh(y, y.sizes(), y.scalar_type()), dw = fresh(weights, weights.sizes(), weights.scalar_type());
     if (sk_combine_backward(d_out.data_ptr(), y.data_ptr(), dtype_of(y.scalar_type()), order.data_ptr(), place.data_ptr(), weights.data_ptr(), place.size(0),
                             place.size(1), y.size(1), dy.data_ptr(), dw.data_ptr(), current_stream()) == SK_OK)
       return {dy, dw};
@@ -290,9 +307,9 @@ FiveTensors route_experts_autograd(const Tensor &logits, int64_t k) {
 struct DispatchRows : torch::autograd::Function<DispatchRows> {
   static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &order, const Tensor &place) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    static const auto dispatch = OP(dispatch_rows);
+    static const auto dispatch = OP(dispatch_routed);
     ctx->save_for_backward({place});
-    return dispatch.call(x, order, place.size(1));
+    return dispatch.call(x, order, place);
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     once();
@@ -301,10 +318,6 @@ struct DispatchRows : torch::autograd::Function<DispatchRows> {
     return {combine.call(grads[0], ctx->get_saved_variables()[0], c10::nullopt), Tensor(), Tensor()};
   }
 };
-Tensor dispatch_routed(const Tensor &x, const Tensor &order, const Tensor &place) {
-  at::AutoDispatchBelowADInplaceOrView guard;
-  return dispatch_rows(x, order, place.size(1));
-}
 Tensor dispatch_routed_autograd(const Tensor &x, const Tensor &order, const Tensor &place) {
   if (wanted(x)) return DispatchRows::apply(x, order, place);
   BELOW(dispatch_routed, x, order, place);
@@ -327,7 +340,6 @@ struct CombineRows : torch::autograd::Function<CombineRows> {
   }
 };
 Tensor combine_routed(const Tensor &y, const Tensor &weights, const Tensor &order, const Tensor &place) {
-  at::AutoDispatchBelowADInplaceOrView guard;
   return combine_rows(y, place, weights);
 }
 Tensor combine_routed_autograd(const Tensor &y, const Tensor &weights, const Tensor &order, const Tensor &place) {

@@ -147,7 +147,7 @@ def lib():
     L.sk_route_workspace_bytes.restype = sz
     L.sk_route_experts.argtypes = [vp, ci, i64, i64, i64, i64, vp, vp, vp, vp, vp, vp, sz, vp]
     L.sk_route_backward.argtypes = [vp, vp, vp, i64, i64, i64, ci, vp, vp]
-    L.sk_dispatch_rows.argtypes = [vp, i64, i64, vp, i64, i64, vp, vp]
+    L.sk_dispatch_rows.argtypes = [vp, i64, i64, vp, vp, i64, i64, vp, vp]
     L.sk_combine_rows.argtypes = [vp, ci, vp, vp, i64, i64, i64, vp, vp]
     L.sk_combine_backward.argtypes = [vp, vp, ci, vp, vp, vp, i64, i64, i64, vp, vp, vp]
     for f in ("sk_gemm_i8_scaled", "sk_quantize_i8", "sk_gemm_grouped", "sk_grouped_wgrad", "sk_route_experts", "sk_route_backward",

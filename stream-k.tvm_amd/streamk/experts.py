@@ -195,7 +195,7 @@ def streamk_grouped(A, B, offsets, *, layout="nt", scale_a=None, scale_b=None, o
     once.  Differentiable in A and B without bias, activation, scales and out.  variant: which tiles run (sk_grouped in streamk.h); 0
     lets the sizes decide."""
     activation = activation or "none"
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (A, B, bias, scale_a, scale_b)):
+    if torch.is_grad_enabled() and (A.requires_grad or B.requires_grad or (bias is not None and bias.requires_grad)):
         if bias is not None or activation != "none" or scale_a is not None or scale_b is not None or out is not None:
             raise ValueError("the grouped product has gradients only without bias, activation, scales and out")
         if out_dtype not in (None, A.dtype):
@@ -203,7 +203,7 @@ def streamk_grouped(A, B, offsets, *, layout="nt", scale_a=None, scale_b=None, o
         if not _NATIVE:
             return _GroupedProduct.apply(A, B, offsets, layout, variant)
     if out is None:
-        return _ops.gemm_grouped(A, B, offsets, layout, out_dtype, scale_a, scale_b, bias, activation, variant)
+        return _gemm_grouped(A, B, offsets, layout, out_dtype, scale_a, scale_b, bias, activation, variant)
     _ops.gemm_grouped_out(A, B, offsets, out, layout, out_dtype, scale_a, scale_b, bias, activation, variant)
     return out
 
@@ -291,10 +291,10 @@ def route_experts(logits, k):
     goes to no expert.  Differentiable: weights to logits."""
     if not _NATIVE and torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
         return Route(*_RouteExperts.apply(logits, k))
-    return Route(*_ops.route_experts(logits, k))
+    return Route(*_route_experts(logits, k))
 
 
-def _dispatch(x, order, k):
+def _dispatch(x, order, k, place=None):
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() not in (1, 2):
         raise TypeError("x must be a CUDA/HIP tensor of one or two dimensions")
     _on_device(order, "order", (torch.int32,), 1)
@@ -304,12 +304,15 @@ def _dispatch(x, order, k):
     out = torch.empty((T * k, *x.shape[1:]), dtype=x.dtype, device=x.device)
     if out.numel() == 0:
         return out
+    if place is not None and (place.dtype != torch.int32 or tuple(place.shape) != (T, k) or not place.is_contiguous() or place.device != x.device):
+        raise ValueError(f"place must be contiguous int32 {(T, k)} on {x.device}")
     if x.dim() == 2 and (x.stride(1) != 1 and x.shape[1] > 1 or x.stride(0) < x.shape[1]) or x.dim() == 1 and x.stride(0) < 1:
         x = x.contiguous()
     size = x.element_size()
     row_bytes = size * (x.shape[1] if x.dim() == 2 else 1)
     pitch = size * x.stride(0) if T > 1 else row_bytes
-    rc = _lib.lib().sk_dispatch_rows(x.data_ptr(), row_bytes, pitch, order.data_ptr(), T, k, out.data_ptr(), ops._stream_ptr())
+    rc = _lib.lib().sk_dispatch_rows(x.data_ptr(), row_bytes, pitch, order.data_ptr(), place.data_ptr() if place is not None else None, T, k, out.data_ptr(),
+                                     ops._stream_ptr())
     _lib.check(rc, "sk_dispatch_rows")
     return out
 
@@ -351,7 +354,7 @@ _operator("combine_rows", "(Tensor y, Tensor place, Tensor? weights=None) -> Ten
 _operator("combine_backward", "(Tensor d_out, Tensor y, Tensor order, Tensor place, Tensor weights) -> (Tensor, Tensor)", _combine_backward,
           lambda d_out, y, order, place, weights: (y.new_empty(y.shape), weights.new_empty(weights.shape)))
 # the same with all of a route that their gradients need
-_operator("dispatch_routed", "(Tensor x, Tensor order, Tensor place) -> Tensor", lambda x, order, place: _dispatch(x, order, place.shape[1]),
+_operator("dispatch_routed", "(Tensor x, Tensor order, Tensor place) -> Tensor", lambda x, order, place: _dispatch(x, order, place.shape[1], place),
           lambda x, order, place: _dispatch_fake(x, order, place.shape[1]))
 _operator("combine_routed", "(Tensor y, Tensor weights, Tensor order, Tensor place) -> Tensor",
           lambda y, weights, order, place: _combine(y, place, weights), lambda y, weights, order, place: _combine_fake(y, place))
@@ -390,7 +393,7 @@ def dispatch_rows(x, route):
         _on_device(x, "x", tuple(_TYPES), 2)
         if not _NATIVE:
             return _DispatchRows.apply(x, route.order, route.place)
-    return _ops.dispatch_routed(x, route.order, route.place)
+    return _dispatch_routed(x, route.order, route.place)
 
 
 def combine_rows(y, route):
@@ -398,4 +401,9 @@ def combine_rows(y, route):
     added in fp32, rounded once; a token without experts gets zeros.  Differentiable in y and route.weights."""
     if not _NATIVE and torch.is_grad_enabled() and isinstance(y, torch.Tensor) and (y.requires_grad or route.weights.requires_grad):
         return _CombineRows.apply(y, route.weights, route.order, route.place)
-    return _ops.combine_routed(y, route.weights, route.order, route.place)
+    return _combine_routed(y, route.weights, route.order, route.place)
+
+
+# (the overloads themselves: a call through the packet looks them up)
+_gemm_grouped, _route_experts = _ops.gemm_grouped.default, _ops.route_experts.default
+_dispatch_routed, _combine_routed = _ops.dispatch_routed.default, _ops.combine_routed.default

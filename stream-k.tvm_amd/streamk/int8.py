@@ -86,8 +86,7 @@ def quantize_int8(x):
     """(q int8, scale float32) of the rows of x [..., K] (float16 or bfloat16): scale = max |x| / 127 of each row, q = x / scale to the
     nearest integer (ties to even).  A row of zeros has scale 0; a row with an infinity or a NaN scale NaN and q = 0, so that its
     products are NaN."""
-    _check_quantised(x)
-    return torch.ops.streamk.quantize_i8(x)
+    return _quantize_i8(x)
 
 
 def streamk_int8_scaled(A, B, scale_a, scale_b, *, out_dtype=torch.float16, out=None, plan=None, config=None, bias=None, activation=None, **kw):
@@ -96,6 +95,10 @@ def streamk_int8_scaled(A, B, scale_a, scale_b, *, out_dtype=torch.float16, out=
     rows those that operator calls take."""
     cfg = ops._config_string(plan, config, kw)
     if out is None:
-        return torch.ops.streamk.gemm_i8_scaled(A, B, scale_a, scale_b, out_dtype, cfg, bias, activation or "none")
+        return _gemm_i8_scaled(A, B, scale_a, scale_b, out_dtype, cfg, bias, activation or "none")
     torch.ops.streamk.gemm_i8_scaled_out(A, B, scale_a, scale_b, out, out.dtype, cfg, bias, activation or "none")
     return out
+
+
+# (the overloads themselves: a call through the packet looks them up)
+_quantize_i8, _gemm_i8_scaled = torch.ops.streamk.quantize_i8.default, torch.ops.streamk.gemm_i8_scaled.default

@@ -348,7 +348,8 @@ def test_route_gradient(sk, dtype, T, E, k):
 # ---- dispatch and combination ----
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", sorted(TYPES))
-@pytest.mark.parametrize("T,E,k,H", [(1, 4, 2, 64), (33, 8, 2, 520), (7, 3, 3, 1), (50, 16, 5, 77), (300, 64, 8, 4096), (64, 8, 1, 1000)])
+@pytest.mark.parametrize("T,E,k,H", [(1, 4, 2, 64), (33, 8, 2, 520), (7, 3, 3, 1), (50, 16, 5, 77), (300, 64, 8, 4096), (64, 8, 1, 1000),
+                                     (2100, 16, 3, 300), (2048, 40, 9, 1032)])
 def test_dispatch_and_combine(sk, dtype, T, E, k, H):
     t = TYPES[dtype]
     z = rand((T, E), torch.float32, T)
@@ -420,7 +421,7 @@ def test_calls_are_refused_with_codes(sk):
     assert route(n=4) == -5 and route(ws=None) == -5 and route(ws=p + 2) == -3
     assert L.sk_route_workspace_bytes(16, 64, 8) == 0 and L.sk_route_workspace_bytes(100, 8, 2) > 0 and L.sk_route_workspace_bytes(100, 8, 9) == 0
     assert L.sk_route_backward(p, p, None, 4, 8, 2, 1, p, None) == -1 and L.sk_route_backward(p, p, p, 4, 8, 9, 1, p, None) == -2
-    assert L.sk_dispatch_rows(p, 16, 8, p, 4, 2, p, None) == -2 and L.sk_dispatch_rows(None, 16, 16, p, 4, 2, p, None) == -1
+    assert L.sk_dispatch_rows(p, 16, 8, p, p, 4, 2, p, None) == -2 and L.sk_dispatch_rows(None, 16, 16, p, None, 4, 2, p, None) == -1
     assert L.sk_combine_rows(p, lib.SK_F32, p, p, 4, 2, 8, p, None) == -4 and L.sk_combine_rows(p, 0, p, p, 4, 2, 0, p, None) == -2
     assert L.sk_combine_backward(p, p, 0, p, p, None, 4, 2, 8, p, p, None) == -1
 
