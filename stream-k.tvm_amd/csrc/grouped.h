@@ -159,6 +159,15 @@ __device__ __forceinline__ int grouped_pid(int grid) {
   return x * (grid >> 3) + min(x, grid & 7) + (b >> 3);
 }
 
+// what a policy fetches ahead of a tile's loop
+template <class P>
+__device__ __forceinline__ void prefetch_epilogue(const typename P::Args &a, typename P::Acc &acc, const GroupTile &t, const void *epi) {
+  if constexpr (has_prefetch_bias<P>::value) {
+    if (epi != nullptr) P::prefetch_bias(a, acc, t.pn, epi);
+  }
+  if constexpr (has_prefetch_scales<P>::value) P::prefetch_scales(a, acc, t.pm, t.pn, epi);
+}
+
 template <class P>
 __device__ __forceinline__ void run_grouped(const GroupedArgs &g, int ipt, char *smem) {
   GroupWalk<P::BM> walk(g.offsets, g.E, g.R, g.tiles_n);
@@ -171,9 +180,7 @@ __device__ __forceinline__ void run_grouped(const GroupedArgs &g, int ipt, char 
     }
     const typename P::Args a = expert_args<P>(g, t);
     const void *epi = expert_epilogue(g, t);
-    if constexpr (has_prefetch_bias<P>::value) {
-      if (epi != nullptr) P::prefetch_bias(a, acc, t.pn, epi);
-    }
+    prefetch_epilogue<P>(a, acc, t, epi);
     P::mac(a, acc, t.pm, t.pn, 0, ipt, smem);
     P::store_c(a, acc, t.pm, t.pn, smem, epi);
   }
@@ -225,9 +232,7 @@ __device__ __forceinline__ void run_grouped_sk(const GroupedArgs &g, int ipt, co
     walk.find(tile, t);
     const typename P::Args a = expert_args<P>(g, t);
     const void *epi = expert_epilogue(g, t);
-    if constexpr (has_prefetch_bias<P>::value) {
-      if (epi != nullptr) P::prefetch_bias(a, acc, t.pn, epi);
-    }
+    prefetch_epilogue<P>(a, acc, t, epi);
     P::mac(a, acc, t.pm, t.pn, 0, ipt, smem);
     P::store_c(a, acc, t.pm, t.pn, smem, epi);
   }
@@ -241,9 +246,7 @@ __device__ __forceinline__ void run_grouped_sk(const GroupedArgs &g, int ipt, co
     walk.find(whole + tile, t);
     const typename P::Args a = expert_args<P>(g, t);
     const void *epi = expert_epilogue(g, t);
-    if constexpr (has_prefetch_bias<P>::value) {
-      if (epi != nullptr) P::prefetch_bias(a, acc, t.pn, epi);
-    }
+    prefetch_epilogue<P>(a, acc, t, epi);
     P::mac(a, acc, t.pm, t.pn, k0, n, smem);
     if (n == ipt) {
       P::store_c(a, acc, t.pm, t.pn, smem, epi);
@@ -283,9 +286,7 @@ __device__ __forceinline__ void run_grouped_sk(const GroupedArgs &g, int ipt, co
     if (!complete) continue;
     const typename P::Args a = expert_args<P>(g, cut[c]);
     const void *epi = expert_epilogue(g, cut[c]);
-    if constexpr (has_prefetch_bias<P>::value) {
-      if (epi != nullptr) P::prefetch_bias(a, acc, cut[c].pn, epi);
-    }
+    prefetch_epilogue<P>(a, acc, cut[c], epi);
     P::zero_sums(acc);
     for (int p = p0; p <= p1; ++p) P::add_partial(acc, slot(p, p == p0));
     P::store_c(a, acc, cut[c].pm, cut[c].pn, smem, epi);

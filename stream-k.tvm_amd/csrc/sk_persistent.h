@@ -70,6 +70,11 @@ template <class P, class = void>
 struct has_prefetch_bias { static constexpr bool value = false; };
 template <class P>
 struct has_prefetch_bias<P, std::void_t<decltype(&P::prefetch_bias)>> { static constexpr bool value = true; };
+// prefetch_scales: the same for the scales of its rows and columns (and the bias, if any)
+template <class P, class = void>
+struct has_prefetch_scales { static constexpr bool value = false; };
+template <class P>
+struct has_prefetch_scales<P, std::void_t<decltype(P::SCALES_AHEAD)>> { static constexpr bool value = P::SCALES_AHEAD; };
 template <class P, class = void>
 struct has_halves { static constexpr bool value = false; };
 template <class P>
@@ -141,6 +146,7 @@ __device__ __forceinline__ void run_persistent(const typename P::Args &a, const 
     if constexpr (has_prefetch_bias<P>::value && BIAS) {
       if (bias != nullptr) P::prefetch_bias(a, acc, pn, bias);
     }
+    if constexpr (has_prefetch_scales<P>::value) P::prefetch_scales(a, acc, pm, pn, bias);
     if constexpr (has_prefetch<P>::value) {
       P::mac(a, acc, pm, pn, k0, n, smem, first_stage_requested);
       first_stage_requested = false;

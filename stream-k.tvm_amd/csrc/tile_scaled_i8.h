@@ -121,35 +121,81 @@ struct ScaledDma : P {
   }
 };
 
-// tiles whose waves stream K on their own: a thread holds pieces of four columns of one row
+// Four bias values of C's type as they lie in memory (zeros without a bias)
+__device__ __forceinline__ half4v raw_bias4_at(const half_t *bias, int col, int N) {
+  half4v r = {0, 0, 0, 0};
+  if (bias == nullptr) return r;
+  if (col + 4 <= N && (reinterpret_cast<uintptr_t>(bias) & 7) == 0) return *reinterpret_cast<const half4v *>(bias + col);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (col + e < N) r[e] = bias[col + e];
+  return r;
+}
+template <bool BF16>
+__device__ __forceinline__ floatx4 widen4(half4v h) {
+  floatx4 r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const half_t x = h[e];
+    if constexpr (BF16) r[e] = __builtin_bit_cast(float, (uint32_t)__builtin_bit_cast(uint16_t, x) << 16);
+    else r[e] = (float)x;
+  }
+  return r;
+}
+
+// tiles whose waves stream K on their own: a thread holds pieces of four columns of one row.  Their scales and biases are requested
+// before the tile's loop; behind it their way from memory would be waited for (2 to 5 us of a launch).  Tiles of 64 x 128 have no
+// registers left for that; theirs are read at the end.
 template <class P>
 struct ScaledWaveK : P {
   typedef ScaledArgs<WaveKArgs> Args;
-  typedef typename P::Acc Acc;
-  static __device__ __forceinline__ void store_c(const Args &a, const Acc &acc, int pm, int pn, char *, const void *epi) {
-    by_result(a.s.bf16 != 0, epi, [&](auto bf16, auto with_epi) { store<decltype(bf16)::value, decltype(with_epi)::value>(a, acc, pm, pn, epi); });
-  }
-  template <bool BF16, bool EPI>
-  static __device__ __forceinline__ void store(const Args &a, const Acc &acc, int pm, int pn, const void *epi) {
-    const int tid = pin_here((int)threadIdx.x), act = EPI ? epi_act(epi) : 0;
-    const bool vec_ok = (a.ldc & 3) == 0 && (reinterpret_cast<uintptr_t>(a.C) & 7) == 0;
-    constexpr int COLS = P::ONE_COL ? 1 : P::PIECES;   // (pieces below each other share their columns' scales)
-    floatx4 sb[COLS], b4[COLS];
+  static constexpr bool SCALES_AHEAD = P::BM * P::BN < 64 * 128;
+  static constexpr int COLS = P::ONE_COL ? 1 : P::PIECES;   // (pieces below each other share their columns' scales)
+  struct Ends {
+    floatx4 sb[COLS];
+    half4v b4[COLS];
     float sa[P::PIECES];
+  };
+  struct Nothing {};
+  struct Acc : P::Acc {
+    std::conditional_t<SCALES_AHEAD, Ends, Nothing> ends;
+  };
+  static __device__ __forceinline__ void fetch(const Args &a, Ends &ends, int pm, int pn, const void *epi, int tid) {
 #pragma unroll
-    for (int u = 0; u < P::PIECES; ++u) {   // all loads at once
+    for (int u = 0; u < P::PIECES; ++u) {
       const int row = pm * P::BM + P::piece_row(u, tid), col = pn * P::BN + P::piece_col(u, tid) * 4;
-      sa[u] = row < a.M ? a.s.a[row] : 0.f;
+      ends.sa[u] = a.s.a[min(row, a.M - 1)];
       if (u < COLS) {
-        sb[u] = scale4_at(a.s.b, col, a.N);
-        if constexpr (EPI) b4[u] = bias4_at<BF16>(epi_bias(epi), col, a.N);
+        ends.sb[u] = scale4_at(a.s.b, col, a.N);
+        ends.b4[u] = raw_bias4_at(epi_bias(epi), col, a.N);
       }
     }
+  }
+  static __device__ __forceinline__ void prefetch_scales(const Args &a, Acc &acc, int pm, int pn, const void *epi) {
+    if constexpr (SCALES_AHEAD) fetch(a, acc.ends, pm, pn, epi, threadIdx.x);
+  }
+  static __device__ __forceinline__ void store_c(const Args &a, const Acc &acc, int pm, int pn, char *, const void *epi) {
+    const int tid = pin_here((int)threadIdx.x);
+    if constexpr (SCALES_AHEAD) {
+      store_by_type(a, acc, acc.ends, pm, pn, epi, tid);
+    } else {
+      Ends ends;
+      fetch(a, ends, pm, pn, epi, tid);
+      store_by_type(a, acc, ends, pm, pn, epi, tid);
+    }
+  }
+  static __device__ __forceinline__ void store_by_type(const Args &a, const Acc &acc, const Ends &ends, int pm, int pn, const void *epi, int tid) {
+    by_result(a.s.bf16 != 0, epi, [&](auto bf16, auto with_epi) { store<decltype(bf16)::value, decltype(with_epi)::value>(a, acc, ends, pm, pn, epi, tid); });
+  }
+  template <bool BF16, bool EPI>
+  static __device__ __forceinline__ void store(const Args &a, const Acc &acc, const Ends &ends, int pm, int pn, const void *epi, int tid) {
+    const int act = EPI ? epi_act(epi) : 0;
+    const bool vec_ok = (a.ldc & 3) == 0 && (reinterpret_cast<uintptr_t>(a.C) & 7) == 0;
 #pragma unroll
     for (int u = 0; u < P::PIECES; ++u) {
       const int row = pm * P::BM + P::piece_row(u, tid), col = pn * P::BN + P::piece_col(u, tid) * 4;
       if (row >= a.M || col >= a.N) continue;
-      const half4v h = scaled4<BF16, EPI>(acc.c[u], sa[u], sb[u % COLS], b4[u % COLS], act);
+      const half4v h = scaled4<BF16, EPI>(acc.c[u], ends.sa[u], ends.sb[u % COLS], widen4<BF16>(ends.b4[u % COLS]), act);
       half_t *dst = a.C + (int64_t)row * a.ldc + col;
       if (vec_ok && col + 4 <= a.N) {
         *reinterpret_cast<half4v *>(dst) = h;
@@ -160,25 +206,45 @@ struct ScaledWaveK : P {
   }
 };
 
-// up to 64 rows, the weights streaming through LDS
+// up to 64 rows, the weights streaming through LDS: the same
 template <class P>
 struct ScaledStream : P {
   typedef ScaledArgs<SkinnyArgs> Args;
-  typedef typename P::Acc Acc;
+  static constexpr bool SCALES_AHEAD = true;
+  struct Acc : P::Acc {
+    floatx4 sb[P::NB];
+    half4v b4[P::NB];
+    float sa[P::MB];
+  };
+  static __device__ __forceinline__ void origin(int pm, int pn, int &row0, int &col0) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave % P::WM, wn = wave / P::WM % P::WN;
+    row0 = pm * P::BM + wm * P::MB * 16 + (lane & 15);
+    col0 = pn * P::BN + wn * P::NB * 16 + 4 * (lane >> 4);
+  }
+  static __device__ __forceinline__ void prefetch_scales(const Args &a, Acc &acc, int pm, int pn, const void *epi) {
+    int row0, col0;
+    origin(pm, pn, row0, col0);
+#pragma unroll
+    for (int i = 0; i < P::MB; ++i) acc.sa[i] = a.s.a[min(row0 + 16 * i, a.M - 1)];
+#pragma unroll
+    for (int j = 0; j < P::NB; ++j) {
+      acc.sb[j] = scale4_at(a.s.b, col0 + 16 * j, a.N);
+      acc.b4[j] = raw_bias4_at(epi_bias(epi), col0 + 16 * j, a.N);
+    }
+  }
   static __device__ __forceinline__ void store_c(const Args &a, const Acc &acc, int pm, int pn, char *, const void *epi) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (wave >= P::WM * P::WN) return;
-    const int wm = wave % P::WM, wn = wave / P::WM;
-    const int row0 = pm * P::BM + wm * P::MB * 16, col0 = pn * P::BN + wn * P::NB * 16;
+    if ((int)(threadIdx.x >> 6) >= P::WM * P::WN) return;
+    int row0, col0;
+    origin(pm, pn, row0, col0);
+    const int act = epi_act(epi);
     const bool vec_ok = (a.ldc & 3) == 0 && (reinterpret_cast<uintptr_t>(a.C) & 7) == 0;
     by_result(a.s.bf16 != 0, epi, [&](auto bf16, auto with_epi) {
-      const ScaleRegs<P::MB, P::NB, decltype(bf16)::value, decltype(with_epi)::value> r(a, row0, col0, epi);
       static_for<0, P::MB>([&](auto i) {
-        const int row = row0 + 16 * i + (lane & 15);
         static_for<0, P::NB>([&](auto j) {
-          const int col = col0 + 16 * j + 4 * (lane >> 4);
+          const int row = row0 + 16 * i, col = col0 + 16 * j;
           if (row >= a.M || col >= a.N) return;
-          const half4v h = r.template values<decltype(i)::value, decltype(j)::value>(acc.c[i][j]);
+          const half4v h = scaled4<decltype(bf16)::value, decltype(with_epi)::value>(acc.c[i][j], acc.sa[i], acc.sb[j],
+                                                                                     widen4<decltype(bf16)::value>(acc.b4[j]), act);
           half_t *dst = a.C + (int64_t)row * a.ldc + col;
           if (vec_ok && col + 4 <= a.N) {
             *reinterpret_cast<half4v *>(dst) = h;
