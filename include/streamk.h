@@ -447,8 +447,8 @@ typedef struct sk_grouped {
   int64_t lda, ldb, ldc, expert_b;
   const void *bias, *scale_a, *scale_b;
   int64_t variant;                                /* the tiles: 0 by size; 1: 128 x 128; 2: 256 x 256 (K a multiple of
-                                                     64, int8: 128); 3 to 6 (SK_LAYOUT_NT): 16 x 64, 32 x 64, 64 x 64,
-                                                     64 x 128, whose waves stream K on their own */
+                                                     64, int8: 128); 3 to 6: 16 x 64, 32 x 64, 64 x 64, 64 x 128,
+                                                     whose waves stream K on their own (SK_LAYOUT_NN: only 64 x 64) */
   int64_t reserved;                               /* 0 */
 } sk_grouped;
 size_t sk_grouped_workspace_bytes(const sk_grouped *g);   /* for this shape and variant, on the current device; 0 is possible */

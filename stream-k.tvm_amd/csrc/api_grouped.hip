@@ -49,6 +49,7 @@ extern "C" int sk_gemm_grouped(const sk_grouped *g, void *ws, size_t ws_bytes, v
     return SK_ERR_ALIGN;
   if (reinterpret_cast<uintptr_t>(g->bias) >> EPI_ACT_SHIFT) return SK_ERR_CONFIG;   // not a device address
   if (sk_device_info(&h.cus, nullptr, nullptr) != SK_OK) return SK_ERR_DEVICE;
+  h.variant = grouped_variant(h);
   Workspace w;
   if (int rc = take_workspace(ws, ws_bytes, grouped_workspace(h), &w)) return rc;
   const int64_t pairs = i8 ? 2 : 1;

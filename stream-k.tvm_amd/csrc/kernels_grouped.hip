@@ -1,4 +1,6 @@
 // Products grouped by expert and the gradient of the experts' weights (grouped.h, tile_tn.h): kernel entries and launchers.
+#include <cmath>
+
 #include "grouped.h"
 #include "grouped_launch.h"
 #include "tile_tn.h"
@@ -11,54 +13,74 @@ __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_grouped_kernel(Grou
   run_grouped<P>(g, ipt, smem);
 }
 
-// The host knows the rows and the experts, not who has how many: an expert is taken to have R / E rows, spread by half a tile.
-//
-// Up to 8 and 20 rows the 16- and 32-row tiles, whose rings hold the most weights: us, 8 experts of 11008 x 4096 and 64 of 2048 x
-// 4096, fp16, 16- / 32- / 64-row tiles: 8 rows each 127 / 130 / 133 and 181 / 180 / 184, 16 rows 134 / 131 / 135, 32 rows 176 / 142 /
-// 140.  Above, the tile with the least estimated time: the rounds of the CUs that the tiles make, each of tau iterations of K (128 bytes
-// of a row) and o for a tile's beginning and end, against the weights' and rows' way from memory at the rate the tile reaches.
-// Estimated / measured us of 64 x 64, 64 x 128, 128 x 128, 256 x 256 tiles: 8 experts, 11008 x 4096, 48 rows each 166 / 145, 165 / 140,
-// 192 / 192, 209 / 196; 187 rows 306 / 297, 260 / 264, 240 / 240, 196 / 220; 1024 rows (bfloat16) the last 530 / 565; 64 experts,
-// 2048 x 4096, 64 rows 246 / 241, 244 / 232, 278 / 282, 304 / 262, 128 rows 352 / 347, 302 / 314, 282 / 271, 308 / 289.
+// The tile with the least estimated time.  The host knows the rows and the experts, not who has how many: the rows are taken to fall on
+// the experts by chance, spread by half a tile.
+//     time = 2 + sqrt(busy^2 + memory^2)
+//   busy    the rounds of the CUs that the tiles make, each of `tau` for 8 KB of K and `o` for a tile's beginning and end; what whole
+//           rounds leave costs its share and `cut` (tiles of waves that stream K: cut evenly, pieces of four iterations at least), `cut` of
+//           tau (128 x 128, a tile with its CU for itself), or a part of a round and `cut` (256 x 256, cut in two or four)
+//   memory  the weights of the experts that have rows, and the rows, once at `rate`
+// Fitted to 1150 products (1 to 64 experts, 1 to 2000 rows to an expert, N 256 to 12288, K 64 to 12288, even and skewed; mean |log error|
+// 6 to 12 %).  On 210 others its choice takes 1.014 of the fastest tile's time on average, 1.5 at worst, and more than 1.1 in ten.
 struct TileCost {
   int variant, bm, bn, per_cu;
-  double tau, o, rate;   // us per 64 iterations of a CU's tiles, us, bytes per us
+  double tau, o, rate, cut;   // us, us, bytes per us, see above
 };
-static const TileCost TILE_COSTS[] = {{GV_WAVEK64, 64, 64, 1, 13.0, 2.5, 5.2e6},
-                                      {GV_WAVEK64W, 64, 128, 1, 22.0, 3.5, 5.2e6},
-                                      {GV_TILE128, 128, 128, 2, 69.0, 3.0, 4.3e6},
-                                      {GV_ASM256, 256, 256, 1, 75.0, 7.0, 3.9e6}};
-static double estimate(const GroupedShape &h, const TileCost &c) {
-  const double experts = (double)(h.E < h.R ? h.E : h.R), rows = h.R / experts, bytes = h.type == GT_I8 ? 1.0 : 2.0;
+static const TileCost COSTS_16[6] = {{GV_WAVEK16, 16, 64, 1, 9.7, 1.25, 6.13e6, 5.62},
+                                     {GV_WAVEK32, 32, 64, 1, 11.3, 1.44, 6.18e6, 6.30},
+                                     {GV_WAVEK64, 64, 64, 1, 13.7, 1.98, 6.17e6, 7.32},
+                                     {GV_WAVEK64W, 64, 128, 1, 22.7, 3.43, 5.67e6, 10.29},
+                                     {GV_TILE128, 128, 128, 2, 64.2, 2.53, 6.46e6, 0.71},
+                                     {GV_ASM256, 256, 256, 1, 74.6, 5.49, 8.00e6, 18.10}};
+static const TileCost COSTS_NN[3] = {{GV_WAVEK64, 64, 64, 1, 17.1, 2.03, 5.72e6, 7.73},
+                                     {GV_TILE128, 128, 128, 2, 66.0, 2.57, 6.15e6, 0.69},
+                                     {GV_ASM256, 256, 256, 1, 78.0, 6.09, 6.01e6, 19.82}};
+static const TileCost COSTS_I8[6] = {{GV_WAVEK16, 16, 64, 1, 9.2, 1.58, 5.63e6, 6.41},
+                                     {GV_WAVEK32, 32, 64, 1, 11.3, 1.78, 5.70e6, 7.00},
+                                     {GV_WAVEK64, 64, 64, 1, 14.3, 2.32, 5.91e6, 7.53},
+                                     {GV_WAVEK64W, 64, 128, 1, 22.5, 4.50, 4.99e6, 10.10},
+                                     {GV_TILE128, 128, 128, 2, 61.7, 3.52, 5.17e6, 0.67},
+                                     {GV_ASM256, 256, 256, 1, 72.5, 9.01, 7.49e6, 17.71}};
+static double estimate(const GroupedShape &h, double experts, const TileCost &c) {
+  const double bytes = h.type == GT_I8 ? 1.0 : 2.0, rows = h.R / experts;
   const double high = h.E == 1 ? (double)((h.R + c.bm - 1) / c.bm) : rows / c.bm + 0.5;
   const double tiles = experts * (high > 1.0 ? high : 1.0) * (double)((h.N + c.bn - 1) / c.bn);
   const double iters = h.K * bytes / 8192.0, round = c.tau * iters + c.o, slots = (double)h.cus * c.per_cu;
   const double whole = (double)(int64_t)(tiles / slots), rest = tiles / slots - whole;
   double busy = whole * round;
-  if (c.variant == GV_WAVEK64 || c.variant == GV_WAVEK64W) {
-    busy += rest * round + (whole > 0 ? 5.0 : 10.0);            // (cut evenly)
+  if (rest > 0 && c.variant >= GV_WAVEK16) {
+    const double least = iters < 0.25 ? iters : 0.25;
+    busy += c.tau * (rest * iters > least ? rest * iters : least) + c.o + c.cut;
   } else if (rest > 0 && c.variant == GV_TILE128) {
-    busy += rest <= 0.5 ? 0.58 * c.tau * iters + c.o : round;   // (a tile that has its CU for itself)
+    busy += rest <= 0.5 ? c.cut * c.tau * iters + c.o : round;
   } else if (rest > 0) {
     const int parts = iters < 0.5 ? 1 : (rest <= 0.25 ? 4 : (rest <= 0.5 ? 2 : 1));
-    busy += parts == 1 ? round : c.tau * iters / parts + c.o + 20.0;
+    busy += parts == 1 ? round : c.tau * iters / parts + c.o + c.cut;
   }
   const double memory = (experts * h.N * h.K * bytes + h.R * (h.K * bytes + 2.0 * h.N)) / c.rate;
-  return busy > memory ? busy + 0.15 * memory : memory + 0.15 * busy;   // (they overlap but for a part)
+  return 2.0 + sqrt(busy * busy + memory * memory);
 }
 int grouped_variant(const GroupedShape &h) {
   if (h.variant != GV_RULE) return h.variant;
-  const int64_t experts = h.E < h.R ? h.E : h.R, rows = h.R / experts;
-  if (!h.nn && rows <= 20) return rows <= 8 ? GV_WAVEK16 : GV_WAVEK32;
+  const double experts = h.E == 1 ? 1.0 : h.E * (1 - pow(1 - 1.0 / h.E, (double)h.R));   // that have a row
   int best = GV_TILE128;
   double least = 0;
-  for (const TileCost &c : TILE_COSTS) {
-    if ((h.nn && c.variant >= GV_WAVEK16) || (c.variant == GV_ASM256 && !grouped_asm_takes(h))) continue;
-    const double t = estimate(h, c);
+  auto consider = [&](const TileCost &c) {
+    // (many low tiles, beyond what the constants were fitted to: the higher ones are as fast from 8 and 30 rows on)
+    if ((c.variant == GV_WAVEK16 && h.R > 40 * h.E) || (c.variant == GV_WAVEK32 && h.R > 150 * h.E) || (c.variant == GV_ASM256 && !grouped_asm_takes(h)))
+      return;
+    const double t = estimate(h, experts, c);
     if (least == 0 || t < least) {
       least = t;
       best = c.variant;
     }
+  };
+  if (h.type == GT_I8) {
+    for (const TileCost &c : COSTS_I8) consider(c);
+  } else if (h.nn) {
+    for (const TileCost &c : COSTS_NN) consider(c);
+  } else {
+    for (const TileCost &c : COSTS_16) consider(c);
   }
   return best;
 }
@@ -78,10 +100,8 @@ static int launch_grouped_policy(GroupedArgs g, const GroupedShape &h, hipStream
 }
 
 int launch_grouped(const GroupedArgs &g, const GroupedShape &h, const Workspace &ws, hipStream_t s) {
-  GroupedShape with = h;
-  with.variant = grouped_variant(h);
-  if (with.variant >= GV_WAVEK16) return h.nn ? (int)hipErrorNotSupported : launch_grouped_wavek(g, with, ws, s);
-  if (with.variant == GV_ASM256) return grouped_asm_takes(h) ? launch_grouped_asm(g, h, ws, s) : (int)hipErrorNotSupported;
+  if (h.variant >= GV_WAVEK16) return launch_grouped_wavek(g, h, ws, s);
+  if (h.variant == GV_ASM256) return grouped_asm_takes(h) ? launch_grouped_asm(g, h, ws, s) : (int)hipErrorNotSupported;
   if (h.type == GT_I8) return launch_grouped_policy<ScaledDma<TileF16NTDma<128, 128, 2, 2, false, 64, true, false, 3>>>(g, h, s);
   if (h.nn) {
     if (h.type == GT_BF16) return launch_grouped_policy<TileF16NTDma<128, 128, 2, 2, true, 64, true, true>>(g, h, s);

@@ -28,7 +28,7 @@ static int launch(GroupedArgs g, const GroupedShape &h, const Workspace &ws, hip
   return (int)hipGetLastError();
 }
 
-// variant -> blocks of 16 rows, of 16 weight rows:  X(variant, FM, FN)
+// variant -> blocks of 16 rows, of 16 columns:  X(variant, FM, FN)
 #define GROUP_WAVEKS(X)  \
   X(GV_WAVEK16, 1, 4)    \
   X(GV_WAVEK32, 2, 4)    \
@@ -42,13 +42,20 @@ size_t grouped_wavek_workspace(int variant, int cus) {
 #undef X
   return 0;
 }
-int launch_grouped_wavek(const GroupedArgs &g, const GroupedShape &h, const Workspace &ws, hipStream_t s) {
-#define X(V, FM, FN)                                                                                    \
-  if (h.variant == V) {                                                                                 \
-    if (h.type == GT_I8) return launch<ScaledWaveK<TileWaveK<WK_I8, FM, FN, false>>>(g, h, ws, s);          \
-    if (h.type == GT_BF16) return launch<TileWaveK<WK_BF16, FM, FN, false>>(g, h, ws, s);                   \
-    return launch<TileWaveK<WK_F16, FM, FN, false>>(g, h, ws, s);                                           \
+template <int FM, int FN>
+static int launch_by_type(const GroupedArgs &g, const GroupedShape &h, const Workspace &ws, hipStream_t s) {
+  if (h.nn) {
+    // (the lower ones are behind 64 x 64 from one row on: 100 rows, 8 experts of 4096 x 11008 158, 157 and 148 us; of 64 x 128 the ring
+    // would hold one chunk only)
+    if constexpr (FM == 4 && FN == 4) return h.type == GT_BF16 ? launch<TileWaveK<WK_BF16, FM, FN, true>>(g, h, ws, s) : launch<TileWaveK<WK_F16, FM, FN, true>>(g, h, ws, s);
+    return (int)hipErrorNotSupported;
   }
+  if (h.type == GT_I8) return launch<ScaledWaveK<TileWaveK<WK_I8, FM, FN, false>>>(g, h, ws, s);
+  return h.type == GT_BF16 ? launch<TileWaveK<WK_BF16, FM, FN, false>>(g, h, ws, s) : launch<TileWaveK<WK_F16, FM, FN, false>>(g, h, ws, s);
+}
+int launch_grouped_wavek(const GroupedArgs &g, const GroupedShape &h, const Workspace &ws, hipStream_t s) {
+#define X(V, FM, FN) \
+  if (h.variant == V) return launch_by_type<FM, FN>(g, h, ws, s);
   GROUP_WAVEKS(X)
 #undef X
   return (int)hipErrorNotSupported;

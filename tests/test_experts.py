@@ -514,6 +514,30 @@ def test_grouped_variants(sk, variant, kind, sizes, N, K, padding):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("sizes", sorted(SIZES))
+@pytest.mark.parametrize("N,K,padding", [(520, 256, 0), (264, 36, 24), (1032, 645, 0), (64, 1536, 0), (8, 1, 8)])
+def test_grouped_kn_weights_on_tiles_that_stream_k(sk, dtype, sizes, N, K, padding):
+    sizes = SIZES[sizes]
+    R, E = sum(sizes) + 2, len(sizes)
+    whole = torch.zeros(R, (K + 7) // 8 * 8, dtype=TYPES[dtype], device="cuda")
+    A, B, bias = whole[:, :K], rand((E, K, N), TYPES[dtype], N, 1 / math.sqrt(K)), rand((E, N), TYPES[dtype], 5)
+    A.copy_(rand((R, K), TYPES[dtype], R))
+    out = torch.full((R, N + padding), 7.0, dtype=TYPES[dtype], device="cuda")
+    pre, magnitudes = plain(A, B, sizes, "nn")
+    for e, at in groups(sizes):
+        pre[at] += bias[e].double()
+    sk.streamk_grouped(A, B, offsets_of(sizes), layout="nn", variant=5, out=out[:, :N], bias=bias, activation="gelu_tanh")
+    want = activate(pre, "gelu_tanh")
+    want[R - 2:] = 0
+    assert_near(out[:, :N], want, K, 1.2 * magnitudes, pre)
+    assert (out[:, N:] == 7).all()
+    again = torch.full_like(out, 7.0)
+    sk.streamk_grouped(A, B, offsets_of(sizes), layout="nn", variant=5, out=again[:, :N], bias=bias, activation="gelu_tanh")
+    assert torch.equal(out, again)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("variant", [1, 2])
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("sizes", sorted(SIZES))
