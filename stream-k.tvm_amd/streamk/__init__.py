@@ -7,4 +7,5 @@ from .autotune import autotune, candidate_configs  # noqa: F401
 from .experts import (Route, combine_rows, dispatch_rows, route_experts, streamk_grouped, streamk_grouped_wgrad)  # noqa: F401
 from .int8 import quantize_int8, streamk_int8_scaled  # noqa: F401
 from .linear import StreamKLinear  # noqa: F401
+from .moe import StreamKMoE  # noqa: F401
 from .plan import cta_range, make_config, make_plan, num_cus, tile_coords, tuned_config  # noqa: F401

@@ -2,7 +2,7 @@
 
 The reference stops at kernel scripts; wrapping them as an operator of a model is its open item
 ("integrate with BitBLAS", README.md:21).  This module is that wrapper for this library: it owns
-the weight in the layout the kernels read ([N, K] fp16 or bfloat16, or packed nibbles + scales), flattens the
+the weight in the layout the kernels read ([N, K] fp16 or bfloat16, packed nibbles + scales, or int8 + a scale for each row), flattens the
 leading dimensions of the input into M, and keeps one plan per M it has seen (a decode step calls
 with M = batch, a prefill with M = batch * tokens), each taken from the tuned cache when the shape
 is in it.  Inference only: the GEMM is not recorded by autograd.
@@ -10,18 +10,23 @@ is in it.  Inference only: the GEMM is not recorded by autograd.
 import torch
 
 from . import ops
+from .int8 import quantize_int8
 from .plan import make_plan, operator_config
 
 
 class StreamKLinear(torch.nn.Module):
     def __init__(self, in_features, out_features, bias=False, *, weight_format="float16", group=128, zero=8,
-                 activation=None, device=None):
+                 activation=None, device=None, dtype=None):
+        """weight_format 'int8': weights and activations in int8 with a scale for each output channel and for each row of the input
+        (quantised on the way in); input, bias and output are `dtype`, float16 or bfloat16 (by default float16)."""
         super().__init__()
         if activation not in (None, "relu", "gelu_tanh", "silu"):
             raise ValueError("activation must be None, 'relu', 'gelu_tanh' or 'silu'")
         self.activation = activation  # applied in the GEMM's epilogue, after the bias
-        if weight_format not in ("float16", "bfloat16", "q4", "q4_zp"):
-            raise ValueError("weight_format must be 'float16', 'bfloat16', 'q4' or 'q4_zp' (one zero point per group)")
+        if weight_format not in ("float16", "bfloat16", "q4", "q4_zp", "int8"):
+            raise ValueError("weight_format must be 'float16', 'bfloat16', 'q4', 'q4_zp' (one zero point per group) or 'int8'")
+        if weight_format == "int8" and in_features % 16:
+            raise ValueError("int8 weights need in_features a multiple of 16")
         if weight_format in ("q4", "q4_zp") and (group != 128 or in_features % 128):
             raise ValueError("Q4 weights need group == 128 and in_features a multiple of 128")
         if in_features % 8:
@@ -29,10 +34,17 @@ class StreamKLinear(torch.nn.Module):
         self.in_features, self.out_features = in_features, out_features
         self.weight_format, self.group, self.zero = weight_format, group, zero
         N, K = out_features, in_features
-        # activations, bias and output are bfloat16 with bfloat16 weights, fp16 otherwise
+        # activations, bias and output are bfloat16 with bfloat16 weights, fp16 otherwise (int8: as the caller says)
         self.dtype = torch.bfloat16 if weight_format == "bfloat16" else torch.float16
+        if dtype is not None and dtype != self.dtype:
+            if weight_format != "int8" or dtype != torch.bfloat16:
+                raise ValueError(f"weight_format '{weight_format}' does not go with {dtype}")
+            self.dtype = dtype
         if weight_format in ("float16", "bfloat16"):
             self.register_buffer("weight", torch.zeros(N, K, dtype=self.dtype, device=device))
+        elif weight_format == "int8":
+            self.register_buffer("qweight", torch.zeros(N, K, dtype=torch.int8, device=device))
+            self.register_buffer("weight_scale", torch.zeros(N, dtype=torch.float32, device=device))
         else:
             self.register_buffer("qweight", torch.zeros(N, K // 2, dtype=torch.uint8, device=device))
             self.register_buffer("scales", torch.zeros(N, K // group, dtype=torch.float16, device=device))
@@ -43,13 +55,18 @@ class StreamKLinear(torch.nn.Module):
     @classmethod
     def from_linear(cls, linear, *, weight_format="float16", group=128, zero=8, activation=None):
         """Takes over the weight (and bias) of a torch.nn.Linear; weight_format='q4' / 'q4_zp' quantises
-        it with `quantize_q4` (symmetric around `zero` / asymmetric with a zero point per group) on the
-        device it lives on."""
-        w = linear.weight.detach().to(torch.bfloat16 if weight_format == "bfloat16" else torch.float16).contiguous()
+        it with `quantize_q4` (symmetric around `zero` / asymmetric with a zero point per group), weight_format='int8' with
+        `quantize_int8` (input and output are bfloat16 if the weight is), on the device it lives on."""
+        keeps = weight_format == "bfloat16" or (weight_format == "int8" and linear.weight.dtype == torch.bfloat16)
+        w = linear.weight.detach().to(torch.bfloat16 if keeps else torch.float16).contiguous()
         m = cls(linear.in_features, linear.out_features, linear.bias is not None, weight_format=weight_format,
-                group=group, zero=zero, activation=activation, device=w.device)
+                group=group, zero=zero, activation=activation, device=w.device, dtype=w.dtype if weight_format == "int8" else None)
         if weight_format in ("float16", "bfloat16"):
             m.weight.copy_(w)
+        elif weight_format == "int8":
+            q, s = quantize_int8(w)
+            m.qweight.copy_(q)
+            m.weight_scale.copy_(s)
         elif weight_format == "q4_zp":
             q, s, z = ops.quantize_q4(w, group=group, asymmetric=True)
             m.qweight.copy_(q)
@@ -88,6 +105,9 @@ class StreamKLinear(torch.nn.Module):
             c = torch.ops.streamk.gemm_f16(a, self.weight, "nt", "", self.bias, act)
         elif self.weight_format == "bfloat16":
             c = torch.ops.streamk.gemm_bf16(a, self.weight, "nt", "", self.bias, act)
+        elif self.weight_format == "int8":
+            q, scale = torch.ops.streamk.quantize_i8(a)
+            c = torch.ops.streamk.gemm_i8_scaled(q, self.qweight, scale, self.weight_scale, self.dtype, "", self.bias, act)
         else:
             zeros = self.zeros if self.weight_format == "q4_zp" else None
             c = torch.ops.streamk.gemm_q4(a, self.qweight, self.scales, zeros, self.zero, self.group, False, "",
