@@ -58,6 +58,13 @@ TN layout (A is [K, M], B is [K, N]; SK_TILE_ASM_*_TN): both halves of a stage a
 registers (%[rat0] .. %[rat7]), second lane offset (v123) and step (%[kas]).  Row groups 0-3 of an operand are the rows of K-step 0
 and groups 4-7 those of K-step 1, so here EARLY and LATE split a stage by K-step: the rows of K-step 0 are free once block 0 has read
 its late fragments, those of K-step 1 once block 1 has, and every block again carries eight loads.
+
+Low tiles (NT; SK_TILE_ASM_*_LOW): at most 128 rows of A, 64 to a wave, whose blocks 0-3 they are; blocks 4-7 do not exist.  The rows
+stand where blocks 0-3 of a full tile's waves do, so A has EARLY row groups only, and these are 32 consecutive rows of A each.  A
+block of the loop is 32 MFMAs with four loads (block 0) and eight (block 1); the loop's state rides with the reads at the top.
+
+SK_TILE_ASM_LOOP_WRAP and _LOW (NT): a segment may start anywhere in K and wrap around; iteration %[wrap] is that of the first K, and from
+the one before it the offsets move by %[back].
 """
 
 A0, B0, A1, B1 = 128, 160, 192, 224     # first registers of the fragment buffers
@@ -71,7 +78,7 @@ TOP = 8     # gaps at the top of a block that carry the reads of the late fragme
 LD_LAST, RD_LAST = 61, 53    # last gap of a block that may carry a load / a fragment read of the next K-step
 
 
-def mfma_order():
+def mfma_order(low=False):
     """the 8 x 8 blocks quadrant by quadrant -- (A 0-3, B 0-3), (A 0-3, B 4-7), (A 4-7, B 4-7), (A 4-7, B 0-3) -- so that
     the fragments of blocks 4-7 are needed only from the 17th (B) and the 33rd (A) instruction on; consecutive
     instructions share one operand"""
@@ -81,6 +88,8 @@ def mfma_order():
             out += [(i, j) for j in (cols if n % 2 == 0 else cols[::-1])]
         return out
     lo, hi = [0, 1, 2, 3], [4, 5, 6, 7]
+    if low:
+        return snake(lo, lo) + snake(lo[::-1], hi)
     return snake(lo, lo) + snake(lo[::-1], hi) + snake(hi, hi) + snake(hi[::-1], lo[::-1])
 
 
@@ -103,17 +112,18 @@ class LdsTracker:
         return f'"s_waitcnt lgkmcnt({min(allowed, 15)})'
 
 
-def load_parts(x, nn, voa, vob, vob1, lds, ka, kb, prev=None, voa1=None):
+def load_parts(x, nn, voa, vob, vob1, lds, ka, kb, prev=None, voa1=None, low=False):
     """load x of a stage: 0..7 row groups of A, 8..15 of B (a wave's groups are 4 KB apart in LDS).  Returns
     (instructions that go before the m0 write, the m0 write, the load); s[S_T] walks the global offsets of the
     groups -- `prev` is the group the walk comes from (None: x is the first of its operand in this sequence) --,
     `lds` is the stage's LDS address for this wave"""
     base, step, first = (ka, "%[gas", 0) if x < 8 else (kb, "%[gbs", 8)
+    rows_of = (lambda g: EARLY_X.index(g)) if low and x < 8 else (lambda g: g)   # (in units of `step`)
     if prev is None:
-        skip = x - first
+        skip = rows_of(x) - first
         pre = [f'"s_mov_b32 s{S_T}, {base}'] if skip == 0 else [f'"s_add_u32 s{S_T}, {base}, {step}{skip}]']
     else:
-        pre = [f'"s_add_u32 s{S_T}, s{S_T}, {step}{x - prev}]']
+        pre = [f'"s_add_u32 s{S_T}, s{S_T}, {step}{rows_of(x) - rows_of(prev)}]']
     pre = [t.replace("gas1]", "gas]").replace("gbs1]", "gbs]") for t in pre]
     lds_off = (x * 4096) if x < 8 else (32768 + (x - 8) * 4096)
     m0 = f'"s_add_u32 m0, {lds}, {lds_off}'
@@ -124,18 +134,18 @@ def load_parts(x, nn, voa, vob, vob1, lds, ka, kb, prev=None, voa1=None):
     return pre, m0, ld
 
 
-def load_sequence(xs, nn, voa, vob, vob1, lds, ka, kb, voa1=None):
+def load_sequence(xs, nn, voa, vob, vob1, lds, ka, kb, voa1=None, low=False):
     """load_parts for the groups xs (ascending; A before B), with the walk chained through them"""
     out, prev = [], None
     for x in xs:
         if prev is not None and (prev < 8) != (x < 8):
             prev = None
-        out.append(load_parts(x, nn, voa, vob, vob1, lds, ka, kb, prev, voa1))
+        out.append(load_parts(x, nn, voa, vob, vob1, lds, ka, kb, prev, voa1, low))
         prev = x
     return out
 
 
-def early_groups(nn):
+def early_groups(nn, low=False):
     """the loads that must have landed a block ahead of the others: rows of blocks 0-3 (NN: and all of B, whose loads
     fill whole K-rows; TN: the rows of K-step 0)"""
     if nn == "tn":
@@ -143,16 +153,18 @@ def early_groups(nn):
     return list(EARLY_X) + ([8 + x for x in range(8)] if nn else [8 + x for x in EARLY_X])
 
 
-def late_groups(nn):
+def late_groups(nn, low=False):
+    if low:
+        return [8 + x for x in LATE_X]
     if nn == "tn":
         return [x for x in range(16) if x % 8 >= 4]
     return list(LATE_X) + ([] if nn else [8 + x for x in LATE_X])
 
 
-def stage_loads_text(nn, xs):
+def stage_loads_text(nn, xs, low=False):
     """the loads xs of one stage, back to back (operands: the stage's LDS address, global offsets and lane offsets)"""
     L = []
-    for pre, m0, ld in load_sequence(xs, nn, "%[voa]", "%[vob]", "%[vob1]", "%[lds]", "%[ga]", "%[gb]", "%[voa1]"):
+    for pre, m0, ld in load_sequence(xs, nn, "%[voa]", "%[vob]", "%[vob1]", "%[lds]", "%[ga]", "%[gb]", "%[voa1]", low):
         L += pre + [m0, '"s_nop 0', ld]
     return L
 
@@ -168,8 +180,8 @@ def offsets_for(nn, ahead):
     return out
 
 
-def zero_accumulators(L):
-    for r in range(256):
+def zero_accumulators(L, low=False):
+    for r in range(128 if low else 256):
         L.append(f'"v_accvgpr_write_b32 a{r}, 0')
 
 
@@ -181,8 +193,8 @@ def spread(plan, groups, first, last):
         plan[free[(k * len(free)) // len(groups)]] = item
 
 
-def loop_text(nn):
-    """The loop for the NT (nn = False), the NN (True) or the TN layout ("tn").  The two blocks of an iteration are built alike; block b
+def loop_text(nn, low=False, wrap=False):
+    """The loop for the NT (nn = False; low: of a low tile; wrap: see above), the NN (True) or the TN layout ("tn").  The two blocks of an iteration are built alike; block b
     (K-step b of iteration `it`, fragment set b, stage cur = it % 2, nxt the other one):
       top      reads of the LATE fragments (blocks 4-7 of A and B) of set b from cur -- their rows were the last to
                be loaded and are the last to be overwritten
@@ -196,8 +208,9 @@ def loop_text(nn):
     kb_step = "%[kbs]" if nn else "128"
     tn = nn == "tn"
     ka_step = "%[kas]" if tn else "128"
-    order = mfma_order()
-    n_early, n_late = len(early_groups(nn)), len(late_groups(nn))
+    order = mfma_order(low)
+    n_early, n_late = len(early_groups(nn, low)), len(late_groups(nn, low))
+    top, last, ld_last, rd_last = (4, 31, 30, 29) if low else (TOP, 63, LD_LAST, RD_LAST)
 
     def mf(i, j, ab, bb):
         c = (8 * i + j) * 4
@@ -227,12 +240,12 @@ def loop_text(nn):
         return [read_a(0, kk)] + [read_b(j, kk) for j in range(4)] + [read_a(i, kk) for i in range(1, 4)]
 
     def late_reads(kk):     # B 4-7 are needed from the 17th MFMA on, A 4-7 from the 33rd
-        return [read_b(j, kk) for j in range(4, 8)] + [read_a(i, kk) for i in range(4, 8)]
+        return [read_b(j, kk) for j in range(4, 8)] + ([] if low else [read_a(i, kk) for i in range(4, 8)])
 
     def load_groups(xs):
         """loads as rider groups: the scalar instructions of a load share a gap, the load has its own"""
         groups = []
-        for pre, m0, ld in load_sequence(xs, nn, f"v{VOA}", f"v{VOB}", f"v{VOB1}", f"s{S_LDS}", f"s{S_KA}", f"s{S_KB}", f"v{VOA1}"):
+        for pre, m0, ld in load_sequence(xs, nn, f"v{VOA}", f"v{VOB}", f"v{VOB1}", f"s{S_LDS}", f"s{S_KA}", f"s{S_KB}", f"v{VOA1}", low):
             groups += [(None, pre + [m0]), (None, [ld])]
         return groups
 
@@ -247,14 +260,19 @@ def loop_text(nn):
             L.extend(texts)
             for t in tags or []:
                 tr.issue(t)
-        assert all(0 <= g < 64 for g in plan), sorted(plan)
+        assert all(0 <= g <= last for g in plan), sorted(plan)
         L.extend(closing)
 
     # ---- entry: accumulators to zero while the first stage is on its way; the loop's state: the loads of block 0 are
     # those of iteration 1, into the second stage
-    zero_accumulators(L)
+    zero_accumulators(L, low)
     e(f'"s_mov_b32 s{S_IT}, 0')
     e(f'"s_xor_b32 s{S_LDS}, %[lds], 0x10000')
+    wrap = wrap or low
+    if wrap:
+        e('"s_cmp_eq_u32 %[wrap], 1')
+        e(f'"s_cselect_b32 s{S_M0}, %[back], 128')
+        ka_step = kb_step = f"s{S_M0}"
     e(f'"s_add_u32 s{S_KA}, %[ga0], {ka_step}')
     e(f'"s_add_u32 s{S_KB}, %[gb0], {kb_step}')
     L.extend(offsets_for(nn, 1))
@@ -274,12 +292,12 @@ def loop_text(nn):
         plan = {}
         for g, item in enumerate(late_reads(0)):
             plan[g] = item
-        spread(plan, load_groups(late_groups(nn)), TOP, LD_LAST)
-        spread(plan, early_reads(1), TOP, RD_LAST)
+        spread(plan, load_groups(late_groups(nn, low)), top, ld_last)
+        spread(plan, early_reads(1), top, rd_last)
         # the addresses of set 0 move to the other stage behind the reads at the top (block 1 reads the early fragments
         # of the next iteration with them); NN: one register per block of B serves both K-steps -- those of blocks 0-3
         # flip between the early reads of block 0 and of block 1, those of blocks 4-7 behind the top reads of block 1
-        spread(plan, ([] if tn else [flip("%[ra0]")]) + ([] if nn else [flip("%[rb0]")]), TOP, 63)
+        spread(plan, ([] if tn else [flip("%[ra0]")]) + ([] if nn else [flip("%[rb0]")]), top, last)
         # both ways into the loop: the early fragments of set 0 may still be in flight
         block(0, LdsTracker(at_top), plan,
               [f'"s_waitcnt vmcnt({n_late}) lgkmcnt(0)', '"s_barrier'])       # (the early loads, issued a block ago, have landed)
@@ -296,13 +314,24 @@ def loop_text(nn):
             state += [flip(f"%[rbt{j}]") for j in range(4)]
         if tn:
             state += [flip(f"%[rat{i}]") for i in range(4)]
-        for g, item in enumerate(state):
-            plan[TOP + g] = item
-        after_state = TOP + len(state)
-        plan[63] = (None, [f'"s_add_u32 s{S_IT}, s{S_IT}, 1'])
-        spread(plan, load_groups(early_groups(nn)), after_state, LD_LAST)
-        spread(plan, early_reads(0), after_state, RD_LAST)
-        spread(plan, ([flip(f"%[rat{i}]") for i in range(4, 8)] if tn else [flip("%[ra1]")]) + ([flip(f"%[rbt{j}]") for j in range(4, 8)] if nn else [flip("%[rb1]")]), after_state, 62)
+        if wrap:
+            state[:3] = [(None, [f'"s_add_u32 s{S_T2}, s{S_IT}, 2', f'"s_cmp_eq_u32 s{S_T2}, %[wrap]', f'"s_cselect_b32 s{S_M0}, %[back], 128']),
+                         (None, [f'"s_add_u32 s{S_KA}, s{S_KA}, s{S_M0}', f'"s_add_u32 s{S_KB}, s{S_KB}, s{S_M0}']),
+                         (None, [f'"s_cmp_lt_u32 s{S_T2}, %[n]', f'"s_cselect_b32 s{S_OOB}, 0, 0x80000000', f'"s_xor_b32 s{S_LDS}, s{S_LDS}, 0x10000'])]
+        if low:     # (32 gaps for 4 + 8 reads, eight loads, two flips and this)
+            for g, (_, texts) in enumerate(state[:top]):
+                plan[g] = (plan[g][0], plan[g][1] + texts)
+            plan[top] = state[top]
+            assert len(state) == top + 1
+            after_state = top + 1
+        else:
+            for g, item in enumerate(state):
+                plan[top + g] = item
+            after_state = top + len(state)
+        plan[last] = (None, [f'"s_add_u32 s{S_IT}, s{S_IT}, 1'])
+        spread(plan, load_groups(early_groups(nn, low)), after_state, ld_last)
+        spread(plan, early_reads(0), after_state, rd_last)
+        spread(plan, ([flip(f"%[rat{i}]") for i in range(4, 8)] if tn else [flip("%[ra1]")]) + ([flip(f"%[rbt{j}]") for j in range(4, 8)] if nn else [flip("%[rb1]")]), after_state, last - 1)
         block(1, LdsTracker(), plan,
               [f'"s_waitcnt vmcnt({n_early}) lgkmcnt(0)', '"s_barrier',           # (the late loads of iteration it + 1 have landed)
                f'"s_cmp_lt_u32 s{S_IT}, %[n]', '"s_cbranch_scc1 L_sk_loop%='])
@@ -493,7 +522,7 @@ def emit_macro(name, params, lines):
 def main():
     print("// Generated by gen_tile_asm.py -- do not edit; see that file for the register plan and the schedule.")
     print("// SK_TILE_ASM_LOADS / _LOADS_NN / _LOADS_TN: the 16 loads of one stage.  SK_TILE_ASM_LOOP(MF) / _LOOP_NN(MF) / _LOOP_TN(MF): the loop")
-    print("// for the NT / NN / TN layout, MF = the MFMA mnemonic as a string literal.  SK_TILE_ASM_LOOP_F8(MF, MOD): fp8 operands, MOD =")
+    print("// (_LOW: tiles of at most 128 rows) for the NT / NN / TN layout, MF = the MFMA mnemonic as a string literal.  SK_TILE_ASM_LOOP_F8(MF, MOD): fp8 operands, MOD =")
     print("// the format modifiers of the MFMA (\"\" for e4m3).  SK_TILE_ASM_STORE_x(CVT): the epilogue that leaves the stages alone.")
     print("#pragma once")
     emit_macro("SK_TILE_ASM_LOADS", "", stage_loads_text(False, range(16)))
@@ -502,7 +531,11 @@ def main():
     emit_macro("SK_TILE_ASM_LOADS_EARLY_NN", "", stage_loads_text(True, early_groups(True)))
     emit_macro("SK_TILE_ASM_LOADS_TN", "", stage_loads_text("tn", range(16)))
     emit_macro("SK_TILE_ASM_LOADS_EARLY_TN", "", stage_loads_text("tn", early_groups("tn")))
+    emit_macro("SK_TILE_ASM_LOADS_LOW", "", stage_loads_text(False, sorted(early_groups(False, True) + late_groups(False, True)), True))
+    emit_macro("SK_TILE_ASM_LOADS_EARLY_LOW", "", stage_loads_text(False, early_groups(False, True), True))
     emit_macro("SK_TILE_ASM_LOOP", "(MF)", loop_text(False))
+    emit_macro("SK_TILE_ASM_LOOP_WRAP", "(MF)", loop_text(False, False, True))
+    emit_macro("SK_TILE_ASM_LOOP_LOW", "(MF)", loop_text(False, True))
     emit_macro("SK_TILE_ASM_LOOP_NN", "(MF)", loop_text(True))
     emit_macro("SK_TILE_ASM_LOOP_TN", "(MF)", loop_text("tn"))
     emit_macro("SK_TILE_ASM_LOOP_F8", "(MF, MOD)", loop_text_f8())

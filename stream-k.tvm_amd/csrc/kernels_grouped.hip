@@ -21,7 +21,7 @@ __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_grouped_kernel(Grou
 //           tau (128 x 128, a tile with its CU for itself), or a part of a round and `cut` (256 x 256, cut in two or four)
 //   memory  the weights of the experts that have rows, and the rows, once at `rate`
 // Fitted to 1150 products (1 to 64 experts, 1 to 2000 rows to an expert, N 256 to 12288, K 64 to 12288, even and skewed; mean |log error|
-// 6 to 12 %).  On 210 others its choice takes 1.014 of the fastest tile's time on average, 1.5 at worst, and more than 1.1 in ten.
+// 6 to 12 %).  On 600 others its choice takes 1.02 of the fastest tile's time on average, 1.5 at worst, and more than 1.1 in 35.
 struct TileCost {
   int variant, bm, bn, per_cu;
   double tau, o, rate, cut;   // us, us, bytes per us, see above

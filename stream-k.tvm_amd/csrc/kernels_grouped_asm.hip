@@ -25,8 +25,9 @@ struct Cuts {
 // flag, the last one -- the others are past their loops by then and wait for nobody, so the wait is a short one whatever else the
 // device does -- adds them to its own in the order of the parts, which is the same on every launch.  True: acc has the tile's sums.
 // flags: [grid] of the CTAs, then a counter for each cut tile; all zero before and after.
+// (low: the lower half of the accumulators)
 template <class P>
-__device__ __forceinline__ bool join_parts(typename P::Acc &acc, int tile, int part, int parts, int grid, const Workspace &ws) {
+__device__ __forceinline__ bool join_parts(typename P::Acc &acc, int tile, int part, int parts, int grid, const Workspace &ws, bool low) {
   int *ticket = ws.flags + grid + tile, *flags = ws.flags + tile * parts, *word = reinterpret_cast<int *>(P::lds() + 2 * P::STAGE_BYTES);
   auto slot = [&](int q) { return ws.partials + (size_t)(tile * parts + q) * P::TILE_ELEMS; };
   if (threadIdx.x == 0) *word = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -34,7 +35,8 @@ __device__ __forceinline__ bool join_parts(typename P::Acc &acc, int tile, int p
   const bool last = *word == parts - 1;
   __syncthreads();
   if (!last) {
-    P::store_partial(acc, slot(part));
+    if (low) P::store_partial_half(acc, slot(part), 0);
+    else P::store_partial(acc, slot(part));
     signal_partial_ready<true>(flags + part, ws.status + WS_DIRTY, (int)(((size_t)(tile * parts + part + 1) * P::TILE_ELEMS * 4 + 255) >> 8));
     return false;
   }
@@ -58,6 +60,7 @@ __device__ __forceinline__ bool join_parts(typename P::Acc &acc, int tile, int p
   const uint32_t off = (uint32_t)pin_here((int)threadIdx.x) * 16;
   static_for<0, P::NV4 / BATCH>([&](auto b) {
     constexpr int base = decltype(b)::value * BATCH;
+    if (base >= P::NV4 / 2 && low) return;
     typedef typename std::conditional<P::I8, typename P::intx4, floatx4>::type Sum;
     Sum sum[BATCH];
     for (int q = 0; q < parts; ++q) {
@@ -80,8 +83,14 @@ __device__ __forceinline__ bool join_parts(typename P::Acc &acc, int tile, int p
   return true;
 }
 
-template <class P>
+// A row tile of at most 128 rows -- the last of half of the groups -- is a low one ([N, K] weights): half the MFMAs, three quarters of the
+// loads; 8 experts of 11008 x 4096, 800 rows, 179 -> 154 us with them and the starts below, 16 of 4096 x 4096, 1900 int8 rows 76 -> 62.
+// It keeps its place among its expert's tiles, which share the weights: behind all others 64 experts of 2048 x 4096, 16384 rows, take 356 us
+// and not 347.  (Tiles drawn from a counter as CTAs become free, and not dealt out: 356.)
+template <class P, bool NN>
 __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_grouped_asm_kernel(GroupedArgs g, int ipt, Workspace ws) {
+  constexpr bool LOW = !NN;
+  constexpr int ROT_EXPERT = 11;
   GroupWalk<P::BM, false> walk(g.offsets, g.E, g.R, g.tiles_n);
   const int pid = grouped_pid(g.grid);
   zero_unowned(g, pid, P::NT);
@@ -90,51 +99,82 @@ __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_grouped_asm_kernel(
   struct Segment {
     GroupTile t;
     int cut, part, k0, n;   // (cut: number among the cut tiles, or -1)
+    bool low;
   };
-  int dp_tile = pid;
-  bool part_left = pid < (tiles - cuts.whole) * cuts.parts;
-  auto next_segment = [&](Segment &s) {
-    if (dp_tile < cuts.whole) {
-      walk.find(dp_tile, s.t);
-      s.cut = -1;
-      s.k0 = 0;
-      s.n = ipt;
-      dp_tile += g.grid;
-      return true;
+  const int items = cuts.whole + (tiles - cuts.whole) * cuts.parts;
+  auto find = [&](int tile, Segment &s) {
+    walk.find(tile, s.t);
+    s.low = LOW && s.t.rows - s.t.pm * P::BM <= P::BM / 2;
+  };
+  // Weights come straight from memory where few tiles share them, and all CTAs at the same K of rows whose pitch is a large power of two
+  // meet in the same channels (see rotation_of).  A row tile's CTAs start one iteration apart, so that they still share its rows in the
+  // L2s, those of different experts further apart, those that share weights at the same K.
+  auto rot_of = [&](const Segment &s) { return __builtin_amdgcn_readfirstlane((int)((unsigned)(s.t.pn + ROT_EXPERT * s.t.group) % (unsigned)s.n)); };
+  auto segment = [&](int item, Segment &s) {
+    if (item >= items) return false;
+    s.cut = -1;
+    s.k0 = 0;
+    s.n = ipt;
+    int tile = item;
+    if (item >= cuts.whole) {
+      const int rest = item - cuts.whole;
+      s.cut = cuts.parts == 4 ? rest >> 2 : rest >> 1;
+      s.part = rest - s.cut * cuts.parts;
+      s.k0 = s.part * ipt / cuts.parts;
+      s.n = (s.part + 1) * ipt / cuts.parts - s.k0;
+      tile = cuts.whole + s.cut;
     }
-    if (!part_left) return false;
-    part_left = false;
-    s.cut = cuts.parts == 4 ? pid >> 2 : pid >> 1;
-    s.part = pid - s.cut * cuts.parts;
-    s.k0 = s.part * ipt / cuts.parts;
-    s.n = (s.part + 1) * ipt / cuts.parts - s.k0;
-    walk.find(cuts.whole + s.cut, s.t);
+    find(tile, s);
     return true;
   };
   typename P::Acc acc;
   Segment s, next;
-  bool have = next_segment(s), requested = false;
+  int item = pid;
+  bool have = segment(item, s), requested = false;
   while (have) {
-    const typename P::Args a = expert_args<P>(g, s.t);
+    typename P::Args a = expert_args<P>(g, s.t);
     const void *epi = expert_epilogue(g, s.t);
-    P::mac(a, acc, s.t.pm, s.t.pn, s.k0, s.n, nullptr, requested);
+    if constexpr (LOW) {
+      if (s.low) P::template mac<P::LOW_TILE>(a, acc, s.t.pm, s.t.pn, s.k0, s.n, nullptr, requested, rot_of(s));
+      else P::template mac<P::WRAPPED_TILE>(a, acc, s.t.pm, s.t.pn, s.k0, s.n, nullptr, requested, rot_of(s));
+    } else {
+      P::mac(a, acc, s.t.pm, s.t.pn, s.k0, s.n, nullptr, requested);
+    }
     requested = false;
-    have = next_segment(next);   // (a part comes last)
+    item += g.grid;
+    have = segment(item, next);
     if (have && P::epilogue_lds_free(a, s.t.pn, epi)) {
-      P::prefetch_first_stage(expert_args<P>(g, next.t), next.t.pm, next.t.pn, next.k0, next.n);
+      const typename P::Args b = expert_args<P>(g, next.t);
+      if constexpr (LOW) {
+        if (next.low) P::template prefetch_first_stage<P::LOW_TILE>(b, next.t.pm, next.t.pn, next.k0, next.n, rot_of(next));
+        else P::template prefetch_first_stage<P::WRAPPED_TILE>(b, next.t.pm, next.t.pn, next.k0, next.n, rot_of(next));
+      } else {
+        P::prefetch_first_stage(b, next.t.pm, next.t.pn, next.k0, next.n);
+      }
       requested = true;
     }
-    if (s.cut < 0 || join_parts<P>(acc, s.cut, s.part, cuts.parts, g.grid, ws)) P::store_c(a, acc, s.t.pm, s.t.pn, nullptr, epi);
+    if (s.cut < 0 || join_parts<P>(acc, s.cut, s.part, cuts.parts, g.grid, ws, s.low)) {
+      if (s.low) {
+        // the lower half of each wave's 128 rows; the second wave's are the tile's rows 64 .., not 128 ..: C moved back by 64
+        const int back = (threadIdx.x >> 7) * (P::WTM / 2);
+        a.C -= (int64_t)back * a.ldc;
+        a.M += back;
+        if constexpr (is_scaled<typename P::Args>::value) a.s.a -= back;
+        P::store_c_half(a, acc, s.t.pm, s.t.pn, nullptr, epi, 0);
+      } else {
+        P::store_c(a, acc, s.t.pm, s.t.pn, nullptr, epi);
+      }
+    }
     s = next;
   }
 }
 
-template <class P>
+template <class P, bool NN = false>
 static int launch_asm(GroupedArgs g, const GroupedShape &h, int ipt, const Workspace &ws, hipStream_t s) {
   g.tiles_n = (g.N + P::BN - 1) / P::BN;
   if (grouped_tiles(h, P::BM) * g.tiles_n > 0x7fffffff) return (int)hipErrorNotSupported;
   g.grid = h.cus;
-  hipLaunchKernelGGL((sk_grouped_asm_kernel<P>), dim3(g.grid), dim3(P::NT), 0, s, g, ipt, ws);
+  hipLaunchKernelGGL((sk_grouped_asm_kernel<P, NN>), dim3(g.grid), dim3(P::NT), 0, s, g, ipt, ws);
   return (int)hipGetLastError();
 }
 
@@ -145,7 +185,7 @@ bool grouped_asm_takes(const GroupedShape &h) { return h.K % (h.type == GT_I8 ? 
 int launch_grouped_asm(const GroupedArgs &g, const GroupedShape &h, const Workspace &ws, hipStream_t s) {
   const int ipt = (int)(h.K / (h.type == GT_I8 ? 128 : 64));
   if (h.type == GT_I8) return launch_asm<ScaledAsm>(g, h, ipt, ws, s);
-  if (h.nn) return h.type == GT_BF16 ? launch_asm<TileF16Asm<1, true>>(g, h, ipt, ws, s) : launch_asm<TileF16Asm<0, true>>(g, h, ipt, ws, s);
+  if (h.nn) return h.type == GT_BF16 ? launch_asm<TileF16Asm<1, true>, true>(g, h, ipt, ws, s) : launch_asm<TileF16Asm<0, true>, true>(g, h, ipt, ws, s);
   return h.type == GT_BF16 ? launch_asm<TileF16Asm<1, false>>(g, h, ipt, ws, s) : launch_asm<TileF16Asm<0, false>>(g, h, ipt, ws, s);
 }
 

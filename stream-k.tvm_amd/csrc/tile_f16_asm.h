@@ -146,18 +146,28 @@ struct TileF16Asm {
   // the 16 loads of stage `stage` (iteration k0 + stage of the segment; nothing is fetched if the segment is shorter),
   // or -- EARLY_ONLY -- just those the loop does not send itself: the row groups that hold blocks 0-3 of the wave tiles
   // (NN: and all of B); see gen_tile_asm.py
-  template <bool EARLY_ONLY = false>
-  static __device__ __forceinline__ void stage_loads(const Ctx &c, int stage, int n) {
+  // LOW_TILE: at most 128 rows, 64 to a wave: 12 loads of a stage, no late row groups of A.  WRAPPED_TILE and LOW_TILE (NT): the segment
+  // starts `rot` iterations into its K and wraps around, iteration `wrap` being the first K's.
+  enum Kind { WHOLE_TILE, WRAPPED_TILE, LOW_TILE };
+  template <bool EARLY_ONLY = false, Kind KIND = WHOLE_TILE>
+  static __device__ __forceinline__ void stage_loads(const Ctx &c, int stage, int n, int wrap = -1) {
     const uint32_t oob = stage < n ? 0u : OOB_OFFSET;
     const uint32_t voa = c.voff_a | oob, vob = c.voff_b | oob, vob1 = c.voff_b1 | oob;
-    const uint32_t ga = c.goff_a + (uint32_t)stage * 128, gb = c.goff_b + (uint32_t)stage * c.kstep_b;
+    constexpr bool LOW = KIND == LOW_TILE, WRAPS = KIND != WHOLE_TILE;
+    const uint32_t step = (uint32_t)stage * 128 - (WRAPS && stage == wrap ? (uint32_t)n * 128 : 0u);
+    const uint32_t ga = c.goff_a + step, gb = c.goff_b + (WRAPS ? step : (uint32_t)stage * c.kstep_b);
     const uint32_t lds_stage = c.lds_wave + (uint32_t)stage * STAGE_BYTES;
 #define SK_ASM_LOAD_OPERANDS                                                                                             \
   : : [rsa] "s"(c.rsrc_a), [rsb] "s"(c.rsrc_b), [voa] "v"(voa), [vob] "v"(vob), [vob1] "v"(vob1), [ga] "s"(ga),            \
       [gb] "s"(gb), [gas] "s"(c.gstep_a), [gas2] "s"(2 * c.gstep_a), [gas3] "s"(3 * c.gstep_a), [gbs] "s"(c.gstep_b),     \
       [gbs2] "s"(2 * c.gstep_b), [gbs3] "s"(3 * c.gstep_b), [lds] "s"(lds_stage)                                          \
   : "memory", "m0", "scc", "s83"
-    if constexpr (NN_ && EARLY_ONLY) {
+    static_assert(!WRAPS || (!NN_ && F8 == 0), "see gen_tile_asm.py");
+    if constexpr (LOW && EARLY_ONLY) {
+      asm volatile(SK_TILE_ASM_LOADS_EARLY_LOW SK_ASM_LOAD_OPERANDS);
+    } else if constexpr (LOW) {
+      asm volatile(SK_TILE_ASM_LOADS_LOW SK_ASM_LOAD_OPERANDS);
+    } else if constexpr (NN_ && EARLY_ONLY) {
       asm volatile(SK_TILE_ASM_LOADS_EARLY_NN SK_ASM_LOAD_OPERANDS);
     } else if constexpr (NN_) {
       asm volatile(SK_TILE_ASM_LOADS_NN SK_ASM_LOAD_OPERANDS);
@@ -173,18 +183,21 @@ struct TileF16Asm {
   // wave has left the loop of the current one, ahead of an epilogue that does not use LDS, and mac() is then told
   // that the stage is on its way.
   static constexpr bool CROSS_TILE_PREFETCH = true;
-  static __device__ __forceinline__ void prefetch_first_stage(const Args &a, int pm, int pn, int k0, int n) {
-    const Ctx c = make_ctx(a, pm, pn, k0);
-    stage_loads(c, 0, n);
+  template <Kind KIND = WHOLE_TILE>
+  static __device__ __forceinline__ void prefetch_first_stage(const Args &a, int pm, int pn, int k0, int n, int rot = 0) {
+    const Ctx c = make_ctx(a, pm, pn, k0 + rot);
+    stage_loads<false, KIND>(c, 0, n);
   }
 
+  template <Kind KIND = WHOLE_TILE>
   static __device__ __forceinline__ void mac(const Args &a, Acc &, int pm, int pn, int k0, int n, char *,
-                                             bool first_stage_requested = false) {
-    Ctx c = make_ctx(a, pm, pn, k0);
-    if (!first_stage_requested) stage_loads(c, 0, n);
+                                             bool first_stage_requested = false, int rot = 0) {
+    const uint32_t wrap = (uint32_t)(n - rot), back = 128u - (uint32_t)n * 128u;
+    Ctx c = make_ctx(a, pm, pn, k0 + rot);
+    if (!first_stage_requested) stage_loads<false, KIND>(c, 0, n);
     // (directly ahead of the loop, whose first wait counts on these being the youngest operations; the 16-bit loops
     // send the late row groups of the second stage themselves)
-    stage_loads<F8 == 0>(c, 1, n);
+    stage_loads<F8 == 0, KIND>(c, 1, n, (int)wrap);
     const uint32_t iters = (uint32_t)n;
     if constexpr (NN_) {
 #define SK_ASM_NN_OPERANDS                                                                                            \
@@ -207,7 +220,26 @@ struct TileF16Asm {
     [gb0] "s"(c.goff_b), [gas] "s"(c.gstep_a), [gas2] "s"(2 * c.gstep_a), [gas3] "s"(3 * c.gstep_a),                  \
     [gbs] "s"(c.gstep_b), [gbs2] "s"(2 * c.gstep_b), [gbs3] "s"(3 * c.gstep_b), [n] "s"(iters), [lds] "s"(c.lds_wave)  \
   : "memory", "m0", "scc", SK_TILE_ASM_CLOBBERS
-      if constexpr (F8 == 1) {
+#define SK_ASM_WRAP_OPERANDS                                                                                        \
+  : [ra0] "+v"(c.ra0), [ra1] "+v"(c.ra1), [rb0] "+v"(c.rb0), [rb1] "+v"(c.rb1)                                      \
+  : [rsa] "s"(c.rsrc_a), [rsb] "s"(c.rsrc_b), [voa] "v"(c.voff_a), [vob] "v"(c.voff_b), [ga0] "s"(c.goff_a),          \
+    [gb0] "s"(c.goff_b), [gas] "s"(c.gstep_a), [gas2] "s"(2 * c.gstep_a), [gas3] "s"(3 * c.gstep_a),                  \
+    [gbs] "s"(c.gstep_b), [gbs2] "s"(2 * c.gstep_b), [gbs3] "s"(3 * c.gstep_b), [n] "s"(iters), [lds] "s"(c.lds_wave), \
+    [wrap] "s"(wrap), [back] "s"(back)                                                                                \
+  : "memory", "m0", "scc", SK_TILE_ASM_CLOBBERS
+      if constexpr (KIND == LOW_TILE && I8) {
+        asm volatile(SK_TILE_ASM_LOOP_LOW("v_mfma_i32_16x16x64_i8") SK_ASM_WRAP_OPERANDS);
+      } else if constexpr (KIND == LOW_TILE && BF16_) {
+        asm volatile(SK_TILE_ASM_LOOP_LOW("v_mfma_f32_16x16x32_bf16") SK_ASM_WRAP_OPERANDS);
+      } else if constexpr (KIND == LOW_TILE) {
+        asm volatile(SK_TILE_ASM_LOOP_LOW("v_mfma_f32_16x16x32_f16") SK_ASM_WRAP_OPERANDS);
+      } else if constexpr (KIND == WRAPPED_TILE && I8) {
+        asm volatile(SK_TILE_ASM_LOOP_WRAP("v_mfma_i32_16x16x64_i8") SK_ASM_WRAP_OPERANDS);
+      } else if constexpr (KIND == WRAPPED_TILE && BF16_) {
+        asm volatile(SK_TILE_ASM_LOOP_WRAP("v_mfma_f32_16x16x32_bf16") SK_ASM_WRAP_OPERANDS);
+      } else if constexpr (KIND == WRAPPED_TILE) {
+        asm volatile(SK_TILE_ASM_LOOP_WRAP("v_mfma_f32_16x16x32_f16") SK_ASM_WRAP_OPERANDS);
+      } else if constexpr (F8 == 1) {
         asm volatile(SK_TILE_ASM_LOOP_F8("v_mfma_f32_16x16x128_f8f6f4", "") SK_ASM_NT_OPERANDS);
       } else if constexpr (F8 == 2) {
         asm volatile(SK_TILE_ASM_LOOP_F8("v_mfma_f32_16x16x128_f8f6f4", "cbsz:1 blgp:1") SK_ASM_NT_OPERANDS);
@@ -218,6 +250,7 @@ struct TileF16Asm {
       } else {
         asm volatile(SK_TILE_ASM_LOOP("v_mfma_f32_16x16x32_f16") SK_ASM_NT_OPERANDS);
       }
+#undef SK_ASM_WRAP_OPERANDS
 #undef SK_ASM_NT_OPERANDS
     }
     // every wave has left the loop and its own loads have landed: both stages are free (for the epilogue's patches,

@@ -1,6 +1,6 @@
 // Generated by gen_tile_asm.py -- do not edit; see that file for the register plan and the schedule.
 // SK_TILE_ASM_LOADS / _LOADS_NN / _LOADS_TN: the 16 loads of one stage.  SK_TILE_ASM_LOOP(MF) / _LOOP_NN(MF) / _LOOP_TN(MF): the loop
-// for the NT / NN / TN layout, MF = the MFMA mnemonic as a string literal.  SK_TILE_ASM_LOOP_F8(MF, MOD): fp8 operands, MOD =
+// (_LOW: tiles of at most 128 rows) for the NT / NN / TN layout, MF = the MFMA mnemonic as a string literal.  SK_TILE_ASM_LOOP_F8(MF, MOD): fp8 operands, MOD =
 // the format modifiers of the MFMA ("" for e4m3).  SK_TILE_ASM_STORE_x(CVT): the epilogue that leaves the stages alone.
 #pragma once
 #define SK_TILE_ASM_LOADS \
@@ -318,6 +318,90 @@
   "s_add_u32 m0, %[lds], 45056\n\t" \
   "s_nop 0\n\t" \
   "buffer_load_dwordx4 %[vob1], %[rsb], s83 offen lds\n\t" \
+  ""
+#define SK_TILE_ASM_LOADS_LOW \
+  "s_mov_b32 s83, %[ga]\n\t" \
+  "s_add_u32 m0, %[lds], 0\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[voa], %[rsa], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, %[lds], 4096\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[voa], %[rsa], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, %[lds], 16384\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[voa], %[rsa], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, %[lds], 20480\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[voa], %[rsa], s83 offen lds\n\t" \
+  "s_mov_b32 s83, %[gb]\n\t" \
+  "s_add_u32 m0, %[lds], 32768\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob], %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, %[lds], 36864\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob], %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, %[lds], 40960\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob], %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, %[lds], 45056\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob], %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, %[lds], 49152\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob], %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, %[lds], 53248\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob], %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, %[lds], 57344\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob], %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, %[lds], 61440\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob], %[rsb], s83 offen lds\n\t" \
+  ""
+#define SK_TILE_ASM_LOADS_EARLY_LOW \
+  "s_mov_b32 s83, %[ga]\n\t" \
+  "s_add_u32 m0, %[lds], 0\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[voa], %[rsa], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, %[lds], 4096\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[voa], %[rsa], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, %[lds], 16384\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[voa], %[rsa], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, %[lds], 20480\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[voa], %[rsa], s83 offen lds\n\t" \
+  "s_mov_b32 s83, %[gb]\n\t" \
+  "s_add_u32 m0, %[lds], 32768\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob], %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, %[lds], 36864\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob], %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs3]\n\t" \
+  "s_add_u32 m0, %[lds], 49152\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob], %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, %[lds], 53248\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob], %[rsb], s83 offen lds\n\t" \
   ""
 #define SK_TILE_ASM_LOOP(MF) \
   "v_accvgpr_write_b32 a0, 0\n\t" \
@@ -842,6 +926,860 @@
   MF " a[132:135], v[228:231], v[208:211], a[132:135]\n\t" \
   MF " a[136:139], v[232:235], v[208:211], a[136:139]\n\t" \
   MF " a[140:143], v[236:239], v[208:211], a[140:143]\n\t" \
+  "s_add_u32 s80, s80, 1\n\t" \
+  "s_waitcnt vmcnt(8) lgkmcnt(0)\n\t" \
+  "s_barrier\n\t" \
+  "s_cmp_lt_u32 s80, %[n]\n\t" \
+  "s_cbranch_scc1 L_sk_loop%=\n\t" \
+  "s_waitcnt vmcnt(0) lgkmcnt(0)\n\t" \
+  "s_nop 7\n\t" \
+  "s_nop 7\n\t" \
+  "s_nop 7\n\t" \
+  ""
+#define SK_TILE_ASM_LOOP_WRAP(MF) \
+  "v_accvgpr_write_b32 a0, 0\n\t" \
+  "v_accvgpr_write_b32 a1, 0\n\t" \
+  "v_accvgpr_write_b32 a2, 0\n\t" \
+  "v_accvgpr_write_b32 a3, 0\n\t" \
+  "v_accvgpr_write_b32 a4, 0\n\t" \
+  "v_accvgpr_write_b32 a5, 0\n\t" \
+  "v_accvgpr_write_b32 a6, 0\n\t" \
+  "v_accvgpr_write_b32 a7, 0\n\t" \
+  "v_accvgpr_write_b32 a8, 0\n\t" \
+  "v_accvgpr_write_b32 a9, 0\n\t" \
+  "v_accvgpr_write_b32 a10, 0\n\t" \
+  "v_accvgpr_write_b32 a11, 0\n\t" \
+  "v_accvgpr_write_b32 a12, 0\n\t" \
+  "v_accvgpr_write_b32 a13, 0\n\t" \
+  "v_accvgpr_write_b32 a14, 0\n\t" \
+  "v_accvgpr_write_b32 a15, 0\n\t" \
+  "v_accvgpr_write_b32 a16, 0\n\t" \
+  "v_accvgpr_write_b32 a17, 0\n\t" \
+  "v_accvgpr_write_b32 a18, 0\n\t" \
+  "v_accvgpr_write_b32 a19, 0\n\t" \
+  "v_accvgpr_write_b32 a20, 0\n\t" \
+  "v_accvgpr_write_b32 a21, 0\n\t" \
+  "v_accvgpr_write_b32 a22, 0\n\t" \
+  "v_accvgpr_write_b32 a23, 0\n\t" \
+  "v_accvgpr_write_b32 a24, 0\n\t" \
+  "v_accvgpr_write_b32 a25, 0\n\t" \
+  "v_accvgpr_write_b32 a26, 0\n\t" \
+  "v_accvgpr_write_b32 a27, 0\n\t" \
+  "v_accvgpr_write_b32 a28, 0\n\t" \
+  "v_accvgpr_write_b32 a29, 0\n\t" \
+  "v_accvgpr_write_b32 a30, 0\n\t" \
+  "v_accvgpr_write_b32 a31, 0\n\t" \
+  "v_accvgpr_write_b32 a32, 0\n\t" \
+  "v_accvgpr_write_b32 a33, 0\n\t" \
+  "v_accvgpr_write_b32 a34, 0\n\t" \
+  "v_accvgpr_write_b32 a35, 0\n\t" \
+  "v_accvgpr_write_b32 a36, 0\n\t" \
+  "v_accvgpr_write_b32 a37, 0\n\t" \
+  "v_accvgpr_write_b32 a38, 0\n\t" \
+  "v_accvgpr_write_b32 a39, 0\n\t" \
+  "v_accvgpr_write_b32 a40, 0\n\t" \
+  "v_accvgpr_write_b32 a41, 0\n\t" \
+  "v_accvgpr_write_b32 a42, 0\n\t" \
+  "v_accvgpr_write_b32 a43, 0\n\t" \
+  "v_accvgpr_write_b32 a44, 0\n\t" \
+  "v_accvgpr_write_b32 a45, 0\n\t" \
+  "v_accvgpr_write_b32 a46, 0\n\t" \
+  "v_accvgpr_write_b32 a47, 0\n\t" \
+  "v_accvgpr_write_b32 a48, 0\n\t" \
+  "v_accvgpr_write_b32 a49, 0\n\t" \
+  "v_accvgpr_write_b32 a50, 0\n\t" \
+  "v_accvgpr_write_b32 a51, 0\n\t" \
+  "v_accvgpr_write_b32 a52, 0\n\t" \
+  "v_accvgpr_write_b32 a53, 0\n\t" \
+  "v_accvgpr_write_b32 a54, 0\n\t" \
+  "v_accvgpr_write_b32 a55, 0\n\t" \
+  "v_accvgpr_write_b32 a56, 0\n\t" \
+  "v_accvgpr_write_b32 a57, 0\n\t" \
+  "v_accvgpr_write_b32 a58, 0\n\t" \
+  "v_accvgpr_write_b32 a59, 0\n\t" \
+  "v_accvgpr_write_b32 a60, 0\n\t" \
+  "v_accvgpr_write_b32 a61, 0\n\t" \
+  "v_accvgpr_write_b32 a62, 0\n\t" \
+  "v_accvgpr_write_b32 a63, 0\n\t" \
+  "v_accvgpr_write_b32 a64, 0\n\t" \
+  "v_accvgpr_write_b32 a65, 0\n\t" \
+  "v_accvgpr_write_b32 a66, 0\n\t" \
+  "v_accvgpr_write_b32 a67, 0\n\t" \
+  "v_accvgpr_write_b32 a68, 0\n\t" \
+  "v_accvgpr_write_b32 a69, 0\n\t" \
+  "v_accvgpr_write_b32 a70, 0\n\t" \
+  "v_accvgpr_write_b32 a71, 0\n\t" \
+  "v_accvgpr_write_b32 a72, 0\n\t" \
+  "v_accvgpr_write_b32 a73, 0\n\t" \
+  "v_accvgpr_write_b32 a74, 0\n\t" \
+  "v_accvgpr_write_b32 a75, 0\n\t" \
+  "v_accvgpr_write_b32 a76, 0\n\t" \
+  "v_accvgpr_write_b32 a77, 0\n\t" \
+  "v_accvgpr_write_b32 a78, 0\n\t" \
+  "v_accvgpr_write_b32 a79, 0\n\t" \
+  "v_accvgpr_write_b32 a80, 0\n\t" \
+  "v_accvgpr_write_b32 a81, 0\n\t" \
+  "v_accvgpr_write_b32 a82, 0\n\t" \
+  "v_accvgpr_write_b32 a83, 0\n\t" \
+  "v_accvgpr_write_b32 a84, 0\n\t" \
+  "v_accvgpr_write_b32 a85, 0\n\t" \
+  "v_accvgpr_write_b32 a86, 0\n\t" \
+  "v_accvgpr_write_b32 a87, 0\n\t" \
+  "v_accvgpr_write_b32 a88, 0\n\t" \
+  "v_accvgpr_write_b32 a89, 0\n\t" \
+  "v_accvgpr_write_b32 a90, 0\n\t" \
+  "v_accvgpr_write_b32 a91, 0\n\t" \
+  "v_accvgpr_write_b32 a92, 0\n\t" \
+  "v_accvgpr_write_b32 a93, 0\n\t" \
+  "v_accvgpr_write_b32 a94, 0\n\t" \
+  "v_accvgpr_write_b32 a95, 0\n\t" \
+  "v_accvgpr_write_b32 a96, 0\n\t" \
+  "v_accvgpr_write_b32 a97, 0\n\t" \
+  "v_accvgpr_write_b32 a98, 0\n\t" \
+  "v_accvgpr_write_b32 a99, 0\n\t" \
+  "v_accvgpr_write_b32 a100, 0\n\t" \
+  "v_accvgpr_write_b32 a101, 0\n\t" \
+  "v_accvgpr_write_b32 a102, 0\n\t" \
+  "v_accvgpr_write_b32 a103, 0\n\t" \
+  "v_accvgpr_write_b32 a104, 0\n\t" \
+  "v_accvgpr_write_b32 a105, 0\n\t" \
+  "v_accvgpr_write_b32 a106, 0\n\t" \
+  "v_accvgpr_write_b32 a107, 0\n\t" \
+  "v_accvgpr_write_b32 a108, 0\n\t" \
+  "v_accvgpr_write_b32 a109, 0\n\t" \
+  "v_accvgpr_write_b32 a110, 0\n\t" \
+  "v_accvgpr_write_b32 a111, 0\n\t" \
+  "v_accvgpr_write_b32 a112, 0\n\t" \
+  "v_accvgpr_write_b32 a113, 0\n\t" \
+  "v_accvgpr_write_b32 a114, 0\n\t" \
+  "v_accvgpr_write_b32 a115, 0\n\t" \
+  "v_accvgpr_write_b32 a116, 0\n\t" \
+  "v_accvgpr_write_b32 a117, 0\n\t" \
+  "v_accvgpr_write_b32 a118, 0\n\t" \
+  "v_accvgpr_write_b32 a119, 0\n\t" \
+  "v_accvgpr_write_b32 a120, 0\n\t" \
+  "v_accvgpr_write_b32 a121, 0\n\t" \
+  "v_accvgpr_write_b32 a122, 0\n\t" \
+  "v_accvgpr_write_b32 a123, 0\n\t" \
+  "v_accvgpr_write_b32 a124, 0\n\t" \
+  "v_accvgpr_write_b32 a125, 0\n\t" \
+  "v_accvgpr_write_b32 a126, 0\n\t" \
+  "v_accvgpr_write_b32 a127, 0\n\t" \
+  "v_accvgpr_write_b32 a128, 0\n\t" \
+  "v_accvgpr_write_b32 a129, 0\n\t" \
+  "v_accvgpr_write_b32 a130, 0\n\t" \
+  "v_accvgpr_write_b32 a131, 0\n\t" \
+  "v_accvgpr_write_b32 a132, 0\n\t" \
+  "v_accvgpr_write_b32 a133, 0\n\t" \
+  "v_accvgpr_write_b32 a134, 0\n\t" \
+  "v_accvgpr_write_b32 a135, 0\n\t" \
+  "v_accvgpr_write_b32 a136, 0\n\t" \
+  "v_accvgpr_write_b32 a137, 0\n\t" \
+  "v_accvgpr_write_b32 a138, 0\n\t" \
+  "v_accvgpr_write_b32 a139, 0\n\t" \
+  "v_accvgpr_write_b32 a140, 0\n\t" \
+  "v_accvgpr_write_b32 a141, 0\n\t" \
+  "v_accvgpr_write_b32 a142, 0\n\t" \
+  "v_accvgpr_write_b32 a143, 0\n\t" \
+  "v_accvgpr_write_b32 a144, 0\n\t" \
+  "v_accvgpr_write_b32 a145, 0\n\t" \
+  "v_accvgpr_write_b32 a146, 0\n\t" \
+  "v_accvgpr_write_b32 a147, 0\n\t" \
+  "v_accvgpr_write_b32 a148, 0\n\t" \
+  "v_accvgpr_write_b32 a149, 0\n\t" \
+  "v_accvgpr_write_b32 a150, 0\n\t" \
+  "v_accvgpr_write_b32 a151, 0\n\t" \
+  "v_accvgpr_write_b32 a152, 0\n\t" \
+  "v_accvgpr_write_b32 a153, 0\n\t" \
+  "v_accvgpr_write_b32 a154, 0\n\t" \
+  "v_accvgpr_write_b32 a155, 0\n\t" \
+  "v_accvgpr_write_b32 a156, 0\n\t" \
+  "v_accvgpr_write_b32 a157, 0\n\t" \
+  "v_accvgpr_write_b32 a158, 0\n\t" \
+  "v_accvgpr_write_b32 a159, 0\n\t" \
+  "v_accvgpr_write_b32 a160, 0\n\t" \
+  "v_accvgpr_write_b32 a161, 0\n\t" \
+  "v_accvgpr_write_b32 a162, 0\n\t" \
+  "v_accvgpr_write_b32 a163, 0\n\t" \
+  "v_accvgpr_write_b32 a164, 0\n\t" \
+  "v_accvgpr_write_b32 a165, 0\n\t" \
+  "v_accvgpr_write_b32 a166, 0\n\t" \
+  "v_accvgpr_write_b32 a167, 0\n\t" \
+  "v_accvgpr_write_b32 a168, 0\n\t" \
+  "v_accvgpr_write_b32 a169, 0\n\t" \
+  "v_accvgpr_write_b32 a170, 0\n\t" \
+  "v_accvgpr_write_b32 a171, 0\n\t" \
+  "v_accvgpr_write_b32 a172, 0\n\t" \
+  "v_accvgpr_write_b32 a173, 0\n\t" \
+  "v_accvgpr_write_b32 a174, 0\n\t" \
+  "v_accvgpr_write_b32 a175, 0\n\t" \
+  "v_accvgpr_write_b32 a176, 0\n\t" \
+  "v_accvgpr_write_b32 a177, 0\n\t" \
+  "v_accvgpr_write_b32 a178, 0\n\t" \
+  "v_accvgpr_write_b32 a179, 0\n\t" \
+  "v_accvgpr_write_b32 a180, 0\n\t" \
+  "v_accvgpr_write_b32 a181, 0\n\t" \
+  "v_accvgpr_write_b32 a182, 0\n\t" \
+  "v_accvgpr_write_b32 a183, 0\n\t" \
+  "v_accvgpr_write_b32 a184, 0\n\t" \
+  "v_accvgpr_write_b32 a185, 0\n\t" \
+  "v_accvgpr_write_b32 a186, 0\n\t" \
+  "v_accvgpr_write_b32 a187, 0\n\t" \
+  "v_accvgpr_write_b32 a188, 0\n\t" \
+  "v_accvgpr_write_b32 a189, 0\n\t" \
+  "v_accvgpr_write_b32 a190, 0\n\t" \
+  "v_accvgpr_write_b32 a191, 0\n\t" \
+  "v_accvgpr_write_b32 a192, 0\n\t" \
+  "v_accvgpr_write_b32 a193, 0\n\t" \
+  "v_accvgpr_write_b32 a194, 0\n\t" \
+  "v_accvgpr_write_b32 a195, 0\n\t" \
+  "v_accvgpr_write_b32 a196, 0\n\t" \
+  "v_accvgpr_write_b32 a197, 0\n\t" \
+  "v_accvgpr_write_b32 a198, 0\n\t" \
+  "v_accvgpr_write_b32 a199, 0\n\t" \
+  "v_accvgpr_write_b32 a200, 0\n\t" \
+  "v_accvgpr_write_b32 a201, 0\n\t" \
+  "v_accvgpr_write_b32 a202, 0\n\t" \
+  "v_accvgpr_write_b32 a203, 0\n\t" \
+  "v_accvgpr_write_b32 a204, 0\n\t" \
+  "v_accvgpr_write_b32 a205, 0\n\t" \
+  "v_accvgpr_write_b32 a206, 0\n\t" \
+  "v_accvgpr_write_b32 a207, 0\n\t" \
+  "v_accvgpr_write_b32 a208, 0\n\t" \
+  "v_accvgpr_write_b32 a209, 0\n\t" \
+  "v_accvgpr_write_b32 a210, 0\n\t" \
+  "v_accvgpr_write_b32 a211, 0\n\t" \
+  "v_accvgpr_write_b32 a212, 0\n\t" \
+  "v_accvgpr_write_b32 a213, 0\n\t" \
+  "v_accvgpr_write_b32 a214, 0\n\t" \
+  "v_accvgpr_write_b32 a215, 0\n\t" \
+  "v_accvgpr_write_b32 a216, 0\n\t" \
+  "v_accvgpr_write_b32 a217, 0\n\t" \
+  "v_accvgpr_write_b32 a218, 0\n\t" \
+  "v_accvgpr_write_b32 a219, 0\n\t" \
+  "v_accvgpr_write_b32 a220, 0\n\t" \
+  "v_accvgpr_write_b32 a221, 0\n\t" \
+  "v_accvgpr_write_b32 a222, 0\n\t" \
+  "v_accvgpr_write_b32 a223, 0\n\t" \
+  "v_accvgpr_write_b32 a224, 0\n\t" \
+  "v_accvgpr_write_b32 a225, 0\n\t" \
+  "v_accvgpr_write_b32 a226, 0\n\t" \
+  "v_accvgpr_write_b32 a227, 0\n\t" \
+  "v_accvgpr_write_b32 a228, 0\n\t" \
+  "v_accvgpr_write_b32 a229, 0\n\t" \
+  "v_accvgpr_write_b32 a230, 0\n\t" \
+  "v_accvgpr_write_b32 a231, 0\n\t" \
+  "v_accvgpr_write_b32 a232, 0\n\t" \
+  "v_accvgpr_write_b32 a233, 0\n\t" \
+  "v_accvgpr_write_b32 a234, 0\n\t" \
+  "v_accvgpr_write_b32 a235, 0\n\t" \
+  "v_accvgpr_write_b32 a236, 0\n\t" \
+  "v_accvgpr_write_b32 a237, 0\n\t" \
+  "v_accvgpr_write_b32 a238, 0\n\t" \
+  "v_accvgpr_write_b32 a239, 0\n\t" \
+  "v_accvgpr_write_b32 a240, 0\n\t" \
+  "v_accvgpr_write_b32 a241, 0\n\t" \
+  "v_accvgpr_write_b32 a242, 0\n\t" \
+  "v_accvgpr_write_b32 a243, 0\n\t" \
+  "v_accvgpr_write_b32 a244, 0\n\t" \
+  "v_accvgpr_write_b32 a245, 0\n\t" \
+  "v_accvgpr_write_b32 a246, 0\n\t" \
+  "v_accvgpr_write_b32 a247, 0\n\t" \
+  "v_accvgpr_write_b32 a248, 0\n\t" \
+  "v_accvgpr_write_b32 a249, 0\n\t" \
+  "v_accvgpr_write_b32 a250, 0\n\t" \
+  "v_accvgpr_write_b32 a251, 0\n\t" \
+  "v_accvgpr_write_b32 a252, 0\n\t" \
+  "v_accvgpr_write_b32 a253, 0\n\t" \
+  "v_accvgpr_write_b32 a254, 0\n\t" \
+  "v_accvgpr_write_b32 a255, 0\n\t" \
+  "s_mov_b32 s80, 0\n\t" \
+  "s_xor_b32 s86, %[lds], 0x10000\n\t" \
+  "s_cmp_eq_u32 %[wrap], 1\n\t" \
+  "s_cselect_b32 s85, %[back], 128\n\t" \
+  "s_add_u32 s81, %[ga0], s85\n\t" \
+  "s_add_u32 s82, %[gb0], s85\n\t" \
+  "s_add_u32 s87, s80, 1\n\t" \
+  "s_cmp_lt_u32 s87, %[n]\n\t" \
+  "s_cselect_b32 s84, 0, 0x80000000\n\t" \
+  "v_or_b32 v120, s84, %[voa]\n\t" \
+  "v_or_b32 v121, s84, %[vob]\n\t" \
+  "s_waitcnt vmcnt(8)\n\t" \
+  "s_barrier\n\t" \
+  "ds_read_b128 v[128:131], %[ra0] offset:0\n\t" \
+  "ds_read_b128 v[160:163], %[rb0] offset:0\n\t" \
+  "ds_read_b128 v[164:167], %[rb0] offset:2048\n\t" \
+  "ds_read_b128 v[168:171], %[rb0] offset:4096\n\t" \
+  "ds_read_b128 v[172:175], %[rb0] offset:6144\n\t" \
+  "ds_read_b128 v[132:135], %[ra0] offset:2048\n\t" \
+  "ds_read_b128 v[136:139], %[ra0] offset:4096\n\t" \
+  "ds_read_b128 v[140:143], %[ra0] offset:6144\n\t" \
+  "s_nop 7\n\t" \
+  "L_sk_loop%=:\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  MF " a[0:3], v[160:163], v[128:131], a[0:3]\n\t" \
+  "ds_read_b128 v[176:179], %[rb0] offset:8192\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  MF " a[4:7], v[164:167], v[128:131], a[4:7]\n\t" \
+  "ds_read_b128 v[180:183], %[rb0] offset:10240\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  MF " a[8:11], v[168:171], v[128:131], a[8:11]\n\t" \
+  "ds_read_b128 v[184:187], %[rb0] offset:12288\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  MF " a[12:15], v[172:175], v[128:131], a[12:15]\n\t" \
+  "ds_read_b128 v[188:191], %[rb0] offset:14336\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  MF " a[44:47], v[172:175], v[132:135], a[44:47]\n\t" \
+  "ds_read_b128 v[144:147], %[ra0] offset:8192\n\t" \
+  MF " a[40:43], v[168:171], v[132:135], a[40:43]\n\t" \
+  "ds_read_b128 v[148:151], %[ra0] offset:10240\n\t" \
+  MF " a[36:39], v[164:167], v[132:135], a[36:39]\n\t" \
+  "ds_read_b128 v[152:155], %[ra0] offset:12288\n\t" \
+  MF " a[32:35], v[160:163], v[132:135], a[32:35]\n\t" \
+  "ds_read_b128 v[156:159], %[ra0] offset:14336\n\t" \
+  "s_waitcnt lgkmcnt(9)\n\t" \
+  MF " a[64:67], v[160:163], v[136:139], a[64:67]\n\t" \
+  "s_add_u32 s83, s81, %[gas2]\n\t" \
+  "s_add_u32 m0, s86, 8192\n\t" \
+  MF " a[68:71], v[164:167], v[136:139], a[68:71]\n\t" \
+  "ds_read_b128 v[192:195], %[ra1] offset:0\n\t" \
+  MF " a[72:75], v[168:171], v[136:139], a[72:75]\n\t" \
+  "v_xor_b32 %[ra0], 0x10000, %[ra0]\n\t" \
+  MF " a[76:79], v[172:175], v[136:139], a[76:79]\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  "s_waitcnt lgkmcnt(9)\n\t" \
+  MF " a[108:111], v[172:175], v[140:143], a[108:111]\n\t" \
+  MF " a[104:107], v[168:171], v[140:143], a[104:107]\n\t" \
+  MF " a[100:103], v[164:167], v[140:143], a[100:103]\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, s86, 12288\n\t" \
+  MF " a[96:99], v[160:163], v[140:143], a[96:99]\n\t" \
+  "ds_read_b128 v[224:227], %[rb1] offset:0\n\t" \
+  "s_waitcnt lgkmcnt(9)\n\t" \
+  MF " a[112:115], v[176:179], v[140:143], a[112:115]\n\t" \
+  "s_waitcnt lgkmcnt(8)\n\t" \
+  MF " a[116:119], v[180:183], v[140:143], a[116:119]\n\t" \
+  "s_waitcnt lgkmcnt(7)\n\t" \
+  MF " a[120:123], v[184:187], v[140:143], a[120:123]\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  MF " a[124:127], v[188:191], v[140:143], a[124:127]\n\t" \
+  MF " a[92:95], v[188:191], v[136:139], a[92:95]\n\t" \
+  "ds_read_b128 v[228:231], %[rb1] offset:2048\n\t" \
+  MF " a[88:91], v[184:187], v[136:139], a[88:91]\n\t" \
+  "s_add_u32 s83, s83, %[gas3]\n\t" \
+  "s_add_u32 m0, s86, 24576\n\t" \
+  MF " a[84:87], v[180:183], v[136:139], a[84:87]\n\t" \
+  MF " a[80:83], v[176:179], v[136:139], a[80:83]\n\t" \
+  MF " a[48:51], v[176:179], v[132:135], a[48:51]\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  MF " a[52:55], v[180:183], v[132:135], a[52:55]\n\t" \
+  MF " a[56:59], v[184:187], v[132:135], a[56:59]\n\t" \
+  "ds_read_b128 v[232:235], %[rb1] offset:4096\n\t" \
+  MF " a[60:63], v[188:191], v[132:135], a[60:63]\n\t" \
+  MF " a[28:31], v[188:191], v[128:131], a[28:31]\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, s86, 28672\n\t" \
+  MF " a[24:27], v[184:187], v[128:131], a[24:27]\n\t" \
+  MF " a[20:23], v[180:183], v[128:131], a[20:23]\n\t" \
+  MF " a[16:19], v[176:179], v[128:131], a[16:19]\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  "s_waitcnt lgkmcnt(7)\n\t" \
+  MF " a[144:147], v[176:179], v[144:147], a[144:147]\n\t" \
+  "ds_read_b128 v[236:239], %[rb1] offset:6144\n\t" \
+  MF " a[148:151], v[180:183], v[144:147], a[148:151]\n\t" \
+  MF " a[152:155], v[184:187], v[144:147], a[152:155]\n\t" \
+  MF " a[156:159], v[188:191], v[144:147], a[156:159]\n\t" \
+  "s_add_u32 s83, s82, %[gbs2]\n\t" \
+  "s_add_u32 m0, s86, 40960\n\t" \
+  "s_waitcnt lgkmcnt(7)\n\t" \
+  MF " a[188:191], v[188:191], v[148:151], a[188:191]\n\t" \
+  MF " a[184:187], v[184:187], v[148:151], a[184:187]\n\t" \
+  "ds_read_b128 v[196:199], %[ra1] offset:2048\n\t" \
+  MF " a[180:183], v[180:183], v[148:151], a[180:183]\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  MF " a[176:179], v[176:179], v[148:151], a[176:179]\n\t" \
+  "s_waitcnt lgkmcnt(7)\n\t" \
+  MF " a[208:211], v[176:179], v[152:155], a[208:211]\n\t" \
+  "v_xor_b32 %[rb0], 0x10000, %[rb0]\n\t" \
+  MF " a[212:215], v[180:183], v[152:155], a[212:215]\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 45056\n\t" \
+  MF " a[216:219], v[184:187], v[152:155], a[216:219]\n\t" \
+  MF " a[220:223], v[188:191], v[152:155], a[220:223]\n\t" \
+  "ds_read_b128 v[200:203], %[ra1] offset:4096\n\t" \
+  "s_waitcnt lgkmcnt(7)\n\t" \
+  MF " a[252:255], v[188:191], v[156:159], a[252:255]\n\t" \
+  MF " a[248:251], v[184:187], v[156:159], a[248:251]\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  MF " a[244:247], v[180:183], v[156:159], a[244:247]\n\t" \
+  MF " a[240:243], v[176:179], v[156:159], a[240:243]\n\t" \
+  MF " a[236:239], v[172:175], v[156:159], a[236:239]\n\t" \
+  "s_add_u32 s83, s83, %[gbs3]\n\t" \
+  "s_add_u32 m0, s86, 57344\n\t" \
+  MF " a[232:235], v[168:171], v[156:159], a[232:235]\n\t" \
+  "ds_read_b128 v[204:207], %[ra1] offset:6144\n\t" \
+  MF " a[228:231], v[164:167], v[156:159], a[228:231]\n\t" \
+  MF " a[224:227], v[160:163], v[156:159], a[224:227]\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  MF " a[192:195], v[160:163], v[152:155], a[192:195]\n\t" \
+  MF " a[196:199], v[164:167], v[152:155], a[196:199]\n\t" \
+  MF " a[200:203], v[168:171], v[152:155], a[200:203]\n\t" \
+  MF " a[204:207], v[172:175], v[152:155], a[204:207]\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 61440\n\t" \
+  MF " a[172:175], v[172:175], v[148:151], a[172:175]\n\t" \
+  MF " a[168:171], v[168:171], v[148:151], a[168:171]\n\t" \
+  MF " a[164:167], v[164:167], v[148:151], a[164:167]\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  MF " a[160:163], v[160:163], v[148:151], a[160:163]\n\t" \
+  MF " a[128:131], v[160:163], v[144:147], a[128:131]\n\t" \
+  MF " a[132:135], v[164:167], v[144:147], a[132:135]\n\t" \
+  MF " a[136:139], v[168:171], v[144:147], a[136:139]\n\t" \
+  MF " a[140:143], v[172:175], v[144:147], a[140:143]\n\t" \
+  "s_waitcnt vmcnt(8) lgkmcnt(0)\n\t" \
+  "s_barrier\n\t" \
+  MF " a[0:3], v[224:227], v[192:195], a[0:3]\n\t" \
+  "ds_read_b128 v[240:243], %[rb1] offset:8192\n\t" \
+  MF " a[4:7], v[228:231], v[192:195], a[4:7]\n\t" \
+  "ds_read_b128 v[244:247], %[rb1] offset:10240\n\t" \
+  MF " a[8:11], v[232:235], v[192:195], a[8:11]\n\t" \
+  "ds_read_b128 v[248:251], %[rb1] offset:12288\n\t" \
+  MF " a[12:15], v[236:239], v[192:195], a[12:15]\n\t" \
+  "ds_read_b128 v[252:255], %[rb1] offset:14336\n\t" \
+  MF " a[44:47], v[236:239], v[196:199], a[44:47]\n\t" \
+  "ds_read_b128 v[208:211], %[ra1] offset:8192\n\t" \
+  MF " a[40:43], v[232:235], v[196:199], a[40:43]\n\t" \
+  "ds_read_b128 v[212:215], %[ra1] offset:10240\n\t" \
+  MF " a[36:39], v[228:231], v[196:199], a[36:39]\n\t" \
+  "ds_read_b128 v[216:219], %[ra1] offset:12288\n\t" \
+  MF " a[32:35], v[224:227], v[196:199], a[32:35]\n\t" \
+  "ds_read_b128 v[220:223], %[ra1] offset:14336\n\t" \
+  MF " a[64:67], v[224:227], v[200:203], a[64:67]\n\t" \
+  "s_add_u32 s87, s80, 2\n\t" \
+  "s_cmp_eq_u32 s87, %[wrap]\n\t" \
+  "s_cselect_b32 s85, %[back], 128\n\t" \
+  MF " a[68:71], v[228:231], v[200:203], a[68:71]\n\t" \
+  "s_add_u32 s81, s81, s85\n\t" \
+  "s_add_u32 s82, s82, s85\n\t" \
+  MF " a[72:75], v[232:235], v[200:203], a[72:75]\n\t" \
+  "s_cmp_lt_u32 s87, %[n]\n\t" \
+  "s_cselect_b32 s84, 0, 0x80000000\n\t" \
+  "s_xor_b32 s86, s86, 0x10000\n\t" \
+  MF " a[76:79], v[236:239], v[200:203], a[76:79]\n\t" \
+  "v_or_b32 v120, s84, %[voa]\n\t" \
+  MF " a[108:111], v[236:239], v[204:207], a[108:111]\n\t" \
+  "v_or_b32 v121, s84, %[vob]\n\t" \
+  MF " a[104:107], v[232:235], v[204:207], a[104:107]\n\t" \
+  "s_mov_b32 s83, s81\n\t" \
+  "s_add_u32 m0, s86, 0\n\t" \
+  MF " a[100:103], v[228:231], v[204:207], a[100:103]\n\t" \
+  "ds_read_b128 v[128:131], %[ra0] offset:0\n\t" \
+  MF " a[96:99], v[224:227], v[204:207], a[96:99]\n\t" \
+  "v_xor_b32 %[ra1], 0x10000, %[ra1]\n\t" \
+  "s_waitcnt lgkmcnt(8)\n\t" \
+  MF " a[112:115], v[240:243], v[204:207], a[112:115]\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  "s_waitcnt lgkmcnt(7)\n\t" \
+  MF " a[116:119], v[244:247], v[204:207], a[116:119]\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  MF " a[120:123], v[248:251], v[204:207], a[120:123]\n\t" \
+  "ds_read_b128 v[160:163], %[rb0] offset:0\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  MF " a[124:127], v[252:255], v[204:207], a[124:127]\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, s86, 4096\n\t" \
+  MF " a[92:95], v[252:255], v[200:203], a[92:95]\n\t" \
+  MF " a[88:91], v[248:251], v[200:203], a[88:91]\n\t" \
+  MF " a[84:87], v[244:247], v[200:203], a[84:87]\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  MF " a[80:83], v[240:243], v[200:203], a[80:83]\n\t" \
+  "ds_read_b128 v[164:167], %[rb0] offset:2048\n\t" \
+  MF " a[48:51], v[240:243], v[196:199], a[48:51]\n\t" \
+  MF " a[52:55], v[244:247], v[196:199], a[52:55]\n\t" \
+  "s_add_u32 s83, s83, %[gas3]\n\t" \
+  "s_add_u32 m0, s86, 16384\n\t" \
+  MF " a[56:59], v[248:251], v[196:199], a[56:59]\n\t" \
+  MF " a[60:63], v[252:255], v[196:199], a[60:63]\n\t" \
+  MF " a[28:31], v[252:255], v[192:195], a[28:31]\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  MF " a[24:27], v[248:251], v[192:195], a[24:27]\n\t" \
+  "ds_read_b128 v[168:171], %[rb0] offset:4096\n\t" \
+  MF " a[20:23], v[244:247], v[192:195], a[20:23]\n\t" \
+  MF " a[16:19], v[240:243], v[192:195], a[16:19]\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, s86, 20480\n\t" \
+  "s_waitcnt lgkmcnt(7)\n\t" \
+  MF " a[144:147], v[240:243], v[208:211], a[144:147]\n\t" \
+  MF " a[148:151], v[244:247], v[208:211], a[148:151]\n\t" \
+  "ds_read_b128 v[172:175], %[rb0] offset:6144\n\t" \
+  MF " a[152:155], v[248:251], v[208:211], a[152:155]\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  MF " a[156:159], v[252:255], v[208:211], a[156:159]\n\t" \
+  "s_waitcnt lgkmcnt(7)\n\t" \
+  MF " a[188:191], v[252:255], v[212:215], a[188:191]\n\t" \
+  MF " a[184:187], v[248:251], v[212:215], a[184:187]\n\t" \
+  "s_mov_b32 s83, s82\n\t" \
+  "s_add_u32 m0, s86, 32768\n\t" \
+  MF " a[180:183], v[244:247], v[212:215], a[180:183]\n\t" \
+  "ds_read_b128 v[132:135], %[ra0] offset:2048\n\t" \
+  MF " a[176:179], v[240:243], v[212:215], a[176:179]\n\t" \
+  "s_waitcnt lgkmcnt(7)\n\t" \
+  MF " a[208:211], v[240:243], v[216:219], a[208:211]\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  MF " a[212:215], v[244:247], v[216:219], a[212:215]\n\t" \
+  MF " a[216:219], v[248:251], v[216:219], a[216:219]\n\t" \
+  "v_xor_b32 %[rb1], 0x10000, %[rb1]\n\t" \
+  MF " a[220:223], v[252:255], v[216:219], a[220:223]\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 36864\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  MF " a[252:255], v[252:255], v[220:223], a[252:255]\n\t" \
+  "ds_read_b128 v[136:139], %[ra0] offset:4096\n\t" \
+  MF " a[248:251], v[248:251], v[220:223], a[248:251]\n\t" \
+  MF " a[244:247], v[244:247], v[220:223], a[244:247]\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  MF " a[240:243], v[240:243], v[220:223], a[240:243]\n\t" \
+  MF " a[236:239], v[236:239], v[220:223], a[236:239]\n\t" \
+  "ds_read_b128 v[140:143], %[ra0] offset:6144\n\t" \
+  MF " a[232:235], v[232:235], v[220:223], a[232:235]\n\t" \
+  "s_add_u32 s83, s83, %[gbs3]\n\t" \
+  "s_add_u32 m0, s86, 49152\n\t" \
+  MF " a[228:231], v[228:231], v[220:223], a[228:231]\n\t" \
+  MF " a[224:227], v[224:227], v[220:223], a[224:227]\n\t" \
+  MF " a[192:195], v[224:227], v[216:219], a[192:195]\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  MF " a[196:199], v[228:231], v[216:219], a[196:199]\n\t" \
+  MF " a[200:203], v[232:235], v[216:219], a[200:203]\n\t" \
+  MF " a[204:207], v[236:239], v[216:219], a[204:207]\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 53248\n\t" \
+  MF " a[172:175], v[236:239], v[212:215], a[172:175]\n\t" \
+  MF " a[168:171], v[232:235], v[212:215], a[168:171]\n\t" \
+  MF " a[164:167], v[228:231], v[212:215], a[164:167]\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  MF " a[160:163], v[224:227], v[212:215], a[160:163]\n\t" \
+  MF " a[128:131], v[224:227], v[208:211], a[128:131]\n\t" \
+  MF " a[132:135], v[228:231], v[208:211], a[132:135]\n\t" \
+  MF " a[136:139], v[232:235], v[208:211], a[136:139]\n\t" \
+  MF " a[140:143], v[236:239], v[208:211], a[140:143]\n\t" \
+  "s_add_u32 s80, s80, 1\n\t" \
+  "s_waitcnt vmcnt(8) lgkmcnt(0)\n\t" \
+  "s_barrier\n\t" \
+  "s_cmp_lt_u32 s80, %[n]\n\t" \
+  "s_cbranch_scc1 L_sk_loop%=\n\t" \
+  "s_waitcnt vmcnt(0) lgkmcnt(0)\n\t" \
+  "s_nop 7\n\t" \
+  "s_nop 7\n\t" \
+  "s_nop 7\n\t" \
+  ""
+#define SK_TILE_ASM_LOOP_LOW(MF) \
+  "v_accvgpr_write_b32 a0, 0\n\t" \
+  "v_accvgpr_write_b32 a1, 0\n\t" \
+  "v_accvgpr_write_b32 a2, 0\n\t" \
+  "v_accvgpr_write_b32 a3, 0\n\t" \
+  "v_accvgpr_write_b32 a4, 0\n\t" \
+  "v_accvgpr_write_b32 a5, 0\n\t" \
+  "v_accvgpr_write_b32 a6, 0\n\t" \
+  "v_accvgpr_write_b32 a7, 0\n\t" \
+  "v_accvgpr_write_b32 a8, 0\n\t" \
+  "v_accvgpr_write_b32 a9, 0\n\t" \
+  "v_accvgpr_write_b32 a10, 0\n\t" \
+  "v_accvgpr_write_b32 a11, 0\n\t" \
+  "v_accvgpr_write_b32 a12, 0\n\t" \
+  "v_accvgpr_write_b32 a13, 0\n\t" \
+  "v_accvgpr_write_b32 a14, 0\n\t" \
+  "v_accvgpr_write_b32 a15, 0\n\t" \
+  "v_accvgpr_write_b32 a16, 0\n\t" \
+  "v_accvgpr_write_b32 a17, 0\n\t" \
+  "v_accvgpr_write_b32 a18, 0\n\t" \
+  "v_accvgpr_write_b32 a19, 0\n\t" \
+  "v_accvgpr_write_b32 a20, 0\n\t" \
+  "v_accvgpr_write_b32 a21, 0\n\t" \
+  "v_accvgpr_write_b32 a22, 0\n\t" \
+  "v_accvgpr_write_b32 a23, 0\n\t" \
+  "v_accvgpr_write_b32 a24, 0\n\t" \
+  "v_accvgpr_write_b32 a25, 0\n\t" \
+  "v_accvgpr_write_b32 a26, 0\n\t" \
+  "v_accvgpr_write_b32 a27, 0\n\t" \
+  "v_accvgpr_write_b32 a28, 0\n\t" \
+  "v_accvgpr_write_b32 a29, 0\n\t" \
+  "v_accvgpr_write_b32 a30, 0\n\t" \
+  "v_accvgpr_write_b32 a31, 0\n\t" \
+  "v_accvgpr_write_b32 a32, 0\n\t" \
+  "v_accvgpr_write_b32 a33, 0\n\t" \
+  "v_accvgpr_write_b32 a34, 0\n\t" \
+  "v_accvgpr_write_b32 a35, 0\n\t" \
+  "v_accvgpr_write_b32 a36, 0\n\t" \
+  "v_accvgpr_write_b32 a37, 0\n\t" \
+  "v_accvgpr_write_b32 a38, 0\n\t" \
+  "v_accvgpr_write_b32 a39, 0\n\t" \
+  "v_accvgpr_write_b32 a40, 0\n\t" \
+  "v_accvgpr_write_b32 a41, 0\n\t" \
+  "v_accvgpr_write_b32 a42, 0\n\t" \
+  "v_accvgpr_write_b32 a43, 0\n\t" \
+  "v_accvgpr_write_b32 a44, 0\n\t" \
+  "v_accvgpr_write_b32 a45, 0\n\t" \
+  "v_accvgpr_write_b32 a46, 0\n\t" \
+  "v_accvgpr_write_b32 a47, 0\n\t" \
+  "v_accvgpr_write_b32 a48, 0\n\t" \
+  "v_accvgpr_write_b32 a49, 0\n\t" \
+  "v_accvgpr_write_b32 a50, 0\n\t" \
+  "v_accvgpr_write_b32 a51, 0\n\t" \
+  "v_accvgpr_write_b32 a52, 0\n\t" \
+  "v_accvgpr_write_b32 a53, 0\n\t" \
+  "v_accvgpr_write_b32 a54, 0\n\t" \
+  "v_accvgpr_write_b32 a55, 0\n\t" \
+  "v_accvgpr_write_b32 a56, 0\n\t" \
+  "v_accvgpr_write_b32 a57, 0\n\t" \
+  "v_accvgpr_write_b32 a58, 0\n\t" \
+  "v_accvgpr_write_b32 a59, 0\n\t" \
+  "v_accvgpr_write_b32 a60, 0\n\t" \
+  "v_accvgpr_write_b32 a61, 0\n\t" \
+  "v_accvgpr_write_b32 a62, 0\n\t" \
+  "v_accvgpr_write_b32 a63, 0\n\t" \
+  "v_accvgpr_write_b32 a64, 0\n\t" \
+  "v_accvgpr_write_b32 a65, 0\n\t" \
+  "v_accvgpr_write_b32 a66, 0\n\t" \
+  "v_accvgpr_write_b32 a67, 0\n\t" \
+  "v_accvgpr_write_b32 a68, 0\n\t" \
+  "v_accvgpr_write_b32 a69, 0\n\t" \
+  "v_accvgpr_write_b32 a70, 0\n\t" \
+  "v_accvgpr_write_b32 a71, 0\n\t" \
+  "v_accvgpr_write_b32 a72, 0\n\t" \
+  "v_accvgpr_write_b32 a73, 0\n\t" \
+  "v_accvgpr_write_b32 a74, 0\n\t" \
+  "v_accvgpr_write_b32 a75, 0\n\t" \
+  "v_accvgpr_write_b32 a76, 0\n\t" \
+  "v_accvgpr_write_b32 a77, 0\n\t" \
+  "v_accvgpr_write_b32 a78, 0\n\t" \
+  "v_accvgpr_write_b32 a79, 0\n\t" \
+  "v_accvgpr_write_b32 a80, 0\n\t" \
+  "v_accvgpr_write_b32 a81, 0\n\t" \
+  "v_accvgpr_write_b32 a82, 0\n\t" \
+  "v_accvgpr_write_b32 a83, 0\n\t" \
+  "v_accvgpr_write_b32 a84, 0\n\t" \
+  "v_accvgpr_write_b32 a85, 0\n\t" \
+  "v_accvgpr_write_b32 a86, 0\n\t" \
+  "v_accvgpr_write_b32 a87, 0\n\t" \
+  "v_accvgpr_write_b32 a88, 0\n\t" \
+  "v_accvgpr_write_b32 a89, 0\n\t" \
+  "v_accvgpr_write_b32 a90, 0\n\t" \
+  "v_accvgpr_write_b32 a91, 0\n\t" \
+  "v_accvgpr_write_b32 a92, 0\n\t" \
+  "v_accvgpr_write_b32 a93, 0\n\t" \
+  "v_accvgpr_write_b32 a94, 0\n\t" \
+  "v_accvgpr_write_b32 a95, 0\n\t" \
+  "v_accvgpr_write_b32 a96, 0\n\t" \
+  "v_accvgpr_write_b32 a97, 0\n\t" \
+  "v_accvgpr_write_b32 a98, 0\n\t" \
+  "v_accvgpr_write_b32 a99, 0\n\t" \
+  "v_accvgpr_write_b32 a100, 0\n\t" \
+  "v_accvgpr_write_b32 a101, 0\n\t" \
+  "v_accvgpr_write_b32 a102, 0\n\t" \
+  "v_accvgpr_write_b32 a103, 0\n\t" \
+  "v_accvgpr_write_b32 a104, 0\n\t" \
+  "v_accvgpr_write_b32 a105, 0\n\t" \
+  "v_accvgpr_write_b32 a106, 0\n\t" \
+  "v_accvgpr_write_b32 a107, 0\n\t" \
+  "v_accvgpr_write_b32 a108, 0\n\t" \
+  "v_accvgpr_write_b32 a109, 0\n\t" \
+  "v_accvgpr_write_b32 a110, 0\n\t" \
+  "v_accvgpr_write_b32 a111, 0\n\t" \
+  "v_accvgpr_write_b32 a112, 0\n\t" \
+  "v_accvgpr_write_b32 a113, 0\n\t" \
+  "v_accvgpr_write_b32 a114, 0\n\t" \
+  "v_accvgpr_write_b32 a115, 0\n\t" \
+  "v_accvgpr_write_b32 a116, 0\n\t" \
+  "v_accvgpr_write_b32 a117, 0\n\t" \
+  "v_accvgpr_write_b32 a118, 0\n\t" \
+  "v_accvgpr_write_b32 a119, 0\n\t" \
+  "v_accvgpr_write_b32 a120, 0\n\t" \
+  "v_accvgpr_write_b32 a121, 0\n\t" \
+  "v_accvgpr_write_b32 a122, 0\n\t" \
+  "v_accvgpr_write_b32 a123, 0\n\t" \
+  "v_accvgpr_write_b32 a124, 0\n\t" \
+  "v_accvgpr_write_b32 a125, 0\n\t" \
+  "v_accvgpr_write_b32 a126, 0\n\t" \
+  "v_accvgpr_write_b32 a127, 0\n\t" \
+  "s_mov_b32 s80, 0\n\t" \
+  "s_xor_b32 s86, %[lds], 0x10000\n\t" \
+  "s_cmp_eq_u32 %[wrap], 1\n\t" \
+  "s_cselect_b32 s85, %[back], 128\n\t" \
+  "s_add_u32 s81, %[ga0], s85\n\t" \
+  "s_add_u32 s82, %[gb0], s85\n\t" \
+  "s_add_u32 s87, s80, 1\n\t" \
+  "s_cmp_lt_u32 s87, %[n]\n\t" \
+  "s_cselect_b32 s84, 0, 0x80000000\n\t" \
+  "v_or_b32 v120, s84, %[voa]\n\t" \
+  "v_or_b32 v121, s84, %[vob]\n\t" \
+  "s_waitcnt vmcnt(8)\n\t" \
+  "s_barrier\n\t" \
+  "ds_read_b128 v[128:131], %[ra0] offset:0\n\t" \
+  "ds_read_b128 v[160:163], %[rb0] offset:0\n\t" \
+  "ds_read_b128 v[164:167], %[rb0] offset:2048\n\t" \
+  "ds_read_b128 v[168:171], %[rb0] offset:4096\n\t" \
+  "ds_read_b128 v[172:175], %[rb0] offset:6144\n\t" \
+  "ds_read_b128 v[132:135], %[ra0] offset:2048\n\t" \
+  "ds_read_b128 v[136:139], %[ra0] offset:4096\n\t" \
+  "ds_read_b128 v[140:143], %[ra0] offset:6144\n\t" \
+  "s_nop 7\n\t" \
+  "L_sk_loop%=:\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  MF " a[0:3], v[160:163], v[128:131], a[0:3]\n\t" \
+  "ds_read_b128 v[176:179], %[rb0] offset:8192\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  MF " a[4:7], v[164:167], v[128:131], a[4:7]\n\t" \
+  "ds_read_b128 v[180:183], %[rb0] offset:10240\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  MF " a[8:11], v[168:171], v[128:131], a[8:11]\n\t" \
+  "ds_read_b128 v[184:187], %[rb0] offset:12288\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  MF " a[12:15], v[172:175], v[128:131], a[12:15]\n\t" \
+  "ds_read_b128 v[188:191], %[rb0] offset:14336\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  MF " a[44:47], v[172:175], v[132:135], a[44:47]\n\t" \
+  "s_add_u32 s83, s82, %[gbs2]\n\t" \
+  "s_add_u32 m0, s86, 40960\n\t" \
+  MF " a[40:43], v[168:171], v[132:135], a[40:43]\n\t" \
+  "ds_read_b128 v[192:195], %[ra1] offset:0\n\t" \
+  MF " a[36:39], v[164:167], v[132:135], a[36:39]\n\t" \
+  "v_xor_b32 %[ra0], 0x10000, %[ra0]\n\t" \
+  MF " a[32:35], v[160:163], v[132:135], a[32:35]\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  MF " a[64:67], v[160:163], v[136:139], a[64:67]\n\t" \
+  "ds_read_b128 v[224:227], %[rb1] offset:0\n\t" \
+  MF " a[68:71], v[164:167], v[136:139], a[68:71]\n\t" \
+  MF " a[72:75], v[168:171], v[136:139], a[72:75]\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 45056\n\t" \
+  MF " a[76:79], v[172:175], v[136:139], a[76:79]\n\t" \
+  "ds_read_b128 v[228:231], %[rb1] offset:2048\n\t" \
+  "s_waitcnt lgkmcnt(7)\n\t" \
+  MF " a[108:111], v[172:175], v[140:143], a[108:111]\n\t" \
+  MF " a[104:107], v[168:171], v[140:143], a[104:107]\n\t" \
+  "ds_read_b128 v[232:235], %[rb1] offset:4096\n\t" \
+  MF " a[100:103], v[164:167], v[140:143], a[100:103]\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  MF " a[96:99], v[160:163], v[140:143], a[96:99]\n\t" \
+  "s_waitcnt lgkmcnt(7)\n\t" \
+  MF " a[112:115], v[176:179], v[140:143], a[112:115]\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  MF " a[116:119], v[180:183], v[140:143], a[116:119]\n\t" \
+  "s_add_u32 s83, s83, %[gbs3]\n\t" \
+  "s_add_u32 m0, s86, 57344\n\t" \
+  "s_waitcnt lgkmcnt(5)\n\t" \
+  MF " a[120:123], v[184:187], v[140:143], a[120:123]\n\t" \
+  "ds_read_b128 v[236:239], %[rb1] offset:6144\n\t" \
+  "s_waitcnt lgkmcnt(5)\n\t" \
+  MF " a[124:127], v[188:191], v[140:143], a[124:127]\n\t" \
+  MF " a[92:95], v[188:191], v[136:139], a[92:95]\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  MF " a[88:91], v[184:187], v[136:139], a[88:91]\n\t" \
+  "ds_read_b128 v[196:199], %[ra1] offset:2048\n\t" \
+  MF " a[84:87], v[180:183], v[136:139], a[84:87]\n\t" \
+  "v_xor_b32 %[rb0], 0x10000, %[rb0]\n\t" \
+  MF " a[80:83], v[176:179], v[136:139], a[80:83]\n\t" \
+  "ds_read_b128 v[200:203], %[ra1] offset:4096\n\t" \
+  MF " a[48:51], v[176:179], v[132:135], a[48:51]\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 61440\n\t" \
+  MF " a[52:55], v[180:183], v[132:135], a[52:55]\n\t" \
+  MF " a[56:59], v[184:187], v[132:135], a[56:59]\n\t" \
+  "ds_read_b128 v[204:207], %[ra1] offset:6144\n\t" \
+  MF " a[60:63], v[188:191], v[132:135], a[60:63]\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  MF " a[28:31], v[188:191], v[128:131], a[28:31]\n\t" \
+  MF " a[24:27], v[184:187], v[128:131], a[24:27]\n\t" \
+  MF " a[20:23], v[180:183], v[128:131], a[20:23]\n\t" \
+  MF " a[16:19], v[176:179], v[128:131], a[16:19]\n\t" \
+  "s_waitcnt vmcnt(4) lgkmcnt(0)\n\t" \
+  "s_barrier\n\t" \
+  MF " a[0:3], v[224:227], v[192:195], a[0:3]\n\t" \
+  "ds_read_b128 v[240:243], %[rb1] offset:8192\n\t" \
+  "s_add_u32 s87, s80, 2\n\t" \
+  "s_cmp_eq_u32 s87, %[wrap]\n\t" \
+  "s_cselect_b32 s85, %[back], 128\n\t" \
+  MF " a[4:7], v[228:231], v[192:195], a[4:7]\n\t" \
+  "ds_read_b128 v[244:247], %[rb1] offset:10240\n\t" \
+  "s_add_u32 s81, s81, s85\n\t" \
+  "s_add_u32 s82, s82, s85\n\t" \
+  MF " a[8:11], v[232:235], v[192:195], a[8:11]\n\t" \
+  "ds_read_b128 v[248:251], %[rb1] offset:12288\n\t" \
+  "s_cmp_lt_u32 s87, %[n]\n\t" \
+  "s_cselect_b32 s84, 0, 0x80000000\n\t" \
+  "s_xor_b32 s86, s86, 0x10000\n\t" \
+  MF " a[12:15], v[236:239], v[192:195], a[12:15]\n\t" \
+  "ds_read_b128 v[252:255], %[rb1] offset:14336\n\t" \
+  "v_or_b32 v120, s84, %[voa]\n\t" \
+  MF " a[44:47], v[236:239], v[196:199], a[44:47]\n\t" \
+  "v_or_b32 v121, s84, %[vob]\n\t" \
+  MF " a[40:43], v[232:235], v[196:199], a[40:43]\n\t" \
+  "s_mov_b32 s83, s81\n\t" \
+  "s_add_u32 m0, s86, 0\n\t" \
+  MF " a[36:39], v[228:231], v[196:199], a[36:39]\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  MF " a[32:35], v[224:227], v[196:199], a[32:35]\n\t" \
+  "ds_read_b128 v[128:131], %[ra0] offset:0\n\t" \
+  MF " a[64:67], v[224:227], v[200:203], a[64:67]\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, s86, 4096\n\t" \
+  MF " a[68:71], v[228:231], v[200:203], a[68:71]\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  MF " a[72:75], v[232:235], v[200:203], a[72:75]\n\t" \
+  "ds_read_b128 v[160:163], %[rb0] offset:0\n\t" \
+  MF " a[76:79], v[236:239], v[200:203], a[76:79]\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, s86, 16384\n\t" \
+  MF " a[108:111], v[236:239], v[204:207], a[108:111]\n\t" \
+  "ds_read_b128 v[164:167], %[rb0] offset:2048\n\t" \
+  MF " a[104:107], v[232:235], v[204:207], a[104:107]\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  MF " a[100:103], v[228:231], v[204:207], a[100:103]\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, s86, 20480\n\t" \
+  MF " a[96:99], v[224:227], v[204:207], a[96:99]\n\t" \
+  "ds_read_b128 v[168:171], %[rb0] offset:4096\n\t" \
+  "s_waitcnt lgkmcnt(7)\n\t" \
+  MF " a[112:115], v[240:243], v[204:207], a[112:115]\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  MF " a[116:119], v[244:247], v[204:207], a[116:119]\n\t" \
+  "ds_read_b128 v[172:175], %[rb0] offset:6144\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  MF " a[120:123], v[248:251], v[204:207], a[120:123]\n\t" \
+  "s_mov_b32 s83, s82\n\t" \
+  "s_add_u32 m0, s86, 32768\n\t" \
+  "s_waitcnt lgkmcnt(5)\n\t" \
+  MF " a[124:127], v[252:255], v[204:207], a[124:127]\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  MF " a[92:95], v[252:255], v[200:203], a[92:95]\n\t" \
+  "ds_read_b128 v[132:135], %[ra0] offset:2048\n\t" \
+  MF " a[88:91], v[248:251], v[200:203], a[88:91]\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 36864\n\t" \
+  MF " a[84:87], v[244:247], v[200:203], a[84:87]\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  MF " a[80:83], v[240:243], v[200:203], a[80:83]\n\t" \
+  "ds_read_b128 v[136:139], %[ra0] offset:4096\n\t" \
+  MF " a[48:51], v[240:243], v[196:199], a[48:51]\n\t" \
+  "s_add_u32 s83, s83, %[gbs3]\n\t" \
+  "s_add_u32 m0, s86, 49152\n\t" \
+  MF " a[52:55], v[244:247], v[196:199], a[52:55]\n\t" \
+  "ds_read_b128 v[140:143], %[ra0] offset:6144\n\t" \
+  MF " a[56:59], v[248:251], v[196:199], a[56:59]\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  MF " a[60:63], v[252:255], v[196:199], a[60:63]\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 53248\n\t" \
+  MF " a[28:31], v[252:255], v[192:195], a[28:31]\n\t" \
+  "v_xor_b32 %[ra1], 0x10000, %[ra1]\n\t" \
+  MF " a[24:27], v[248:251], v[192:195], a[24:27]\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  MF " a[20:23], v[244:247], v[192:195], a[20:23]\n\t" \
+  "v_xor_b32 %[rb1], 0x10000, %[rb1]\n\t" \
+  MF " a[16:19], v[240:243], v[192:195], a[16:19]\n\t" \
   "s_add_u32 s80, s80, 1\n\t" \
   "s_waitcnt vmcnt(8) lgkmcnt(0)\n\t" \
   "s_barrier\n\t" \

@@ -538,6 +538,40 @@ def test_grouped_kn_weights_on_tiles_that_stream_k(sk, dtype, sizes, N, K, paddi
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["float16", "bfloat16", "int8"])
+@pytest.mark.parametrize("sizes", [[1, 64, 65, 0, 128, 129, 192], [256, 257, 384, 385, 320], [127], [128, 128], [700, 60], [100] * 70])
+@pytest.mark.parametrize("N,K", [(256, 128), (520, 640), (1024, 4096), (72, 256)])
+def test_grouped_tiles_of_half_the_rows(sk, kind, sizes, N, K):
+    """256 x 256 tiles of which at most 128 rows are used are another kind, also where they are cut along K."""
+    R, E = sum(sizes) + 1, len(sizes)
+    out = torch.full((R, N), 7.0, dtype=torch.float16 if kind == "int8" else TYPES[kind], device="cuda")
+    bias, kw = rand((E, N), out.dtype, 5), {}
+    if kind == "int8":
+        g = torch.Generator().manual_seed(R + N)
+        A = torch.randint(-127, 128, (R, K), generator=g, dtype=torch.int8).cuda()
+        B = torch.randint(-127, 128, (E, N, K), generator=g, dtype=torch.int8).cuda()
+        sa, sb = (torch.rand(R, generator=g) + 0.5).cuda() * 0.01, (torch.rand(E, N, generator=g) + 0.5).cuda() / (73 * math.sqrt(K))
+        kw = dict(scale_a=sa, scale_b=sb)
+        pre, magnitudes = plain(A, B, sizes)
+        pre, magnitudes = pre * sa.double()[:, None], 0
+        for e, at in groups(sizes):
+            pre[at] *= sb[e].double()
+    else:
+        A, B = rand((R, K), out.dtype, R), rand((E, N, K), out.dtype, N, 1 / math.sqrt(K))
+        pre, magnitudes = plain(A, B, sizes)
+    C = sk.streamk_grouped(A, B, offsets_of(sizes), variant=2, out_dtype=out.dtype, **kw)
+    assert_near(C, pre, K, magnitudes, pre)
+    assert not C[R - 1:].any()
+    for e, at in groups(sizes):
+        pre[at] += bias[e].double()
+    sk.streamk_grouped(A, B, offsets_of(sizes), variant=2, out=out, bias=bias, activation="silu", **kw)
+    want = activate(pre, "silu")
+    want[R - 1:] = 0
+    assert_near(out, want, K, 1.2 * magnitudes, pre)
+    assert torch.equal(C, sk.streamk_grouped(A, B, offsets_of(sizes), variant=2, out_dtype=out.dtype, **kw))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("variant", [1, 2])
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("sizes", sorted(SIZES))
