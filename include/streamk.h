@@ -399,8 +399,8 @@ int sk_q4_quantize(const void *W, int64_t N, int64_t K, int64_t ldw, int group, 
  * int8 products with scales, and their quantiser.  No counterpart in the reference.
  *
  * sk_gemm_i8_scaled: C[m][n] = activation(a[m] * b[n] * sum_k A[m][k] B[n][k] + bias[n]) for int8 A [M,K] and B [N,K], one fp32
- * scale for each row of A (token) and of B (output channel), C fp16 or bfloat16 (ldc in its elements).  The sums are exact int32;
- * each becomes fp32 (rounded beyond 24 bits), is multiplied by a[m], then by b[n], and rounded once to C's type behind bias (C's
+ * scale for each row of A (token) and of B (output channel), C fp16 or bfloat16 (ldc in its elements).  The sums are exact int32 (up to
+ * K = 131071 whatever the values); each becomes fp32 (rounded beyond 24 bits), is multiplied by a[m], then by b[n], and rounded once to C's type behind bias (C's
  * type) and activation.  The plan is made with dtype SK_I8 as for sk_gemm_i8; SK_ERR_CONFIG for plans of kernels that have no form
  * with scales (the general small-M kernels: a plan of up to 64 rows is made with reserved[0] = 9 or 12).  Every schedule and
  * fix-up gives the same bits.  Alignment as for sk_gemm_i8; C 2-byte, the scales 4-byte aligned.

@@ -59,9 +59,9 @@ registers (%[rat0] .. %[rat7]), second lane offset (v123) and step (%[kas]).  Ro
 and groups 4-7 those of K-step 1, so here EARLY and LATE split a stage by K-step: the rows of K-step 0 are free once block 0 has read
 its late fragments, those of K-step 1 once block 1 has, and every block again carries eight loads.
 
-Low tiles (NT; SK_TILE_ASM_*_LOW): at most 128 rows of A, 64 to a wave, whose blocks 0-3 they are; blocks 4-7 do not exist.  The rows
+Low tiles (SK_TILE_ASM_*_LOW, _LOW_NN): at most 128 rows of A, 64 to a wave, whose blocks 0-3 they are; blocks 4-7 do not exist.  The rows
 stand where blocks 0-3 of a full tile's waves do, so A has EARLY row groups only, and these are 32 consecutive rows of A each.  A
-block of the loop is 32 MFMAs with four loads (block 0) and eight (block 1); the loop's state rides with the reads at the top.
+block of the loop is 32 MFMAs with four loads (block 0) and eight (block 1); the loop's state rides with the reads at the top.  NN: B's row groups are split by K-step, as in the TN layout.
 
 SK_TILE_ASM_LOOP_WRAP and _LOW (NT): a segment may start anywhere in K and wrap around; iteration %[wrap] is that of the first K, and from
 the one before it the offsets move by %[back].
@@ -150,12 +150,14 @@ def early_groups(nn, low=False):
     fill whole K-rows; TN: the rows of K-step 0)"""
     if nn == "tn":
         return [x for x in range(16) if x % 8 < 4]
+    if nn and low:
+        return list(EARLY_X) + [8 + x for x in range(4)]
     return list(EARLY_X) + ([8 + x for x in range(8)] if nn else [8 + x for x in EARLY_X])
 
 
 def late_groups(nn, low=False):
     if low:
-        return [8 + x for x in LATE_X]
+        return [8 + x for x in (range(4, 8) if nn else LATE_X)]
     if nn == "tn":
         return [x for x in range(16) if x % 8 >= 4]
     return list(LATE_X) + ([] if nn else [8 + x for x in LATE_X])
@@ -210,7 +212,7 @@ def loop_text(nn, low=False, wrap=False):
     ka_step = "%[kas]" if tn else "128"
     order = mfma_order(low)
     n_early, n_late = len(early_groups(nn, low)), len(late_groups(nn, low))
-    top, last, ld_last, rd_last = (4, 31, 30, 29) if low else (TOP, 63, LD_LAST, RD_LAST)
+    top, last, ld_last, rd_last = (4, 31, 30, 30 if nn else 29) if low else (TOP, 63, LD_LAST, RD_LAST)
 
     def mf(i, j, ab, bb):
         c = (8 * i + j) * 4
@@ -268,7 +270,7 @@ def loop_text(nn, low=False, wrap=False):
     zero_accumulators(L, low)
     e(f'"s_mov_b32 s{S_IT}, 0')
     e(f'"s_xor_b32 s{S_LDS}, %[lds], 0x10000')
-    wrap = wrap or low
+    wrap = wrap or (low and not nn)
     if wrap:
         e('"s_cmp_eq_u32 %[wrap], 1')
         e(f'"s_cselect_b32 s{S_M0}, %[back], 128')
@@ -321,9 +323,12 @@ def loop_text(nn, low=False, wrap=False):
         if low:     # (32 gaps for 4 + 8 reads, eight loads, two flips and this)
             for g, (_, texts) in enumerate(state[:top]):
                 plan[g] = (plan[g][0], plan[g][1] + texts)
-            plan[top] = state[top]
-            assert len(state) == top + 1
-            after_state = top + 1
+            rest = [t for _, texts in state[top:] for t in texts]
+            if nn:
+                rest += [t for r in ["%[ra1]"] + [f"%[rbt{j}]" for j in range(4, 8)] for t in flip(r)[1]]
+            for g in range(0, len(rest), 4):
+                plan[top + g // 4] = (None, rest[g:g + 4])
+            after_state = top + -(-len(rest) // 4)
         else:
             for g, item in enumerate(state):
                 plan[top + g] = item
@@ -331,7 +336,8 @@ def loop_text(nn, low=False, wrap=False):
         plan[last] = (None, [f'"s_add_u32 s{S_IT}, s{S_IT}, 1'])
         spread(plan, load_groups(early_groups(nn, low)), after_state, ld_last)
         spread(plan, early_reads(0), after_state, rd_last)
-        spread(plan, ([flip(f"%[rat{i}]") for i in range(4, 8)] if tn else [flip("%[ra1]")]) + ([flip(f"%[rbt{j}]") for j in range(4, 8)] if nn else [flip("%[rb1]")]), after_state, last - 1)
+        if not (low and nn):
+            spread(plan, ([flip(f"%[rat{i}]") for i in range(4, 8)] if tn else [flip("%[ra1]")]) + ([flip(f"%[rbt{j}]") for j in range(4, 8)] if nn else [flip("%[rb1]")]), after_state, last - 1)
         block(1, LdsTracker(), plan,
               [f'"s_waitcnt vmcnt({n_early}) lgkmcnt(0)', '"s_barrier',           # (the late loads of iteration it + 1 have landed)
                f'"s_cmp_lt_u32 s{S_IT}, %[n]', '"s_cbranch_scc1 L_sk_loop%='])
@@ -533,9 +539,12 @@ def main():
     emit_macro("SK_TILE_ASM_LOADS_EARLY_TN", "", stage_loads_text("tn", early_groups("tn")))
     emit_macro("SK_TILE_ASM_LOADS_LOW", "", stage_loads_text(False, sorted(early_groups(False, True) + late_groups(False, True)), True))
     emit_macro("SK_TILE_ASM_LOADS_EARLY_LOW", "", stage_loads_text(False, early_groups(False, True), True))
+    emit_macro("SK_TILE_ASM_LOADS_LOW_NN", "", stage_loads_text(True, sorted(early_groups(True, True) + late_groups(True, True)), True))
+    emit_macro("SK_TILE_ASM_LOADS_EARLY_LOW_NN", "", stage_loads_text(True, early_groups(True, True), True))
     emit_macro("SK_TILE_ASM_LOOP", "(MF)", loop_text(False))
     emit_macro("SK_TILE_ASM_LOOP_WRAP", "(MF)", loop_text(False, False, True))
     emit_macro("SK_TILE_ASM_LOOP_LOW", "(MF)", loop_text(False, True))
+    emit_macro("SK_TILE_ASM_LOOP_LOW_NN", "(MF)", loop_text(True, True))
     emit_macro("SK_TILE_ASM_LOOP_NN", "(MF)", loop_text(True))
     emit_macro("SK_TILE_ASM_LOOP_TN", "(MF)", loop_text("tn"))
     emit_macro("SK_TILE_ASM_LOOP_F8", "(MF, MOD)", loop_text_f8())

@@ -83,14 +83,14 @@ __device__ __forceinline__ bool join_parts(typename P::Acc &acc, int tile, int p
   return true;
 }
 
-// A row tile of at most 128 rows -- the last of half of the groups -- is a low one ([N, K] weights): half the MFMAs, three quarters of the
+// A row tile of at most 128 rows -- the last of half of the groups -- is a low one: half the MFMAs, three quarters of the
 // loads; 8 experts of 11008 x 4096, 800 rows, 179 -> 154 us with them and the starts below, 16 of 4096 x 4096, 1900 int8 rows 76 -> 62.
 // It keeps its place among its expert's tiles, which share the weights: behind all others 64 experts of 2048 x 4096, 16384 rows, take 356 us
 // and not 347.  (Tiles drawn from a counter as CTAs become free, and not dealt out: 356.)
 template <class P, bool NN>
 __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_grouped_asm_kernel(GroupedArgs g, int ipt, Workspace ws) {
-  constexpr bool LOW = !NN;
   constexpr int ROT_EXPERT = 11;
+  constexpr auto LOW = P::LOW_TILE, FULL = NN ? P::WHOLE_TILE : P::WRAPPED_TILE;
   GroupWalk<P::BM, false> walk(g.offsets, g.E, g.R, g.tiles_n);
   const int pid = grouped_pid(g.grid);
   zero_unowned(g, pid, P::NT);
@@ -104,12 +104,13 @@ __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_grouped_asm_kernel(
   const int items = cuts.whole + (tiles - cuts.whole) * cuts.parts;
   auto find = [&](int tile, Segment &s) {
     walk.find(tile, s.t);
-    s.low = LOW && s.t.rows - s.t.pm * P::BM <= P::BM / 2;
+    s.low = s.t.rows - s.t.pm * P::BM <= P::BM / 2;
   };
   // Weights come straight from memory where few tiles share them, and all CTAs at the same K of rows whose pitch is a large power of two
   // meet in the same channels (see rotation_of).  A row tile's CTAs start one iteration apart, so that they still share its rows in the
-  // L2s, those of different experts further apart, those that share weights at the same K.
-  auto rot_of = [&](const Segment &s) { return __builtin_amdgcn_readfirstlane((int)((unsigned)(s.t.pn + ROT_EXPERT * s.t.group) % (unsigned)s.n)); };
+  // L2s, those of different experts further apart, those that share weights at the same K.  ([K, N] weights: neighbouring tiles read
+  // neighbouring pieces of the same rows.)
+  auto rot_of = [&](const Segment &s) { return NN ? 0 : __builtin_amdgcn_readfirstlane((int)((unsigned)(s.t.pn + ROT_EXPERT * s.t.group) % (unsigned)s.n)); };
   auto segment = [&](int item, Segment &s) {
     if (item >= items) return false;
     s.cut = -1;
@@ -134,23 +135,15 @@ __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_grouped_asm_kernel(
   while (have) {
     typename P::Args a = expert_args<P>(g, s.t);
     const void *epi = expert_epilogue(g, s.t);
-    if constexpr (LOW) {
-      if (s.low) P::template mac<P::LOW_TILE>(a, acc, s.t.pm, s.t.pn, s.k0, s.n, nullptr, requested, rot_of(s));
-      else P::template mac<P::WRAPPED_TILE>(a, acc, s.t.pm, s.t.pn, s.k0, s.n, nullptr, requested, rot_of(s));
-    } else {
-      P::mac(a, acc, s.t.pm, s.t.pn, s.k0, s.n, nullptr, requested);
-    }
+    if (s.low) P::template mac<LOW>(a, acc, s.t.pm, s.t.pn, s.k0, s.n, nullptr, requested, rot_of(s));
+    else P::template mac<FULL>(a, acc, s.t.pm, s.t.pn, s.k0, s.n, nullptr, requested, rot_of(s));
     requested = false;
     item += g.grid;
     have = segment(item, next);
     if (have && P::epilogue_lds_free(a, s.t.pn, epi)) {
       const typename P::Args b = expert_args<P>(g, next.t);
-      if constexpr (LOW) {
-        if (next.low) P::template prefetch_first_stage<P::LOW_TILE>(b, next.t.pm, next.t.pn, next.k0, next.n, rot_of(next));
-        else P::template prefetch_first_stage<P::WRAPPED_TILE>(b, next.t.pm, next.t.pn, next.k0, next.n, rot_of(next));
-      } else {
-        P::prefetch_first_stage(b, next.t.pm, next.t.pn, next.k0, next.n);
-      }
+      if (next.low) P::template prefetch_first_stage<LOW>(b, next.t.pm, next.t.pn, next.k0, next.n, rot_of(next));
+      else P::template prefetch_first_stage<FULL>(b, next.t.pm, next.t.pn, next.k0, next.n, rot_of(next));
       requested = true;
     }
     if (s.cut < 0 || join_parts<P>(acc, s.cut, s.part, cuts.parts, g.grid, ws, s.low)) {

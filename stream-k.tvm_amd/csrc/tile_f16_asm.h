@@ -146,14 +146,14 @@ struct TileF16Asm {
   // the 16 loads of stage `stage` (iteration k0 + stage of the segment; nothing is fetched if the segment is shorter),
   // or -- EARLY_ONLY -- just those the loop does not send itself: the row groups that hold blocks 0-3 of the wave tiles
   // (NN: and all of B); see gen_tile_asm.py
-  // LOW_TILE: at most 128 rows, 64 to a wave: 12 loads of a stage, no late row groups of A.  WRAPPED_TILE and LOW_TILE (NT): the segment
+  // LOW_TILE: at most 128 rows, 64 to a wave: 12 loads of a stage, no late row groups of A.  NT WRAPPED_TILE and LOW_TILE: the segment
   // starts `rot` iterations into its K and wraps around, iteration `wrap` being the first K's.
   enum Kind { WHOLE_TILE, WRAPPED_TILE, LOW_TILE };
   template <bool EARLY_ONLY = false, Kind KIND = WHOLE_TILE>
   static __device__ __forceinline__ void stage_loads(const Ctx &c, int stage, int n, int wrap = -1) {
     const uint32_t oob = stage < n ? 0u : OOB_OFFSET;
     const uint32_t voa = c.voff_a | oob, vob = c.voff_b | oob, vob1 = c.voff_b1 | oob;
-    constexpr bool LOW = KIND == LOW_TILE, WRAPS = KIND != WHOLE_TILE;
+    constexpr bool LOW = KIND == LOW_TILE, WRAPS = KIND != WHOLE_TILE && !NN_;
     const uint32_t step = (uint32_t)stage * 128 - (WRAPS && stage == wrap ? (uint32_t)n * 128 : 0u);
     const uint32_t ga = c.goff_a + step, gb = c.goff_b + (WRAPS ? step : (uint32_t)stage * c.kstep_b);
     const uint32_t lds_stage = c.lds_wave + (uint32_t)stage * STAGE_BYTES;
@@ -162,8 +162,12 @@ struct TileF16Asm {
       [gb] "s"(gb), [gas] "s"(c.gstep_a), [gas2] "s"(2 * c.gstep_a), [gas3] "s"(3 * c.gstep_a), [gbs] "s"(c.gstep_b),     \
       [gbs2] "s"(2 * c.gstep_b), [gbs3] "s"(3 * c.gstep_b), [lds] "s"(lds_stage)                                          \
   : "memory", "m0", "scc", "s83"
-    static_assert(!WRAPS || (!NN_ && F8 == 0), "see gen_tile_asm.py");
-    if constexpr (LOW && EARLY_ONLY) {
+    static_assert(KIND == WHOLE_TILE || (F8 == 0 && (KIND == LOW_TILE || !NN_)), "see gen_tile_asm.py");
+    if constexpr (NN_ && LOW && EARLY_ONLY) {
+      asm volatile(SK_TILE_ASM_LOADS_EARLY_LOW_NN SK_ASM_LOAD_OPERANDS);
+    } else if constexpr (NN_ && LOW) {
+      asm volatile(SK_TILE_ASM_LOADS_LOW_NN SK_ASM_LOAD_OPERANDS);
+    } else if constexpr (LOW && EARLY_ONLY) {
       asm volatile(SK_TILE_ASM_LOADS_EARLY_LOW SK_ASM_LOAD_OPERANDS);
     } else if constexpr (LOW) {
       asm volatile(SK_TILE_ASM_LOADS_LOW SK_ASM_LOAD_OPERANDS);
@@ -205,9 +209,14 @@ struct TileF16Asm {
     [rbt3] "+v"(c.rbt[3]), [rbt4] "+v"(c.rbt[4]), [rbt5] "+v"(c.rbt[5]), [rbt6] "+v"(c.rbt[6]), [rbt7] "+v"(c.rbt[7])  \
   : [rsa] "s"(c.rsrc_a), [rsb] "s"(c.rsrc_b), [voa] "v"(c.voff_a), [vob] "v"(c.voff_b), [vob1] "v"(c.voff_b1),          \
     [ga0] "s"(c.goff_a), [gb0] "s"(c.goff_b), [gas] "s"(c.gstep_a), [gas2] "s"(2 * c.gstep_a),                          \
-    [gas3] "s"(3 * c.gstep_a), [gbs] "s"(c.gstep_b), [kbs] "s"(c.kstep_b), [n] "s"(iters), [lds] "s"(c.lds_wave)        \
+    [gas3] "s"(3 * c.gstep_a), [gbs] "s"(c.gstep_b), [gbs4] "s"(4 * c.gstep_b), [kbs] "s"(c.kstep_b), [n] "s"(iters),   \
+    [lds] "s"(c.lds_wave)                                                                                             \
   : "memory", "m0", "scc", SK_TILE_ASM_CLOBBERS
-      if constexpr (BF16_) {
+      if constexpr (KIND == LOW_TILE && BF16_) {
+        asm volatile(SK_TILE_ASM_LOOP_LOW_NN("v_mfma_f32_16x16x32_bf16") SK_ASM_NN_OPERANDS);
+      } else if constexpr (KIND == LOW_TILE) {
+        asm volatile(SK_TILE_ASM_LOOP_LOW_NN("v_mfma_f32_16x16x32_f16") SK_ASM_NN_OPERANDS);
+      } else if constexpr (BF16_) {
         asm volatile(SK_TILE_ASM_LOOP_NN("v_mfma_f32_16x16x32_bf16") SK_ASM_NN_OPERANDS);
       } else {
         asm volatile(SK_TILE_ASM_LOOP_NN("v_mfma_f32_16x16x32_f16") SK_ASM_NN_OPERANDS);

@@ -403,6 +403,90 @@
   "s_nop 0\n\t" \
   "buffer_load_dwordx4 %[vob], %[rsb], s83 offen lds\n\t" \
   ""
+#define SK_TILE_ASM_LOADS_LOW_NN \
+  "s_mov_b32 s83, %[ga]\n\t" \
+  "s_add_u32 m0, %[lds], 0\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[voa], %[rsa], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, %[lds], 4096\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[voa], %[rsa], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, %[lds], 16384\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[voa], %[rsa], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, %[lds], 20480\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[voa], %[rsa], s83 offen lds\n\t" \
+  "s_mov_b32 s83, %[gb]\n\t" \
+  "s_add_u32 m0, %[lds], 32768\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob], %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, %[lds], 36864\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob1], %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, %[lds], 40960\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob], %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, %[lds], 45056\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob1], %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, %[lds], 49152\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob], %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, %[lds], 53248\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob1], %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, %[lds], 57344\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob], %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, %[lds], 61440\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob1], %[rsb], s83 offen lds\n\t" \
+  ""
+#define SK_TILE_ASM_LOADS_EARLY_LOW_NN \
+  "s_mov_b32 s83, %[ga]\n\t" \
+  "s_add_u32 m0, %[lds], 0\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[voa], %[rsa], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, %[lds], 4096\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[voa], %[rsa], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, %[lds], 16384\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[voa], %[rsa], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, %[lds], 20480\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[voa], %[rsa], s83 offen lds\n\t" \
+  "s_mov_b32 s83, %[gb]\n\t" \
+  "s_add_u32 m0, %[lds], 32768\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob], %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, %[lds], 36864\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob1], %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, %[lds], 40960\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob], %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, %[lds], 45056\n\t" \
+  "s_nop 0\n\t" \
+  "buffer_load_dwordx4 %[vob1], %[rsb], s83 offen lds\n\t" \
+  ""
 #define SK_TILE_ASM_LOOP(MF) \
   "v_accvgpr_write_b32 a0, 0\n\t" \
   "v_accvgpr_write_b32 a1, 0\n\t" \
@@ -1779,6 +1863,347 @@
   "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
   MF " a[20:23], v[244:247], v[192:195], a[20:23]\n\t" \
   "v_xor_b32 %[rb1], 0x10000, %[rb1]\n\t" \
+  MF " a[16:19], v[240:243], v[192:195], a[16:19]\n\t" \
+  "s_add_u32 s80, s80, 1\n\t" \
+  "s_waitcnt vmcnt(8) lgkmcnt(0)\n\t" \
+  "s_barrier\n\t" \
+  "s_cmp_lt_u32 s80, %[n]\n\t" \
+  "s_cbranch_scc1 L_sk_loop%=\n\t" \
+  "s_waitcnt vmcnt(0) lgkmcnt(0)\n\t" \
+  "s_nop 7\n\t" \
+  "s_nop 7\n\t" \
+  "s_nop 7\n\t" \
+  ""
+#define SK_TILE_ASM_LOOP_LOW_NN(MF) \
+  "v_accvgpr_write_b32 a0, 0\n\t" \
+  "v_accvgpr_write_b32 a1, 0\n\t" \
+  "v_accvgpr_write_b32 a2, 0\n\t" \
+  "v_accvgpr_write_b32 a3, 0\n\t" \
+  "v_accvgpr_write_b32 a4, 0\n\t" \
+  "v_accvgpr_write_b32 a5, 0\n\t" \
+  "v_accvgpr_write_b32 a6, 0\n\t" \
+  "v_accvgpr_write_b32 a7, 0\n\t" \
+  "v_accvgpr_write_b32 a8, 0\n\t" \
+  "v_accvgpr_write_b32 a9, 0\n\t" \
+  "v_accvgpr_write_b32 a10, 0\n\t" \
+  "v_accvgpr_write_b32 a11, 0\n\t" \
+  "v_accvgpr_write_b32 a12, 0\n\t" \
+  "v_accvgpr_write_b32 a13, 0\n\t" \
+  "v_accvgpr_write_b32 a14, 0\n\t" \
+  "v_accvgpr_write_b32 a15, 0\n\t" \
+  "v_accvgpr_write_b32 a16, 0\n\t" \
+  "v_accvgpr_write_b32 a17, 0\n\t" \
+  "v_accvgpr_write_b32 a18, 0\n\t" \
+  "v_accvgpr_write_b32 a19, 0\n\t" \
+  "v_accvgpr_write_b32 a20, 0\n\t" \
+  "v_accvgpr_write_b32 a21, 0\n\t" \
+  "v_accvgpr_write_b32 a22, 0\n\t" \
+  "v_accvgpr_write_b32 a23, 0\n\t" \
+  "v_accvgpr_write_b32 a24, 0\n\t" \
+  "v_accvgpr_write_b32 a25, 0\n\t" \
+  "v_accvgpr_write_b32 a26, 0\n\t" \
+  "v_accvgpr_write_b32 a27, 0\n\t" \
+  "v_accvgpr_write_b32 a28, 0\n\t" \
+  "v_accvgpr_write_b32 a29, 0\n\t" \
+  "v_accvgpr_write_b32 a30, 0\n\t" \
+  "v_accvgpr_write_b32 a31, 0\n\t" \
+  "v_accvgpr_write_b32 a32, 0\n\t" \
+  "v_accvgpr_write_b32 a33, 0\n\t" \
+  "v_accvgpr_write_b32 a34, 0\n\t" \
+  "v_accvgpr_write_b32 a35, 0\n\t" \
+  "v_accvgpr_write_b32 a36, 0\n\t" \
+  "v_accvgpr_write_b32 a37, 0\n\t" \
+  "v_accvgpr_write_b32 a38, 0\n\t" \
+  "v_accvgpr_write_b32 a39, 0\n\t" \
+  "v_accvgpr_write_b32 a40, 0\n\t" \
+  "v_accvgpr_write_b32 a41, 0\n\t" \
+  "v_accvgpr_write_b32 a42, 0\n\t" \
+  "v_accvgpr_write_b32 a43, 0\n\t" \
+  "v_accvgpr_write_b32 a44, 0\n\t" \
+  "v_accvgpr_write_b32 a45, 0\n\t" \
+  "v_accvgpr_write_b32 a46, 0\n\t" \
+  "v_accvgpr_write_b32 a47, 0\n\t" \
+  "v_accvgpr_write_b32 a48, 0\n\t" \
+  "v_accvgpr_write_b32 a49, 0\n\t" \
+  "v_accvgpr_write_b32 a50, 0\n\t" \
+  "v_accvgpr_write_b32 a51, 0\n\t" \
+  "v_accvgpr_write_b32 a52, 0\n\t" \
+  "v_accvgpr_write_b32 a53, 0\n\t" \
+  "v_accvgpr_write_b32 a54, 0\n\t" \
+  "v_accvgpr_write_b32 a55, 0\n\t" \
+  "v_accvgpr_write_b32 a56, 0\n\t" \
+  "v_accvgpr_write_b32 a57, 0\n\t" \
+  "v_accvgpr_write_b32 a58, 0\n\t" \
+  "v_accvgpr_write_b32 a59, 0\n\t" \
+  "v_accvgpr_write_b32 a60, 0\n\t" \
+  "v_accvgpr_write_b32 a61, 0\n\t" \
+  "v_accvgpr_write_b32 a62, 0\n\t" \
+  "v_accvgpr_write_b32 a63, 0\n\t" \
+  "v_accvgpr_write_b32 a64, 0\n\t" \
+  "v_accvgpr_write_b32 a65, 0\n\t" \
+  "v_accvgpr_write_b32 a66, 0\n\t" \
+  "v_accvgpr_write_b32 a67, 0\n\t" \
+  "v_accvgpr_write_b32 a68, 0\n\t" \
+  "v_accvgpr_write_b32 a69, 0\n\t" \
+  "v_accvgpr_write_b32 a70, 0\n\t" \
+  "v_accvgpr_write_b32 a71, 0\n\t" \
+  "v_accvgpr_write_b32 a72, 0\n\t" \
+  "v_accvgpr_write_b32 a73, 0\n\t" \
+  "v_accvgpr_write_b32 a74, 0\n\t" \
+  "v_accvgpr_write_b32 a75, 0\n\t" \
+  "v_accvgpr_write_b32 a76, 0\n\t" \
+  "v_accvgpr_write_b32 a77, 0\n\t" \
+  "v_accvgpr_write_b32 a78, 0\n\t" \
+  "v_accvgpr_write_b32 a79, 0\n\t" \
+  "v_accvgpr_write_b32 a80, 0\n\t" \
+  "v_accvgpr_write_b32 a81, 0\n\t" \
+  "v_accvgpr_write_b32 a82, 0\n\t" \
+  "v_accvgpr_write_b32 a83, 0\n\t" \
+  "v_accvgpr_write_b32 a84, 0\n\t" \
+  "v_accvgpr_write_b32 a85, 0\n\t" \
+  "v_accvgpr_write_b32 a86, 0\n\t" \
+  "v_accvgpr_write_b32 a87, 0\n\t" \
+  "v_accvgpr_write_b32 a88, 0\n\t" \
+  "v_accvgpr_write_b32 a89, 0\n\t" \
+  "v_accvgpr_write_b32 a90, 0\n\t" \
+  "v_accvgpr_write_b32 a91, 0\n\t" \
+  "v_accvgpr_write_b32 a92, 0\n\t" \
+  "v_accvgpr_write_b32 a93, 0\n\t" \
+  "v_accvgpr_write_b32 a94, 0\n\t" \
+  "v_accvgpr_write_b32 a95, 0\n\t" \
+  "v_accvgpr_write_b32 a96, 0\n\t" \
+  "v_accvgpr_write_b32 a97, 0\n\t" \
+  "v_accvgpr_write_b32 a98, 0\n\t" \
+  "v_accvgpr_write_b32 a99, 0\n\t" \
+  "v_accvgpr_write_b32 a100, 0\n\t" \
+  "v_accvgpr_write_b32 a101, 0\n\t" \
+  "v_accvgpr_write_b32 a102, 0\n\t" \
+  "v_accvgpr_write_b32 a103, 0\n\t" \
+  "v_accvgpr_write_b32 a104, 0\n\t" \
+  "v_accvgpr_write_b32 a105, 0\n\t" \
+  "v_accvgpr_write_b32 a106, 0\n\t" \
+  "v_accvgpr_write_b32 a107, 0\n\t" \
+  "v_accvgpr_write_b32 a108, 0\n\t" \
+  "v_accvgpr_write_b32 a109, 0\n\t" \
+  "v_accvgpr_write_b32 a110, 0\n\t" \
+  "v_accvgpr_write_b32 a111, 0\n\t" \
+  "v_accvgpr_write_b32 a112, 0\n\t" \
+  "v_accvgpr_write_b32 a113, 0\n\t" \
+  "v_accvgpr_write_b32 a114, 0\n\t" \
+  "v_accvgpr_write_b32 a115, 0\n\t" \
+  "v_accvgpr_write_b32 a116, 0\n\t" \
+  "v_accvgpr_write_b32 a117, 0\n\t" \
+  "v_accvgpr_write_b32 a118, 0\n\t" \
+  "v_accvgpr_write_b32 a119, 0\n\t" \
+  "v_accvgpr_write_b32 a120, 0\n\t" \
+  "v_accvgpr_write_b32 a121, 0\n\t" \
+  "v_accvgpr_write_b32 a122, 0\n\t" \
+  "v_accvgpr_write_b32 a123, 0\n\t" \
+  "v_accvgpr_write_b32 a124, 0\n\t" \
+  "v_accvgpr_write_b32 a125, 0\n\t" \
+  "v_accvgpr_write_b32 a126, 0\n\t" \
+  "v_accvgpr_write_b32 a127, 0\n\t" \
+  "s_mov_b32 s80, 0\n\t" \
+  "s_xor_b32 s86, %[lds], 0x10000\n\t" \
+  "s_add_u32 s81, %[ga0], 128\n\t" \
+  "s_add_u32 s82, %[gb0], %[kbs]\n\t" \
+  "s_add_u32 s87, s80, 1\n\t" \
+  "s_cmp_lt_u32 s87, %[n]\n\t" \
+  "s_cselect_b32 s84, 0, 0x80000000\n\t" \
+  "v_or_b32 v120, s84, %[voa]\n\t" \
+  "v_or_b32 v121, s84, %[vob]\n\t" \
+  "v_or_b32 v122, s84, %[vob1]\n\t" \
+  "s_waitcnt vmcnt(8)\n\t" \
+  "s_barrier\n\t" \
+  "ds_read_b128 v[128:131], %[ra0] offset:0\n\t" \
+  "ds_read_b64_tr_b16 v[160:161], %[rbt0] offset:0\n\t" \
+  "ds_read_b64_tr_b16 v[162:163], %[rbt0] offset:2048\n\t" \
+  "ds_read_b64_tr_b16 v[164:165], %[rbt1] offset:0\n\t" \
+  "ds_read_b64_tr_b16 v[166:167], %[rbt1] offset:2048\n\t" \
+  "ds_read_b64_tr_b16 v[168:169], %[rbt2] offset:0\n\t" \
+  "ds_read_b64_tr_b16 v[170:171], %[rbt2] offset:2048\n\t" \
+  "ds_read_b64_tr_b16 v[172:173], %[rbt3] offset:0\n\t" \
+  "ds_read_b64_tr_b16 v[174:175], %[rbt3] offset:2048\n\t" \
+  "ds_read_b128 v[132:135], %[ra0] offset:2048\n\t" \
+  "ds_read_b128 v[136:139], %[ra0] offset:4096\n\t" \
+  "ds_read_b128 v[140:143], %[ra0] offset:6144\n\t" \
+  "s_nop 7\n\t" \
+  "L_sk_loop%=:\n\t" \
+  "s_waitcnt lgkmcnt(9)\n\t" \
+  MF " a[0:3], v[160:163], v[128:131], a[0:3]\n\t" \
+  "ds_read_b64_tr_b16 v[176:177], %[rbt4] offset:0\n\t" \
+  "ds_read_b64_tr_b16 v[178:179], %[rbt4] offset:2048\n\t" \
+  "s_waitcnt lgkmcnt(9)\n\t" \
+  MF " a[4:7], v[164:167], v[128:131], a[4:7]\n\t" \
+  "ds_read_b64_tr_b16 v[180:181], %[rbt5] offset:0\n\t" \
+  "ds_read_b64_tr_b16 v[182:183], %[rbt5] offset:2048\n\t" \
+  "s_waitcnt lgkmcnt(9)\n\t" \
+  MF " a[8:11], v[168:171], v[128:131], a[8:11]\n\t" \
+  "ds_read_b64_tr_b16 v[184:185], %[rbt6] offset:0\n\t" \
+  "ds_read_b64_tr_b16 v[186:187], %[rbt6] offset:2048\n\t" \
+  "s_waitcnt lgkmcnt(9)\n\t" \
+  MF " a[12:15], v[172:175], v[128:131], a[12:15]\n\t" \
+  "ds_read_b64_tr_b16 v[188:189], %[rbt7] offset:0\n\t" \
+  "ds_read_b64_tr_b16 v[190:191], %[rbt7] offset:2048\n\t" \
+  "s_waitcnt lgkmcnt(10)\n\t" \
+  MF " a[44:47], v[172:175], v[132:135], a[44:47]\n\t" \
+  "s_add_u32 s83, s82, %[gbs4]\n\t" \
+  "s_add_u32 m0, s86, 49152\n\t" \
+  MF " a[40:43], v[168:171], v[132:135], a[40:43]\n\t" \
+  "ds_read_b128 v[192:195], %[ra1] offset:0\n\t" \
+  MF " a[36:39], v[164:167], v[132:135], a[36:39]\n\t" \
+  "v_xor_b32 %[ra0], 0x10000, %[ra0]\n\t" \
+  MF " a[32:35], v[160:163], v[132:135], a[32:35]\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  "s_waitcnt lgkmcnt(10)\n\t" \
+  MF " a[64:67], v[160:163], v[136:139], a[64:67]\n\t" \
+  "ds_read_b64_tr_b16 v[224:225], %[rbt0] offset:16384\n\t" \
+  "ds_read_b64_tr_b16 v[226:227], %[rbt0] offset:18432\n\t" \
+  MF " a[68:71], v[164:167], v[136:139], a[68:71]\n\t" \
+  MF " a[72:75], v[168:171], v[136:139], a[72:75]\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 53248\n\t" \
+  MF " a[76:79], v[172:175], v[136:139], a[76:79]\n\t" \
+  "ds_read_b64_tr_b16 v[228:229], %[rbt1] offset:16384\n\t" \
+  "ds_read_b64_tr_b16 v[230:231], %[rbt1] offset:18432\n\t" \
+  "s_waitcnt lgkmcnt(13)\n\t" \
+  MF " a[108:111], v[172:175], v[140:143], a[108:111]\n\t" \
+  MF " a[104:107], v[168:171], v[140:143], a[104:107]\n\t" \
+  MF " a[100:103], v[164:167], v[140:143], a[100:103]\n\t" \
+  "buffer_load_dwordx4 v122, %[rsb], s83 offen lds\n\t" \
+  MF " a[96:99], v[160:163], v[140:143], a[96:99]\n\t" \
+  "ds_read_b64_tr_b16 v[232:233], %[rbt2] offset:16384\n\t" \
+  "ds_read_b64_tr_b16 v[234:235], %[rbt2] offset:18432\n\t" \
+  "s_waitcnt lgkmcnt(13)\n\t" \
+  MF " a[112:115], v[176:179], v[140:143], a[112:115]\n\t" \
+  "s_waitcnt lgkmcnt(11)\n\t" \
+  MF " a[116:119], v[180:183], v[140:143], a[116:119]\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 57344\n\t" \
+  "s_waitcnt lgkmcnt(9)\n\t" \
+  MF " a[120:123], v[184:187], v[140:143], a[120:123]\n\t" \
+  "ds_read_b64_tr_b16 v[236:237], %[rbt3] offset:16384\n\t" \
+  "ds_read_b64_tr_b16 v[238:239], %[rbt3] offset:18432\n\t" \
+  "s_waitcnt lgkmcnt(9)\n\t" \
+  MF " a[124:127], v[188:191], v[140:143], a[124:127]\n\t" \
+  MF " a[92:95], v[188:191], v[136:139], a[92:95]\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  MF " a[88:91], v[184:187], v[136:139], a[88:91]\n\t" \
+  "ds_read_b128 v[196:199], %[ra1] offset:2048\n\t" \
+  MF " a[84:87], v[180:183], v[136:139], a[84:87]\n\t" \
+  MF " a[80:83], v[176:179], v[136:139], a[80:83]\n\t" \
+  MF " a[48:51], v[176:179], v[132:135], a[48:51]\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 61440\n\t" \
+  MF " a[52:55], v[180:183], v[132:135], a[52:55]\n\t" \
+  "ds_read_b128 v[200:203], %[ra1] offset:4096\n\t" \
+  MF " a[56:59], v[184:187], v[132:135], a[56:59]\n\t" \
+  MF " a[60:63], v[188:191], v[132:135], a[60:63]\n\t" \
+  "buffer_load_dwordx4 v122, %[rsb], s83 offen lds\n\t" \
+  MF " a[28:31], v[188:191], v[128:131], a[28:31]\n\t" \
+  "ds_read_b128 v[204:207], %[ra1] offset:6144\n\t" \
+  MF " a[24:27], v[184:187], v[128:131], a[24:27]\n\t" \
+  MF " a[20:23], v[180:183], v[128:131], a[20:23]\n\t" \
+  MF " a[16:19], v[176:179], v[128:131], a[16:19]\n\t" \
+  "s_waitcnt vmcnt(4) lgkmcnt(0)\n\t" \
+  "s_barrier\n\t" \
+  MF " a[0:3], v[224:227], v[192:195], a[0:3]\n\t" \
+  "ds_read_b64_tr_b16 v[240:241], %[rbt4] offset:16384\n\t" \
+  "ds_read_b64_tr_b16 v[242:243], %[rbt4] offset:18432\n\t" \
+  "s_add_u32 s81, s81, 128\n\t" \
+  "s_add_u32 s82, s82, %[kbs]\n\t" \
+  MF " a[4:7], v[228:231], v[192:195], a[4:7]\n\t" \
+  "ds_read_b64_tr_b16 v[244:245], %[rbt5] offset:16384\n\t" \
+  "ds_read_b64_tr_b16 v[246:247], %[rbt5] offset:18432\n\t" \
+  "s_xor_b32 s86, s86, 0x10000\n\t" \
+  "s_add_u32 s87, s80, 2\n\t" \
+  MF " a[8:11], v[232:235], v[192:195], a[8:11]\n\t" \
+  "ds_read_b64_tr_b16 v[248:249], %[rbt6] offset:16384\n\t" \
+  "ds_read_b64_tr_b16 v[250:251], %[rbt6] offset:18432\n\t" \
+  "s_cmp_lt_u32 s87, %[n]\n\t" \
+  "s_cselect_b32 s84, 0, 0x80000000\n\t" \
+  MF " a[12:15], v[236:239], v[192:195], a[12:15]\n\t" \
+  "ds_read_b64_tr_b16 v[252:253], %[rbt7] offset:16384\n\t" \
+  "ds_read_b64_tr_b16 v[254:255], %[rbt7] offset:18432\n\t" \
+  "v_or_b32 v120, s84, %[voa]\n\t" \
+  MF " a[44:47], v[236:239], v[196:199], a[44:47]\n\t" \
+  "v_or_b32 v121, s84, %[vob]\n\t" \
+  "v_or_b32 v122, s84, %[vob1]\n\t" \
+  "v_xor_b32 %[rbt0], 0x10000, %[rbt0]\n\t" \
+  "v_xor_b32 %[rbt1], 0x10000, %[rbt1]\n\t" \
+  MF " a[40:43], v[232:235], v[196:199], a[40:43]\n\t" \
+  "v_xor_b32 %[rbt2], 0x10000, %[rbt2]\n\t" \
+  "v_xor_b32 %[rbt3], 0x10000, %[rbt3]\n\t" \
+  "v_xor_b32 %[ra1], 0x10000, %[ra1]\n\t" \
+  "v_xor_b32 %[rbt4], 0x10000, %[rbt4]\n\t" \
+  MF " a[36:39], v[228:231], v[196:199], a[36:39]\n\t" \
+  "v_xor_b32 %[rbt5], 0x10000, %[rbt5]\n\t" \
+  "v_xor_b32 %[rbt6], 0x10000, %[rbt6]\n\t" \
+  "v_xor_b32 %[rbt7], 0x10000, %[rbt7]\n\t" \
+  MF " a[32:35], v[224:227], v[196:199], a[32:35]\n\t" \
+  "s_mov_b32 s83, s81\n\t" \
+  "s_add_u32 m0, s86, 0\n\t" \
+  MF " a[64:67], v[224:227], v[200:203], a[64:67]\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  MF " a[68:71], v[228:231], v[200:203], a[68:71]\n\t" \
+  "ds_read_b128 v[128:131], %[ra0] offset:0\n\t" \
+  MF " a[72:75], v[232:235], v[200:203], a[72:75]\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, s86, 4096\n\t" \
+  MF " a[76:79], v[236:239], v[200:203], a[76:79]\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  MF " a[108:111], v[236:239], v[204:207], a[108:111]\n\t" \
+  "ds_read_b64_tr_b16 v[160:161], %[rbt0] offset:0\n\t" \
+  "ds_read_b64_tr_b16 v[162:163], %[rbt0] offset:2048\n\t" \
+  MF " a[104:107], v[232:235], v[204:207], a[104:107]\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, s86, 16384\n\t" \
+  MF " a[100:103], v[228:231], v[204:207], a[100:103]\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  MF " a[96:99], v[224:227], v[204:207], a[96:99]\n\t" \
+  "ds_read_b64_tr_b16 v[164:165], %[rbt1] offset:0\n\t" \
+  "ds_read_b64_tr_b16 v[166:167], %[rbt1] offset:2048\n\t" \
+  "s_waitcnt lgkmcnt(11)\n\t" \
+  MF " a[112:115], v[240:243], v[204:207], a[112:115]\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, s86, 20480\n\t" \
+  "s_waitcnt lgkmcnt(9)\n\t" \
+  MF " a[116:119], v[244:247], v[204:207], a[116:119]\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  "s_waitcnt lgkmcnt(7)\n\t" \
+  MF " a[120:123], v[248:251], v[204:207], a[120:123]\n\t" \
+  "ds_read_b64_tr_b16 v[168:169], %[rbt2] offset:0\n\t" \
+  "ds_read_b64_tr_b16 v[170:171], %[rbt2] offset:2048\n\t" \
+  "s_waitcnt lgkmcnt(7)\n\t" \
+  MF " a[124:127], v[252:255], v[204:207], a[124:127]\n\t" \
+  "s_mov_b32 s83, s82\n\t" \
+  "s_add_u32 m0, s86, 32768\n\t" \
+  MF " a[92:95], v[252:255], v[200:203], a[92:95]\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  MF " a[88:91], v[248:251], v[200:203], a[88:91]\n\t" \
+  "ds_read_b64_tr_b16 v[172:173], %[rbt3] offset:0\n\t" \
+  "ds_read_b64_tr_b16 v[174:175], %[rbt3] offset:2048\n\t" \
+  MF " a[84:87], v[244:247], v[200:203], a[84:87]\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 36864\n\t" \
+  MF " a[80:83], v[240:243], v[200:203], a[80:83]\n\t" \
+  "buffer_load_dwordx4 v122, %[rsb], s83 offen lds\n\t" \
+  MF " a[48:51], v[240:243], v[196:199], a[48:51]\n\t" \
+  "ds_read_b128 v[132:135], %[ra0] offset:2048\n\t" \
+  MF " a[52:55], v[244:247], v[196:199], a[52:55]\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 40960\n\t" \
+  MF " a[56:59], v[248:251], v[196:199], a[56:59]\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  MF " a[60:63], v[252:255], v[196:199], a[60:63]\n\t" \
+  "ds_read_b128 v[136:139], %[ra0] offset:4096\n\t" \
+  MF " a[28:31], v[252:255], v[192:195], a[28:31]\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 45056\n\t" \
+  MF " a[24:27], v[248:251], v[192:195], a[24:27]\n\t" \
+  "buffer_load_dwordx4 v122, %[rsb], s83 offen lds\n\t" \
+  MF " a[20:23], v[244:247], v[192:195], a[20:23]\n\t" \
+  "ds_read_b128 v[140:143], %[ra0] offset:6144\n\t" \
   MF " a[16:19], v[240:243], v[192:195], a[16:19]\n\t" \
   "s_add_u32 s80, s80, 1\n\t" \
   "s_waitcnt vmcnt(8) lgkmcnt(0)\n\t" \

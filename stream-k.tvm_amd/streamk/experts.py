@@ -53,6 +53,12 @@ def _pitch(t):
 
 
 # ---- the grouped product ----
+def _rows(t):
+    """t as the kernels can read it; a row that stands for many (a broadcast gradient) is written out."""
+    t = ops._aligned_rows(t)
+    return t.contiguous() if t.shape[0] > 1 and t.stride(0) < t.shape[1] else t
+
+
 def _grouped(A, B, offsets, layout="nt", out_dtype=None, scale_a=None, scale_b=None, bias=None, activation="none", variant=0, out=None):
     if layout not in ("nt", "nn"):
         raise ValueError("layout must be 'nt' (B is [E, N, K]) or 'nn' (B is [E, K, N])")
@@ -96,7 +102,7 @@ def _grouped(A, B, offsets, layout="nt", out_dtype=None, scale_a=None, scale_b=N
     C = torch.empty((R, N), dtype=out_dtype, device=A.device) if out is None else out
     if R == 0:
         return C
-    A = ops._aligned_rows(A)
+    A = _rows(A)
     ldb = B.stride(1) if B.shape[1] > 1 else (B.shape[2] + 15) // 16 * 16
     g = _lib.SkGrouped(dtype=_lib.SK_I8 if int8 else _TYPES[A.dtype], layout=ops._plan_mod._LAYOUTS[layout], out_dtype=_TYPES[out_dtype],
                        activation=_lib.ACTIVATIONS[activation], E=E, R=R, N=N, K=K, A=A.data_ptr(), B=B.data_ptr(),
@@ -129,7 +135,7 @@ def _padded(t):
     """t with its columns filled up with zeros to a multiple of 8, its rows as the kernels read them."""
     if t.shape[1] % 8:
         return torch.nn.functional.pad(t, (0, 8 - t.shape[1] % 8))
-    return ops._aligned_rows(t)
+    return _rows(t)
 
 
 def _wgrad(A, B, offsets, variant=0):
@@ -147,7 +153,7 @@ def _wgrad(A, B, offsets, variant=0):
     C = torch.empty((E, M, N), dtype=A.dtype, device=A.device)
     if A.shape[0] == 0 or C.numel() == 0:
         return C.zero_()
-    A, B = _padded(A), ops._aligned_rows(B)
+    A, B = _padded(A), _rows(B)
     rc = _lib.lib().sk_grouped_wgrad(A.data_ptr(), B.data_ptr(), offsets.data_ptr(), C.data_ptr(), _TYPES[C.dtype], E, A.shape[0], M, N, _pitch(A),
                                      _pitch(B), variant, ops._stream_ptr())
     _lib.check(rc, "sk_grouped_wgrad")

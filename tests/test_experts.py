@@ -538,13 +538,30 @@ def test_grouped_kn_weights_on_tiles_that_stream_k(sk, dtype, sizes, N, K, paddi
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("kind", ["float16", "bfloat16", "int8"])
+@pytest.mark.parametrize("N", [40, 37])
+def test_rows_that_stand_for_many(sk, N):
+    """Broadcast rows of A and broadcast gradients (those of a sum over the rows) have stride 0."""
+    sizes, K = [5, 0, 25, 7], 64
+    offsets, R = offsets_of(sizes), sum(sizes)
+    B, row, d = rand((4, N, K), torch.float16, 1, 0.125), rand((1, K), torch.float16, 2), rand((1, N), torch.float16, 3)
+    A = row.expand(R, K)
+    assert torch.equal(sk.streamk_grouped(A, B, offsets), sk.streamk_grouped(A.contiguous(), B, offsets))
+    for one, other in ((A, d.expand(R, N)), (A.contiguous(), d.expand(R, N)), (A, d.expand(R, N).contiguous())):
+        x, w = one.detach().requires_grad_(), B.clone().requires_grad_()
+        dx, dw = torch.autograd.grad(sk.streamk_grouped(x, w, offsets), (x, w), other)
+        for e, at in groups(sizes):
+            assert_near(dx[at], other[at].double() @ B[e].double(), N, other[at].double().abs() @ B[e].double().abs())
+            assert_near(dw[e], other[at].double().T @ one[at].double(), sizes[e], other[at].double().abs().T @ one[at].double().abs())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["float16", "bfloat16", "float16 nn", "bfloat16 nn", "int8"])
 @pytest.mark.parametrize("sizes", [[1, 64, 65, 0, 128, 129, 192], [256, 257, 384, 385, 320], [127], [128, 128], [700, 60], [100] * 70])
 @pytest.mark.parametrize("N,K", [(256, 128), (520, 640), (1024, 4096), (72, 256)])
 def test_grouped_tiles_of_half_the_rows(sk, kind, sizes, N, K):
     """256 x 256 tiles of which at most 128 rows are used are another kind, also where they are cut along K."""
     R, E = sum(sizes) + 1, len(sizes)
-    out = torch.full((R, N), 7.0, dtype=torch.float16 if kind == "int8" else TYPES[kind], device="cuda")
+    out = torch.full((R, N), 7.0, dtype=torch.float16 if kind == "int8" else TYPES[kind.split()[0]], device="cuda")
     bias, kw = rand((E, N), out.dtype, 5), {}
     if kind == "int8":
         g = torch.Generator().manual_seed(R + N)
@@ -557,8 +574,10 @@ def test_grouped_tiles_of_half_the_rows(sk, kind, sizes, N, K):
         for e, at in groups(sizes):
             pre[at] *= sb[e].double()
     else:
-        A, B = rand((R, K), out.dtype, R), rand((E, N, K), out.dtype, N, 1 / math.sqrt(K))
-        pre, magnitudes = plain(A, B, sizes)
+        layout = "nn" if kind.endswith("nn") else "nt"
+        A, B = rand((R, K), out.dtype, R), rand((E, N, K) if layout == "nt" else (E, K, N), out.dtype, N, 1 / math.sqrt(K))
+        kw = dict(layout=layout)
+        pre, magnitudes = plain(A, B, sizes, layout)
     C = sk.streamk_grouped(A, B, offsets_of(sizes), variant=2, out_dtype=out.dtype, **kw)
     assert_near(C, pre, K, magnitudes, pre)
     assert not C[R - 1:].any()
