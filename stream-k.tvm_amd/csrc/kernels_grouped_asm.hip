@@ -91,7 +91,6 @@ __device__ __forceinline__ bool join_parts(typename P::Acc &acc, int tile, int p
 // and not 347.  (Tiles drawn from a counter as CTAs become free, and not dealt out: 356.)
 template <class P, bool NN>
 __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_grouped_asm_kernel(GroupedArgs g, int ipt, Workspace ws) {
-  constexpr int ROT_EXPERT = 11;
   constexpr auto LOW = P::LOW_TILE, FULL = NN ? P::WHOLE_TILE : P::WRAPPED_TILE;
   GroupWalk<P::BM, false> walk(g.offsets, g.E, g.R, g.tiles_n);
   const int pid = grouped_pid(g.grid);
@@ -109,10 +108,11 @@ __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_grouped_asm_kernel(
     s.low = s.t.rows - s.t.pm * P::BM <= P::BM / 2;
   };
   // Weights come straight from memory where few tiles share them, and all CTAs at the same K of rows whose pitch is a large power of two
-  // meet in the same channels (see rotation_of).  A row tile's CTAs start one iteration apart, so that they still share its rows in the
-  // L2s, those of different experts further apart, those that share weights at the same K.  ([K, N] weights: neighbouring tiles read
-  // neighbouring pieces of the same rows.)
-  auto rot_of = [&](const Segment &s) { return NN ? 0 : __builtin_amdgcn_readfirstlane((int)((unsigned)(s.t.pn + ROT_EXPERT * s.t.group) % (unsigned)s.n)); };
+  // meet in the same channels (see rotation_of): 128 rows against 65536 x 4096 135 us, with these starts 101.  Eight neighbours of a row
+  // tile, which share its rows in an L2, and all tiles that share weights are at the same K; the next eight, and other experts, elsewhere
+  // (every tile one iteration from the one beside it: up to 3 % slower).  [K, N] weights: neighbouring tiles read neighbouring
+  // pieces of the same rows.
+  auto rot_of = [&](const Segment &s) { return NN ? 0 : __builtin_amdgcn_readfirstlane((int)((unsigned)(5 * (s.t.pn >> 3) + 11 * s.t.group) % (unsigned)s.n)); };
   auto segment = [&](int item, Segment &s) {
     if (item >= items) return false;
     s.cut = -1;
