@@ -18,7 +18,7 @@ import torch
 from . import _lib, ops
 
 _TYPES = {torch.float16: _lib.SK_F16, torch.bfloat16: _lib.SK_BF16}
-_MAX_EXPERTS, _MAX_CHOSEN = 1024, 64
+MAX_EXPERTS, MAX_CHOSEN = 1024, 64
 _ops = torch.ops.streamk
 _NATIVE = _lib.torch_lib() is not None
 
@@ -236,8 +236,8 @@ _LOGITS = {torch.float16: _lib.SK_F16, torch.bfloat16: _lib.SK_BF16, torch.float
 def _route(logits, k):
     _on_device(logits, "logits", tuple(_LOGITS), 2)
     T, E = logits.shape
-    if not 1 <= E <= _MAX_EXPERTS or not 1 <= k <= min(E, _MAX_CHOSEN):
-        raise ValueError(f"1 to {_MAX_EXPERTS} experts, of which 1 to {_MAX_CHOSEN} are chosen: got {E} and k = {k}")
+    if not 1 <= E <= MAX_EXPERTS or not 1 <= k <= min(E, MAX_CHOSEN):
+        raise ValueError(f"1 to {MAX_EXPERTS} experts, of which 1 to {MAX_CHOSEN} are chosen: got {E} and k = {k}")
     if logits.stride(1) != 1 and E > 1 or logits.stride(0) < E:
         logits = logits.contiguous()
     new = lambda *shape: torch.empty(shape, dtype=torch.int32, device=logits.device)  # noqa: E731

@@ -13,7 +13,7 @@ import math
 
 import torch
 
-from .experts import combine_rows, dispatch_rows, route_experts, streamk_grouped
+from .experts import MAX_CHOSEN, MAX_EXPERTS, combine_rows, dispatch_rows, route_experts, streamk_grouped
 from .int8 import quantize_int8
 
 _ACTIVATIONS = {"relu": torch.nn.functional.relu, "gelu_tanh": lambda x: torch.nn.functional.gelu(x, approximate="tanh"), "silu": torch.nn.functional.silu}
@@ -35,8 +35,8 @@ class StreamKMoE(torch.nn.Module):
         step = 16 if weight_format == "int8" else 8
         if hidden % step or intermediate % step:
             raise ValueError(f"hidden and intermediate must be multiples of {step} with {weight_format} weights")
-        if not 1 <= chosen <= experts:
-            raise ValueError(f"1 to {experts} experts can be chosen, not {chosen}")
+        if not 1 <= experts <= MAX_EXPERTS or not 1 <= chosen <= min(experts, MAX_CHOSEN):
+            raise ValueError(f"1 to {MAX_EXPERTS} experts, of which 1 to {MAX_CHOSEN} are chosen: got {experts} and {chosen}")
         self.hidden, self.intermediate, self.experts, self.chosen = hidden, intermediate, experts, chosen
         self.activation, self.weight_format, self.dtype = activation, weight_format, own
         shapes = {"up": (experts, intermediate, hidden), "down": (experts, hidden, intermediate)}
@@ -74,10 +74,10 @@ class StreamKMoE(torch.nn.Module):
         rows = x.reshape(-1, self.hidden)
         if rows.shape[0] == 0:
             return torch.zeros_like(x)
-        route = self.route(rows)
         if self.weight_format == "int8":
-            out = self._int8(rows, route)
-        elif torch.is_grad_enabled() and (rows.requires_grad or self.up.requires_grad or self.down.requires_grad):
+            return self._int8(rows).view(x.shape)
+        route = self.route(rows)
+        if torch.is_grad_enabled() and (rows.requires_grad or self.up.requires_grad or self.down.requires_grad):
             h = streamk_grouped(dispatch_rows(rows, route), self.up, route.offsets)
             out = streamk_grouped(_ACTIVATIONS[self.activation](h), self.down, route.offsets)
         else:
@@ -85,12 +85,14 @@ class StreamKMoE(torch.nn.Module):
             out = streamk_grouped(h, self.down, route.offsets)
         return combine_rows(out, route).view(x.shape)
 
-    def _int8(self, x, route):
+    @torch.no_grad()   # (inference only, as the other quantised layers)
+    def _int8(self, x):
+        route = self.route(x)
         q, scale = quantize_int8(x)
         h = streamk_grouped(dispatch_rows(q, route), self.up, route.offsets, scale_a=dispatch_rows(scale, route), scale_b=self.up_scale,
                             out_dtype=self.dtype, activation=self.activation)
         q, scale = quantize_int8(h)
-        return streamk_grouped(q, self.down, route.offsets, scale_a=scale, scale_b=self.down_scale, out_dtype=self.dtype)
+        return combine_rows(streamk_grouped(q, self.down, route.offsets, scale_a=scale, scale_b=self.down_scale, out_dtype=self.dtype), route)
 
     def extra_repr(self):
         return (f"hidden={self.hidden}, intermediate={self.intermediate}, experts={self.experts}, chosen={self.chosen}, "

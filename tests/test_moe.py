@@ -102,6 +102,7 @@ def test_experts_layer_in_int8(sk, dtype, size):
         assert torch.equal(small.route(x).experts, layer.route(x).experts)
     assert got.dtype == x.dtype and off(got, want) <= 0.05
     assert not list(small.parameters())
+    assert not small(x.clone().requires_grad_()).requires_grad
 
 
 @pytest.mark.gpu
@@ -133,7 +134,7 @@ def test_experts_layer_without_tokens(sk):
 
 
 def test_experts_layer_refusals(sk):
-    for args, kw in (((64, 64, 4, 5), {}), ((64, 64, 4, 0), {}), ((60, 64, 4, 2), {}), ((72, 64, 4, 2), dict(weight_format="int8")), ((64, 64, 4, 2), dict(activation="tanh")),
+    for args, kw in (((64, 64, 4, 5), {}), ((64, 64, 1025, 1), {}), ((64, 64, 100, 65), {}), ((64, 64, 4, 0), {}), ((60, 64, 4, 2), {}), ((72, 64, 4, 2), dict(weight_format="int8")), ((64, 64, 4, 2), dict(activation="tanh")),
                      ((64, 64, 4, 2), dict(weight_format="q4")), ((64, 64, 4, 2), dict(dtype=torch.float16)), ((64, 64, 4, 2), dict(weight_format="int8", dtype=torch.float32))):
         with pytest.raises(ValueError):
             sk.StreamKMoE(*args, **kw)
