@@ -119,12 +119,6 @@ __device__ __forceinline__ void set_operands(WaveKArgs &a, const GroupedArgs &g,
   set_operands(static_cast<GemmArgs &>(a), g, B);
   a.start_scale = 0xffffffffu / (unsigned)g.tiles_n;   // an eighth of the columns start at an eighth of K each
 }
-__device__ __forceinline__ void set_operands(SkinnyArgs &a, const GroupedArgs &g, const half_t *B) {
-  a.W = B;
-  a.ldw = g.ldb;
-  a.scales = a.zeros = nullptr;
-  a.zero = a.groups = 0;
-}
 template <class P>
 __device__ __forceinline__ typename P::Args expert_args(const GroupedArgs &g, const GroupTile &t) {
   typename P::Args a;
