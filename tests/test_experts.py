@@ -702,3 +702,80 @@ def test_gradients_of_gradients_are_refused(sk):
     with pytest.raises(RuntimeError):
         g, = torch.autograd.grad(C.float().square().sum(), A, create_graph=True)
         g.sum().backward()
+
+
+# ---- offsets that 32 bits do not hold ----
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", [0, 1, 2, 3, 6])
+@pytest.mark.parametrize("kind", ["bfloat16", "int8"])
+def test_weights_beyond_4_gib(sk, variant, kind):
+    E, N, K, sizes = (5, 8192, 65536, [2, 0, 130, 1, 3]) if kind == "bfloat16" else (5, 16384, 65536, [2, 0, 130, 1, 3])
+    R = sum(sizes)
+    if kind == "int8":
+        B = torch.empty((E, N, K), dtype=torch.int8, device="cuda").random_(-127, 128)
+        A = torch.empty((R, K), dtype=torch.int8, device="cuda").random_(-127, 128)
+        sa, sb = torch.rand(R, device="cuda") + 0.5, (torch.rand(E, N, device="cuda") + 0.5) / (73 ** 2 * 256)
+        C = sk.streamk_grouped(A, B, offsets_of(sizes), scale_a=sa, scale_b=sb, variant=variant)
+    else:
+        B = torch.empty((E, N, K), dtype=torch.bfloat16, device="cuda").normal_(0, 1 / 256)
+        A = rand((R, K), torch.bfloat16, 3)
+        C = sk.streamk_grouped(A, B, offsets_of(sizes), variant=variant)
+    for e, at in groups(sizes):
+        for cols in (slice(0, 40), slice(N - 40, N)):
+            pre = A[at].double() @ B[e, cols].double().T
+            magnitudes = A[at].double().abs() @ B[e, cols].double().abs().T
+            if kind == "int8":
+                pre, magnitudes = pre * sa[at, None].double() * sb[e, cols].double(), 0
+            assert_near(C[at, cols], pre, K, magnitudes, pre)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout,variant", [("nt", 0), ("nt", 1), ("nt", 2), ("nt", 6), ("nn", 1), ("nn", 2), ("nn", 5)])
+def test_rows_beyond_4_gib(sk, layout, variant):
+    R, N, K = 140_000, 16384, 64
+    sizes = [R - 300, 300]
+    A, B = rand((R, K), torch.bfloat16, 1), rand((2, N, K) if layout == "nt" else (2, K, N), torch.bfloat16, 2, 0.125)
+    C = sk.streamk_grouped(A, B, offsets_of(sizes), layout=layout, variant=variant)
+    assert C.numel() * 2 > 2 ** 32
+    for rows in (slice(0, 5), slice(131_070, 131_075), slice(R - 305, R - 300), slice(R - 5, R)):
+        e = int(rows.start >= sizes[0])
+        W = B[e].double().T if layout == "nt" else B[e].double()
+        assert_near(C[rows], A[rows].double() @ W, K, A[rows].double().abs() @ W.abs())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", [0, 1, 2])
+def test_weight_gradients_beyond_4_gib(sk, variant):
+    sizes, N, K = [100, 0, 30, 0, 0, 0, 1, 0, 90], 16384, 16384
+    dC, A = rand((sum(sizes), N), torch.bfloat16, 1), rand((sum(sizes), K), torch.bfloat16, 2)
+    dW = sk.streamk_grouped_wgrad(dC, A, offsets_of(sizes), variant=variant)
+    assert dW.numel() * 2 > 2 ** 32
+    for e, at in groups(sizes):
+        for rows in (slice(0, 8), slice(N - 8, N)):
+            assert_near(dW[e, rows], dC[at, rows].double().T @ A[at].double(), sizes[e], dC[at, rows].double().abs().T @ A[at].double().abs())
+
+
+@pytest.mark.gpu
+def test_exchange_beyond_4_gib(sk):
+    T, E, k, H = 70_000, 16, 4, 8192
+    logits = torch.randn(T, E, device="cuda")
+    route = sk.route_experts(logits, k)
+    x = torch.randn(T, H, device="cuda", dtype=torch.bfloat16)
+    rows = sk.dispatch_rows(x, route)
+    assert rows.numel() * 2 > 2 ** 32
+    for at in (slice(0, 10), slice(T * k - 10, T * k), slice(262_100, 262_200)):
+        assert torch.equal(rows[at], x[route.order[at].long() // k])
+    out = sk.combine_rows(rows, route)
+    # (the same row k times, with weights that sum to one up to k fp32 roundings)
+    assert ((out.float() - x.float()).abs() <= (2.0 ** -8 + 8 * 2.0 ** -24) * x.float().abs() + 1e-30).all()
+    rows.requires_grad_()
+    weights = route.weights.clone().requires_grad_()
+    d_out = torch.randn(T, H, device="cuda", dtype=torch.bfloat16)
+    d_rows, d_weights = torch.autograd.grad(sk.combine_rows(rows, route._replace(weights=weights)), (rows, weights), d_out)
+    last = torch.arange(T * k - 10, T * k, device="cuda")
+    slots = route.order[last].long()
+    want = (weights.detach().flatten()[slots, None] * d_out[slots // k].float()).bfloat16()
+    assert torch.equal(d_rows[last], want)
+    y = rows.detach()[route.place[T - 1].long()].double()
+    off = (d_weights[T - 1].double() - y @ d_out[T - 1].double()).abs()
+    assert (off <= 2 * H * 2.0 ** -24 * (y.abs() @ d_out[T - 1].double().abs())).all()
