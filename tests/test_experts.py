@@ -779,3 +779,95 @@ def test_exchange_beyond_4_gib(sk):
     y = rows.detach()[route.place[T - 1].long()].double()
     off = (d_weights[T - 1].double() - y @ d_out[T - 1].double()).abs()
     assert (off <= 2 * H * 2.0 ** -24 * (y.abs() @ d_out[T - 1].double().abs())).all()
+
+
+# ---- NaN and infinities stay where they belong ----
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", VARIANTS)
+@pytest.mark.parametrize("kind", ["float16 nt", "bfloat16 nn", "int8"])
+def test_bad_rows_and_weights_of_other_experts(sk, variant, kind):
+    """Experts 0, 2 and 5 own bad rows or weights; 1 and 6 have no rows, bad weights and no part in anything."""
+    sizes, N, K = [3, 0, 130, 70, 257, 1, 0, 40], 264, 256
+    if kind.endswith("nn") and variant not in (1, 2, 5):
+        return   # ([E, N, K] weights only)
+    R, offsets = sum(sizes) + 4, offsets_of(sizes)
+    at = dict(groups(sizes))
+    if kind == "int8":
+        A, B = torch.empty((R, K), dtype=torch.int8, device="cuda").random_(-127, 128), torch.empty((len(sizes), N, K), dtype=torch.int8, device="cuda").random_(-127, 128)
+        sa, sb = torch.rand(R, device="cuda") + 0.5, (torch.rand(len(sizes), N, device="cuda") + 0.5) / 73 ** 2
+        clean = sk.streamk_grouped(A, B, offsets, scale_a=sa, scale_b=sb, variant=variant)
+        sa[at[0].start] = float("nan")
+        sa[at[2].stop - 1] = float("inf")
+        sa[R - 4:] = float("nan")
+        sb[1] = sb[6] = sb[5] = float("nan")
+        C = sk.streamk_grouped(A, B, offsets, scale_a=sa, scale_b=sb, variant=variant)
+    else:
+        dtype, layout = TYPES[kind.split()[0]], kind.split()[1]
+        A, B = rand((R, K), dtype, 1), rand((len(sizes), N, K) if layout == "nt" else (len(sizes), K, N), dtype, 2, 1 / 16)
+        clean = sk.streamk_grouped(A, B, offsets, layout=layout, variant=variant)
+        A[at[0].start, 5] = float("nan")
+        A[at[2].stop - 1, K - 1] = float("inf")
+        A[R - 4:] = float("nan")
+        B[1] = B[6] = B[5] = float("nan")
+        C = sk.streamk_grouped(A, B, offsets, layout=layout, variant=variant)
+    bad = torch.zeros(R, dtype=torch.bool, device="cuda")
+    bad[at[0].start] = bad[at[2].stop - 1] = bad[at[5]] = True
+    assert torch.equal(C[~bad], clean[~bad])
+    assert not torch.isfinite(C[bad]).any(1).any() if kind != "int8" else torch.isnan(C[at[0].start]).all() and torch.isnan(C[at[5]]).all()
+    assert not C[R - 4:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", [1, 2])
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_bad_rows_in_weight_gradients(sk, variant, dtype):
+    sizes, N, K = [3, 0, 130, 70, 257], 264, 256
+    R, offsets, at = sum(sizes) + 4, offsets_of(sizes), dict(groups(sizes))
+    dC, A = rand((R, N), TYPES[dtype], 1), rand((R, K), TYPES[dtype], 2)
+    clean = sk.streamk_grouped_wgrad(dC, A, offsets, variant=variant)
+    A[at[2].start] = float("nan")
+    dC[at[2].stop - 1] = float("inf")
+    A[R - 4:] = dC[R - 4:] = float("nan")
+    dW = sk.streamk_grouped_wgrad(dC, A, offsets, variant=variant)
+    for e in (0, 1, 3, 4):
+        assert torch.equal(dW[e], clean[e])
+    assert torch.isnan(dW[2]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [5, 300])
+def test_bad_rows_in_the_exchange(sk, T):
+    """Tokens without experts, with fewer than k, and with bad rows: none of it reaches another token."""
+    E, k, H = 6, 3, 72
+    logits = torch.randn(T, E, device="cuda")
+    logits[0] = float("-inf")
+    logits[1, 1:] = float("-inf")
+    logits[3, 2] = float("nan")
+    route = sk.route_experts(logits, k)
+    assert (route.experts[0] == -1).all() and (route.experts[1, 1:] == -1).all() and not (route.experts[3] == 2).any()
+    x = torch.randn(T, H, device="cuda").bfloat16()
+    x[2] = float("nan")
+    rows = sk.dispatch_rows(x, route)
+    of = route.order.long()
+    assert torch.equal(torch.isnan(rows).all(1), (of >= 0) & (of // k == 2)) and not rows[of < 0].any()
+    clean = torch.randn(T * k, H, device="cuda").bfloat16()
+    # sorted row 0 and the rows of token 2 are bad; so are those that belong to no slot
+    y = clean.clone()
+    y[0] = float("nan")
+    y[route.place[2].long()] = float("inf")
+    y[of < 0] = float("nan")
+    token = of[0] // k
+    got, want = sk.combine_rows(y, route), sk.combine_rows(clean, route)
+    good = torch.ones(T, dtype=torch.bool, device="cuda")
+    good[token] = good[2] = False
+    assert torch.equal(got[good], want[good]) and not torch.isfinite(got[~good]).any() and not got[0].any()
+    y.requires_grad_()
+    weights = route.weights.clone().requires_grad_()
+    d_out = torch.randn(T, H, device="cuda").bfloat16()
+    d_out[2] = float("nan")
+    dy, dw = torch.autograd.grad(sk.combine_rows(y, route._replace(weights=weights)), (y, weights), d_out)
+    mine = (of >= 0) & (of // k == 2)
+    assert torch.isfinite(dy[~mine]).all() and torch.isfinite(dw[good]).all() and not dy[of < 0].any() and not dw[0].any()
+    dx, = torch.autograd.grad(sk.dispatch_rows(x.requires_grad_(), route), x, torch.where(mine[:, None], float("nan"), torch.ones(T * k, H, device="cuda").bfloat16()))
+    keep = torch.arange(T, device="cuda") != 2
+    assert torch.equal(dx[keep], (route.experts >= 0).sum(1, keepdim=True).expand(T, H)[keep].bfloat16())
