@@ -10,6 +10,26 @@
 
 namespace sk {
 
+// The 16-bit policies with an end that leaves the stages alone whatever the tile's columns and epilogue are
+template <bool BF16, bool NN>
+struct GroupedAsm16 : TileF16Asm<BF16 ? 1 : 0, NN> {
+  typedef TileF16Asm<BF16 ? 1 : 0, NN> P;
+  static __device__ __forceinline__ void store_rows(const typename P::Args &a, int pm, int pn, const void *epi, int i1) {
+    const int wave = threadIdx.x >> 6, row0 = pm * P::BM + (wave >> 1) * P::WTM, col0 = pn * P::BN + (wave & 1) * P::WTN;
+    by_epilogue(epi, [&](auto e) {
+      AsmEnd<P, false, BF16, decltype(e)::value>::store(a.C, a.ldc, a.M, a.N, row0, col0, nullptr, nullptr, epi_bias(epi), 0, i1);
+    });
+  }
+  static __device__ __forceinline__ void store_c(const typename P::Args &a, const typename P::Acc &, int pm, int pn, char *, const void *epi) {
+    if (P::direct_store_ok(a, pn, epi)) P::template store_c_direct<-1>(a, pm, pn);
+    else store_rows(a, pm, pn, epi, P::FM);
+  }
+  static __device__ __forceinline__ void store_c_half(const typename P::Args &a, const typename P::Acc &, int pm, int pn, char *, const void *epi, int) {
+    if (P::direct_store_ok(a, pn, epi)) P::template store_c_direct<0>(a, pm, pn);
+    else store_rows(a, pm, pn, epi, P::FM / 2);
+  }
+};
+
 // How the tiles that are left when every CTA has had its whole rounds are cut: K in `parts` equal parts, one to a CTA.  (Aligned cuts: the
 // CTAs stay at the same K of their tiles and share rows and weights in the L2s.  Runs of equal length that begin anywhere, as for the
 // small tiles in grouped.h, write 90 MB of sums and cost 100 us here: 8 x 11008 x 4096, 3000 rows, bfloat16 307 us, whole tiles 284.)
@@ -142,7 +162,7 @@ __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_grouped_asm_kernel(
     requested = false;
     item += g.grid;
     have = segment(item, next);
-    if (have && P::epilogue_lds_free(a, s.t.pn, epi)) {
+    if (have) {   // (every end here leaves the stages alone)
       const typename P::Args b = expert_args<P>(g, next.t);
       if (next.low) P::template prefetch_first_stage<LOW>(b, next.t.pm, next.t.pn, next.k0, next.n, rot_of(next));
       else P::template prefetch_first_stage<FULL>(b, next.t.pm, next.t.pn, next.k0, next.n, rot_of(next));
@@ -180,8 +200,8 @@ bool grouped_asm_takes(const GroupedShape &h) { return h.K % (h.type == GT_I8 ? 
 int launch_grouped_asm(const GroupedArgs &g, const GroupedShape &h, const Workspace &ws, hipStream_t s) {
   const int ipt = (int)(h.K / (h.type == GT_I8 ? 128 : 64));
   if (h.type == GT_I8) return launch_asm<ScaledAsm>(g, h, ipt, ws, s);
-  if (h.nn) return h.type == GT_BF16 ? launch_asm<TileF16Asm<1, true>, true>(g, h, ipt, ws, s) : launch_asm<TileF16Asm<0, true>, true>(g, h, ipt, ws, s);
-  return h.type == GT_BF16 ? launch_asm<TileF16Asm<1, false>>(g, h, ipt, ws, s) : launch_asm<TileF16Asm<0, false>>(g, h, ipt, ws, s);
+  if (h.nn) return h.type == GT_BF16 ? launch_asm<GroupedAsm16<true, true>, true>(g, h, ipt, ws, s) : launch_asm<GroupedAsm16<false, true>, true>(g, h, ipt, ws, s);
+  return h.type == GT_BF16 ? launch_asm<GroupedAsm16<true, false>>(g, h, ipt, ws, s) : launch_asm<GroupedAsm16<false, false>>(g, h, ipt, ws, s);
 }
 
 // ---- dW[e] = dC[rows of e]^T A[rows of e] ----

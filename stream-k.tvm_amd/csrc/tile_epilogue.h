@@ -5,20 +5,17 @@
 
 namespace sk {
 
-// four fp32 values, rounded once to bfloat16 or fp16 (C and the patches carry 16-bit patterns)
+// four fp32 values, rounded to bfloat16 or fp16 (C and the patches carry 16-bit patterns).  The conversion is an instruction of its own: the
+// compiler may merge one to fp16 with the multiplication in front of it, which rounds once where another kernel rounds twice.
 template <bool BF16>
 __device__ __forceinline__ half4v round4(floatx4 x) {
-  half4v h;
+  union { uint32_t w[2]; half4v h; } r;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    if constexpr (BF16) {
-      const __bf16 b = (__bf16)x[e];
-      h[e] = __builtin_bit_cast(half_t, b);
-    } else {
-      h[e] = (half_t)x[e];
-    }
+  for (int i = 0; i < 2; ++i) {
+    if constexpr (BF16) asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(r.w[i]) : "v"(x[2 * i]), "v"(x[2 * i + 1]));
+    else asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(r.w[i]) : "v"(x[2 * i]), "v"(x[2 * i + 1]));
   }
-  return h;
+  return r.h;
 }
 
 // Stores FM x FN blocks of a wave, the first of which stands at (row0, col0) of C, through a patch of LDS of the wave's own

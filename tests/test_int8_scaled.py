@@ -150,6 +150,21 @@ def test_epilogue(sk, M, activation):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("activation", [None, "relu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_every_tile_rounds_alike(sk, dtype, activation, with_bias):
+    M, N, K = 300, 520, 768
+    A, B, sa, sb = operands(M, N, K, 9)
+    bias = torch.randn(N, device="cuda").to(TYPES[dtype]) if with_bias else None
+    run = lambda **config: sk.streamk_int8_scaled(A, B, sa, sb, out_dtype=TYPES[dtype], bias=bias, activation=activation, **config)  # noqa: E731
+    want = run(bm=64, bn=64, variant=11)
+    assert_scaled(want, product(A, B, sa, sb) + (bias.double() if with_bias else 0), activation)
+    for config in (dict(bm=256, bn=256), dict(bm=128, bn=128, bk=64), dict(bm=128, bn=128, bk=128), dict(bm=64, bn=128, bk=64), dict(bm=128, bn=64, variant=11)):
+        assert torch.equal(run(**config), want), config
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("config", [dict(variant=9), dict(variant=12), dict(bm=128, bn=128), dict(bm=64, bn=128, bk=64), dict(bm=256, bn=256), dict(bm=256, bn=256, schedule="splitk", split=2),
                                     dict(bm=128, bn=128, schedule="splitk", split=4), dict(bm=64, bn=64, variant=11),
                                     dict(bm=128, bn=128, schedule="basic", grid=24, fixup="atomic")])
