@@ -76,14 +76,17 @@ std::tuple<Tensor, Tensor> quantize_i8(const Tensor &x) {
 }
 
 // ---- the grouped product ----
-bool grouped(const Tensor &A, const Tensor &B, const Tensor &offsets, std::string_view layout, MaybeType out_dtype, const MaybeTensor &scale_a,
+bool grouped(const Tensor &rows, const Tensor &B, const Tensor &offsets, std::string_view layout, MaybeType out_dtype, const MaybeTensor &scale_a,
              const MaybeTensor &scale_b, const MaybeTensor &bias, std::string_view activation, int64_t variant, Tensor &C) {
-  const at::ScalarType type = A.scalar_type();
+  const at::ScalarType type = rows.scalar_type();
   const bool i8 = type == at::kChar, nn = layout == "nn";
+  // ([K, N] weights multiply A's last piece of eight columns whole, those past K by zeros: they have to be finite, so they become zeros)
+  const bool pad = nn && rows.is_cuda() && rows.dim() == 2 && rows.numel() > 0 && rows.size(1) % 8 != 0;
+  const Tensor A = pad ? at::constant_pad_nd(rows, {0, 8 - rows.size(1) % 8}) : rows;
   if ((!i8 && !is16(A)) || (!nn && layout != "nt") || (nn && i8) || B.scalar_type() != type || B.dim() != 3 || B.device() != A.device()) return false;
   if (!rows_in_place(A) && !one_row_in_place(A)) return false;
   const int64_t E = B.size(0), N = B.size(nn ? 2 : 1), K = B.size(nn ? 1 : 2), R = A.size(0);
-  if (E == 0 || N == 0 || K == 0 || A.size(1) != K || B.stride(2) != 1 || B.size(1) < 2 || !is_ints(offsets, A, 1) || offsets.size(0) != E + 1) return false;
+  if (E == 0 || N == 0 || K == 0 || rows.size(1) != K || B.stride(2) != 1 || B.size(1) < 2 || !is_ints(offsets, A, 1) || offsets.size(0) != E + 1) return false;
   const at::ScalarType out = i8 ? out_dtype.value_or(at::kHalf) : type;
   if ((out != at::kHalf && out != at::kBFloat16) || (!i8 && out_dtype.has_value() && *out_dtype != type)) return false;
   sk_grouped g{};
@@ -261,10 +264,8 @@ struct GroupedProduct : torch::autograd::Function<GroupedProduct> {
     const bool nn = ctx->saved_data["nn"].toBool();
     Tensor dA, dB;
     if (ctx->needs_input_grad(0)) {
-      // ('nt': dC [R, N] times B[e] [N, K]; that product takes any N where the rows are padded with zeros)
-      const int64_t N = dC.size(1);
-      const Tensor rows = nn || N % 8 == 0 ? dC : at::constant_pad_nd(dC, {0, 8 - N % 8}).narrow(1, 0, N);
-      dA = product.call(rows, B, offsets, nn ? "nt" : "nn", c10::nullopt, c10::nullopt, c10::nullopt, c10::nullopt, "none", 0);
+      // ('nt': dC [R, N] times B[e] [N, K], any N)
+      dA = product.call(dC, B, offsets, nn ? "nt" : "nn", c10::nullopt, c10::nullopt, c10::nullopt, c10::nullopt, "none", 0);
     }
     if (ctx->needs_input_grad(1)) dB = nn ? wgrad.call(A, dC, offsets, 0) : wgrad.call(dC, A, offsets, 0);
     return {dA, dB, Tensor(), Tensor(), Tensor()};

@@ -59,6 +59,13 @@ def _rows(t):
     return t.contiguous() if t.shape[0] > 1 and t.stride(0) < t.shape[1] else t
 
 
+def _padded(t):
+    """t with its columns filled up with zeros to a multiple of 8, its rows as the kernels read them."""
+    if t.shape[1] % 8:
+        return torch.nn.functional.pad(t, (0, 8 - t.shape[1] % 8))
+    return _rows(t)
+
+
 def _grouped(A, B, offsets, layout="nt", out_dtype=None, scale_a=None, scale_b=None, bias=None, activation="none", variant=0, out=None):
     if layout not in ("nt", "nn"):
         raise ValueError("layout must be 'nt' (B is [E, N, K]) or 'nn' (B is [E, K, N])")
@@ -102,7 +109,9 @@ def _grouped(A, B, offsets, layout="nt", out_dtype=None, scale_a=None, scale_b=N
     C = torch.empty((R, N), dtype=out_dtype, device=A.device) if out is None else out
     if R == 0:
         return C
-    A = _rows(A)
+    # ([K, N] weights and a K that is no multiple of 8: the last piece of eight columns of A is multiplied whole, its columns past K by
+    # zeros -- but zero times what lies beside a view may be NaN)
+    A = _padded(A)[:, :K] if layout == "nn" and K % 8 else _rows(A)
     ldb = B.stride(1) if B.shape[1] > 1 else (B.shape[2] + 15) // 16 * 16
     g = _lib.SkGrouped(dtype=_lib.SK_I8 if int8 else _TYPES[A.dtype], layout=ops._plan_mod._LAYOUTS[layout], out_dtype=_TYPES[out_dtype],
                        activation=_lib.ACTIVATIONS[activation], E=E, R=R, N=N, K=K, A=A.data_ptr(), B=B.data_ptr(),
@@ -131,13 +140,6 @@ _operator("gemm_grouped_out", f"(Tensor A, Tensor B, Tensor offsets, Tensor(a!) 
 
 
 # ---- the gradient of its weights ----
-def _padded(t):
-    """t with its columns filled up with zeros to a multiple of 8, its rows as the kernels read them."""
-    if t.shape[1] % 8:
-        return torch.nn.functional.pad(t, (0, 8 - t.shape[1] % 8))
-    return _rows(t)
-
-
 def _wgrad(A, B, offsets, variant=0):
     _on_device(A, "A", tuple(_TYPES), 2)
     _on_device(B, "B", (A.dtype,), 2)
@@ -176,28 +178,18 @@ class _GroupedProduct(torch.autograd.Function):
         A, B, offsets = ctx.saved_tensors
         dA = dB = None
         if ctx.needs_input_grad[0]:
-            if ctx.layout == "nn":
-                dA = _ops.gemm_grouped(dC, B, offsets, "nt")
-            else:
-                dA = _grouped_rows_grad(dC, B, offsets)
+            dA = _ops.gemm_grouped(dC, B, offsets, "nt" if ctx.layout == "nn" else "nn")
         if ctx.needs_input_grad[1]:
             dB = _ops.grouped_wgrad(dC, A, offsets) if ctx.layout == "nt" else _ops.grouped_wgrad(A, dC, offsets)
         return dA, dB, None, None, None
-
-
-def _grouped_rows_grad(dC, B, offsets):
-    """dC [R, N] times B[e] [N, K]: the 'nn' product, whose K (here N) may be any number where A's rows are padded with zeros."""
-    N = dC.shape[1]
-    if N % 8 == 0:
-        return _ops.gemm_grouped(dC, B, offsets, "nn")
-    return _ops.gemm_grouped(_padded(dC)[:, :N], B, offsets, "nn")
 
 
 def streamk_grouped(A, B, offsets, *, layout="nt", scale_a=None, scale_b=None, out_dtype=None, out=None, bias=None, activation=None, variant=0):
     """Rows offsets[e] <= r < offsets[e + 1] of A [R, K] times the weights of expert e: C[r] = activation(A[r] @ B[e].T + bias[e]) for B
     [E, N, K] (layout 'nt'), A[r] @ B[e] for B [E, K, N] ('nn'); float16, bfloat16, or int8 ('nt') with scale_a [R] and scale_b
     [E, N] (float32), whose result is `out_dtype` (float16 by default).  offsets: int32 [E + 1] on the device, ascending from 0;
-    groups of any size; rows behind the last group come out as zeros.  bias: [E, N] in C's type.  Sums in fp32 (int8: exact), rounded
+    groups of any size; rows behind the last group come out as zeros.  K is a multiple of 8 (int8: 16) for 'nt', N of 8 for 'nn', whose K
+    may be any number (rows of a K that is no multiple of 8 are copied).  bias: [E, N] in C's type.  Sums in fp32 (int8: exact), rounded
     once.  Differentiable in A and B without bias, activation, scales and out.  variant: which tiles run (sk_grouped in streamk.h); 0
     lets the sizes decide."""
     activation = activation or "none"
