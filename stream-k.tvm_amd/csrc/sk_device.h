@@ -340,7 +340,7 @@ __device__ __forceinline__ const half_t *epi_bias(const void *word) {
 // activation applied in fp32 after the bias, before the rounding to C's type; act is uniform over the grid
 // (codes are sk_activation's: 1 relu, 2 gelu in its tanh form, 3 silu)
 __device__ __forceinline__ float activate(float x, int act) {
-  if (act == 1) return fmaxf(x, 0.f);
+  if (act == 1) return x <= 0.f ? 0.f : x;   // (fmaxf(NaN, 0) is 0; a NaN has to stay one)
   if (act == 2) {
     // 0.5 x (1 + tanh(u)) = x / (1 + exp(-2u)),  u = sqrt(2/pi) (x + 0.044715 x^3)
     const float u = 0.7978845608028654f * (x + 0.044715f * x * x * x);

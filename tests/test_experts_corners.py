@@ -85,3 +85,128 @@ def test_columns_beside_a_gradient_do_not_count(sk, dtype):
     for e, at in groups(sizes):
         assert_near(dx[at], d[at].double() @ B[e].double(), N, d[at].double().abs() @ B[e].double().abs())
         assert_near(dw[e], d[at].double().T @ A[at].double(), sizes[e], d[at].double().abs().T @ A[at].double().abs())
+
+
+# ---- activations of what is not finite ----
+ACTIVATIONS = ["relu", "gelu_tanh", "silu"]
+
+
+def bad_row(A, B):
+    """Row 1 of A makes NaN of every column, row 2 +infinity of the even columns of B [N, K] and -infinity of the odd ones, row 3 zeros."""
+    A[1, 5] = math.nan
+    A[2:4] = 0
+    A[2, 0] = math.inf
+    B[0::2, 0], B[1::2, 0] = 1, -1
+
+
+def assert_bad_rows(C, clean, activation):
+    assert torch.isnan(C[1]).all()
+    assert torch.isposinf(C[2, 0::2]).all()
+    # (gelu and silu of -infinity are the product -infinity * 0)
+    assert (C[2, 1::2] == 0).all() if activation == "relu" else torch.isnan(C[2, 1::2]).all()
+    assert not C[3].any()
+    assert torch.equal(C[4:], clean[4:]) and torch.equal(C[0], clean[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("M,kw", [(8, {}), (20, {}), (60, {}), (100, dict(bm=128, bn=128)), (300, dict(bm=256, bn=256)), (100, dict(variant=11)), (100, dict(layout="nn")), (300, dict(layout="nn"))])
+def test_products_keep_nan_through_activations(sk, activation, dtype, M, kw):
+    N, K, t = 264, 256, TYPES[dtype]
+    run = sk.streamk_fp16 if dtype == "float16" else sk.streamk_bf16
+    A, B = rand((M, K), t, 1), rand((N, K), t, 2, 1 / 16)
+    good = A.clone()
+    bad_row(A, B)
+    W = B.T.contiguous() if kw.get("layout") == "nn" else B
+    assert_bad_rows(run(A, W, activation=activation, **kw), run(good, W, activation=activation, **kw), activation)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+@pytest.mark.parametrize("kind", ["float16 nt", "bfloat16 nt", "float16 nn", "bfloat16 nn"])
+@pytest.mark.parametrize("variant", [1, 2, 3, 4, 5, 6])
+def test_grouped_products_keep_nan_through_activations(sk, activation, kind, variant):
+    dtype, layout = kind.split()
+    if layout == "nn" and variant not in (1, 2, 5):
+        pytest.skip("no such tile for [K, N] weights")
+    sizes, N, K, t = [70, 0, 130], 264, 256, TYPES[dtype]
+    A, B, bias = rand((200, K), t, 1), rand((3, N, K), t, 2, 1 / 16), torch.zeros(3, N, dtype=t, device="cuda")
+    good = A.clone()
+    bad_row(A, B[0])
+    W = B.transpose(1, 2).contiguous() if layout == "nn" else B
+    run = lambda a, **kw: sk.streamk_grouped(a, W, offsets_of(sizes), layout=layout, variant=variant, activation=activation, **kw)  # noqa: E731
+    assert_bad_rows(run(A), run(good), activation)
+    assert_bad_rows(run(A, bias=bias), run(good, bias=bias), activation)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+@pytest.mark.parametrize("out", sorted(TYPES))
+@pytest.mark.parametrize("variant", [1, 2, 3, 4, 5, 6])
+def test_grouped_int8_products_keep_nan_through_activations(sk, activation, out, variant):
+    sizes, N, K = [70, 0, 130], 264, 256
+    g = torch.Generator().manual_seed(1)
+    A, B = (torch.randint(-127, 128, s, generator=g, dtype=torch.int8).cuda() for s in ((200, K), (3, N, K)))
+    sa, sb = torch.rand(200, device="cuda") * 0.01, torch.rand(3, N, device="cuda") * 0.01
+    run = lambda: sk.streamk_grouped(A, B, offsets_of(sizes), scale_a=sa, scale_b=sb, out_dtype=TYPES[out], variant=variant, activation=activation)  # noqa: E731
+    clean = run()
+    sa[1], sb[2, 7] = math.nan, math.nan
+    C, bad = run(), torch.zeros(200, N, dtype=torch.bool, device="cuda")
+    bad[1], bad[70:, 7] = True, True
+    assert torch.equal(torch.isnan(C), bad) and torch.equal(C[~bad], clean[~bad])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+@pytest.mark.parametrize("out", sorted(TYPES))
+@pytest.mark.parametrize("M,config", [(1, {}), (20, {}), (60, dict(variant=9)), (60, dict(variant=12)), (100, {}), (300, dict(bm=64, bn=64, variant=11)), (300, dict(bm=128, bn=128)), (300, dict(bm=64, bn=128, bk=64)),
+                                      (300, dict(bm=256, bn=256)), (300, dict(bm=256, bn=256, schedule="splitk", split=2)), (300, dict(bm=128, bn=128, schedule="splitk", split=4))])
+def test_int8_products_keep_nan_through_activations(sk, activation, out, M, config):
+    N, K = 264, 512
+    g = torch.Generator().manual_seed(1)
+    A, B = (torch.randint(-127, 128, s, generator=g, dtype=torch.int8).cuda() for s in ((M, K), (N, K)))
+    sa, sb = torch.rand(M, device="cuda") * 0.01, torch.rand(N, device="cuda") * 0.01
+    run = lambda: sk.streamk_int8_scaled(A, B, sa, sb, out_dtype=TYPES[out], activation=activation, **config)  # noqa: E731
+    clean = run()
+    sa[M // 2], sb[7] = math.nan, math.nan
+    C, bad = run(), torch.zeros(M, N, dtype=torch.bool, device="cuda")
+    bad[M // 2], bad[:, 7] = True, True
+    assert torch.equal(torch.isnan(C), bad) and torch.equal(C[~bad], clean[~bad])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 7, 40, 200])
+def test_other_products_keep_nan_through_relu(sk, M):
+    N, K = 256, 512
+    A = rand((M, K), torch.float16, 1)
+    A[M // 2, 3] = math.nan
+    q, s = sk.quantize_q4(rand((N, K), torch.float16, 2))
+    f8 = A.to(torch.float8_e4m3fn)
+    assert torch.isnan(f8[M // 2, 3].float())
+    for C in (sk.streamk_q4(A, q, s, activation="relu"), sk.streamk_fp8(f8, rand((N, K), torch.float16, 3).to(torch.float8_e4m3fn), activation="relu")):
+        bad = torch.isnan(C).all(1)
+        assert bad[M // 2] and bad.sum() == 1 and torch.isnan(C).any(1).sum() == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+@pytest.mark.parametrize("weights", ["float16", "bfloat16", "int8"])
+def test_a_bad_token_stays_bad_through_a_layer_of_experts(sk, activation, weights):
+    torch.manual_seed(0)
+    layer = sk.StreamKMoE(64, 96, 4, 2, activation=activation, weight_format="bfloat16" if weights == "int8" else weights, device="cuda")
+    layer = sk.StreamKMoE.quantized(layer) if weights == "int8" else layer
+    x = torch.randn(20, 64, device="cuda").to(layer.dtype)
+    with torch.no_grad():
+        # (the routes of the clean tokens: a NaN logit is never chosen, and such a token would go to no expert)
+        route, clean = layer.route(x), layer(x)
+        bad = x.clone()
+        bad[3, 7] = math.nan
+        layer.route = lambda rows: route
+        runs = [layer(bad)]
+    if weights != "int8":
+        runs.append(layer(bad.requires_grad_()).detach())   # (recorded: the activation is an operation of its own)
+    keep = torch.arange(20, device="cuda") != 3
+    for out in runs:
+        assert torch.isnan(out[3]).all() and torch.isfinite(out[keep]).all()
+    assert torch.equal(runs[0][keep], clean[keep])
