@@ -13,6 +13,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <initializer_list>
 #include <mutex>
 #include <optional>
 #include <shared_mutex>
@@ -245,6 +246,11 @@ using torch::autograd::variable_list;
   } while (0)
 void once() { TORCH_CHECK(!at::GradMode::is_enabled(), "streamk: these gradients are not differentiable again (create_graph)"); }
 bool wanted(const Tensor &t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+// (a dual tensor does not require a gradient: below autograd its tangent would be lost without a word)
+void no_tangent(const char *what, std::initializer_list<Tensor> operands) {
+  for (const Tensor &t : operands)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), "streamk: ", what, " has no forward-mode derivative");
+}
 
 struct GroupedProduct : torch::autograd::Function<GroupedProduct> {
   static Tensor forward(AutogradContext *ctx, const Tensor &A, const Tensor &B, const Tensor &offsets, std::string layout, int64_t variant) {
@@ -273,6 +279,7 @@ struct GroupedProduct : torch::autograd::Function<GroupedProduct> {
 };
 Tensor gemm_grouped_autograd(const Tensor &A, const Tensor &B, const Tensor &offsets, c10::string_view layout, MaybeType out_dtype, const MaybeTensor &scale_a,
                              const MaybeTensor &scale_b, const MaybeTensor &bias, c10::string_view activation, int64_t variant) {
+  no_tangent("the grouped product", {A, B, scale_a.value_or(Tensor()), scale_b.value_or(Tensor()), bias.value_or(Tensor())});
   const bool plain = !scale_a.has_value() && !scale_b.has_value() && !bias.has_value() && activation == "none" &&
                      (!out_dtype.has_value() || *out_dtype == A.scalar_type()) && (layout == "nt" || layout == "nn");
   if (plain && (wanted(A) || wanted(B))) return GroupedProduct::apply(A, B, offsets, std::string(layout.data(), layout.size()), variant);
@@ -299,6 +306,7 @@ struct RouteExperts : torch::autograd::Function<RouteExperts> {
   }
 };
 FiveTensors route_experts_autograd(const Tensor &logits, int64_t k) {
+  no_tangent("route_experts", {logits});
   if (!wanted(logits)) BELOW(route_experts, logits, k);
   const variable_list r = RouteExperts::apply(logits, k);
   return {r[0], r[1], r[2], r[3], r[4]};
@@ -320,6 +328,7 @@ struct DispatchRows : torch::autograd::Function<DispatchRows> {
   }
 };
 Tensor dispatch_routed_autograd(const Tensor &x, const Tensor &order, const Tensor &place) {
+  no_tangent("dispatch_rows", {x});
   if (wanted(x)) return DispatchRows::apply(x, order, place);
   BELOW(dispatch_routed, x, order, place);
 }
@@ -344,6 +353,7 @@ Tensor combine_routed(const Tensor &y, const Tensor &weights, const Tensor &orde
   return combine_rows(y, place, weights);
 }
 Tensor combine_routed_autograd(const Tensor &y, const Tensor &weights, const Tensor &order, const Tensor &place) {
+  no_tangent("combine_rows", {y, weights});
   if (wanted(y) || wanted(weights)) return CombineRows::apply(y, weights, order, place);
   BELOW(combine_routed, y, weights, order, place);
 }

@@ -5,8 +5,9 @@
     h = streamk_grouped(rows, up, route.offsets, activation="silu")      # each expert's rows times its own weights
     out = combine_rows(streamk_grouped(h, down, route.offsets), route)   # the weighted sum of each token's rows
 
-Every function is an operator of the `streamk` namespace and, under autograd, differentiable in its floating operands (the grouped
-product without bias and activation).  Sizes of groups stay on the device: no call waits for it.  Ordinary calls run, and record their
+Every function is an operator of the `streamk` namespace and, under autograd, differentiable (backward) in its floating operands but for
+`streamk_grouped_wgrad`, which is a gradient itself, and the grouped product with bias, activation or scales; forward-mode derivatives are
+refused.  Sizes of groups stay on the device: no call waits for it.  Ordinary calls run, and record their
 gradients, in native code (csrc/torch_ops_experts.cpp), which passes every other one on to the implementations here, registered as
 `<name>_general`; without the native library those and the autograd functions here stand in.
 """
@@ -30,6 +31,12 @@ def _operator(name, schema, run, fake):
         if suffix or not _NATIVE:
             ops._LIBRARY.impl(name + suffix, run, "CUDA")
     torch.library.register_fake(f"streamk::{name}", fake, lib=ops._LIBRARY)
+
+
+def _no_tangent(what, *operands):
+    """(the native library's autograd implementations refuse by themselves)"""
+    if not _NATIVE and any(isinstance(t, torch.Tensor) and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in operands):
+        raise NotImplementedError(f"streamk: {what} has no forward-mode derivative")
 
 
 def _on_device(t, name, dtypes, dims):
@@ -193,6 +200,7 @@ def streamk_grouped(A, B, offsets, *, layout="nt", scale_a=None, scale_b=None, o
     once.  Differentiable in A and B without bias, activation, scales and out.  variant: which tiles run (sk_grouped in streamk.h); 0
     lets the sizes decide."""
     activation = activation or "none"
+    _no_tangent("the grouped product", A, B, bias, scale_a, scale_b)
     if torch.is_grad_enabled() and (A.requires_grad or B.requires_grad or (bias is not None and bias.requires_grad)):
         if bias is not None or activation != "none" or scale_a is not None or scale_b is not None or out is not None:
             raise ValueError("the grouped product has gradients only without bias, activation, scales and out")
@@ -287,6 +295,7 @@ def route_experts(logits, k):
     """Route of the tokens whose router logits are [T, E] (float32, float16 or bfloat16): the k largest of each, the largest first, equal
     ones by number.  -inf and NaN are never chosen: a token with fewer others has -1 and weight 0 in its last places, and one with none
     goes to no expert.  Differentiable: weights to logits."""
+    _no_tangent("route_experts", logits)
     if not _NATIVE and torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
         return Route(*_RouteExperts.apply(logits, k))
     return Route(*_route_experts(logits, k))
@@ -387,6 +396,7 @@ class _CombineRows(torch.autograd.Function):
 def dispatch_rows(x, route):
     """The tokens' rows in the experts' order: [T k, H] for x [T, H] of any type (or [T k] for [T], such as the tokens' scales); zeros for
     the rows behind route.offsets[E].  Differentiable in x (float16 or bfloat16, two dimensions)."""
+    _no_tangent("dispatch_rows", x)
     if torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad:
         _on_device(x, "x", tuple(_TYPES), 2)
         if not _NATIVE:
@@ -397,6 +407,7 @@ def dispatch_rows(x, route):
 def combine_rows(y, route):
     """out[t] = sum over its experts of their weight times their row of y: [T, H] for y [T k, H] (float16 or bfloat16) in the experts' order;
     added in fp32, rounded once; a token without experts gets zeros.  Differentiable in y and route.weights."""
+    _no_tangent("combine_rows", y, route.weights)
     if not _NATIVE and torch.is_grad_enabled() and isinstance(y, torch.Tensor) and (y.requires_grad or route.weights.requires_grad):
         return _CombineRows.apply(y, route.weights, route.order, route.place)
     return _combine_routed(y, route.weights, route.order, route.place)

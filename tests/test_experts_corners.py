@@ -1,6 +1,10 @@
 """Operands, recordings and plans at the edge of what the operators for experts and int8 take.  Tolerances as in test_experts.py: fp32 sums
 of n terms within 2 n 2^-24 of the sum of the terms' magnitudes, one rounding to the result's type."""
 import math
+import os
+import subprocess
+import sys
+import textwrap
 
 import pytest
 import torch
@@ -210,3 +214,51 @@ def test_a_bad_token_stays_bad_through_a_layer_of_experts(sk, activation, weight
     for out in runs:
         assert torch.isnan(out[3]).all() and torch.isfinite(out[keep]).all()
     assert torch.equal(runs[0][keep], clean[keep])
+
+
+# ---- derivatives that do not exist are refused, in the native operators and in the ones that stand in for them ----
+PACKAGE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "stream-k.tvm_amd", "streamk")
+
+
+@pytest.fixture(params=["native", "without the native library"])
+def run_with_fakes(request, tmp_path):
+    """Runs code in a process of its own, under FakeTensorMode: operands A [10, 64], B [3, 32, 64], offsets, a route, and `new` for more."""
+    package = tmp_path / "streamk"
+    package.mkdir()
+    for name in os.listdir(PACKAGE):
+        if name != "__pycache__" and (request.param == "native" or name != "libstreamk_torch.so"):
+            (package / name).symlink_to(os.path.join(PACKAGE, name))
+    head = f"""
+        import sys
+        sys.path.insert(0, {str(tmp_path)!r})
+        import torch, streamk as sk, streamk.experts as experts
+        import torch.autograd.forward_ad as fw
+        from torch._subclasses.fake_tensor import FakeTensorMode
+        assert experts._NATIVE == {request.param == "native"}
+        FakeTensorMode().__enter__()
+        new = lambda *s, dtype=torch.float16: torch.empty(*s, dtype=dtype, device="cuda")
+        A, B, offsets, logits = new(10, 64), new(3, 32, 64), new(4, dtype=torch.int32), new(5, 4, dtype=torch.float32)
+        route = sk.route_experts(logits, 2)
+        def refused(error, f):
+            try:
+                f()
+            except error as e:
+                return str(e)
+            raise SystemExit("not refused")
+        """
+    env = {**os.environ, "PYTHONDONTWRITEBYTECODE": "1"}
+    return lambda code: subprocess.run([sys.executable, "-c", textwrap.dedent(head) + textwrap.dedent(code)], check=True, timeout=100, env=env)
+
+
+def test_forward_mode_is_refused(run_with_fakes):
+    run_with_fakes("""
+        with fw.dual_level():
+            dual = lambda t: fw.make_dual(t, t.clone())
+            for f in (lambda: sk.streamk_grouped(dual(A), B, offsets), lambda: sk.streamk_grouped(A, dual(B), offsets),
+                      lambda: sk.streamk_grouped(A, B, offsets, bias=dual(new(3, 32)), activation="silu"),
+                      lambda: sk.route_experts(dual(logits), 2), lambda: sk.dispatch_rows(dual(new(5, 64)), route),
+                      lambda: sk.combine_rows(dual(A), route), lambda: sk.combine_rows(A, route._replace(weights=dual(route.weights)))):
+                assert "forward-mode" in refused(NotImplementedError, f)
+            sk.streamk_grouped(A, B, offsets)
+        refused(NotImplementedError, lambda: torch.func.jvp(lambda a: sk.streamk_grouped(a, B, offsets), (A,), (A.clone(),)))
+        """)
