@@ -19,6 +19,7 @@
 #include <shared_mutex>
 #include <string>
 #include <tuple>
+#include <vector>
 
 #include "streamk.h"
 #include "torch_ops.h"
@@ -252,6 +253,15 @@ void no_tangent(const char *what, std::initializer_list<Tensor> operands) {
     TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), "streamk: ", what, " has no forward-mode derivative");
 }
 
+// Passes a result on; who asks for its derivative by one of the operands that require one gets an error with the reason.
+struct Refused : torch::autograd::Function<Refused> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &result, at::TensorList, const std::string &why) {
+    ctx->saved_data["why"] = why;
+    return result;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list) { TORCH_CHECK(false, "streamk: ", ctx->saved_data["why"].toStringRef()); }
+};
+
 struct GroupedProduct : torch::autograd::Function<GroupedProduct> {
   static Tensor forward(AutogradContext *ctx, const Tensor &A, const Tensor &B, const Tensor &offsets, std::string layout, int64_t variant) {
     at::AutoDispatchBelowADInplaceOrView guard;
@@ -283,7 +293,12 @@ Tensor gemm_grouped_autograd(const Tensor &A, const Tensor &B, const Tensor &off
   const bool plain = !scale_a.has_value() && !scale_b.has_value() && !bias.has_value() && activation == "none" &&
                      (!out_dtype.has_value() || *out_dtype == A.scalar_type()) && (layout == "nt" || layout == "nn");
   if (plain && (wanted(A) || wanted(B))) return GroupedProduct::apply(A, B, offsets, std::string(layout.data(), layout.size()), variant);
-  BELOW(gemm_grouped, A, B, offsets, layout, out_dtype, scale_a, scale_b, bias, activation, variant);
+  const auto below = [&]() -> Tensor { BELOW(gemm_grouped, A, B, offsets, layout, out_dtype, scale_a, scale_b, bias, activation, variant); };
+  std::vector<Tensor> recorded;
+  for (const Tensor *t : {&A, &B, scale_a ? &*scale_a : nullptr, scale_b ? &*scale_b : nullptr, bias ? &*bias : nullptr})
+    if (t && wanted(*t)) recorded.push_back(*t);
+  if (recorded.empty()) return below();
+  return Refused::apply(below(), at::TensorList(recorded), "the grouped product has gradients only without bias, activation, scales and out");
 }
 
 struct RouteExperts : torch::autograd::Function<RouteExperts> {

@@ -262,3 +262,27 @@ def test_forward_mode_is_refused(run_with_fakes):
             sk.streamk_grouped(A, B, offsets)
         refused(NotImplementedError, lambda: torch.func.jvp(lambda a: sk.streamk_grouped(a, B, offsets), (A,), (A.clone(),)))
         """)
+
+
+@pytest.mark.gpu
+def test_a_product_without_gradients_says_so(sk):
+    """Bias, activation and scales of a recorded call: the operator's result has a derivative that raises, not none."""
+    o, offsets = torch.ops.streamk, offsets_of([12, 8])
+    A, B, bias = rand((20, 64), torch.float16, 1), rand((2, 32, 64), torch.float16, 2), rand((2, 32), torch.float16, 3)
+    q, s = sk.quantize_int8(A)
+    w, sw = sk.quantize_int8(B)
+    a, b, c, t = (x.clone().requires_grad_() for x in (A, B, bias, sw))
+    calls = [((a, B, offsets, "nt", None, None, None, None, "silu"), (A, B, offsets, "nt", None, None, None, None, "silu")),
+             ((A, b, offsets, "nt", None, None, None, bias, "none"), (A, B, offsets, "nt", None, None, None, bias, "none")),
+             ((A, B, offsets, "nt", None, None, None, c, "relu"), (A, B, offsets, "nt", None, None, None, bias, "relu")),
+             ((q, w, offsets, "nt", None, s, t), (q, w, offsets, "nt", None, s, sw))]
+    for recorded, ordinary in calls:
+        want, got = o.gemm_grouped(*ordinary), o.gemm_grouped(*recorded)
+        assert got.requires_grad and not want.requires_grad and torch.equal(got, want)
+        with pytest.raises(RuntimeError, match="has gradients only without bias"):
+            got.sum().backward()
+        with torch.no_grad():
+            assert not o.gemm_grouped(*recorded).requires_grad
+    # (what is not differentiated runs on: int8 scales that a recorded quantiser has made)
+    q, s = sk.quantize_int8(a)
+    assert torch.equal(sk.streamk_grouped(q, w, offsets, scale_a=s, scale_b=sw), o.gemm_grouped(q, w, offsets, "nt", None, s.detach(), sw))
