@@ -245,7 +245,6 @@ using torch::autograd::variable_list;
     at::AutoDispatchBelowADInplaceOrView guard;      \
     return handle.call(__VA_ARGS__);                 \
   } while (0)
-void once() { TORCH_CHECK(!at::GradMode::is_enabled(), "streamk: these gradients are not differentiable again (create_graph)"); }
 bool wanted(const Tensor &t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 // (a dual tensor does not require a gradient: below autograd its tangent would be lost without a word)
 void no_tangent(const char *what, std::initializer_list<Tensor> operands) {
@@ -262,6 +261,12 @@ struct Refused : torch::autograd::Function<Refused> {
   static variable_list backward(AutogradContext *ctx, variable_list) { TORCH_CHECK(false, "streamk: ", ctx->saved_data["why"].toStringRef()); }
 };
 
+// A gradient made of these tensors, which is not differentiable again (of interest with create_graph only).
+Tensor once(const Tensor &gradient, std::initializer_list<Tensor> of) {
+  if (!gradient.defined() || !at::GradMode::is_enabled()) return gradient;
+  return Refused::apply(gradient, at::TensorList(of), "the gradients of the operators for experts are not differentiable again");
+}
+
 struct GroupedProduct : torch::autograd::Function<GroupedProduct> {
   static Tensor forward(AutogradContext *ctx, const Tensor &A, const Tensor &B, const Tensor &offsets, std::string layout, int64_t variant) {
     at::AutoDispatchBelowADInplaceOrView guard;
@@ -271,7 +276,6 @@ struct GroupedProduct : torch::autograd::Function<GroupedProduct> {
     return product.call(A, B, offsets, layout, c10::nullopt, c10::nullopt, c10::nullopt, c10::nullopt, "none", variant);
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
-    once();
     static const auto product = OP(gemm_grouped);
     static const auto wgrad = OP(grouped_wgrad);
     const auto saved = ctx->get_saved_variables();
@@ -279,12 +283,13 @@ struct GroupedProduct : torch::autograd::Function<GroupedProduct> {
     if (!dC.defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     const bool nn = ctx->saved_data["nn"].toBool();
     Tensor dA, dB;
-    if (ctx->needs_input_grad(0)) {
+    {
+      at::AutoDispatchBelowADInplaceOrView guard;
       // ('nt': dC [R, N] times B[e] [N, K], any N)
-      dA = product.call(dC, B, offsets, nn ? "nt" : "nn", c10::nullopt, c10::nullopt, c10::nullopt, c10::nullopt, "none", 0);
+      if (ctx->needs_input_grad(0)) dA = product.call(dC, B, offsets, nn ? "nt" : "nn", c10::nullopt, c10::nullopt, c10::nullopt, c10::nullopt, "none", 0);
+      if (ctx->needs_input_grad(1)) dB = nn ? wgrad.call(A, dC, offsets, 0) : wgrad.call(dC, A, offsets, 0);
     }
-    if (ctx->needs_input_grad(1)) dB = nn ? wgrad.call(A, dC, offsets, 0) : wgrad.call(dC, A, offsets, 0);
-    return {dA, dB, Tensor(), Tensor(), Tensor()};
+    return {once(dA, {dC, B}), once(dB, {dC, A}), Tensor(), Tensor(), Tensor()};
   }
 };
 Tensor gemm_grouped_autograd(const Tensor &A, const Tensor &B, const Tensor &offsets, c10::string_view layout, MaybeType out_dtype, const MaybeTensor &scale_a,
@@ -313,11 +318,15 @@ struct RouteExperts : torch::autograd::Function<RouteExperts> {
     return {std::get<0>(r), std::get<1>(r), std::get<2>(r), std::get<3>(r), std::get<4>(r)};
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
-    once();
     static const auto back = OP(route_backward);
     const auto saved = ctx->get_saved_variables();
     if (!grads[0].defined()) return {Tensor(), Tensor()};
-    return {back.call(saved[0], saved[1], grads[0], ctx->saved_data["E"].toInt(), (at::ScalarType)ctx->saved_data["dtype"].toInt()), Tensor()};
+    Tensor dlogits;
+    {
+      at::AutoDispatchBelowADInplaceOrView guard;
+      dlogits = back.call(saved[0], saved[1], grads[0], ctx->saved_data["E"].toInt(), (at::ScalarType)ctx->saved_data["dtype"].toInt());
+    }
+    return {once(dlogits, {saved[0], grads[0]}), Tensor()};
   }
 };
 FiveTensors route_experts_autograd(const Tensor &logits, int64_t k) {
@@ -336,10 +345,14 @@ struct DispatchRows : torch::autograd::Function<DispatchRows> {
     return dispatch.call(x, order, place);
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
-    once();
     static const auto combine = OP(combine_rows);
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
-    return {combine.call(grads[0], ctx->get_saved_variables()[0], c10::nullopt), Tensor(), Tensor()};
+    Tensor dx;
+    {
+      at::AutoDispatchBelowADInplaceOrView guard;
+      dx = combine.call(grads[0], ctx->get_saved_variables()[0], c10::nullopt);
+    }
+    return {once(dx, {grads[0]}), Tensor(), Tensor()};
   }
 };
 Tensor dispatch_routed_autograd(const Tensor &x, const Tensor &order, const Tensor &place) {
@@ -356,12 +369,15 @@ struct CombineRows : torch::autograd::Function<CombineRows> {
     return combine.call(y, place, weights);
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
-    once();
     static const auto back = OP(combine_backward);
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
-    const auto [dy, dw] = back.call(grads[0], saved[0], saved[2], saved[3], saved[1]);
-    return {dy, dw, Tensor(), Tensor()};
+    Tensor dy, dw;
+    {
+      at::AutoDispatchBelowADInplaceOrView guard;
+      std::tie(dy, dw) = back.call(grads[0], saved[0], saved[2], saved[3], saved[1]);
+    }
+    return {once(dy, {grads[0], saved[1]}), once(dw, {grads[0], saved[0]}), Tensor(), Tensor()};
   }
 };
 Tensor combine_routed(const Tensor &y, const Tensor &weights, const Tensor &order, const Tensor &place) {

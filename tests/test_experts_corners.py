@@ -286,3 +286,42 @@ def test_a_product_without_gradients_says_so(sk):
     # (what is not differentiated runs on: int8 scales that a recorded quantiser has made)
     q, s = sk.quantize_int8(a)
     assert torch.equal(sk.streamk_grouped(q, w, offsets, scale_a=s, scale_b=sw), o.gemm_grouped(q, w, offsets, "nt", None, s.detach(), sw))
+
+
+@pytest.mark.gpu
+def test_gradients_with_create_graph(sk):
+    """create_graph gives the gradients; only differentiating them again is refused, by whatever they were made of."""
+    offsets, logits = offsets_of([12, 8]), rand((10, 4), torch.float32, 4)
+    A, B, x, y = rand((20, 64), torch.float16, 1), rand((2, 32, 64), torch.float16, 2), rand((10, 64), torch.float16, 3), rand((20, 64), torch.float16, 5)
+    route = sk.route_experts(logits, 2)
+    A, B, logits, x, y = (t.requires_grad_() for t in (A, B, logits, x, y))
+    weights = route.weights.clone().requires_grad_()
+    calls = [(lambda: sk.streamk_grouped(A, B, offsets), (A, B)), (lambda: sk.streamk_grouped(A, B.transpose(1, 2).contiguous(), offsets, layout="nn"), (A, B)),
+             (lambda: sk.route_experts(logits, 2).weights, (logits,)), (lambda: sk.dispatch_rows(x, route), (x,)),
+             (lambda: sk.combine_rows(y, route._replace(weights=weights)), (y, weights))]
+    for call, leaves in calls:
+        d = rand(call().shape, call().dtype, 7)
+        want = torch.autograd.grad(call(), leaves, d)
+        for g, w in zip(torch.autograd.grad(call(), leaves, d, create_graph=True), want):
+            assert torch.equal(g, w)
+        # the incoming gradient requires one
+        d = d.requires_grad_()
+        got = torch.autograd.grad(call(), leaves, d, create_graph=True)
+        for i, (g, w) in enumerate(zip(got, want)):
+            assert torch.equal(g, w) and g.requires_grad
+            with pytest.raises(RuntimeError, match="not differentiable again"):
+                torch.autograd.grad(g.float().sum(), d, retain_graph=True)
+    # dB is made of A, dA of B
+    dA, dB = torch.autograd.grad(sk.streamk_grouped(A, B, offsets), (A, B), d_of(A, B), create_graph=True)
+    for g, leaf in ((dA, B), (dB, A)):
+        with pytest.raises(RuntimeError, match="not differentiable again"):
+            torch.autograd.grad(g.float().sum(), leaf, retain_graph=True)
+    # a penalty on another layer's gradient
+    z = rand((20, 64), torch.float32, 8).requires_grad_()
+    loss = (sk.streamk_grouped(A, B, offsets).float().sum() + z.pow(3).sum())
+    _, gz = torch.autograd.grad(loss, (A, z), create_graph=True)
+    assert torch.allclose(torch.autograd.grad(gz.sum(), z)[0], 6 * z)
+
+
+def d_of(A, B):
+    return rand((A.shape[0], B.shape[1]), A.dtype, 9)
