@@ -402,7 +402,8 @@ int sk_q4_quantize(const void *W, int64_t N, int64_t K, int64_t ldw, int group, 
  * scale for each row of A (token) and of B (output channel), C fp16 or bfloat16 (ldc in its elements).  The sums are exact int32 (up to
  * K = 131071 whatever the values); each becomes fp32 (rounded beyond 24 bits), is multiplied by a[m], then by b[n], and rounded once to C's type behind bias (C's
  * type) and activation.  The plan is made with dtype SK_I8 as for sk_gemm_i8; SK_ERR_CONFIG for plans of kernels that have no form
- * with scales (the general small-M kernels: a plan of up to 64 rows is made with reserved[0] = 9 or 12).  Every schedule and
+ * with scales (the general small-M kernels: a plan of up to 64 rows is made with reserved[0] = 9 or 12; sk_i8_scaled_takes says whether
+ * it would run, 1 or 0).  Every schedule and
  * fix-up gives the same bits.  Alignment as for sk_gemm_i8; C 2-byte, the scales 4-byte aligned.
  *
  * sk_quantize_i8: rows of X (SK_F16 or SK_BF16, row pitch ldx elements, M x K) to int8 Q (pitch ldq) and one fp32 scale a row:
@@ -417,6 +418,7 @@ typedef struct sk_scales {
 } sk_scales;
 int sk_gemm_i8_scaled(const void *A, const void *B, void *C, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t ldc,
                       const sk_scales *scales, const sk_plan *plan, void *ws, size_t ws_bytes, void *stream, const sk_epilogue *epi);
+int sk_i8_scaled_takes(const sk_plan *plan);
 int sk_quantize_i8(const void *X, int dtype, int64_t M, int64_t K, int64_t ldx, void *Q, int64_t ldq, void *scales, void *stream);
 
 /*

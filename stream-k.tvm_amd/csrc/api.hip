@@ -501,6 +501,14 @@ extern "C" int sk_gemm_i8(const void *A, const void *B, void *C, int64_t M, int6
   return gemm_8bit(SK_I8, A, B, C, M, N, K, lda, ldb, ldc, 1.f, plan, ws, ws_bytes, stream);
 }
 
+extern "C" int sk_i8_scaled_takes(const sk_plan *plan) {
+  if (!plan || plan->dtype != SK_I8 || plan->layout != SK_LAYOUT_NT || !has_scaled_i8(plan->kernel_id)) return 0;
+  const DeviceInfo d = device_info();
+  if (!d.ok || plan->streamk_tiles == 0 || !is_reduce(plan->fixup)) return 1;
+  const int occupancy = cached_occupancy(plan->kernel_id, 3);   // (as make_dev_plan asks)
+  return occupancy > 0 && plan->grid <= d.cus * occupancy;
+}
+
 extern "C" int sk_gemm_i8_scaled(const void *A, const void *B, void *C, int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb,
                                  int64_t ldc, const sk_scales *scales, const sk_plan *plan, void *ws, size_t ws_bytes, void *stream,
                                  const sk_epilogue *epi) {

@@ -105,6 +105,16 @@ static int launch_scaled_policy(const GemmArgs &g, const Scales &sc, const DevPl
   return (int)hipGetLastError();
 }
 
+bool has_scaled_i8(int id) {
+  switch (id) {
+#define F(ID, P) case ID:
+    FOR_SCALED_KERNELS
+#undef F
+    return true;
+  }
+  return has_scaled_i8_asm(id);
+}
+
 int launch_scaled_i8(int id, const GemmArgs &a, const Scales &sc, const DevPlan &p, const Workspace &ws, hipStream_t s, const void *bias) {
   switch (id) {
 #define F(ID, P) case ID: return launch_scaled_policy<unparen<void P>::type>(a, sc, p, ws, s, bias);

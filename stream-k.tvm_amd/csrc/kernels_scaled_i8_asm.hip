@@ -13,6 +13,8 @@ __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_scaled_asm_kernel(t
   run_persistent<P, FIXUP, true>(a, plan, ws, smem, bias);
 }
 
+bool has_scaled_i8_asm(int id) { return id == ASM_I8_ID; }
+
 int launch_scaled_i8_asm(int id, const GemmArgs &g, const Scales &sc, const DevPlan &p, const Workspace &ws, hipStream_t s, const void *bias) {
   if (id != ASM_I8_ID) return (int)hipErrorInvalidValue;
   ScaledAsm::Args a;

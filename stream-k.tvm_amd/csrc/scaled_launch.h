@@ -5,9 +5,11 @@
 
 namespace sk {
 
+bool has_scaled_i8(int id);
 // hipError_t as int (hipErrorInvalidValue: an id without an instance); co-resident CTAs per CU, 0 without an instance
 int launch_scaled_i8(int id, const GemmArgs &a, const Scales &sc, const DevPlan &p, const Workspace &ws, hipStream_t s, const void *bias);
 int occupancy_scaled_i8(int id);
+bool has_scaled_i8_asm(int id);
 int launch_scaled_i8_asm(int id, const GemmArgs &a, const Scales &sc, const DevPlan &p, const Workspace &ws, hipStream_t s, const void *bias);
 int occupancy_scaled_i8_asm(int id);
 

@@ -138,6 +138,7 @@ def lib():
               "sk_q4_untile_host", "sk_q4_tile"):
         getattr(L, f).restype = ci
     L.sk_gemm_i8_scaled.argtypes = [vp, vp, vp, i64, i64, i64, i64, i64, i64, P(SkScales), P(SkPlan), vp, sz, vp, P(SkEpilogue)]
+    L.sk_i8_scaled_takes.argtypes = [P(SkPlan)]
     L.sk_quantize_i8.argtypes = [vp, ci, i64, i64, i64, vp, i64, vp, vp]
     L.sk_gemm_grouped.argtypes = [P(SkGrouped), vp, sz, vp]
     L.sk_grouped_workspace_bytes.argtypes = [P(SkGrouped)]
@@ -150,7 +151,7 @@ def lib():
     L.sk_dispatch_rows.argtypes = [vp, i64, i64, vp, vp, i64, i64, vp, vp]
     L.sk_combine_rows.argtypes = [vp, ci, vp, vp, i64, i64, i64, vp, vp]
     L.sk_combine_backward.argtypes = [vp, vp, ci, vp, vp, vp, i64, i64, i64, vp, vp, vp]
-    for f in ("sk_gemm_i8_scaled", "sk_quantize_i8", "sk_gemm_grouped", "sk_grouped_wgrad", "sk_route_experts", "sk_route_backward",
+    for f in ("sk_gemm_i8_scaled", "sk_i8_scaled_takes", "sk_quantize_i8", "sk_gemm_grouped", "sk_grouped_wgrad", "sk_route_experts", "sk_route_backward",
               "sk_dispatch_rows", "sk_combine_rows", "sk_combine_backward"):
         getattr(L, f).restype = ci
     for f in ("sk_device_info", "sk_make_plan", "sk_plan_cta_range", "sk_plan_tile_coords",

@@ -23,6 +23,16 @@ def _check_out_dtype(dtype):
         raise ValueError("out_dtype must be torch.float16 or torch.bfloat16")
 
 
+def plan_for(config, M, N, K, pitch_a=0, pitch_b=0):
+    """The plan of an int8 product with scales: that of the int32 product, but for tuned entries of kernels that have no form with
+    scales (a search of up to 64 rows may end with one), which do not count here."""
+    plan = ops._plan_for(config, M, N, K, "int8", "nt", pitch_a, pitch_b)
+    if config != "" or _lib.lib().sk_i8_scaled_takes(ctypes.byref(plan)):
+        return plan
+    plan = ops._plan_of(ops._UNTUNED, M, N, K, "int8", "nt")
+    return plan if ops._takes_rows(plan, pitch_a, pitch_b) else ops._plan_of(ops._UNTUNED_LONG_ROWS, M, N, K, "int8", "nt")
+
+
 def _run_i8_scaled(A, B, scale_a, scale_b, C, out_dtype, config="", bias=None, activation="none"):
     _check_out_dtype(out_dtype)
     A = ops._aligned_rows(A)
@@ -35,7 +45,7 @@ def _run_i8_scaled(A, B, scale_a, scale_b, C, out_dtype, config="", bias=None, a
     _check_scale(scale_a, "scale_a", M, A.device)
     _check_scale(scale_b, "scale_b", N, A.device)
     ops._check_out(C, M, N, out_dtype)
-    plan = ops._plan_for(config, M, N, K, "int8", "nt", A.stride(0), B.stride(0))
+    plan = plan_for(config, M, N, K, A.stride(0), B.stride(0))
     epi = ops._epilogue(bias, N, out_dtype, A.device, ops._act(activation))
     scales = _lib.SkScales(a=scale_a.data_ptr(), b=scale_b.data_ptr(), out_dtype=_OUT_TYPES[out_dtype])
     rc = _lib.lib().sk_gemm_i8_scaled(A.data_ptr(), B.data_ptr(), C.data_ptr(), M, N, K, A.stride(0), B.stride(0), C.stride(0),

@@ -9,7 +9,7 @@ is in it.  Inference only: the GEMM is not recorded by autograd.
 """
 import torch
 
-from . import ops
+from . import int8, ops
 from .int8 import quantize_int8
 from .plan import make_plan, operator_config
 
@@ -86,7 +86,7 @@ class StreamKLinear(torch.nn.Module):
         N, K, dtype = self.out_features, self.in_features, self.weight_format
         if dtype in ("q4", "q4_zp") and ops._dequantises(M, N, K, dtype == "q4_zp"):
             return make_plan(M, N, K, dtype, "nt", operator_config(M, N, K, dtype, "nt") if dtype == "q4_zp" else None)
-        return ops._plan_for("", M, N, K, dtype, "nt")
+        return int8.plan_for("", M, N, K) if dtype == "int8" else ops._plan_for("", M, N, K, dtype, "nt")
 
     @torch.no_grad()
     def forward(self, x):

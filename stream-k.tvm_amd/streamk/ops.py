@@ -149,6 +149,8 @@ def _takes_rows(plan, pitch_a, pitch_b):
 # configuration of a call that names none and whose rows are too far apart for the plan of "": see operator_config (no string, so that
 # no caller's is taken for it)
 _LONG_ROWS = ("long rows",)
+# the same without the tuned cache, for calls that do not take the plan of an entry
+_UNTUNED, _UNTUNED_LONG_ROWS = ("untuned",), ("untuned", "long rows")
 
 
 def _plan_of(config, M, N, K, dtype, layout):
@@ -158,9 +160,12 @@ def _plan_of(config, M, N, K, dtype, layout):
     key = (M, N, K, dtype, layout, config, generation, device)
     plan = _plan_cache.get(key)
     if plan is None:
-        named = config not in ("", _LONG_ROWS)
-        plan = make_plan(M, N, K, dtype, layout,
-                         _parse_config(config) if named else _plan_mod.operator_config(M, N, K, dtype, layout, config == _LONG_ROWS))
+        if config in (_UNTUNED, _UNTUNED_LONG_ROWS):
+            plan = make_plan(M, N, K, dtype, layout, _plan_mod.untuned_operator_config(M, dtype, layout, config == _UNTUNED_LONG_ROWS), use_tuned=False)
+        else:
+            named = config not in ("", _LONG_ROWS)
+            plan = make_plan(M, N, K, dtype, layout,
+                             _parse_config(config) if named else _plan_mod.operator_config(M, N, K, dtype, layout, config == _LONG_ROWS))
         if len(_plan_cache) < 4096:
             _plan_cache[key] = plan
             if config == "":   # from now on the native implementation answers calls of this shape

@@ -1,7 +1,9 @@
 """Operands, recordings and plans at the edge of what the operators for experts and int8 take.  Tolerances as in test_experts.py: fp32 sums
 of n terms within 2 n 2^-24 of the sum of the terms' magnitudes, one rounding to the result's type."""
+import ctypes
 import math
 import os
+import random
 import subprocess
 import sys
 import textwrap
@@ -325,3 +327,100 @@ def test_gradients_with_create_graph(sk):
 
 def d_of(A, B):
     return rand((A.shape[0], B.shape[1]), A.dtype, 9)
+
+
+# ---- int8 products with scales and the tuned cache of the int32 ones ----
+@pytest.fixture
+def tuned(sk, monkeypatch):
+    """entries(M, N, K, config) puts an int8 entry of the newest search into the tuned cache, for this test."""
+    from streamk import ops
+    from streamk import plan as plan_mod
+
+    def enter(M, N, K, config):
+        plan_mod.invalidate_tuned_cache()
+        monkeypatch.setattr(plan_mod, "_tuned", {f"gfx950/int8/nt/{M}x{N}x{K}": {"config": config, "search": sys.modules["streamk.autotune"].SEARCH}})
+        ops._plan_cache.clear()
+    yield enter
+    monkeypatch.undo()
+    plan_mod.invalidate_tuned_cache()
+    ops._plan_cache.clear()
+
+
+def test_plans_without_scales_are_not_taken_from_the_tuned_cache(sk, tuned, monkeypatch):
+    from streamk import int8, ops
+    from streamk import plan as plan_mod
+    monkeypatch.setattr(plan_mod, "num_cus", lambda: 256)
+    takes = lambda p: sk.lib().sk_i8_scaled_takes(ctypes.byref(p))  # noqa: E731
+    refused = 0
+    for M, N, K in ((1, 4096, 4096), (16, 4096, 4096), (20, 520, 1040), (64, 2048, 8192), (100, 4096, 4096), (700, 1031, 2064)):
+        for config in sk.candidate_configs(M, N, K, "int8", cus=256):
+            try:
+                plan = sk.make_plan(M, N, K, "int8", "nt", config)
+            except sk.StreamKError:
+                continue
+            if takes(plan):
+                continue
+            refused += 1
+            tuned(M, N, K, config)
+            assert ops._plan_for("", M, N, K, "int8", "nt").kernel_id == plan.kernel_id   # (the int32 product's)
+            for pitch in (0, 1 << 25):
+                own = int8.plan_for("", M, N, K, pitch, pitch)
+                assert takes(own) and (own.M, own.N, own.K) == (M, N, K) and own.kernel_id != plan.kernel_id
+            assert int8.plan_for("variant=1", M, N, K).kernel_id == sk.make_plan(M, N, K, "int8", "nt", variant=1).kernel_id   # (what a caller names stays)
+            assert takes(sk.StreamKLinear(K, N, weight_format="int8").plan_for(M))
+    assert refused > 50
+
+
+def test_untuned_plans_have_a_form_with_scales(sk, monkeypatch):
+    from streamk import ops
+    from streamk import plan as plan_mod
+    monkeypatch.setattr(plan_mod, "num_cus", lambda: 256)
+    rng = random.Random(5)
+    for _ in range(400):
+        M, N, K = (int(math.exp(rng.uniform(0, math.log(top)))) for top in (9000, 30000, 1200))
+        for config in (ops._UNTUNED, ops._UNTUNED_LONG_ROWS):
+            plan = ops._plan_of(config, M, N, 16 * K, "int8", "nt")
+            assert sk.lib().sk_i8_scaled_takes(ctypes.byref(plan)), (M, N, 16 * K, sk.kernel_name(plan.kernel_id))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K,config", [(16, 512, 1024, dict(bm=16, bn=16, bk=1024, schedule="dp")), (3, 260, 4096, dict(bm=16, bn=32, bk=1024, schedule="sk2", grid=256, fixup="reduce")),
+                                          (60, 512, 1024, dict(bm=64, bn=64, bk=512, schedule="dp"))])
+def test_int8_calls_after_a_search(sk, tuned, M, N, K, config):
+    from streamk import ops
+    assert not sk.lib().sk_i8_scaled_takes(ctypes.byref(sk.make_plan(M, N, K, "int8", "nt", config)))
+    g = torch.Generator().manual_seed(1)
+    A, B = (torch.randint(-127, 128, s, generator=g, dtype=torch.int8).cuda() for s in ((M, K), (N, K)))
+    sa, sb = torch.rand(M, device="cuda") * 0.01, torch.rand(N, device="cuda") * 0.01
+    run = lambda: sk.streamk_int8_scaled(A, B, sa, sb)  # noqa: E731
+    want = run()
+    layer = sk.StreamKLinear.from_linear(torch.nn.Linear(K, N, device="cuda", dtype=torch.float16), weight_format="int8")
+    x = torch.randn(M, K, device="cuda").half()
+    y = layer(x)
+    tuned(M, N, K, config)
+    for _ in range(2):   # (the second time the native operator knows the int32 product's plan)
+        assert torch.equal(sk.streamk_int8(A, B).double(), A.double() @ B.double().T)
+        assert torch.equal(run(), want) and torch.equal(layer(x), y)
+    assert ops._plan_for("", M, N, K, "int8", "nt").kernel_id == sk.make_plan(M, N, K, "int8", "nt", config).kernel_id
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(16, 512, 1024), (64, 512, 4096), (200, 512, 2048), (600, 1024, 1024)])
+def test_every_plan_that_is_said_to_run_does(sk, M, N, K):
+    g = torch.Generator().manual_seed(1)
+    A, B = (torch.randint(-127, 128, s, generator=g, dtype=torch.int8).cuda() for s in ((M, K), (N, K)))
+    sa, sb = torch.rand(M, device="cuda") * 0.01, torch.rand(N, device="cuda") * 0.01
+    want, ran = sk.streamk_int8_scaled(A, B, sa, sb), 0
+    for config in sk.candidate_configs(M, N, K, "int8"):
+        try:
+            plan = sk.make_plan(M, N, K, "int8", "nt", config)
+        except sk.StreamKError:
+            continue
+        if sk.lib().sk_i8_scaled_takes(ctypes.byref(plan)):
+            assert torch.equal(sk.streamk_int8_scaled(A, B, sa, sb, plan=plan), want), config
+            ran += 1
+        else:
+            with pytest.raises(sk.StreamKError):
+                sk.streamk_int8_scaled(A, B, sa, sb, plan=plan)
+    sk.workspace_status()
+    assert ran > 10
