@@ -432,7 +432,9 @@ int sk_quantize_i8(const void *X, int dtype, int64_t M, int64_t K, int64_t ldx, 
  * no content of theirs leads outside the operands.  B: E matrices, expert_b elements apart, each [N, K] (SK_LAYOUT_NT, pitch ldb) or
  * [K, N] (SK_LAYOUT_NN, 16-bit types).  bias: [E, N] in C's type, contiguous, or null.  lda, ldb and expert_b multiples of 8 (int8:
  * 16), SK_LAYOUT_NT: K too; SK_LAYOUT_NN: N too, and where K is none, A has zeros in its columns from K to the next; A and B 16-byte, C and bias 2-byte, scales 4-byte aligned.  The same bits on every launch.
- * ws: as for the other products (sk_workspace_init has run on it); no launch waits for part of itself.
+ * ws: as for the other products (sk_workspace_init has run on it).  Variant 2 may cut a tile along K; the CTA that comes last to it waits
+ * for the others' stores, spin_limit polls at most.  If it gives up, the tile is not stored and sk_workspace_status says
+ * SK_ERR_TIMEOUT.  No other variant waits for part of itself.
  *
  * sk_grouped_wgrad: C[e] = sum over the rows r of group e of A[r]^T B[r] with A [R, M] and B [R, N] in SK_F16 or SK_BF16, C [E, M, N]
  * contiguous in that type, sums in fp32; a group without rows gives zeros.  With A the gradient of a grouped product's result and B
@@ -451,7 +453,7 @@ typedef struct sk_grouped {
   int64_t variant;                                /* the tiles: 0 by size; 1: 128 x 128; 2: 256 x 256 (K a multiple of
                                                      64, int8: 128); 3 to 6: 16 x 64, 32 x 64, 64 x 64, 64 x 128,
                                                      whose waves stream K on their own (SK_LAYOUT_NN: only 64 x 64) */
-  int64_t reserved;                               /* 0 */
+  int64_t spin_limit;                             /* 0: 2^22 polls; negative: none (to test the way out) */
 } sk_grouped;
 size_t sk_grouped_workspace_bytes(const sk_grouped *g);   /* for this shape and variant, on the current device; 0 is possible */
 int sk_gemm_grouped(const sk_grouped *g, void *ws, size_t ws_bytes, void *stream);

@@ -20,7 +20,7 @@ static int check_shape(const sk_grouped *g, GroupedShape *h) {
   if (!i8 && g->dtype != SK_F16 && g->dtype != SK_BF16) return SK_ERR_CONFIG;
   if ((!nn && g->layout != SK_LAYOUT_NT) || (nn && i8)) return SK_ERR_CONFIG;
   if (i8 ? g->out_dtype != SK_F16 && g->out_dtype != SK_BF16 : g->out_dtype != g->dtype) return SK_ERR_CONFIG;
-  if (g->activation < SK_ACT_NONE || g->activation > SK_ACT_SILU || g->variant < 0 || g->reserved) return SK_ERR_CONFIG;
+  if (g->activation < SK_ACT_NONE || g->activation > SK_ACT_SILU || g->variant < 0) return SK_ERR_CONFIG;
   if (g->E <= 0 || g->R <= 0 || g->N <= 0 || g->K <= 0 || g->E > (1 << 20) || g->R > MAX_INT || g->N > MAX_INT || g->K > MAX_INT) return SK_ERR_SHAPE;
   if (g->lda < (nn ? (g->K + 7) / 8 * 8 : g->K) || g->ldb < (nn ? g->N : g->K) || g->ldc < g->N || g->expert_b < 0) return SK_ERR_SHAPE;
   const int64_t step = i8 ? 16 : 8;
@@ -69,6 +69,7 @@ extern "C" int sk_gemm_grouped(const sk_grouped *g, void *ws, size_t ws_bytes, v
   a.N = (int)g->N;
   a.K = (int)(g->K / pairs);
   a.act = g->activation;
+  a.spin_limit = g->spin_limit == 0 || g->spin_limit > MAX_INT ? 1 << 22 : (int)(g->spin_limit < 0 ? 0 : g->spin_limit);
   return status_of(launch_grouped(a, h, w, (hipStream_t)stream));
 }
 

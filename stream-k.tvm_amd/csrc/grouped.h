@@ -26,6 +26,7 @@ struct GroupedArgs {
   int64_t lda, ldb, ldc, expert_b;   // expert_b: elements of B from one expert to the next
   int E, R, N, K;                // one-byte operands: K, lda, ldb, expert_b in pairs
   int act, tiles_n, grid;
+  int spin_limit;                // polls of a wait for the other parts of a tile (kernels_grouped_asm.hip)
 };
 
 struct GroupTile {

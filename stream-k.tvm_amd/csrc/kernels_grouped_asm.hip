@@ -49,7 +49,7 @@ struct Cuts {
 // flags: [grid] of the CTAs, then a counter for each cut tile; all zero before and after.
 // (low: the lower half of the accumulators)
 template <class P>
-__device__ __forceinline__ bool join_parts(typename P::Acc &acc, int tile, int part, int parts, int grid, const Workspace &ws, bool low) {
+__device__ __forceinline__ bool join_parts(typename P::Acc &acc, int tile, int part, int parts, int grid, int spin_limit, const Workspace &ws, bool low) {
   int *ticket = ws.flags + grid + tile, *flags = ws.flags + tile * parts, *word = reinterpret_cast<int *>(P::lds() + 2 * P::STAGE_BYTES);
   auto slot = [&](int q) { return ws.partials + (size_t)(tile * parts + q) * P::TILE_ELEMS; };
   if (threadIdx.x == 0) *word = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -67,7 +67,7 @@ __device__ __forceinline__ bool join_parts(typename P::Acc &acc, int tile, int p
     for (int q = 0; q < parts; ++q) {
       if (q == part) continue;
       int got = 0;
-      for (int spin = 0; spin < (1 << 22) && !got; ++spin) {
+      for (int spin = 0; spin < spin_limit && !got; ++spin) {
         got = __hip_atomic_load(flags + q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         if (!got) __builtin_amdgcn_s_sleep(1);
       }
@@ -76,7 +76,12 @@ __device__ __forceinline__ bool join_parts(typename P::Acc &acc, int tile, int p
     if (threadIdx.x == 0) *word = ok;
   }
   __syncthreads();
-  if (*word == 0 && threadIdx.x == 0) ws.status[WS_STATUS] = -8;   // SK_ERR_TIMEOUT
+  const bool complete = *word != 0;
+  __syncthreads();   // (the patches of the tile's end overlap the word)
+  if (!complete) {
+    if (threadIdx.x == 0) ws.status[WS_STATUS] = -8;   // SK_ERR_TIMEOUT
+    return false;
+  }
   // eight groups at a time: the parts in front of this one, this one, the parts behind it
   constexpr int BATCH = 8;
   const uint32_t off = (uint32_t)pin_here((int)threadIdx.x) * 16;
@@ -168,7 +173,7 @@ __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_grouped_asm_kernel(
       else P::template prefetch_first_stage<FULL>(b, next.t.pm, next.t.pn, next.k0, next.n, rot_of(next));
       requested = true;
     }
-    if (s.cut < 0 || join_parts<P>(acc, s.cut, s.part, cuts.parts, g.grid, ws, s.low)) {
+    if (s.cut < 0 || join_parts<P>(acc, s.cut, s.part, cuts.parts, g.grid, g.spin_limit, ws, s.low)) {
       if (s.low) {
         // the lower half of each wave's 128 rows; the second wave's are the tile's rows 64 .., not 128 ..: C moved back by 64
         const int back = (threadIdx.x >> 7) * (P::WTM / 2);

@@ -56,7 +56,7 @@ class SkGrouped(ctypes.Structure):
         (n, ctypes.c_int64) for n in ("E", "R", "N", "K")] + [
         (n, ctypes.c_void_p) for n in ("A", "B", "offsets", "C")] + [
         (n, ctypes.c_int64) for n in ("lda", "ldb", "ldc", "expert_b")] + [
-        (n, ctypes.c_void_p) for n in ("bias", "scale_a", "scale_b")] + [("variant", ctypes.c_int64), ("reserved", ctypes.c_int64)]
+        (n, ctypes.c_void_p) for n in ("bias", "scale_a", "scale_b")] + [("variant", ctypes.c_int64), ("spin_limit", ctypes.c_int64)]
 
 
 class StreamKError(RuntimeError):

@@ -424,3 +424,66 @@ def test_every_plan_that_is_said_to_run_does(sk, M, N, K):
                 sk.streamk_int8_scaled(A, B, sa, sb, plan=plan)
     sk.workspace_status()
     assert ran > 10
+
+
+# ---- tiles that several CTAs share ----
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_a_wait_that_gives_up_leaves_its_tile_alone(sk, dtype):
+    """No polls at all: whoever comes last to a tile that is cut gives up.  Its part of C stays as it was, the workspace says so and is refused
+    until it is a new one, and the flags of the late parts stand in nobody's way."""
+    from streamk import _lib, ops
+    E, R, N, K, t = 1, 256, 512, 4096, TYPES[dtype]   # (two tiles, each cut in four)
+    A, B, offsets = rand((R, K), t, 1), rand((E, N, K), t, 2, 1 / 64), offsets_of([R])
+    want = sk.streamk_grouped(A, B, offsets, variant=2)
+    C = torch.full((R, N), 7.0, dtype=t, device="cuda")
+    g = _lib.SkGrouped(dtype=_lib.SK_F16 if t == torch.float16 else _lib.SK_BF16, layout=0, out_dtype=_lib.SK_F16 if t == torch.float16 else _lib.SK_BF16, E=E, R=R, N=N, K=K,
+                       A=A.data_ptr(), B=B.data_ptr(), offsets=offsets.data_ptr(), C=C.data_ptr(), lda=K, ldb=K, ldc=N, variant=2, spin_limit=-1)
+    L = sk.lib()
+    ws = ops._workspace(L.sk_grouped_workspace_bytes(ctypes.byref(g)), A.device)
+    launch = lambda: L.sk_gemm_grouped(ctypes.byref(g), ws.data_ptr(), ws.numel(), ops._stream_ptr())  # noqa: E731
+    try:
+        assert launch() == 0
+        torch.cuda.synchronize()
+        assert (C == 7).all()
+        flags = ws[256:256 + 4 * 1024].view(torch.int32)
+        assert flags[:8].sum() == 6 and (flags[256:258] == 4).all()   # (three of four parts of each tile; the counters)
+        with pytest.raises(sk.StreamKError) as e:
+            sk.workspace_status()
+        assert e.value.status == -8 and launch() == -8
+        with pytest.raises(sk.StreamKError):
+            sk.streamk_grouped(A, B, offsets, variant=2)
+    finally:
+        sk.reset_workspaces()
+    assert torch.equal(sk.streamk_grouped(A, B, offsets, variant=2), want)
+    sk.workspace_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["float16 nt", "bfloat16 nt", "float16 nn", "bfloat16 nn", "int8"])
+@pytest.mark.parametrize("variant,sizes,N,K", [(2, [300, 0, 200], 512, 4096), (2, [300, 0, 200], 512, 4224), (2, [100, 60, 0, 7], 1024, 8192), (2, [2000], 2304, 4096), (2, [40, 4000], 4352, 4096),
+                                               (5, [70, 200], 1000, 2048), (5, [1, 3, 0, 500], 264, 8192), (5, [64] * 8, 2048, 1024)])
+def test_shared_tiles_leave_the_workspace_as_it_was(sk, kind, variant, sizes, N, K):
+    from streamk import ops
+    R, E, offsets = sum(sizes), len(sizes), offsets_of(sizes)
+    if kind == "int8":
+        g = torch.Generator().manual_seed(R)
+        A, B = (torch.randint(-127, 128, s, generator=g, dtype=torch.int8).cuda() for s in ((R, K), (E, N, K)))
+        sa, sb = (torch.rand(R, generator=g) + 0.5).cuda() * 0.01, (torch.rand(E, N, generator=g) + 0.5).cuda() / (73 * math.sqrt(K))
+        run = lambda: sk.streamk_grouped(A, B, offsets, scale_a=sa, scale_b=sb, variant=variant)  # noqa: E731
+        want = torch.cat([(A[at].double() @ B[e].double().T) * sa[at].double()[:, None] * sb[e].double() for e, at in groups(sizes)])
+        terms, magnitudes = 2, want.abs()
+    else:
+        dtype, layout = kind.split()
+        A, W = rand((R, K), TYPES[dtype], R), rand((E, K, N), TYPES[dtype], N, 1 / math.sqrt(K))
+        B = W if layout == "nn" else W.transpose(1, 2).contiguous()
+        run = lambda: sk.streamk_grouped(A, B, offsets, layout=layout, variant=variant)  # noqa: E731
+        want, magnitudes = plain_kn(A, W, sizes)
+        terms = K
+    C = run()
+    assert_near(C, want, terms, magnitudes)
+    for _ in range(5):
+        assert torch.equal(run(), C)
+    sk.workspace_status()
+    words = ops._workspaces[(0, torch.cuda.current_stream().cuda_stream)][:256 + 4 * 1024].view(torch.int32)
+    assert words[0] == 0 and not words[64:].any()   # (status; flags and counters)
