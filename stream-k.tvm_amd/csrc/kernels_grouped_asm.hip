@@ -46,7 +46,11 @@ struct Cuts {
 // The end of a part of a cut tile.  Each CTA of the tile takes a ticket; all but the last put their sums into the workspace and raise a
 // flag, the last one -- the others are past their loops by then and wait for nobody, so the wait is a short one whatever else the
 // device does -- adds them to its own in the order of the parts, which is the same on every launch.  True: acc has the tile's sums.
-// flags: [grid] of the CTAs, then a counter for each cut tile; all zero before and after.
+// flags: [grid] of the CTAs, then a counter for each cut tile; all zero before and after.  A wait that gives up after spin_limit polls says
+// so in the workspace's status and leaves tile, flags and counter as they are, for a late part may still raise its flag: the next
+// launch must not count on zeros, and is refused once sk_workspace_status has seen it.  (With a count in place of the wait, every part
+// put down and the last to have done so adding up, 8 x 11008 x 4096, 800 rows take 160 us and not 154: a third more, or twice as many,
+// sums go through memory at the same time.)
 // (low: the lower half of the accumulators)
 template <class P>
 __device__ __forceinline__ bool join_parts(typename P::Acc &acc, int tile, int part, int parts, int grid, int spin_limit, const Workspace &ws, bool low) {
