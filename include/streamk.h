@@ -431,7 +431,8 @@ int sk_quantize_i8(const void *X, int dtype, int64_t M, int64_t K, int64_t ldx, 
  * included.  Rows that no group holds are set to zero.  Offsets are clamped to 0 .. R and to ascending order before they are used, so
  * no content of theirs leads outside the operands.  B: E matrices, expert_b elements apart, each [N, K] (SK_LAYOUT_NT, pitch ldb) or
  * [K, N] (SK_LAYOUT_NN, 16-bit types).  bias: [E, N] in C's type, contiguous, or null.  lda, ldb and expert_b multiples of 8 (int8:
- * 16), SK_LAYOUT_NT: K too; SK_LAYOUT_NN: N too, and where K is none, A has zeros in its columns from K to the next; A and B 16-byte, C and bias 2-byte, scales 4-byte aligned.  The same bits on every launch.
+ * 16), SK_LAYOUT_NT: K too; SK_LAYOUT_NN: N too, and where K is none, A has zeros in its columns from K to the next; A and B 16-byte, C and bias 2-byte, scales 4-byte aligned.  256 rows of A, of C and of
+ * [N, K] weights, and K + 64 rows of [K, N] weights (an expert's all), span less than 2 GiB.  The same bits on every launch.
  * ws: as for the other products (sk_workspace_init has run on it).  Variant 2 may cut a tile along K; the CTA that comes last to it waits
  * for the others' stores, spin_limit polls at most.  If it gives up, the tile is not stored and sk_workspace_status says
  * SK_ERR_TIMEOUT.  No other variant waits for part of itself.

@@ -118,7 +118,13 @@ def _grouped(A, B, offsets, layout="nt", out_dtype=None, scale_a=None, scale_b=N
         return C
     # ([K, N] weights and a K that is no multiple of 8: the last piece of eight columns of A is multiplied whole, its columns past K by
     # zeros -- but zero times what lies beside a view may be NaN)
-    A = _padded(A)[:, :K] if layout == "nn" and K % 8 else _rows(A)
+    A = _padded(A) if layout == "nn" and K % 8 else _rows(A)
+    if layout == "nn" and 2 * B.stride(1) * (K + 64) >= 1 << 31:
+        # the tiles address all rows of a [K, N] expert by 32-bit offsets, those of an [N, K] one a tile at a time
+        turned = B.new_zeros((E, N, A.shape[1]))
+        turned[:, :, :K].copy_(B.transpose(1, 2))
+        B, K, layout = turned, A.shape[1], "nt"
+    A = A[:, :K]
     ldb = B.stride(1) if B.shape[1] > 1 else (B.shape[2] + 15) // 16 * 16
     g = _lib.SkGrouped(dtype=_lib.SK_I8 if int8 else _TYPES[A.dtype], layout=ops._plan_mod._LAYOUTS[layout], out_dtype=_TYPES[out_dtype],
                        activation=_lib.ACTIVATIONS[activation], E=E, R=R, N=N, K=K, A=A.data_ptr(), B=B.data_ptr(),
@@ -196,7 +202,7 @@ def streamk_grouped(A, B, offsets, *, layout="nt", scale_a=None, scale_b=None, o
     [E, N, K] (layout 'nt'), A[r] @ B[e] for B [E, K, N] ('nn'); float16, bfloat16, or int8 ('nt') with scale_a [R] and scale_b
     [E, N] (float32), whose result is `out_dtype` (float16 by default).  offsets: int32 [E + 1] on the device, ascending from 0;
     groups of any size; rows behind the last group come out as zeros.  K is a multiple of 8 (int8: 16) for 'nt', N of 8 for 'nn', whose K
-    may be any number (rows of a K that is no multiple of 8 are copied).  bias: [E, N] in C's type.  Sums in fp32 (int8: exact), rounded
+    may be any number (rows of a K that is no multiple of 8 are copied, and so are an expert's [K, N] weights from 2 GiB on).  bias: [E, N] in C's type.  Sums in fp32 (int8: exact), rounded
     once.  Differentiable in A and B without bias, activation, scales and out.  variant: which tiles run (sk_grouped in streamk.h); 0
     lets the sizes decide."""
     activation = activation or "none"

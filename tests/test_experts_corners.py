@@ -487,3 +487,39 @@ def test_shared_tiles_leave_the_workspace_as_it_was(sk, kind, variant, sizes, N,
     sk.workspace_status()
     words = ops._workspaces[(0, torch.cuda.current_stream().cuda_stream)][:256 + 4 * 1024].view(torch.int32)
     assert words[0] == 0 and not words[64:].any()   # (status; flags and counters)
+
+
+# ---- experts whose weights span 2 GiB ----
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,E,sizes", [(262144, 1, [20]), (262149, 2, [3, 130])])
+def test_gradients_of_large_experts(sk, N, E, sizes):
+    """The product takes them ([N, K] weights are addressed by tiles); so do the gradients, whose [K, N] form goes through a copy."""
+    K, R, offsets = 4096, sum(sizes), offsets_of(sizes)
+    A, d = rand((R, K), torch.bfloat16, 1), rand((R, N), torch.bfloat16, 2)
+    B = torch.empty((E, N, K), dtype=torch.bfloat16, device="cuda").normal_(0, 1 / 64)
+    assert B[0].numel() * 2 >= 2 ** 31
+    x, w = A.clone().requires_grad_(), B.requires_grad_()
+    dx, dw = torch.autograd.grad(sk.streamk_grouped(x, w, offsets), (x, w), d)
+    B = B.detach()
+    for e, at in groups(sizes):
+        want, magnitudes = torch.zeros(sizes[e], K, dtype=torch.float64, device="cuda"), torch.zeros(sizes[e], K, dtype=torch.float64, device="cuda")
+        for n in range(0, N, 32768):
+            part, rows = B[e, n:n + 32768].double(), d[at, n:n + 32768].double()
+            want += rows @ part
+            magnitudes += rows.abs() @ part.abs()
+        assert_near(dx[at], want, N, magnitudes)
+        for cols in (slice(0, 9), slice(N - 9, N)):
+            assert_near(dw[e, cols], d[at, cols].double().T @ A[at].double(), sizes[e], d[at, cols].double().abs().T @ A[at].double().abs())
+    assert torch.equal(sk.streamk_grouped(d, B, offsets, layout="nn"), dx)
+
+
+@pytest.mark.gpu
+def test_large_experts_with_a_pitch_are_no_different(sk):
+    """Few columns far apart: the span counts, not the size."""
+    E, N, K, sizes = 2, 64, 1030, [5, 12]
+    wide = torch.zeros((E, K, 1 << 20), dtype=torch.float16, device="cuda")
+    B = wide[:, :, :N]
+    B.copy_(rand((E, K, N), torch.float16, 2, 1 / 32))
+    A = rand((17, K), torch.float16, 1)
+    want, magnitudes = plain_kn(A, B, sizes)
+    assert_near(sk.streamk_grouped(A, B, offsets_of(sizes), layout="nn"), want, K, magnitudes)
