@@ -7,11 +7,26 @@ leading dimensions of the input into M, and keeps one plan per M it has seen (a 
 with M = batch, a prefill with M = batch * tokens), each taken from the tuned cache when the shape
 is in it.  Inference only: the GEMM is not recorded by autograd.
 """
+import math
+
 import torch
 
 from . import int8, ops
 from .int8 import quantize_int8
 from .plan import make_plan, operator_config
+
+
+def _quantize_rows(w):
+    """quantize_int8 of a layer's weights.  Those of more bits are not rounded to 16 first, where a weight beyond fp16's largest number
+    would make its channel NaN: the same formula in 64 bits, once for a layer."""
+    if w.dtype in (torch.float16, torch.bfloat16):
+        return quantize_int8(w.contiguous())
+    w = w.double()
+    scale = (w.abs().amax(1) / 127).float()
+    finite = torch.isfinite(scale)
+    step = torch.where(finite & (scale > 0), scale, math.inf).double()
+    q = torch.where(finite[:, None], torch.round(w / step[:, None]).clamp(-127, 127), 0)
+    return q.to(torch.int8), torch.where(finite, scale, math.nan)
 
 
 class StreamKLinear(torch.nn.Module):
@@ -56,17 +71,23 @@ class StreamKLinear(torch.nn.Module):
     def from_linear(cls, linear, *, weight_format="float16", group=128, zero=8, activation=None):
         """Takes over the weight (and bias) of a torch.nn.Linear; weight_format='q4' / 'q4_zp' quantises
         it with `quantize_q4` (symmetric around `zero` / asymmetric with a zero point per group), weight_format='int8' with
-        `quantize_int8` (input and output are bfloat16 if the weight is), on the device it lives on."""
-        keeps = weight_format == "bfloat16" or (weight_format == "int8" and linear.weight.dtype == torch.bfloat16)
-        w = linear.weight.detach().to(torch.bfloat16 if keeps else torch.float16).contiguous()
-        m = cls(linear.in_features, linear.out_features, linear.bias is not None, weight_format=weight_format,
-                group=group, zero=zero, activation=activation, device=w.device, dtype=w.dtype if weight_format == "int8" else None)
-        if weight_format in ("float16", "bfloat16"):
-            m.weight.copy_(w)
-        elif weight_format == "int8":
-            q, s = quantize_int8(w)
+        `quantize_int8` (weights of other types from what they are, by the same formula; input and output are bfloat16 if the weight is), on
+        the device it lives on."""
+        if weight_format == "int8":
+            keeps = linear.weight.dtype == torch.bfloat16
+            m = cls(linear.in_features, linear.out_features, linear.bias is not None, weight_format="int8", activation=activation,
+                    device=linear.weight.device, dtype=torch.bfloat16 if keeps else torch.float16)
+            q, s = _quantize_rows(linear.weight.detach())
             m.qweight.copy_(q)
             m.weight_scale.copy_(s)
+            if linear.bias is not None:
+                m.bias.copy_(linear.bias.detach().to(m.dtype))
+            return m
+        w = linear.weight.detach().to(torch.bfloat16 if weight_format == "bfloat16" else torch.float16).contiguous()
+        m = cls(linear.in_features, linear.out_features, linear.bias is not None, weight_format=weight_format,
+                group=group, zero=zero, activation=activation, device=w.device)
+        if weight_format in ("float16", "bfloat16"):
+            m.weight.copy_(w)
         elif weight_format == "q4_zp":
             q, s, z = ops.quantize_q4(w, group=group, asymmetric=True)
             m.qweight.copy_(q)

@@ -523,3 +523,40 @@ def test_large_experts_with_a_pitch_are_no_different(sk):
     A = rand((17, K), torch.float16, 1)
     want, magnitudes = plain_kn(A, B, sizes)
     assert_near(sk.streamk_grouped(A, B, offsets_of(sizes), layout="nn"), want, K, magnitudes)
+
+
+# ---- int8 layers of weights with more than 16 bits ----
+def test_int8_layer_of_fp32_weights(sk):
+    """On the CPU: quantised from what they are -- beyond fp16's largest number, below its smallest, next to a tie that fp16 would move."""
+    linear = torch.nn.Linear(64, 9, bias=True)
+    w = linear.weight.data
+    w[1, 3] = 7e4
+    w[2] = torch.arange(64) * 1e-12
+    w[3] = 0
+    w[4, 5] = math.inf
+    w[5, 6] = math.nan
+    w[6] = 0
+    w[6, :3] = torch.tensor([127.0, 0.5 + 2.0 ** -20, 2.5])   # scale 1
+    w[7, 0] = -3e38
+    layer = sk.StreamKLinear.from_linear(linear, weight_format="int8", activation="relu")
+    q, s = layer.qweight, layer.weight_scale
+    assert layer.dtype == torch.float16 and layer.activation == "relu" and torch.equal(layer.bias, linear.bias.half())
+    assert torch.isnan(s[4:6]).all() and not q[4:6].any() and s[3] == 0 and not q[3].any()
+    assert q[6, :3].tolist() == [127, 1, 2] and q[7, 0] == -127 and torch.isfinite(s[[0, 1, 2, 6, 7, 8]]).all()
+    for r in (0, 1, 2, 7, 8):
+        want = w[r].double().abs().max() / 127
+        assert s[r] == want.float() and torch.equal(q[r].double(), torch.round(w[r].double() / s[r].double()))
+
+
+@pytest.mark.gpu
+def test_int8_layer_of_fp32_weights_like_that_of_16_bits(sk):
+    linear = torch.nn.Linear(512, 300, device="cuda", dtype=torch.float16)
+    wide = torch.nn.Linear(512, 300, device="cuda")
+    wide.load_state_dict({k: v.float() for k, v in linear.state_dict().items()})
+    a, b = (sk.StreamKLinear.from_linear(m, weight_format="int8") for m in (linear, wide))
+    for x, y in zip(a.state_dict().values(), b.state_dict().values()):
+        assert x.dtype == y.dtype and torch.equal(x, y)
+    wide.weight.data[7, 100] = 1e5
+    c = sk.StreamKLinear.from_linear(wide, weight_format="int8")
+    x = torch.randn(20, 512, device="cuda").half() * 1e-3
+    assert torch.isfinite(c(x)).all()
