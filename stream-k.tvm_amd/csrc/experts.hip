@@ -11,6 +11,7 @@
 
 #include "sk_device.h"
 #include "streamk.h"
+#include "wide_grid.h"
 
 using namespace sk;
 
@@ -312,7 +313,7 @@ __global__ __launch_bounds__(64 * WAVES) void route_backward_kernel(const float 
                                                                     int E, int k, void *dlogits) {
   extern __shared__ float row_lds[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t t = (int64_t)blockIdx.x * WAVES + wave;
+  const int64_t t = wide_block() * WAVES + wave;
   float *row = row_lds + wave * E;
   if (t < T) {
     for (int e = lane; e < E; e += 64) row[e] = 0.f;
@@ -334,7 +335,7 @@ template <class Unit>
 __global__ __launch_bounds__(64 * WAVES) void dispatch_kernel(const Unit *x, int64_t ldx, const int *order, int T, int k, int64_t rows, int units,
                                                               Unit *out) {
   const int lane = threadIdx.x & 63;
-  const int64_t p = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6);
+  const int64_t p = wide_block() * WAVES + (threadIdx.x >> 6);
   if (p >= rows) return;
   const int slot = order[p], t = slot >= 0 ? (int)((unsigned)slot / (unsigned)k) : -1;
   Unit *dst = out + p * units;
@@ -360,7 +361,7 @@ template <class Unit>
 __global__ __launch_bounds__(64 * WAVES) void dispatch_tokens_kernel(const Unit *x, int64_t ldx, const int *order, const int *place, int T, int k,
                                                                      int units, Unit *out) {
   const int lane = threadIdx.x & 63;
-  const int64_t t = (int64_t)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), rows = (int64_t)T * k;
+  const int64_t t = wide_block() * WAVES + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), rows = (int64_t)T * k;
   if (t >= T) return;
   const Unit *src = x + t * ldx;
   const int mine = lane < k ? place[t * k + lane] : -1, at = lane < k ? order[t * k + lane] : 0;   // (k <= 64)
@@ -424,7 +425,7 @@ __device__ __forceinline__ void store8(uint16_t *row, int c, int H, ushort8v v) 
 template <bool BF16, bool VEC>
 __global__ __launch_bounds__(64 * WAVES) void combine_kernel(const uint16_t *y, const int *place, const float *weights, int k, int H, int64_t T,
                                                              uint16_t *out, int pieces) {
-  const int64_t item = (int64_t)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), t = item / pieces, rows = T * k;
+  const int64_t item = wide_block() * WAVES + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), t = item / pieces, rows = T * k;
   if (t >= T) return;
   const int c = ((int)(item - t * pieces) * 64 + (threadIdx.x & 63)) * 8;
   if (c < H) {
@@ -461,7 +462,7 @@ template <bool BF16, bool VEC>
 __global__ __launch_bounds__(64 * WAVES) void combine_backward_kernel(const uint16_t *d_out, const uint16_t *y, const int *order, const int *place,
                                                                       const float *weights, int k, int H, int64_t rows, uint16_t *dy, float *dw) {
   const int lane = threadIdx.x & 63;
-  const int64_t slot = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6);
+  const int64_t slot = wide_block() * WAVES + (threadIdx.x >> 6);
   if (slot >= rows) return;
   if (order[slot] < 0)
     for (int c = lane * 8; c < H; c += 512) store8<VEC>(dy + slot * H, c, H, ushort8v{0, 0, 0, 0, 0, 0, 0, 0});
@@ -523,7 +524,7 @@ extern "C" int sk_route_backward(const void *weights, const void *experts, const
   if (element_of(dtype) < 0) return SK_ERR_CONFIG;
   if (int rc = check_route_shape(T, E, k)) return rc;
   if (!weights || !experts || !dweights || !dlogits) return SK_ERR_NULL;
-  const dim3 grid((unsigned)((T + WAVES - 1) / WAVES)), block(64 * WAVES);
+  const dim3 grid = wide_grid((T + WAVES - 1) / WAVES), block(64 * WAVES);
   const size_t lds = sizeof(float) * WAVES * E;
 #define SK_ROUTE_BACKWARD(EL)                                                                                                            \
   hipLaunchKernelGGL((route_backward_kernel<EL>), grid, block, lds, (hipStream_t)stream, (const float *)weights, (const int *)experts,    \
@@ -540,11 +541,11 @@ extern "C" int sk_dispatch_rows(const void *x, int64_t row_bytes, int64_t x_pitc
   if (!x || !order || !rows) return SK_ERR_NULL;
   if (T <= 0 || k <= 0 || T * k > 0x7fffffff / 2 || row_bytes <= 0 || row_bytes > 0x7fffffff || x_pitch < row_bytes) return SK_ERR_SHAPE;
   const int64_t n = T * k;
-  const dim3 grid((unsigned)((n + WAVES - 1) / WAVES)), block(64 * WAVES);
+  const dim3 grid = wide_grid((n + WAVES - 1) / WAVES), block(64 * WAVES);
   const uint64_t all = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(rows) | (uint64_t)row_bytes | (uint64_t)x_pitch;
   // (many tokens: fewer waves than rows fill the device)
   const bool by_tokens = place && k <= MAX_CHOSEN && T >= 2048;
-  const dim3 tokens_grid((unsigned)((T + WAVES - 1) / WAVES));
+  const dim3 tokens_grid = wide_grid((T + WAVES - 1) / WAVES);
 #define SK_DISPATCH(UNIT)                                                                                                            \
   if (by_tokens)                                                                                                                     \
     hipLaunchKernelGGL((dispatch_tokens_kernel<UNIT>), tokens_grid, block, 0, (hipStream_t)stream, (const UNIT *)x,                   \
@@ -574,7 +575,7 @@ extern "C" int sk_combine_rows(const void *y, int dtype, const void *place, cons
   if (blocks > 0x7fffffff) return SK_ERR_SHAPE;
   const bool vec = H % 8 == 0 && aligned16(y) && aligned16(out);
 #define SK_COMBINE(BF, VEC)                                                                                                            \
-  hipLaunchKernelGGL((combine_kernel<BF, VEC>), dim3((unsigned)blocks), dim3(64 * WAVES), 0, (hipStream_t)stream, (const uint16_t *)y,   \
+  hipLaunchKernelGGL((combine_kernel<BF, VEC>), wide_grid(blocks), dim3(64 * WAVES), 0, (hipStream_t)stream, (const uint16_t *)y,   \
                      (const int *)place, (const float *)weights, (int)k, (int)H, T, (uint16_t *)out, pieces)
   if (dtype == SK_BF16) {
     if (vec) SK_COMBINE(true, true);
@@ -593,7 +594,7 @@ extern "C" int sk_combine_backward(const void *d_out, const void *y, int dtype, 
   if (!d_out || !y || !order || !place || !weights || !dy || !dweights) return SK_ERR_NULL;
   if (T <= 0 || k <= 0 || H <= 0 || T * k > 0x7fffffff / 2 || H > 0x7fffff00) return SK_ERR_SHAPE;
   const bool vec = H % 8 == 0 && aligned16(d_out) && aligned16(y) && aligned16(dy);
-  const dim3 grid((unsigned)((T * k + WAVES - 1) / WAVES)), block(64 * WAVES);
+  const dim3 grid = wide_grid((T * k + WAVES - 1) / WAVES), block(64 * WAVES);
 #define SK_COMBINE_BACKWARD(BF, VEC)                                                                                                  \
   hipLaunchKernelGGL((combine_backward_kernel<BF, VEC>), grid, block, 0, (hipStream_t)stream, (const uint16_t *)d_out, (const uint16_t *)y, \
                      (const int *)order, (const int *)place, (const float *)weights, (int)k, (int)H, T * k, (uint16_t *)dy, (float *)dweights)

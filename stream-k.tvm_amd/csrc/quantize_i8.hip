@@ -7,6 +7,7 @@
 
 #include "sk_device.h"
 #include "streamk.h"
+#include "wide_grid.h"
 
 using namespace sk;
 
@@ -58,10 +59,12 @@ __device__ __forceinline__ uint64_t quantise8(ushort8v v, float s, float inv) {
 }
 
 template <bool BF16>
-__global__ __launch_bounds__(THREADS) void quantize_i8_kernel(const uint16_t *X, int K, int64_t ldx, int8_t *Q, int64_t ldq, float *scales,
-                                                              int vec) {
-  const uint16_t *x = X + (int64_t)blockIdx.x * ldx;
-  int8_t *q = Q + (int64_t)blockIdx.x * ldq;
+__global__ __launch_bounds__(THREADS) void quantize_i8_kernel(const uint16_t *X, int M, int K, int64_t ldx, int8_t *Q, int64_t ldq,
+                                                              float *scales, int vec) {
+  const int64_t row = wide_block();
+  if (row >= M) return;
+  const uint16_t *x = X + row * ldx;
+  int8_t *q = Q + row * ldq;
   const int pieces = (K + 7) / 8, tid = threadIdx.x;
   auto load = [&](int p) {
     ushort8v v = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -102,7 +105,7 @@ __global__ __launch_bounds__(THREADS) void quantize_i8_kernel(const uint16_t *X,
   // a row with an infinity or a NaN has no scale: NaN, so that whatever is made of it is NaN too
   const bool finite = most < (BF16 ? 0x7f80u : 0x7c00u);
   const float s = finite ? widen<BF16>((uint16_t)most) / 127.f : __builtin_nanf("");
-  if (tid == 0) scales[blockIdx.x] = s;
+  if (tid == 0) scales[row] = s;
   const bool any = s > 0.f, small = s < 1e-37f;   // (the reciprocal of a smaller scale overflows)
   const float inv = any && !small ? 1.f / s : 0.f;
   auto store = [&](int p, ushort8v v) {
@@ -137,10 +140,10 @@ extern "C" int sk_quantize_i8(const void *X, int dtype, int64_t M, int64_t K, in
   if ((reinterpret_cast<uintptr_t>(X) & 1) || (reinterpret_cast<uintptr_t>(scales) & 3)) return SK_ERR_ALIGN;
   const int vec = K % 8 == 0 && ldx % 8 == 0 && ldq % 8 == 0 && (reinterpret_cast<uintptr_t>(X) & 15) == 0 && (reinterpret_cast<uintptr_t>(Q) & 7) == 0;
   if (dtype == SK_BF16)
-    hipLaunchKernelGGL((quantize_i8_kernel<true>), dim3((unsigned)M), dim3(THREADS), 0, (hipStream_t)stream, (const uint16_t *)X, (int)K, ldx,
+    hipLaunchKernelGGL((quantize_i8_kernel<true>), wide_grid(M), dim3(THREADS), 0, (hipStream_t)stream, (const uint16_t *)X, (int)M, (int)K, ldx,
                        (int8_t *)Q, ldq, (float *)scales, vec);
   else
-    hipLaunchKernelGGL((quantize_i8_kernel<false>), dim3((unsigned)M), dim3(THREADS), 0, (hipStream_t)stream, (const uint16_t *)X, (int)K, ldx,
+    hipLaunchKernelGGL((quantize_i8_kernel<false>), wide_grid(M), dim3(THREADS), 0, (hipStream_t)stream, (const uint16_t *)X, (int)M, (int)K, ldx,
                        (int8_t *)Q, ldq, (float *)scales, vec);
   return hipGetLastError() == hipSuccess ? SK_OK : SK_ERR_LAUNCH;
 }

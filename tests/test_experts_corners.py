@@ -560,3 +560,37 @@ def test_int8_layer_of_fp32_weights_like_that_of_16_bits(sk):
     c = sk.StreamKLinear.from_linear(wide, weight_format="int8")
     x = torch.randn(20, 512, device="cuda").half() * 1e-3
     assert torch.isfinite(c(x)).all()
+
+
+# ---- more rows than a launch has threads for in one dimension ----
+@pytest.mark.gpu
+def test_quantiser_of_very_many_rows(sk):
+    M = 2 ** 24 + 77
+    x = torch.randn(M, 2, device="cuda").half()
+    q, s = sk.quantize_int8(x)
+    for at in (slice(0, 1000), slice(2 ** 21 - 500, 2 ** 21 + 500), slice(2 ** 24 - 500, M)):
+        amax = x[at].double().abs().amax(1)
+        assert torch.equal(s[at], (amax / 127).float())
+        assert torch.equal(q[at].double(), torch.round(x[at].double() / s[at].double()[:, None]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,k", [(2 ** 25 + 5, 2), (2 ** 26 + 3, 1)])
+def test_exchange_of_very_many_rows(sk, T, k):
+    logits = torch.randn(T, 3, device="cuda").requires_grad_()
+    route = sk.route_experts(logits, k)
+    x = torch.arange(T, device="cuda", dtype=torch.int32)
+    rows = sk.dispatch_rows(x, route)
+    assert torch.equal(rows, torch.div(route.order, k, rounding_mode="floor"))
+    by_rows = torch.ops.streamk.dispatch_rows(x, route.order, k)   # (a wave a row, and not a wave a token)
+    assert torch.equal(by_rows, rows)
+    y = (rows % 1024)[:, None].half().requires_grad_()   # (exact in fp16, and so is the sum of a token's two)
+    ones = torch.ones_like(route.weights).requires_grad_()
+    out = sk.combine_rows(y, route._replace(weights=ones))
+    assert torch.equal(out[:, 0], (k * (x % 1024)).half())
+    dy, dw = torch.autograd.grad(out, (y, ones), (x % 512)[:, None].half())
+    assert torch.equal(dy[:, 0], (rows % 512).half())
+    assert torch.equal(dw, ((x % 1024).float() * (x % 512).float())[:, None].expand(T, k))
+    dz, = torch.autograd.grad(route.weights, logits, torch.ones_like(route.weights))
+    # (weights that sum to one: their sum has no gradient)
+    assert dz[-1000:].abs().max() <= 8 * 2.0 ** -24
