@@ -55,8 +55,8 @@ def _check_offsets(offsets, E, device):
 
 
 def _pitch(t):
-    """Row pitch of a matrix whose rows are taken as they stand (a single row's stride is arbitrary)."""
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16 if t.stride(0) < t.shape[1] else t.stride(0)
+    """Row pitch of a matrix whose rows are taken as they stand (that of a single row says nothing, and need not be aligned)."""
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
 
 
 # ---- the grouped product ----

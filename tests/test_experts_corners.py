@@ -594,3 +594,25 @@ def test_exchange_of_very_many_rows(sk, T, k):
     dz, = torch.autograd.grad(route.weights, logits, torch.ones_like(route.weights))
     # (weights that sum to one: their sum has no gradient)
     assert dz[-1000:].abs().max() <= 8 * 2.0 ** -24
+
+
+# ---- a single row, whose stride says nothing ----
+@pytest.mark.gpu
+@pytest.mark.parametrize("stride", [64, 97, 61, 1])
+def test_a_single_row_of_any_stride(sk, stride):
+    """Also where the native operator passes the call on: one column of weights, gradients of one row."""
+    base = rand((200,), torch.float16, 1)
+    row, offsets = base.as_strided((1, 64), (stride, 1)), offsets_of([1, 0])
+    B = rand((2, 32, 64), torch.float16, 2)
+    for weights in (B, B[:, :1]):
+        assert_near(sk.streamk_grouped(row, weights, offsets), row.double() @ weights[0].double().T, 64, row.double().abs() @ weights[0].double().abs().T)
+    W = rand((2, 64, 32), torch.float16, 3)
+    assert torch.equal(sk.streamk_grouped(row, W, offsets, layout="nn"), sk.streamk_grouped(row.contiguous(), W, offsets, layout="nn"))
+    d = base.as_strided((1, 32), (stride, 1), 80)
+    for left in (d, base.as_strided((1, 29), (stride, 1), 80)):
+        dw = sk.streamk_grouped_wgrad(left, row, offsets)
+        assert torch.equal(dw[0], (left.double().T @ row.double()).half()) and not dw[1].any()
+    q = torch.randint(-127, 128, (200,), dtype=torch.int8, device="cuda").as_strided((1, 64), (stride, 1))
+    w, s, sw = torch.randint(-127, 128, (2, 1, 64), dtype=torch.int8, device="cuda"), torch.rand(1, device="cuda"), torch.rand(2, 1, device="cuda") * 1e-3
+    want = (q.double() @ w[0].double().T) * s.double() * sw[0].double()
+    assert_near(sk.streamk_grouped(q, w, offsets, scale_a=s, scale_b=sw), want, 2, want.abs())
