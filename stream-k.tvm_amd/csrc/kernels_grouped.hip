@@ -150,9 +150,26 @@ static int launch_wgrad_policy(WgradArgs g, int cus, hipStream_t s) {
   return (int)hipGetLastError();
 }
 
+// A round of 256 x 256 tiles, one to a CU, takes 1.1 to 1.5 times as long as one of 128 x 128 tiles, two to a CU: they pay where there are
+// fewer rounds of them, and rows enough for their longer beginning and end.  bfloat16, times of 256 x 256 tiles by those of 128 x 128:
+//   one round against one    1 x 2048 x 2048, 8192 rows 1.49; 1 x 4096 x 2048, 128 rows 1.31, 8192 rows 1.11
+//   one or two against two   of 64 rows an expert .94 to 1.08, 128 rows .91 to 1.06, 512 rows .77 to .91, 8192 rows .60 to .75
+//   or four
+//   two against three        128 rows 1.11 to 1.22, 512 rows .98 to 1.05, 2048 rows .92 to .94
+//   four and six             24 rows 1.00 to 1.13, 64 rows .90 to 1.03, 512 rows .75 to .84
+//   eight and more           16 rows .80 to .92, 1024 rows .65 to .75
+//   nine against thirteen    712 rows .82
+// On 84 random sizes (1 to 64 experts, 8 to 4000 rows each) the choice takes 1.00 of the faster tiles' time on average, 1.1 at worst
+// (256 x 256 from 64 rows an expert on, whatever their number: 1.10 and 1.9).
+static bool wgrad_asm_pays(const WgradArgs &g, int cus) {
+  const auto rounds = [&](int64_t b, int per_cu) { return (g.E * ((g.N + b - 1) / b) * ((g.K + b - 1) / b) + cus * per_cu - 1) / (cus * per_cu); };
+  const int64_t large = rounds(256, 1), small = rounds(128, 2);
+  if (4 * small < 7 * large) return 5 * small >= 7 * large && g.R >= (int64_t)512 * g.E;
+  return g.R >= (int64_t)(large < 4 ? 128 : (large < 8 ? 64 : 0)) * g.E;
+}
 int launch_wgrad(const WgradArgs &g, bool bf16, int cus, int variant, hipStream_t s) {
   if (variant > GV_ASM256 || (variant == GV_ASM256 && !wgrad_asm_takes(g))) return (int)hipErrorNotSupported;
-  if (variant == GV_ASM256 || (variant == GV_RULE && wgrad_asm_takes(g) && g.R >= 64 * g.E)) return launch_wgrad_asm(g, bf16, cus, s);
+  if (variant == GV_ASM256 || (variant == GV_RULE && wgrad_asm_takes(g) && wgrad_asm_pays(g, cus))) return launch_wgrad_asm(g, bf16, cus, s);
   return bf16 ? launch_wgrad_policy<TileTN<128, 128, 2, 2, true>>(g, cus, s) : launch_wgrad_policy<TileTN<128, 128, 2, 2, false>>(g, cus, s);
 }
 
