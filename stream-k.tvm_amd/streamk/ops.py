@@ -35,17 +35,22 @@ def _stream_ptr():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+_outgrown = []   # workspaces that larger ones have replaced
+
+
 def _workspace(nbytes, device):
-    """One self-cleaning workspace per (device, stream), grown on demand and zeroed once."""
+    """One self-cleaning workspace per (device, stream), grown on demand and zeroed once.  One that has become too small stays allocated:
+    a graph that was recorded with it goes on writing to it."""
     if nbytes == 0:
         return None
     key = (device.index if device.index is not None else torch.cuda.current_device(),
            torch.cuda.current_stream().cuda_stream)
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
-        if ws is not None:  # the library must not take a later allocation at this address for this workspace
+        if ws is not None:
             _lib.tell_native_operators("sk_torch_set_workspace", *key, None, 0)
             _lib.lib().sk_workspace_release(ws.data_ptr())
+            _outgrown.append(ws)
         ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
         _lib.check(_lib.lib().sk_workspace_init(ws.data_ptr(), ws.numel(), _stream_ptr()),
                    "sk_workspace_init")
@@ -63,11 +68,13 @@ def _ws_args(plan, device):
 def reset_workspaces():
     """Drops cached workspaces.  Needed after workspace_status() (or a launch) has raised StreamKError
     with status SK_ERR_TIMEOUT: the library refuses a workspace on which a fix-up wait gave up until it
-    has been initialised again, which the next call on a fresh workspace does."""
-    for key, ws in _workspaces.items():
+    has been initialised again, which the next call on a fresh workspace does.  Graphs recorded before it are not to be
+    replayed any more: their workspaces may belong to others."""
+    for key, ws in _workspaces.items():   # (the library must not take a later allocation at such an address for this workspace)
         _lib.tell_native_operators("sk_torch_set_workspace", *key, None, 0)
         _lib.lib().sk_workspace_release(ws.data_ptr())
     _workspaces.clear()
+    _outgrown.clear()
 
 
 def workspace_status():

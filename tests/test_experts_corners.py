@@ -616,3 +616,35 @@ def test_a_single_row_of_any_stride(sk, stride):
     w, s, sw = torch.randint(-127, 128, (2, 1, 64), dtype=torch.int8, device="cuda"), torch.rand(1, device="cuda"), torch.rand(2, 1, device="cuda") * 1e-3
     want = (q.double() @ w[0].double().T) * s.double() * sw[0].double()
     assert_near(sk.streamk_grouped(q, w, offsets, scale_a=s, scale_b=sw), want, 2, want.abs())
+
+
+# ---- a recorded call and a later one that needs a larger workspace ----
+@pytest.mark.gpu
+def test_a_recorded_call_keeps_its_workspace(sk):
+    from streamk import ops
+    sizes = [3, 0, 9]
+    A, B, offsets = rand((12, 4096), torch.float16, 1), rand((3, 520, 4096), torch.float16, 2, 1 / 64), offsets_of(sizes)
+    large_a, large_b, large_o = rand((700, 4096), torch.float16, 3), rand((2, 512, 4096), torch.float16, 4, 1 / 64), offsets_of([300, 400])
+    small, large = (lambda: sk.streamk_grouped(A, B, offsets, variant=3)), (lambda: sk.streamk_grouped(large_a, large_b, large_o, variant=2))
+    want, stream, graph = small(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        small()
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            C = small()
+        key = (0, stream.cuda_stream)
+        old = ops._workspaces[key]
+        size, address = old.numel(), old.data_ptr()
+        del old
+        large()
+        assert ops._workspaces[key].numel() > size
+        # whoever gets memory now must not get the recorded call's
+        others = [torch.full((size,), 85, dtype=torch.uint8, device="cuda") for _ in range(8)]
+        assert not any(t.data_ptr() <= address < t.data_ptr() + size for t in others)
+        for _ in range(3):
+            C.zero_()
+            graph.replay()
+            stream.synchronize()
+            assert torch.equal(C, want) and all((t == 85).all() for t in others)
+            large()
