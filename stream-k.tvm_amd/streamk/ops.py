@@ -452,13 +452,12 @@ _LIBRARY = torch.library.Library("streamk", "DEF")
 _EPI = "Tensor? bias=None, str activation=\"none\""
 
 
-def _register(name, before_out, after_out, run, out_meta, native=None):
+def _register(name, before_out, after_out, run, out_meta):
     """Defines streamk::<name>(before_out, after_out) -> Tensor and streamk::<name>_out(before_out, out,
     after_out) -> ().  run(*args) with C at position len(before_out arguments) performs the launch;
     out_meta(*functional args) -> (shape, dtype) of C."""
     out_pos = before_out.count("Tensor")
-    # csrc/torch_ops.cpp implements these and calls <name>_general for the rest
-    native = name.startswith("gemm_") if native is None else native
+    native = name.startswith("gemm_")   # csrc/torch_ops.cpp implements these and calls <name>_general for the rest
     general = "_general" if native else ""
     for suffix in ("", general) if native else ("",):
         _LIBRARY.define(f"{name}{suffix}({before_out}, {after_out}) -> Tensor")
