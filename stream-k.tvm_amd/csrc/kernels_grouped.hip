@@ -153,8 +153,8 @@ static int launch_wgrad_policy(WgradArgs g, int cus, hipStream_t s) {
 // A round of 256 x 256 tiles, one to a CU, takes 1.1 to 1.5 times as long as one of 128 x 128 tiles, two to a CU: they pay where there are
 // fewer rounds of them, and rows enough for their longer beginning and end.  bfloat16, times of 256 x 256 tiles by those of 128 x 128:
 //   one round against one    1 x 2048 x 2048, 8192 rows 1.49; 1 x 4096 x 2048, 128 rows 1.31, 8192 rows 1.11
-//   one or two against two   of 64 rows an expert .94 to 1.08, 128 rows .91 to 1.06, 512 rows .77 to .91, 8192 rows .60 to .75
-//   or four
+//   one against two, two     64 rows an expert .94 to 1.08, 128 rows .91 to 1.06, 512 rows .77 to .91, 8192 rows .60 to .75
+//   against four
 //   two against three        128 rows 1.11 to 1.22, 512 rows .98 to 1.05, 2048 rows .92 to .94
 //   four and six             24 rows 1.00 to 1.13, 64 rows .90 to 1.03, 512 rows .75 to .84
 //   eight and more           16 rows .80 to .92, 1024 rows .65 to .75

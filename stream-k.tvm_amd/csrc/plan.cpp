@@ -781,9 +781,10 @@ static bool wavek_pays(const sk_plan &other, int num_cus, const Times &wavek) {
       times.us[from] *= unaligned_rows(rows[from], nn ? 2 * N : (b16 ? 2 * K : K));
     // ([K, N] weights and up to 128 rows, which fill the others' tiles: 128 x 5120 x 5120 from HBM 30.1 us on those, 35.3 here against a
     // predicted 29, from the cache 25.2 / 23.1)
-    // (int8 and a K from 3000 on, where the others' own times are up to half above their predicted ones: of 100 random sizes of 65 to
-    // 320 rows those that go to the wave-K tiles by this take .67 to 1.0 of the others' time, one 1.1; 100 x 11008 x 4096 14.5 us here
-    // and 23.6 there.  Below that K a margin above 1 loses up to 1.16.)
+    // (int8 and a K from 3000 on, where the others' own times are up to half above their predicted ones.  Of 100 random sizes of 65 to
+    // 4000 rows that go to the wave-K tiles by this and not by 0.95 these take, of the others' time, .70 to 1.10 from the cache and .63
+    // to 1.06 from HBM; on average .90 and .80 up to 320 rows, .92 and .79 beyond; 100 x 11008 x 4096 14.5 us here and 23.6 there.
+    // Below that K a margin above 1 loses up to 1.16.)
     margin = ring ? 0.97 : (nn ? (M <= 128 ? 0.85 : 0.93) : (dtype == SK_I8 && K >= 3000 ? 1.05 : 0.95));
     // (products that take the others several full rounds: predicted closer than that they took 1.0 of the time from the cache and .97
     // from HBM, 1.4 at worst, int8 534 x 24608 x 9056 183 us there and 255 here)
