@@ -648,3 +648,13 @@ def test_a_recorded_call_keeps_its_workspace(sk):
             stream.synchronize()
             assert torch.equal(C, want) and all((t == 85).all() for t in others)
             large()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", [3, 4, 6])
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_tiles_that_kn_weights_do_not_have(sk, variant, dtype):
+    A, B = rand((20, 64), TYPES[dtype], 1), rand((2, 64, 32), TYPES[dtype], 2)
+    with pytest.raises(sk.StreamKError) as e:
+        sk.streamk_grouped(A, B, offsets_of([12, 8]), layout="nn", variant=variant)
+    assert e.value.status == -4
