@@ -84,7 +84,7 @@ bool grouped(const Tensor &rows, const Tensor &B, const Tensor &offsets, std::st
   const bool i8 = type == at::kChar, nn = layout == "nn";
   // ([K, N] weights multiply A's last piece of eight columns whole, those past K by zeros: they have to be finite, so they become zeros)
   const bool pad = nn && rows.is_cuda() && rows.dim() == 2 && rows.numel() > 0 && rows.size(1) % 8 != 0;
-  const Tensor A = pad ? at::constant_pad_nd(rows, {0, 8 - rows.size(1) % 8}) : rows;
+  const Tensor padded = pad ? at::constant_pad_nd(rows, {0, 8 - rows.size(1) % 8}) : Tensor(), &A = pad ? padded : rows;
   if ((!i8 && !is16(A)) || (!nn && layout != "nt") || (nn && i8) || B.scalar_type() != type || B.dim() != 3 || B.device() != A.device()) return false;
   if (!rows_in_place(A) && !one_row_in_place(A)) return false;
   const int64_t E = B.size(0), N = B.size(nn ? 2 : 1), K = B.size(nn ? 1 : 2), R = A.size(0);
@@ -247,10 +247,11 @@ using torch::autograd::variable_list;
   } while (0)
 bool wanted(const Tensor &t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 // (a dual tensor does not require a gradient: below autograd its tangent would be lost without a word)
-void no_tangent(const char *what, std::initializer_list<Tensor> operands) {
-  for (const Tensor &t : operands)
-    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), "streamk: ", what, " has no forward-mode derivative");
+void no_tangent(const char *what, std::initializer_list<const Tensor *> operands) {
+  for (const Tensor *t : operands)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->defined() || !t->_fw_grad(0).defined(), "streamk: ", what, " has no forward-mode derivative");
 }
+const Tensor *get(const MaybeTensor &t) { return t.has_value() ? &*t : nullptr; }
 
 // Passes a result on; who asks for its derivative by one of the operands that require one gets an error with the reason.
 struct Refused : torch::autograd::Function<Refused> {
@@ -294,14 +295,15 @@ struct GroupedProduct : torch::autograd::Function<GroupedProduct> {
 };
 Tensor gemm_grouped_autograd(const Tensor &A, const Tensor &B, const Tensor &offsets, c10::string_view layout, MaybeType out_dtype, const MaybeTensor &scale_a,
                              const MaybeTensor &scale_b, const MaybeTensor &bias, c10::string_view activation, int64_t variant) {
-  no_tangent("the grouped product", {A, B, scale_a.value_or(Tensor()), scale_b.value_or(Tensor()), bias.value_or(Tensor())});
+  no_tangent("the grouped product", {&A, &B, get(scale_a), get(scale_b), get(bias)});
   const bool plain = !scale_a.has_value() && !scale_b.has_value() && !bias.has_value() && activation == "none" &&
                      (!out_dtype.has_value() || *out_dtype == A.scalar_type()) && (layout == "nt" || layout == "nn");
   if (plain && (wanted(A) || wanted(B))) return GroupedProduct::apply(A, B, offsets, std::string(layout.data(), layout.size()), variant);
   const auto below = [&]() -> Tensor { BELOW(gemm_grouped, A, B, offsets, layout, out_dtype, scale_a, scale_b, bias, activation, variant); };
+  if (!at::GradMode::is_enabled()) return below();
   std::vector<Tensor> recorded;
-  for (const Tensor *t : {&A, &B, scale_a ? &*scale_a : nullptr, scale_b ? &*scale_b : nullptr, bias ? &*bias : nullptr})
-    if (t && wanted(*t)) recorded.push_back(*t);
+  for (const Tensor *t : {&A, &B, get(scale_a), get(scale_b), get(bias)})
+    if (t && t->requires_grad()) recorded.push_back(*t);
   if (recorded.empty()) return below();
   return Refused::apply(below(), at::TensorList(recorded), "the grouped product has gradients only without bias, activation, scales and out");
 }
@@ -330,7 +332,7 @@ struct RouteExperts : torch::autograd::Function<RouteExperts> {
   }
 };
 FiveTensors route_experts_autograd(const Tensor &logits, int64_t k) {
-  no_tangent("route_experts", {logits});
+  no_tangent("route_experts", {&logits});
   if (!wanted(logits)) BELOW(route_experts, logits, k);
   const variable_list r = RouteExperts::apply(logits, k);
   return {r[0], r[1], r[2], r[3], r[4]};
@@ -356,7 +358,7 @@ struct DispatchRows : torch::autograd::Function<DispatchRows> {
   }
 };
 Tensor dispatch_routed_autograd(const Tensor &x, const Tensor &order, const Tensor &place) {
-  no_tangent("dispatch_rows", {x});
+  no_tangent("dispatch_rows", {&x});
   if (wanted(x)) return DispatchRows::apply(x, order, place);
   BELOW(dispatch_routed, x, order, place);
 }
@@ -384,7 +386,7 @@ Tensor combine_routed(const Tensor &y, const Tensor &weights, const Tensor &orde
   return combine_rows(y, place, weights);
 }
 Tensor combine_routed_autograd(const Tensor &y, const Tensor &weights, const Tensor &order, const Tensor &place) {
-  no_tangent("combine_rows", {y, weights});
+  no_tangent("combine_rows", {&y, &weights});
   if (wanted(y) || wanted(weights)) return CombineRows::apply(y, weights, order, place);
   BELOW(combine_routed, y, weights, order, place);
 }

@@ -34,8 +34,8 @@ def _operator(name, schema, run, fake):
 
 
 def _no_tangent(what, *operands):
-    """(the native library's autograd implementations refuse by themselves)"""
-    if not _NATIVE and any(isinstance(t, torch.Tensor) and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in operands):
+    """(without the native library, whose autograd implementations refuse by themselves)"""
+    if any(isinstance(t, torch.Tensor) and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in operands):
         raise NotImplementedError(f"streamk: {what} has no forward-mode derivative")
 
 
@@ -206,7 +206,8 @@ def streamk_grouped(A, B, offsets, *, layout="nt", scale_a=None, scale_b=None, o
     once.  Differentiable in A and B without bias, activation, scales and out.  variant: which tiles run (sk_grouped in streamk.h); 0
     lets the sizes decide."""
     activation = activation or "none"
-    _no_tangent("the grouped product", A, B, bias, scale_a, scale_b)
+    if not _NATIVE:
+        _no_tangent("the grouped product", A, B, bias, scale_a, scale_b)
     if torch.is_grad_enabled() and (A.requires_grad or B.requires_grad or (bias is not None and bias.requires_grad)):
         if bias is not None or activation != "none" or scale_a is not None or scale_b is not None or out is not None:
             raise ValueError("the grouped product has gradients only without bias, activation, scales and out")
@@ -301,7 +302,8 @@ def route_experts(logits, k):
     """Route of the tokens whose router logits are [T, E] (float32, float16 or bfloat16): the k largest of each, the largest first, equal
     ones by number.  -inf and NaN are never chosen: a token with fewer others has -1 and weight 0 in its last places, and one with none
     goes to no expert.  Differentiable: weights to logits."""
-    _no_tangent("route_experts", logits)
+    if not _NATIVE:
+        _no_tangent("route_experts", logits)
     if not _NATIVE and torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
         return Route(*_RouteExperts.apply(logits, k))
     return Route(*_route_experts(logits, k))
@@ -402,7 +404,8 @@ class _CombineRows(torch.autograd.Function):
 def dispatch_rows(x, route):
     """The tokens' rows in the experts' order: [T k, H] for x [T, H] of any type (or [T k] for [T], such as the tokens' scales); zeros for
     the rows behind route.offsets[E].  Differentiable in x (float16 or bfloat16, two dimensions)."""
-    _no_tangent("dispatch_rows", x)
+    if not _NATIVE:
+        _no_tangent("dispatch_rows", x)
     if torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad:
         _on_device(x, "x", tuple(_TYPES), 2)
         if not _NATIVE:
@@ -413,7 +416,8 @@ def dispatch_rows(x, route):
 def combine_rows(y, route):
     """out[t] = sum over its experts of their weight times their row of y: [T, H] for y [T k, H] (float16 or bfloat16) in the experts' order;
     added in fp32, rounded once; a token without experts gets zeros.  Differentiable in y and route.weights."""
-    _no_tangent("combine_rows", y, route.weights)
+    if not _NATIVE:
+        _no_tangent("combine_rows", y, route.weights)
     if not _NATIVE and torch.is_grad_enabled() and isinstance(y, torch.Tensor) and (y.requires_grad or route.weights.requires_grad):
         return _CombineRows.apply(y, route.weights, route.order, route.place)
     return _combine_routed(y, route.weights, route.order, route.place)
