@@ -400,10 +400,10 @@ int sk_q4_quantize(const void *W, int64_t N, int64_t K, int64_t ldw, int group, 
  *
  * sk_gemm_i8_scaled: C[m][n] = activation(a[m] * b[n] * sum_k A[m][k] B[n][k] + bias[n]) for int8 A [M,K] and B [N,K], one fp32
  * scale for each row of A (token) and of B (output channel), C fp16 or bfloat16 (ldc in its elements).  The sums are exact int32 (up to
- * K = 131071 whatever the values); each becomes fp32 (rounded beyond 24 bits), is multiplied by a[m], then by b[n], and rounded once to C's type behind bias (C's
- * type) and activation.  The plan is made with dtype SK_I8 as for sk_gemm_i8; SK_ERR_CONFIG for plans of kernels that have no form
- * with scales (the general small-M kernels: a plan of up to 64 rows is made with reserved[0] = 9 or 12; sk_i8_scaled_takes says whether
- * it would run, 1 or 0).  Every schedule and
+ * K = 131071 whatever the values; beyond, one that does not fit wraps around, as in the int32 products); each becomes fp32 (rounded beyond
+ * 24 bits), is multiplied by a[m], then by b[n], and rounded once to C's type behind bias (C's type) and activation.  The plan is made
+ * with dtype SK_I8 as for sk_gemm_i8; SK_ERR_CONFIG for plans of kernels that have no form with scales (the general small-M kernels: a
+ * plan of up to 64 rows is made with reserved[0] = 9 or 12; sk_i8_scaled_takes says whether it would run, 1 or 0).  Every schedule and
  * fix-up gives the same bits.  Alignment as for sk_gemm_i8; C 2-byte, the scales 4-byte aligned.
  *
  * sk_quantize_i8: rows of X (SK_F16 or SK_BF16, row pitch ldx elements, M x K) to int8 Q (pitch ldq) and one fp32 scale a row:
@@ -426,13 +426,14 @@ int sk_quantize_i8(const void *X, int dtype, int64_t M, int64_t K, int64_t ldx, 
  *
  * sk_gemm_grouped: for offsets[e] <= r < offsets[e + 1]
  *   C[r] = activation(A[r] * op(B[e]) + bias[e])          SK_F16, SK_BF16
- *   C[r] = activation(scale_a[r] * scale_b[e][n] * (A[r] * B[e]^T)[n] + bias[e][n])      SK_I8, C in out_dtype
+ *   C[r] = activation(scale_a[r] * scale_b[e][n] * (A[r] * B[e]^T)[n] + bias[e][n])      SK_I8, C in out_dtype, sums as sk_gemm_i8_scaled's
  * offsets: E + 1 int32 in device memory, ascending from 0 to at most R (the host does not read them); groups of any size, zero
- * included.  Rows that no group holds are set to zero.  Offsets are clamped to 0 .. R and to ascending order before they are used, so
- * no content of theirs leads outside the operands.  B: E matrices, expert_b elements apart, each [N, K] (SK_LAYOUT_NT, pitch ldb) or
- * [K, N] (SK_LAYOUT_NN, 16-bit types).  bias: [E, N] in C's type, contiguous, or null.  lda, ldb and expert_b multiples of 8 (int8:
- * 16), SK_LAYOUT_NT: K too; SK_LAYOUT_NN: N too, and where K is none, A has zeros in its columns from K to the next; A and B 16-byte, C and bias 2-byte, scales 4-byte aligned.  256 rows of A, of C and of
- * [N, K] weights, and K + 64 rows of [K, N] weights (an expert's all), span less than 2 GiB.  The same bits on every launch.
+ * included.  Rows that no group holds are set to zero.  Offsets are clamped to 0 .. R and a group's end to its start before they
+ * are used, so no content of theirs leads outside the operands.  B: E matrices, expert_b elements apart, each [N, K] (SK_LAYOUT_NT,
+ * pitch ldb) or [K, N] (SK_LAYOUT_NN, 16-bit types).  bias: [E, N] in C's type, contiguous, or null.  lda, ldb and expert_b multiples of 8 (int8:
+ * 16), SK_LAYOUT_NT: K too; SK_LAYOUT_NN: N too, and where K is none, A has zeros in its columns from K to the next; A and B 16-byte, C
+ * and bias 2-byte, scales 4-byte aligned.  256 rows of A, of C and of [N, K] weights, and K + 64 rows of [K, N] weights (an expert's
+ * all), span less than 2 GiB.  The same bits on every launch.
  * ws: as for the other products (sk_workspace_init has run on it).  Variant 2 may cut a tile along K; the CTA that comes last to it waits
  * for the others' stores, spin_limit polls at most.  If it gives up, the tile is not stored and sk_workspace_status says
  * SK_ERR_TIMEOUT.  No other variant waits for part of itself.

@@ -100,7 +100,8 @@ def quantize_int8(x):
 
 
 def streamk_int8_scaled(A, B, scale_a, scale_b, *, out_dtype=torch.float16, out=None, plan=None, config=None, bias=None, activation=None, **kw):
-    """C = activation(scale_a[:, None] * scale_b * (A @ B.T) + bias) for int8 A [M, K] and B [N, K]: exact int32 sums, scales float32
+    """C = activation(scale_a[:, None] * scale_b * (A @ B.T) + bias) for int8 A [M, K] and B [N, K]: exact int32 sums (whatever the
+    values up to K = 131071), scales float32
     [M] and [N], C float16 or bfloat16 (`out_dtype`, which bias shares), rounded once.  Plans are those of streamk_int8; up to 64
     rows those that operator calls take."""
     cfg = ops._config_string(plan, config, kw)

@@ -63,7 +63,10 @@ class StreamKMoE(torch.nn.Module):
         return m
 
     def route(self, x):
-        """The route of x [T, hidden].  The router's product is one group of all rows; its logits are rounded to x's type."""
+        """The route of x [T, hidden].  The router's product is one group of all rows.  Its logits come in x's type, as those of a linear
+        layer in that type do: a half unit of a logit, 2^-8 of it in bfloat16, moves its token's weights by about as much and decides
+        between experts that are that close.  Who wants them finer makes them in float32 and calls route_experts.  A token with a NaN
+        has NaN logits, which are never chosen: it goes to no expert and comes back as zeros."""
         T = x.shape[0]
         everyone = torch.arange(0, 2 * T, T, dtype=torch.int32, device=x.device)
         return route_experts(streamk_grouped(x, self.router[None], everyone), self.chosen)
