@@ -428,8 +428,8 @@ int sk_quantize_i8(const void *X, int dtype, int64_t M, int64_t K, int64_t ldx, 
  *   C[r] = activation(A[r] * op(B[e]) + bias[e])          SK_F16, SK_BF16
  *   C[r] = activation(scale_a[r] * scale_b[e][n] * (A[r] * B[e]^T)[n] + bias[e][n])      SK_I8, C in out_dtype, sums as sk_gemm_i8_scaled's
  * offsets: E + 1 int32 in device memory, ascending from 0 to at most R (the host does not read them); groups of any size, zero
- * included.  Rows that no group holds are set to zero.  Offsets are clamped to 0 .. R and a group's end to its start before they
- * are used, so no content of theirs leads outside the operands.  B: E matrices, expert_b elements apart, each [N, K] (SK_LAYOUT_NT,
+ * included.  Rows that no group holds are set to zero.  Offsets are clamped to 0 .. R and to ascending order (one below another
+ * in front of it counts as that) before they are used, so no content of theirs leads outside the operands.  B: E matrices, expert_b elements apart, each [N, K] (SK_LAYOUT_NT,
  * pitch ldb) or [K, N] (SK_LAYOUT_NN, 16-bit types).  bias: [E, N] in C's type, contiguous, or null.  lda, ldb and expert_b multiples of 8 (int8:
  * 16), SK_LAYOUT_NT: K too; SK_LAYOUT_NN: N too, and where K is none, A has zeros in its columns from K to the next; A and B 16-byte, C
  * and bias 2-byte, scales 4-byte aligned.  256 rows of A, of C and of [N, K] weights, and K + 64 rows of [K, N] weights (an expert's

@@ -7,7 +7,8 @@
 // of 64 groups, done once where there are no more (the tiles of a CTA come in ascending order).
 //
 // Groups 0 and E + 1 are the rows in front of offsets[0] and behind offsets[E], which no expert owns: zeros are stored for them, so
-// that every row of C is written.  Offsets are clamped to 0 <= lo <= hi <= R, whatever they hold: no access leaves the operands.
+// that every row of C is written.  Offsets are clamped to 0 .. R and none counts that is below one in front of it: whatever they hold, the
+// groups lie side by side, no access leaves the operands, and there are no more tiles than the host reckons with.
 //
 // The tiles themselves are those of the ordinary products, each with its arguments moved to the expert's operands.
 #pragma once
@@ -53,18 +54,18 @@ struct GroupWalk {
   const int *offsets;
   int E, R, tiles_n;
   int chunk, before;             // groups 64 chunk .. + 63 are in the lanes; tiles of the groups in front of them
+  int reached;                   // the largest offset of this chunk and those in front of it
   int lo, rows, ends;            // this lane's group: first row, rows, tiles of the chunk up to its last one
 
   __device__ __forceinline__ GroupWalk(const int *o, int E_, int R_, int tn) : offsets(o), E(E_), R(R_), tiles_n(tn), before(0) { load(0); }
   __device__ __forceinline__ void load(int c) {
     chunk = c;
-    const int lane = threadIdx.x & 63, g = 64 * c + lane;
-    lo = rows = 0;
-    if (g <= E + 1) {
-      lo = g == 0 ? 0 : min(max(offsets[g - 1], 0), R);
-      rows = (g == E + 1 ? R : min(max(offsets[g], lo), R)) - lo;
-      if (!UNOWNED && (g == 0 || g == E + 1)) rows = 0;
-    }
+    const int lane = threadIdx.x & 63, g = 64 * c + lane, before_chunk = c == 0 ? 0 : reached;
+    // this group's end, and the one in front of it (from the lane below: 0x138)
+    const int end = max((int)wave_max_up_to((uint32_t)min(max(offsets[min(g, E)], 0), R)), before_chunk);
+    lo = __builtin_amdgcn_update_dpp(before_chunk, end, 0x138, 0xf, 0xf, false);
+    rows = UNOWNED ? (g == E + 1 ? R : end) - lo : (g == 0 ? 0 : end - lo);   // (behind E: end is lo)
+    reached = __builtin_amdgcn_readlane(end, 63);
     int x = (int)((unsigned)(rows + BM - 1) / BM) * tiles_n;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -73,14 +74,17 @@ struct GroupWalk {
     }
     ends = x;
   }
-  // tiles of all groups (before the first find)
-  __device__ __forceinline__ int total_tiles() {
+  // tiles of all groups (before the first find); front, back: the rows in front of all experts' and behind them begin and end there
+  __device__ __forceinline__ int total_tiles(int &front, int &back) {
     int sum = __builtin_amdgcn_readlane(ends, 63);
+    front = __builtin_amdgcn_readlane(lo, 1);
+    back = reached;
     if (E + 1 < 64) return sum;
     for (int c = 1; 64 * c <= E + 1; ++c) {
       load(c);
       sum += __builtin_amdgcn_readlane(ends, 63);
     }
+    back = reached;
     load(0);
     return sum;
   }
@@ -204,8 +208,7 @@ struct SkRuns {
   }
 };
 // rows without an expert become zeros, shared out over the grid
-__device__ __forceinline__ void zero_unowned(const GroupedArgs &g, int pid, int threads) {
-  const int front = min(max(g.offsets[0], 0), g.R), back = min(max(g.offsets[g.E], front), g.R);
+__device__ __forceinline__ void zero_unowned(const GroupedArgs &g, int pid, int threads, int front, int back) {
   const int rows = front + g.R - back;
   for (int r = pid; r < rows; r += g.grid) {
     half_t *C = g.C + (int64_t)(r < front ? r : back + r - front) * g.ldc;
@@ -219,8 +222,9 @@ __device__ __forceinline__ void run_grouped_sk(const GroupedArgs &g, int ipt, co
   static_assert(P::COHERENT_PARTIALS && P::FIXUP_WORD_IN_LDS, "see above");
   GroupWalk<P::BM, false> walk(g.offsets, g.E, g.R, g.tiles_n);
   const int pid = grouped_pid(g.grid);
-  zero_unowned(g, pid, P::NT);
-  const int tiles = walk.total_tiles(), whole = tiles - (int)((unsigned)tiles % (unsigned)g.grid);
+  int front, back;
+  const int tiles = walk.total_tiles(front, back), whole = tiles - (int)((unsigned)tiles % (unsigned)g.grid);
+  zero_unowned(g, pid, P::NT, front, back);
   auto slot = [&](int p, int which) { return ws.partials + (size_t)(2 * p + which) * P::TILE_ELEMS; };
   typename P::Acc acc;
   GroupTile t;

@@ -123,8 +123,9 @@ __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_grouped_asm_kernel(
   constexpr auto LOW = P::LOW_TILE, FULL = NN ? P::WHOLE_TILE : P::WRAPPED_TILE;
   GroupWalk<P::BM, false> walk(g.offsets, g.E, g.R, g.tiles_n);
   const int pid = grouped_pid(g.grid);
-  zero_unowned(g, pid, P::NT);
-  const int tiles = walk.total_tiles();
+  int front, back;
+  const int tiles = walk.total_tiles(front, back);
+  zero_unowned(g, pid, P::NT, front, back);
   const Cuts cuts(tiles, g.grid, ipt);
   struct Segment {
     GroupTile t;

@@ -257,8 +257,8 @@ __device__ __forceinline__ uint4v ld_coherent16(BufferRsrc r, uint32_t off, uint
   return __builtin_bit_cast(uint4v, __builtin_amdgcn_raw_buffer_load_b128(r, off, uoff, CACHE_POLICY_SC1));
 }
 
-// the largest value of a wave's lanes, in every lane
-__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+// the largest value of a wave's lanes up to each lane
+__device__ __forceinline__ uint32_t wave_max_up_to(uint32_t x) {
 #define SK_MAX_STEP(CTRL, ROWS) x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false))
   SK_MAX_STEP(0x111, 0xf);   // rows of 16 lanes: from 1, 2, 4, 8 lanes below; then the last lane of a row to the next row, and of
   SK_MAX_STEP(0x112, 0xf);   // the lower half to the upper
@@ -267,8 +267,10 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
   SK_MAX_STEP(0x142, 0xa);
   SK_MAX_STEP(0x143, 0xc);
 #undef SK_MAX_STEP
-  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+  return x;
 }
+// of all of them, in every lane
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_max_up_to(x), 63); }
 
 // Direct global -> LDS load, 16 bytes per lane: lane l's data lands at lds_base + 16*l.  Issued as
 // inline assembly on purpose: the compiler's wait-count insertion cannot tell which LDS stage an

@@ -658,3 +658,38 @@ def test_tiles_that_kn_weights_do_not_have(sk, variant, dtype):
     with pytest.raises(sk.StreamKError) as e:
         sk.streamk_grouped(A, B, offsets_of([12, 8]), layout="nn", variant=variant)
     assert e.value.status == -4
+
+
+# ---- offsets that are no offsets ----
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["float16 nt", "bfloat16 nn", "int8"])
+@pytest.mark.parametrize("variant", [0, 1, 2, 3, 4, 5, 6])
+@pytest.mark.parametrize("offsets", [[0, 30, 10, 50], [-5, 20, 90, 40], [100, 0, 100, 0], [60, 50, 40, 30], [7, 7, 3, 100000], [0, 100] * 40 + [0], [(37 * i) % 101 for i in range(200)]])
+def test_offsets_out_of_order(sk, kind, variant, offsets):
+    """They are clamped to 0 .. R and to ascending order, one below another in front of it counting as that."""
+    R, N, K, E = 100, 264, 256, len(offsets) - 1
+    if kind.endswith("nn") and variant in (3, 4, 6):
+        pytest.skip("no such tile for [K, N] weights")
+    wild = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    sane = wild.clamp(0, R).cummax(0).values
+    if kind == "int8":
+        g = torch.Generator().manual_seed(R)
+        A, B = (torch.randint(-127, 128, s, generator=g, dtype=torch.int8).cuda() for s in ((R, K), (E, N, K)))
+        sa, sb = torch.rand(R, generator=g).cuda(), (torch.rand(E, N, generator=g) / (73 * math.sqrt(K))).cuda()
+        run = lambda o: sk.streamk_grouped(A, B, o, scale_a=sa, scale_b=sb, variant=variant)  # noqa: E731
+    else:
+        dtype, layout = kind.split()
+        A, B = rand((R, K), TYPES[dtype], 1), rand((E, N, K) if layout == "nt" else (E, K, N), TYPES[dtype], 2, 1 / 16)
+        run = lambda o: sk.streamk_grouped(A, B, o, layout=layout, variant=variant)  # noqa: E731
+    C = run(sane.int())
+    assert torch.equal(run(wild), C) and not C[:int(sane[0])].any() and not C[int(sane[-1]):].any()
+
+
+@pytest.mark.gpu
+def test_offsets_out_of_order_make_no_more_tiles(sk):
+    """As they stand they would name 2^31 iterations and more."""
+    R, N, K, E = 40960, 2048, 4096, 1024
+    A, B = rand((R, K), torch.float16, 1), rand((1, N, K), torch.float16, 2, 1 / 64)
+    wild = torch.tensor([0, R] * (E // 2) + [0], dtype=torch.int32, device="cuda")
+    C = sk.streamk_grouped(A, B.expand(E, N, K), wild, variant=3)
+    assert torch.equal(C, sk.streamk_grouped(A, B, offsets_of([R]), variant=3))
