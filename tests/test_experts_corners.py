@@ -93,6 +93,11 @@ def test_columns_beside_a_gradient_do_not_count(sk, dtype):
         assert_near(dw[e], d[at].double().T @ A[at].double(), sizes[e], d[at].double().abs().T @ A[at].double().abs())
 
 
+def tiles_of(*kinds):
+    """(kind, variant) of the tiles that there are: [K, N] weights have three of the six"""
+    return [(kind, variant) for kind in kinds for variant in ((1, 2, 5) if kind.endswith("nn") else (1, 2, 3, 4, 5, 6))]
+
+
 # ---- activations of what is not finite ----
 ACTIVATIONS = ["relu", "gelu_tanh", "silu"]
 
@@ -130,12 +135,9 @@ def test_products_keep_nan_through_activations(sk, activation, dtype, M, kw):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("activation", ACTIVATIONS)
-@pytest.mark.parametrize("kind", ["float16 nt", "bfloat16 nt", "float16 nn", "bfloat16 nn"])
-@pytest.mark.parametrize("variant", [1, 2, 3, 4, 5, 6])
+@pytest.mark.parametrize("kind,variant", tiles_of("float16 nt", "bfloat16 nt", "float16 nn", "bfloat16 nn"))
 def test_grouped_products_keep_nan_through_activations(sk, activation, kind, variant):
     dtype, layout = kind.split()
-    if layout == "nn" and variant not in (1, 2, 5):
-        pytest.skip("no such tile for [K, N] weights")
     sizes, N, K, t = [70, 0, 130], 264, 256, TYPES[dtype]
     A, B, bias = rand((200, K), t, 1), rand((3, N, K), t, 2, 1 / 16), torch.zeros(3, N, dtype=t, device="cuda")
     good = A.clone()
@@ -662,14 +664,11 @@ def test_tiles_that_kn_weights_do_not_have(sk, variant, dtype):
 
 # ---- offsets that are no offsets ----
 @pytest.mark.gpu
-@pytest.mark.parametrize("kind", ["float16 nt", "bfloat16 nn", "int8"])
-@pytest.mark.parametrize("variant", [0, 1, 2, 3, 4, 5, 6])
+@pytest.mark.parametrize("kind,variant", [(kind, 0) for kind in ("float16 nt", "bfloat16 nn", "int8")] + tiles_of("float16 nt", "bfloat16 nn", "int8"))
 @pytest.mark.parametrize("offsets", [[0, 30, 10, 50], [-5, 20, 90, 40], [100, 0, 100, 0], [60, 50, 40, 30], [7, 7, 3, 100000], [0, 100] * 40 + [0], [(37 * i) % 101 for i in range(200)]])
 def test_offsets_out_of_order(sk, kind, variant, offsets):
     """They are clamped to 0 .. R and to ascending order, one below another in front of it counting as that."""
     R, N, K, E = 100, 264, 256, len(offsets) - 1
-    if kind.endswith("nn") and variant in (3, 4, 6):
-        pytest.skip("no such tile for [K, N] weights")
     wild = torch.tensor(offsets, dtype=torch.int32, device="cuda")
     sane = wild.clamp(0, R).cummax(0).values
     if kind == "int8":
