@@ -479,6 +479,24 @@ int sk_grouped_wgrad(const void *A, const void *B, const void *offsets, void *C,
  * added in fp32 in the order of j.  With weights null it is the gradient of sk_dispatch_rows.
  * sk_combine_backward: dy [T * k, H] (zeros for rows without a slot) and dweights [T, k] of sk_combine_rows.
  */
+/*
+ * sk_route_scored: the same with scores s = softmax(z) over the token's experts or s = sigmoid(z), and c = s + bias[e] (fp32 [E], or null).
+ * Of `groups` equal groups of neighbouring experts (1 to 64, a divisor of E) the chosen_groups stay open whose two largest c (of a group
+ * with one expert that can be chosen: its c) have the largest sums; the k largest c among the open experts are chosen -- without a
+ * bias the k largest logits --, equal ones by number, groups too.  An expert whose c is -infinity or NaN is never chosen.  weights = s of the
+ * chosen (without the bias), divided by their sum if `renormalize`, times `scale`.  Scores, sums and comparisons are in 64 bits.
+ * sk_route_scored_backward: dlogits of it, of the same logits and the experts that it chose; the bias has no part in it.
+ */
+typedef enum sk_scores_kind { SK_SCORES_SOFTMAX = 0, SK_SCORES_SIGMOID = 1 } sk_scores_kind;
+typedef struct sk_route_scores {
+  const void *bias;
+  double scale;
+  int32_t scores, renormalize, groups, chosen_groups;
+} sk_route_scores;
+int sk_route_scored(const void *logits, int dtype, int64_t T, int64_t E, int64_t k, int64_t ld, const sk_route_scores *scores, void *weights, void *experts,
+                    void *offsets, void *order, void *place, void *ws, size_t ws_bytes, void *stream);
+int sk_route_scored_backward(const void *logits, int dtype, int64_t T, int64_t E, int64_t k, int64_t ld, const sk_route_scores *scores, const void *experts,
+                             const void *dweights, void *dlogits, void *stream);
 size_t sk_route_workspace_bytes(int64_t T, int64_t E, int64_t k);
 int sk_route_experts(const void *logits, int dtype, int64_t T, int64_t E, int64_t k, int64_t ld, void *weights, void *experts, void *offsets,
                      void *order, void *place, void *ws, size_t ws_bytes, void *stream);

@@ -17,7 +17,7 @@ using namespace sk;
 
 namespace {
 
-constexpr int MAX_EXPERTS = 1024, MAX_CHOSEN = 64;
+constexpr int MAX_EXPERTS = 1024, MAX_CHOSEN = 64, MAX_GROUPS = 64;
 enum { EL_F16 = 0, EL_BF16 = 1, EL_F32 = 2 };
 
 template <int EL>
@@ -90,6 +90,152 @@ __device__ __forceinline__ void choose(const void *logits, int64_t ld, int t, in
   weight = expert >= 0 ? e / sum : 0.f;
 }
 
+// ---- scores, a bias for balance, groups ----
+//   s = sigmoid(z), or softmax(z) over all experts;  c = s + bias
+//   of `groups` equal groups of experts, neighbours in number, the chosen_groups with the largest sum of their two largest c stay open;
+//   the k largest c among the open (without a bias: the k largest z, in whose order the scores are), ties to the lower number;
+//   weights = s of the chosen, divided by their sum if renormalised, times a factor.
+// Two experts' c may differ by less than 32 bits tell, and the choice is a whole number that two programs should agree on: scores, sums and
+// comparisons are in 64 bits.  The arithmetic is a few dozen 64-bit operations a logit; what bounds the kernel is the chain of reductions
+// over the wave that a token is, two for each group and one for each of the k.
+struct Scores {
+  const float *bias;   // [E] or null
+  double scale;
+  int groups, chosen_groups;
+  bool sigmoid, renormalize;
+};
+
+// doubles as unsigned numbers in the same order; 0: not to be chosen
+__device__ __forceinline__ uint64_t order_key64(double c) {
+  c += 0.;
+  const uint64_t b = __builtin_bit_cast(uint64_t, c);
+  if (!(c > -__builtin_inf())) return 0;
+  return b >> 63 ? ~b : b | 1ull << 63;
+}
+__device__ __forceinline__ double value_of_key(uint64_t k) { return __builtin_bit_cast(double, k >> 63 ? k ^ 1ull << 63 : ~k); }
+__device__ __forceinline__ double wave_sum(double x) {
+#pragma unroll
+  for (int d = 32; d > 0; d /= 2) x += __shfl_xor(x, d, 64);
+  return x;
+}
+// the largest of all lanes, and the first lane that has it: most often the upper halves tell
+__device__ __forceinline__ uint64_t wave_max64(uint64_t x, int &lane) {
+  const uint32_t hi = (uint32_t)(x >> 32), top = wave_max(hi);
+  uint64_t at = __builtin_amdgcn_ballot_w64(hi == top);
+  uint32_t low = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, __builtin_ctzll(at));
+  if (at & (at - 1)) {   // (uniform)
+    low = wave_max(hi == top ? (uint32_t)x : 0);
+    at = __builtin_amdgcn_ballot_w64(hi == top && (uint32_t)x == low);
+  }
+  lane = __builtin_ctzll(at);
+  return (uint64_t)top << 32 | low;
+}
+__device__ __forceinline__ double sigmoid64(double z) { return 1. / (1. + exp(-z)); }
+// e^(z - m); infinities of both as the limit
+__device__ __forceinline__ double exp_from(double z, double m) { return z == m ? 1. : exp(z - m); }
+
+// The weights of the lanes' chosen experts, whose logits are z (expert < 0: none); most, sum: of all experts (softmax not renormalised).
+// share: before the factor.
+__device__ __forceinline__ double chosen_share(const Scores &p, int expert, float z, double most, double sum) {
+  if (!p.renormalize) return expert < 0 ? 0. : (p.sigmoid ? sigmoid64(z) : exp_from(z, most) / sum);
+  // scores that underflow have quotients all the same: sigmoid(z) = e^(z - m) / (1 + e^z) times e^m
+  const uint32_t top = wave_max(expert < 0 ? 0 : order_key(z));
+  const double m = __builtin_bit_cast(float, top & 0x80000000u ? top ^ 0x80000000u : ~top);
+  double s = 0.;
+  if (expert >= 0) s = p.sigmoid ? (m < -600. ? exp_from(z, m) / (1. + exp((double)z)) : sigmoid64(z)) : exp_from(z, m);
+  const double all = wave_sum(s);
+  return expert < 0 ? 0. : s / all;
+}
+
+// As choose(): lane l holds the logits S l .. S l + S - 1, so that its first is the lowest.
+template <int EL, int S>
+__device__ __forceinline__ void choose_scored(const void *logits, int64_t ld, int t, int E, int k, const Scores &p, int &expert, float &weight) {
+  const int lane = threadIdx.x & 63;
+  float z[S];
+  bool there[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    z[s] = S * lane + s < E ? load_el<EL>(logits, t * ld + S * lane + s) : -__builtin_inff();
+    there[s] = z[s] > -__builtin_inff();   // (neither -inf nor NaN)
+  }
+  double most = 0., sum = 1.;
+  if (!p.sigmoid && (p.bias || p.groups > 1 || !p.renormalize)) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int s = 0; s < S; ++s) top = max(top, order_key(z[s]));
+    top = wave_max(top);
+    most = __builtin_bit_cast(float, top & 0x80000000u ? top ^ 0x80000000u : ~top);
+    double part = 0.;
+#pragma unroll
+    for (int s = 0; s < S; ++s) part += there[s] ? exp_from(z[s], most) : 0.;
+    sum = wave_sum(part);
+  }
+  uint64_t key[S];
+  if (p.bias || p.groups > 1) {   // (uniform)
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      double c = p.sigmoid ? sigmoid64(z[s]) : exp_from(z[s], most) / sum;
+      if (p.bias && there[s]) c += (double)p.bias[S * lane + s];
+      key[s] = there[s] ? order_key64(c) : 0;
+    }
+  }
+  if (p.groups > 1) {
+    const int size = (int)((unsigned)E / (unsigned)p.groups);
+    uint64_t mine = 0;   // lane g: group g's
+    for (int g = 0; g < p.groups; ++g) {
+      uint64_t first = 0, second = 0;
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        const bool in = (unsigned)(S * lane + s - g * size) < (unsigned)size;
+        const uint64_t x = in ? key[s] : 0;
+        second = max(second, min(first, x));
+        first = max(first, x);
+      }
+      int at;
+      const uint64_t a = wave_max64(first, at);
+      if (a == 0) continue;
+      int unused;
+      const uint64_t b = wave_max64(lane == at ? second : first, unused);
+      const double c = value_of_key(a) + (b ? value_of_key(b) : 0.);
+      if (lane == g) mine = order_key64(c);
+    }
+    uint64_t open = 0;
+    for (int j = 0; j < p.chosen_groups; ++j) {
+      int at;
+      if (wave_max64(mine, at) == 0) break;
+      open |= 1ull << at;
+      if (lane == at) mine = 0;
+    }
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      if (!(open >> min(63u, (unsigned)(S * lane + s) / (unsigned)size) & 1)) key[s] = 0;
+  }
+  if (!p.bias) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) key[s] = p.groups > 1 && key[s] == 0 ? 0 : (uint64_t)order_key(z[s]) << 32;
+  }
+  expert = -1;
+  for (int j = 0; j < k; ++j) {
+    uint64_t best = key[0];
+    int which = 0;
+#pragma unroll
+    for (int s = 1; s < S; ++s)
+      if (key[s] > best) {
+        best = key[s];
+        which = s;
+      }
+    int at;
+    if (wave_max64(best, at) == 0) break;
+    const int e = __builtin_amdgcn_readlane(S * lane + which, at);
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      if (S * lane + s == e) key[s] = 0;
+    if (lane == j) expert = e;
+  }
+  const float own = expert >= 0 ? load_el<EL>(logits, t * ld + expert) : 0.f;
+  weight = (float)(p.scale * chosen_share(p, expert, own, most, sum));
+}
+
 struct RouteArgs {
   const void *logits;
   int64_t ld;
@@ -98,7 +244,14 @@ struct RouteArgs {
   int *experts, *offsets, *order, *place;  // [T, k], [E + 1], [T k], [T k]
   int *counts;                             // [blocks, E]: slots of a block's tokens by expert
   int tokens;                              // of a block
+  Scores scores;
 };
+// SCORED: by scores, bias and groups
+template <int EL, int S, bool SCORED>
+__device__ __forceinline__ void choose_by(const RouteArgs &a, int t, int &expert, float &weight) {
+  if constexpr (SCORED) choose_scored<EL, S>(a.logits, a.ld, t, a.E, a.k, a.scores, expert, weight);
+  else choose<EL, S>(a.logits, a.ld, t, a.E, a.k, expert, weight);
+}
 
 // The slots of a range, in order, 64 at a time by each of the block's waves, which own consecutive parts of it: start[e] + slots with
 // expert e in front.  have: LDS, [waves][E] counts of the waves' parts, replaced by where their rows go.
@@ -172,7 +325,7 @@ __device__ __forceinline__ int scan_experts(int *total, int E, int *word) {
 constexpr int FEW_TOKENS = 64, FEW_EXPERTS = 256, FEW_WAVES = 16;   // one workgroup does it all
 // (two launches take about 4 us more than one; 64 tokens are four for each wave of the workgroup)
 
-template <int EL, int S>
+template <int EL, int S, bool SCORED>
 __global__ __launch_bounds__(64 * FEW_WAVES) void route_few_kernel(RouteArgs a) {
   extern __shared__ int lds[];
   int *experts = lds, *have = lds + FEW_TOKENS * a.k, *total = have + FEW_WAVES * a.E, *word = total + a.E;
@@ -180,7 +333,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void route_few_kernel(RouteArgs a) 
   for (int t = wave; t < a.T; t += FEW_WAVES) {
     int e;
     float w;
-    choose<EL, S>(a.logits, a.ld, t, a.E, a.k, e, w);
+    choose_by<EL, S, SCORED>(a, t, e, w);
     if (lane < a.k) {
       experts[t * a.k + lane] = e;
       a.experts[t * a.k + lane] = e;
@@ -213,17 +366,21 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void route_few_kernel(RouteArgs a) 
 
 // More tokens: choice and counts by blocks, then places.  8192 tokens, 8 of 64 experts: 4 and 9 us (four waves a block for the choice 28 us:
 // a token is a chain of k reductions).
-constexpr int WAVES = 4, CHOOSE_WAVES = 16;
-template <int EL, int S>
-__global__ __launch_bounds__(64 * CHOOSE_WAVES) void route_choose_kernel(RouteArgs a) {
+// (sixteen scores in 64 bits to a lane do not fit the registers of sixteen waves)
+constexpr int WAVES = 4;
+template <int S, bool SCORED>
+constexpr int choose_threads = SCORED && S == 16 ? 512 : 1024;
+template <int EL, int S, bool SCORED>
+__global__ __launch_bounds__((choose_threads<S, SCORED>)) void route_choose_kernel(RouteArgs a) {
   extern __shared__ int lds[];   // [E] counts of the block
+  constexpr int CHOOSE_WAVES = choose_threads<S, SCORED> / 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t0 = blockIdx.x * a.tokens, t1 = min(a.T, t0 + a.tokens);
   for (int e = threadIdx.x; e < a.E; e += 64 * CHOOSE_WAVES) lds[e] = 0;
   __syncthreads();
   for (int t = t0 + wave; t < t1; t += CHOOSE_WAVES) {
     int e;
     float w;
-    choose<EL, S>(a.logits, a.ld, t, a.E, a.k, e, w);
+    choose_by<EL, S, SCORED>(a, t, e, w);
     if (lane < a.k) {
       a.experts[(int64_t)t * a.k + lane] = e;
       a.weights[(int64_t)t * a.k + lane] = w;
@@ -287,24 +444,31 @@ int route_blocks(int64_t T, int64_t E) {
   return T <= FEW_TOKENS && E <= FEW_EXPERTS ? 0 : (int)((T + route_tokens(T) - 1) / route_tokens(T));
 }
 
-template <int EL, int S>
+template <int EL, int S, bool SCORED>
 int launch_route(const RouteArgs &a, int blocks, hipStream_t s) {
-  if (blocks == 0) {
-    const size_t lds = sizeof(int) * (FEW_TOKENS * a.k + (FEW_WAVES + 1) * a.E + 1);
-    hipLaunchKernelGGL((route_few_kernel<EL, S>), dim3(1), dim3(64 * FEW_WAVES), lds, s, a);
-    return (int)hipGetLastError();
+  if constexpr (64 * S <= FEW_EXPERTS) {
+    if (blocks == 0) {
+      const size_t lds = sizeof(int) * (FEW_TOKENS * a.k + (FEW_WAVES + 1) * a.E + 1);
+      hipLaunchKernelGGL((route_few_kernel<EL, S, SCORED>), dim3(1), dim3(64 * FEW_WAVES), lds, s, a);
+      return (int)hipGetLastError();
+    }
   }
-  hipLaunchKernelGGL((route_choose_kernel<EL, S>), dim3(blocks), dim3(64 * CHOOSE_WAVES), sizeof(int) * a.E, s, a);
+  hipLaunchKernelGGL((route_choose_kernel<EL, S, SCORED>), dim3(blocks), dim3((choose_threads<S, SCORED>)), sizeof(int) * a.E, s, a);
   if (hipGetLastError() != hipSuccess) return 1;
   hipLaunchKernelGGL(route_place_kernel, dim3(blocks), dim3(64 * WAVES), sizeof(int) * ((WAVES + 2) * a.E + 1), s, a);
   return (int)hipGetLastError();
 }
-template <int EL>
+template <int EL, bool SCORED>
 int launch_route_of(const RouteArgs &a, int blocks, hipStream_t s) {
-  if (a.E <= 64) return launch_route<EL, 1>(a, blocks, s);
-  if (a.E <= 128) return launch_route<EL, 2>(a, blocks, s);
-  if (a.E <= 256) return launch_route<EL, 4>(a, blocks, s);
-  return launch_route<EL, 16>(a, blocks, s);
+  if (a.E <= 64) return launch_route<EL, 1, SCORED>(a, blocks, s);
+  if (a.E <= 128) return launch_route<EL, 2, SCORED>(a, blocks, s);
+  if (a.E <= 256) return launch_route<EL, 4, SCORED>(a, blocks, s);
+  return launch_route<EL, 16, SCORED>(a, blocks, s);
+}
+template <bool SCORED>
+int launch_route_by(int el, const RouteArgs &a, int blocks, hipStream_t s) {
+  return el == EL_F16 ? launch_route_of<EL_F16, SCORED>(a, blocks, s)
+                      : (el == EL_BF16 ? launch_route_of<EL_BF16, SCORED>(a, blocks, s) : launch_route_of<EL_F32, SCORED>(a, blocks, s));
 }
 
 // d logits[t][e_j] = w_j (dw_j - sum_i w_i dw_i); one wave per token (8192 tokens, 64 experts: 5 us)
@@ -328,6 +492,78 @@ __global__ __launch_bounds__(64 * WAVES) void route_backward_kernel(const float 
   __syncthreads();
   if (t < T)
     for (int e = lane; e < E; e += 64) store_el<EL>(dlogits, t * E + e, row[e]);
+}
+
+// The same with scores: with g = factor * dw, r the shares and s the scores of the chosen, by the scores' own formula
+//   sigmoid   g_j s_j (1 - s_j), renormalised r_j (1 - s_j) (g_j - sum r g)
+//   softmax   s_e (g_e - sum s g) for every expert of the token (g is 0 for the others), renormalised r_j (g_j - sum r g)
+// computed again from the logits in 64 bits: differences of nearly equal gradients keep their digits.
+template <int EL, int S>
+__global__ __launch_bounds__(64 * WAVES) void route_scored_backward_kernel(const void *logits, int64_t ld, const int *experts, const float *dweights, int T, int E,
+                                                                           int k, Scores p, void *dlogits) {
+  extern __shared__ float row_lds[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t t = wide_block() * WAVES + wave;
+  if (t >= T) return;   // (a wave's rows are its own: no barrier)
+  float *row = row_lds + wave * E;
+  double most = 0., sum = 1.;
+  float z[S];
+  const bool all = !p.sigmoid && !p.renormalize;
+  if (all) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      z[s] = 64 * s + lane < E ? load_el<EL>(logits, t * ld + 64 * s + lane) : -__builtin_inff();
+      top = max(top, order_key(z[s]));
+    }
+    top = wave_max(top);
+    most = __builtin_bit_cast(float, top & 0x80000000u ? top ^ 0x80000000u : ~top);
+    double part = 0.;
+#pragma unroll
+    for (int s = 0; s < S; ++s) part += z[s] > -__builtin_inff() ? exp_from(z[s], most) : 0.;
+    sum = wave_sum(part);
+  }
+  const int e = lane < k ? experts[t * k + lane] : -1;
+  const bool mine = e >= 0 && e < E;
+  const float own = mine ? load_el<EL>(logits, t * ld + e) : 0.f;
+  const double g = mine ? p.scale * (double)dweights[t * k + lane] : 0.;
+  const double r = chosen_share(p, mine ? e : -1, own, most, sum);
+  double d;
+  if (p.sigmoid && !p.renormalize) {
+    d = g * r * (1. / (1. + exp((double)own)));
+  } else {
+    const double dot = wave_sum(r * g);
+    d = r * (g - dot);
+    if (p.sigmoid) d *= 1. / (1. + exp((double)own));
+    if (all) {
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+        if (64 * s + lane < E) row[64 * s + lane] = z[s] > -__builtin_inff() ? (float)(-(exp_from(z[s], most) / sum) * dot) : 0.f;
+    }
+  }
+  if (!all)
+    for (int i = lane; i < E; i += 64) row[i] = 0.f;
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  if (mine) row[e] = (float)d;
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  for (int i = lane; i < E; i += 64) store_el<EL>(dlogits, t * E + i, row[i]);
+}
+template <int EL>
+int launch_scored_backward(const void *logits, int64_t ld, const int *experts, const float *dweights, int T, int E, int k, const Scores &p, void *dlogits,
+                           hipStream_t s) {
+  const dim3 grid = wide_grid((T + WAVES - 1) / WAVES), block(64 * WAVES);
+  const size_t lds = sizeof(float) * WAVES * E;
+#define SK_SCORED_BACKWARD(S) \
+  hipLaunchKernelGGL((route_scored_backward_kernel<EL, S>), grid, block, lds, s, logits, ld, experts, dweights, T, E, k, p, dlogits)
+  if (E <= 64) SK_SCORED_BACKWARD(1);
+  else if (E <= 256) SK_SCORED_BACKWARD(4);
+  else SK_SCORED_BACKWARD(16);
+#undef SK_SCORED_BACKWARD
+  return (int)hipGetLastError();
 }
 
 // rows[p] = x[order[p] / k]: one wave per row, pieces of UNIT bytes
@@ -502,8 +738,9 @@ extern "C" size_t sk_route_workspace_bytes(int64_t T, int64_t E, int64_t k) {
   return check_route_shape(T, E, k) == SK_OK ? sizeof(int) * (size_t)route_blocks(T, E) * (size_t)E : 0;
 }
 
-extern "C" int sk_route_experts(const void *logits, int dtype, int64_t T, int64_t E, int64_t k, int64_t ld, void *weights, void *experts,
-                                void *offsets, void *order, void *place, void *ws, size_t ws_bytes, void *stream) {
+// p: null for the plain route
+static int route(const void *logits, int dtype, int64_t T, int64_t E, int64_t k, int64_t ld, const Scores *p, void *weights, void *experts, void *offsets, void *order,
+                 void *place, void *ws, size_t ws_bytes, void *stream) {
   if (element_of(dtype) < 0) return SK_ERR_CONFIG;
   if (int rc = check_route_shape(T, E, k)) return rc;
   if (!logits || !weights || !experts || !offsets || !order || !place) return SK_ERR_NULL;
@@ -512,11 +749,47 @@ extern "C" int sk_route_experts(const void *logits, int dtype, int64_t T, int64_
   if (ws_bytes < sk_route_workspace_bytes(T, E, k) || (blocks > 0 && !ws)) return SK_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(ws) & 3) return SK_ERR_ALIGN;
   RouteArgs a{logits, ld, (int)T, (int)E, (int)k, (float *)weights, (int *)experts, (int *)offsets, (int *)order, (int *)place, (int *)ws,
-              route_tokens(T)};
-  hipStream_t s = (hipStream_t)stream;
-  const int el = element_of(dtype);
-  const int herr = el == EL_F16 ? launch_route_of<EL_F16>(a, blocks, s) : (el == EL_BF16 ? launch_route_of<EL_BF16>(a, blocks, s) : launch_route_of<EL_F32>(a, blocks, s));
+              route_tokens(T), p ? *p : Scores{}};
+  const int herr = p ? launch_route_by<true>(element_of(dtype), a, blocks, (hipStream_t)stream) : launch_route_by<false>(element_of(dtype), a, blocks, (hipStream_t)stream);
   return herr == 0 ? SK_OK : SK_ERR_LAUNCH;
+}
+// fills p; sk_status
+static int check_scores(const sk_route_scores *s, int64_t E, int64_t k, Scores *p) {
+  if (!s) return SK_ERR_NULL;
+  if ((s->scores != SK_SCORES_SOFTMAX && s->scores != SK_SCORES_SIGMOID) || !(s->scale > -__builtin_inf() && s->scale < __builtin_inf())) return SK_ERR_CONFIG;
+  if (s->groups < 1 || s->groups > MAX_GROUPS || E % s->groups || s->chosen_groups < 1 || s->chosen_groups > s->groups || k > E / s->groups * s->chosen_groups)
+    return SK_ERR_SHAPE;
+  if (reinterpret_cast<uintptr_t>(s->bias) & 3) return SK_ERR_ALIGN;
+  // (all groups open: none is asked)
+  const int groups = s->chosen_groups == s->groups ? 1 : s->groups;
+  *p = Scores{(const float *)s->bias, s->scale, groups, s->chosen_groups, s->scores == SK_SCORES_SIGMOID, s->renormalize != 0};
+  return SK_OK;
+}
+
+extern "C" int sk_route_experts(const void *logits, int dtype, int64_t T, int64_t E, int64_t k, int64_t ld, void *weights, void *experts,
+                                void *offsets, void *order, void *place, void *ws, size_t ws_bytes, void *stream) {
+  return route(logits, dtype, T, E, k, ld, nullptr, weights, experts, offsets, order, place, ws, ws_bytes, stream);
+}
+
+extern "C" int sk_route_scored(const void *logits, int dtype, int64_t T, int64_t E, int64_t k, int64_t ld, const sk_route_scores *scores, void *weights,
+                               void *experts, void *offsets, void *order, void *place, void *ws, size_t ws_bytes, void *stream) {
+  if (int rc = check_route_shape(T, E, k)) return rc;
+  Scores p;
+  if (int rc = check_scores(scores, E, k, &p)) return rc;
+  return route(logits, dtype, T, E, k, ld, &p, weights, experts, offsets, order, place, ws, ws_bytes, stream);
+}
+
+extern "C" int sk_route_scored_backward(const void *logits, int dtype, int64_t T, int64_t E, int64_t k, int64_t ld, const sk_route_scores *scores,
+                                        const void *experts, const void *dweights, void *dlogits, void *stream) {
+  if (element_of(dtype) < 0) return SK_ERR_CONFIG;
+  if (int rc = check_route_shape(T, E, k)) return rc;
+  Scores p;
+  if (int rc = check_scores(scores, E, k, &p)) return rc;
+  if (!logits || !experts || !dweights || !dlogits) return SK_ERR_NULL;
+  if (ld < E) return SK_ERR_SHAPE;
+  const int el = element_of(dtype);
+  const auto launch = el == EL_F16 ? launch_scored_backward<EL_F16> : (el == EL_BF16 ? launch_scored_backward<EL_BF16> : launch_scored_backward<EL_F32>);
+  return launch(logits, ld, (const int *)experts, (const float *)dweights, (int)T, (int)E, (int)k, p, dlogits, (hipStream_t)stream) == 0 ? SK_OK : SK_ERR_LAUNCH;
 }
 
 extern "C" int sk_route_backward(const void *weights, const void *experts, const void *dweights, int64_t T, int64_t E, int64_t k, int dtype,

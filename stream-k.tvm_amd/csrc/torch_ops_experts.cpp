@@ -187,6 +187,48 @@ Tensor route_backward(const Tensor &weights, const Tensor &experts, const Tensor
   }
   GENERAL("route_backward", decltype(route_backward), weights, experts, dweights, E, dtype);
 }
+// by scores, with a bias, in groups; false: what the general implementation refuses
+bool scores_of(c10::string_view scores, bool renormalize, int64_t groups, int64_t chosen_groups, double scale, sk_route_scores *by) {
+  if ((scores != "softmax" && scores != "sigmoid") || groups < 1 || groups > 64 || chosen_groups < 1 || chosen_groups > groups) return false;
+  *by = sk_route_scores{nullptr, scale, scores == "sigmoid" ? SK_SCORES_SIGMOID : SK_SCORES_SOFTMAX, renormalize, (int32_t)groups, (int32_t)chosen_groups};
+  return true;
+}
+FiveTensors route_scored(const Tensor &logits, int64_t k, const MaybeTensor &bias, c10::string_view scores, bool renormalize, int64_t groups,
+                         int64_t chosen_groups, double scale) {
+  at::AutoDispatchBelowADInplaceOrView guard;
+  const int dtype = dtype_of(logits.scalar_type());
+  sk_route_scores by;
+  if (logits.is_cuda() && dtype >= 0 && dtype != SK_I8 && logits.dim() == 2 && logits.size(0) > 0 && logits.is_contiguous() && k >= 1 && k <= logits.size(1) &&
+      scores_of(scores, renormalize, groups, chosen_groups, scale, &by) &&
+      (!bias.has_value() || (bias->scalar_type() == at::kFloat && bias->dim() == 1 && bias->size(0) == logits.size(1) && bias->is_contiguous() && bias->device() == logits.device()))) {
+    const int64_t T = logits.size(0), E = logits.size(1);
+    by.bias = bias.has_value() ? bias->data_ptr() : nullptr;
+    Tensor weights = fresh(logits, {T, k}, at::kFloat), experts = ints(logits, {T, k}), offsets = ints(logits, {E + 1}),
+           order = ints(logits, {T * k}), place = ints(logits, {T, k});
+    const size_t bytes = sk_route_workspace_bytes(T, E, k);
+    Tensor ws;
+    if (bytes > 0) ws = fresh(logits, {(int64_t)bytes}, at::kByte);
+    if (sk_route_scored(logits.data_ptr(), dtype, T, E, k, E, &by, weights.data_ptr(), experts.data_ptr(), offsets.data_ptr(), order.data_ptr(), place.data_ptr(),
+                        bytes > 0 ? ws.data_ptr() : nullptr, bytes, current_stream()) == SK_OK)
+      return {weights, experts, offsets, order, place};
+  }
+  GENERAL("route_scored", decltype(route_scored), logits, k, bias, scores, renormalize, groups, chosen_groups, scale);
+}
+Tensor route_scored_backward(const Tensor &logits, const Tensor &experts, const Tensor &dweights, c10::string_view scores, bool renormalize, int64_t groups,
+                             int64_t chosen_groups, double scale) {
+  at::AutoDispatchBelowADInplaceOrView guard;
+  const int dtype = dtype_of(logits.scalar_type());
+  sk_route_scores by;
+  if (logits.is_cuda() && dtype >= 0 && dtype != SK_I8 && logits.dim() == 2 && logits.size(0) > 0 && logits.is_contiguous() && is_ints(experts, logits, 2) &&
+      experts.size(0) == logits.size(0) && dweights.scalar_type() == at::kFloat && dweights.sizes() == experts.sizes() && dweights.is_contiguous() &&
+      dweights.device() == logits.device() && scores_of(scores, renormalize, groups, chosen_groups, scale, &by)) {
+    Tensor dlogits = fresh(logits, logits.sizes(), logits.scalar_type());
+    if (sk_route_scored_backward(logits.data_ptr(), dtype, logits.size(0), logits.size(1), experts.size(1), logits.size(1), &by, experts.data_ptr(),
+                                 dweights.data_ptr(), dlogits.data_ptr(), current_stream()) == SK_OK)
+      return dlogits;
+  }
+  GENERAL("route_scored_backward", decltype(route_scored_backward), logits, experts, dweights, scores, renormalize, groups, chosen_groups, scale);
+}
 // (place undefined: none) an undefined tensor: not the ordinary case
 Tensor dispatched(const Tensor &x, const Tensor &order, const Tensor &place, int64_t k) {
   if (!x.is_cuda() || (x.dim() != 1 && x.dim() != 2) || x.numel() == 0 || !x.is_contiguous() || k < 1 || !is_ints(order, x, 1) || order.size(0) != x.size(0) * k) return {};
@@ -338,6 +380,44 @@ FiveTensors route_experts_autograd(const Tensor &logits, int64_t k) {
   return {r[0], r[1], r[2], r[3], r[4]};
 }
 
+struct RouteScored : torch::autograd::Function<RouteScored> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &logits, int64_t k, const MaybeTensor &bias, std::string scores, bool renormalize,
+                               int64_t groups, int64_t chosen_groups, double scale) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    static const auto route = OP(route_scored);
+    const FiveTensors r = route.call(logits, k, bias, scores, renormalize, groups, chosen_groups, scale);
+    ctx->save_for_backward({logits, std::get<1>(r)});
+    ctx->saved_data["scores"] = scores;
+    ctx->saved_data["renormalize"] = renormalize;
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["chosen_groups"] = chosen_groups;
+    ctx->saved_data["scale"] = scale;
+    ctx->mark_non_differentiable({std::get<1>(r), std::get<2>(r), std::get<3>(r), std::get<4>(r)});
+    return {std::get<0>(r), std::get<1>(r), std::get<2>(r), std::get<3>(r), std::get<4>(r)};
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    static const auto back = OP(route_scored_backward);
+    const auto saved = ctx->get_saved_variables();
+    variable_list none(8);
+    if (!grads[0].defined()) return none;
+    Tensor dlogits;
+    {
+      at::AutoDispatchBelowADInplaceOrView guard;
+      dlogits = back.call(saved[0], saved[1], grads[0], ctx->saved_data["scores"].toStringRef(), ctx->saved_data["renormalize"].toBool(),
+                          ctx->saved_data["groups"].toInt(), ctx->saved_data["chosen_groups"].toInt(), ctx->saved_data["scale"].toDouble());
+    }
+    none[0] = once(dlogits, {saved[0], grads[0]});
+    return none;
+  }
+};
+FiveTensors route_scored_autograd(const Tensor &logits, int64_t k, const MaybeTensor &bias, c10::string_view scores, bool renormalize, int64_t groups,
+                                  int64_t chosen_groups, double scale) {
+  no_tangent("route_experts", {&logits, get(bias)});
+  if (!wanted(logits)) BELOW(route_scored, logits, k, bias, scores, renormalize, groups, chosen_groups, scale);
+  const variable_list r = RouteScored::apply(logits, k, bias, std::string(scores.data(), scores.size()), renormalize, groups, chosen_groups, scale);
+  return {r[0], r[1], r[2], r[3], r[4]};
+}
+
 // (place: for the gradient of dispatch_rows, which is a combination without weights)
 struct DispatchRows : torch::autograd::Function<DispatchRows> {
   static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &order, const Tensor &place) {
@@ -400,6 +480,8 @@ TORCH_LIBRARY_IMPL(streamk, CUDA, m) {
   m.impl("grouped_wgrad", &grouped_wgrad);
   m.impl("route_experts", &route_experts);
   m.impl("route_backward", &route_backward);
+  m.impl("route_scored", &route_scored);
+  m.impl("route_scored_backward", &route_scored_backward);
   m.impl("dispatch_rows", &dispatch_rows);
   m.impl("dispatch_routed", &dispatch_routed);
   m.impl("combine_rows", &combine_rows);
@@ -409,6 +491,7 @@ TORCH_LIBRARY_IMPL(streamk, CUDA, m) {
 TORCH_LIBRARY_IMPL(streamk, AutogradCUDA, m) {
   m.impl("gemm_grouped", &gemm_grouped_autograd);
   m.impl("route_experts", &route_experts_autograd);
+  m.impl("route_scored", &route_scored_autograd);
   m.impl("dispatch_routed", &dispatch_routed_autograd);
   m.impl("combine_routed", &combine_routed_autograd);
 }

@@ -59,6 +59,15 @@ class SkGrouped(ctypes.Structure):
         (n, ctypes.c_void_p) for n in ("bias", "scale_a", "scale_b")] + [("variant", ctypes.c_int64), ("spin_limit", ctypes.c_int64)]
 
 
+SK_SCORES_SOFTMAX, SK_SCORES_SIGMOID = 0, 1
+
+
+class SkRouteScores(ctypes.Structure):
+    """sk_route_scores: what a route goes by."""
+    _fields_ = [("bias", ctypes.c_void_p), ("scale", ctypes.c_double)] + [
+        (n, ctypes.c_int32) for n in ("scores", "renormalize", "groups", "chosen_groups")]
+
+
 class StreamKError(RuntimeError):
     def __init__(self, status, where):
         self.status = status
@@ -148,11 +157,13 @@ def lib():
     L.sk_route_workspace_bytes.restype = sz
     L.sk_route_experts.argtypes = [vp, ci, i64, i64, i64, i64, vp, vp, vp, vp, vp, vp, sz, vp]
     L.sk_route_backward.argtypes = [vp, vp, vp, i64, i64, i64, ci, vp, vp]
+    L.sk_route_scored.argtypes = [vp, ci, i64, i64, i64, i64, P(SkRouteScores), vp, vp, vp, vp, vp, vp, sz, vp]
+    L.sk_route_scored_backward.argtypes = [vp, ci, i64, i64, i64, i64, P(SkRouteScores), vp, vp, vp, vp]
     L.sk_dispatch_rows.argtypes = [vp, i64, i64, vp, vp, i64, i64, vp, vp]
     L.sk_combine_rows.argtypes = [vp, ci, vp, vp, i64, i64, i64, vp, vp]
     L.sk_combine_backward.argtypes = [vp, vp, ci, vp, vp, vp, i64, i64, i64, vp, vp, vp]
     for f in ("sk_gemm_i8_scaled", "sk_i8_scaled_takes", "sk_quantize_i8", "sk_gemm_grouped", "sk_grouped_wgrad", "sk_route_experts", "sk_route_backward",
-              "sk_dispatch_rows", "sk_combine_rows", "sk_combine_backward"):
+              "sk_route_scored", "sk_route_scored_backward", "sk_dispatch_rows", "sk_combine_rows", "sk_combine_backward"):
         getattr(L, f).restype = ci
     for f in ("sk_device_info", "sk_make_plan", "sk_plan_cta_range", "sk_plan_tile_coords",
               "sk_workspace_init", "sk_workspace_status", "sk_gemm_f16", "sk_gemm_f32",

@@ -12,6 +12,7 @@ gradients, in native code (csrc/torch_ops_experts.cpp), which passes every other
 `<name>_general`; without the native library those and the autograd functions here stand in.
 """
 import ctypes
+import math
 from typing import NamedTuple
 
 import torch
@@ -230,8 +231,8 @@ def streamk_grouped_wgrad(dC, A, offsets, *, variant=0):
 # ---- routing ----
 class Route(NamedTuple):
     """Where tokens go.  Slot t k + j is token t's j-th expert."""
-    weights: torch.Tensor   # float32 [T, k]: softmax of the chosen logits, 0 where there is no expert
-    experts: torch.Tensor   # int32 [T, k]: the largest logit's first; -1 where fewer than k can be chosen
+    weights: torch.Tensor   # float32 [T, k]: scores of the chosen (by default softmax of their logits), 0 where there is no expert
+    experts: torch.Tensor   # int32 [T, k]: the best first; -1 where fewer than k can be chosen
     offsets: torch.Tensor   # int32 [E + 1]: where each expert's rows begin
     order: torch.Tensor     # int32 [T k]: the slot of each sorted row, -1 from offsets[E] on
     place: torch.Tensor     # int32 [T, k]: the sorted row of each slot, -1 without an expert
@@ -282,6 +283,97 @@ _operator("route_backward", "(Tensor weights, Tensor experts, Tensor dweights, i
           lambda weights, experts, dweights, E, dtype: weights.new_empty((weights.shape[0], E), dtype=dtype))
 
 
+# by scores, with a bias, in groups
+_SCORES = {"softmax": _lib.SK_SCORES_SOFTMAX, "sigmoid": _lib.SK_SCORES_SIGMOID}
+MAX_GROUPS = 64
+
+
+def _check_scored(logits, k, bias, scores, groups, chosen_groups, scale):
+    _on_device(logits, "logits", tuple(_LOGITS), 2)
+    E = logits.shape[1]
+    if not 1 <= E <= MAX_EXPERTS or not 1 <= k <= min(E, MAX_CHOSEN):
+        raise ValueError(f"1 to {MAX_EXPERTS} experts, of which 1 to {MAX_CHOSEN} are chosen: got {E} and k = {k}")
+    if scores not in _SCORES:
+        raise ValueError("scores must be 'softmax' or 'sigmoid'")
+    if not 1 <= groups <= MAX_GROUPS or E % groups or not 1 <= chosen_groups <= groups:
+        raise ValueError(f"1 to {MAX_GROUPS} equal groups of the {E} experts, of which one at least is chosen: got {groups} and chosen_groups = {chosen_groups}")
+    if k > E // groups * chosen_groups:
+        raise ValueError(f"{chosen_groups} groups of {E // groups} experts have no {k} to choose")
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite, got {scale}")
+    if bias is not None:
+        _on_device(bias, "bias", (torch.float32,), 1)
+        if bias.shape[0] != E or not bias.is_contiguous() or bias.device != logits.device:
+            raise ValueError(f"bias must be a contiguous float32 vector of {E} elements on {logits.device}")
+
+
+def _route_scores(bias, scores, renormalize, groups, chosen_groups, scale):
+    return _lib.SkRouteScores(bias=bias.data_ptr() if bias is not None else None, scale=scale, scores=_SCORES[scores], renormalize=renormalize, groups=groups,
+                              chosen_groups=chosen_groups)
+
+
+def _logit_rows(logits):
+    return logits.contiguous() if logits.stride(1) != 1 and logits.shape[1] > 1 or logits.stride(0) < logits.shape[1] else logits
+
+
+def _route_scored(logits, k, bias, scores, renormalize, groups, chosen_groups, scale):
+    _check_scored(logits, k, bias, scores, groups, chosen_groups, scale)
+    logits = _logit_rows(logits)
+    T, E = logits.shape
+    new = lambda *shape: torch.empty(shape, dtype=torch.int32, device=logits.device)  # noqa: E731
+    weights, experts, offsets, order, place = torch.empty((T, k), dtype=torch.float32, device=logits.device), new(T, k), new(E + 1), new(T * k), new(T, k)
+    if T == 0:
+        offsets.zero_()
+        return weights, experts, offsets, order, place
+    L = _lib.lib()
+    nbytes = L.sk_route_workspace_bytes(T, E, k)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
+    by = _route_scores(bias, scores, renormalize, groups, chosen_groups, scale)
+    rc = L.sk_route_scored(logits.data_ptr(), _LOGITS[logits.dtype], T, E, k, max(logits.stride(0), E), ctypes.byref(by), weights.data_ptr(), experts.data_ptr(),
+                           offsets.data_ptr(), order.data_ptr(), place.data_ptr(), ws.data_ptr() if nbytes else None, nbytes, ops._stream_ptr())
+    _lib.check(rc, "sk_route_scored")
+    return weights, experts, offsets, order, place
+
+
+def _route_scored_backward(logits, experts, dweights, scores, renormalize, groups, chosen_groups, scale):
+    k = experts.shape[1]
+    _check_scored(logits, k, None, scores, groups, chosen_groups, scale)
+    logits = _logit_rows(logits)
+    T, E = logits.shape
+    _on_device(experts, "experts", (torch.int32,), 2)
+    _on_device(dweights, "dweights", (torch.float32,), 2)
+    if experts.shape[0] != T or dweights.shape != experts.shape or experts.device != logits.device or dweights.device != logits.device:
+        raise ValueError(f"experts and dweights must be {(T, k)} on {logits.device}")
+    dlogits = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
+    if T:
+        by = _route_scores(None, scores, renormalize, groups, chosen_groups, scale)
+        rc = _lib.lib().sk_route_scored_backward(logits.data_ptr(), _LOGITS[logits.dtype], T, E, k, max(logits.stride(0), E), ctypes.byref(by),
+                                                 experts.contiguous().data_ptr(), dweights.contiguous().data_ptr(), dlogits.data_ptr(), ops._stream_ptr())
+        _lib.check(rc, "sk_route_scored_backward")
+    return dlogits
+
+
+_operator("route_scored", "(Tensor logits, int k, Tensor? bias, str scores, bool renormalize, int groups, int chosen_groups, float scale) -> "
+          "(Tensor, Tensor, Tensor, Tensor, Tensor)", _route_scored, lambda logits, k, *rest: _route_fake(logits, k))
+_operator("route_scored_backward", "(Tensor logits, Tensor experts, Tensor dweights, str scores, bool renormalize, int groups, int chosen_groups, float scale) -> Tensor",
+          _route_scored_backward, lambda logits, *rest: logits.new_empty(logits.shape))
+
+
+class _RouteScored(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, k, bias, *by):
+        out = _ops.route_scored(logits, k, bias, *by)
+        ctx.save_for_backward(logits, out[1])
+        ctx.by = by
+        ctx.mark_non_differentiable(*out[1:])
+        return tuple(out)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dweights, *_):
+        return (_ops.route_scored_backward(*ctx.saved_tensors, dweights, *ctx.by), None, None, None, None, None, None, None)
+
+
 class _RouteExperts(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, k):
@@ -298,15 +390,27 @@ class _RouteExperts(torch.autograd.Function):
         return _ops.route_backward(weights, experts, dweights, ctx.E, ctx.dtype), None
 
 
-def route_experts(logits, k):
-    """Route of the tokens whose router logits are [T, E] (float32, float16 or bfloat16): the k largest of each, the largest first, equal
+def route_experts(logits, k, *, scores="softmax", bias=None, groups=1, chosen_groups=1, renormalize=True, scale=1.0):
+    """Route of the tokens whose router logits z are [T, E] (float32, float16 or bfloat16): the k largest of each, the largest first, equal
     ones by number.  -inf and NaN are never chosen: a token with fewer others has -1 and weight 0 in its last places, and one with none
-    goes to no expert.  Differentiable: weights to logits."""
+    goes to no expert.  Differentiable: weights to logits.
+
+    scores: s = 'softmax' of a token's logits or their 'sigmoid'.  weights: s of the chosen experts, divided by their sum with
+    `renormalize`, times `scale`.
+    bias (float32 [E]): the experts are chosen, and stand in the route, by s + bias; the weights are those without it.  It has no gradient: a
+    rule that counts each expert's tokens (route.offsets) sets it.  -inf and NaN close an expert.
+    groups, chosen_groups: of `groups` equal groups of neighbouring experts only the chosen_groups whose two best experts have the largest
+    sums of s + bias are open to a token (equal ones by number).
+    Scores, sums and comparisons are in 64 bits wherever the choice goes by more than the logits."""
     if not _NATIVE:
-        _no_tangent("route_experts", logits)
-    if not _NATIVE and torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
-        return Route(*_RouteExperts.apply(logits, k))
-    return Route(*_route_experts(logits, k))
+        _no_tangent("route_experts", logits, bias)
+    # (all groups open: as without)
+    plain = scores == "softmax" and bias is None and renormalize and scale == 1.0 and groups == 1 and chosen_groups == 1
+    recorded = not _NATIVE and torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad
+    if plain:
+        return Route(*(_RouteExperts.apply(logits, k) if recorded else _route_experts(logits, k)))
+    by = (scores, bool(renormalize), groups, chosen_groups, float(scale))
+    return Route(*(_RouteScored.apply(logits, k, bias, *by) if recorded else _route_scored_op(logits, k, bias, *by)))
 
 
 def _dispatch(x, order, k, place=None):
@@ -424,5 +528,5 @@ def combine_rows(y, route):
 
 
 # (the overloads themselves: a call through the packet looks them up)
-_gemm_grouped, _route_experts = _ops.gemm_grouped.default, _ops.route_experts.default
+_gemm_grouped, _route_experts, _route_scored_op = _ops.gemm_grouped.default, _ops.route_experts.default, _ops.route_scored.default
 _dispatch_routed, _combine_routed = _ops.dispatch_routed.default, _ops.combine_routed.default
