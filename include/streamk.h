@@ -95,6 +95,7 @@ typedef enum sk_dtype {
   SK_I8 = 6,       /* A and B int8, C int32 */
   SK_Q4_ZP = 7,    /* as SK_Q4 with one zero point per scale group and row (sk_gemm_q4_zp) */
   SK_F8E5M2 = 8,   /* as SK_F8E4M3 for OCP e5m2 bytes (the upper byte of an fp16: bias 15, infinities and NaNs) */
+  SK_MXFP4 = 10,   /* A and B in pairs of e2m1 values with a power of two for each 32 of K (sk_gemm_grouped, sk_quantize_mxfp4); no plans */
   SK_Q4_ZP_TILED = 9 /* as SK_Q4_ZP with the nibbles in the tiled layout of SK_Q4_TILED (scales and zero points row-major) */
 } sk_dtype;
 
@@ -456,11 +457,33 @@ typedef struct sk_grouped {
                                                      64, int8: 128); 3 to 6: 16 x 64, 32 x 64, 64 x 64, 64 x 128,
                                                      whose waves stream K on their own (SK_LAYOUT_NN: only 64 x 64) */
   int64_t spin_limit;                             /* 0: 2^22 polls; negative: none (to test the way out) */
+  int64_t scale_pitch_a, scale_pitch_b;           /* SK_MXFP4: bytes from row to row of scale_a and scale_b, even, 0: K / 32 */
 } sk_grouped;
 size_t sk_grouped_workspace_bytes(const sk_grouped *g);   /* for this shape and variant, on the current device; 0 is possible */
 int sk_gemm_grouped(const sk_grouped *g, void *ws, size_t ws_bytes, void *stream);
 int sk_grouped_wgrad(const void *A, const void *B, const void *offsets, void *C, int dtype, int64_t E, int64_t R, int64_t M, int64_t N,
                      int64_t lda, int64_t ldb, int variant, void *stream);
+
+/*
+ * Microscaled 4-bit floating point.  No counterpart in the reference.
+ *
+ * A row of K values (K a multiple of 32) is K / 2 bytes of e2m1 codes, value 2 i in the low half of byte i, and K / 32 bytes: block b of
+ * 32 values is multiplied by 2^(byte - 127), 255 is NaN.
+ * sk_quantize_mxfp4: X (SK_F16, SK_BF16 or SK_F32, M x K, pitch ldx elements) to Q [M, K / 2] and scales [M, K / 32], both contiguous:
+ * byte = floor(log2 max |x|) + 125 of the block, at least 0; each x / 2^(byte - 127) becomes the nearest code (ties to even), at most 6.  A
+ * block with an infinity or a NaN has byte 255 and codes 0, so that its products are NaN.
+ * sk_dequantize_mxfp4: the values, in SK_F16, SK_BF16 or SK_F32, rounded once where the type has no such number.
+ * sk_pad_mx_scales: rows of `blocks` bytes to a pitch (a multiple of 16) with zeros behind them.
+ *
+ * sk_gemm_grouped with dtype SK_MXFP4 multiplies them (SK_LAYOUT_NT): C[r] = activation(A[r] * B[e]^T + bias[e]), C in out_dtype, sums in
+ * fp32, rounded once.  scale_a: [R] rows of exponents, scale_b: [E, N] rows, scale_pitch_a and _b bytes apart.  offsets null and E = 1: all
+ * rows are the one expert's.  K, lda, ldb and expert_b are multiples of 32 values; a row's exponents are read two at a time: the pitches are even,
+ * and where K is no multiple of 64 the byte behind a row's last is read, and must not be 255 (sk_mx_scale_pitch, sk_pad_mx_scales).
+ */
+int sk_quantize_mxfp4(const void *X, int dtype, int64_t M, int64_t K, int64_t ldx, void *Q, void *scales, void *stream);
+int sk_dequantize_mxfp4(const void *Q, const void *scales, int64_t M, int64_t K, int dtype, void *X, void *stream);
+int64_t sk_mx_scale_pitch(const sk_grouped *g);   /* 0, or the pitch that sk_pad_mx_scales is to give both scales of this product, on the current device */
+int sk_pad_mx_scales(const void *scales, int64_t rows, int64_t blocks, int64_t pitch, void *out, void *stream);
 
 /*
  * Routing of tokens to experts.  No counterpart in the reference.

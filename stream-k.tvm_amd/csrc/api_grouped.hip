@@ -2,6 +2,7 @@
 #include <hip/hip_runtime.h>
 
 #include "grouped_launch.h"
+#include "grouped_mx.h"
 #include "launch.h"
 #include "streamk.h"
 
@@ -14,52 +15,78 @@ constexpr int64_t MAX_INT = 0x7fffff00;
 int status_of(int herr) { return herr == 0 ? SK_OK : (herr == (int)hipErrorNotSupported ? SK_ERR_CONFIG : SK_ERR_LAUNCH); }
 }  // namespace
 
+// bytes from one row's exponents to the next row's
+static int64_t mx_pitch(int64_t given, int64_t K) { return given == 0 ? K / 32 : given; }
 // everything but the operands' addresses; fills h
 static int check_shape(const sk_grouped *g, GroupedShape *h) {
-  const bool i8 = g->dtype == SK_I8, nn = g->layout == SK_LAYOUT_NN;
-  if (!i8 && g->dtype != SK_F16 && g->dtype != SK_BF16) return SK_ERR_CONFIG;
-  if ((!nn && g->layout != SK_LAYOUT_NT) || (nn && i8)) return SK_ERR_CONFIG;
-  if (i8 ? g->out_dtype != SK_F16 && g->out_dtype != SK_BF16 : g->out_dtype != g->dtype) return SK_ERR_CONFIG;
+  const bool i8 = g->dtype == SK_I8, mx = g->dtype == SK_MXFP4, nn = g->layout == SK_LAYOUT_NN;
+  if (!i8 && !mx && g->dtype != SK_F16 && g->dtype != SK_BF16) return SK_ERR_CONFIG;
+  if ((!nn && g->layout != SK_LAYOUT_NT) || (nn && (i8 || mx))) return SK_ERR_CONFIG;
+  if (i8 || mx ? g->out_dtype != SK_F16 && g->out_dtype != SK_BF16 : g->out_dtype != g->dtype) return SK_ERR_CONFIG;
   if (g->activation < SK_ACT_NONE || g->activation > SK_ACT_SILU || g->variant < 0) return SK_ERR_CONFIG;
   if (g->E <= 0 || g->R <= 0 || g->N <= 0 || g->K <= 0 || g->E > (1 << 20) || g->R > MAX_INT || g->N > MAX_INT || g->K > MAX_INT) return SK_ERR_SHAPE;
   if (g->lda < (nn ? (g->K + 7) / 8 * 8 : g->K) || g->ldb < (nn ? g->N : g->K) || g->ldc < g->N || g->expert_b < 0) return SK_ERR_SHAPE;
-  const int64_t step = i8 ? 16 : 8;
+  const int64_t step = mx ? 32 : (i8 ? 16 : 8);
   if ((!nn && (g->K % step)) || (g->lda % step) || (g->ldb % step) || (g->expert_b % step) || (nn && (g->N % 8))) return SK_ERR_ALIGN;
-  *h = GroupedShape{i8 ? GT_I8 : (g->dtype == SK_BF16 ? GT_BF16 : GT_F16), nn, g->E, g->R, g->N, g->K, 0, (int)g->variant};
+  *h = GroupedShape{mx ? GT_MX : i8 ? GT_I8 : (g->dtype == SK_BF16 ? GT_BF16 : GT_F16), nn, g->E, g->R, g->N, g->K, 0, (int)g->variant};
   // a tile's rows (NN: all K rows of an expert's weights) are addressed with 32-bit byte offsets
-  const int64_t bytes = i8 ? 1 : 2;
-  if (g->lda * bytes * 256 >= (int64_t)1 << 31 || g->ldb * bytes * (nn ? g->K + 64 : 256) >= (int64_t)1 << 31 || g->ldc * 2 * 256 >= (int64_t)1 << 31)
+  const int64_t pairs = mx ? 4 : (i8 ? 2 : 1);   // values in 16 bits
+  if (g->lda / pairs * 2 * 256 >= (int64_t)1 << 31 || g->ldb / pairs * 2 * (nn ? g->K + 64 : 256) >= (int64_t)1 << 31 || g->ldc * 2 * 256 >= (int64_t)1 << 31)
     return SK_ERR_SHAPE;
+  if (mx) {
+    // exponents are read two at a time
+    if (mx_pitch(g->scale_pitch_a, g->K) < g->K / 32 || mx_pitch(g->scale_pitch_b, g->K) < g->K / 32) return SK_ERR_SHAPE;
+    if (mx_pitch(g->scale_pitch_a, g->K) * 256 >= (int64_t)1 << 31 || mx_pitch(g->scale_pitch_b, g->K) * 256 >= (int64_t)1 << 31) return SK_ERR_SHAPE;
+    if (mx_pitch(g->scale_pitch_a, g->K) % 2 || mx_pitch(g->scale_pitch_b, g->K) % 2) return SK_ERR_ALIGN;
+  }
   return SK_OK;
 }
 
 extern "C" size_t sk_grouped_workspace_bytes(const sk_grouped *g) {
   GroupedShape h;
-  return g && check_shape(g, &h) == SK_OK && sk_device_info(&h.cus, nullptr, nullptr) == SK_OK ? grouped_workspace(h) : 0;
+  if (!g || check_shape(g, &h) != SK_OK || sk_device_info(&h.cus, nullptr, nullptr) != SK_OK) return 0;
+  return h.type == GT_MX ? mx_workspace(h) : grouped_workspace(h);
+}
+
+extern "C" int64_t sk_mx_scale_pitch(const sk_grouped *g) {
+  GroupedShape h;
+  if (!g || g->dtype != SK_MXFP4) return 0;
+  sk_grouped even = *g;   // (whatever the pitches are now)
+  even.scale_pitch_a = even.scale_pitch_b = (g->K / 32 + 15) / 16 * 16;
+  if (check_shape(&even, &h) != SK_OK || sk_device_info(&h.cus, nullptr, nullptr) != SK_OK) return 0;
+  return g->K % mx_scale_step(h) ? even.scale_pitch_a : 0;
 }
 
 extern "C" int sk_gemm_grouped(const sk_grouped *g, void *ws, size_t ws_bytes, void *stream) {
-  if (!g || !g->A || !g->B || !g->C || !g->offsets) return SK_ERR_NULL;
-  const bool i8 = g->dtype == SK_I8;
-  if (i8 ? !g->scale_a || !g->scale_b : g->scale_a || g->scale_b) return i8 ? SK_ERR_NULL : SK_ERR_CONFIG;
+  if (!g || !g->A || !g->B || !g->C) return SK_ERR_NULL;
+  const bool i8 = g->dtype == SK_I8, mx = g->dtype == SK_MXFP4, scaled = i8 || mx;
+  if (!g->offsets && (!mx || g->E != 1)) return SK_ERR_NULL;
+  if (scaled ? !g->scale_a || !g->scale_b : g->scale_a || g->scale_b) return scaled ? SK_ERR_NULL : SK_ERR_CONFIG;
   GroupedShape h;
   if (int rc = check_shape(g, &h)) return rc;
   if (misaligned(g->A, 15) || misaligned(g->B, 15) || misaligned(g->C, 1) || misaligned(g->bias, 1) || misaligned(g->offsets, 3) ||
-      misaligned(g->scale_a, 3) || misaligned(g->scale_b, 3))
+      misaligned(g->scale_a, mx ? 1 : 3) || misaligned(g->scale_b, mx ? 1 : 3))
     return SK_ERR_ALIGN;
   if (reinterpret_cast<uintptr_t>(g->bias) >> EPI_ACT_SHIFT) return SK_ERR_CONFIG;   // not a device address
   if (sk_device_info(&h.cus, nullptr, nullptr) != SK_OK) return SK_ERR_DEVICE;
-  h.variant = grouped_variant(h);
+  h.variant = mx ? mx_variant(h) : grouped_variant(h);
   Workspace w;
-  if (int rc = take_workspace(ws, ws_bytes, grouped_workspace(h), &w)) return rc;
-  const int64_t pairs = i8 ? 2 : 1;
-  GroupedArgs a{};
+  if (int rc = take_workspace(ws, ws_bytes, mx ? mx_workspace(h) : grouped_workspace(h), &w)) return rc;
+  const int64_t pairs = mx ? 4 : (i8 ? 2 : 1);
+  MxOperands a{};
   a.A = (const half_t *)g->A;
   a.B = (const half_t *)g->B;
   a.C = (half_t *)g->C;
   a.offsets = (const int *)g->offsets;
   a.bias = (const half_t *)g->bias;
-  a.s = Scales{(const float *)g->scale_a, (const float *)g->scale_b, g->out_dtype == SK_BF16};
+  if (mx) {
+    a.ea = (const uint8_t *)g->scale_a;
+    a.eb = (const uint8_t *)g->scale_b;
+    a.pitch_a = (int)mx_pitch(g->scale_pitch_a, g->K);
+    a.pitch_b = (int)mx_pitch(g->scale_pitch_b, g->K);
+  } else {
+    a.s = Scales{(const float *)g->scale_a, (const float *)g->scale_b, g->out_dtype == SK_BF16};
+  }
   a.lda = g->lda / pairs;
   a.ldb = g->ldb / pairs;
   a.ldc = g->ldc;
@@ -70,7 +97,7 @@ extern "C" int sk_gemm_grouped(const sk_grouped *g, void *ws, size_t ws_bytes, v
   a.K = (int)(g->K / pairs);
   a.act = g->activation;
   a.spin_limit = g->spin_limit == 0 || g->spin_limit > MAX_INT ? 1 << 22 : (int)(g->spin_limit < 0 ? 0 : g->spin_limit);
-  return status_of(launch_grouped(a, h, w, (hipStream_t)stream));
+  return status_of(mx ? launch_mx(a, h, g->out_dtype == SK_BF16, w, (hipStream_t)stream) : launch_grouped(a, h, w, (hipStream_t)stream));
 }
 
 extern "C" int sk_grouped_wgrad(const void *A, const void *B, const void *offsets, void *C, int dtype, int64_t E, int64_t R, int64_t M,

@@ -48,8 +48,8 @@ __device__ __forceinline__ void group_raster(int local, int tm, int tn, int &pm,
   pn = c;
 }
 
-// UNOWNED: groups 0 and E + 1 have tiles too
-template <int BM, bool UNOWNED = true>
+// UNOWNED: groups 0 and E + 1 have tiles too.  DENSE: no offsets, one expert has all rows.
+template <int BM, bool UNOWNED = true, bool DENSE = false>
 struct GroupWalk {
   const int *offsets;
   int E, R, tiles_n;
@@ -60,6 +60,14 @@ struct GroupWalk {
   __device__ __forceinline__ GroupWalk(const int *o, int E_, int R_, int tn) : offsets(o), E(E_), R(R_), tiles_n(tn), before(0) { load(0); }
   __device__ __forceinline__ void load(int c) {
     chunk = c;
+    if constexpr (DENSE) {
+      const int lane = threadIdx.x & 63;
+      lo = lane > 1 ? R : 0;
+      rows = lane == 1 ? R : 0;
+      ends = lane >= 1 ? (int)((unsigned)(R + BM - 1) / BM) * tiles_n : 0;
+      reached = R;
+      return;
+    }
     const int lane = threadIdx.x & 63, g = 64 * c + lane, before_chunk = c == 0 ? 0 : reached;
     // this group's end, and the one in front of it (from the lane below: 0x138)
     const int end = max((int)wave_max_up_to((uint32_t)min(max(offsets[min(g, E)], 0), R)), before_chunk);
@@ -216,11 +224,18 @@ __device__ __forceinline__ void zero_unowned(const GroupedArgs &g, int pid, int 
   }
 }
 
-// P: a policy whose partial tiles are coherent (store_partial, add_partial) and whose LDS is dead between two calls of mac
-template <class P>
-__device__ __forceinline__ void run_grouped_sk(const GroupedArgs &g, int ipt, const Workspace &ws, char *smem) {
+// arguments of one product without groups (dense, below): a member of that name
+template <class G, class = void>
+struct is_dense { static constexpr bool value = false; };
+template <class G>
+struct is_dense<G, std::void_t<decltype(G::DENSE)>> { static constexpr bool value = G::DENSE; };
+
+// P: a policy whose partial tiles are coherent (store_partial, add_partial) and whose LDS is dead between two calls of mac.  G: GroupedArgs,
+// or what is derived from it and has expert_args of its own
+template <class P, class G>
+__device__ __forceinline__ void run_grouped_sk(const G &g, int ipt, const Workspace &ws, char *smem) {
   static_assert(P::COHERENT_PARTIALS && P::FIXUP_WORD_IN_LDS, "see above");
-  GroupWalk<P::BM, false> walk(g.offsets, g.E, g.R, g.tiles_n);
+  GroupWalk<P::BM, false, is_dense<G>::value> walk(g.offsets, g.E, g.R, g.tiles_n);
   const int pid = grouped_pid(g.grid);
   int front, back;
   const int tiles = walk.total_tiles(front, back), whole = tiles - (int)((unsigned)tiles % (unsigned)g.grid);

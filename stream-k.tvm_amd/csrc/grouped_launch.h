@@ -6,7 +6,7 @@
 
 namespace sk {
 
-enum GroupedType { GT_F16 = 0, GT_BF16 = 1, GT_I8 = 2 };
+enum GroupedType { GT_F16 = 0, GT_BF16 = 1, GT_I8 = 2, GT_MX = 3 };
 struct GroupedShape {
   int type;      // GroupedType
   bool nn;       // weights [E, K, N]
@@ -30,6 +30,13 @@ int launch_grouped(const GroupedArgs &g, const GroupedShape &h, const Workspace 
 // up to some dozen rows to an expert (kernels_grouped_wavek.hip)
 size_t grouped_wavek_workspace(int variant, int cus);
 int launch_grouped_wavek(const GroupedArgs &g, const GroupedShape &h, const Workspace &ws, hipStream_t s);
+
+// microscaled 4-bit operands (kernels_mx.hip)
+struct MxOperands;
+int mx_variant(const GroupedShape &h);
+size_t mx_workspace(const GroupedShape &h);
+int mx_scale_step(const GroupedShape &h);   // K is a multiple of it, or the exponents have to be padded
+int launch_mx(const MxOperands &g, const GroupedShape &h, bool bf16, const Workspace &ws, hipStream_t s);
 
 struct WgradArgs {
   const half_t *dC, *A;   // [R, N] (width readable columns), [R, K]

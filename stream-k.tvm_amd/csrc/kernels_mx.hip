@@ -1,0 +1,65 @@
+// Products of microscaled 4-bit operands on tiles whose waves stream K on their own (tile_mx.h), by expert or of one matrix.
+#include "grouped_launch.h"
+#include "grouped_mx.h"
+#include "kernel_table.h"
+
+namespace sk {
+
+template <class P>
+struct MxWithZero : P {
+  static __device__ __forceinline__ void zero_sums(typename P::Acc &acc) {
+#pragma unroll
+    for (int u = 0; u < P::NQ; ++u) acc.c[u] = typename P::AccV{0, 0, 0, 0};
+  }
+};
+template <class P, bool DENSE>
+__global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_mx_kernel(MxGrouped<DENSE> g, int ipt, Workspace ws) {
+  __shared__ __attribute__((aligned(1024))) char smem[P::LDS_BYTES];
+  run_grouped_sk<MxWithZero<P>>(g, ipt, ws, smem);
+}
+
+template <class P, bool DENSE>
+static int launch(const MxOperands &operands, const GroupedShape &h, const Workspace &ws, hipStream_t s) {
+  MxGrouped<DENSE> g;
+  static_cast<MxOperands &>(g) = operands;
+  g.tiles_n = (g.N + P::BN - 1) / P::BN;
+  const int ipt = (g.K + P::BK - 1) / P::BK;
+  if (grouped_tiles(h, P::BM) * g.tiles_n * ipt >= 0x7fffffff) return (int)hipErrorNotSupported;   // (iterations are numbered in 32 bits)
+  g.grid = h.cus;
+  hipLaunchKernelGGL((sk_mx_kernel<P, DENSE>), dim3(g.grid), dim3(P::NT), 0, s, g, ipt, ws);
+  return (int)hipGetLastError();
+}
+
+// variant -> blocks of 16 rows, of 16 columns:  X(variant, FM, FN)
+#define MX_TILES(X)      \
+  X(GV_WAVEK16, 1, 4)    \
+  X(GV_WAVEK32, 2, 4)    \
+  X(GV_WAVEK64, 4, 4)
+
+int mx_variant(const GroupedShape &h) {
+  if (h.variant != GV_RULE) return h.variant;
+  const int64_t rows = (h.R + h.E - 1) / h.E;
+  return rows <= 16 ? GV_WAVEK16 : (rows <= 32 ? GV_WAVEK32 : GV_WAVEK64);
+}
+size_t mx_workspace(const GroupedShape &h) {
+  const int v = mx_variant(h);
+#define X(V, FM, FN) \
+  if (v == V) return (size_t)WS_PART_OFF + (size_t)2 * h.cus * (16 * FM) * (16 * FN) * 4;
+  MX_TILES(X)
+#undef X
+  return 0;
+}
+int mx_scale_step(const GroupedShape &) { return 64; }
+int launch_mx(const MxOperands &g, const GroupedShape &h, bool bf16, const Workspace &ws, hipStream_t s) {
+  const bool dense = g.offsets == nullptr;
+#define X(V, FM, FN)                                                                                                             \
+  if (h.variant == V) {                                                                                                          \
+    if (dense) return bf16 ? launch<TileWaveKMx<true, FM, FN>, true>(g, h, ws, s) : launch<TileWaveKMx<false, FM, FN>, true>(g, h, ws, s); \
+    return bf16 ? launch<TileWaveKMx<true, FM, FN>, false>(g, h, ws, s) : launch<TileWaveKMx<false, FM, FN>, false>(g, h, ws, s);          \
+  }
+  MX_TILES(X)
+#undef X
+  return (int)hipErrorNotSupported;
+}
+
+}  // namespace sk

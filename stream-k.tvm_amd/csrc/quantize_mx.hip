@@ -1,0 +1,247 @@
+// Microscaled 4-bit floating point: 32 neighbours of a row share a power of two X = 2^(floor(log2 max|x|) - 2) (at least 2^-127), kept as its
+// biased exponent in a byte, and each becomes x / X to the nearest e2m1 number (0, .5, 1, 1.5, 2, 3, 4, 6; ties to the even code), at most 6.
+// Value 2 i of a row is the low half of byte i.  A block with an infinity or a NaN has scale 255, the format's NaN, and codes 0.
+//
+// Both directions are one pass over memory, 16 bits and 17/32 of a byte a value, and what bounds them is that: a thread has eight values
+// (the conversions of this target take two at a time), four neighbours a block, whose maximum is two steps within a quad.
+#include <hip/hip_runtime.h>
+
+#include "sk_device.h"
+#include "streamk.h"
+#include "wide_grid.h"
+
+using namespace sk;
+
+namespace {
+
+constexpr int THREADS = 256, PIECES = 4;   // pieces of eight values that a thread has in flight
+enum { EL_F16 = 0, EL_BF16 = 1, EL_F32 = 2 };
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+template <int EL>
+struct Eight {
+  uint32_t w[EL == EL_F32 ? 8 : 4];
+};
+
+// the largest magnitude as the bits of a float: infinities and NaN are above every number
+template <int EL>
+__device__ __forceinline__ uint32_t largest(const Eight<EL> &v) {
+  if constexpr (EL == EL_F32) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, v.w[i] & 0x7fffffffu);
+    return most;
+  } else {
+    typedef uint16_t ushort2v __attribute__((ext_vector_type(2)));
+    ushort2v pair = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pair = __builtin_elementwise_max(pair, __builtin_bit_cast(ushort2v, v.w[i] & 0x7fff7fffu));
+    const uint32_t most = max((uint32_t)pair[0], (uint32_t)pair[1]);
+    if constexpr (EL == EL_BF16) return most << 16;
+    const float f = (float)__builtin_bit_cast(half_t, (uint16_t)most);   // (exact, infinities and NaN as well)
+    return __builtin_bit_cast(uint32_t, f);
+  }
+}
+// of the four threads of a block
+__device__ __forceinline__ uint32_t quad_max(uint32_t x) {
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xb1, 0xf, 0xf, true));   // lanes 1 0 3 2
+  return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4e, 0xf, 0xf, true));   // lanes 2 3 0 1
+}
+__device__ __forceinline__ uint32_t scale_byte(uint32_t most) {
+  const uint32_t field = most >> 23;   // floor(log2) + 127, 0 below the normal numbers
+  return field == 255 ? 255 : (field < 2 ? 0 : field - 2);
+}
+// 2^(byte - 127)
+__device__ __forceinline__ float scale_value(uint32_t byte) { return __builtin_bit_cast(float, byte == 0 ? 0x00400000u : byte << 23); }
+
+template <int EL>
+__device__ __forceinline__ uint32_t encode(const Eight<EL> &v, uint32_t byte) {
+  const float x = scale_value(byte);
+  uint32_t q = 0;
+  if constexpr (EL == EL_F32) {
+    const float *f = reinterpret_cast<const float *>(v.w);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[0], f[1], x, 0);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[2], f[3], x, 1);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[4], f[5], x, 2);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[6], f[7], x, 3);
+  } else if constexpr (EL == EL_BF16) {
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, __builtin_bit_cast(bf16x2, v.w[0]), x, 0);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, __builtin_bit_cast(bf16x2, v.w[1]), x, 1);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, __builtin_bit_cast(bf16x2, v.w[2]), x, 2);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, __builtin_bit_cast(bf16x2, v.w[3]), x, 3);
+  } else {
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, __builtin_bit_cast(half2v, v.w[0]), x, 0);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, __builtin_bit_cast(half2v, v.w[1]), x, 1);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, __builtin_bit_cast(half2v, v.w[2]), x, 2);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, __builtin_bit_cast(half2v, v.w[3]), x, 3);
+  }
+  return byte == 255 ? 0 : q;
+}
+
+// Rows of `pieces` pieces, `blocks` workgroups to a row.  (Rows without a gap between them are one row.)
+template <int EL, bool VEC>
+__global__ __launch_bounds__(THREADS) void quantize_kernel(const char *X, int64_t rows, int64_t pieces, int64_t ldx_bytes, int64_t blocks, uint32_t *Q,
+                                                           uint8_t *scales) {
+  constexpr int BYTES = EL == EL_F32 ? 32 : 16;
+  const int64_t block = wide_block(), row = block / blocks;
+  if (row >= rows) return;
+  const int64_t first = (block - row * blocks) * (THREADS * PIECES) + threadIdx.x;
+  const char *x = X + row * ldx_bytes;
+  Eight<EL> v[PIECES];
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const int64_t p = first + i * THREADS;
+    if (p >= pieces) continue;   // (a block's four threads all or none: pieces is a multiple of four)
+    if constexpr (VEC) {
+      v[i] = *reinterpret_cast<const Eight<EL> *>(__builtin_assume_aligned(x + p * BYTES, 16));
+    } else {
+      typedef typename std::conditional<EL == EL_F32, uint32_t, uint16_t>::type Word;
+      const Word *from = reinterpret_cast<const Word *>(x + p * BYTES);
+      Word *to = reinterpret_cast<Word *>(v[i].w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) to[e] = from[e];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const int64_t p = first + i * THREADS;
+    if (p >= pieces) continue;
+    const uint32_t byte = scale_byte(quad_max(largest<EL>(v[i])));
+    Q[row * pieces + p] = encode<EL>(v[i], byte);
+    if ((threadIdx.x & 3) == 0) scales[(row * pieces + p) >> 2] = (uint8_t)byte;
+  }
+}
+
+template <int EL>
+__global__ __launch_bounds__(THREADS) void dequantize_kernel(const uint32_t *Q, const uint8_t *scales, int64_t pieces, char *X, bool vec) {
+  const int64_t first = wide_block() * (THREADS * PIECES) + threadIdx.x;
+  uint32_t q[PIECES], byte[PIECES];
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const int64_t p = first + i * THREADS;
+    q[i] = byte[i] = 0;
+    if (p < pieces) {
+      q[i] = Q[p];
+      byte[i] = scales[p >> 2];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const int64_t p = first + i * THREADS;
+    if (p >= pieces) continue;
+    const float x = byte[i] == 255 ? __builtin_nanf("") : scale_value(byte[i]);
+    float f[8];   // (the code's number is exact, and so is its product unless it is NaN, or infinite)
+    auto two = [&](int at, auto pair) {
+      f[at] = pair[0] * x;
+      f[at + 1] = pair[1] * x;
+    };
+    two(0, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i], 1.f, 0));
+    two(2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i], 1.f, 1));
+    two(4, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i], 1.f, 2));
+    two(6, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i], 1.f, 3));
+    if constexpr (EL == EL_F32) {
+      float *to = reinterpret_cast<float *>(X) + 8 * p;
+      if (vec) {
+        *reinterpret_cast<floatx4 *>(to) = floatx4{f[0], f[1], f[2], f[3]};
+        *reinterpret_cast<floatx4 *>(to + 4) = floatx4{f[4], f[5], f[6], f[7]};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) to[e] = f[e];
+      }
+    } else {
+      union { uint16_t h[8]; uint4v w; } o;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (EL == EL_BF16) o.h[e] = __builtin_bit_cast(uint16_t, (__bf16)f[e]);
+        else o.h[e] = __builtin_bit_cast(uint16_t, (half_t)f[e]);
+      }
+      uint16_t *to = reinterpret_cast<uint16_t *>(X) + 8 * p;
+      if (vec) {
+        *reinterpret_cast<uint4v *>(to) = o.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) to[e] = o.h[e];
+      }
+    }
+  }
+}
+
+// The scales of rows of blocks blocks each, with zeros behind them up to `pitch` (a multiple of 16): the tiles read them 2, 8 or 16 bytes at
+// a time.  A thread has 16 bytes.
+__global__ __launch_bounds__(THREADS) void pad_scales_kernel(const uint8_t *S, int64_t rows, int blocks, int pitch, uint8_t *out) {
+  const int64_t i = wide_block() * THREADS + threadIdx.x, units = pitch / 16, row = i / units;
+  if (row >= rows) return;
+  const int b0 = (int)(i - row * units) * 16;
+  const uint8_t *from = S + row * blocks + b0;
+  union { uint8_t b[16]; uint4v w; } o;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) o.b[e] = b0 + e < blocks ? from[e] : 0;
+  *reinterpret_cast<uint4v *>(out + row * pitch + b0) = o.w;
+}
+
+int element_of(int dtype) { return dtype == SK_F16 ? EL_F16 : (dtype == SK_BF16 ? EL_BF16 : (dtype == SK_F32 ? EL_F32 : -1)); }
+bool misaligned(const void *p, uintptr_t mask) { return (reinterpret_cast<uintptr_t>(p) & mask) != 0; }
+// rows and values of a launch: every index counts in 64 bits, blocks in those of a launch
+bool fits(int64_t M, int64_t K) { return M > 0 && K > 0 && M <= ((int64_t)1 << 40) && K <= ((int64_t)1 << 31) && M <= ((int64_t)1 << 45) / K; }
+
+}  // namespace
+
+extern "C" int sk_quantize_mxfp4(const void *X, int dtype, int64_t M, int64_t K, int64_t ldx, void *Q, void *scales, void *stream) {
+  const int el = element_of(dtype);
+  if (el < 0) return SK_ERR_CONFIG;
+  if (!X || !Q || !scales) return SK_ERR_NULL;
+  if (!fits(M, K) || ldx < K || ldx > ((int64_t)1 << 40)) return SK_ERR_SHAPE;
+  const int size = el == EL_F32 ? 4 : 2;
+  if (K % 32 || misaligned(X, size - 1) || misaligned(Q, 3)) return SK_ERR_ALIGN;
+  const bool vec = !misaligned(X, 15) && (M == 1 || ldx * size % 16 == 0);
+  int64_t rows = M, pieces = K / 8;
+  if (ldx == K || M == 1) {   // one row
+    pieces *= M;
+    rows = 1;
+  }
+  const int64_t blocks = (pieces + THREADS * PIECES - 1) / (THREADS * PIECES);
+#define SK_QUANTIZE(EL, VEC)                                                                                                                       \
+  hipLaunchKernelGGL((quantize_kernel<EL, VEC>), wide_grid(rows * blocks), dim3(THREADS), 0, (hipStream_t)stream, (const char *)X, rows, pieces, \
+                     ldx * size, blocks, (uint32_t *)Q, (uint8_t *)scales)
+  if (el == EL_F16) {
+    if (vec) SK_QUANTIZE(EL_F16, true);
+    else SK_QUANTIZE(EL_F16, false);
+  } else if (el == EL_BF16) {
+    if (vec) SK_QUANTIZE(EL_BF16, true);
+    else SK_QUANTIZE(EL_BF16, false);
+  } else {
+    if (vec) SK_QUANTIZE(EL_F32, true);
+    else SK_QUANTIZE(EL_F32, false);
+  }
+#undef SK_QUANTIZE
+  return hipGetLastError() == hipSuccess ? SK_OK : SK_ERR_LAUNCH;
+}
+
+extern "C" int sk_dequantize_mxfp4(const void *Q, const void *scales, int64_t M, int64_t K, int dtype, void *X, void *stream) {
+  const int el = element_of(dtype);
+  if (el < 0) return SK_ERR_CONFIG;
+  if (!X || !Q || !scales) return SK_ERR_NULL;
+  if (!fits(M, K)) return SK_ERR_SHAPE;
+  if (K % 32 || misaligned(X, el == EL_F32 ? 3 : 1) || misaligned(Q, 3)) return SK_ERR_ALIGN;
+  const int64_t pieces = M * (K / 8);
+  const dim3 grid = wide_grid((pieces + THREADS * PIECES - 1) / (THREADS * PIECES));
+  const bool vec = !misaligned(X, 15);
+#define SK_DEQUANTIZE(EL)                                                                                                                     \
+  hipLaunchKernelGGL((dequantize_kernel<EL>), grid, dim3(THREADS), 0, (hipStream_t)stream, (const uint32_t *)Q, (const uint8_t *)scales, pieces, \
+                     (char *)X, vec)
+  if (el == EL_F16) SK_DEQUANTIZE(EL_F16);
+  else if (el == EL_BF16) SK_DEQUANTIZE(EL_BF16);
+  else SK_DEQUANTIZE(EL_F32);
+#undef SK_DEQUANTIZE
+  return hipGetLastError() == hipSuccess ? SK_OK : SK_ERR_LAUNCH;
+}
+
+extern "C" int sk_pad_mx_scales(const void *scales, int64_t rows, int64_t blocks, int64_t pitch, void *out, void *stream) {
+  if (!scales || !out) return SK_ERR_NULL;
+  if (!fits(rows, blocks) || pitch < blocks || pitch > 0x7fffff00) return SK_ERR_SHAPE;
+  if (pitch % 16 || misaligned(out, 15)) return SK_ERR_ALIGN;
+  const int64_t units = rows * (pitch / 16);
+  hipLaunchKernelGGL(pad_scales_kernel, wide_grid((units + THREADS - 1) / THREADS), dim3(THREADS), 0, (hipStream_t)stream, (const uint8_t *)scales, rows,
+                     (int)blocks, (int)pitch, (uint8_t *)out);
+  return hipGetLastError() == hipSuccess ? SK_OK : SK_ERR_LAUNCH;
+}

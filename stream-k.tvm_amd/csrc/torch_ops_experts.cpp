@@ -125,10 +125,117 @@ bool grouped(const Tensor &rows, const Tensor &B, const Tensor &offsets, std::st
   if (need > 0 && !streamk_torch::find_workspace((int)c10::hip::current_device(), stream, need, &ws)) return false;
   return sk_gemm_grouped(&g, ws.ptr, ws.bytes, stream) == SK_OK;
 }
+// ---- microscaled 4-bit operands ----
+std::tuple<Tensor, Tensor> quantize_mxfp4(const Tensor &x) {
+  at::AutoDispatchBelowADInplaceOrView guard;
+  const int dtype = dtype_of(x.scalar_type());
+  if (x.is_cuda() && dtype >= 0 && dtype != SK_I8 && x.dim() >= 1 && x.numel() > 0 && x.size(-1) % 32 == 0 && x.is_contiguous()) {
+    const int64_t K = x.size(-1), M = x.numel() / K;
+    c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = K / 2;
+    Tensor q = fresh(x, shape, at::kByte);
+    shape.back() = K / 32;
+    Tensor scale = fresh(x, shape, at::kByte);
+    if (sk_quantize_mxfp4(x.data_ptr(), dtype, M, K, K, q.data_ptr(), scale.data_ptr(), current_stream()) == SK_OK) return {q, scale};
+  }
+  GENERAL("quantize_mxfp4", decltype(quantize_mxfp4), x);
+}
+Tensor dequantize_mxfp4(const Tensor &q, const Tensor &scale, at::ScalarType dtype) {
+  at::AutoDispatchBelowADInplaceOrView guard;
+  const int to = dtype_of(dtype);
+  if (q.is_cuda() && q.scalar_type() == at::kByte && q.dim() >= 1 && q.numel() > 0 && q.size(-1) % 16 == 0 && q.is_contiguous() && aligned(q, 4) &&
+      scale.scalar_type() == at::kByte && scale.dim() == q.dim() && scale.is_contiguous() && scale.device() == q.device() && to >= 0 && to != SK_I8 &&
+      scale.size(-1) * 16 == q.size(-1) && scale.sizes().slice(0, q.dim() - 1) == q.sizes().slice(0, q.dim() - 1)) {
+    const int64_t K = 2 * q.size(-1);
+    c10::SmallVector<int64_t, 6> shape(q.sizes().begin(), q.sizes().end());
+    shape.back() = K;
+    Tensor x = fresh(q, shape, dtype);
+    if (sk_dequantize_mxfp4(q.data_ptr(), scale.data_ptr(), x.numel() / K, K, to, x.data_ptr(), current_stream()) == SK_OK) return x;
+  }
+  GENERAL("dequantize_mxfp4", decltype(dequantize_mxfp4), q, scale, dtype);
+}
+// offsets null: one matrix, B [N, K / 2]
+bool mx_product(const Tensor &A, const Tensor &B, const Tensor *offsets, MaybeType out_dtype, const Tensor *scale_a, const Tensor *scale_b, const Tensor *bias,
+                std::string_view activation, int64_t variant, Tensor &C) {
+  const int64_t dims = offsets ? 3 : 2;
+  if (A.scalar_type() != at::kByte || B.scalar_type() != at::kByte || B.dim() != dims || B.device() != A.device() || !scale_a || !scale_b) return false;
+  if (!rows_in_place(A) && !one_row_in_place(A)) return false;
+  const int64_t E = offsets ? B.size(0) : 1, N = B.size(-2), K = 2 * B.size(-1), R = A.size(0);
+  if (E == 0 || N < 2 || K == 0 || K % 32 || 2 * A.size(1) != K || B.stride(-1) != 1) return false;
+  if (offsets && (!is_ints(*offsets, A, 1) || offsets->size(0) != E + 1)) return false;
+  const auto of = [&](const Tensor &t, at::ScalarType want, int64_t rows, int64_t last, bool of_b) {   // contiguous [rows, last], of B with its leading sizes
+    const int64_t dim = (of_b ? dims - 1 : 1) + (last ? 1 : 0);
+    if (t.scalar_type() != want || t.dim() != dim || !t.is_contiguous() || t.device() != A.device() || (last && t.size(-1) != last)) return false;
+    return of_b && offsets ? t.size(0) == E && t.size(1) == N : t.size(0) == rows;
+  };
+  if (!of(*scale_a, at::kByte, R, K / 32, false) || !of(*scale_b, at::kByte, N, K / 32, true)) return false;
+  const at::ScalarType out = out_dtype.value_or(at::kHalf);
+  if ((out != at::kHalf && out != at::kBFloat16) || (bias && !of(*bias, out, N, 0, true))) return false;
+  sk_grouped g{};
+  if (activation == "none") g.activation = SK_ACT_NONE;
+  else if (activation == "relu") g.activation = SK_ACT_RELU;
+  else if (activation == "gelu_tanh") g.activation = SK_ACT_GELU_TANH;
+  else if (activation == "silu") g.activation = SK_ACT_SILU;
+  else return false;
+  if (C.defined()) {
+    if (!C.is_cuda() || C.scalar_type() != out || C.dim() != 2 || C.size(0) != R || C.size(1) != N || C.stride(1) != 1 || (R > 1 && C.stride(0) < N) || C.device() != A.device()) return false;
+  } else {
+    C = fresh(A, {R, N}, out);
+  }
+  g.dtype = SK_MXFP4;
+  g.layout = SK_LAYOUT_NT;
+  g.out_dtype = dtype_of(out);
+  g.E = E, g.R = R, g.N = N, g.K = K;
+  g.A = A.data_ptr(), g.B = B.data_ptr(), g.offsets = offsets ? offsets->data_ptr() : nullptr, g.C = C.data_ptr();
+  g.lda = 2 * pitch(A), g.ldb = 2 * B.stride(-2), g.ldc = R > 1 ? C.stride(0) : N, g.expert_b = E > 1 ? 2 * B.stride(0) : 0;
+  g.bias = bias ? bias->data_ptr() : nullptr;
+  g.scale_a = scale_a->data_ptr();
+  g.scale_b = scale_b->data_ptr();
+  g.variant = variant;
+  void *stream = current_stream();
+  Tensor padded[2];   // (freed in stream order)
+  if (const int64_t wide = sk_mx_scale_pitch(&g)) {
+    const Tensor *from[2] = {scale_a, scale_b};
+    for (int i = 0; i < 2; ++i) {
+      const int64_t rows = i ? E * N : R;
+      padded[i] = fresh(A, {rows, wide}, at::kByte);
+      if (sk_pad_mx_scales(from[i]->data_ptr(), rows, K / 32, wide, padded[i].data_ptr(), stream) != SK_OK) return false;
+    }
+    g.scale_a = padded[0].data_ptr();
+    g.scale_b = padded[1].data_ptr();
+    g.scale_pitch_a = g.scale_pitch_b = wide;
+  }
+  const size_t need = sk_grouped_workspace_bytes(&g);
+  std::shared_lock<std::shared_mutex> lock(streamk_torch::g_mutex);
+  streamk_torch::Buffer ws;
+  if (need > 0 && !streamk_torch::find_workspace((int)c10::hip::current_device(), stream, need, &ws)) return false;
+  return sk_gemm_grouped(&g, ws.ptr, ws.bytes, stream) == SK_OK;
+}
+const Tensor *get(const MaybeTensor &t) { return t.has_value() ? &*t : nullptr; }
+std::string_view view(c10::string_view s) { return std::string_view(s.data(), s.size()); }
+Tensor gemm_mxfp4(const Tensor &A, const Tensor &B, const Tensor &scale_a, const Tensor &scale_b, at::ScalarType out_dtype, const MaybeTensor &bias,
+                  c10::string_view activation, int64_t variant) {
+  at::AutoDispatchBelowADInplaceOrView guard;
+  Tensor C;
+  if (mx_product(A, B, nullptr, out_dtype, &scale_a, &scale_b, get(bias), view(activation), variant, C)) return C;
+  GENERAL("gemm_mxfp4", decltype(gemm_mxfp4), A, B, scale_a, scale_b, out_dtype, bias, activation, variant);
+}
+void gemm_mxfp4_out(const Tensor &A, const Tensor &B, const Tensor &scale_a, const Tensor &scale_b, const Tensor &out, const MaybeTensor &bias,
+                    c10::string_view activation, int64_t variant) {
+  at::AutoDispatchBelowADInplaceOrView guard;
+  Tensor C = out;
+  if (mx_product(A, B, nullptr, out.scalar_type(), &scale_a, &scale_b, get(bias), view(activation), variant, C)) return;
+  GENERAL("gemm_mxfp4_out", decltype(gemm_mxfp4_out), A, B, scale_a, scale_b, out, bias, activation, variant);
+}
+
 Tensor gemm_grouped(const Tensor &A, const Tensor &B, const Tensor &offsets, c10::string_view layout, MaybeType out_dtype, const MaybeTensor &scale_a,
                     const MaybeTensor &scale_b, const MaybeTensor &bias, c10::string_view activation, int64_t variant) {
   at::AutoDispatchBelowADInplaceOrView guard;
   Tensor C;
+  if (A.scalar_type() == at::kByte && layout == "nt" &&
+      mx_product(A, B, &offsets, out_dtype, get(scale_a), get(scale_b), get(bias), view(activation), variant, C))
+    return C;
+  C = Tensor();
   if (grouped(A, B, offsets, std::string_view(layout.data(), layout.size()), out_dtype, scale_a, scale_b, bias,
               std::string_view(activation.data(), activation.size()), variant, C))
     return C;
@@ -138,6 +245,9 @@ void gemm_grouped_out(const Tensor &A, const Tensor &B, const Tensor &offsets, c
                       const MaybeTensor &scale_a, const MaybeTensor &scale_b, const MaybeTensor &bias, c10::string_view activation, int64_t variant) {
   at::AutoDispatchBelowADInplaceOrView guard;
   Tensor C = out;
+  if (A.scalar_type() == at::kByte && layout == "nt" &&
+      mx_product(A, B, &offsets, out_dtype.has_value() ? out_dtype : MaybeType(out.scalar_type()), get(scale_a), get(scale_b), get(bias), view(activation), variant, C))
+    return;
   if (grouped(A, B, offsets, std::string_view(layout.data(), layout.size()), out_dtype.has_value() ? out_dtype : MaybeType(out.scalar_type()), scale_a,
               scale_b, bias, std::string_view(activation.data(), activation.size()), variant, C))
     return;
@@ -293,7 +403,6 @@ void no_tangent(const char *what, std::initializer_list<const Tensor *> operands
   for (const Tensor *t : operands)
     TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->defined() || !t->_fw_grad(0).defined(), "streamk: ", what, " has no forward-mode derivative");
 }
-const Tensor *get(const MaybeTensor &t) { return t.has_value() ? &*t : nullptr; }
 
 // Passes a result on; who asks for its derivative by one of the operands that require one gets an error with the reason.
 struct Refused : torch::autograd::Function<Refused> {
@@ -475,6 +584,10 @@ Tensor combine_routed_autograd(const Tensor &y, const Tensor &weights, const Ten
 
 TORCH_LIBRARY_IMPL(streamk, CUDA, m) {
   m.impl("quantize_i8", &quantize_i8);
+  m.impl("quantize_mxfp4", &quantize_mxfp4);
+  m.impl("dequantize_mxfp4", &dequantize_mxfp4);
+  m.impl("gemm_mxfp4", &gemm_mxfp4);
+  m.impl("gemm_mxfp4_out", &gemm_mxfp4_out);
   m.impl("gemm_grouped", &gemm_grouped);
   m.impl("gemm_grouped_out", &gemm_grouped_out);
   m.impl("grouped_wgrad", &grouped_wgrad);

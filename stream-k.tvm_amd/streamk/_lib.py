@@ -11,6 +11,7 @@ LIB_PATH = os.path.join(_HERE, "libstreamk.so")
 TORCH_LIB_PATH = os.path.join(_HERE, "libstreamk_torch.so")
 
 SK_F16, SK_F32, SK_Q4, SK_BF16, SK_Q4_TILED, SK_F8E4M3, SK_I8, SK_Q4_ZP, SK_F8E5M2, SK_Q4_ZP_TILED = 0, 1, 2, 3, 4, 5, 6, 7, 8, 9
+SK_MXFP4 = 10
 LAYOUT_NT, LAYOUT_NN = 0, 1
 SCHEDULES = {"auto": 0, "dp": 1, "sk2": 2, "sk1": 3, "basic": 4, "splitk": 5}
 FIXUPS = {"auto": 0, "atomic": 1, "reduce": 2, "atomic_c": 3, "reduce16": 4}
@@ -56,7 +57,8 @@ class SkGrouped(ctypes.Structure):
         (n, ctypes.c_int64) for n in ("E", "R", "N", "K")] + [
         (n, ctypes.c_void_p) for n in ("A", "B", "offsets", "C")] + [
         (n, ctypes.c_int64) for n in ("lda", "ldb", "ldc", "expert_b")] + [
-        (n, ctypes.c_void_p) for n in ("bias", "scale_a", "scale_b")] + [("variant", ctypes.c_int64), ("spin_limit", ctypes.c_int64)]
+        (n, ctypes.c_void_p) for n in ("bias", "scale_a", "scale_b")] + [
+        (n, ctypes.c_int64) for n in ("variant", "spin_limit", "scale_pitch_a", "scale_pitch_b")]
 
 
 SK_SCORES_SOFTMAX, SK_SCORES_SIGMOID = 0, 1
@@ -159,11 +161,17 @@ def lib():
     L.sk_route_backward.argtypes = [vp, vp, vp, i64, i64, i64, ci, vp, vp]
     L.sk_route_scored.argtypes = [vp, ci, i64, i64, i64, i64, P(SkRouteScores), vp, vp, vp, vp, vp, vp, sz, vp]
     L.sk_route_scored_backward.argtypes = [vp, ci, i64, i64, i64, i64, P(SkRouteScores), vp, vp, vp, vp]
+    L.sk_quantize_mxfp4.argtypes = [vp, ci, i64, i64, i64, vp, vp, vp]
+    L.sk_dequantize_mxfp4.argtypes = [vp, vp, i64, i64, ci, vp, vp]
+    L.sk_pad_mx_scales.argtypes = [vp, i64, i64, i64, vp, vp]
+    L.sk_mx_scale_pitch.argtypes = [P(SkGrouped)]
+    L.sk_mx_scale_pitch.restype = i64
     L.sk_dispatch_rows.argtypes = [vp, i64, i64, vp, vp, i64, i64, vp, vp]
     L.sk_combine_rows.argtypes = [vp, ci, vp, vp, i64, i64, i64, vp, vp]
     L.sk_combine_backward.argtypes = [vp, vp, ci, vp, vp, vp, i64, i64, i64, vp, vp, vp]
     for f in ("sk_gemm_i8_scaled", "sk_i8_scaled_takes", "sk_quantize_i8", "sk_gemm_grouped", "sk_grouped_wgrad", "sk_route_experts", "sk_route_backward",
-              "sk_route_scored", "sk_route_scored_backward", "sk_dispatch_rows", "sk_combine_rows", "sk_combine_backward"):
+              "sk_route_scored", "sk_route_scored_backward", "sk_quantize_mxfp4", "sk_dequantize_mxfp4", "sk_pad_mx_scales",
+              "sk_dispatch_rows", "sk_combine_rows", "sk_combine_backward"):
         getattr(L, f).restype = ci
     for f in ("sk_device_info", "sk_make_plan", "sk_plan_cta_range", "sk_plan_tile_coords",
               "sk_workspace_init", "sk_workspace_status", "sk_gemm_f16", "sk_gemm_f32",

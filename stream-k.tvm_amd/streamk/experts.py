@@ -74,9 +74,88 @@ def _padded(t):
     return _rows(t)
 
 
+# microscaled 4-bit operands: bytes of two values, and an exponent for each 32 (mxfp4.py)
+def _bytes(t):
+    """torch's own types of such bytes, as they are"""
+    return t.view(torch.uint8) if isinstance(t, torch.Tensor) and t.dtype in _BYTE_TYPES else t
+
+
+_BYTE_TYPES = tuple(getattr(torch, n) for n in ("float4_e2m1fn_x2", "float8_e8m0fnu") if hasattr(torch, n))
+
+
+def _exponents(t, name, shape, device):
+    _on_device(t, name, (torch.uint8,), len(shape))
+    if tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{name} must be contiguous uint8 {shape} on {device}, got {tuple(t.shape)} on {t.device}")
+    return t
+
+
+def _padded_exponents(t, pitch):
+    """Rows of exponents at this pitch, zeros behind them."""
+    blocks = t.shape[-1]
+    rows = t.numel() // blocks
+    out = torch.empty((rows, pitch), dtype=torch.uint8, device=t.device)
+    _lib.check(_lib.lib().sk_pad_mx_scales(t.data_ptr(), rows, blocks, pitch, out.data_ptr(), ops._stream_ptr()), "sk_pad_mx_scales")
+    return out
+
+
+def _mx_product(A, B, offsets, scale_a, scale_b, out_dtype, bias, activation, variant, out):
+    """offsets None: one matrix, B [N, K / 2]."""
+    _on_device(A, "A", (torch.uint8,), 2)
+    dense = offsets is None
+    _on_device(B, "B", (torch.uint8,), 2 if dense else 3)
+    if A.device != B.device:
+        raise ValueError(f"A is on {A.device}, B on {B.device}")
+    lead, N = tuple(B.shape[:-1]), B.shape[-2]
+    E, R, K = 1 if dense else B.shape[0], A.shape[0], 2 * A.shape[1]
+    if 2 * B.shape[-1] != K:
+        raise ValueError(f"K mismatch: A is {tuple(A.shape)}, B is {tuple(B.shape)} (bytes of two values)")
+    if E == 0 or N == 0 or K == 0 or K % 32:
+        raise ValueError(f"B must not be empty and K a multiple of 32, got {tuple(B.shape)} (bytes of two values)")
+    if B.stride(-1) != 1:
+        raise ValueError("B must have unit stride along its last dimension")
+    if not dense:
+        _check_offsets(offsets, E, A.device)
+    if scale_a is None or scale_b is None:
+        raise ValueError("4-bit operands need scale_a and scale_b")
+    _exponents(scale_a, "scale_a", (R, K // 32), A.device)
+    _exponents(scale_b, "scale_b", (*lead, K // 32), A.device)
+    if out_dtype not in _TYPES:
+        raise ValueError("out_dtype must be torch.float16 or torch.bfloat16")
+    if activation not in _lib.ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(k for k in _lib.ACTIVATIONS if k)} or None")
+    if bias is not None and (not isinstance(bias, torch.Tensor) or bias.dtype != out_dtype or tuple(bias.shape) != lead or not bias.is_contiguous() or bias.device != A.device):
+        raise ValueError(f"bias must be contiguous {out_dtype} {lead} on {A.device}")
+    if out is not None:
+        ops._check_out(out, R, N, out_dtype)
+        if out.device != A.device:
+            raise ValueError(f"A is on {A.device}, out on {out.device}")
+    C = torch.empty((R, N), dtype=out_dtype, device=A.device) if out is None else out
+    if R == 0:
+        return C
+    A = _rows(A)
+    g = _lib.SkGrouped(dtype=_lib.SK_MXFP4, layout=ops._plan_mod._LAYOUTS["nt"], out_dtype=_TYPES[out_dtype], activation=_lib.ACTIVATIONS[activation], E=E, R=R, N=N,
+                       K=K, A=A.data_ptr(), B=B.data_ptr(), offsets=offsets.data_ptr() if not dense else None, C=C.data_ptr(), lda=2 * _pitch(A),
+                       ldb=2 * (B.stride(-2) if N > 1 else K // 2), ldc=max(C.stride(0), N), expert_b=2 * B.stride(0) if E > 1 else 0,
+                       bias=bias.data_ptr() if bias is not None else None, scale_a=scale_a.data_ptr(), scale_b=scale_b.data_ptr(), variant=variant)
+    pitch = _lib.lib().sk_mx_scale_pitch(ctypes.byref(g))
+    if pitch:
+        scale_a, scale_b = _padded_exponents(scale_a, pitch), _padded_exponents(scale_b, pitch)
+        g.scale_a, g.scale_b, g.scale_pitch_a, g.scale_pitch_b = scale_a.data_ptr(), scale_b.data_ptr(), pitch, pitch
+    ws = ops._workspace(_lib.lib().sk_grouped_workspace_bytes(ctypes.byref(g)), A.device)
+    _lib.check(_lib.lib().sk_gemm_grouped(ctypes.byref(g), ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
+                                          ops._stream_ptr()), "sk_gemm_grouped")
+    return C
+
+
 def _grouped(A, B, offsets, layout="nt", out_dtype=None, scale_a=None, scale_b=None, bias=None, activation="none", variant=0, out=None):
     if layout not in ("nt", "nn"):
         raise ValueError("layout must be 'nt' (B is [E, N, K]) or 'nn' (B is [E, K, N])")
+    if isinstance(A, torch.Tensor) and A.dtype == torch.uint8:
+        if layout != "nt":
+            raise ValueError("4-bit weights are [E, N, K / 2] ('nt')")
+        _on_device(offsets, "offsets", (torch.int32,), 1)
+        return _mx_product(A, B, offsets, scale_a, scale_b, torch.float16 if out_dtype is None else out_dtype, bias, activation, variant, out)
     int8 = isinstance(A, torch.Tensor) and A.dtype == torch.int8
     _on_device(A, "A", (torch.int8,) if int8 else tuple(_TYPES), 2)
     _on_device(B, "B", (A.dtype,), 3)
@@ -142,7 +221,7 @@ _GROUPED_TAIL = "str layout=\"nt\", ScalarType? out_dtype=None, Tensor? scale_a=
 
 
 def _grouped_fake(A, B, offsets, layout="nt", out_dtype=None, *rest):
-    return A.new_empty((A.shape[0], B.shape[1 if layout == "nt" else 2]), dtype=out_dtype or (torch.float16 if A.dtype == torch.int8 else A.dtype))
+    return A.new_empty((A.shape[0], B.shape[1 if layout == "nt" else 2]), dtype=out_dtype or (torch.float16 if A.dtype in (torch.int8, torch.uint8) else A.dtype))
 
 
 def _grouped_out(A, B, offsets, out, layout="nt", out_dtype=None, scale_a=None, scale_b=None, bias=None, activation="none", variant=0):
@@ -201,7 +280,8 @@ class _GroupedProduct(torch.autograd.Function):
 def streamk_grouped(A, B, offsets, *, layout="nt", scale_a=None, scale_b=None, out_dtype=None, out=None, bias=None, activation=None, variant=0):
     """Rows offsets[e] <= r < offsets[e + 1] of A [R, K] times the weights of expert e: C[r] = activation(A[r] @ B[e].T + bias[e]) for B
     [E, N, K] (layout 'nt'), A[r] @ B[e] for B [E, K, N] ('nn'); float16, bfloat16, or int8 ('nt') with scale_a [R] and scale_b
-    [E, N] (float32), whose result is `out_dtype` (float16 by default).  offsets: int32 [E + 1] on the device, ascending from 0;
+    [E, N] (float32), or microscaled 4-bit values ('nt') as quantize_mxfp4 makes them: bytes [R, K / 2] and [E, N, K / 2] with exponents
+    scale_a [R, K / 32] and scale_b [E, N, K / 32] (all uint8, K a multiple of 32); the result of these is `out_dtype` (float16 by default).  offsets: int32 [E + 1] on the device, ascending from 0;
     groups of any size; rows behind the last group come out as zeros.  K is a multiple of 8 (int8: 16) for 'nt', N of 8 for 'nn', whose K
     may be any number (rows of a K that is no multiple of 8 are copied, and so are an expert's [K, N] weights from 2 GiB on).  bias: [E, N] in C's type.  Sums in fp32 (int8: exact), rounded
     once.  Differentiable in A and B without bias, activation, scales and out.  variant: which tiles run (sk_grouped in streamk.h); 0
@@ -209,6 +289,7 @@ def streamk_grouped(A, B, offsets, *, layout="nt", scale_a=None, scale_b=None, o
     activation = activation or "none"
     if not _NATIVE:
         _no_tangent("the grouped product", A, B, bias, scale_a, scale_b)
+    A, B, scale_a, scale_b = (_bytes(t) for t in (A, B, scale_a, scale_b))
     if torch.is_grad_enabled() and (A.requires_grad or B.requires_grad or (bias is not None and bias.requires_grad)):
         if bias is not None or activation != "none" or scale_a is not None or scale_b is not None or out is not None:
             raise ValueError("the grouped product has gradients only without bias, activation, scales and out")
