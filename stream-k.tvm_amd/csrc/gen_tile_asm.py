@@ -63,9 +63,23 @@ Low tiles (SK_TILE_ASM_*_LOW, _LOW_NN): at most 128 rows of A, 64 to a wave, who
 stand where blocks 0-3 of a full tile's waves do, so A has EARLY row groups only, and these are 32 consecutive rows of A each.  A
 block of the loop is 32 MFMAs with four loads (block 0) and eight (block 1); the loop's state rides with the reads at the top.  NN: B's row groups are split by K-step, as in the TN layout.
 
+Microscaled 4-bit operands (tile_mx_asm_gen.h, written with the argument `mx`; SK_TILE_ASM_LOOP_MX): the bytes travel as the 16-bit loop's, so that
+an iteration is 256 values of K and a block one v_mfma_scale_f32_16x16x128_f8f6f4 of 128 for each pair of fragments -- as many cycles as the
+16-bit MFMA of 32.  Lane group g takes the 16-byte chunks 2 g (block 0) and 2 g + 1 (block 1) of a row, 32 values each, whose exponents
+are two neighbouring bytes: one register per 16 rows holds both, and the MFMA picks the block's byte.
+  v[88:103] v[104:119]   exponents of the even / odd iterations: A's eight 16-row blocks, then B's
+  v122                   what the last iteration of a K that is no multiple of 256 may not load
+  v[124:127]             the second chunk's fragment addresses of A and B, the addresses of the exponents
+  s88 s89                where the next exponents go in LDS, how far they are into the rows
+Exponents come in pairs of iterations, 16 bytes for each of the 512 rows: 16 KB behind the stages, two pairs of 8 KB.  Each wave fetches
+64 rows of A and 64 of B in block 0 of an even iteration, for the pair behind this one; each block reads eight registers for the next iteration.
+The loop has two iterations in its body.
+
 SK_TILE_ASM_LOOP_WRAP and _LOW (NT): a segment may start anywhere in K and wrap around; iteration %[wrap] is that of the first K, and from
 the one before it the offsets move by %[back].
 """
+
+import sys
 
 A0, B0, A1, B1 = 128, 160, 192, 224     # first registers of the fragment buffers
 VOA, VOB, VOB1, VOA1 = 120, 121, 122, 123   # v120 / v121 (/ v122, v123: odd row groups of B, of A, in the [K, ..] layouts): load offsets of this iteration
@@ -353,6 +367,135 @@ def loop_text(nn, low=False, wrap=False):
     return L
 
 
+MX_RA1, MX_RB1, MX_RDA, MX_RDB, MX_TAIL = 124, 125, 126, 127, 122
+S_EL, S_EK = 88, 89
+
+
+def loop_text_mx():
+    """The 16-bit NT loop on microscaled 4-bit operands; see above.  %[tail]: 0x80000000 in the lanes whose chunk lies behind K in the
+    last iteration, else 0; %[rea], %[reb], %[vea], %[veb], %[ek], %[el]: descriptors, lane offsets, offset in the rows and LDS address (the wave's 64
+    rows) of the exponents behind the first pair's; %[rda], %[rdb]: where the lane reads the first ones."""
+    L = []
+    e = L.append
+    order = mfma_order()
+    early, late = early_groups(False), late_groups(False)
+
+    def exponents(p):
+        return 88 if p == 0 else 104
+
+    def mf(i, j, kk, p):
+        c, x = (8 * i + j) * 4, exponents(p)
+        ab, bb = (A0, B0) if kk == 0 else (A1, B1)
+        e(f'"v_mfma_scale_f32_16x16x128_f8f6f4 a[{c}:{c + 3}], v[{bb + 4 * j}:{bb + 4 * j + 3}], v[{ab + 4 * i}:{ab + 4 * i + 3}], a[{c}:{c + 3}], '
+          f'v{x + 8 + j}, v{x + i} op_sel:[{kk},{kk},0] op_sel_hi:[0,0,0] cbsz:4 blgp:4')
+
+    def read(which, i, kk):
+        base = {("A", 0): A0, ("A", 1): A1, ("B", 0): B0, ("B", 1): B1}[(which, kk)]
+        addr = {("A", 0): "%[ra0]", ("A", 1): f"v{MX_RA1}", ("B", 0): "%[rb0]", ("B", 1): f"v{MX_RB1}"}[(which, kk)]
+        return ([(which, kk, i)], [f'"ds_read_b128 v[{base + 4 * i}:{base + 4 * i + 3}], {addr} offset:{i * 2048}'])
+
+    def read_exponents(p, which):      # for an iteration of parity p
+        x = exponents(p) + (0 if which == "A" else 8)
+        return [([("E", which, i)], [f'"ds_read_u16 v{x + i}, v{MX_RDA if which == "A" else MX_RDB} offset:{i * 256 + 8 * p}']) for i in range(8)]
+
+    def early_reads(kk):
+        return [read("A", 0, kk)] + [read("B", j, kk) for j in range(4)] + [read("A", i, kk) for i in range(1, 4)]
+
+    def late_reads(kk):
+        return [read("B", j, kk) for j in range(4, 8)] + [read("A", i, kk) for i in range(4, 8)]
+
+    def load_groups(xs):
+        groups = []
+        for pre, m0, ld in load_sequence(xs, False, f"v{VOA}", f"v{VOB}", None, f"s{S_LDS}", f"s{S_KA}", f"s{S_KB}"):
+            groups += [(None, pre + [m0]), (None, [ld])]
+        return groups
+
+    def load_exponents():              # of the next pair
+        return [(None, [f'"s_mov_b32 m0, s{S_EL}']), (None, [f'"buffer_load_dwordx4 %[vea], %[rea], s{S_EK} offen lds']),
+                (None, [f'"s_add_u32 m0, s{S_EL}, 4096', f'"s_xor_b32 s{S_EL}, s{S_EL}, 0x2000']),
+                (None, [f'"buffer_load_dwordx4 %[veb], %[reb], s{S_EK} offen lds', f'"s_add_u32 s{S_EK}, s{S_EK}, 16'])]
+
+    def offsets(ahead):                # as offsets_for, with the last iteration's mask
+        return [[f'"s_add_u32 s{S_T2}, s{S_IT}, {ahead}', f'"s_cmp_lt_u32 s{S_T2}, %[n]', f'"s_cselect_b32 s{S_OOB}, 0, 0x80000000'],
+                [f'"s_add_u32 s{S_T2}, s{S_T2}, 1', f'"s_cmp_eq_u32 s{S_T2}, %[n]', f'"s_cselect_b32 s{S_M0}, 0x80000000, 0'],
+                [f'"v_and_b32 v{MX_TAIL}, s{S_M0}, %[tail]'], [f'"v_or3_b32 v{VOA}, s{S_OOB}, %[voa], v{MX_TAIL}'], [f'"v_or3_b32 v{VOB}, s{S_OOB}, %[vob], v{MX_TAIL}']]
+
+    def flip(reg, bits="0x10000"):
+        return (None, [f'"v_xor_b32 {reg}, {bits}, {reg}'])
+
+    def block(b, p, tr, plan, closing):
+        for m, (i, j) in enumerate(order):
+            w = tr.wait_for({("A", b, i), ("B", b, j)})
+            if w:
+                e(w)
+            mf(i, j, b, p)
+            tags, texts = plan.get(m, (None, []))
+            L.extend(texts)
+            for t in tags or []:
+                tr.issue(t)
+        assert all(0 <= g <= 63 for g in plan), sorted(plan)
+        L.extend(closing)
+
+    # ---- entry, as in the 16-bit loop
+    zero_accumulators(L)
+    e(f'"s_mov_b32 s{S_IT}, 0')
+    e(f'"s_xor_b32 s{S_LDS}, %[lds], 0x10000')
+    e(f'"s_add_u32 s{S_KA}, %[ga0], 128')
+    e(f'"s_add_u32 s{S_KB}, %[gb0], 128')
+    e(f'"s_mov_b32 s{S_EL}, %[el]')
+    e(f'"s_mov_b32 s{S_EK}, %[ek]')
+    e(f'"v_xor_b32 v{MX_RA1}, 16, %[ra0]')
+    e(f'"v_xor_b32 v{MX_RB1}, 16, %[rb0]')
+    e(f'"v_mov_b32 v{MX_RDA}, %[rda]')
+    e(f'"v_mov_b32 v{MX_RDB}, %[rdb]')
+    for texts in offsets(1):
+        L.extend(texts)
+    e(f'"s_waitcnt vmcnt({len(early)})')
+    e('"s_barrier')
+    at_top = []
+    for tags, texts in read_exponents(0, "A") + read_exponents(0, "B") + early_reads(0):
+        L.extend(texts)
+        at_top += tags
+    e('"s_nop 7')
+
+    def body(p):
+        # ---- block 0 (the exponents' address moves on with the pair)
+        plan = dict(enumerate(late_reads(0)))
+        first = TOP
+        if p == 1:
+            plan[first] = (None, flip(f"v{MX_RDA}", "0x2000")[1] + flip(f"v{MX_RDB}", "0x2000")[1])
+            first += 1
+        spread(plan, load_groups(late) + (load_exponents() if p == 0 else []), first, LD_LAST)
+        spread(plan, early_reads(1), first, RD_LAST)
+        spread(plan, read_exponents(1 - p, "A"), first, RD_LAST)
+        spread(plan, [flip("%[ra0]"), flip("%[rb0]")], first, 63)
+        block(0, p, LdsTracker(at_top if p == 0 else ()), plan, [f'"s_waitcnt vmcnt({len(late) + (2 if p == 0 else 0)}) lgkmcnt(0)', '"s_barrier'])
+        # ---- block 1
+        plan = dict(enumerate(late_reads(1)))
+        state = [[f'"s_add_u32 s{S_KA}, s{S_KA}, 128', f'"s_add_u32 s{S_KB}, s{S_KB}, 128', f'"s_xor_b32 s{S_LDS}, s{S_LDS}, 0x10000']] + offsets(2)
+        for g, texts in enumerate(state):
+            plan[TOP + g] = (None, texts)
+        after = TOP + len(state)
+        plan[63] = (None, [f'"s_add_u32 s{S_IT}, s{S_IT}, 1'])
+        spread(plan, load_groups(early), after, LD_LAST)
+        spread(plan, early_reads(0), after, RD_LAST)
+        spread(plan, read_exponents(1 - p, "B"), after, RD_LAST)
+        spread(plan, [flip(f"v{MX_RA1}"), flip(f"v{MX_RB1}")], after, 62)
+        block(1, p, LdsTracker(), plan, [f'"s_waitcnt vmcnt({len(early)}) lgkmcnt(0)', '"s_barrier', f'"s_cmp_lt_u32 s{S_IT}, %[n]',
+                                         '"s_cbranch_scc0 L_sk_end%=' if p == 0 else '"s_cbranch_scc1 L_sk_loop%='])
+
+    e('"L_sk_loop%=:')
+    body(0)
+    body(1)
+    e('"L_sk_end%=:')
+    for a, b in zip(L, L[1:]):
+        assert not ("m0" in a and "buffer_load" in b), (a, b)
+    e('"s_waitcnt vmcnt(0) lgkmcnt(0)')
+    for _ in range(3):
+        e('"s_nop 7')
+    return L
+
+
 def loop_text_f8():
     """fp8 operands (SK_TILE_ASM_LOOP_F8): one v_mfma_f32_16x16x128_f8f6f4 per accumulator block and iteration, on
     32-byte fragments made of the two 16-byte fragments of the 16-bit loop (which K-values a lane's bytes stand for
@@ -525,6 +668,16 @@ def emit_macro(name, params, lines):
     print("  \"\"")
 
 
+def main_mx():
+    print("// Generated by gen_tile_asm.py mx -- do not edit; see that file for the register plan and the schedule.")
+    print("#pragma once")
+    emit_macro("SK_TILE_ASM_LOOP_MX", "", loop_text_mx())
+    clob = [f'"a{r}"' for r in range(256)] + [f'"v{r}"' for r in range(88, 256)] + [f'"s{r}"' for r in range(80, 90)]
+    print("#define SK_TILE_ASM_CLOBBERS_MX \\")
+    for k in range(0, len(clob), 16):
+        print("  " + ", ".join(clob[k:k + 16]) + (", \\" if k + 16 < len(clob) else ""))
+
+
 def main():
     print("// Generated by gen_tile_asm.py -- do not edit; see that file for the register plan and the schedule.")
     print("// SK_TILE_ASM_LOADS / _LOADS_NN / _LOADS_TN: the 16 loads of one stage.  SK_TILE_ASM_LOOP(MF) / _LOOP_NN(MF) / _LOOP_TN(MF): the loop")
@@ -559,4 +712,4 @@ def main():
 
 
 if __name__ == "__main__":
-    main()
+    main_mx() if sys.argv[1:] == ["mx"] else main()

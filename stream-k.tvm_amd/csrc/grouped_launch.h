@@ -36,6 +36,8 @@ struct MxOperands;
 int mx_variant(const GroupedShape &h);
 size_t mx_workspace(const GroupedShape &h);
 int mx_scale_step(const GroupedShape &h);   // K is a multiple of it, or the exponents have to be padded
+size_t mx_asm_workspace(int cus);           // kernels_mx_asm.hip
+int launch_mx_asm(const MxOperands &g, const GroupedShape &h, bool bf16, const Workspace &ws, hipStream_t s);
 int launch_mx(const MxOperands &g, const GroupedShape &h, bool bf16, const Workspace &ws, hipStream_t s);
 
 struct WgradArgs {

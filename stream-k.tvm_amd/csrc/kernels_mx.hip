@@ -39,19 +39,22 @@ static int launch(const MxOperands &operands, const GroupedShape &h, const Works
 int mx_variant(const GroupedShape &h) {
   if (h.variant != GV_RULE) return h.variant;
   const int64_t rows = (h.R + h.E - 1) / h.E;
+  if (rows > 512) return GV_ASM256;
   return rows <= 16 ? GV_WAVEK16 : (rows <= 32 ? GV_WAVEK32 : GV_WAVEK64);
 }
 size_t mx_workspace(const GroupedShape &h) {
   const int v = mx_variant(h);
+  if (v == GV_ASM256) return mx_asm_workspace(h.cus);
 #define X(V, FM, FN) \
   if (v == V) return (size_t)WS_PART_OFF + (size_t)2 * h.cus * (16 * FM) * (16 * FN) * 4;
   MX_TILES(X)
 #undef X
   return 0;
 }
-int mx_scale_step(const GroupedShape &) { return 64; }
+int mx_scale_step(const GroupedShape &h) { return mx_variant(h) == GV_ASM256 ? 512 : 64; }
 int launch_mx(const MxOperands &g, const GroupedShape &h, bool bf16, const Workspace &ws, hipStream_t s) {
   const bool dense = g.offsets == nullptr;
+  if (h.variant == GV_ASM256) return launch_mx_asm(g, h, bf16, ws, s);
 #define X(V, FM, FN)                                                                                                             \
   if (h.variant == V) {                                                                                                          \
     if (dense) return bf16 ? launch<TileWaveKMx<true, FM, FN>, true>(g, h, ws, s) : launch<TileWaveKMx<false, FM, FN>, true>(g, h, ws, s); \

@@ -58,7 +58,7 @@ struct AsmEnd {
   static __device__ __forceinline__ void store(half_t *C, int64_t ldc, int M, int N, int row0, int col0, const float *sa, const float *sb, const half_t *bias,
                                                int i0, int i1) {
     const int lane = pin_here((int)threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    char *patch = P::lds() + 2 * P::STAGE_BYTES + wave * P::FAST_PATCH_BYTES;
+    char *patch = P::lds() + P::PATCHES_AT + wave * P::FAST_PATCH_BYTES;
     char *to = patch + (lane & 15) * STRIDE + (lane >> 4) * 16;
     const char *from = patch + (lane >> 3) * STRIDE + (lane & 7) * 32;
     const int col = col0 + (lane & 7) * 8;

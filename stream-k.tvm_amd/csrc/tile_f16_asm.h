@@ -49,13 +49,14 @@ __device__ __forceinline__ void agpr_write4(floatx4 x) {
 // MODE_: 0 fp16, 1 bfloat16, 2 int8 (int32 C; the bytes travel as pairs, so K and the leading dimensions of A
 // and B arrive in 16-bit units and the loop is the fp16 one with v_mfma_i32_16x16x64_i8 on the same fragments),
 // 3 / 4 fp8 e4m3 / e5m2 (fp16 C scaled by alpha; bytes as pairs again, one v_mfma_f32_16x16x128_f8f6f4 per block
-// and iteration in a two-phase loop of its own, see gen_tile_asm.py)
+// and iteration in a two-phase loop of its own, see gen_tile_asm.py), 5 / 6 microscaled 4-bit values with fp16 / bfloat16 C (tile_mx_asm.h has
+// their loads and loop; their exponents stand between the stages and the patches, which overlap the last KB of them)
 template <int MODE_ = 0, bool NN_ = false>
 struct TileF16Asm {
   static_assert(!(NN_ && MODE_ >= 2), "one-byte operands: NT layout only");
   typedef GemmArgs Args;
-  static constexpr bool BF16_ = MODE_ == 1, I8 = MODE_ == 2;
-  static constexpr int F8 = MODE_ >= 3 ? MODE_ - 2 : 0;  // 1: e4m3, 2: e5m2
+  static constexpr bool BF16_ = MODE_ == 1 || MODE_ == 6, I8 = MODE_ == 2, MX = MODE_ >= 5;
+  static constexpr int F8 = MODE_ >= 3 && !MX ? MODE_ - 2 : 0;  // 1: e4m3, 2: e5m2
   typedef int intx4 __attribute__((ext_vector_type(4)));
   static constexpr bool LEAN_ENTRY = true;  // see run_persistent
   static constexpr int BM = 256, BN = 256, BK = 64, WM = 2, WN = 2, NW = 4, NT = 256;
@@ -63,7 +64,8 @@ struct TileF16Asm {
   static constexpr int ROW_BYTES = 128, A_BYTES = BM * ROW_BYTES, STAGE_BYTES = 2 * A_BYTES;
   // behind the two stages: one patch of 16 rows x 272 bytes per wave for the epilogue that leaves the stages alone
   static constexpr int PATCH_STRIDE = 272, FAST_PATCH_BYTES = 16 * PATCH_STRIDE;
-  static constexpr int LDS_TOTAL = 2 * STAGE_BYTES + NW * FAST_PATCH_BYTES, LDS_BYTES = 16;
+  static constexpr int LDS_TOTAL = MX ? 160 * 1024 : 2 * STAGE_BYTES + NW * FAST_PATCH_BYTES, LDS_BYTES = 16;
+  static constexpr int PATCHES_AT = LDS_TOTAL - NW * FAST_PATCH_BYTES;
   static constexpr int TILE_ELEMS = BM * BN, NV4 = FM * FN;
   static constexpr int CTAS_PER_CU = 1, WAVES_PER_EU = 1;
   static constexpr int LDC = WTN + 8, PATCH_ROWS = 64;  // epilogue patch: 64 rows x 136 halfs per wave and pass
@@ -288,7 +290,7 @@ struct TileF16Asm {
     const uint32_t bytes = rows > 0 ? (uint32_t)(((int64_t)(rows - 1) * a.ldc + WTN) * 2) : 0u;
     const uint4v words = make_rsrc_words(a.C + (int64_t)row0 * a.ldc + col0, bytes);
     const uint4v rsrc_c = uniform_rsrc(words);  // (it depends on the wave's index)
-    const uint32_t patch = lds_address(lds()) + 2 * STAGE_BYTES + (uint32_t)wave * FAST_PATCH_BYTES;
+    const uint32_t patch = lds_address(lds()) + PATCHES_AT + (uint32_t)wave * FAST_PATCH_BYTES;
     const uint32_t wr = patch + (uint32_t)((lane & 15) * PATCH_STRIDE + (lane >> 4) * 8);
     const uint32_t rd = patch + (uint32_t)((lane >> 4) * PATCH_STRIDE + (lane & 15) * 16);
     const uint32_t voff = (uint32_t)((lane >> 4) * a.ldc + (lane & 15) * 8) * 2;

@@ -147,7 +147,7 @@ def assert_near(C, want, terms, magnitudes, pre=None):
     assert (off <= tol).all(), f"largest excess {(off - tol).max().item():.3g} of {int((off > tol).sum())} values"
 
 
-VARIANTS = (0, 3, 4, 5)
+VARIANTS = (0, 2, 3, 4, 5)
 
 
 @pytest.mark.gpu
