@@ -224,6 +224,11 @@ __device__ __forceinline__ void zero_unowned(const GroupedArgs &g, int pid, int 
   }
 }
 
+// iterations of a run, that its fix-up is worth (a cut costs about as much as two iterations; policies with longer ones say so)
+template <class P, class = void>
+struct least_run { static constexpr int value = 4; };
+template <class P>
+struct least_run<P, std::void_t<decltype(P::LEAST_RUN)>> { static constexpr int value = P::LEAST_RUN; };
 // arguments of one product without groups (dense, below): a member of that name
 template <class G, class = void>
 struct is_dense { static constexpr bool value = false; };
@@ -251,7 +256,7 @@ __device__ __forceinline__ void run_grouped_sk(const G &g, int ipt, const Worksp
     P::mac(a, acc, t.pm, t.pn, 0, ipt, smem);
     P::store_c(a, acc, t.pm, t.pn, smem, epi);
   }
-  const SkRuns runs((tiles - whole) * ipt, g.grid, 4);   // (a cut costs about as much as two iterations)
+  const SkRuns runs((tiles - whole) * ipt, g.grid, least_run<P>::value);
   if (pid >= runs.ctas || runs.total == 0) return;
   int at = runs.start(pid), left = runs.length(pid);
   int cut_tile[2] = {-1, -1}, cut_n[2];   // [0]: entered in the middle, [1]: its start is here

@@ -1,7 +1,9 @@
-// Products of microscaled 4-bit operands on tiles whose waves stream K on their own (tile_mx.h), by expert or of one matrix.
+// Products of microscaled 4-bit operands on tiles whose waves stream K on their own (tile_mx.h) or share the tile (tile_mx_shared.h), by expert
+// or of one matrix.
 #include "grouped_launch.h"
 #include "grouped_mx.h"
 #include "kernel_table.h"
+#include "tile_mx_shared.h"
 
 namespace sk {
 
@@ -15,7 +17,7 @@ struct MxWithZero : P {
 template <class P, bool DENSE>
 __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_mx_kernel(MxGrouped<DENSE> g, int ipt, Workspace ws) {
   __shared__ __attribute__((aligned(1024))) char smem[P::LDS_BYTES];
-  run_grouped_sk<MxWithZero<P>>(g, ipt, ws, smem);
+  run_grouped_sk<P>(g, ipt, ws, smem);
 }
 
 template <class P, bool DENSE>
@@ -30,12 +32,16 @@ static int launch(const MxOperands &operands, const GroupedShape &h, const Works
   return (int)hipGetLastError();
 }
 
-// variant -> blocks of 16 rows, of 16 columns:  X(variant, FM, FN)
-#define MX_TILES(X)      \
-  X(GV_WAVEK16, 1, 4)    \
-  X(GV_WAVEK32, 2, 4)    \
-  X(GV_WAVEK64, 4, 4)
+template <bool BF16, int FM, int FN>
+using MxWaveK = MxWithZero<TileWaveKMx<BF16, FM, FN>>;
 
+// variant -> policy (BF16: C's type):  X(variant, policy)
+#define MX_TILES(X)                                                 \
+  X(GV_WAVEK16, MxWaveK<BF16, 1, 4>)                              \
+  X(GV_WAVEK32, MxWaveK<BF16, 2, 4>)                              \
+  X(GV_WAVEK64, MxWaveK<BF16, 4, 4>)                              \
+  X(GV_SHARED64, TileMxShared<BF16, 64, 128, 2, 2, 4>)            \
+  X(GV_TILE128, TileMxShared<BF16, 128, 128, 2, 2, 4>)
 int mx_variant(const GroupedShape &h) {
   if (h.variant != GV_RULE) return h.variant;
   const int64_t rows = (h.R + h.E - 1) / h.E;
@@ -43,26 +49,28 @@ int mx_variant(const GroupedShape &h) {
   return rows <= 16 ? GV_WAVEK16 : (rows <= 32 ? GV_WAVEK32 : GV_WAVEK64);
 }
 size_t mx_workspace(const GroupedShape &h) {
+  constexpr bool BF16 = false;
   const int v = mx_variant(h);
   if (v == GV_ASM256) return mx_asm_workspace(h.cus);
-#define X(V, FM, FN) \
-  if (v == V) return (size_t)WS_PART_OFF + (size_t)2 * h.cus * (16 * FM) * (16 * FN) * 4;
+#define X(V, ...) \
+  if (v == V) return (size_t)WS_PART_OFF + (size_t)2 * h.cus * __VA_ARGS__::TILE_ELEMS * 4;
   MX_TILES(X)
 #undef X
   return 0;
 }
-int mx_scale_step(const GroupedShape &h) { return mx_variant(h) == GV_ASM256 ? 512 : 64; }
-int launch_mx(const MxOperands &g, const GroupedShape &h, bool bf16, const Workspace &ws, hipStream_t s) {
-  const bool dense = g.offsets == nullptr;
-  if (h.variant == GV_ASM256) return launch_mx_asm(g, h, bf16, ws, s);
-#define X(V, FM, FN)                                                                                                             \
-  if (h.variant == V) {                                                                                                          \
-    if (dense) return bf16 ? launch<TileWaveKMx<true, FM, FN>, true>(g, h, ws, s) : launch<TileWaveKMx<false, FM, FN>, true>(g, h, ws, s); \
-    return bf16 ? launch<TileWaveKMx<true, FM, FN>, false>(g, h, ws, s) : launch<TileWaveKMx<false, FM, FN>, false>(g, h, ws, s);          \
-  }
+int mx_scale_step(const GroupedShape &h) { return mx_variant(h) == GV_ASM256 ? 512 : 128; }
+template <bool BF16, bool DENSE>
+static int launch_by_variant(const MxOperands &g, const GroupedShape &h, const Workspace &ws, hipStream_t s) {
+#define X(V, ...) \
+  if (h.variant == V) return launch<__VA_ARGS__, DENSE>(g, h, ws, s);
   MX_TILES(X)
 #undef X
   return (int)hipErrorNotSupported;
+}
+int launch_mx(const MxOperands &g, const GroupedShape &h, bool bf16, const Workspace &ws, hipStream_t s) {
+  if (h.variant == GV_ASM256) return launch_mx_asm(g, h, bf16, ws, s);
+  if (g.offsets == nullptr) return bf16 ? launch_by_variant<true, true>(g, h, ws, s) : launch_by_variant<false, true>(g, h, ws, s);
+  return bf16 ? launch_by_variant<true, false>(g, h, ws, s) : launch_by_variant<false, false>(g, h, ws, s);
 }
 
 }  // namespace sk

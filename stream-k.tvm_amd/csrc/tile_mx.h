@@ -4,9 +4,10 @@
 // the block's exponent in a byte of a register.  Which block of a chunk that is does not matter as long as both operands agree: lane group g
 // takes blocks 2 g (step 0) and 2 g + 1 (step 1) of a chunk's eight, so that its two exponents are neighbours in memory.
 //
-// The rings, the order of loads, reads and refills, the sums over the waves and the end are those of tile_wavek.h.  Here a ring's unit is a
-// block of 16 rows: two loads of 8 rows x 128 bytes, 256 values a row, and one of a row's exponents, two bytes to a lane (64 x 4 bytes of
-// LDS).  What bounds it with few rows is the weights' way from memory, with many what a CU takes in.
+// The rings, the order of loads, reads and refills, the sums over the waves and the end are those of tile_wavek.h.  A wave takes two
+// neighbouring chunks of 256 values of an iteration's eight, and fetches their exponents together, 16 bytes to a row.  (Two bytes to
+// a lane with every 16 rows: 12 more loads beside the 32 of a 64 x 64 tile's two chunks, 1024 x 8192 x 8192 114 us and, without any exponents
+// but wrong, 78.)  What bounds it with few rows is the weights' way from memory, with many what a CU takes in.
 #pragma once
 #include "tile_wavek.h"
 
@@ -26,24 +27,26 @@ struct TileWaveKMx : WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> {
   typedef int intx4 __attribute__((ext_vector_type(4)));
   typedef int intx8 __attribute__((ext_vector_type(8)));
   static constexpr int FM = FM_, FN = FN_, BM = Base::BM, BN = Base::BN, WAVES = Base::WAVES, NT = Base::NT, NB = Base::NB;
-  static constexpr int KV = 64, BK = KV * WAVES;      // pairs of bytes: of a chunk, of an iteration
-  static constexpr int L = FM + FN, LOADS = 3;        // blocks of a chunk, loads of a block
-  static constexpr int MOST = 17;                     // blocks that a wave's quarter of the LDS holds
-  static constexpr int R = L > MOST / 2 ? MOST : (4 * L < MOST ? 4 * L : MOST / L * L), S = R / L, PART = R % L;
-  static_assert(S >= 1, "a chunk fits the ring");
-  static constexpr int EXPONENTS = R * 2048, RING = R * (2048 + 256), LDS_BYTES = WAVES * RING, LDS_TOTAL = LDS_BYTES;
-  static_assert(LDS_BYTES <= 160 * 1024, "LDS of a CU");
-  static constexpr int CTAS_PER_CU = 1, WAVES_PER_EU = 1;
+  static constexpr int KV = 64, BK = 2 * KV * WAVES;  // pairs of bytes: of a chunk, of an iteration
+  static constexpr int L = FM + FN;                   // blocks of a chunk, of two loads each
+  static constexpr int CHUNK = L * 2048, PAIR = L * 256;   // bytes: of a chunk, of the exponents of two
+  static constexpr int MOST = 40 * 1024;              // a wave's quarter of the LDS
+  static constexpr int S = (MOST - 2 * PAIR) / CHUNK >= 3 ? 3 : 2, PAIRS = 2;   // chunks, pairs in the ring
+  static constexpr int EXPONENTS = S * CHUNK, RING = EXPONENTS + PAIRS * PAIR, LDS_BYTES = WAVES * RING, LDS_TOTAL = LDS_BYTES;
+  static_assert(RING <= MOST, "LDS of a CU");
+  static constexpr int CTAS_PER_CU = 1, WAVES_PER_EU = 1, LEAST_RUN = 1;
   static constexpr int NMFMA = 2 * NB;                // of a chunk
   static constexpr int H = NB, HR = H - (H + 3) / 4;  // of a phase, of those that have fragments read beside them
-  static_assert(LOADS * ((S - 1) * L + PART) < 64, "the wait counter's range");
 
-  // the loads of a chunk behind which `left` more chunks of the segment follow (the last PART blocks of a segment fetch nothing)
+  // loads of a chunk of this parity, and of the `behind` chunks that follow one of parity P
+  static constexpr int loads(int parity) { return 2 * L + (parity == 0 ? 2 : 0); }
+  static constexpr int loads_behind(int P, int behind) { return behind == 0 ? 0 : loads_behind(P, behind - 1) + loads((P + behind) & 1); }
+  // a chunk of parity P behind which `left` more chunks of the segment follow
+  template <int P>
   static __device__ __forceinline__ void wait_chunk(int left) {
-    if (left >= S - 1) wavek_wait_loads<LOADS *(R - L)>();
-    else if (left == 0) wavek_wait_loads<LOADS * PART>();
-    else if (left == 1) wavek_wait_loads<LOADS *(L + PART)>();
-    else wavek_wait_loads<LOADS *(2 * L + PART)>();
+    if (left >= S - 1) wavek_wait_loads<loads_behind(P, S - 1)>();
+    else if (left == 0) wavek_wait_loads<0>();
+    else wavek_wait_loads<loads_behind(P, 1)>();
   }
   struct Frags {
     intx4 v[L][2];   // [step]; A's blocks, then the weights'
@@ -70,9 +73,8 @@ struct TileWaveKMx : WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> {
     const uint4v rsrc_ea = uniform_rsrc(make_rsrc_words(a.sa + (int64_t)pm * BM * a.pitch_a, (uint32_t)rows_a * a.pitch_a));
     const uint4v rsrc_eb = uniform_rsrc(make_rsrc_words(a.sb + (int64_t)pn * BN * a.pitch_b, (uint32_t)rows_b * a.pitch_b));
     // load e of a block: its rows 8 e .. 8 e + 7, lane's row lane / 8, piece p (16 bytes, 32 values) of row r of a block at position
-    // p ^ ((r >> 1) & 7); exponents: lane (i, g) those of pieces 2 g and 2 g + 1 of row i
+    // p ^ ((r >> 1) & 7); exponents: lane's row, 16 bytes
     const int row8 = lane >> 3, fi = lane & 15, fg = lane >> 4;
-    // (the block is in the uniform part of the address)
     uint32_t off_a[2], off_b[2];
     int kp[2];
 #pragma unroll
@@ -81,125 +83,116 @@ struct TileWaveKMx : WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> {
       off_a[e] = (uint32_t)(8 * e + row8) * lda_bytes + (uint32_t)kp[e] * 2;
       off_b[e] = (uint32_t)(8 * e + row8) * ldb_bytes + (uint32_t)kp[e] * 2;
     }
-    const uint32_t off_ea = (uint32_t)(fi * a.pitch_a + 2 * fg), off_eb = (uint32_t)(fi * a.pitch_b + 2 * fg);
+    const uint32_t off_ea = (uint32_t)(lane * a.pitch_a), off_eb = (uint32_t)(lane * a.pitch_b);
     const uint32_t ring = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_address(smem) + wave * RING);
     // one row of tiles: see rotation_of.  Several: the CTAs of an XCD share A as well as the weights and stay on the same K
     const int rot = a.M <= BM ? rotation_of(pn, n) : Base::start_of(a, pn, n);
-    // a chunk that starts kbytes into the rows and `left` pairs of bytes before K's end, pos: where it starts in the ring, in blocks.
-    // (Pieces past K fetch nothing: zeros arrive and the wait counts stay exact.)
+    const int chunks = 2 * n;
+    // a chunk that starts kbytes into the rows and `left` pairs of bytes before K's end.  (Pieces past K fetch nothing: zeros arrive and
+    // the wait counts stay exact; a chunk past K or past the segment must not carry its offset either.)
+    auto left_of = [&](int t) { return t < chunks ? a.K - (((k0 + rotated_iteration(t >> 1, rot, n)) * WAVES + wave) * 2 + (t & 1)) * KV : 0; };
     struct Chunk {
-      uint32_t kbytes;
-      int left, pos;
-      uint32_t base, base_e;   // LDS addresses of block 0, were the ring long enough
+      uint32_t kbytes, base, pair;   // base, pair: LDS addresses
+      int left;
     };
-    auto chunk = [&](int t, int pos) {
-      const int kk = ((k0 + rotated_iteration(t, rot, n)) * WAVES + wave) * KV, left = t < n ? a.K - kk : 0;
-      // (a chunk past K or past the segment must not carry its offset either)
-      const uint32_t kbytes = (uint32_t)__builtin_amdgcn_readfirstlane(left > 0 ? kk * 2 : 0);
-      return Chunk{kbytes, left, pos, ring + (uint32_t)pos * 2048, ring + EXPONENTS + (uint32_t)pos * 256};
+    auto chunk = [&](int t, int slot, int pair) {
+      const int left = left_of(t);
+      const uint32_t kbytes = (uint32_t)__builtin_amdgcn_readfirstlane(left > 0 ? (a.K - left) * 2 : 0);
+      return Chunk{kbytes, ring + (uint32_t)slot * CHUNK, ring + EXPONENTS + (uint32_t)pair * PAIR, left};
     };
     auto issue = [&](auto li, const Chunk &q) {
       constexpr int l = decltype(li)::value;
-      uint32_t base = q.base, base_e = q.base_e;
-      if (R % L != 0 && q.pos >= R - l) {
-        base -= R * 2048;
-        base_e -= R * 256;
-      }
-      const bool whole = q.left >= KV;
       constexpr bool A = l < FM;
+      const bool whole = q.left >= KV;
       const uint32_t rows = q.kbytes + (A ? l * 16 * lda_bytes : (l - FM) * 16 * ldb_bytes);
-      const uint32_t rows_e = q.kbytes / 16 + (A ? l * 16 * (uint32_t)a.pitch_a : (l - FM) * 16 * (uint32_t)a.pitch_b);
-      wavek_dma_16<l * 2048>(A ? rsrc_a : rsrc_b, base, whole || kp[0] < q.left ? (A ? off_a : off_b)[0] : OOB_OFFSET, rows);
-      wavek_dma_16<l * 2048 + 1024>(A ? rsrc_a : rsrc_b, base, whole || kp[1] < q.left ? (A ? off_a : off_b)[1] : OOB_OFFSET, rows);
-      wavek_dma_2<l * 256>(A ? rsrc_ea : rsrc_eb, base_e, whole || 16 * fg < q.left ? (A ? off_ea : off_eb) : OOB_OFFSET, rows_e);
+      wavek_dma_16<l * 2048>(A ? rsrc_a : rsrc_b, q.base, whole || kp[0] < q.left ? (A ? off_a : off_b)[0] : OOB_OFFSET, rows);
+      wavek_dma_16<l * 2048 + 1024>(A ? rsrc_a : rsrc_b, q.base, whole || kp[1] < q.left ? (A ? off_a : off_b)[1] : OOB_OFFSET, rows);
+    };
+    // (the exponents of a row's end and of what lies behind it arrive together; see read_exponents)
+    auto issue_exponents = [&](const Chunk &q) {
+      const uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)q.kbytes / 16), to = (uint32_t)__builtin_amdgcn_readfirstlane((int)q.pair);
+      if (lane < BM) wavek_dma_16<0>(rsrc_ea, to, q.left > 0 ? off_ea : OOB_OFFSET, at);
+      if (lane < BN) wavek_dma_16<FM * 256>(rsrc_eb, to, q.left > 0 ? off_eb : OOB_OFFSET, at);
     };
 #pragma unroll
     for (int t = 0; t < S; ++t)
-      if (t < n) {
-        const Chunk q = chunk(t, t * L);
+      if (t < chunks) {
+        const Chunk q = chunk(t, t, t >> 1);
+        if (t % 2 == 0) issue_exponents(q);
         static_for<0, L>([&](auto l) { issue(l, q); });
       }
-    {
-      const Chunk q = chunk(S, S * L);
-      static_for<0, PART>([&](auto l) { issue(l, q); });
-    }
 
     // fragments: lane (i, g) takes piece 2 g + s of its row for step s
     const char *mine = smem + wave * RING;
     const char *rd0 = mine + fi * 128 + ((2 * fg) ^ ((fi >> 1) & 7)) * 16, *rd1 = mine + fi * 128 + ((2 * fg + 1) ^ ((fi >> 1) & 7)) * 16;
-    const char *rd_e = mine + EXPONENTS + lane * 4;
-    constexpr int READS = LOADS * L;
-    // read r of a chunk: the fragments of step 0 and the exponents, block by block, then the fragments of step 1
-    auto read = [&](auto ri, Frags &f, int pos) {
+    const char *rd_e = mine + EXPONENTS + fi * 16 + 2 * fg;
+    constexpr int READS = 3 * L;
+    int slot = 0, pair = 0;   // of the chunk that is read next
+    // read r of a chunk of parity P: the fragments of step 0 and the exponents, block by block, then the fragments of step 1
+    auto read = [&](auto ri, auto parity, Frags &f) {
       constexpr int r = decltype(ri)::value, what = r < 2 * L ? r % 2 : 2, b = r < 2 * L ? r / 2 : r - 2 * L;
-      int p = pos;
-      if (R % L != 0 && pos >= R - b) p -= R;
-      if constexpr (what == 1) f.e[b] = *reinterpret_cast<const int *>(rd_e + p * 256 + b * 256);
-      else f.v[b][what / 2] = *reinterpret_cast<const intx4 *>((what ? rd1 : rd0) + p * 2048 + b * 2048);
+      if constexpr (what == 1) f.e[b] = *reinterpret_cast<const uint16_t *>(rd_e + pair * PAIR + b * 256 + 8 * decltype(parity)::value);
+      else f.v[b][what / 2] = *reinterpret_cast<const intx4 *>((what ? rd1 : rd0) + slot * CHUNK + b * 2048);
     };
-    int pos = 0;   // of the chunk that is read next
-    auto advance = [&] {
-      pos += L;
-      if (pos >= R) pos -= R;
+    // the last chunk of K: blocks behind K are zeros, and their exponents, which are another row's, have to be numbers
+    auto mask_exponents = [&](int left, Frags &f) {
+      if (left >= KV) return;
+      const int mask = (16 * fg < left ? 0xff : 0) | (16 * fg + 8 < left ? 0xff00 : 0);
+#pragma unroll
+      for (int b = 0; b < L; ++b) f.e[b] &= mask;
     };
-    // the place of the chunk just read (t) takes the rest of chunk t + S and the first PART blocks of chunk t + S + 1
-    Chunk q0, q1;
-    auto refill_begin = [&](int t) {
-      int p = pos + S * L;
-      if (p >= R) p -= R;
-      q0 = chunk(t + S, p);
-      p += L;
-      if (p >= R) p -= R;
-      if (PART > 0) q1 = chunk(t + S + 1, p);
-    };
-    auto refill = [&](auto xi) {
-      constexpr int x = decltype(xi)::value;
-      if constexpr (x < L - PART) issue(std::integral_constant<int, x + PART>{}, q0);
-      else issue(std::integral_constant<int, x - (L - PART)>{}, q1);
-    };
-    // X: fragments of chunk t, Y: of chunk t + 1, read while the first half of chunk t is multiplied; their place is refilled
-    // during the second half
-    auto body = [&](int t, const Frags &x, Frags &y) {
-      if (t + 1 < n) {
-        wait_chunk(n - 2 - t);
+    // X: fragments of chunk t (parity P), Y: of chunk t + 1, read while the first half of chunk t is multiplied; their place is refilled
+    // during the second half with chunk t + 1 + S
+    auto body = [&](int t, auto parity, const Frags &x, Frags &y) {
+      constexpr int P = decltype(parity)::value;
+      if (t + 1 < chunks) {
+        wait_chunk<1 - P>(chunks - 2 - t);
         static_for<0, H>([&](auto m) {
           mfma<m>(c, x);
           // (none beside the last MFMAs: they are waited for behind those)
-          static_for<(m * READS / HR < READS ? m * READS / HR : READS), ((m + 1) * READS / HR < READS ? (m + 1) * READS / HR : READS)>([&](auto r) { read(r, y, pos); });
+          static_for<(m * READS / HR < READS ? m * READS / HR : READS), ((m + 1) * READS / HR < READS ? (m + 1) * READS / HR : READS)>(
+              [&](auto r) { read(r, std::integral_constant<int, 1 - P>{}, y); });
           __builtin_amdgcn_sched_barrier(0);
         });
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        mask_exponents(left_of(t + 1), y);
       } else {
         static_for<0, H>([&](auto m) { mfma<m>(c, x); });
       }
-      if (t + 1 + S < n) {
-        refill_begin(t + 1);
+      if (t + 1 + S < chunks) {
+        const Chunk q = chunk(t + 1 + S, slot, P == 1 ? (pair + S / 2) % PAIRS : (pair + 1 + S / 2) % PAIRS);
+        // (chunk t + 1 is of the pair `pair`)
+        constexpr bool FIRST = ((P + 1 + S) & 1) == 0;
+        if constexpr (FIRST) issue_exponents(q);
         static_for<0, NMFMA - H>([&](auto m) {
           mfma<H + m>(c, x);
-          static_for<m * L / (NMFMA - H), (m + 1) * L / (NMFMA - H)>([&](auto l) { refill(l); });
+          static_for<m * L / (NMFMA - H), (m + 1) * L / (NMFMA - H)>([&](auto l) { issue(l, q); });
           __builtin_amdgcn_sched_barrier(0);
         });
       } else {
         static_for<H, NMFMA>([&](auto m) { mfma<m>(c, x); });
       }
-      advance();
+      slot = slot + 1 == S ? 0 : slot + 1;
+      if constexpr (P == 0) pair ^= 1;   // (chunk t + 2 begins the next pair)
     };
     Frags x, y;
-    wait_chunk(n - 1);
-    static_for<0, READS>([&](auto r) { read(r, x, pos); });
+    constexpr std::integral_constant<int, 0> even;
+    constexpr std::integral_constant<int, 1> odd;
+    wait_chunk<0>(chunks - 1);
+    static_for<0, READS>([&](auto r) { read(r, even, x); });
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (S < n) {
-      refill_begin(0);
-      static_for<0, L>([&](auto l) { refill(l); });
+    mask_exponents(left_of(0), x);
+    if (S < chunks) {
+      const Chunk q = chunk(S, 0, S / 2 % PAIRS);
+      if constexpr (S % 2 == 0) issue_exponents(q);
+      static_for<0, L>([&](auto l) { issue(l, q); });
     }
-    advance();
-    for (int t = 0;;) {
-      body(t, x, y);
-      if (++t == n) break;
-      body(t, y, x);
-      if (++t == n) break;
+    slot = 1;
+    for (int t = 0; t < chunks; t += 2) {
+      body(t, even, x, y);
+      body(t + 1, odd, y, x);
     }
-    wavek_wait_loads<0>();   // the loads past the segment write LDS too
+    wavek_wait_loads<0>();
     Base::template add_waves<RING>(c, acc, smem);
   }
 };
