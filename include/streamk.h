@@ -457,7 +457,7 @@ typedef struct sk_grouped {
                                                      64, int8: 128); 3 to 6: 16 x 64, 32 x 64, 64 x 64, 64 x 128,
                                                      whose waves stream K on their own (SK_LAYOUT_NN: only 64 x 64) */
   int64_t spin_limit;                             /* 0: 2^22 polls; negative: none (to test the way out) */
-  int64_t scale_pitch_a, scale_pitch_b;           /* SK_MXFP4: bytes from row to row of scale_a and scale_b, even, 0: K / 32 */
+  int64_t scales_tiled;                           /* SK_MXFP4: not 0: scale_a and scale_b as sk_tile_mx_scales lays them out */
 } sk_grouped;
 size_t sk_grouped_workspace_bytes(const sk_grouped *g);   /* for this shape and variant, on the current device; 0 is possible */
 int sk_gemm_grouped(const sk_grouped *g, void *ws, size_t ws_bytes, void *stream);
@@ -473,17 +473,19 @@ int sk_grouped_wgrad(const void *A, const void *B, const void *offsets, void *C,
  * byte = floor(log2 max |x|) + 125 of the block, at least 0; each x / 2^(byte - 127) becomes the nearest code (ties to even), at most 6.  A
  * block with an infinity or a NaN has byte 255 and codes 0, so that its products are NaN.
  * sk_dequantize_mxfp4: the values, in SK_F16, SK_BF16 or SK_F32, rounded once where the type has no such number.
- * sk_pad_mx_scales: rows of `blocks` bytes to a pitch (a multiple of 16) with zeros behind them.
+ * sk_tile_mx_scales: two arrays of rows of `blocks` bytes (K / 32) as some tiles read them: 16 bytes for 512 values of a row, those of all rows
+ * together, [ceil(blocks / 16), rows, 16] with zeros behind a row's last.
  *
  * sk_gemm_grouped with dtype SK_MXFP4 multiplies them (SK_LAYOUT_NT): C[r] = activation(A[r] * B[e]^T + bias[e]), C in out_dtype, sums in
- * fp32, rounded once.  scale_a: [R] rows of exponents, scale_b: [E, N] rows, scale_pitch_a and _b bytes apart.  offsets null and E = 1: all
- * rows are the one expert's.  K, lda, ldb and expert_b are multiples of 32 values; a row's exponents are read two at a time: the pitches are even,
- * and where K is no multiple of 64 the byte behind a row's last is read, and must not be 255 (sk_mx_scale_pitch, sk_pad_mx_scales).
+ * fp32, rounded once.  scale_a: [R] rows of K / 32 bytes, scale_b: [E, N] rows, 4-byte aligned; or, with scales_tiled, both tiled, 16-byte
+ * aligned.  sk_mx_scales_tiled says whether a product (its shape and variant, on the current device) is to have them tiled; some refuse others
+ * with SK_ERR_CONFIG.  offsets null and E = 1: all rows are the one expert's.  K, lda, ldb and expert_b are multiples of 32 values.
+ * The bytes of either array's scales tiled stay below 2 GiB.
  */
 int sk_quantize_mxfp4(const void *X, int dtype, int64_t M, int64_t K, int64_t ldx, void *Q, void *scales, void *stream);
 int sk_dequantize_mxfp4(const void *Q, const void *scales, int64_t M, int64_t K, int dtype, void *X, void *stream);
-int64_t sk_mx_scale_pitch(const sk_grouped *g);   /* 0, or the pitch that sk_pad_mx_scales is to give both scales of this product, on the current device */
-int sk_pad_mx_scales(const void *scales, int64_t rows, int64_t blocks, int64_t pitch, void *out, void *stream);
+int sk_tile_mx_scales(const void *a, int64_t rows_a, void *tiled_a, const void *b, int64_t rows_b, void *tiled_b, int64_t blocks, void *stream);
+int sk_mx_scales_tiled(const sk_grouped *g);
 
 /*
  * Routing of tokens to experts.  No counterpart in the reference.

@@ -15,8 +15,6 @@ constexpr int64_t MAX_INT = 0x7fffff00;
 int status_of(int herr) { return herr == 0 ? SK_OK : (herr == (int)hipErrorNotSupported ? SK_ERR_CONFIG : SK_ERR_LAUNCH); }
 }  // namespace
 
-// bytes from one row's exponents to the next row's
-static int64_t mx_pitch(int64_t given, int64_t K) { return given == 0 ? K / 32 : given; }
 // everything but the operands' addresses; fills h
 static int check_shape(const sk_grouped *g, GroupedShape *h) {
   const bool i8 = g->dtype == SK_I8, mx = g->dtype == SK_MXFP4, nn = g->layout == SK_LAYOUT_NN;
@@ -33,12 +31,10 @@ static int check_shape(const sk_grouped *g, GroupedShape *h) {
   const int64_t pairs = mx ? 4 : (i8 ? 2 : 1);   // values in 16 bits
   if (g->lda / pairs * 2 * 256 >= (int64_t)1 << 31 || g->ldb / pairs * 2 * (nn ? g->K + 64 : 256) >= (int64_t)1 << 31 || g->ldc * 2 * 256 >= (int64_t)1 << 31)
     return SK_ERR_SHAPE;
-  if (mx) {
-    // exponents are read two at a time
-    if (mx_pitch(g->scale_pitch_a, g->K) < g->K / 32 || mx_pitch(g->scale_pitch_b, g->K) < g->K / 32) return SK_ERR_SHAPE;
-    if (mx_pitch(g->scale_pitch_a, g->K) * 256 >= (int64_t)1 << 31 || mx_pitch(g->scale_pitch_b, g->K) * 256 >= (int64_t)1 << 31) return SK_ERR_SHAPE;
-    if (mx_pitch(g->scale_pitch_a, g->K) % 2 || mx_pitch(g->scale_pitch_b, g->K) % 2) return SK_ERR_ALIGN;
-  }
+  if (mx && !g->scales_tiled && g->K / 32 * 256 >= (int64_t)1 << 31) return SK_ERR_SHAPE;
+  if (mx && g->scales_tiled && (g->E * g->N > ((int64_t)1 << 27) - 256 || g->R > ((int64_t)1 << 27) - 256 ||
+                                (g->R > g->E * g->N ? g->R : g->E * g->N) * ((g->K + 511) / 512) >= (int64_t)1 << 27))
+    return SK_ERR_SHAPE;   // (offsets from a pair of chunks to another count in 32 bits)
   return SK_OK;
 }
 
@@ -48,13 +44,10 @@ extern "C" size_t sk_grouped_workspace_bytes(const sk_grouped *g) {
   return h.type == GT_MX ? mx_workspace(h) : grouped_workspace(h);
 }
 
-extern "C" int64_t sk_mx_scale_pitch(const sk_grouped *g) {
+extern "C" int sk_mx_scales_tiled(const sk_grouped *g) {
   GroupedShape h;
-  if (!g || g->dtype != SK_MXFP4) return 0;
-  sk_grouped even = *g;   // (whatever the pitches are now)
-  even.scale_pitch_a = even.scale_pitch_b = (g->K / 32 + 15) / 16 * 16;
-  if (check_shape(&even, &h) != SK_OK || sk_device_info(&h.cus, nullptr, nullptr) != SK_OK) return 0;
-  return g->K % mx_scale_step(h) ? even.scale_pitch_a : 0;
+  if (!g || g->dtype != SK_MXFP4 || check_shape(g, &h) != SK_OK || sk_device_info(&h.cus, nullptr, nullptr) != SK_OK) return 0;
+  return mx_wants_tiled(h);
 }
 
 extern "C" int sk_gemm_grouped(const sk_grouped *g, void *ws, size_t ws_bytes, void *stream) {
@@ -65,11 +58,12 @@ extern "C" int sk_gemm_grouped(const sk_grouped *g, void *ws, size_t ws_bytes, v
   GroupedShape h;
   if (int rc = check_shape(g, &h)) return rc;
   if (misaligned(g->A, 15) || misaligned(g->B, 15) || misaligned(g->C, 1) || misaligned(g->bias, 1) || misaligned(g->offsets, 3) ||
-      misaligned(g->scale_a, mx ? 1 : 3) || misaligned(g->scale_b, mx ? 1 : 3))
+      misaligned(g->scale_a, mx && g->scales_tiled ? 15 : 3) || misaligned(g->scale_b, mx && g->scales_tiled ? 15 : 3))
     return SK_ERR_ALIGN;
   if (reinterpret_cast<uintptr_t>(g->bias) >> EPI_ACT_SHIFT) return SK_ERR_CONFIG;   // not a device address
   if (sk_device_info(&h.cus, nullptr, nullptr) != SK_OK) return SK_ERR_DEVICE;
   h.variant = mx ? mx_variant(h) : grouped_variant(h);
+  if (mx && !g->scales_tiled && mx_needs_tiled(h)) return SK_ERR_CONFIG;
   Workspace w;
   if (int rc = take_workspace(ws, ws_bytes, mx ? mx_workspace(h) : grouped_workspace(h), &w)) return rc;
   const int64_t pairs = mx ? 4 : (i8 ? 2 : 1);
@@ -80,10 +74,14 @@ extern "C" int sk_gemm_grouped(const sk_grouped *g, void *ws, size_t ws_bytes, v
   a.offsets = (const int *)g->offsets;
   a.bias = (const half_t *)g->bias;
   if (mx) {
-    a.ea = (const uint8_t *)g->scale_a;
-    a.eb = (const uint8_t *)g->scale_b;
-    a.pitch_a = (int)mx_pitch(g->scale_pitch_a, g->K);
-    a.pitch_b = (int)mx_pitch(g->scale_pitch_b, g->K);
+    // (tiled: 16 bytes for 512 values of a row, all rows of these 512 together)
+    const auto exponents = [&](const void *p, int64_t rows) {
+      const int64_t blocks = g->K / 32, pairs = (g->K + 511) / 512;
+      const uint8_t *at = (const uint8_t *)p;
+      return g->scales_tiled ? MxExponents{at, at + rows * pairs * 16, 16, (int)(rows * 16)} : MxExponents{at, at + rows * blocks, (int)blocks, 16};
+    };
+    a.ea = exponents(g->scale_a, g->R);
+    a.eb = exponents(g->scale_b, g->E * g->N);
   } else {
     a.s = Scales{(const float *)g->scale_a, (const float *)g->scale_b, g->out_dtype == SK_BF16};
   }

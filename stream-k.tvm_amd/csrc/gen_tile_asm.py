@@ -65,12 +65,13 @@ block of the loop is 32 MFMAs with four loads (block 0) and eight (block 1); the
 
 Microscaled 4-bit operands (tile_mx_asm_gen.h, written with the argument `mx`; SK_TILE_ASM_LOOP_MX): the bytes travel as the 16-bit loop's, so that
 an iteration is 256 values of K and a block one v_mfma_scale_f32_16x16x128_f8f6f4 of 128 for each pair of fragments -- as many cycles as the
-16-bit MFMA of 32.  Lane group g takes the 16-byte chunks 2 g (block 0) and 2 g + 1 (block 1) of a row, 32 values each, whose exponents
+16-bit MFMA of 32.  (With 32 x 32 x 64 instead, which a wave alone on its SIMD issues more easily, an iteration takes 1.69 us and not 1.57
+on random operands, where the power drawn sets the clock, and 1.00 and not 1.06 on zeros.)  Lane group g takes the 16-byte chunks 2 g (block 0) and 2 g + 1 (block 1) of a row, 32 values each, whose exponents
 are two neighbouring bytes: one register per 16 rows holds both, and the MFMA picks the block's byte.
   v[88:103] v[104:119]   exponents of the even / odd iterations: A's eight 16-row blocks, then B's
   v122                   what the last iteration of a K that is no multiple of 256 may not load
   v[124:127]             the second chunk's fragment addresses of A and B, the addresses of the exponents
-  s88 s89                where the next exponents go in LDS, how far they are into the rows
+  s[88:90]               where the next exponents go in LDS, their offsets
 Exponents come in pairs of iterations, 16 bytes for each of the 512 rows: 16 KB behind the stages, two pairs of 8 KB.  Each wave fetches
 64 rows of A and 64 of B in block 0 of an even iteration, for the pair behind this one; each block reads eight registers for the next iteration.
 The loop has two iterations in its body.
@@ -368,13 +369,13 @@ def loop_text(nn, low=False, wrap=False):
 
 
 MX_RA1, MX_RB1, MX_RDA, MX_RDB, MX_TAIL = 124, 125, 126, 127, 122
-S_EL, S_EK = 88, 89
+S_EL, S_EKA, S_EKB = 88, 89, 90
 
 
 def loop_text_mx():
     """The 16-bit NT loop on microscaled 4-bit operands; see above.  %[tail]: 0x80000000 in the lanes whose chunk lies behind K in the
-    last iteration, else 0; %[rea], %[reb], %[vea], %[veb], %[ek], %[el]: descriptors, lane offsets, offset in the rows and LDS address (the wave's 64
-    rows) of the exponents behind the first pair's; %[rda], %[rdb]: where the lane reads the first ones."""
+    last iteration, else 0; %[rea], %[reb], %[ve], %[eka], %[ekb], %[esa], %[esb], %[el]: descriptors, lane offset, offsets and LDS address (the
+    wave's 64 rows) of the exponents behind the first pair's, and the steps from pair to pair; %[rda], %[rdb]: where the lane reads the first ones."""
     L = []
     e = L.append
     order = mfma_order()
@@ -411,9 +412,9 @@ def loop_text_mx():
         return groups
 
     def load_exponents():              # of the next pair
-        return [(None, [f'"s_mov_b32 m0, s{S_EL}']), (None, [f'"buffer_load_dwordx4 %[vea], %[rea], s{S_EK} offen lds']),
+        return [(None, [f'"s_mov_b32 m0, s{S_EL}']), (None, [f'"buffer_load_dwordx4 %[ve], %[rea], s{S_EKA} offen lds', f'"s_add_u32 s{S_EKA}, s{S_EKA}, %[esa]']),
                 (None, [f'"s_add_u32 m0, s{S_EL}, 4096', f'"s_xor_b32 s{S_EL}, s{S_EL}, 0x2000']),
-                (None, [f'"buffer_load_dwordx4 %[veb], %[reb], s{S_EK} offen lds', f'"s_add_u32 s{S_EK}, s{S_EK}, 16'])]
+                (None, [f'"buffer_load_dwordx4 %[ve], %[reb], s{S_EKB} offen lds', f'"s_add_u32 s{S_EKB}, s{S_EKB}, %[esb]'])]
 
     def offsets(ahead):                # as offsets_for, with the last iteration's mask
         return [[f'"s_add_u32 s{S_T2}, s{S_IT}, {ahead}', f'"s_cmp_lt_u32 s{S_T2}, %[n]', f'"s_cselect_b32 s{S_OOB}, 0, 0x80000000'],
@@ -443,7 +444,8 @@ def loop_text_mx():
     e(f'"s_add_u32 s{S_KA}, %[ga0], 128')
     e(f'"s_add_u32 s{S_KB}, %[gb0], 128')
     e(f'"s_mov_b32 s{S_EL}, %[el]')
-    e(f'"s_mov_b32 s{S_EK}, %[ek]')
+    e(f'"s_mov_b32 s{S_EKA}, %[eka]')
+    e(f'"s_mov_b32 s{S_EKB}, %[ekb]')
     e(f'"v_xor_b32 v{MX_RA1}, 16, %[ra0]')
     e(f'"v_xor_b32 v{MX_RB1}, 16, %[rb0]')
     e(f'"v_mov_b32 v{MX_RDA}, %[rda]')
@@ -606,7 +608,7 @@ def loop_text_f8():
     return L
 
 
-def store_text(ii0, ii1, scaled):
+def store_text(ii0, ii1, scaled, hint=""):
     """Epilogue for block rows ii0 .. ii1 - 1 of the wave's 128 x 128 result that leaves the two stages alone: lane l
     of block (ii, j) holds row 16 ii + l % 16, columns 16 j + 4 (l / 16) .. + 3 in a[(8 ii + j) 4 .. + 3].  Per block
     row the 32 values become 16 registers of 16-bit pairs (CVT = the packing conversion of C's type, round to nearest
@@ -616,7 +618,8 @@ def store_text(ii0, ii1, scaled):
     %[voff] = its byte offset in the wave's block of C (row l / 16, columns 8 (l % 16) ..), s83 / s84 / s85 / s87 the
     offsets of rows 0-3 / 4-7 / 8-11 / 12-15 of the block row (%[rowstep] = 16 rows of C, %[q1] = 4 rows); rows past M
     lie beyond the descriptor's range and are dropped.  The conversions of block row ii + 1 overlap the trip of block
-    row ii through the patch.  scaled: the fp32 sums are multiplied by %[alpha] first (one-byte operands)."""
+    row ii through the patch.  scaled: the fp32 sums are multiplied by %[alpha] first (one-byte operands).  hint: of the stores; C that does not
+    stay in the L2s leaves them to the operands (microscaled operands, 4096^3: 37.7 us, without 39.3)."""
     L = []
     e = L.append
     SO = (S_T, S_OOB, S_M0, S_T2)     # s83, s84, s85, s87
@@ -640,7 +643,7 @@ def store_text(ii0, ii1, scaled):
 
     def stores(ii):
         for k in range(4):
-            e(f'"buffer_store_dwordx4 v[{out_regs(ii) + 4 * k}:{out_regs(ii) + 4 * k + 3}], %[voff], %[rsc], s{SO[k]} offen')
+            e(f'"buffer_store_dwordx4 v[{out_regs(ii) + 4 * k}:{out_regs(ii) + 4 * k + 3}], %[voff], %[rsc], s{SO[k]} offen{hint}')
         for k in range(4):
             e(f'"s_add_u32 s{SO[k]}, s{SO[k]}, %[rowstep]')
 
@@ -672,7 +675,7 @@ def main_mx():
     print("// Generated by gen_tile_asm.py mx -- do not edit; see that file for the register plan and the schedule.")
     print("#pragma once")
     emit_macro("SK_TILE_ASM_LOOP_MX", "", loop_text_mx())
-    clob = [f'"a{r}"' for r in range(256)] + [f'"v{r}"' for r in range(88, 256)] + [f'"s{r}"' for r in range(80, 90)]
+    clob = [f'"a{r}"' for r in range(256)] + [f'"v{r}"' for r in range(88, 256)] + [f'"s{r}"' for r in range(80, 91)]
     print("#define SK_TILE_ASM_CLOBBERS_MX \\")
     for k in range(0, len(clob), 16):
         print("  " + ", ".join(clob[k:k + 16]) + (", \\" if k + 16 < len(clob) else ""))
@@ -704,6 +707,7 @@ def main():
     for name, (ii0, ii1) in (("ALL", (0, 8)), ("HALF0", (0, 4)), ("HALF1", (4, 8))):
         emit_macro(f"SK_TILE_ASM_STORE_{name}", "(CVT)", store_text(ii0, ii1, False))
         emit_macro(f"SK_TILE_ASM_STORE_{name}_SCALED", "(CVT)", store_text(ii0, ii1, True))
+        emit_macro(f"SK_TILE_ASM_STORE_{name}_NT", "(CVT)", store_text(ii0, ii1, False, " nt"))
     clob = [f'"a{r}"' for r in range(256)] + [f'"v{r}"' for r in range(120, 256)] + [f'"s{r}"' for r in range(80, 88)]
     print("#define SK_TILE_ASM_CLOBBERS \\")
     for k in range(0, len(clob), 16):

@@ -203,8 +203,14 @@ __device__ __forceinline__ void run_grouped(const GroupedArgs &g, int ipt, char 
 struct SkRuns {
   int total, ctas, each, extra;   // iterations, CTAs that have some, of each CTA, CTAs with one more
   // least: iterations of a run, that its fix-up is worth
-  __device__ __forceinline__ SkRuns(int total_, int grid, int least) : total(total_) {
-    ctas = min(grid, max(1, total / least));
+  __device__ __forceinline__ SkRuns(int total_, int grid, int least) : total(total_) { deal(min(grid, max(1, total / least))); }
+  // tiles whole, or cut where that saves more than `cost` iterations
+  __device__ __forceinline__ SkRuns(int tiles, int ipt, int grid, int cost) : total(tiles * ipt) {
+    const int run = (int)((unsigned)(total + grid - 1) / (unsigned)grid);
+    deal(run + cost < ipt ? min(grid, total) : max(1, tiles));
+  }
+  __device__ __forceinline__ void deal(int ctas_) {
+    ctas = ctas_;
     each = (int)((unsigned)total / (unsigned)ctas);
     extra = total - each * ctas;
   }
@@ -224,11 +230,12 @@ __device__ __forceinline__ void zero_unowned(const GroupedArgs &g, int pid, int 
   }
 }
 
-// iterations of a run, that its fix-up is worth (a cut costs about as much as two iterations; policies with longer ones say so)
+// What a cut costs, in iterations, where a policy says so: tiles that are left stay whole, one to a CTA, unless runs are shorter than a tile
+// by more than that.  (0: all are cut, into runs of four iterations at least)
 template <class P, class = void>
-struct least_run { static constexpr int value = 4; };
+struct cut_cost { static constexpr int value = 0; };
 template <class P>
-struct least_run<P, std::void_t<decltype(P::LEAST_RUN)>> { static constexpr int value = P::LEAST_RUN; };
+struct cut_cost<P, std::void_t<decltype(P::CUT_COST)>> { static constexpr int value = P::CUT_COST; };
 // arguments of one product without groups (dense, below): a member of that name
 template <class G, class = void>
 struct is_dense { static constexpr bool value = false; };
@@ -256,9 +263,11 @@ __device__ __forceinline__ void run_grouped_sk(const G &g, int ipt, const Worksp
     P::mac(a, acc, t.pm, t.pn, 0, ipt, smem);
     P::store_c(a, acc, t.pm, t.pn, smem, epi);
   }
-  const SkRuns runs((tiles - whole) * ipt, g.grid, least_run<P>::value);
-  if (pid >= runs.ctas || runs.total == 0) return;
-  int at = runs.start(pid), left = runs.length(pid);
+  const SkRuns runs = cut_cost<P>::value > 0 ? SkRuns(tiles - whole, ipt, g.grid, cut_cost<P>::value) : SkRuns((tiles - whole) * ipt, g.grid, 4);   // (a cut costs about as much as two iterations)
+  // (runs that are fewer than CTAs go to the workgroups that begin first, which stand on all CUs and XCDs)
+  const int run = cut_cost<P>::value == 0 ? pid : ((int)blockIdx.x < runs.ctas ? grouped_pid(runs.ctas) : runs.ctas);
+  if (run >= runs.ctas || runs.total == 0) return;
+  int at = runs.start(run), left = runs.length(run);
   int cut_tile[2] = {-1, -1}, cut_n[2];   // [0]: entered in the middle, [1]: its start is here
   GroupTile cut[2];
   while (left > 0) {
@@ -271,7 +280,7 @@ __device__ __forceinline__ void run_grouped_sk(const G &g, int ipt, const Worksp
     if (n == ipt) {
       P::store_c(a, acc, t.pm, t.pn, smem, epi);
     } else {
-      P::store_partial(acc, slot(pid, k0 == 0));
+      P::store_partial(acc, slot(run, k0 == 0));
       if (k0 == 0) {
         cut_tile[1] = tile;
         cut_n[1] = n;
@@ -290,7 +299,7 @@ __device__ __forceinline__ void run_grouped_sk(const G &g, int ipt, const Worksp
   __syncthreads();
   int *word = reinterpret_cast<int *>(smem);
   if (threadIdx.x == 0)
-    __hip_atomic_fetch_max(ws.status + WS_DIRTY, (int)(((size_t)(2 * pid + 2) * P::TILE_ELEMS * 4 + 255) >> 8), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_fetch_max(ws.status + WS_DIRTY, (int)(((size_t)(2 * run + 2) * P::TILE_ELEMS * 4 + 255) >> 8), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     if (cut_tile[c] < 0) continue;   // (uniform)

@@ -35,7 +35,7 @@ int launch_grouped_wavek(const GroupedArgs &g, const GroupedShape &h, const Work
 struct MxOperands;
 int mx_variant(const GroupedShape &h);
 size_t mx_workspace(const GroupedShape &h);
-int mx_scale_step(const GroupedShape &h);   // K is a multiple of it, or the exponents have to be padded
+bool mx_needs_tiled(const GroupedShape &h), mx_wants_tiled(const GroupedShape &h);   // the exponents' layout (tile_mx.h): that it takes, that it is fast with
 size_t mx_asm_workspace(int cus);           // kernels_mx_asm.hip
 int launch_mx_asm(const MxOperands &g, const GroupedShape &h, bool bf16, const Workspace &ws, hipStream_t s);
 int launch_mx(const MxOperands &g, const GroupedShape &h, bool bf16, const Workspace &ws, hipStream_t s);

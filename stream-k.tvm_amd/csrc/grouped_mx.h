@@ -7,8 +7,7 @@
 namespace sk {
 
 struct MxOperands : GroupedArgs {   // (K, lda, ldb, expert_b in pairs of bytes, four values)
-  const uint8_t *ea, *eb;           // exponents of A's rows [R], of the weights' rows [E, N]
-  int pitch_a, pitch_b;             // bytes from row to row
+  MxExponents ea, eb;               // of A's rows [R], of the weights' rows [E, N]
 };
 template <bool DENSE_>
 struct MxGrouped : MxOperands {
@@ -27,10 +26,8 @@ __device__ __forceinline__ typename P::Args expert_args(const MxGrouped<DENSE> &
   a.K = g.K;
   a.lda = g.lda;
   a.ldc = g.ldc;
-  a.sa = g.ea + (int64_t)lo * g.pitch_a;
-  a.sb = g.eb + (int64_t)e * g.N * g.pitch_b;
-  a.pitch_a = g.pitch_a;
-  a.pitch_b = g.pitch_b;
+  a.ea = g.ea.row(lo);
+  a.eb = g.eb.row((int64_t)e * g.N);
   return a;
 }
 

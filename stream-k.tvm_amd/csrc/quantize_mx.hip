@@ -166,17 +166,43 @@ __global__ __launch_bounds__(THREADS) void dequantize_kernel(const uint32_t *Q, 
   }
 }
 
-// The scales of rows of blocks blocks each, with zeros behind them up to `pitch` (a multiple of 16): the tiles read them 2, 8 or 16 bytes at
-// a time.  A thread has 16 bytes.
-__global__ __launch_bounds__(THREADS) void pad_scales_kernel(const uint8_t *S, int64_t rows, int blocks, int pitch, uint8_t *out) {
-  const int64_t i = wide_block() * THREADS + threadIdx.x, units = pitch / 16, row = i / units;
-  if (row >= rows) return;
-  const int b0 = (int)(i - row * units) * 16;
-  const uint8_t *from = S + row * blocks + b0;
-  union { uint8_t b[16]; uint4v w; } o;
+// Scales as the tiles with many rows read them: 16 bytes for 512 values of a row, those of all rows together, pair by pair of 256 values,
+// with zeros behind the last.  A workgroup turns 64 rows of up to 256 bytes through LDS; two arrays in one launch.
+struct TileScales {
+  const uint8_t *from;
+  uint8_t *to;
+  int64_t rows;
+};
+template <bool VEC>
+__global__ __launch_bounds__(THREADS) void tile_scales_kernel(TileScales a, TileScales b, int64_t blocks_a, int blocks) {
+  __shared__ uint4v part[64][17];   // [row][16 bytes], a column of padding
+  const bool second = (int64_t)blockIdx.x >= blocks_a;
+  const TileScales &t = second ? b : a;
+  const int64_t row0 = ((int64_t)blockIdx.x - (second ? blocks_a : 0)) * 64;
+  const int pieces = (blocks + 15) / 16, p0 = (int)blockIdx.y * 16;
+  for (int i = threadIdx.x; i < 64 * 16; i += THREADS) {
+    const int64_t row = row0 + i / 16;
+    const int p = p0 + i % 16;
+    union { uint8_t c[16]; uint4v w; } o;
+    o.w = uint4v{0, 0, 0, 0};
+    if (row < t.rows && p < pieces) {
+      const uint8_t *from = t.from + row * blocks + 16 * p;
+      if constexpr (VEC) {
+        o.w = *reinterpret_cast<const uint4v *>(from);
+      } else {
 #pragma unroll
-  for (int e = 0; e < 16; ++e) o.b[e] = b0 + e < blocks ? from[e] : 0;
-  *reinterpret_cast<uint4v *>(out + row * pitch + b0) = o.w;
+        for (int e = 0; e < 16; ++e)
+          if (16 * p + e < blocks) o.c[e] = from[e];
+      }
+    }
+    part[i / 16][i % 16] = o.w;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 64 * 16; i += THREADS) {
+    const int64_t row = row0 + i % 64;
+    const int p = p0 + i / 64;
+    if (row < t.rows && p < pieces) *reinterpret_cast<uint4v *>(t.to + (p * t.rows + row) * 16) = part[i % 64][i / 64];
+  }
 }
 
 int element_of(int dtype) { return dtype == SK_F16 ? EL_F16 : (dtype == SK_BF16 ? EL_BF16 : (dtype == SK_F32 ? EL_F32 : -1)); }
@@ -236,12 +262,17 @@ extern "C" int sk_dequantize_mxfp4(const void *Q, const void *scales, int64_t M,
   return hipGetLastError() == hipSuccess ? SK_OK : SK_ERR_LAUNCH;
 }
 
-extern "C" int sk_pad_mx_scales(const void *scales, int64_t rows, int64_t blocks, int64_t pitch, void *out, void *stream) {
-  if (!scales || !out) return SK_ERR_NULL;
-  if (!fits(rows, blocks) || pitch < blocks || pitch > 0x7fffff00) return SK_ERR_SHAPE;
-  if (pitch % 16 || misaligned(out, 15)) return SK_ERR_ALIGN;
-  const int64_t units = rows * (pitch / 16);
-  hipLaunchKernelGGL(pad_scales_kernel, wide_grid((units + THREADS - 1) / THREADS), dim3(THREADS), 0, (hipStream_t)stream, (const uint8_t *)scales, rows,
-                     (int)blocks, (int)pitch, (uint8_t *)out);
+extern "C" int sk_tile_mx_scales(const void *a, int64_t rows_a, void *tiled_a, const void *b, int64_t rows_b, void *tiled_b, int64_t blocks, void *stream) {
+  if (!a || !tiled_a || !b || !tiled_b) return SK_ERR_NULL;
+  if (!fits(rows_a, blocks) || !fits(rows_b, blocks) || rows_a > 0x7fffffff || rows_b > 0x7fffffff || blocks > (1 << 24)) return SK_ERR_SHAPE;
+  if (misaligned(tiled_a, 15) || misaligned(tiled_b, 15)) return SK_ERR_ALIGN;
+  const int64_t blocks_a = (rows_a + 63) / 64, all = blocks_a + (rows_b + 63) / 64;
+  const dim3 grid((unsigned)all, (unsigned)((blocks + 255) / 256));
+  if (grid.y > 65535) return SK_ERR_SHAPE;
+  const TileScales ta{(const uint8_t *)a, (uint8_t *)tiled_a, rows_a}, tb{(const uint8_t *)b, (uint8_t *)tiled_b, rows_b};
+  if (blocks % 16 == 0 && !misaligned(a, 15) && !misaligned(b, 15))
+    hipLaunchKernelGGL((tile_scales_kernel<true>), grid, dim3(THREADS), 0, (hipStream_t)stream, ta, tb, blocks_a, (int)blocks);
+  else
+    hipLaunchKernelGGL((tile_scales_kernel<false>), grid, dim3(THREADS), 0, (hipStream_t)stream, ta, tb, blocks_a, (int)blocks);
   return hipGetLastError() == hipSuccess ? SK_OK : SK_ERR_LAUNCH;
 }

@@ -299,7 +299,11 @@ struct TileF16Asm {
   : : [rsc] "s"(rsrc_c), [voff] "v"(voff), [wr] "v"(wr), [rd] "v"(rd), [rowstep] "s"(rowstep), [q1] "s"(q1),         \
       [alpha] "s"(a.alpha) : "memory", "scc", SK_TILE_ASM_CLOBBERS
 #define SK_ASM_STORE(WHICH)                                                                            \
-  if constexpr (F8 != 0) {                                                                             \
+  if constexpr (MX && BF16_) {                                                                         \
+    asm volatile(SK_TILE_ASM_STORE_##WHICH##_NT("v_cvt_pk_bf16_f32") SK_ASM_STORE_OPERANDS);           \
+  } else if constexpr (MX) {                                                                           \
+    asm volatile(SK_TILE_ASM_STORE_##WHICH##_NT("v_cvt_pk_f16_f32") SK_ASM_STORE_OPERANDS);            \
+  } else if constexpr (F8 != 0) {                                                                      \
     asm volatile(SK_TILE_ASM_STORE_##WHICH##_SCALED("v_cvt_pk_f16_f32") SK_ASM_STORE_OPERANDS);        \
   } else if constexpr (BF16_) {                                                                        \
     asm volatile(SK_TILE_ASM_STORE_##WHICH("v_cvt_pk_bf16_f32") SK_ASM_STORE_OPERANDS);                \

@@ -5227,6 +5227,573 @@
   "s_add_u32 s85, s85, %[rowstep]\n\t" \
   "s_add_u32 s87, s87, %[rowstep]\n\t" \
   ""
+#define SK_TILE_ASM_STORE_ALL_NT(CVT) \
+  "s_mul_i32 s83, %[rowstep], 0\n\t" \
+  "s_add_u32 s84, s83, %[q1]\n\t" \
+  "s_add_u32 s85, s84, %[q1]\n\t" \
+  "s_add_u32 s87, s85, %[q1]\n\t" \
+  "v_accvgpr_read_b32 v128, a0\n\t" \
+  "v_accvgpr_read_b32 v129, a1\n\t" \
+  "v_accvgpr_read_b32 v130, a2\n\t" \
+  "v_accvgpr_read_b32 v131, a3\n\t" \
+  "v_accvgpr_read_b32 v132, a4\n\t" \
+  "v_accvgpr_read_b32 v133, a5\n\t" \
+  "v_accvgpr_read_b32 v134, a6\n\t" \
+  "v_accvgpr_read_b32 v135, a7\n\t" \
+  "v_accvgpr_read_b32 v136, a8\n\t" \
+  "v_accvgpr_read_b32 v137, a9\n\t" \
+  "v_accvgpr_read_b32 v138, a10\n\t" \
+  "v_accvgpr_read_b32 v139, a11\n\t" \
+  "v_accvgpr_read_b32 v140, a12\n\t" \
+  "v_accvgpr_read_b32 v141, a13\n\t" \
+  "v_accvgpr_read_b32 v142, a14\n\t" \
+  "v_accvgpr_read_b32 v143, a15\n\t" \
+  "v_accvgpr_read_b32 v144, a16\n\t" \
+  "v_accvgpr_read_b32 v145, a17\n\t" \
+  "v_accvgpr_read_b32 v146, a18\n\t" \
+  "v_accvgpr_read_b32 v147, a19\n\t" \
+  "v_accvgpr_read_b32 v148, a20\n\t" \
+  "v_accvgpr_read_b32 v149, a21\n\t" \
+  "v_accvgpr_read_b32 v150, a22\n\t" \
+  "v_accvgpr_read_b32 v151, a23\n\t" \
+  "v_accvgpr_read_b32 v152, a24\n\t" \
+  "v_accvgpr_read_b32 v153, a25\n\t" \
+  "v_accvgpr_read_b32 v154, a26\n\t" \
+  "v_accvgpr_read_b32 v155, a27\n\t" \
+  "v_accvgpr_read_b32 v156, a28\n\t" \
+  "v_accvgpr_read_b32 v157, a29\n\t" \
+  "v_accvgpr_read_b32 v158, a30\n\t" \
+  "v_accvgpr_read_b32 v159, a31\n\t" \
+  CVT " v160, v128, v129\n\t" \
+  CVT " v161, v130, v131\n\t" \
+  CVT " v162, v132, v133\n\t" \
+  CVT " v163, v134, v135\n\t" \
+  CVT " v164, v136, v137\n\t" \
+  CVT " v165, v138, v139\n\t" \
+  CVT " v166, v140, v141\n\t" \
+  CVT " v167, v142, v143\n\t" \
+  CVT " v168, v144, v145\n\t" \
+  CVT " v169, v146, v147\n\t" \
+  CVT " v170, v148, v149\n\t" \
+  CVT " v171, v150, v151\n\t" \
+  CVT " v172, v152, v153\n\t" \
+  CVT " v173, v154, v155\n\t" \
+  CVT " v174, v156, v157\n\t" \
+  CVT " v175, v158, v159\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_write_b64 %[wr], v[160:161] offset:0\n\t" \
+  "ds_write_b64 %[wr], v[162:163] offset:32\n\t" \
+  "ds_write_b64 %[wr], v[164:165] offset:64\n\t" \
+  "ds_write_b64 %[wr], v[166:167] offset:96\n\t" \
+  "ds_write_b64 %[wr], v[168:169] offset:128\n\t" \
+  "ds_write_b64 %[wr], v[170:171] offset:160\n\t" \
+  "ds_write_b64 %[wr], v[172:173] offset:192\n\t" \
+  "ds_write_b64 %[wr], v[174:175] offset:224\n\t" \
+  "v_accvgpr_read_b32 v192, a32\n\t" \
+  "v_accvgpr_read_b32 v193, a33\n\t" \
+  "v_accvgpr_read_b32 v194, a34\n\t" \
+  "v_accvgpr_read_b32 v195, a35\n\t" \
+  "v_accvgpr_read_b32 v196, a36\n\t" \
+  "v_accvgpr_read_b32 v197, a37\n\t" \
+  "v_accvgpr_read_b32 v198, a38\n\t" \
+  "v_accvgpr_read_b32 v199, a39\n\t" \
+  "v_accvgpr_read_b32 v200, a40\n\t" \
+  "v_accvgpr_read_b32 v201, a41\n\t" \
+  "v_accvgpr_read_b32 v202, a42\n\t" \
+  "v_accvgpr_read_b32 v203, a43\n\t" \
+  "v_accvgpr_read_b32 v204, a44\n\t" \
+  "v_accvgpr_read_b32 v205, a45\n\t" \
+  "v_accvgpr_read_b32 v206, a46\n\t" \
+  "v_accvgpr_read_b32 v207, a47\n\t" \
+  "v_accvgpr_read_b32 v208, a48\n\t" \
+  "v_accvgpr_read_b32 v209, a49\n\t" \
+  "v_accvgpr_read_b32 v210, a50\n\t" \
+  "v_accvgpr_read_b32 v211, a51\n\t" \
+  "v_accvgpr_read_b32 v212, a52\n\t" \
+  "v_accvgpr_read_b32 v213, a53\n\t" \
+  "v_accvgpr_read_b32 v214, a54\n\t" \
+  "v_accvgpr_read_b32 v215, a55\n\t" \
+  "v_accvgpr_read_b32 v216, a56\n\t" \
+  "v_accvgpr_read_b32 v217, a57\n\t" \
+  "v_accvgpr_read_b32 v218, a58\n\t" \
+  "v_accvgpr_read_b32 v219, a59\n\t" \
+  "v_accvgpr_read_b32 v220, a60\n\t" \
+  "v_accvgpr_read_b32 v221, a61\n\t" \
+  "v_accvgpr_read_b32 v222, a62\n\t" \
+  "v_accvgpr_read_b32 v223, a63\n\t" \
+  CVT " v224, v192, v193\n\t" \
+  CVT " v225, v194, v195\n\t" \
+  CVT " v226, v196, v197\n\t" \
+  CVT " v227, v198, v199\n\t" \
+  CVT " v228, v200, v201\n\t" \
+  CVT " v229, v202, v203\n\t" \
+  CVT " v230, v204, v205\n\t" \
+  CVT " v231, v206, v207\n\t" \
+  CVT " v232, v208, v209\n\t" \
+  CVT " v233, v210, v211\n\t" \
+  CVT " v234, v212, v213\n\t" \
+  CVT " v235, v214, v215\n\t" \
+  CVT " v236, v216, v217\n\t" \
+  CVT " v237, v218, v219\n\t" \
+  CVT " v238, v220, v221\n\t" \
+  CVT " v239, v222, v223\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_read_b128 v[176:179], %[rd] offset:0\n\t" \
+  "ds_read_b128 v[180:183], %[rd] offset:1088\n\t" \
+  "ds_read_b128 v[184:187], %[rd] offset:2176\n\t" \
+  "ds_read_b128 v[188:191], %[rd] offset:3264\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_write_b64 %[wr], v[224:225] offset:0\n\t" \
+  "ds_write_b64 %[wr], v[226:227] offset:32\n\t" \
+  "ds_write_b64 %[wr], v[228:229] offset:64\n\t" \
+  "ds_write_b64 %[wr], v[230:231] offset:96\n\t" \
+  "ds_write_b64 %[wr], v[232:233] offset:128\n\t" \
+  "ds_write_b64 %[wr], v[234:235] offset:160\n\t" \
+  "ds_write_b64 %[wr], v[236:237] offset:192\n\t" \
+  "ds_write_b64 %[wr], v[238:239] offset:224\n\t" \
+  "buffer_store_dwordx4 v[176:179], %[voff], %[rsc], s83 offen nt\n\t" \
+  "buffer_store_dwordx4 v[180:183], %[voff], %[rsc], s84 offen nt\n\t" \
+  "buffer_store_dwordx4 v[184:187], %[voff], %[rsc], s85 offen nt\n\t" \
+  "buffer_store_dwordx4 v[188:191], %[voff], %[rsc], s87 offen nt\n\t" \
+  "s_add_u32 s83, s83, %[rowstep]\n\t" \
+  "s_add_u32 s84, s84, %[rowstep]\n\t" \
+  "s_add_u32 s85, s85, %[rowstep]\n\t" \
+  "s_add_u32 s87, s87, %[rowstep]\n\t" \
+  "v_accvgpr_read_b32 v128, a64\n\t" \
+  "v_accvgpr_read_b32 v129, a65\n\t" \
+  "v_accvgpr_read_b32 v130, a66\n\t" \
+  "v_accvgpr_read_b32 v131, a67\n\t" \
+  "v_accvgpr_read_b32 v132, a68\n\t" \
+  "v_accvgpr_read_b32 v133, a69\n\t" \
+  "v_accvgpr_read_b32 v134, a70\n\t" \
+  "v_accvgpr_read_b32 v135, a71\n\t" \
+  "v_accvgpr_read_b32 v136, a72\n\t" \
+  "v_accvgpr_read_b32 v137, a73\n\t" \
+  "v_accvgpr_read_b32 v138, a74\n\t" \
+  "v_accvgpr_read_b32 v139, a75\n\t" \
+  "v_accvgpr_read_b32 v140, a76\n\t" \
+  "v_accvgpr_read_b32 v141, a77\n\t" \
+  "v_accvgpr_read_b32 v142, a78\n\t" \
+  "v_accvgpr_read_b32 v143, a79\n\t" \
+  "v_accvgpr_read_b32 v144, a80\n\t" \
+  "v_accvgpr_read_b32 v145, a81\n\t" \
+  "v_accvgpr_read_b32 v146, a82\n\t" \
+  "v_accvgpr_read_b32 v147, a83\n\t" \
+  "v_accvgpr_read_b32 v148, a84\n\t" \
+  "v_accvgpr_read_b32 v149, a85\n\t" \
+  "v_accvgpr_read_b32 v150, a86\n\t" \
+  "v_accvgpr_read_b32 v151, a87\n\t" \
+  "v_accvgpr_read_b32 v152, a88\n\t" \
+  "v_accvgpr_read_b32 v153, a89\n\t" \
+  "v_accvgpr_read_b32 v154, a90\n\t" \
+  "v_accvgpr_read_b32 v155, a91\n\t" \
+  "v_accvgpr_read_b32 v156, a92\n\t" \
+  "v_accvgpr_read_b32 v157, a93\n\t" \
+  "v_accvgpr_read_b32 v158, a94\n\t" \
+  "v_accvgpr_read_b32 v159, a95\n\t" \
+  CVT " v160, v128, v129\n\t" \
+  CVT " v161, v130, v131\n\t" \
+  CVT " v162, v132, v133\n\t" \
+  CVT " v163, v134, v135\n\t" \
+  CVT " v164, v136, v137\n\t" \
+  CVT " v165, v138, v139\n\t" \
+  CVT " v166, v140, v141\n\t" \
+  CVT " v167, v142, v143\n\t" \
+  CVT " v168, v144, v145\n\t" \
+  CVT " v169, v146, v147\n\t" \
+  CVT " v170, v148, v149\n\t" \
+  CVT " v171, v150, v151\n\t" \
+  CVT " v172, v152, v153\n\t" \
+  CVT " v173, v154, v155\n\t" \
+  CVT " v174, v156, v157\n\t" \
+  CVT " v175, v158, v159\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_read_b128 v[240:243], %[rd] offset:0\n\t" \
+  "ds_read_b128 v[244:247], %[rd] offset:1088\n\t" \
+  "ds_read_b128 v[248:251], %[rd] offset:2176\n\t" \
+  "ds_read_b128 v[252:255], %[rd] offset:3264\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_write_b64 %[wr], v[160:161] offset:0\n\t" \
+  "ds_write_b64 %[wr], v[162:163] offset:32\n\t" \
+  "ds_write_b64 %[wr], v[164:165] offset:64\n\t" \
+  "ds_write_b64 %[wr], v[166:167] offset:96\n\t" \
+  "ds_write_b64 %[wr], v[168:169] offset:128\n\t" \
+  "ds_write_b64 %[wr], v[170:171] offset:160\n\t" \
+  "ds_write_b64 %[wr], v[172:173] offset:192\n\t" \
+  "ds_write_b64 %[wr], v[174:175] offset:224\n\t" \
+  "buffer_store_dwordx4 v[240:243], %[voff], %[rsc], s83 offen nt\n\t" \
+  "buffer_store_dwordx4 v[244:247], %[voff], %[rsc], s84 offen nt\n\t" \
+  "buffer_store_dwordx4 v[248:251], %[voff], %[rsc], s85 offen nt\n\t" \
+  "buffer_store_dwordx4 v[252:255], %[voff], %[rsc], s87 offen nt\n\t" \
+  "s_add_u32 s83, s83, %[rowstep]\n\t" \
+  "s_add_u32 s84, s84, %[rowstep]\n\t" \
+  "s_add_u32 s85, s85, %[rowstep]\n\t" \
+  "s_add_u32 s87, s87, %[rowstep]\n\t" \
+  "v_accvgpr_read_b32 v192, a96\n\t" \
+  "v_accvgpr_read_b32 v193, a97\n\t" \
+  "v_accvgpr_read_b32 v194, a98\n\t" \
+  "v_accvgpr_read_b32 v195, a99\n\t" \
+  "v_accvgpr_read_b32 v196, a100\n\t" \
+  "v_accvgpr_read_b32 v197, a101\n\t" \
+  "v_accvgpr_read_b32 v198, a102\n\t" \
+  "v_accvgpr_read_b32 v199, a103\n\t" \
+  "v_accvgpr_read_b32 v200, a104\n\t" \
+  "v_accvgpr_read_b32 v201, a105\n\t" \
+  "v_accvgpr_read_b32 v202, a106\n\t" \
+  "v_accvgpr_read_b32 v203, a107\n\t" \
+  "v_accvgpr_read_b32 v204, a108\n\t" \
+  "v_accvgpr_read_b32 v205, a109\n\t" \
+  "v_accvgpr_read_b32 v206, a110\n\t" \
+  "v_accvgpr_read_b32 v207, a111\n\t" \
+  "v_accvgpr_read_b32 v208, a112\n\t" \
+  "v_accvgpr_read_b32 v209, a113\n\t" \
+  "v_accvgpr_read_b32 v210, a114\n\t" \
+  "v_accvgpr_read_b32 v211, a115\n\t" \
+  "v_accvgpr_read_b32 v212, a116\n\t" \
+  "v_accvgpr_read_b32 v213, a117\n\t" \
+  "v_accvgpr_read_b32 v214, a118\n\t" \
+  "v_accvgpr_read_b32 v215, a119\n\t" \
+  "v_accvgpr_read_b32 v216, a120\n\t" \
+  "v_accvgpr_read_b32 v217, a121\n\t" \
+  "v_accvgpr_read_b32 v218, a122\n\t" \
+  "v_accvgpr_read_b32 v219, a123\n\t" \
+  "v_accvgpr_read_b32 v220, a124\n\t" \
+  "v_accvgpr_read_b32 v221, a125\n\t" \
+  "v_accvgpr_read_b32 v222, a126\n\t" \
+  "v_accvgpr_read_b32 v223, a127\n\t" \
+  CVT " v224, v192, v193\n\t" \
+  CVT " v225, v194, v195\n\t" \
+  CVT " v226, v196, v197\n\t" \
+  CVT " v227, v198, v199\n\t" \
+  CVT " v228, v200, v201\n\t" \
+  CVT " v229, v202, v203\n\t" \
+  CVT " v230, v204, v205\n\t" \
+  CVT " v231, v206, v207\n\t" \
+  CVT " v232, v208, v209\n\t" \
+  CVT " v233, v210, v211\n\t" \
+  CVT " v234, v212, v213\n\t" \
+  CVT " v235, v214, v215\n\t" \
+  CVT " v236, v216, v217\n\t" \
+  CVT " v237, v218, v219\n\t" \
+  CVT " v238, v220, v221\n\t" \
+  CVT " v239, v222, v223\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_read_b128 v[176:179], %[rd] offset:0\n\t" \
+  "ds_read_b128 v[180:183], %[rd] offset:1088\n\t" \
+  "ds_read_b128 v[184:187], %[rd] offset:2176\n\t" \
+  "ds_read_b128 v[188:191], %[rd] offset:3264\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_write_b64 %[wr], v[224:225] offset:0\n\t" \
+  "ds_write_b64 %[wr], v[226:227] offset:32\n\t" \
+  "ds_write_b64 %[wr], v[228:229] offset:64\n\t" \
+  "ds_write_b64 %[wr], v[230:231] offset:96\n\t" \
+  "ds_write_b64 %[wr], v[232:233] offset:128\n\t" \
+  "ds_write_b64 %[wr], v[234:235] offset:160\n\t" \
+  "ds_write_b64 %[wr], v[236:237] offset:192\n\t" \
+  "ds_write_b64 %[wr], v[238:239] offset:224\n\t" \
+  "buffer_store_dwordx4 v[176:179], %[voff], %[rsc], s83 offen nt\n\t" \
+  "buffer_store_dwordx4 v[180:183], %[voff], %[rsc], s84 offen nt\n\t" \
+  "buffer_store_dwordx4 v[184:187], %[voff], %[rsc], s85 offen nt\n\t" \
+  "buffer_store_dwordx4 v[188:191], %[voff], %[rsc], s87 offen nt\n\t" \
+  "s_add_u32 s83, s83, %[rowstep]\n\t" \
+  "s_add_u32 s84, s84, %[rowstep]\n\t" \
+  "s_add_u32 s85, s85, %[rowstep]\n\t" \
+  "s_add_u32 s87, s87, %[rowstep]\n\t" \
+  "v_accvgpr_read_b32 v128, a128\n\t" \
+  "v_accvgpr_read_b32 v129, a129\n\t" \
+  "v_accvgpr_read_b32 v130, a130\n\t" \
+  "v_accvgpr_read_b32 v131, a131\n\t" \
+  "v_accvgpr_read_b32 v132, a132\n\t" \
+  "v_accvgpr_read_b32 v133, a133\n\t" \
+  "v_accvgpr_read_b32 v134, a134\n\t" \
+  "v_accvgpr_read_b32 v135, a135\n\t" \
+  "v_accvgpr_read_b32 v136, a136\n\t" \
+  "v_accvgpr_read_b32 v137, a137\n\t" \
+  "v_accvgpr_read_b32 v138, a138\n\t" \
+  "v_accvgpr_read_b32 v139, a139\n\t" \
+  "v_accvgpr_read_b32 v140, a140\n\t" \
+  "v_accvgpr_read_b32 v141, a141\n\t" \
+  "v_accvgpr_read_b32 v142, a142\n\t" \
+  "v_accvgpr_read_b32 v143, a143\n\t" \
+  "v_accvgpr_read_b32 v144, a144\n\t" \
+  "v_accvgpr_read_b32 v145, a145\n\t" \
+  "v_accvgpr_read_b32 v146, a146\n\t" \
+  "v_accvgpr_read_b32 v147, a147\n\t" \
+  "v_accvgpr_read_b32 v148, a148\n\t" \
+  "v_accvgpr_read_b32 v149, a149\n\t" \
+  "v_accvgpr_read_b32 v150, a150\n\t" \
+  "v_accvgpr_read_b32 v151, a151\n\t" \
+  "v_accvgpr_read_b32 v152, a152\n\t" \
+  "v_accvgpr_read_b32 v153, a153\n\t" \
+  "v_accvgpr_read_b32 v154, a154\n\t" \
+  "v_accvgpr_read_b32 v155, a155\n\t" \
+  "v_accvgpr_read_b32 v156, a156\n\t" \
+  "v_accvgpr_read_b32 v157, a157\n\t" \
+  "v_accvgpr_read_b32 v158, a158\n\t" \
+  "v_accvgpr_read_b32 v159, a159\n\t" \
+  CVT " v160, v128, v129\n\t" \
+  CVT " v161, v130, v131\n\t" \
+  CVT " v162, v132, v133\n\t" \
+  CVT " v163, v134, v135\n\t" \
+  CVT " v164, v136, v137\n\t" \
+  CVT " v165, v138, v139\n\t" \
+  CVT " v166, v140, v141\n\t" \
+  CVT " v167, v142, v143\n\t" \
+  CVT " v168, v144, v145\n\t" \
+  CVT " v169, v146, v147\n\t" \
+  CVT " v170, v148, v149\n\t" \
+  CVT " v171, v150, v151\n\t" \
+  CVT " v172, v152, v153\n\t" \
+  CVT " v173, v154, v155\n\t" \
+  CVT " v174, v156, v157\n\t" \
+  CVT " v175, v158, v159\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_read_b128 v[240:243], %[rd] offset:0\n\t" \
+  "ds_read_b128 v[244:247], %[rd] offset:1088\n\t" \
+  "ds_read_b128 v[248:251], %[rd] offset:2176\n\t" \
+  "ds_read_b128 v[252:255], %[rd] offset:3264\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_write_b64 %[wr], v[160:161] offset:0\n\t" \
+  "ds_write_b64 %[wr], v[162:163] offset:32\n\t" \
+  "ds_write_b64 %[wr], v[164:165] offset:64\n\t" \
+  "ds_write_b64 %[wr], v[166:167] offset:96\n\t" \
+  "ds_write_b64 %[wr], v[168:169] offset:128\n\t" \
+  "ds_write_b64 %[wr], v[170:171] offset:160\n\t" \
+  "ds_write_b64 %[wr], v[172:173] offset:192\n\t" \
+  "ds_write_b64 %[wr], v[174:175] offset:224\n\t" \
+  "buffer_store_dwordx4 v[240:243], %[voff], %[rsc], s83 offen nt\n\t" \
+  "buffer_store_dwordx4 v[244:247], %[voff], %[rsc], s84 offen nt\n\t" \
+  "buffer_store_dwordx4 v[248:251], %[voff], %[rsc], s85 offen nt\n\t" \
+  "buffer_store_dwordx4 v[252:255], %[voff], %[rsc], s87 offen nt\n\t" \
+  "s_add_u32 s83, s83, %[rowstep]\n\t" \
+  "s_add_u32 s84, s84, %[rowstep]\n\t" \
+  "s_add_u32 s85, s85, %[rowstep]\n\t" \
+  "s_add_u32 s87, s87, %[rowstep]\n\t" \
+  "v_accvgpr_read_b32 v192, a160\n\t" \
+  "v_accvgpr_read_b32 v193, a161\n\t" \
+  "v_accvgpr_read_b32 v194, a162\n\t" \
+  "v_accvgpr_read_b32 v195, a163\n\t" \
+  "v_accvgpr_read_b32 v196, a164\n\t" \
+  "v_accvgpr_read_b32 v197, a165\n\t" \
+  "v_accvgpr_read_b32 v198, a166\n\t" \
+  "v_accvgpr_read_b32 v199, a167\n\t" \
+  "v_accvgpr_read_b32 v200, a168\n\t" \
+  "v_accvgpr_read_b32 v201, a169\n\t" \
+  "v_accvgpr_read_b32 v202, a170\n\t" \
+  "v_accvgpr_read_b32 v203, a171\n\t" \
+  "v_accvgpr_read_b32 v204, a172\n\t" \
+  "v_accvgpr_read_b32 v205, a173\n\t" \
+  "v_accvgpr_read_b32 v206, a174\n\t" \
+  "v_accvgpr_read_b32 v207, a175\n\t" \
+  "v_accvgpr_read_b32 v208, a176\n\t" \
+  "v_accvgpr_read_b32 v209, a177\n\t" \
+  "v_accvgpr_read_b32 v210, a178\n\t" \
+  "v_accvgpr_read_b32 v211, a179\n\t" \
+  "v_accvgpr_read_b32 v212, a180\n\t" \
+  "v_accvgpr_read_b32 v213, a181\n\t" \
+  "v_accvgpr_read_b32 v214, a182\n\t" \
+  "v_accvgpr_read_b32 v215, a183\n\t" \
+  "v_accvgpr_read_b32 v216, a184\n\t" \
+  "v_accvgpr_read_b32 v217, a185\n\t" \
+  "v_accvgpr_read_b32 v218, a186\n\t" \
+  "v_accvgpr_read_b32 v219, a187\n\t" \
+  "v_accvgpr_read_b32 v220, a188\n\t" \
+  "v_accvgpr_read_b32 v221, a189\n\t" \
+  "v_accvgpr_read_b32 v222, a190\n\t" \
+  "v_accvgpr_read_b32 v223, a191\n\t" \
+  CVT " v224, v192, v193\n\t" \
+  CVT " v225, v194, v195\n\t" \
+  CVT " v226, v196, v197\n\t" \
+  CVT " v227, v198, v199\n\t" \
+  CVT " v228, v200, v201\n\t" \
+  CVT " v229, v202, v203\n\t" \
+  CVT " v230, v204, v205\n\t" \
+  CVT " v231, v206, v207\n\t" \
+  CVT " v232, v208, v209\n\t" \
+  CVT " v233, v210, v211\n\t" \
+  CVT " v234, v212, v213\n\t" \
+  CVT " v235, v214, v215\n\t" \
+  CVT " v236, v216, v217\n\t" \
+  CVT " v237, v218, v219\n\t" \
+  CVT " v238, v220, v221\n\t" \
+  CVT " v239, v222, v223\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_read_b128 v[176:179], %[rd] offset:0\n\t" \
+  "ds_read_b128 v[180:183], %[rd] offset:1088\n\t" \
+  "ds_read_b128 v[184:187], %[rd] offset:2176\n\t" \
+  "ds_read_b128 v[188:191], %[rd] offset:3264\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_write_b64 %[wr], v[224:225] offset:0\n\t" \
+  "ds_write_b64 %[wr], v[226:227] offset:32\n\t" \
+  "ds_write_b64 %[wr], v[228:229] offset:64\n\t" \
+  "ds_write_b64 %[wr], v[230:231] offset:96\n\t" \
+  "ds_write_b64 %[wr], v[232:233] offset:128\n\t" \
+  "ds_write_b64 %[wr], v[234:235] offset:160\n\t" \
+  "ds_write_b64 %[wr], v[236:237] offset:192\n\t" \
+  "ds_write_b64 %[wr], v[238:239] offset:224\n\t" \
+  "buffer_store_dwordx4 v[176:179], %[voff], %[rsc], s83 offen nt\n\t" \
+  "buffer_store_dwordx4 v[180:183], %[voff], %[rsc], s84 offen nt\n\t" \
+  "buffer_store_dwordx4 v[184:187], %[voff], %[rsc], s85 offen nt\n\t" \
+  "buffer_store_dwordx4 v[188:191], %[voff], %[rsc], s87 offen nt\n\t" \
+  "s_add_u32 s83, s83, %[rowstep]\n\t" \
+  "s_add_u32 s84, s84, %[rowstep]\n\t" \
+  "s_add_u32 s85, s85, %[rowstep]\n\t" \
+  "s_add_u32 s87, s87, %[rowstep]\n\t" \
+  "v_accvgpr_read_b32 v128, a192\n\t" \
+  "v_accvgpr_read_b32 v129, a193\n\t" \
+  "v_accvgpr_read_b32 v130, a194\n\t" \
+  "v_accvgpr_read_b32 v131, a195\n\t" \
+  "v_accvgpr_read_b32 v132, a196\n\t" \
+  "v_accvgpr_read_b32 v133, a197\n\t" \
+  "v_accvgpr_read_b32 v134, a198\n\t" \
+  "v_accvgpr_read_b32 v135, a199\n\t" \
+  "v_accvgpr_read_b32 v136, a200\n\t" \
+  "v_accvgpr_read_b32 v137, a201\n\t" \
+  "v_accvgpr_read_b32 v138, a202\n\t" \
+  "v_accvgpr_read_b32 v139, a203\n\t" \
+  "v_accvgpr_read_b32 v140, a204\n\t" \
+  "v_accvgpr_read_b32 v141, a205\n\t" \
+  "v_accvgpr_read_b32 v142, a206\n\t" \
+  "v_accvgpr_read_b32 v143, a207\n\t" \
+  "v_accvgpr_read_b32 v144, a208\n\t" \
+  "v_accvgpr_read_b32 v145, a209\n\t" \
+  "v_accvgpr_read_b32 v146, a210\n\t" \
+  "v_accvgpr_read_b32 v147, a211\n\t" \
+  "v_accvgpr_read_b32 v148, a212\n\t" \
+  "v_accvgpr_read_b32 v149, a213\n\t" \
+  "v_accvgpr_read_b32 v150, a214\n\t" \
+  "v_accvgpr_read_b32 v151, a215\n\t" \
+  "v_accvgpr_read_b32 v152, a216\n\t" \
+  "v_accvgpr_read_b32 v153, a217\n\t" \
+  "v_accvgpr_read_b32 v154, a218\n\t" \
+  "v_accvgpr_read_b32 v155, a219\n\t" \
+  "v_accvgpr_read_b32 v156, a220\n\t" \
+  "v_accvgpr_read_b32 v157, a221\n\t" \
+  "v_accvgpr_read_b32 v158, a222\n\t" \
+  "v_accvgpr_read_b32 v159, a223\n\t" \
+  CVT " v160, v128, v129\n\t" \
+  CVT " v161, v130, v131\n\t" \
+  CVT " v162, v132, v133\n\t" \
+  CVT " v163, v134, v135\n\t" \
+  CVT " v164, v136, v137\n\t" \
+  CVT " v165, v138, v139\n\t" \
+  CVT " v166, v140, v141\n\t" \
+  CVT " v167, v142, v143\n\t" \
+  CVT " v168, v144, v145\n\t" \
+  CVT " v169, v146, v147\n\t" \
+  CVT " v170, v148, v149\n\t" \
+  CVT " v171, v150, v151\n\t" \
+  CVT " v172, v152, v153\n\t" \
+  CVT " v173, v154, v155\n\t" \
+  CVT " v174, v156, v157\n\t" \
+  CVT " v175, v158, v159\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_read_b128 v[240:243], %[rd] offset:0\n\t" \
+  "ds_read_b128 v[244:247], %[rd] offset:1088\n\t" \
+  "ds_read_b128 v[248:251], %[rd] offset:2176\n\t" \
+  "ds_read_b128 v[252:255], %[rd] offset:3264\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_write_b64 %[wr], v[160:161] offset:0\n\t" \
+  "ds_write_b64 %[wr], v[162:163] offset:32\n\t" \
+  "ds_write_b64 %[wr], v[164:165] offset:64\n\t" \
+  "ds_write_b64 %[wr], v[166:167] offset:96\n\t" \
+  "ds_write_b64 %[wr], v[168:169] offset:128\n\t" \
+  "ds_write_b64 %[wr], v[170:171] offset:160\n\t" \
+  "ds_write_b64 %[wr], v[172:173] offset:192\n\t" \
+  "ds_write_b64 %[wr], v[174:175] offset:224\n\t" \
+  "buffer_store_dwordx4 v[240:243], %[voff], %[rsc], s83 offen nt\n\t" \
+  "buffer_store_dwordx4 v[244:247], %[voff], %[rsc], s84 offen nt\n\t" \
+  "buffer_store_dwordx4 v[248:251], %[voff], %[rsc], s85 offen nt\n\t" \
+  "buffer_store_dwordx4 v[252:255], %[voff], %[rsc], s87 offen nt\n\t" \
+  "s_add_u32 s83, s83, %[rowstep]\n\t" \
+  "s_add_u32 s84, s84, %[rowstep]\n\t" \
+  "s_add_u32 s85, s85, %[rowstep]\n\t" \
+  "s_add_u32 s87, s87, %[rowstep]\n\t" \
+  "v_accvgpr_read_b32 v192, a224\n\t" \
+  "v_accvgpr_read_b32 v193, a225\n\t" \
+  "v_accvgpr_read_b32 v194, a226\n\t" \
+  "v_accvgpr_read_b32 v195, a227\n\t" \
+  "v_accvgpr_read_b32 v196, a228\n\t" \
+  "v_accvgpr_read_b32 v197, a229\n\t" \
+  "v_accvgpr_read_b32 v198, a230\n\t" \
+  "v_accvgpr_read_b32 v199, a231\n\t" \
+  "v_accvgpr_read_b32 v200, a232\n\t" \
+  "v_accvgpr_read_b32 v201, a233\n\t" \
+  "v_accvgpr_read_b32 v202, a234\n\t" \
+  "v_accvgpr_read_b32 v203, a235\n\t" \
+  "v_accvgpr_read_b32 v204, a236\n\t" \
+  "v_accvgpr_read_b32 v205, a237\n\t" \
+  "v_accvgpr_read_b32 v206, a238\n\t" \
+  "v_accvgpr_read_b32 v207, a239\n\t" \
+  "v_accvgpr_read_b32 v208, a240\n\t" \
+  "v_accvgpr_read_b32 v209, a241\n\t" \
+  "v_accvgpr_read_b32 v210, a242\n\t" \
+  "v_accvgpr_read_b32 v211, a243\n\t" \
+  "v_accvgpr_read_b32 v212, a244\n\t" \
+  "v_accvgpr_read_b32 v213, a245\n\t" \
+  "v_accvgpr_read_b32 v214, a246\n\t" \
+  "v_accvgpr_read_b32 v215, a247\n\t" \
+  "v_accvgpr_read_b32 v216, a248\n\t" \
+  "v_accvgpr_read_b32 v217, a249\n\t" \
+  "v_accvgpr_read_b32 v218, a250\n\t" \
+  "v_accvgpr_read_b32 v219, a251\n\t" \
+  "v_accvgpr_read_b32 v220, a252\n\t" \
+  "v_accvgpr_read_b32 v221, a253\n\t" \
+  "v_accvgpr_read_b32 v222, a254\n\t" \
+  "v_accvgpr_read_b32 v223, a255\n\t" \
+  CVT " v224, v192, v193\n\t" \
+  CVT " v225, v194, v195\n\t" \
+  CVT " v226, v196, v197\n\t" \
+  CVT " v227, v198, v199\n\t" \
+  CVT " v228, v200, v201\n\t" \
+  CVT " v229, v202, v203\n\t" \
+  CVT " v230, v204, v205\n\t" \
+  CVT " v231, v206, v207\n\t" \
+  CVT " v232, v208, v209\n\t" \
+  CVT " v233, v210, v211\n\t" \
+  CVT " v234, v212, v213\n\t" \
+  CVT " v235, v214, v215\n\t" \
+  CVT " v236, v216, v217\n\t" \
+  CVT " v237, v218, v219\n\t" \
+  CVT " v238, v220, v221\n\t" \
+  CVT " v239, v222, v223\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_read_b128 v[176:179], %[rd] offset:0\n\t" \
+  "ds_read_b128 v[180:183], %[rd] offset:1088\n\t" \
+  "ds_read_b128 v[184:187], %[rd] offset:2176\n\t" \
+  "ds_read_b128 v[188:191], %[rd] offset:3264\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_write_b64 %[wr], v[224:225] offset:0\n\t" \
+  "ds_write_b64 %[wr], v[226:227] offset:32\n\t" \
+  "ds_write_b64 %[wr], v[228:229] offset:64\n\t" \
+  "ds_write_b64 %[wr], v[230:231] offset:96\n\t" \
+  "ds_write_b64 %[wr], v[232:233] offset:128\n\t" \
+  "ds_write_b64 %[wr], v[234:235] offset:160\n\t" \
+  "ds_write_b64 %[wr], v[236:237] offset:192\n\t" \
+  "ds_write_b64 %[wr], v[238:239] offset:224\n\t" \
+  "buffer_store_dwordx4 v[176:179], %[voff], %[rsc], s83 offen nt\n\t" \
+  "buffer_store_dwordx4 v[180:183], %[voff], %[rsc], s84 offen nt\n\t" \
+  "buffer_store_dwordx4 v[184:187], %[voff], %[rsc], s85 offen nt\n\t" \
+  "buffer_store_dwordx4 v[188:191], %[voff], %[rsc], s87 offen nt\n\t" \
+  "s_add_u32 s83, s83, %[rowstep]\n\t" \
+  "s_add_u32 s84, s84, %[rowstep]\n\t" \
+  "s_add_u32 s85, s85, %[rowstep]\n\t" \
+  "s_add_u32 s87, s87, %[rowstep]\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_read_b128 v[240:243], %[rd] offset:0\n\t" \
+  "ds_read_b128 v[244:247], %[rd] offset:1088\n\t" \
+  "ds_read_b128 v[248:251], %[rd] offset:2176\n\t" \
+  "ds_read_b128 v[252:255], %[rd] offset:3264\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "buffer_store_dwordx4 v[240:243], %[voff], %[rsc], s83 offen nt\n\t" \
+  "buffer_store_dwordx4 v[244:247], %[voff], %[rsc], s84 offen nt\n\t" \
+  "buffer_store_dwordx4 v[248:251], %[voff], %[rsc], s85 offen nt\n\t" \
+  "buffer_store_dwordx4 v[252:255], %[voff], %[rsc], s87 offen nt\n\t" \
+  "s_add_u32 s83, s83, %[rowstep]\n\t" \
+  "s_add_u32 s84, s84, %[rowstep]\n\t" \
+  "s_add_u32 s85, s85, %[rowstep]\n\t" \
+  "s_add_u32 s87, s87, %[rowstep]\n\t" \
+  ""
 #define SK_TILE_ASM_STORE_HALF0(CVT) \
   "s_mul_i32 s83, %[rowstep], 0\n\t" \
   "s_add_u32 s84, s83, %[q1]\n\t" \
@@ -5929,6 +6496,293 @@
   "s_add_u32 s85, s85, %[rowstep]\n\t" \
   "s_add_u32 s87, s87, %[rowstep]\n\t" \
   ""
+#define SK_TILE_ASM_STORE_HALF0_NT(CVT) \
+  "s_mul_i32 s83, %[rowstep], 0\n\t" \
+  "s_add_u32 s84, s83, %[q1]\n\t" \
+  "s_add_u32 s85, s84, %[q1]\n\t" \
+  "s_add_u32 s87, s85, %[q1]\n\t" \
+  "v_accvgpr_read_b32 v128, a0\n\t" \
+  "v_accvgpr_read_b32 v129, a1\n\t" \
+  "v_accvgpr_read_b32 v130, a2\n\t" \
+  "v_accvgpr_read_b32 v131, a3\n\t" \
+  "v_accvgpr_read_b32 v132, a4\n\t" \
+  "v_accvgpr_read_b32 v133, a5\n\t" \
+  "v_accvgpr_read_b32 v134, a6\n\t" \
+  "v_accvgpr_read_b32 v135, a7\n\t" \
+  "v_accvgpr_read_b32 v136, a8\n\t" \
+  "v_accvgpr_read_b32 v137, a9\n\t" \
+  "v_accvgpr_read_b32 v138, a10\n\t" \
+  "v_accvgpr_read_b32 v139, a11\n\t" \
+  "v_accvgpr_read_b32 v140, a12\n\t" \
+  "v_accvgpr_read_b32 v141, a13\n\t" \
+  "v_accvgpr_read_b32 v142, a14\n\t" \
+  "v_accvgpr_read_b32 v143, a15\n\t" \
+  "v_accvgpr_read_b32 v144, a16\n\t" \
+  "v_accvgpr_read_b32 v145, a17\n\t" \
+  "v_accvgpr_read_b32 v146, a18\n\t" \
+  "v_accvgpr_read_b32 v147, a19\n\t" \
+  "v_accvgpr_read_b32 v148, a20\n\t" \
+  "v_accvgpr_read_b32 v149, a21\n\t" \
+  "v_accvgpr_read_b32 v150, a22\n\t" \
+  "v_accvgpr_read_b32 v151, a23\n\t" \
+  "v_accvgpr_read_b32 v152, a24\n\t" \
+  "v_accvgpr_read_b32 v153, a25\n\t" \
+  "v_accvgpr_read_b32 v154, a26\n\t" \
+  "v_accvgpr_read_b32 v155, a27\n\t" \
+  "v_accvgpr_read_b32 v156, a28\n\t" \
+  "v_accvgpr_read_b32 v157, a29\n\t" \
+  "v_accvgpr_read_b32 v158, a30\n\t" \
+  "v_accvgpr_read_b32 v159, a31\n\t" \
+  CVT " v160, v128, v129\n\t" \
+  CVT " v161, v130, v131\n\t" \
+  CVT " v162, v132, v133\n\t" \
+  CVT " v163, v134, v135\n\t" \
+  CVT " v164, v136, v137\n\t" \
+  CVT " v165, v138, v139\n\t" \
+  CVT " v166, v140, v141\n\t" \
+  CVT " v167, v142, v143\n\t" \
+  CVT " v168, v144, v145\n\t" \
+  CVT " v169, v146, v147\n\t" \
+  CVT " v170, v148, v149\n\t" \
+  CVT " v171, v150, v151\n\t" \
+  CVT " v172, v152, v153\n\t" \
+  CVT " v173, v154, v155\n\t" \
+  CVT " v174, v156, v157\n\t" \
+  CVT " v175, v158, v159\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_write_b64 %[wr], v[160:161] offset:0\n\t" \
+  "ds_write_b64 %[wr], v[162:163] offset:32\n\t" \
+  "ds_write_b64 %[wr], v[164:165] offset:64\n\t" \
+  "ds_write_b64 %[wr], v[166:167] offset:96\n\t" \
+  "ds_write_b64 %[wr], v[168:169] offset:128\n\t" \
+  "ds_write_b64 %[wr], v[170:171] offset:160\n\t" \
+  "ds_write_b64 %[wr], v[172:173] offset:192\n\t" \
+  "ds_write_b64 %[wr], v[174:175] offset:224\n\t" \
+  "v_accvgpr_read_b32 v192, a32\n\t" \
+  "v_accvgpr_read_b32 v193, a33\n\t" \
+  "v_accvgpr_read_b32 v194, a34\n\t" \
+  "v_accvgpr_read_b32 v195, a35\n\t" \
+  "v_accvgpr_read_b32 v196, a36\n\t" \
+  "v_accvgpr_read_b32 v197, a37\n\t" \
+  "v_accvgpr_read_b32 v198, a38\n\t" \
+  "v_accvgpr_read_b32 v199, a39\n\t" \
+  "v_accvgpr_read_b32 v200, a40\n\t" \
+  "v_accvgpr_read_b32 v201, a41\n\t" \
+  "v_accvgpr_read_b32 v202, a42\n\t" \
+  "v_accvgpr_read_b32 v203, a43\n\t" \
+  "v_accvgpr_read_b32 v204, a44\n\t" \
+  "v_accvgpr_read_b32 v205, a45\n\t" \
+  "v_accvgpr_read_b32 v206, a46\n\t" \
+  "v_accvgpr_read_b32 v207, a47\n\t" \
+  "v_accvgpr_read_b32 v208, a48\n\t" \
+  "v_accvgpr_read_b32 v209, a49\n\t" \
+  "v_accvgpr_read_b32 v210, a50\n\t" \
+  "v_accvgpr_read_b32 v211, a51\n\t" \
+  "v_accvgpr_read_b32 v212, a52\n\t" \
+  "v_accvgpr_read_b32 v213, a53\n\t" \
+  "v_accvgpr_read_b32 v214, a54\n\t" \
+  "v_accvgpr_read_b32 v215, a55\n\t" \
+  "v_accvgpr_read_b32 v216, a56\n\t" \
+  "v_accvgpr_read_b32 v217, a57\n\t" \
+  "v_accvgpr_read_b32 v218, a58\n\t" \
+  "v_accvgpr_read_b32 v219, a59\n\t" \
+  "v_accvgpr_read_b32 v220, a60\n\t" \
+  "v_accvgpr_read_b32 v221, a61\n\t" \
+  "v_accvgpr_read_b32 v222, a62\n\t" \
+  "v_accvgpr_read_b32 v223, a63\n\t" \
+  CVT " v224, v192, v193\n\t" \
+  CVT " v225, v194, v195\n\t" \
+  CVT " v226, v196, v197\n\t" \
+  CVT " v227, v198, v199\n\t" \
+  CVT " v228, v200, v201\n\t" \
+  CVT " v229, v202, v203\n\t" \
+  CVT " v230, v204, v205\n\t" \
+  CVT " v231, v206, v207\n\t" \
+  CVT " v232, v208, v209\n\t" \
+  CVT " v233, v210, v211\n\t" \
+  CVT " v234, v212, v213\n\t" \
+  CVT " v235, v214, v215\n\t" \
+  CVT " v236, v216, v217\n\t" \
+  CVT " v237, v218, v219\n\t" \
+  CVT " v238, v220, v221\n\t" \
+  CVT " v239, v222, v223\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_read_b128 v[176:179], %[rd] offset:0\n\t" \
+  "ds_read_b128 v[180:183], %[rd] offset:1088\n\t" \
+  "ds_read_b128 v[184:187], %[rd] offset:2176\n\t" \
+  "ds_read_b128 v[188:191], %[rd] offset:3264\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_write_b64 %[wr], v[224:225] offset:0\n\t" \
+  "ds_write_b64 %[wr], v[226:227] offset:32\n\t" \
+  "ds_write_b64 %[wr], v[228:229] offset:64\n\t" \
+  "ds_write_b64 %[wr], v[230:231] offset:96\n\t" \
+  "ds_write_b64 %[wr], v[232:233] offset:128\n\t" \
+  "ds_write_b64 %[wr], v[234:235] offset:160\n\t" \
+  "ds_write_b64 %[wr], v[236:237] offset:192\n\t" \
+  "ds_write_b64 %[wr], v[238:239] offset:224\n\t" \
+  "buffer_store_dwordx4 v[176:179], %[voff], %[rsc], s83 offen nt\n\t" \
+  "buffer_store_dwordx4 v[180:183], %[voff], %[rsc], s84 offen nt\n\t" \
+  "buffer_store_dwordx4 v[184:187], %[voff], %[rsc], s85 offen nt\n\t" \
+  "buffer_store_dwordx4 v[188:191], %[voff], %[rsc], s87 offen nt\n\t" \
+  "s_add_u32 s83, s83, %[rowstep]\n\t" \
+  "s_add_u32 s84, s84, %[rowstep]\n\t" \
+  "s_add_u32 s85, s85, %[rowstep]\n\t" \
+  "s_add_u32 s87, s87, %[rowstep]\n\t" \
+  "v_accvgpr_read_b32 v128, a64\n\t" \
+  "v_accvgpr_read_b32 v129, a65\n\t" \
+  "v_accvgpr_read_b32 v130, a66\n\t" \
+  "v_accvgpr_read_b32 v131, a67\n\t" \
+  "v_accvgpr_read_b32 v132, a68\n\t" \
+  "v_accvgpr_read_b32 v133, a69\n\t" \
+  "v_accvgpr_read_b32 v134, a70\n\t" \
+  "v_accvgpr_read_b32 v135, a71\n\t" \
+  "v_accvgpr_read_b32 v136, a72\n\t" \
+  "v_accvgpr_read_b32 v137, a73\n\t" \
+  "v_accvgpr_read_b32 v138, a74\n\t" \
+  "v_accvgpr_read_b32 v139, a75\n\t" \
+  "v_accvgpr_read_b32 v140, a76\n\t" \
+  "v_accvgpr_read_b32 v141, a77\n\t" \
+  "v_accvgpr_read_b32 v142, a78\n\t" \
+  "v_accvgpr_read_b32 v143, a79\n\t" \
+  "v_accvgpr_read_b32 v144, a80\n\t" \
+  "v_accvgpr_read_b32 v145, a81\n\t" \
+  "v_accvgpr_read_b32 v146, a82\n\t" \
+  "v_accvgpr_read_b32 v147, a83\n\t" \
+  "v_accvgpr_read_b32 v148, a84\n\t" \
+  "v_accvgpr_read_b32 v149, a85\n\t" \
+  "v_accvgpr_read_b32 v150, a86\n\t" \
+  "v_accvgpr_read_b32 v151, a87\n\t" \
+  "v_accvgpr_read_b32 v152, a88\n\t" \
+  "v_accvgpr_read_b32 v153, a89\n\t" \
+  "v_accvgpr_read_b32 v154, a90\n\t" \
+  "v_accvgpr_read_b32 v155, a91\n\t" \
+  "v_accvgpr_read_b32 v156, a92\n\t" \
+  "v_accvgpr_read_b32 v157, a93\n\t" \
+  "v_accvgpr_read_b32 v158, a94\n\t" \
+  "v_accvgpr_read_b32 v159, a95\n\t" \
+  CVT " v160, v128, v129\n\t" \
+  CVT " v161, v130, v131\n\t" \
+  CVT " v162, v132, v133\n\t" \
+  CVT " v163, v134, v135\n\t" \
+  CVT " v164, v136, v137\n\t" \
+  CVT " v165, v138, v139\n\t" \
+  CVT " v166, v140, v141\n\t" \
+  CVT " v167, v142, v143\n\t" \
+  CVT " v168, v144, v145\n\t" \
+  CVT " v169, v146, v147\n\t" \
+  CVT " v170, v148, v149\n\t" \
+  CVT " v171, v150, v151\n\t" \
+  CVT " v172, v152, v153\n\t" \
+  CVT " v173, v154, v155\n\t" \
+  CVT " v174, v156, v157\n\t" \
+  CVT " v175, v158, v159\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_read_b128 v[240:243], %[rd] offset:0\n\t" \
+  "ds_read_b128 v[244:247], %[rd] offset:1088\n\t" \
+  "ds_read_b128 v[248:251], %[rd] offset:2176\n\t" \
+  "ds_read_b128 v[252:255], %[rd] offset:3264\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_write_b64 %[wr], v[160:161] offset:0\n\t" \
+  "ds_write_b64 %[wr], v[162:163] offset:32\n\t" \
+  "ds_write_b64 %[wr], v[164:165] offset:64\n\t" \
+  "ds_write_b64 %[wr], v[166:167] offset:96\n\t" \
+  "ds_write_b64 %[wr], v[168:169] offset:128\n\t" \
+  "ds_write_b64 %[wr], v[170:171] offset:160\n\t" \
+  "ds_write_b64 %[wr], v[172:173] offset:192\n\t" \
+  "ds_write_b64 %[wr], v[174:175] offset:224\n\t" \
+  "buffer_store_dwordx4 v[240:243], %[voff], %[rsc], s83 offen nt\n\t" \
+  "buffer_store_dwordx4 v[244:247], %[voff], %[rsc], s84 offen nt\n\t" \
+  "buffer_store_dwordx4 v[248:251], %[voff], %[rsc], s85 offen nt\n\t" \
+  "buffer_store_dwordx4 v[252:255], %[voff], %[rsc], s87 offen nt\n\t" \
+  "s_add_u32 s83, s83, %[rowstep]\n\t" \
+  "s_add_u32 s84, s84, %[rowstep]\n\t" \
+  "s_add_u32 s85, s85, %[rowstep]\n\t" \
+  "s_add_u32 s87, s87, %[rowstep]\n\t" \
+  "v_accvgpr_read_b32 v192, a96\n\t" \
+  "v_accvgpr_read_b32 v193, a97\n\t" \
+  "v_accvgpr_read_b32 v194, a98\n\t" \
+  "v_accvgpr_read_b32 v195, a99\n\t" \
+  "v_accvgpr_read_b32 v196, a100\n\t" \
+  "v_accvgpr_read_b32 v197, a101\n\t" \
+  "v_accvgpr_read_b32 v198, a102\n\t" \
+  "v_accvgpr_read_b32 v199, a103\n\t" \
+  "v_accvgpr_read_b32 v200, a104\n\t" \
+  "v_accvgpr_read_b32 v201, a105\n\t" \
+  "v_accvgpr_read_b32 v202, a106\n\t" \
+  "v_accvgpr_read_b32 v203, a107\n\t" \
+  "v_accvgpr_read_b32 v204, a108\n\t" \
+  "v_accvgpr_read_b32 v205, a109\n\t" \
+  "v_accvgpr_read_b32 v206, a110\n\t" \
+  "v_accvgpr_read_b32 v207, a111\n\t" \
+  "v_accvgpr_read_b32 v208, a112\n\t" \
+  "v_accvgpr_read_b32 v209, a113\n\t" \
+  "v_accvgpr_read_b32 v210, a114\n\t" \
+  "v_accvgpr_read_b32 v211, a115\n\t" \
+  "v_accvgpr_read_b32 v212, a116\n\t" \
+  "v_accvgpr_read_b32 v213, a117\n\t" \
+  "v_accvgpr_read_b32 v214, a118\n\t" \
+  "v_accvgpr_read_b32 v215, a119\n\t" \
+  "v_accvgpr_read_b32 v216, a120\n\t" \
+  "v_accvgpr_read_b32 v217, a121\n\t" \
+  "v_accvgpr_read_b32 v218, a122\n\t" \
+  "v_accvgpr_read_b32 v219, a123\n\t" \
+  "v_accvgpr_read_b32 v220, a124\n\t" \
+  "v_accvgpr_read_b32 v221, a125\n\t" \
+  "v_accvgpr_read_b32 v222, a126\n\t" \
+  "v_accvgpr_read_b32 v223, a127\n\t" \
+  CVT " v224, v192, v193\n\t" \
+  CVT " v225, v194, v195\n\t" \
+  CVT " v226, v196, v197\n\t" \
+  CVT " v227, v198, v199\n\t" \
+  CVT " v228, v200, v201\n\t" \
+  CVT " v229, v202, v203\n\t" \
+  CVT " v230, v204, v205\n\t" \
+  CVT " v231, v206, v207\n\t" \
+  CVT " v232, v208, v209\n\t" \
+  CVT " v233, v210, v211\n\t" \
+  CVT " v234, v212, v213\n\t" \
+  CVT " v235, v214, v215\n\t" \
+  CVT " v236, v216, v217\n\t" \
+  CVT " v237, v218, v219\n\t" \
+  CVT " v238, v220, v221\n\t" \
+  CVT " v239, v222, v223\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_read_b128 v[176:179], %[rd] offset:0\n\t" \
+  "ds_read_b128 v[180:183], %[rd] offset:1088\n\t" \
+  "ds_read_b128 v[184:187], %[rd] offset:2176\n\t" \
+  "ds_read_b128 v[188:191], %[rd] offset:3264\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_write_b64 %[wr], v[224:225] offset:0\n\t" \
+  "ds_write_b64 %[wr], v[226:227] offset:32\n\t" \
+  "ds_write_b64 %[wr], v[228:229] offset:64\n\t" \
+  "ds_write_b64 %[wr], v[230:231] offset:96\n\t" \
+  "ds_write_b64 %[wr], v[232:233] offset:128\n\t" \
+  "ds_write_b64 %[wr], v[234:235] offset:160\n\t" \
+  "ds_write_b64 %[wr], v[236:237] offset:192\n\t" \
+  "ds_write_b64 %[wr], v[238:239] offset:224\n\t" \
+  "buffer_store_dwordx4 v[176:179], %[voff], %[rsc], s83 offen nt\n\t" \
+  "buffer_store_dwordx4 v[180:183], %[voff], %[rsc], s84 offen nt\n\t" \
+  "buffer_store_dwordx4 v[184:187], %[voff], %[rsc], s85 offen nt\n\t" \
+  "buffer_store_dwordx4 v[188:191], %[voff], %[rsc], s87 offen nt\n\t" \
+  "s_add_u32 s83, s83, %[rowstep]\n\t" \
+  "s_add_u32 s84, s84, %[rowstep]\n\t" \
+  "s_add_u32 s85, s85, %[rowstep]\n\t" \
+  "s_add_u32 s87, s87, %[rowstep]\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_read_b128 v[240:243], %[rd] offset:0\n\t" \
+  "ds_read_b128 v[244:247], %[rd] offset:1088\n\t" \
+  "ds_read_b128 v[248:251], %[rd] offset:2176\n\t" \
+  "ds_read_b128 v[252:255], %[rd] offset:3264\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "buffer_store_dwordx4 v[240:243], %[voff], %[rsc], s83 offen nt\n\t" \
+  "buffer_store_dwordx4 v[244:247], %[voff], %[rsc], s84 offen nt\n\t" \
+  "buffer_store_dwordx4 v[248:251], %[voff], %[rsc], s85 offen nt\n\t" \
+  "buffer_store_dwordx4 v[252:255], %[voff], %[rsc], s87 offen nt\n\t" \
+  "s_add_u32 s83, s83, %[rowstep]\n\t" \
+  "s_add_u32 s84, s84, %[rowstep]\n\t" \
+  "s_add_u32 s85, s85, %[rowstep]\n\t" \
+  "s_add_u32 s87, s87, %[rowstep]\n\t" \
+  ""
 #define SK_TILE_ASM_STORE_HALF1(CVT) \
   "s_mul_i32 s83, %[rowstep], 4\n\t" \
   "s_add_u32 s84, s83, %[q1]\n\t" \
@@ -6626,6 +7480,293 @@
   "buffer_store_dwordx4 v[244:247], %[voff], %[rsc], s84 offen\n\t" \
   "buffer_store_dwordx4 v[248:251], %[voff], %[rsc], s85 offen\n\t" \
   "buffer_store_dwordx4 v[252:255], %[voff], %[rsc], s87 offen\n\t" \
+  "s_add_u32 s83, s83, %[rowstep]\n\t" \
+  "s_add_u32 s84, s84, %[rowstep]\n\t" \
+  "s_add_u32 s85, s85, %[rowstep]\n\t" \
+  "s_add_u32 s87, s87, %[rowstep]\n\t" \
+  ""
+#define SK_TILE_ASM_STORE_HALF1_NT(CVT) \
+  "s_mul_i32 s83, %[rowstep], 4\n\t" \
+  "s_add_u32 s84, s83, %[q1]\n\t" \
+  "s_add_u32 s85, s84, %[q1]\n\t" \
+  "s_add_u32 s87, s85, %[q1]\n\t" \
+  "v_accvgpr_read_b32 v128, a128\n\t" \
+  "v_accvgpr_read_b32 v129, a129\n\t" \
+  "v_accvgpr_read_b32 v130, a130\n\t" \
+  "v_accvgpr_read_b32 v131, a131\n\t" \
+  "v_accvgpr_read_b32 v132, a132\n\t" \
+  "v_accvgpr_read_b32 v133, a133\n\t" \
+  "v_accvgpr_read_b32 v134, a134\n\t" \
+  "v_accvgpr_read_b32 v135, a135\n\t" \
+  "v_accvgpr_read_b32 v136, a136\n\t" \
+  "v_accvgpr_read_b32 v137, a137\n\t" \
+  "v_accvgpr_read_b32 v138, a138\n\t" \
+  "v_accvgpr_read_b32 v139, a139\n\t" \
+  "v_accvgpr_read_b32 v140, a140\n\t" \
+  "v_accvgpr_read_b32 v141, a141\n\t" \
+  "v_accvgpr_read_b32 v142, a142\n\t" \
+  "v_accvgpr_read_b32 v143, a143\n\t" \
+  "v_accvgpr_read_b32 v144, a144\n\t" \
+  "v_accvgpr_read_b32 v145, a145\n\t" \
+  "v_accvgpr_read_b32 v146, a146\n\t" \
+  "v_accvgpr_read_b32 v147, a147\n\t" \
+  "v_accvgpr_read_b32 v148, a148\n\t" \
+  "v_accvgpr_read_b32 v149, a149\n\t" \
+  "v_accvgpr_read_b32 v150, a150\n\t" \
+  "v_accvgpr_read_b32 v151, a151\n\t" \
+  "v_accvgpr_read_b32 v152, a152\n\t" \
+  "v_accvgpr_read_b32 v153, a153\n\t" \
+  "v_accvgpr_read_b32 v154, a154\n\t" \
+  "v_accvgpr_read_b32 v155, a155\n\t" \
+  "v_accvgpr_read_b32 v156, a156\n\t" \
+  "v_accvgpr_read_b32 v157, a157\n\t" \
+  "v_accvgpr_read_b32 v158, a158\n\t" \
+  "v_accvgpr_read_b32 v159, a159\n\t" \
+  CVT " v160, v128, v129\n\t" \
+  CVT " v161, v130, v131\n\t" \
+  CVT " v162, v132, v133\n\t" \
+  CVT " v163, v134, v135\n\t" \
+  CVT " v164, v136, v137\n\t" \
+  CVT " v165, v138, v139\n\t" \
+  CVT " v166, v140, v141\n\t" \
+  CVT " v167, v142, v143\n\t" \
+  CVT " v168, v144, v145\n\t" \
+  CVT " v169, v146, v147\n\t" \
+  CVT " v170, v148, v149\n\t" \
+  CVT " v171, v150, v151\n\t" \
+  CVT " v172, v152, v153\n\t" \
+  CVT " v173, v154, v155\n\t" \
+  CVT " v174, v156, v157\n\t" \
+  CVT " v175, v158, v159\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_write_b64 %[wr], v[160:161] offset:0\n\t" \
+  "ds_write_b64 %[wr], v[162:163] offset:32\n\t" \
+  "ds_write_b64 %[wr], v[164:165] offset:64\n\t" \
+  "ds_write_b64 %[wr], v[166:167] offset:96\n\t" \
+  "ds_write_b64 %[wr], v[168:169] offset:128\n\t" \
+  "ds_write_b64 %[wr], v[170:171] offset:160\n\t" \
+  "ds_write_b64 %[wr], v[172:173] offset:192\n\t" \
+  "ds_write_b64 %[wr], v[174:175] offset:224\n\t" \
+  "v_accvgpr_read_b32 v192, a160\n\t" \
+  "v_accvgpr_read_b32 v193, a161\n\t" \
+  "v_accvgpr_read_b32 v194, a162\n\t" \
+  "v_accvgpr_read_b32 v195, a163\n\t" \
+  "v_accvgpr_read_b32 v196, a164\n\t" \
+  "v_accvgpr_read_b32 v197, a165\n\t" \
+  "v_accvgpr_read_b32 v198, a166\n\t" \
+  "v_accvgpr_read_b32 v199, a167\n\t" \
+  "v_accvgpr_read_b32 v200, a168\n\t" \
+  "v_accvgpr_read_b32 v201, a169\n\t" \
+  "v_accvgpr_read_b32 v202, a170\n\t" \
+  "v_accvgpr_read_b32 v203, a171\n\t" \
+  "v_accvgpr_read_b32 v204, a172\n\t" \
+  "v_accvgpr_read_b32 v205, a173\n\t" \
+  "v_accvgpr_read_b32 v206, a174\n\t" \
+  "v_accvgpr_read_b32 v207, a175\n\t" \
+  "v_accvgpr_read_b32 v208, a176\n\t" \
+  "v_accvgpr_read_b32 v209, a177\n\t" \
+  "v_accvgpr_read_b32 v210, a178\n\t" \
+  "v_accvgpr_read_b32 v211, a179\n\t" \
+  "v_accvgpr_read_b32 v212, a180\n\t" \
+  "v_accvgpr_read_b32 v213, a181\n\t" \
+  "v_accvgpr_read_b32 v214, a182\n\t" \
+  "v_accvgpr_read_b32 v215, a183\n\t" \
+  "v_accvgpr_read_b32 v216, a184\n\t" \
+  "v_accvgpr_read_b32 v217, a185\n\t" \
+  "v_accvgpr_read_b32 v218, a186\n\t" \
+  "v_accvgpr_read_b32 v219, a187\n\t" \
+  "v_accvgpr_read_b32 v220, a188\n\t" \
+  "v_accvgpr_read_b32 v221, a189\n\t" \
+  "v_accvgpr_read_b32 v222, a190\n\t" \
+  "v_accvgpr_read_b32 v223, a191\n\t" \
+  CVT " v224, v192, v193\n\t" \
+  CVT " v225, v194, v195\n\t" \
+  CVT " v226, v196, v197\n\t" \
+  CVT " v227, v198, v199\n\t" \
+  CVT " v228, v200, v201\n\t" \
+  CVT " v229, v202, v203\n\t" \
+  CVT " v230, v204, v205\n\t" \
+  CVT " v231, v206, v207\n\t" \
+  CVT " v232, v208, v209\n\t" \
+  CVT " v233, v210, v211\n\t" \
+  CVT " v234, v212, v213\n\t" \
+  CVT " v235, v214, v215\n\t" \
+  CVT " v236, v216, v217\n\t" \
+  CVT " v237, v218, v219\n\t" \
+  CVT " v238, v220, v221\n\t" \
+  CVT " v239, v222, v223\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_read_b128 v[176:179], %[rd] offset:0\n\t" \
+  "ds_read_b128 v[180:183], %[rd] offset:1088\n\t" \
+  "ds_read_b128 v[184:187], %[rd] offset:2176\n\t" \
+  "ds_read_b128 v[188:191], %[rd] offset:3264\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_write_b64 %[wr], v[224:225] offset:0\n\t" \
+  "ds_write_b64 %[wr], v[226:227] offset:32\n\t" \
+  "ds_write_b64 %[wr], v[228:229] offset:64\n\t" \
+  "ds_write_b64 %[wr], v[230:231] offset:96\n\t" \
+  "ds_write_b64 %[wr], v[232:233] offset:128\n\t" \
+  "ds_write_b64 %[wr], v[234:235] offset:160\n\t" \
+  "ds_write_b64 %[wr], v[236:237] offset:192\n\t" \
+  "ds_write_b64 %[wr], v[238:239] offset:224\n\t" \
+  "buffer_store_dwordx4 v[176:179], %[voff], %[rsc], s83 offen nt\n\t" \
+  "buffer_store_dwordx4 v[180:183], %[voff], %[rsc], s84 offen nt\n\t" \
+  "buffer_store_dwordx4 v[184:187], %[voff], %[rsc], s85 offen nt\n\t" \
+  "buffer_store_dwordx4 v[188:191], %[voff], %[rsc], s87 offen nt\n\t" \
+  "s_add_u32 s83, s83, %[rowstep]\n\t" \
+  "s_add_u32 s84, s84, %[rowstep]\n\t" \
+  "s_add_u32 s85, s85, %[rowstep]\n\t" \
+  "s_add_u32 s87, s87, %[rowstep]\n\t" \
+  "v_accvgpr_read_b32 v128, a192\n\t" \
+  "v_accvgpr_read_b32 v129, a193\n\t" \
+  "v_accvgpr_read_b32 v130, a194\n\t" \
+  "v_accvgpr_read_b32 v131, a195\n\t" \
+  "v_accvgpr_read_b32 v132, a196\n\t" \
+  "v_accvgpr_read_b32 v133, a197\n\t" \
+  "v_accvgpr_read_b32 v134, a198\n\t" \
+  "v_accvgpr_read_b32 v135, a199\n\t" \
+  "v_accvgpr_read_b32 v136, a200\n\t" \
+  "v_accvgpr_read_b32 v137, a201\n\t" \
+  "v_accvgpr_read_b32 v138, a202\n\t" \
+  "v_accvgpr_read_b32 v139, a203\n\t" \
+  "v_accvgpr_read_b32 v140, a204\n\t" \
+  "v_accvgpr_read_b32 v141, a205\n\t" \
+  "v_accvgpr_read_b32 v142, a206\n\t" \
+  "v_accvgpr_read_b32 v143, a207\n\t" \
+  "v_accvgpr_read_b32 v144, a208\n\t" \
+  "v_accvgpr_read_b32 v145, a209\n\t" \
+  "v_accvgpr_read_b32 v146, a210\n\t" \
+  "v_accvgpr_read_b32 v147, a211\n\t" \
+  "v_accvgpr_read_b32 v148, a212\n\t" \
+  "v_accvgpr_read_b32 v149, a213\n\t" \
+  "v_accvgpr_read_b32 v150, a214\n\t" \
+  "v_accvgpr_read_b32 v151, a215\n\t" \
+  "v_accvgpr_read_b32 v152, a216\n\t" \
+  "v_accvgpr_read_b32 v153, a217\n\t" \
+  "v_accvgpr_read_b32 v154, a218\n\t" \
+  "v_accvgpr_read_b32 v155, a219\n\t" \
+  "v_accvgpr_read_b32 v156, a220\n\t" \
+  "v_accvgpr_read_b32 v157, a221\n\t" \
+  "v_accvgpr_read_b32 v158, a222\n\t" \
+  "v_accvgpr_read_b32 v159, a223\n\t" \
+  CVT " v160, v128, v129\n\t" \
+  CVT " v161, v130, v131\n\t" \
+  CVT " v162, v132, v133\n\t" \
+  CVT " v163, v134, v135\n\t" \
+  CVT " v164, v136, v137\n\t" \
+  CVT " v165, v138, v139\n\t" \
+  CVT " v166, v140, v141\n\t" \
+  CVT " v167, v142, v143\n\t" \
+  CVT " v168, v144, v145\n\t" \
+  CVT " v169, v146, v147\n\t" \
+  CVT " v170, v148, v149\n\t" \
+  CVT " v171, v150, v151\n\t" \
+  CVT " v172, v152, v153\n\t" \
+  CVT " v173, v154, v155\n\t" \
+  CVT " v174, v156, v157\n\t" \
+  CVT " v175, v158, v159\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_read_b128 v[240:243], %[rd] offset:0\n\t" \
+  "ds_read_b128 v[244:247], %[rd] offset:1088\n\t" \
+  "ds_read_b128 v[248:251], %[rd] offset:2176\n\t" \
+  "ds_read_b128 v[252:255], %[rd] offset:3264\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_write_b64 %[wr], v[160:161] offset:0\n\t" \
+  "ds_write_b64 %[wr], v[162:163] offset:32\n\t" \
+  "ds_write_b64 %[wr], v[164:165] offset:64\n\t" \
+  "ds_write_b64 %[wr], v[166:167] offset:96\n\t" \
+  "ds_write_b64 %[wr], v[168:169] offset:128\n\t" \
+  "ds_write_b64 %[wr], v[170:171] offset:160\n\t" \
+  "ds_write_b64 %[wr], v[172:173] offset:192\n\t" \
+  "ds_write_b64 %[wr], v[174:175] offset:224\n\t" \
+  "buffer_store_dwordx4 v[240:243], %[voff], %[rsc], s83 offen nt\n\t" \
+  "buffer_store_dwordx4 v[244:247], %[voff], %[rsc], s84 offen nt\n\t" \
+  "buffer_store_dwordx4 v[248:251], %[voff], %[rsc], s85 offen nt\n\t" \
+  "buffer_store_dwordx4 v[252:255], %[voff], %[rsc], s87 offen nt\n\t" \
+  "s_add_u32 s83, s83, %[rowstep]\n\t" \
+  "s_add_u32 s84, s84, %[rowstep]\n\t" \
+  "s_add_u32 s85, s85, %[rowstep]\n\t" \
+  "s_add_u32 s87, s87, %[rowstep]\n\t" \
+  "v_accvgpr_read_b32 v192, a224\n\t" \
+  "v_accvgpr_read_b32 v193, a225\n\t" \
+  "v_accvgpr_read_b32 v194, a226\n\t" \
+  "v_accvgpr_read_b32 v195, a227\n\t" \
+  "v_accvgpr_read_b32 v196, a228\n\t" \
+  "v_accvgpr_read_b32 v197, a229\n\t" \
+  "v_accvgpr_read_b32 v198, a230\n\t" \
+  "v_accvgpr_read_b32 v199, a231\n\t" \
+  "v_accvgpr_read_b32 v200, a232\n\t" \
+  "v_accvgpr_read_b32 v201, a233\n\t" \
+  "v_accvgpr_read_b32 v202, a234\n\t" \
+  "v_accvgpr_read_b32 v203, a235\n\t" \
+  "v_accvgpr_read_b32 v204, a236\n\t" \
+  "v_accvgpr_read_b32 v205, a237\n\t" \
+  "v_accvgpr_read_b32 v206, a238\n\t" \
+  "v_accvgpr_read_b32 v207, a239\n\t" \
+  "v_accvgpr_read_b32 v208, a240\n\t" \
+  "v_accvgpr_read_b32 v209, a241\n\t" \
+  "v_accvgpr_read_b32 v210, a242\n\t" \
+  "v_accvgpr_read_b32 v211, a243\n\t" \
+  "v_accvgpr_read_b32 v212, a244\n\t" \
+  "v_accvgpr_read_b32 v213, a245\n\t" \
+  "v_accvgpr_read_b32 v214, a246\n\t" \
+  "v_accvgpr_read_b32 v215, a247\n\t" \
+  "v_accvgpr_read_b32 v216, a248\n\t" \
+  "v_accvgpr_read_b32 v217, a249\n\t" \
+  "v_accvgpr_read_b32 v218, a250\n\t" \
+  "v_accvgpr_read_b32 v219, a251\n\t" \
+  "v_accvgpr_read_b32 v220, a252\n\t" \
+  "v_accvgpr_read_b32 v221, a253\n\t" \
+  "v_accvgpr_read_b32 v222, a254\n\t" \
+  "v_accvgpr_read_b32 v223, a255\n\t" \
+  CVT " v224, v192, v193\n\t" \
+  CVT " v225, v194, v195\n\t" \
+  CVT " v226, v196, v197\n\t" \
+  CVT " v227, v198, v199\n\t" \
+  CVT " v228, v200, v201\n\t" \
+  CVT " v229, v202, v203\n\t" \
+  CVT " v230, v204, v205\n\t" \
+  CVT " v231, v206, v207\n\t" \
+  CVT " v232, v208, v209\n\t" \
+  CVT " v233, v210, v211\n\t" \
+  CVT " v234, v212, v213\n\t" \
+  CVT " v235, v214, v215\n\t" \
+  CVT " v236, v216, v217\n\t" \
+  CVT " v237, v218, v219\n\t" \
+  CVT " v238, v220, v221\n\t" \
+  CVT " v239, v222, v223\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_read_b128 v[176:179], %[rd] offset:0\n\t" \
+  "ds_read_b128 v[180:183], %[rd] offset:1088\n\t" \
+  "ds_read_b128 v[184:187], %[rd] offset:2176\n\t" \
+  "ds_read_b128 v[188:191], %[rd] offset:3264\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_write_b64 %[wr], v[224:225] offset:0\n\t" \
+  "ds_write_b64 %[wr], v[226:227] offset:32\n\t" \
+  "ds_write_b64 %[wr], v[228:229] offset:64\n\t" \
+  "ds_write_b64 %[wr], v[230:231] offset:96\n\t" \
+  "ds_write_b64 %[wr], v[232:233] offset:128\n\t" \
+  "ds_write_b64 %[wr], v[234:235] offset:160\n\t" \
+  "ds_write_b64 %[wr], v[236:237] offset:192\n\t" \
+  "ds_write_b64 %[wr], v[238:239] offset:224\n\t" \
+  "buffer_store_dwordx4 v[176:179], %[voff], %[rsc], s83 offen nt\n\t" \
+  "buffer_store_dwordx4 v[180:183], %[voff], %[rsc], s84 offen nt\n\t" \
+  "buffer_store_dwordx4 v[184:187], %[voff], %[rsc], s85 offen nt\n\t" \
+  "buffer_store_dwordx4 v[188:191], %[voff], %[rsc], s87 offen nt\n\t" \
+  "s_add_u32 s83, s83, %[rowstep]\n\t" \
+  "s_add_u32 s84, s84, %[rowstep]\n\t" \
+  "s_add_u32 s85, s85, %[rowstep]\n\t" \
+  "s_add_u32 s87, s87, %[rowstep]\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "ds_read_b128 v[240:243], %[rd] offset:0\n\t" \
+  "ds_read_b128 v[244:247], %[rd] offset:1088\n\t" \
+  "ds_read_b128 v[248:251], %[rd] offset:2176\n\t" \
+  "ds_read_b128 v[252:255], %[rd] offset:3264\n\t" \
+  "s_waitcnt lgkmcnt(0)\n\t" \
+  "buffer_store_dwordx4 v[240:243], %[voff], %[rsc], s83 offen nt\n\t" \
+  "buffer_store_dwordx4 v[244:247], %[voff], %[rsc], s84 offen nt\n\t" \
+  "buffer_store_dwordx4 v[248:251], %[voff], %[rsc], s85 offen nt\n\t" \
+  "buffer_store_dwordx4 v[252:255], %[voff], %[rsc], s87 offen nt\n\t" \
   "s_add_u32 s83, s83, %[rowstep]\n\t" \
   "s_add_u32 s84, s84, %[rowstep]\n\t" \
   "s_add_u32 s85, s85, %[rowstep]\n\t" \

@@ -13,12 +13,23 @@
 
 namespace sk {
 
+// Exponents come 16 bytes to a row, for 512 values of K (two chunks): those of row r and pair of chunks q stand at r * pitch + q * step --
+// rows as they are, K / 32 bytes apart, and 16 from pair to pair; or tiled, 16 bytes from row to row and all rows of a pair together, with zeros
+// behind K.  Descriptors reach to the array's end: a row behind the tile's brings numbers or NaN to rows and columns that are not stored.
+struct MxExponents {
+  const uint8_t *at, *end;
+  int pitch, step;
+  __device__ __forceinline__ MxExponents row(int64_t r) const { return MxExponents{at + r * pitch, end, pitch, step}; }
+  __device__ __forceinline__ uint4v rsrc() const {
+    const int64_t n = end - at;
+    return make_rsrc_words(at, (uint32_t)(n > 0x7fffffff ? 0x7fffffff : n));
+  }
+};
 struct MxArgs : WaveKArgs {      // (K, lda, ldb in pairs of bytes, four values)
-  const uint8_t *sa, *sb;        // exponents of A's rows and of the weights'
-  int pitch_a, pitch_b;          // bytes from row to row
+  MxExponents ea, eb;            // of A's rows and of the weights'
 };
 
-template <bool BF16_, int FM_, int FN_>
+template <bool BF16_, int FM_, int FN_, int CTAS_ = 1>
 struct TileWaveKMx : WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> {
   typedef WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> Base;
   typedef MxArgs Args;
@@ -30,13 +41,13 @@ struct TileWaveKMx : WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> {
   static constexpr int KV = 64, BK = 2 * KV * WAVES;  // pairs of bytes: of a chunk, of an iteration
   static constexpr int L = FM + FN;                   // blocks of a chunk, of two loads each
   static constexpr int CHUNK = L * 2048, PAIR = L * 256;   // bytes: of a chunk, of the exponents of two
-  static constexpr int MOST = 40 * 1024;              // a wave's quarter of the LDS
-  static constexpr int S = (MOST - 2 * PAIR) / CHUNK >= 3 ? 3 : 2, PAIRS = 2;   // chunks, pairs in the ring
+  static constexpr int MOST = 40 * 1024 / CTAS_;      // a wave's share of the LDS
+  static constexpr int S = (MOST - 2 * PAIR) / CHUNK >= 3 ? 3 : (MOST - 2 * PAIR) / CHUNK, PAIRS = 2;   // chunks, pairs in the ring
   static constexpr int EXPONENTS = S * CHUNK, RING = EXPONENTS + PAIRS * PAIR, LDS_BYTES = WAVES * RING, LDS_TOTAL = LDS_BYTES;
   static_assert(RING <= MOST, "LDS of a CU");
-  static constexpr int CTAS_PER_CU = 1, WAVES_PER_EU = 1, LEAST_RUN = 1;
+  static constexpr int CTAS_PER_CU = CTAS_, WAVES_PER_EU = CTAS_, CUT_COST = 3;
   static constexpr int NMFMA = 2 * NB;                // of a chunk
-  static constexpr int H = NB, HR = H - (H + 3) / 4;  // of a phase, of those that have fragments read beside them
+  static constexpr int H = NB, HR = H == 1 ? 1 : H - (H + 3) / 4;  // of a phase, of those that have fragments read beside them
 
   // loads of a chunk of this parity, and of the `behind` chunks that follow one of parity P
   static constexpr int loads(int parity) { return 2 * L + (parity == 0 ? 2 : 0); }
@@ -70,8 +81,7 @@ struct TileWaveKMx : WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> {
     const int rows_a = min(BM, a.M - pm * BM), rows_b = min(BN, a.N - pn * BN);
     const uint4v rsrc_a = uniform_rsrc(make_rsrc_words(a.A + (int64_t)pm * BM * a.lda, (uint32_t)rows_a * lda_bytes));
     const uint4v rsrc_b = uniform_rsrc(make_rsrc_words(a.B + (int64_t)pn * BN * a.ldb, (uint32_t)rows_b * ldb_bytes));
-    const uint4v rsrc_ea = uniform_rsrc(make_rsrc_words(a.sa + (int64_t)pm * BM * a.pitch_a, (uint32_t)rows_a * a.pitch_a));
-    const uint4v rsrc_eb = uniform_rsrc(make_rsrc_words(a.sb + (int64_t)pn * BN * a.pitch_b, (uint32_t)rows_b * a.pitch_b));
+    const uint4v rsrc_ea = uniform_rsrc(a.ea.row((int64_t)pm * BM).rsrc()), rsrc_eb = uniform_rsrc(a.eb.row((int64_t)pn * BN).rsrc());
     // load e of a block: its rows 8 e .. 8 e + 7, lane's row lane / 8, piece p (16 bytes, 32 values) of row r of a block at position
     // p ^ ((r >> 1) & 7); exponents: lane's row, 16 bytes
     const int row8 = lane >> 3, fi = lane & 15, fg = lane >> 4;
@@ -83,7 +93,7 @@ struct TileWaveKMx : WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> {
       off_a[e] = (uint32_t)(8 * e + row8) * lda_bytes + (uint32_t)kp[e] * 2;
       off_b[e] = (uint32_t)(8 * e + row8) * ldb_bytes + (uint32_t)kp[e] * 2;
     }
-    const uint32_t off_ea = (uint32_t)(lane * a.pitch_a), off_eb = (uint32_t)(lane * a.pitch_b);
+    const uint32_t off_ea = (uint32_t)(lane * a.ea.pitch), off_eb = (uint32_t)(lane * a.eb.pitch);
     const uint32_t ring = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_address(smem) + wave * RING);
     // one row of tiles: see rotation_of.  Several: the CTAs of an XCD share A as well as the weights and stay on the same K
     const int rot = a.M <= BM ? rotation_of(pn, n) : Base::start_of(a, pn, n);
@@ -110,9 +120,9 @@ struct TileWaveKMx : WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> {
     };
     // (the exponents of a row's end and of what lies behind it arrive together; see read_exponents)
     auto issue_exponents = [&](const Chunk &q) {
-      const uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)q.kbytes / 16), to = (uint32_t)__builtin_amdgcn_readfirstlane((int)q.pair);
-      if (lane < BM) wavek_dma_16<0>(rsrc_ea, to, q.left > 0 ? off_ea : OOB_OFFSET, at);
-      if (lane < BN) wavek_dma_16<FM * 256>(rsrc_eb, to, q.left > 0 ? off_eb : OOB_OFFSET, at);
+      const int at = __builtin_amdgcn_readfirstlane((int)q.kbytes / 256), to = __builtin_amdgcn_readfirstlane((int)q.pair);
+      if (lane < BM) wavek_dma_16<0>(rsrc_ea, (uint32_t)to, q.left > 0 ? off_ea : OOB_OFFSET, (uint32_t)(at * a.ea.step));
+      if (lane < BN) wavek_dma_16<FM * 256>(rsrc_eb, (uint32_t)to, q.left > 0 ? off_eb : OOB_OFFSET, (uint32_t)(at * a.eb.step));
     };
 #pragma unroll
     for (int t = 0; t < S; ++t)
@@ -187,7 +197,7 @@ struct TileWaveKMx : WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> {
       if constexpr (S % 2 == 0) issue_exponents(q);
       static_for<0, L>([&](auto l) { issue(l, q); });
     }
-    slot = 1;
+    slot = S > 1 ? 1 : 0;
     for (int t = 0; t < chunks; t += 2) {
       body(t, even, x, y);
       body(t + 1, odd, y, x);

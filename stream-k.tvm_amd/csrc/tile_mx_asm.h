@@ -3,8 +3,9 @@
 // takes the 16 cycles that one of 16 x 16 x 32 takes in 16 bits.  Lane group g takes chunks 2 g and 2 g + 1 of a row, so that its two exponents
 // are neighbours, and exponents come 16 bytes to a row for two iterations at a time.  gen_tile_asm.py has the register plan.
 //
-// The exponents' rows are a multiple of 16 bytes apart and hold zeros from K on (2^-127 times the zeros that the last iteration's lanes
-// behind K fetch).  A segment starts at an even iteration.
+// The exponents are tiled (MxExponents), 1 KB behind each other for a wave's load of 64 rows: as rows of K / 32 bytes they are 64 lines of the L2,
+// as many as half of the operands' own, and 8192^3 takes 265 us and not 250.  Zeros from K on multiply the zeros that the last
+// iteration's lanes behind K fetch.  A segment starts at an even iteration.
 #pragma once
 #include "tile_asm_epilogue.h"
 #include "tile_mx.h"
@@ -23,8 +24,8 @@ struct TileMxAsm : TileF16Asm<BF16 ? 6 : 5, false> {
 
   struct Ctx {
     uint4v rsrc_a, rsrc_b, rsrc_ea, rsrc_eb;
-    uint32_t voff_a, voff_b, voff_ea, voff_eb, tail;
-    uint32_t goff_a, goff_b, goff_e, gstep_a, gstep_b;
+    uint32_t voff_a, voff_b, voff_e, tail;
+    uint32_t goff_a, goff_b, goff_ea, goff_eb, gstep_a, gstep_b, step_ea, step_eb;
     uint32_t lds_wave, lds_e;
     uint32_t ra0, rb0, rda, rdb;   // where the lane reads fragments and exponents
   };
@@ -36,8 +37,8 @@ struct TileMxAsm : TileF16Asm<BF16 ? 6 : 5, false> {
     // rows past the matrix edge lie beyond the descriptors' ranges and read as zero
     c.rsrc_a = make_rsrc_words(a.A + (int64_t)pm * P::BM * a.lda, (uint32_t)(rows_a * a.lda * 2));
     c.rsrc_b = make_rsrc_words(a.B + (int64_t)pn * P::BN * a.ldb, (uint32_t)(rows_b * a.ldb * 2));
-    c.rsrc_ea = make_rsrc_words(a.sa + (int64_t)pm * P::BM * a.pitch_a, (uint32_t)(rows_a * a.pitch_a));
-    c.rsrc_eb = make_rsrc_words(a.sb + (int64_t)pn * P::BN * a.pitch_b, (uint32_t)(rows_b * a.pitch_b));
+    c.rsrc_ea = a.ea.row((int64_t)pm * P::BM).rsrc();
+    c.rsrc_eb = a.eb.row((int64_t)pn * P::BN).rsrc();
     // (loads and swizzle as in TileF16Asm::make_ctx)
     const int my_chunk = (lane & 7) ^ (((wave & 1) << 2) | (lane >> 4)), my_row = lane >> 3;
     c.voff_a = (uint32_t)(my_row * a.lda + my_chunk * 8) * 2;
@@ -47,9 +48,11 @@ struct TileMxAsm : TileF16Asm<BF16 ? 6 : 5, false> {
     c.goff_b = (uint32_t)k0 * (P::BK * 2) + (uint32_t)(wave * 16 * a.ldb);
     c.gstep_a = (uint32_t)(64 * a.lda);
     c.gstep_b = (uint32_t)(64 * a.ldb);
-    c.voff_ea = (uint32_t)((wave * 64 + lane) * a.pitch_a);
-    c.voff_eb = (uint32_t)((wave * 64 + lane) * a.pitch_b);
-    c.goff_e = (uint32_t)k0 * 8;
+    c.voff_e = (uint32_t)((wave * 64 + lane) * 16);
+    c.goff_ea = (uint32_t)(k0 >> 1) * (uint32_t)a.ea.step;
+    c.goff_eb = (uint32_t)(k0 >> 1) * (uint32_t)a.eb.step;
+    c.step_ea = (uint32_t)a.ea.step;
+    c.step_eb = (uint32_t)a.eb.step;
     const uint32_t base = lds_address(P::lds());
     c.lds_wave = base + wave * 1024;
     c.lds_e = base + EXPONENTS_AT + wave * 1024;
@@ -77,8 +80,8 @@ struct TileMxAsm : TileF16Asm<BF16 ? 6 : 5, false> {
 #undef SK_MX_LOAD_OPERANDS
   }
   static __device__ __forceinline__ void first_loads(const Ctx &c, int n, bool last) {
-    dma_load_16(c.rsrc_ea, c.lds_e, c.voff_ea, c.goff_e);
-    dma_load_16(c.rsrc_eb, c.lds_e + P::BM * 16, c.voff_eb, c.goff_e);
+    dma_load_16(c.rsrc_ea, c.lds_e, c.voff_e, c.goff_ea);
+    dma_load_16(c.rsrc_eb, c.lds_e + P::BM * 16, c.voff_e, c.goff_eb);
     stage_loads<false>(c, 0, n, last);
   }
   // last: the segment ends with K
@@ -91,9 +94,10 @@ struct TileMxAsm : TileF16Asm<BF16 ? 6 : 5, false> {
     asm volatile(SK_TILE_ASM_LOOP_MX
                  : [ra0] "+v"(c.ra0), [rb0] "+v"(c.rb0)
                  : [rsa] "s"(c.rsrc_a), [rsb] "s"(c.rsrc_b), [rea] "s"(c.rsrc_ea), [reb] "s"(c.rsrc_eb), [voa] "v"(c.voff_a), [vob] "v"(c.voff_b),
-                   [vea] "v"(c.voff_ea), [veb] "v"(c.voff_eb), [tail] "v"(last ? c.tail : 0u), [rda] "v"(c.rda), [rdb] "v"(c.rdb), [ga0] "s"(c.goff_a),
+                   [ve] "v"(c.voff_e), [tail] "v"(last ? c.tail : 0u), [rda] "v"(c.rda), [rdb] "v"(c.rdb), [ga0] "s"(c.goff_a),
                    [gb0] "s"(c.goff_b), [gas] "s"(c.gstep_a), [gas2] "s"(2 * c.gstep_a), [gas3] "s"(3 * c.gstep_a), [gbs] "s"(c.gstep_b),
-                   [gbs2] "s"(2 * c.gstep_b), [gbs3] "s"(3 * c.gstep_b), [n] "s"((uint32_t)n), [lds] "s"(c.lds_wave), [ek] "s"(c.goff_e + 16),
+                   [gbs2] "s"(2 * c.gstep_b), [gbs3] "s"(3 * c.gstep_b), [n] "s"((uint32_t)n), [lds] "s"(c.lds_wave), [eka] "s"(c.goff_ea + c.step_ea),
+                   [ekb] "s"(c.goff_eb + c.step_eb), [esa] "s"(c.step_ea), [esb] "s"(c.step_eb),
                    [el] "s"(c.lds_e + PAIR_BYTES)
                  : "memory", "m0", "scc", SK_TILE_ASM_CLOBBERS_MX);
     // every wave has left the loop and its own loads have landed: the stages are free

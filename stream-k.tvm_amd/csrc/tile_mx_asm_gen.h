@@ -262,7 +262,8 @@
   "s_add_u32 s81, %[ga0], 128\n\t" \
   "s_add_u32 s82, %[gb0], 128\n\t" \
   "s_mov_b32 s88, %[el]\n\t" \
-  "s_mov_b32 s89, %[ek]\n\t" \
+  "s_mov_b32 s89, %[eka]\n\t" \
+  "s_mov_b32 s90, %[ekb]\n\t" \
   "v_xor_b32 v124, 16, %[ra0]\n\t" \
   "v_xor_b32 v125, 16, %[rb0]\n\t" \
   "v_mov_b32 v126, %[rda]\n\t" \
@@ -424,7 +425,8 @@
   "s_mov_b32 m0, s88\n\t" \
   "v_mfma_scale_f32_16x16x128_f8f6f4 a[192:195], v[160:163], v[152:155], a[192:195], v96, v94 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
   "v_mfma_scale_f32_16x16x128_f8f6f4 a[196:199], v[164:167], v[152:155], a[196:199], v97, v94 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
-  "buffer_load_dwordx4 %[vea], %[rea], s89 offen lds\n\t" \
+  "buffer_load_dwordx4 %[ve], %[rea], s89 offen lds\n\t" \
+  "s_add_u32 s89, s89, %[esa]\n\t" \
   "v_mfma_scale_f32_16x16x128_f8f6f4 a[200:203], v[168:171], v[152:155], a[200:203], v98, v94 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
   "v_mfma_scale_f32_16x16x128_f8f6f4 a[204:207], v[172:175], v[152:155], a[204:207], v99, v94 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
   "v_mfma_scale_f32_16x16x128_f8f6f4 a[172:175], v[172:175], v[148:151], a[172:175], v99, v93 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
@@ -433,8 +435,8 @@
   "v_mfma_scale_f32_16x16x128_f8f6f4 a[168:171], v[168:171], v[148:151], a[168:171], v98, v93 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
   "v_mfma_scale_f32_16x16x128_f8f6f4 a[164:167], v[164:167], v[148:151], a[164:167], v97, v93 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
   "v_mfma_scale_f32_16x16x128_f8f6f4 a[160:163], v[160:163], v[148:151], a[160:163], v96, v93 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
-  "buffer_load_dwordx4 %[veb], %[reb], s89 offen lds\n\t" \
-  "s_add_u32 s89, s89, 16\n\t" \
+  "buffer_load_dwordx4 %[ve], %[reb], s90 offen lds\n\t" \
+  "s_add_u32 s90, s90, %[esb]\n\t" \
   "v_mfma_scale_f32_16x16x128_f8f6f4 a[128:131], v[160:163], v[144:147], a[128:131], v96, v92 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
   "v_mfma_scale_f32_16x16x128_f8f6f4 a[132:135], v[164:167], v[144:147], a[132:135], v97, v92 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
   "v_mfma_scale_f32_16x16x128_f8f6f4 a[136:139], v[168:171], v[144:147], a[136:139], v98, v92 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
@@ -879,4 +881,4 @@
   "v216", "v217", "v218", "v219", "v220", "v221", "v222", "v223", "v224", "v225", "v226", "v227", "v228", "v229", "v230", "v231", \
   "v232", "v233", "v234", "v235", "v236", "v237", "v238", "v239", "v240", "v241", "v242", "v243", "v244", "v245", "v246", "v247", \
   "v248", "v249", "v250", "v251", "v252", "v253", "v254", "v255", "s80", "s81", "s82", "s83", "s84", "s85", "s86", "s87", \
-  "s88", "s89"
+  "s88", "s89", "s90"

@@ -15,7 +15,7 @@
 
 namespace sk {
 
-template <bool BF16_, int BM_, int BN_, int WM_, int WN_, int STAGES_>
+template <bool BF16_, int BM_, int BN_, int WM_, int WN_, int STAGES_, int CTAS_ = 1>
 struct TileMxShared {
   typedef MxArgs Args;
   typedef int intx4 __attribute__((ext_vector_type(4)));
@@ -27,8 +27,8 @@ struct TileMxShared {
   static constexpr int LW = (BM + BN) / 32;                    // a wave's loads of a chunk, 8 rows each
   static constexpr int LE = (BM + BN + 255) / 256;             // and of two chunks' exponents, 64 rows each
   static constexpr int CHUNK = (BM + BN) * 128, PAIR = LE * 256 * 16, PAIRS = (STAGES + 2) / 2;   // bytes; pairs of chunks whose exponents are kept
-  static constexpr int EXPONENTS = STAGES * CHUNK, LDS_BYTES = EXPONENTS + PAIRS * PAIR, CTAS_PER_CU = 1, WAVES_PER_EU = 1;
-  static_assert(WM * WN == WAVES && BM % 64 == 0 && BN % 64 == 0 && LDS_BYTES <= 160 * 1024, "see above");
+  static constexpr int EXPONENTS = STAGES * CHUNK, LDS_BYTES = EXPONENTS + PAIRS * PAIR, CTAS_PER_CU = CTAS_, WAVES_PER_EU = CTAS_, CUT_COST = 8;
+  static_assert(WM * WN == WAVES && BM % 64 == 0 && BN % 64 == 0 && CTAS_ * LDS_BYTES <= 160 * 1024, "see above");
   typedef BlockPatch<FM, FN> Patch;
   static_assert(WAVES * Patch::BYTES <= LDS_BYTES, "the patches fit the ring");
 
@@ -63,13 +63,12 @@ struct TileMxShared {
     // rows past M / N lie beyond the descriptors' ranges and read as zero
     const uint4v rsrc_a = uniform_rsrc(make_rsrc_words(a.A + (int64_t)pm * BM * a.lda, (uint32_t)rows_a * lda_bytes));
     const uint4v rsrc_b = uniform_rsrc(make_rsrc_words(a.B + (int64_t)pn * BN * a.ldb, (uint32_t)rows_b * ldb_bytes));
-    const uint4v rsrc_ea = uniform_rsrc(make_rsrc_words(a.sa + (int64_t)pm * BM * a.pitch_a, (uint32_t)rows_a * a.pitch_a));
-    const uint4v rsrc_eb = uniform_rsrc(make_rsrc_words(a.sb + (int64_t)pn * BN * a.pitch_b, (uint32_t)rows_b * a.pitch_b));
+    const uint4v rsrc_ea = uniform_rsrc(a.ea.row((int64_t)pm * BM).rsrc()), rsrc_eb = uniform_rsrc(a.eb.row((int64_t)pn * BN).rsrc());
     // load x of a chunk: rows 8 (wave + 4 x) .. + 7 of A's and then the weights', lane's row lane / 8; piece p (16 bytes, 32 values) of row r stands
     // at position p ^ ((r >> 1) & 7)
     const int row8 = lane >> 3, fi = lane & 15, fg = lane >> 4, kp = ((lane & 7) ^ (4 * (wave & 1) + (row8 >> 1))) * 8;
     const uint32_t off_a = (uint32_t)row8 * lda_bytes + (uint32_t)kp * 2, off_b = (uint32_t)row8 * ldb_bytes + (uint32_t)kp * 2;
-    const uint32_t off_ea = (uint32_t)(lane * a.pitch_a), off_eb = (uint32_t)(lane * a.pitch_b);
+    const uint32_t off_ea = (uint32_t)(lane * a.ea.pitch), off_eb = (uint32_t)(lane * a.eb.pitch);
     const uint32_t ring = lds_address(smem) + (uint32_t)wave * 1024;
     const int rot = rotation_of(pn, n), chunks = 2 * n;
     auto left_of = [&](int t) { return t < chunks ? a.K - ((k0 + rotated_iteration(t >> 1, rot, n)) * 2 + (t & 1)) * KV : 0; };
@@ -94,7 +93,8 @@ struct TileMxShared {
         constexpr int y = decltype(yi)::value;
         const int first = 64 * (wave + 4 * y);
         const bool of_a = first < BM, any = first < BM + BN && q.left > 0;
-        const uint32_t rows = q.kbytes / 16 + (uint32_t)(any ? (of_a ? first * a.pitch_a : (first - BM) * a.pitch_b) : 0);
+        const int at = (int)q.kbytes / 256;
+        const uint32_t rows = (uint32_t)(any ? (of_a ? at * a.ea.step + first * a.ea.pitch : at * a.eb.step + (first - BM) * a.eb.pitch) : 0);
         wavek_dma_16<y * 4096>(uniform_rsrc(of_a ? rsrc_ea : rsrc_eb), q.pair, any ? (of_a ? off_ea : off_eb) : OOB_OFFSET,
                                (uint32_t)__builtin_amdgcn_readfirstlane((int)rows));
       });

@@ -48,8 +48,9 @@ struct WaveKTile {
   static constexpr bool COHERENT_PARTIALS = true;
   static constexpr bool FIXUP_WORD_IN_LDS = true;     // the rings are dead between two calls of mac
   static constexpr int TYPE = TYPE_, FM = FM_, FN = FN_, BM = 16 * FM_, BN = 16 * FN_, WAVES = 4, NT = 256;
-  static constexpr int TILE_ELEMS = BM * BN, NB = FM * FN, NQ = NB / WAVES;   // blocks of the tile, of a wave's quarter
-  static_assert(NB % WAVES == 0, "the waves share out the blocks evenly");
+  static constexpr int TILE_ELEMS = BM * BN, NB = FM * FN, NQ = NB < WAVES ? 1 : NB / WAVES;   // blocks of the tile, of a wave's quarter
+  static constexpr bool FEW = NB < WAVES;             // 64 threads to a block, the others have no piece
+  static_assert(FEW || NB % WAVES == 0, "the waves share out the blocks evenly");
   static constexpr bool I8 = TYPE_ == WK_I8, BF16 = TYPE_ == WK_BF16, F8 = TYPE_ == WK_F8E4M3 || TYPE_ == WK_F8E5M2;
   typedef int intx4 __attribute__((ext_vector_type(4)));
   typedef typename std::conditional<I8, intx4, floatx4>::type AccV;
@@ -146,7 +147,7 @@ struct WaveKTile {
 #pragma unroll
     for (int u = 0; u < PIECES; ++u) {
       const int row = pm * BM + piece_row(u, tid), col = pn * BN + piece_col(u, tid) * PW;
-      if (row >= a.M || col >= a.N) continue;
+      if (row >= a.M || col >= a.N || (FEW && tid >= 64 * NB)) continue;
       if constexpr (I8) {   // int32 C straight from the accumulators (ldc counts int32 elements)
         int *dst = reinterpret_cast<int *>(a.C) + (int64_t)row * a.ldc + col;
         if (vec_ok && col + 4 <= a.N) {

@@ -193,17 +193,17 @@ bool mx_product(const Tensor &A, const Tensor &B, const Tensor *offsets, MaybeTy
   g.scale_b = scale_b->data_ptr();
   g.variant = variant;
   void *stream = current_stream();
-  Tensor padded[2];   // (freed in stream order)
-  if (const int64_t wide = sk_mx_scale_pitch(&g)) {
-    const Tensor *from[2] = {scale_a, scale_b};
-    for (int i = 0; i < 2; ++i) {
-      const int64_t rows = i ? E * N : R;
-      padded[i] = fresh(A, {rows, wide}, at::kByte);
-      if (sk_pad_mx_scales(from[i]->data_ptr(), rows, K / 32, wide, padded[i].data_ptr(), stream) != SK_OK) return false;
-    }
-    g.scale_a = padded[0].data_ptr();
-    g.scale_b = padded[1].data_ptr();
-    g.scale_pitch_a = g.scale_pitch_b = wide;
+  Tensor tiled;   // (freed in stream order)
+  if (sk_mx_scales_tiled(&g)) {
+    const int64_t width = (K + 511) / 512 * 16;
+    tiled = fresh(A, {R + E * N, width}, at::kByte);
+    char *to = static_cast<char *>(tiled.data_ptr());
+    if (sk_tile_mx_scales(g.scale_a, R, to, g.scale_b, E * N, to + R * width, K / 32, stream) != SK_OK) return false;
+    g.scale_a = to;
+    g.scale_b = to + R * width;
+    g.scales_tiled = 1;
+  } else if (!aligned(*scale_a, 4) || !aligned(*scale_b, 4)) {
+    return false;
   }
   const size_t need = sk_grouped_workspace_bytes(&g);
   std::shared_lock<std::shared_mutex> lock(streamk_torch::g_mutex);

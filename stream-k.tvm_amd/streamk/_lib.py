@@ -58,7 +58,7 @@ class SkGrouped(ctypes.Structure):
         (n, ctypes.c_void_p) for n in ("A", "B", "offsets", "C")] + [
         (n, ctypes.c_int64) for n in ("lda", "ldb", "ldc", "expert_b")] + [
         (n, ctypes.c_void_p) for n in ("bias", "scale_a", "scale_b")] + [
-        (n, ctypes.c_int64) for n in ("variant", "spin_limit", "scale_pitch_a", "scale_pitch_b")]
+        (n, ctypes.c_int64) for n in ("variant", "spin_limit", "scales_tiled")]
 
 
 SK_SCORES_SOFTMAX, SK_SCORES_SIGMOID = 0, 1
@@ -163,14 +163,13 @@ def lib():
     L.sk_route_scored_backward.argtypes = [vp, ci, i64, i64, i64, i64, P(SkRouteScores), vp, vp, vp, vp]
     L.sk_quantize_mxfp4.argtypes = [vp, ci, i64, i64, i64, vp, vp, vp]
     L.sk_dequantize_mxfp4.argtypes = [vp, vp, i64, i64, ci, vp, vp]
-    L.sk_pad_mx_scales.argtypes = [vp, i64, i64, i64, vp, vp]
-    L.sk_mx_scale_pitch.argtypes = [P(SkGrouped)]
-    L.sk_mx_scale_pitch.restype = i64
+    L.sk_tile_mx_scales.argtypes = [vp, i64, vp, vp, i64, vp, i64, vp]
+    L.sk_mx_scales_tiled.argtypes = [P(SkGrouped)]
     L.sk_dispatch_rows.argtypes = [vp, i64, i64, vp, vp, i64, i64, vp, vp]
     L.sk_combine_rows.argtypes = [vp, ci, vp, vp, i64, i64, i64, vp, vp]
     L.sk_combine_backward.argtypes = [vp, vp, ci, vp, vp, vp, i64, i64, i64, vp, vp, vp]
     for f in ("sk_gemm_i8_scaled", "sk_i8_scaled_takes", "sk_quantize_i8", "sk_gemm_grouped", "sk_grouped_wgrad", "sk_route_experts", "sk_route_backward",
-              "sk_route_scored", "sk_route_scored_backward", "sk_quantize_mxfp4", "sk_dequantize_mxfp4", "sk_pad_mx_scales",
+              "sk_route_scored", "sk_route_scored_backward", "sk_quantize_mxfp4", "sk_dequantize_mxfp4", "sk_tile_mx_scales", "sk_mx_scales_tiled",
               "sk_dispatch_rows", "sk_combine_rows", "sk_combine_backward"):
         getattr(L, f).restype = ci
     for f in ("sk_device_info", "sk_make_plan", "sk_plan_cta_range", "sk_plan_tile_coords",

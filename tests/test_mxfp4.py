@@ -231,6 +231,20 @@ def test_what_lies_behind_a_row_does_not_count(sk, K):
         assert_near(C[::2, ::2], (va @ vb.T)[::2, ::2], K, (va.abs() @ vb.abs().T)[::2, ::2])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows_a,rows_b,blocks", [(1, 1, 1), (5, 64, 16), (65, 7, 17), (300, 130, 129), (64, 200, 256), (3, 70, 500)])
+def test_tiled_scales(sk, rows_a, rows_b, blocks):
+    g = torch.Generator().manual_seed(4)
+    arrays = [torch.randint(0, 256, (rows, blocks), generator=g, dtype=torch.uint8).cuda() for rows in (rows_a, rows_b)]
+    pairs = (blocks + 15) // 16
+    tiled = [torch.full((pairs, rows, 16), 77, dtype=torch.uint8, device="cuda") for rows in (rows_a, rows_b)]
+    stream = torch.cuda.current_stream().cuda_stream
+    assert sk.lib().sk_tile_mx_scales(arrays[0].data_ptr(), rows_a, tiled[0].data_ptr(), arrays[1].data_ptr(), rows_b, tiled[1].data_ptr(), blocks, stream) == 0
+    for t, a in zip(tiled, arrays):
+        padded = torch.nn.functional.pad(a, (0, pairs * 16 - blocks))
+        assert torch.equal(t, padded.view(-1, pairs, 16).transpose(0, 1))
+
+
 SIZES = {"one": [5], "even": [16, 16, 16, 16], "skew": [1, 0, 70, 0, 200, 3], "empty": [0, 0, 0], "large": [300, 130], "many": [3] * 130}
 
 
@@ -380,18 +394,20 @@ def test_calls_are_refused_with_codes(sk):
         assert product(**bad) == -1, bad
     for bad in (dict(layout=1), dict(out_dtype=lib.SK_F32), dict(out_dtype=lib.SK_MXFP4), dict(activation=9), dict(variant=-1)):
         assert product(**bad) == -4, bad
-    for bad in (dict(K=0), dict(lda=32), dict(ldb=32), dict(ldc=63), dict(scale_pitch_a=1), dict(scale_pitch_b=-2), dict(lda=1 << 40), dict(R=1 << 31)):
+    for bad in (dict(K=0), dict(lda=32), dict(ldb=32), dict(ldc=63), dict(lda=1 << 40), dict(R=1 << 31),
+                dict(scales_tiled=1, N=1 << 27), dict(scales_tiled=1, R=1 << 26, K=2048, lda=2048, ldb=2048)):
         assert product(**bad) == -2, bad
-    for bad in (dict(K=48), dict(lda=80), dict(ldb=80), dict(expert_b=4112), dict(A=p + 8), dict(B=p + 2), dict(C=p + 1), dict(scale_a=p + 1), dict(scale_b=p + 1),
-                dict(scale_pitch_a=3), dict(offsets=p + 2)):
+    for bad in (dict(K=48), dict(lda=80), dict(ldb=80), dict(expert_b=4112), dict(A=p + 8), dict(B=p + 2), dict(C=p + 1), dict(scale_a=p + 1), dict(scale_b=p + 2),
+                dict(scales_tiled=1, scale_a=p + 4), dict(offsets=p + 2)):
         assert product(**bad) == -3, bad
     quantize = lambda x=p, t=0, M=4, K=64, ld=64, q=p, s=p: L.sk_quantize_mxfp4(x, t, M, K, ld, q, s, None)  # noqa: E731
     assert quantize(x=None) == -1 and quantize(s=None) == -1 and quantize(t=6) == -4 and quantize(M=0) == -2 and quantize(ld=63) == -2 and quantize(K=40) == -3
     assert quantize(x=p + 1) == -3 and quantize(q=p + 2) == -3 and quantize(M=1 << 40, K=1 << 20, ld=1 << 20) == -2
     values_of = lambda q=p, s=p, M=4, K=64, t=0, x=p: L.sk_dequantize_mxfp4(q, s, M, K, t, x, None)  # noqa: E731
     assert values_of(q=None) == -1 and values_of(t=6) == -4 and values_of(K=40) == -3 and values_of(M=-1) == -2 and values_of(x=p + 1) == -3
-    pad = lambda s=p, rows=4, blocks=3, pitch=16, out=p: L.sk_pad_mx_scales(s, rows, blocks, pitch, out, None)  # noqa: E731
-    assert pad(s=None) == -1 and pad(blocks=17) == -2 and pad(rows=0) == -2 and pad(pitch=24) == -3 and pad(out=p + 4) == -3
+    tile = lambda a=p, rows=4, ta=p, b=p, more=5, tb=p, blocks=3: L.sk_tile_mx_scales(a, rows, ta, b, more, tb, blocks, None)  # noqa: E731
+    assert tile(a=None) == -1 and tile(tb=None) == -1 and tile(rows=0) == -2 and tile(more=1 << 31) == -2 and tile(blocks=0) == -2 and tile(ta=p + 8) == -3
+    assert L.sk_mx_scales_tiled(None) == 0
 
 
 def test_fake_implementations(sk):
