@@ -44,6 +44,9 @@ using MxWaveK2 = MxWithZero<TileWaveKMx<BF16, FM, FN, 2>>;
   X(GV_WAVEK64, MxWaveK<BF16, 4, 4>)                              \
   X(10, MxWaveK2<BF16, 1, 4>) \
   X(11, MxWaveK2<BF16, 2, 4>) \
+  X(12, MxWaveK2<BF16, 4, 4>) \
+  X(18, TileMxShared<BF16, 64, 64, 2, 2, 4, 2>) \
+  X(GV_SHARED256, TileMxShared<BF16, 256, 128, 2, 2, 3>) \
   X(13, TileMxShared<BF16, 64, 128, 2, 2, 3, 2>) \
   X(14, TileMxShared<BF16, 128, 64, 2, 2, 3, 2>) \
   X(15, TileMxShared<BF16, 128, 128, 2, 2, 2, 2>) \

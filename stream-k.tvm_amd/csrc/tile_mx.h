@@ -40,7 +40,7 @@ struct TileWaveKMx : WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> {
   static constexpr int FM = FM_, FN = FN_, BM = Base::BM, BN = Base::BN, WAVES = Base::WAVES, NT = Base::NT, NB = Base::NB;
   static constexpr int KV = 64, BK = 2 * KV * WAVES;  // pairs of bytes: of a chunk, of an iteration
   static constexpr int L = FM + FN;                   // blocks of a chunk, of two loads each
-  static constexpr int CHUNK = L * 2048, PAIR = L * 256;   // bytes: of a chunk, of the exponents of two
+  static constexpr int CHUNK = L * 2048, PAIR = 2 * 1024;   // bytes: of a chunk, of the exponents of two (64 rows of A and of the weights)
   static constexpr int MOST = 40 * 1024 / CTAS_;      // a wave's share of the LDS
   static constexpr int S = (MOST - 2 * PAIR) / CHUNK >= 3 ? 3 : (MOST - 2 * PAIR) / CHUNK, PAIRS = 2;   // chunks, pairs in the ring
   static constexpr int EXPONENTS = S * CHUNK, RING = EXPONENTS + PAIRS * PAIR, LDS_BYTES = WAVES * RING, LDS_TOTAL = LDS_BYTES;
@@ -93,7 +93,7 @@ struct TileWaveKMx : WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> {
       off_a[e] = (uint32_t)(8 * e + row8) * lda_bytes + (uint32_t)kp[e] * 2;
       off_b[e] = (uint32_t)(8 * e + row8) * ldb_bytes + (uint32_t)kp[e] * 2;
     }
-    const uint32_t off_ea = (uint32_t)(lane * a.ea.pitch), off_eb = (uint32_t)(lane * a.eb.pitch);
+    const uint32_t off_ea = lane < BM ? (uint32_t)(lane * a.ea.pitch) : OOB_OFFSET, off_eb = lane < BN ? (uint32_t)(lane * a.eb.pitch) : OOB_OFFSET;
     const uint32_t ring = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_address(smem) + wave * RING);
     // one row of tiles: see rotation_of.  Several: the CTAs of an XCD share A as well as the weights and stay on the same K
     const int rot = a.M <= BM ? rotation_of(pn, n) : Base::start_of(a, pn, n);
@@ -121,8 +121,8 @@ struct TileWaveKMx : WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> {
     // (the exponents of a row's end and of what lies behind it arrive together; see read_exponents)
     auto issue_exponents = [&](const Chunk &q) {
       const int at = __builtin_amdgcn_readfirstlane((int)q.kbytes / 256), to = __builtin_amdgcn_readfirstlane((int)q.pair);
-      if (lane < BM) wavek_dma_16<0>(rsrc_ea, (uint32_t)to, q.left > 0 ? off_ea : OOB_OFFSET, (uint32_t)(at * a.ea.step));
-      if (lane < BN) wavek_dma_16<FM * 256>(rsrc_eb, (uint32_t)to, q.left > 0 ? off_eb : OOB_OFFSET, (uint32_t)(at * a.eb.step));
+      wavek_dma_16<0>(rsrc_ea, (uint32_t)to, q.left > 0 ? off_ea : OOB_OFFSET, (uint32_t)(at * a.ea.step));
+      wavek_dma_16<1024>(rsrc_eb, (uint32_t)to, q.left > 0 ? off_eb : OOB_OFFSET, (uint32_t)(at * a.eb.step));
     };
 #pragma unroll
     for (int t = 0; t < S; ++t)
@@ -141,47 +141,45 @@ struct TileWaveKMx : WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> {
     // read r of a chunk of parity P: the fragments of step 0 and the exponents, block by block, then the fragments of step 1
     auto read = [&](auto ri, auto parity, Frags &f) {
       constexpr int r = decltype(ri)::value, what = r < 2 * L ? r % 2 : 2, b = r < 2 * L ? r / 2 : r - 2 * L;
-      if constexpr (what == 1) f.e[b] = *reinterpret_cast<const uint16_t *>(rd_e + pair * PAIR + b * 256 + 8 * decltype(parity)::value);
+      if constexpr (what == 1) f.e[b] = *reinterpret_cast<const uint16_t *>(rd_e + pair * PAIR + (b < FM ? b * 256 : 1024 + (b - FM) * 256) + 8 * decltype(parity)::value);
       else f.v[b][what / 2] = *reinterpret_cast<const intx4 *>((what ? rd1 : rd0) + slot * CHUNK + b * 2048);
     };
     // the last chunk of K: blocks behind K are zeros, and their exponents, which are another row's, have to be numbers
     auto mask_exponents = [&](int left, Frags &f) {
-      if (left >= KV) return;
       const int mask = (16 * fg < left ? 0xff : 0) | (16 * fg + 8 < left ? 0xff00 : 0);
 #pragma unroll
       for (int b = 0; b < L; ++b) f.e[b] &= mask;
     };
     // X: fragments of chunk t (parity P), Y: of chunk t + 1, read while the first half of chunk t is multiplied; their place is refilled
-    // during the second half with chunk t + 1 + S
-    auto body = [&](int t, auto parity, const Frags &x, Frags &y) {
+    // during the second half with chunk t + 1 + S.  REFILL: it is requested; MORE: there is a chunk t + 1.  (The loops below say which: with the
+    // choice inside, the compiler moves the accumulators between its register files for every MFMA.)
+    auto body = [&](int t, auto parity, auto refill, auto more, const Frags &x, Frags &y) {
       constexpr int P = decltype(parity)::value;
-      if (t + 1 < chunks) {
-        wait_chunk<1 - P>(chunks - 2 - t);
-        static_for<0, H>([&](auto m) {
-          mfma<m>(c, x);
-          // (none beside the last MFMAs: they are waited for behind those)
+      constexpr bool REFILL = decltype(refill)::value, MORE = decltype(more)::value, FIRST = ((P + 1 + S) & 1) == 0;
+      if constexpr (REFILL) wavek_wait_loads<loads_behind(1 - P, S - 1)>();
+      else if constexpr (MORE) wait_chunk<1 - P>(chunks - 2 - t);
+      static_for<0, H>([&](auto m) {
+        mfma<m>(c, x);
+        // (none beside the last MFMAs: they are waited for behind those)
+        if constexpr (MORE)
           static_for<(m * READS / HR < READS ? m * READS / HR : READS), ((m + 1) * READS / HR < READS ? (m + 1) * READS / HR : READS)>(
               [&](auto r) { read(r, std::integral_constant<int, 1 - P>{}, y); });
-          __builtin_amdgcn_sched_barrier(0);
-        });
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      if constexpr (MORE) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         mask_exponents(left_of(t + 1), y);
-      } else {
-        static_for<0, H>([&](auto m) { mfma<m>(c, x); });
       }
-      if (t + 1 + S < chunks) {
-        const Chunk q = chunk(t + 1 + S, slot, P == 1 ? (pair + S / 2) % PAIRS : (pair + 1 + S / 2) % PAIRS);
-        // (chunk t + 1 is of the pair `pair`)
-        constexpr bool FIRST = ((P + 1 + S) & 1) == 0;
+      Chunk q;
+      if constexpr (REFILL) {   // (chunk t + 1 is of the pair `pair`)
+        q = chunk(t + 1 + S, slot, P == 1 ? (pair + S / 2) % PAIRS : (pair + 1 + S / 2) % PAIRS);
         if constexpr (FIRST) issue_exponents(q);
-        static_for<0, NMFMA - H>([&](auto m) {
-          mfma<H + m>(c, x);
-          static_for<m * L / (NMFMA - H), (m + 1) * L / (NMFMA - H)>([&](auto l) { issue(l, q); });
-          __builtin_amdgcn_sched_barrier(0);
-        });
-      } else {
-        static_for<H, NMFMA>([&](auto m) { mfma<m>(c, x); });
       }
+      static_for<0, NMFMA - H>([&](auto m) {
+        mfma<H + m>(c, x);
+        if constexpr (REFILL) static_for<m * L / (NMFMA - H), (m + 1) * L / (NMFMA - H)>([&](auto l) { issue(l, q); });
+        __builtin_amdgcn_sched_barrier(0);
+      });
       slot = slot + 1 == S ? 0 : slot + 1;
       if constexpr (P == 0) pair ^= 1;   // (chunk t + 2 begins the next pair)
     };
@@ -198,10 +196,25 @@ struct TileWaveKMx : WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> {
       static_for<0, L>([&](auto l) { issue(l, q); });
     }
     slot = S > 1 ? 1 : 0;
-    for (int t = 0; t < chunks; t += 2) {
-      body(t, even, x, y);
-      body(t + 1, odd, y, x);
+    constexpr std::true_type yes;
+    constexpr std::false_type no;
+    int t = 0;
+    for (; t + 2 + S < chunks; t += 2) {
+      body(t, even, yes, yes, x, y);
+      body(t + 1, odd, yes, yes, y, x);
     }
+    if constexpr (S % 2 == 0)
+      if (t + 1 + S < chunks) {
+        body(t, even, yes, yes, x, y);
+        body(t + 1, odd, no, yes, y, x);
+        t += 2;
+      }
+    for (; t + 2 < chunks; t += 2) {
+      body(t, even, no, yes, x, y);
+      body(t + 1, odd, no, yes, y, x);
+    }
+    body(t, even, no, yes, x, y);
+    body(t + 1, odd, no, no, y, x);
     wavek_wait_loads<0>();
     Base::template add_waves<RING>(c, acc, smem);
   }

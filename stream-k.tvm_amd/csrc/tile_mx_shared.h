@@ -123,7 +123,6 @@ struct TileMxShared {
     };
     // the last chunk of K: blocks behind K are zeros, and their exponents, which are another row's, have to be numbers
     auto mask_exponents = [&](int left, Exponents &e) {
-      if (left >= KV) return;
       const int mask = (16 * fg < left ? 0xff : 0) | (16 * fg + 8 < left ? 0xff00 : 0);
 #pragma unroll
       for (int i = 0; i < FM; ++i) e.a[i] &= mask;
@@ -140,47 +139,41 @@ struct TileMxShared {
     constexpr int READS = FM + FN;
     int slot = 0, pair = 0;   // of chunk t
     Frags f0, f1;             // of the steps
-    auto body = [&](int t, auto parity, const Exponents &e, Exponents &en) {
+    // REFILL: chunk t + STAGES is requested; MORE: there is a chunk t + 1.  (The loops below say which: with the choice inside, the compiler
+    // moves the accumulators between its register files for every MFMA.)
+    auto body = [&](int t, auto parity, auto refill, auto more, const Exponents &e, Exponents &en) {
       constexpr int P = decltype(parity)::value;
+      constexpr bool REFILL = decltype(refill)::value, MORE = decltype(more)::value, FIRST = ((P + STAGES) & 1) == 0;
       const int next = slot + 1 == STAGES ? 0 : slot + 1, next_pair = P == 0 ? pair : (pair + 1 == PAIRS ? 0 : pair + 1);
       static_for<0, NB>([&](auto v) {
         mfma(v, zero, f0, e);
         static_for<v * READS / NB, (v + 1) * READS / NB>([&](auto r) { read(r, one, f1, slot); });
         __builtin_amdgcn_sched_barrier(0);
       });
-      const bool more = t + 1 < chunks;
-      if (more) wait_chunk<1 - P, STAGES - 2>(chunks - 2 - t);
+      if constexpr (REFILL) wavek_wait_loads<loads_behind(1 - P, STAGES - 2)>();
+      else if constexpr (MORE) wait_chunk<1 - P, STAGES - 2>(chunks - 2 - t);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      // (loops of their own: with the choice inside, the compiler moves accumulators between its register files)
-      if (t + STAGES < chunks) {
-        constexpr bool FIRST = ((P + STAGES) & 1) == 0;
-        const Chunk q = chunk(t + STAGES, slot, (((t + STAGES) >> 1) % PAIRS));
+      Chunk q;
+      if constexpr (REFILL) {
+        q = chunk(t + STAGES, slot, ((t + STAGES) >> 1) % PAIRS);
         if constexpr (FIRST) issue_exponents(q);
-        static_for<0, NB>([&](auto v) {
-          mfma(v, one, f1, e);
-          static_for<v * LW / NB, (v + 1) * LW / NB>([&](auto x) { issue(x, q); });
-          static_for<v * READS / NB, (v + 1) * READS / NB>([&](auto r) {
-            read(r, zero, f0, next);
-            read_exponent(r, std::integral_constant<int, 1 - P>{}, en, next_pair);
-          });
-          __builtin_amdgcn_sched_barrier(0);
-        });
-      } else if (more) {
-        static_for<0, NB>([&](auto v) {
-          mfma(v, one, f1, e);
-          static_for<v * READS / NB, (v + 1) * READS / NB>([&](auto r) {
-            read(r, zero, f0, next);
-            read_exponent(r, std::integral_constant<int, 1 - P>{}, en, next_pair);
-          });
-          __builtin_amdgcn_sched_barrier(0);
-        });
-      } else {
-        static_for<0, NB>([&](auto v) { mfma(v, one, f1, e); });
       }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      mask_exponents(left_of(t + 1), en);
+      static_for<0, NB>([&](auto v) {
+        mfma(v, one, f1, e);
+        if constexpr (REFILL) static_for<v * LW / NB, (v + 1) * LW / NB>([&](auto x) { issue(x, q); });
+        if constexpr (MORE)
+          static_for<v * READS / NB, (v + 1) * READS / NB>([&](auto r) {
+            read(r, zero, f0, next);
+            read_exponent(r, std::integral_constant<int, 1 - P>{}, en, next_pair);
+          });
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      if constexpr (MORE) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        mask_exponents(left_of(t + 1), en);
+      }
       slot = next;
       pair = next_pair;
     };
@@ -194,10 +187,25 @@ struct TileMxShared {
     });
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     mask_exponents(left_of(0), x);
-    for (int t = 0; t < chunks; t += 2) {
-      body(t, zero, x, y);
-      body(t + 1, one, y, x);
+    constexpr std::true_type yes;
+    constexpr std::false_type no;
+    int t = 0;
+    for (; t + 1 + STAGES < chunks; t += 2) {
+      body(t, zero, yes, yes, x, y);
+      body(t + 1, one, yes, yes, y, x);
     }
+    if constexpr (STAGES % 2 == 1)
+      if (t + STAGES < chunks) {
+        body(t, zero, yes, yes, x, y);
+        body(t + 1, one, no, yes, y, x);
+        t += 2;
+      }
+    for (; t + 2 < chunks; t += 2) {
+      body(t, zero, no, yes, x, y);
+      body(t + 1, one, no, yes, y, x);
+    }
+    body(t, zero, no, yes, x, y);
+    body(t + 1, one, no, no, y, x);
     wavek_wait_loads<0>();
     __syncthreads();   // the ring may be used for something else
   }
