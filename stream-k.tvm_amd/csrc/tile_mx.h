@@ -1,8 +1,8 @@
 // Products of microscaled 4-bit operands (rows of e2m1 pairs, a power of two for each 32 of K) on tiles whose waves stream K on their own:
 //   C[m][n] = sum over blocks b of 2^(sa[m][b] + sb[n][b] - 254) sum over the block's 32 k of A[m][k] B[n][k]
 // v_mfma_scale_f32_16x16x128_f8f6f4 takes both scales with the operands: lane (i, g) has 32 values of row i -- one block -- in 16 bytes and
-// the block's exponent in a byte of a register.  Which block of a chunk that is does not matter as long as both operands agree: lane group g
-// takes blocks 2 g (step 0) and 2 g + 1 (step 1) of a chunk's eight, so that its two exponents are neighbours in memory.
+// the block's exponent in a byte of a register.  Which block of a chunk that is does not matter as long as both operands agree: a lane group
+// takes blocks 2 g (step 0) and 2 g + 1 (step 1) of a chunk's eight (mx_group), so that its two exponents are neighbours in memory.
 //
 // The rings, the order of loads, reads and refills, the sums over the waves and the end are those of tile_wavek.h.  A wave takes two
 // neighbouring chunks of 256 values of an iteration's eight, and fetches their exponents together, 16 bytes to a row.  (Two bytes to
@@ -25,6 +25,10 @@ struct MxExponents {
     return make_rsrc_words(at, (uint32_t)(n > 0x7fffffff ? 0x7fffffff : n));
   }
 };
+// The pair of a chunk's pieces that lane group l / 16 takes, 2 g and 2 g + 1.  The 16 lanes that the LDS serves together in a 16-byte read are
+// rows 0-3 and 12-15 of one group and rows 4-11 of the next; pieces of groups 0 and 1, and 2 and 3, that differ in two bits of their
+// position keep these apart, pairs in the groups' order do not (half the cycles of the reads were conflicts).
+__device__ __forceinline__ int mx_group(int lane) { return (3 * (lane >> 4)) & 3; }
 struct MxArgs : WaveKArgs {      // (K, lda, ldb in pairs of bytes, four values)
   MxExponents ea, eb;            // of A's rows and of the weights'
 };
@@ -84,7 +88,7 @@ struct TileWaveKMx : WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> {
     const uint4v rsrc_ea = uniform_rsrc(a.ea.row((int64_t)pm * BM).rsrc()), rsrc_eb = uniform_rsrc(a.eb.row((int64_t)pn * BN).rsrc());
     // load e of a block: its rows 8 e .. 8 e + 7, lane's row lane / 8, piece p (16 bytes, 32 values) of row r of a block at position
     // p ^ ((r >> 1) & 7); exponents: lane's row, 16 bytes
-    const int row8 = lane >> 3, fi = lane & 15, fg = lane >> 4;
+    const int row8 = lane >> 3, fi = lane & 15, fg = mx_group(lane);
     uint32_t off_a[2], off_b[2];
     int kp[2];
 #pragma unroll

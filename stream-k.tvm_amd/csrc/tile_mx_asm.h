@@ -56,13 +56,14 @@ struct TileMxAsm : TileF16Asm<BF16 ? 6 : 5, false> {
     const uint32_t base = lds_address(P::lds());
     c.lds_wave = base + wave * 1024;
     c.lds_e = base + EXPONENTS_AT + wave * 1024;
-    // fragments: lane (r = l % 16, g = l / 16) reads row r of a 16-row block, chunk 2 g + kk at position (2 g + kk) ^ ((r >> 1) & 7): K-step 1
+    // fragments: lane (r = l % 16, g = mx_group(l)) reads row r of a 16-row block, chunk 2 g + kk at position (2 g + kk) ^ ((r >> 1) & 7): K-step 1
     // is K-step 0 with address bit 4 flipped
-    const uint32_t pos0 = (uint32_t)((2 * (lane >> 4)) ^ ((lane >> 1) & 7)) * 16;
+    const int g = mx_group(lane);
+    const uint32_t pos0 = (uint32_t)((2 * g) ^ ((lane >> 1) & 7)) * 16;
     c.ra0 = base + (uint32_t)(wm * P::WTM + (lane & 15)) * P::ROW_BYTES + pos0;
     c.rb0 = base + P::A_BYTES + (uint32_t)(wn * P::WTN + (lane & 15)) * P::ROW_BYTES + pos0;
-    c.rda = base + EXPONENTS_AT + (uint32_t)(wm * P::WTM + (lane & 15)) * 16 + 2 * (lane >> 4);
-    c.rdb = base + EXPONENTS_AT + P::BM * 16 + (uint32_t)(wn * P::WTN + (lane & 15)) * 16 + 2 * (lane >> 4);
+    c.rda = base + EXPONENTS_AT + (uint32_t)(wm * P::WTM + (lane & 15)) * 16 + 2 * g;
+    c.rdb = base + EXPONENTS_AT + P::BM * 16 + (uint32_t)(wn * P::WTN + (lane & 15)) * 16 + 2 * g;
     return c;
   }
   template <bool EARLY_ONLY>

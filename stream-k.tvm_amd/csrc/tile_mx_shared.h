@@ -66,7 +66,7 @@ struct TileMxShared {
     const uint4v rsrc_ea = uniform_rsrc(a.ea.row((int64_t)pm * BM).rsrc()), rsrc_eb = uniform_rsrc(a.eb.row((int64_t)pn * BN).rsrc());
     // load x of a chunk: rows 8 (wave + 4 x) .. + 7 of A's and then the weights', lane's row lane / 8; piece p (16 bytes, 32 values) of row r stands
     // at position p ^ ((r >> 1) & 7)
-    const int row8 = lane >> 3, fi = lane & 15, fg = lane >> 4, kp = ((lane & 7) ^ (4 * (wave & 1) + (row8 >> 1))) * 8;
+    const int row8 = lane >> 3, fi = lane & 15, fg = mx_group(lane), kp = ((lane & 7) ^ (4 * (wave & 1) + (row8 >> 1))) * 8;
     const uint32_t off_a = (uint32_t)row8 * lda_bytes + (uint32_t)kp * 2, off_b = (uint32_t)row8 * ldb_bytes + (uint32_t)kp * 2;
     const uint32_t off_ea = (uint32_t)(lane * a.ea.pitch), off_eb = (uint32_t)(lane * a.eb.pitch);
     const uint32_t ring = lds_address(smem) + (uint32_t)wave * 1024;
