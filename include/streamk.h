@@ -455,7 +455,9 @@ typedef struct sk_grouped {
   const void *bias, *scale_a, *scale_b;
   int64_t variant;                                /* the tiles: 0 by size; 1: 128 x 128; 2: 256 x 256 (K a multiple of
                                                      64, int8: 128); 3 to 6: 16 x 64, 32 x 64, 64 x 64, 64 x 128,
-                                                     whose waves stream K on their own (SK_LAYOUT_NN: only 64 x 64) */
+                                                     whose waves stream K on their own (SK_LAYOUT_NN: only 64 x 64).
+                                                     SK_MXFP4: K any; 1: one to a CU, 7: two to a CU; 6: waves share
+                                                     the tile; 8, 9: 16 x 16, 16 x 32, whose waves stream K */
   int64_t spin_limit;                             /* 0: 2^22 polls; negative: none (to test the way out) */
   int64_t scales_tiled;                           /* SK_MXFP4: not 0: scale_a and scale_b as sk_tile_mx_scales lays them out */
 } sk_grouped;
@@ -478,8 +480,8 @@ int sk_grouped_wgrad(const void *A, const void *B, const void *offsets, void *C,
  *
  * sk_gemm_grouped with dtype SK_MXFP4 multiplies them (SK_LAYOUT_NT): C[r] = activation(A[r] * B[e]^T + bias[e]), C in out_dtype, sums in
  * fp32, rounded once.  scale_a: [R] rows of K / 32 bytes, scale_b: [E, N] rows, 4-byte aligned; or, with scales_tiled, both tiled, 16-byte
- * aligned.  sk_mx_scales_tiled says whether a product (its shape and variant, on the current device) is to have them tiled; some refuse others
- * with SK_ERR_CONFIG.  offsets null and E = 1: all rows are the one expert's.  K, lda, ldb and expert_b are multiples of 32 values.
+ * aligned.  sk_mx_scales_tiled says whether a product (its shape and variant, on the current device) needs them tiled -- K is no multiple of 128, or
+ * the tiles are 256 x 256 --; it refuses others with SK_ERR_CONFIG, and any product takes them.  offsets null and E = 1: all rows are the one expert's.  K, lda, ldb and expert_b are multiples of 32 values.
  * The bytes of either array's scales tiled stay below 2 GiB.
  */
 int sk_quantize_mxfp4(const void *X, int dtype, int64_t M, int64_t K, int64_t ldx, void *Q, void *scales, void *stream);

@@ -47,7 +47,7 @@ extern "C" size_t sk_grouped_workspace_bytes(const sk_grouped *g) {
 extern "C" int sk_mx_scales_tiled(const sk_grouped *g) {
   GroupedShape h;
   if (!g || g->dtype != SK_MXFP4 || check_shape(g, &h) != SK_OK || sk_device_info(&h.cus, nullptr, nullptr) != SK_OK) return 0;
-  return mx_wants_tiled(h);
+  return mx_needs_tiled(h);
 }
 
 extern "C" int sk_gemm_grouped(const sk_grouped *g, void *ws, size_t ws_bytes, void *stream) {

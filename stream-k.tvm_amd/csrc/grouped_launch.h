@@ -15,7 +15,7 @@ struct GroupedShape {
   int variant;   // GroupedVariant
 };
 // which tiles (0: by the rule in kernels_grouped.hip; launches know theirs)
-enum GroupedVariant { GV_RULE = 0, GV_TILE128 = 1, GV_ASM256 = 2, GV_WAVEK16 = 3, GV_WAVEK32 = 4, GV_WAVEK64 = 5, GV_WAVEK64W = 6, GV_SHARED64 = 7, GV_SHARED256 = 8 };
+enum GroupedVariant { GV_RULE = 0, GV_TILE128 = 1, GV_ASM256 = 2, GV_WAVEK16 = 3, GV_WAVEK32 = 4, GV_WAVEK64 = 5, GV_WAVEK64W = 6, GV_MX128_2 = 7, GV_MX16X16 = 8, GV_MX16X32 = 9 };
 // the variant that a call takes (never GV_RULE; what a caller asked for, if anything), and the workspace it needs
 int grouped_variant(const GroupedShape &h);
 size_t grouped_workspace(const GroupedShape &h);
@@ -35,7 +35,7 @@ int launch_grouped_wavek(const GroupedArgs &g, const GroupedShape &h, const Work
 struct MxOperands;
 int mx_variant(const GroupedShape &h);
 size_t mx_workspace(const GroupedShape &h);
-bool mx_needs_tiled(const GroupedShape &h), mx_wants_tiled(const GroupedShape &h);   // the exponents' layout (tile_mx.h): that it takes, that it is fast with
+bool mx_needs_tiled(const GroupedShape &h);   // exponents (tile_mx.h)
 size_t mx_asm_workspace(int cus);           // kernels_mx_asm.hip
 int launch_mx_asm(const MxOperands &g, const GroupedShape &h, bool bf16, const Workspace &ws, hipStream_t s);
 int launch_mx(const MxOperands &g, const GroupedShape &h, bool bf16, const Workspace &ws, hipStream_t s);

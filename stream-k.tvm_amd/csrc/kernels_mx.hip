@@ -1,5 +1,7 @@
 // Products of microscaled 4-bit operands on tiles whose waves stream K on their own (tile_mx.h) or share the tile (tile_mx_shared.h), by expert
 // or of one matrix.
+#include <cmath>
+
 #include "grouped_launch.h"
 #include "grouped_mx.h"
 #include "kernel_table.h"
@@ -32,33 +34,76 @@ static int launch(const MxOperands &operands, const GroupedShape &h, const Works
   return (int)hipGetLastError();
 }
 
-template <bool BF16, int FM, int FN>
-using MxWaveK = MxWithZero<TileWaveKMx<BF16, FM, FN>>;
-template <bool BF16, int FM, int FN>
-using MxWaveK2 = MxWithZero<TileWaveKMx<BF16, FM, FN, 2>>;
+// (two tiles to a CU -- one stores or waits for its first rows while the other computes -- but for 64 x 64, whose registers fill it)
+template <bool BF16, int FM, int FN, int CTAS = 2>
+using MxWaveK = MxWithZero<TileWaveKMx<BF16, FM, FN, CTAS>>;
 
 // variant -> policy (BF16: C's type):  X(variant, policy)
-#define MX_TILES(X)                                                 \
-  X(GV_WAVEK16, MxWaveK<BF16, 1, 4>)                              \
-  X(GV_WAVEK32, MxWaveK<BF16, 2, 4>)                              \
-  X(GV_WAVEK64, MxWaveK<BF16, 4, 4>)                              \
-  X(10, MxWaveK2<BF16, 1, 4>) \
-  X(11, MxWaveK2<BF16, 2, 4>) \
-  X(12, MxWaveK2<BF16, 4, 4>) \
-  X(18, TileMxShared<BF16, 64, 64, 2, 2, 4, 2>) \
-  X(GV_SHARED256, TileMxShared<BF16, 256, 128, 2, 2, 3>) \
-  X(13, TileMxShared<BF16, 64, 128, 2, 2, 3, 2>) \
-  X(14, TileMxShared<BF16, 128, 64, 2, 2, 3, 2>) \
-  X(15, TileMxShared<BF16, 128, 128, 2, 2, 2, 2>) \
-  X(16, MxWaveK2<BF16, 1, 1>) \
-  X(17, MxWaveK2<BF16, 1, 2>) \
-   X(GV_SHARED64, TileMxShared<BF16, 64, 128, 2, 2, 4>)            \
-  X(GV_TILE128, TileMxShared<BF16, 128, 128, 2, 2, 4>)
+#define MX_TILES(X)                                        \
+  X(GV_MX16X16, MxWaveK<BF16, 1, 1>)                       \
+  X(GV_MX16X32, MxWaveK<BF16, 1, 2>)                       \
+  X(GV_WAVEK16, MxWaveK<BF16, 1, 4>)                       \
+  X(GV_WAVEK32, MxWaveK<BF16, 2, 4>)                       \
+  X(GV_WAVEK64, MxWaveK<BF16, 4, 4, 1>)                    \
+  X(GV_WAVEK64W, TileMxShared<BF16, 64, 128, 2, 2, 3, 2>)  \
+  X(GV_TILE128, TileMxShared<BF16, 128, 128, 2, 2, 4>)     \
+  X(GV_MX128_2, TileMxShared<BF16, 128, 128, 2, 2, 2, 2>)
+
+// The tile with the least estimated time, for rows that fall on the experts by chance.
+//     time = start + max(busy, memory) + hidden min(busy, memory), and where exponents are tiled 4 us and their bytes twice at 5 TB/s
+//   busy    iterations of `bk` values of the CU that has most -- whole rounds of tiles, and of those that are left their share and `cut`, or
+//           whole tiles where that is less (256 x 256: halves or quarters) -- each of `alone` or, of `per_cu` tiles at a time, `shared`;
+//           `end` for a tile's beginning and end, `join` for a cut
+//   memory  the operands of the experts that have rows, and C, once at 6 TB/s
+// Fitted to 843 products (none to 256 experts, 1 to 16384 rows, N 20 to 28672, K 256 to 16384; mean |log error| 8 %, 256 x 256: 13 %).  On 1100
+// others its choice takes 1.016 of the fastest tile's time on average, 1.37 at worst, and more than 1.1 in 43.
+struct MxCost {
+  int variant, bm, bn, bk, per_cu, cut;
+  double start, alone, shared, end, join, hidden;   // us (hidden: a part)
+};
+static const MxCost COSTS[9] = {{GV_MX16X16, 16, 16, 2048, 2, 3, 3.84, 0.22, 0.39, 1.16, 5.94, 0.25},
+                                {GV_MX16X32, 16, 32, 2048, 2, 3, 3.75, 0.57, 0.60, 1.14, 5.02, 0.30},
+                                {GV_WAVEK16, 16, 64, 2048, 2, 3, 3.72, 1.15, 1.03, 0.95, 3.90, 0.43},
+                                {GV_WAVEK32, 32, 64, 2048, 2, 3, 3.96, 1.50, 1.29, 1.04, 4.59, 0.40},
+                                {GV_WAVEK64, 64, 64, 2048, 1, 3, 2.99, 1.72, 0.00, 2.66, 4.73, 0.37},
+                                {GV_WAVEK64W, 64, 128, 512, 2, 8, 3.64, 0.64, 0.73, 1.68, 11.88, 0.42},
+                                {GV_MX128_2, 128, 128, 512, 2, 8, 5.09, 1.09, 1.06, 1.11, 18.08, 0.60},
+                                {GV_TILE128, 128, 128, 512, 1, 8, 3.54, 1.29, 0.00, 3.14, 13.70, 0.33},
+                                {GV_ASM256, 256, 256, 256, 1, 0, 5.28, 1.11, 0.00, 7.29, 19.39, 0.39}};
+static double estimate(const GroupedShape &h, double experts, const MxCost &c) {
+  const double rows = h.R / experts, high = h.E == 1 ? (double)((h.R + c.bm - 1) / c.bm) : experts * fmax(1.0, 0.5 + rows / c.bm);
+  const double tiles = ceil(high * (double)((h.N + c.bn - 1) / c.bn) - 1e-9), slots = (double)h.cus * c.per_cu;
+  const double ipt = (double)((h.K + c.bk - 1) / c.bk), whole = floor(tiles / slots), rest = tiles - whole * slots;
+  double iters = whole * ipt, at_once = whole > 0 ? c.per_cu : ceil(rest / h.cus);
+  bool joined = false;
+  if (rest > 0 && c.variant == GV_ASM256) {
+    const int parts = ipt < 64 ? 1 : (4 * rest <= h.cus ? 4 : (2 * rest <= h.cus ? 2 : 1));
+    joined = parts > 1;
+    iters += ipt / parts;
+  } else if (rest > 0) {
+    const double run = ceil(rest * ipt / slots);
+    joined = run + c.cut < ipt;
+    iters += joined ? run : ipt;
+    if (joined) at_once = c.per_cu;
+  }
+  const double busy = iters * fmax(c.alone, at_once * c.shared) + (whole + (rest > 0)) * c.end + (joined ? c.join : 0.0);
+  const double memory = ((experts * h.N + h.R) * h.K * (17.0 / 32) + 2.0 * h.R * h.N) / 6e6;
+  const bool tiled = c.variant == GV_ASM256 || h.K % 128 != 0;
+  return c.start + fmax(busy, memory) + c.hidden * fmin(busy, memory) + (tiled ? 4.0 + (double)(h.E * h.N + h.R) * h.K / 32 * 2 / 5e6 : 0.0);
+}
 int mx_variant(const GroupedShape &h) {
   if (h.variant != GV_RULE) return h.variant;
-  const int64_t rows = (h.R + h.E - 1) / h.E;
-  if (rows > 512) return GV_ASM256;
-  return rows <= 16 ? GV_WAVEK16 : (rows <= 32 ? GV_WAVEK32 : GV_WAVEK64);
+  const double experts = h.E == 1 ? 1.0 : h.E * (1 - pow(1 - 1.0 / h.E, (double)h.R));   // that have a row
+  int best = 0;
+  double least = 0;
+  for (const MxCost &c : COSTS) {
+    const double t = estimate(h, experts, c);
+    if (best == 0 || t < least) {
+      least = t;
+      best = c.variant;
+    }
+  }
+  return best;
 }
 size_t mx_workspace(const GroupedShape &h) {
   constexpr bool BF16 = false;
@@ -72,7 +117,6 @@ size_t mx_workspace(const GroupedShape &h) {
 }
 // (rows of exponents that are no words apart cannot be read 16 bytes at a time)
 bool mx_needs_tiled(const GroupedShape &h) { return h.K % 128 != 0 || mx_variant(h) == GV_ASM256; }
-bool mx_wants_tiled(const GroupedShape &h) { return mx_needs_tiled(h); }
 template <bool BF16, bool DENSE>
 static int launch_by_variant(const MxOperands &g, const GroupedShape &h, const Workspace &ws, hipStream_t s) {
 #define X(V, ...) \

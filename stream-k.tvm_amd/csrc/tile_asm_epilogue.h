@@ -62,7 +62,6 @@ struct AsmEnd {
     char *to = patch + (lane & 15) * STRIDE + (lane >> 4) * 16;
     const char *from = patch + (lane >> 3) * STRIDE + (lane & 7) * 32;
     const int col = col0 + (lane & 7) * 8;
-    const bool vec_ok = (ldc & 7) == 0 && (reinterpret_cast<uintptr_t>(C) & 15) == 0;
     float sa_lo = 0.f, sa_hi = 0.f;   // of rows row0 + lane and row0 + 64 + lane
     if constexpr (SCALED) {
       sa_lo = sa[min(row0 + lane, M - 1)];
@@ -92,9 +91,9 @@ struct AsmEnd {
         }
         if (row < M && c0 < N) {
           half_t *dst = C + (int64_t)row * ldc + c0;
-          if (vec_ok && c0 + 8 <= N) {
-            struct alignas(16) Eight { half4v h[2]; };
-            *reinterpret_cast<Eight *>(dst) = Eight{{h[0], h[1]}};
+          if (c0 + 8 <= N) {
+            struct Eight { half4v h[2]; };
+            reinterpret_cast<AnyPiece *>(dst)->v = __builtin_bit_cast(uint4v, Eight{{h[0], h[1]}});
           } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)

@@ -18,6 +18,11 @@ __device__ __forceinline__ half4v round4(floatx4 x) {
   return r.h;
 }
 
+// 16 bytes anywhere in a row of C: the hardware takes them at any multiple of 2 bytes.
+struct __attribute__((packed, aligned(2))) AnyPiece {
+  uint4v v;
+};
+
 // Stores FM x FN blocks of a wave, the first of which stands at (row0, col0) of C, through a patch of LDS of the wave's own
 // (16 rows of FN * 32 + 16 bytes: the padding keeps the 8-byte writes and the 16-byte reads on different banks), one row of
 // blocks at a time: 16-byte stores along rows of C instead of 8-byte ones down them.  block(ii, jj) gives the lane's four
@@ -29,7 +34,6 @@ struct BlockPatch {
   template <int I0 = 0, int I1 = FM, class Block>
   static __device__ __forceinline__ void store(half_t *C, int64_t ldc, int M, int N, int row0, int col0, char *patch, Block &&block) {
     const int lane = pin_here((int)threadIdx.x) & 63;
-    const bool vec_ok = (ldc & 7) == 0 && (reinterpret_cast<uintptr_t>(C) & 15) == 0;
     static_for<I0, I1>([&](auto bi) {
       constexpr int ii = decltype(bi)::value;
       static_for<0, FN>([&](auto bj) {
@@ -50,8 +54,8 @@ struct BlockPatch {
         const int idx = s * 64 + lane, row = row0 + 16 * ii + idx / PPR, col = col0 + (idx % PPR) * 8;
         if (row < M && col < N) {
           half_t *dst = C + (int64_t)row * ldc + col;
-          if (vec_ok && col + 8 <= N) {
-            *reinterpret_cast<uint4v *>(dst) = v[s];
+          if (col + 8 <= N) {
+            reinterpret_cast<AnyPiece *>(dst)->v = v[s];
           } else {
             union { uint4v q; half_t h[8]; } u;
             u.q = v[s];
