@@ -96,12 +96,14 @@ __device__ __forceinline__ void choose(const void *logits, int64_t ld, int t, in
 //   the k largest c among the open (without a bias: the k largest z, in whose order the scores are), ties to the lower number;
 //   weights = s of the chosen, divided by their sum if renormalised, times a factor.
 // Two experts' c may differ by less than 32 bits tell, and the choice is a whole number that two programs should agree on: scores, sums and
-// comparisons are in 64 bits.  The arithmetic is a few dozen 64-bit operations a logit; what bounds the kernel is the chain of reductions
-// over the wave that a token is, two for each group and one for each of the k.
+// comparisons are in 64 bits.  What bounds the kernel is its instructions, about a thousand to a token of 256 experts: some seventy for each
+// logit of a lane, fifty for each of the k, a hundred for the groups, which are all compared at once.  (One after the other, two
+// reductions over the wave to each: 16 tokens, 8 of 256 experts in 4 of 8 groups 18 us, so 13; 8192 tokens 71 us, with that and the scan of
+// counts below 28.)
 struct Scores {
   const float *bias;   // [E] or null
   double scale;
-  int groups, chosen_groups;
+  int groups, chosen_groups, size, lanes;   // size: of a group; lanes: that hold it (set by the launch)
   bool sigmoid, renormalize;
 };
 
@@ -112,11 +114,39 @@ __device__ __forceinline__ uint64_t order_key64(double c) {
   if (!(c > -__builtin_inf())) return 0;
   return b >> 63 ? ~b : b | 1ull << 63;
 }
-__device__ __forceinline__ double value_of_key(uint64_t k) { return __builtin_bit_cast(double, k >> 63 ? k ^ 1ull << 63 : ~k); }
+__device__ __forceinline__ double read_lane(double x, int lane) {   // (lane: uniform)
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// (no NaN comes here: the builtins make sure of a signalling one's result first, two more instructions each)
+__device__ __forceinline__ double larger(double a, double b) {
+  double r;
+  asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+__device__ __forceinline__ double smaller(double a, double b) {
+  double r;
+  asm("v_min_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+// (the order of wave_max_up_to: within rows of 16 lanes, then from row to row)
 __device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-  for (int d = 32; d > 0; d /= 2) x += __shfl_xor(x, d, 64);
-  return x;
+#define SK_SUM_STEP(CTRL, ROWS)                                                                                        \
+  {                                                                                                                    \
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);                                                                \
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, false);            \
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xf, false);    \
+    x += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);                                                          \
+  }
+  SK_SUM_STEP(0x111, 0xf);
+  SK_SUM_STEP(0x112, 0xf);
+  SK_SUM_STEP(0x114, 0xf);
+  SK_SUM_STEP(0x118, 0xf);
+  SK_SUM_STEP(0x142, 0xa);
+  SK_SUM_STEP(0x143, 0xc);
+#undef SK_SUM_STEP
+  return read_lane(x, 63);
 }
 // the largest of all lanes, and the first lane that has it: most often the upper halves tell
 __device__ __forceinline__ uint64_t wave_max64(uint64_t x, int &lane) {
@@ -147,15 +177,28 @@ __device__ __forceinline__ double chosen_share(const Scores &p, int expert, floa
   return expert < 0 ? 0. : s / all;
 }
 
-// As choose(): lane l holds the logits S l .. S l + S - 1, so that its first is the lowest.
+// The experts that a lane holds: S neighbours, of one group; a group has `lanes` lanes, neighbours too, so that the first of the lanes with
+// a score has the lowest number.
+struct Span {
+  int first, n, group, in_group;   // (in_group: number of the lane among its group's)
+  __device__ __forceinline__ Span(const Scores &p, int S) {
+    const int lane = threadIdx.x & 63;
+    group = (int)((unsigned)lane / (unsigned)p.lanes);
+    in_group = lane - group * p.lanes;
+    first = group * p.size + in_group * S;
+    n = group < p.groups ? min(S, p.size - in_group * S) : 0;
+  }
+};
+// As choose(), by scores.
 template <int EL, int S>
-__device__ __forceinline__ void choose_scored(const void *logits, int64_t ld, int t, int E, int k, const Scores &p, int &expert, float &weight) {
+__device__ __forceinline__ void choose_scored(const void *logits, int64_t ld, int t, int k, const Scores &p, const Span &own, int &expert, float &weight) {
+  constexpr double NONE = -__builtin_inf();
   const int lane = threadIdx.x & 63;
   float z[S];
   bool there[S];
 #pragma unroll
   for (int s = 0; s < S; ++s) {
-    z[s] = S * lane + s < E ? load_el<EL>(logits, t * ld + S * lane + s) : -__builtin_inff();
+    z[s] = s < own.n ? load_el<EL>(logits, t * ld + own.first + s) : -__builtin_inff();
     there[s] = z[s] > -__builtin_inff();   // (neither -inf nor NaN)
   }
   double most = 0., sum = 1.;
@@ -170,50 +213,49 @@ __device__ __forceinline__ void choose_scored(const void *logits, int64_t ld, in
     for (int s = 0; s < S; ++s) part += there[s] ? exp_from(z[s], most) : 0.;
     sum = wave_sum(part);
   }
-  uint64_t key[S];
+  double c[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) c[s] = (double)z[s];
   if (p.bias || p.groups > 1) {   // (uniform)
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      double c = p.sigmoid ? sigmoid64(z[s]) : exp_from(z[s], most) / sum;
-      if (p.bias && there[s]) c += (double)p.bias[S * lane + s];
-      key[s] = there[s] ? order_key64(c) : 0;
+      c[s] = p.sigmoid ? sigmoid64(z[s]) : exp_from(z[s], most) / sum;
+      if (p.bias && there[s]) c[s] += (double)p.bias[own.first + s];
+      there[s] = there[s] && c[s] > NONE;
     }
   }
+  bool open = true;
   if (p.groups > 1) {
-    const int size = (int)((unsigned)E / (unsigned)p.groups);
-    uint64_t mine = 0;   // lane g: group g's
-    for (int g = 0; g < p.groups; ++g) {
-      uint64_t first = 0, second = 0;
+    double first = NONE, second = NONE;
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        const bool in = (unsigned)(S * lane + s - g * size) < (unsigned)size;
-        const uint64_t x = in ? key[s] : 0;
-        second = max(second, min(first, x));
-        first = max(first, x);
+    for (int s = 0; s < S; ++s) {
+      const double x = there[s] ? c[s] : NONE;
+      second = larger(second, smaller(first, x));
+      first = larger(first, x);
+    }
+    // after step d a lane has those of the 2 d lanes from it on, as far as they are its group's
+    for (int d = 1; d < p.lanes; d *= 2) {
+      const double f = __shfl_down(first, d, 64), g = __shfl_down(second, d, 64);
+      if (own.in_group + d < p.lanes) {
+        second = larger(smaller(first, f), larger(second, g));
+        first = larger(first, f);
       }
-      int at;
-      const uint64_t a = wave_max64(first, at);
-      if (a == 0) continue;
-      int unused;
-      const uint64_t b = wave_max64(lane == at ? second : first, unused);
-      const double c = value_of_key(a) + (b ? value_of_key(b) : 0.);
-      if (lane == g) mine = order_key64(c);
     }
-    uint64_t open = 0;
-    for (int j = 0; j < p.chosen_groups; ++j) {
-      int at;
-      if (wave_max64(mine, at) == 0) break;
-      open |= 1ull << at;
-      if (lane == at) mine = 0;
+    const double both = __shfl(first + (second > NONE ? second : 0.), lane - own.in_group, 64);
+    int above = 0;   // groups in front of this lane's
+    for (int g = 0; g < p.groups; ++g) {
+      const double x = read_lane(both, g * p.lanes);
+      above += x > both || (x == both && g < own.group);
     }
+    open = above < p.chosen_groups;
+    if (!p.bias) {
 #pragma unroll
-    for (int s = 0; s < S; ++s)
-      if (!(open >> min(63u, (unsigned)(S * lane + s) / (unsigned)size) & 1)) key[s] = 0;
+      for (int s = 0; s < S; ++s) c[s] = (double)z[s];
+    }
   }
-  if (!p.bias) {
+  uint64_t key[S];
 #pragma unroll
-    for (int s = 0; s < S; ++s) key[s] = p.groups > 1 && key[s] == 0 ? 0 : (uint64_t)order_key(z[s]) << 32;
-  }
+  for (int s = 0; s < S; ++s) key[s] = there[s] && open ? order_key64(c[s]) : 0;
   expert = -1;
   for (int j = 0; j < k; ++j) {
     uint64_t best = key[0];
@@ -226,14 +268,14 @@ __device__ __forceinline__ void choose_scored(const void *logits, int64_t ld, in
       }
     int at;
     if (wave_max64(best, at) == 0) break;
-    const int e = __builtin_amdgcn_readlane(S * lane + which, at);
+    const int e = __builtin_amdgcn_readlane(own.first + which, at);
 #pragma unroll
     for (int s = 0; s < S; ++s)
-      if (S * lane + s == e) key[s] = 0;
+      if (own.first + s == e) key[s] = 0;
     if (lane == j) expert = e;
   }
-  const float own = expert >= 0 ? load_el<EL>(logits, t * ld + expert) : 0.f;
-  weight = (float)(p.scale * chosen_share(p, expert, own, most, sum));
+  const float chosen = expert >= 0 ? load_el<EL>(logits, t * ld + expert) : 0.f;
+  weight = (float)(p.scale * chosen_share(p, expert, chosen, most, sum));
 }
 
 struct RouteArgs {
@@ -242,14 +284,14 @@ struct RouteArgs {
   int T, E, k;
   float *weights;                          // [T, k]
   int *experts, *offsets, *order, *place;  // [T, k], [E + 1], [T k], [T k]
-  int *counts;                             // [blocks, E]: slots of a block's tokens by expert
+  int *counts, *totals;                    // [blocks, E]: slots of a block's tokens by expert, then those in front of the block; [E]: of all
   int tokens;                              // of a block
   Scores scores;
 };
 // SCORED: by scores, bias and groups
 template <int EL, int S, bool SCORED>
-__device__ __forceinline__ void choose_by(const RouteArgs &a, int t, int &expert, float &weight) {
-  if constexpr (SCORED) choose_scored<EL, S>(a.logits, a.ld, t, a.E, a.k, a.scores, expert, weight);
+__device__ __forceinline__ void choose_by(const RouteArgs &a, const Span &own, int t, int &expert, float &weight) {
+  if constexpr (SCORED) choose_scored<EL, S>(a.logits, a.ld, t, a.k, a.scores, own, expert, weight);
   else choose<EL, S>(a.logits, a.ld, t, a.E, a.k, expert, weight);
 }
 
@@ -322,18 +364,20 @@ __device__ __forceinline__ int scan_experts(int *total, int E, int *word) {
   return *word;
 }
 
-constexpr int FEW_TOKENS = 64, FEW_EXPERTS = 256, FEW_WAVES = 16;   // one workgroup does it all
-// (two launches take about 4 us more than one; 64 tokens are four for each wave of the workgroup)
+// One workgroup does it all.  A second launch takes 1 to 2 us more, more tokens than waves take turns: 16 tokens, 6 of 64 experts 5.5 us in
+// one and 7.3 in two, 64 tokens 10 and 7.8; by scores and groups, 8 of 256 experts, 12 tokens 11.5 and 11.7, 32 tokens 21 and 11.6.
+constexpr int FEW_TOKENS = 32, FEW_TOKENS_SCORED = 16, FEW_EXPERTS = 256, FEW_WAVES = 16;
 
 template <int EL, int S, bool SCORED>
 __global__ __launch_bounds__(64 * FEW_WAVES) void route_few_kernel(RouteArgs a) {
   extern __shared__ int lds[];
   int *experts = lds, *have = lds + FEW_TOKENS * a.k, *total = have + FEW_WAVES * a.E, *word = total + a.E;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = a.T * a.k;
+  const Span own(a.scores, S);
   for (int t = wave; t < a.T; t += FEW_WAVES) {
     int e;
     float w;
-    choose_by<EL, S, SCORED>(a, t, e, w);
+    choose_by<EL, S, SCORED>(a, own, t, e, w);
     if (lane < a.k) {
       experts[t * a.k + lane] = e;
       a.experts[t * a.k + lane] = e;
@@ -364,23 +408,23 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void route_few_kernel(RouteArgs a) 
   place_slots<FEW_WAVES>(a, experts, 0, n, have);
 }
 
-// More tokens: choice and counts by blocks, then places.  8192 tokens, 8 of 64 experts: 4 and 9 us (four waves a block for the choice 28 us:
-// a token is a chain of k reductions).
+// More tokens: choice and counts by blocks, sums of the counts in front of each block, then places.  8192 tokens, 8 of 256 experts: 17 us (every
+// block adding up the counts of all by itself 50), by scores 28.
 // (sixteen scores in 64 bits to a lane do not fit the registers of sixteen waves)
 constexpr int WAVES = 4;
 template <int S, bool SCORED>
-constexpr int choose_threads = SCORED && S == 16 ? 512 : 1024;
+constexpr int choose_threads = SCORED && S >= 16 ? 512 : 1024;
 template <int EL, int S, bool SCORED>
 __global__ __launch_bounds__((choose_threads<S, SCORED>)) void route_choose_kernel(RouteArgs a) {
   extern __shared__ int lds[];   // [E] counts of the block
-  constexpr int CHOOSE_WAVES = choose_threads<S, SCORED> / 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t0 = blockIdx.x * a.tokens, t1 = min(a.T, t0 + a.tokens);
-  for (int e = threadIdx.x; e < a.E; e += 64 * CHOOSE_WAVES) lds[e] = 0;
+  const Span own(a.scores, S);
+  for (int e = threadIdx.x; e < a.E; e += blockDim.x) lds[e] = 0;
   __syncthreads();
-  for (int t = t0 + wave; t < t1; t += CHOOSE_WAVES) {
+  for (int t = t0 + wave; t < t1; t += blockDim.x / 64) {
     int e;
     float w;
-    choose_by<EL, S, SCORED>(a, t, e, w);
+    choose_by<EL, S, SCORED>(a, own, t, e, w);
     if (lane < a.k) {
       a.experts[(int64_t)t * a.k + lane] = e;
       a.weights[(int64_t)t * a.k + lane] = w;
@@ -388,35 +432,60 @@ __global__ __launch_bounds__((choose_threads<S, SCORED>)) void route_choose_kern
     }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < a.E; e += 64 * CHOOSE_WAVES) a.counts[(int64_t)blockIdx.x * a.E + e] = lds[e];
+  for (int e = threadIdx.x; e < a.E; e += blockDim.x) a.counts[(int64_t)blockIdx.x * a.E + e] = lds[e];
 }
-// every block adds up the counts of all blocks, and of those in front of it, by itself
+// the counts of SCAN_EXPERTS experts: 64 threads to an expert, each with up to SHARE blocks
+constexpr int MOST_BLOCKS = 256, SHARE = MOST_BLOCKS / 64, SCAN_EXPERTS = 16;
+__global__ __launch_bounds__(64 * SCAN_EXPERTS) void route_scan_kernel(int *counts, int *totals, int blocks, int E) {
+  __shared__ int parts[64][SCAN_EXPERTS + 1];
+  const int e = blockIdx.x * SCAN_EXPERTS + threadIdx.x % SCAN_EXPERTS, share = threadIdx.x / SCAN_EXPERTS, b0 = share * SHARE;
+  int c[SHARE], sum = 0;
+#pragma unroll
+  for (int j = 0; j < SHARE; ++j) c[j] = e < E && b0 + j < blocks ? counts[(b0 + j) * E + e] : 0;
+#pragma unroll
+  for (int j = 0; j < SHARE; ++j) sum += c[j];
+  parts[share][threadIdx.x % SCAN_EXPERTS] = sum;
+  __syncthreads();
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = parts[lane][wave];
+  int x = part;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int y = __shfl_up(x, d, 64);
+    if (lane >= d) x += y;
+  }
+  parts[lane][wave] = x - part;
+  if (lane == 63 && blockIdx.x * SCAN_EXPERTS + wave < E) totals[blockIdx.x * SCAN_EXPERTS + wave] = x;
+  __syncthreads();
+  int before = parts[share][threadIdx.x % SCAN_EXPERTS];
+#pragma unroll
+  for (int j = 0; j < SHARE; ++j) {
+    if (e < E && b0 + j < blocks) counts[(b0 + j) * E + e] = before;
+    before += c[j];
+  }
+}
+// SCANNED: the kernel above has run; of a few blocks every block adds up the counts by itself
+template <bool SCANNED>
 __global__ __launch_bounds__(64 * WAVES) void route_place_kernel(RouteArgs a) {
   extern __shared__ int lds[];
   int *have = lds, *total = have + WAVES * a.E, *front = total + a.E, *word = front + a.E;
   const int t0 = blockIdx.x * a.tokens, t1 = min(a.T, t0 + a.tokens), slot0 = t0 * a.k, n = (t1 - t0) * a.k;
   const int *experts = a.experts + slot0;
-  for (int e = threadIdx.x; e < a.E; e += 64 * WAVES) total[e] = front[e] = 0;
-  __syncthreads();
-  // (SHARE threads to an expert, eight counts in flight each)
-  constexpr int SHARE = 16;
-  for (int i = threadIdx.x; i < SHARE * a.E; i += 64 * WAVES) {
-    const int e = (int)((unsigned)i % (unsigned)a.E), share = (int)((unsigned)i / (unsigned)a.E), blocks = (int)gridDim.x;
+  for (int e = threadIdx.x; e < a.E; e += 64 * WAVES) {
     int sum = 0, before = 0;
-    for (int b0 = share; b0 < blocks; b0 += 8 * SHARE) {
-      int c[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) c[j] = b0 + j * SHARE < blocks ? a.counts[(int64_t)(b0 + j * SHARE) * a.E + e] : 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        sum += c[j];
-        before += b0 + j * SHARE < (int)blockIdx.x ? c[j] : 0;
+    if constexpr (SCANNED) {
+      sum = a.totals[e];
+      before = a.counts[(int64_t)blockIdx.x * a.E + e];
+    } else {
+#pragma unroll 8
+      for (int b = 0; b < (int)gridDim.x; ++b) {
+        const int c = a.counts[(int64_t)b * a.E + e];
+        sum += c;
+        before += b < (int)blockIdx.x ? c : 0;
       }
     }
-    atomicAdd(&total[e], sum);
-    atomicAdd(&front[e], before);
+    total[e] = sum;
+    front[e] = before;
   }
-  __syncthreads();
   count_parts<WAVES>(experts, n, a.E, have);
   const int used = scan_experts(total, a.E, word);
   for (int e = threadIdx.x; e < a.E; e += 64 * WAVES) {
@@ -434,36 +503,54 @@ __global__ __launch_bounds__(64 * WAVES) void route_place_kernel(RouteArgs a) {
   place_slots<WAVES>(a, experts, slot0, n, have);
 }
 
-constexpr int MOST_BLOCKS = 256;   // (each of which reads all blocks' counts)
+constexpr int UNSCANNED_BLOCKS = 64;   // (8 of 256 experts, 128 tokens in 32 blocks: 10.7 us, with the scan 12.3; 256 tokens in 64: 12.1 and 12.4)
 int route_tokens(int64_t T) {
-  int64_t tokens = (T + MOST_BLOCKS - 1) / MOST_BLOCKS;
-  if (tokens < 16) tokens = 16;
-  return (int)tokens;
+  const int64_t tokens = (T + MOST_BLOCKS - 1) / MOST_BLOCKS;
+  return tokens < 4 ? 4 : (int)tokens;
 }
-int route_blocks(int64_t T, int64_t E) {
-  return T <= FEW_TOKENS && E <= FEW_EXPERTS ? 0 : (int)((T + route_tokens(T) - 1) / route_tokens(T));
+int route_blocks(int64_t T, int64_t E, bool scored) {
+  return T <= (scored ? FEW_TOKENS_SCORED : FEW_TOKENS) && E <= FEW_EXPERTS ? 0 : (int)((T + route_tokens(T) - 1) / route_tokens(T));
 }
 
 template <int EL, int S, bool SCORED>
-int launch_route(const RouteArgs &a, int blocks, hipStream_t s) {
-  if constexpr (64 * S <= FEW_EXPERTS) {
+int launch_route(RouteArgs a, int blocks, hipStream_t s) {
+  a.scores.lanes = (a.scores.size + S - 1) / S;
+  if constexpr (S <= FEW_EXPERTS / 64) {
     if (blocks == 0) {
       const size_t lds = sizeof(int) * (FEW_TOKENS * a.k + (FEW_WAVES + 1) * a.E + 1);
       hipLaunchKernelGGL((route_few_kernel<EL, S, SCORED>), dim3(1), dim3(64 * FEW_WAVES), lds, s, a);
       return (int)hipGetLastError();
     }
   }
-  hipLaunchKernelGGL((route_choose_kernel<EL, S, SCORED>), dim3(blocks), dim3((choose_threads<S, SCORED>)), sizeof(int) * a.E, s, a);
+  const int waves = a.tokens * 64 < choose_threads<S, SCORED> ? a.tokens : choose_threads<S, SCORED> / 64;
+  hipLaunchKernelGGL((route_choose_kernel<EL, S, SCORED>), dim3(blocks), dim3(64 * waves), sizeof(int) * a.E, s, a);
   if (hipGetLastError() != hipSuccess) return 1;
-  hipLaunchKernelGGL(route_place_kernel, dim3(blocks), dim3(64 * WAVES), sizeof(int) * ((WAVES + 2) * a.E + 1), s, a);
+  const size_t lds = sizeof(int) * ((WAVES + 2) * a.E + 1);
+  if (blocks <= UNSCANNED_BLOCKS) {
+    hipLaunchKernelGGL(route_place_kernel<false>, dim3(blocks), dim3(64 * WAVES), lds, s, a);
+    return (int)hipGetLastError();
+  }
+  hipLaunchKernelGGL(route_scan_kernel, dim3((a.E + SCAN_EXPERTS - 1) / SCAN_EXPERTS), dim3(64 * SCAN_EXPERTS), 0, s, a.counts, a.totals, blocks, a.E);
+  if (hipGetLastError() != hipSuccess) return 1;
+  hipLaunchKernelGGL(route_place_kernel<true>, dim3(blocks), dim3(64 * WAVES), lds, s, a);
   return (int)hipGetLastError();
 }
+// experts to a lane so that the groups' lanes, whole ones, are no more than a wave's (32 always do, for up to 64 groups and 1024 experts)
+bool fits_wave(const Scores &p, int S) { return p.groups * ((p.size + S - 1) / S) <= 64; }
 template <int EL, bool SCORED>
 int launch_route_of(const RouteArgs &a, int blocks, hipStream_t s) {
-  if (a.E <= 64) return launch_route<EL, 1, SCORED>(a, blocks, s);
-  if (a.E <= 128) return launch_route<EL, 2, SCORED>(a, blocks, s);
-  if (a.E <= 256) return launch_route<EL, 4, SCORED>(a, blocks, s);
-  return launch_route<EL, 16, SCORED>(a, blocks, s);
+  if constexpr (SCORED) {
+    if (fits_wave(a.scores, 1)) return launch_route<EL, 1, true>(a, blocks, s);
+    if (fits_wave(a.scores, 2)) return launch_route<EL, 2, true>(a, blocks, s);
+    if (fits_wave(a.scores, 4)) return launch_route<EL, 4, true>(a, blocks, s);
+    if (fits_wave(a.scores, 8)) return launch_route<EL, 8, true>(a, blocks, s);
+    return fits_wave(a.scores, 16) ? launch_route<EL, 16, true>(a, blocks, s) : launch_route<EL, 32, true>(a, blocks, s);
+  } else {
+    if (a.E <= 64) return launch_route<EL, 1, false>(a, blocks, s);
+    if (a.E <= 128) return launch_route<EL, 2, false>(a, blocks, s);
+    if (a.E <= 256) return launch_route<EL, 4, false>(a, blocks, s);
+    return launch_route<EL, 16, false>(a, blocks, s);
+  }
 }
 template <bool SCORED>
 int launch_route_by(int el, const RouteArgs &a, int blocks, hipStream_t s) {
@@ -735,7 +822,9 @@ int launched() { return hipGetLastError() == hipSuccess ? SK_OK : SK_ERR_LAUNCH;
 }  // namespace
 
 extern "C" size_t sk_route_workspace_bytes(int64_t T, int64_t E, int64_t k) {
-  return check_route_shape(T, E, k) == SK_OK ? sizeof(int) * (size_t)route_blocks(T, E) * (size_t)E : 0;
+  if (check_route_shape(T, E, k) != SK_OK) return 0;
+  const int blocks = route_blocks(T, E, true);   // (whichever takes more)
+  return blocks > 0 ? sizeof(int) * (size_t)(blocks + 1) * (size_t)E : 0;
 }
 
 // p: null for the plain route
@@ -745,11 +834,11 @@ static int route(const void *logits, int dtype, int64_t T, int64_t E, int64_t k,
   if (int rc = check_route_shape(T, E, k)) return rc;
   if (!logits || !weights || !experts || !offsets || !order || !place) return SK_ERR_NULL;
   if (ld < E) return SK_ERR_SHAPE;
-  const int blocks = route_blocks(T, E);
+  const int blocks = route_blocks(T, E, p != nullptr);
   if (ws_bytes < sk_route_workspace_bytes(T, E, k) || (blocks > 0 && !ws)) return SK_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(ws) & 3) return SK_ERR_ALIGN;
   RouteArgs a{logits, ld, (int)T, (int)E, (int)k, (float *)weights, (int *)experts, (int *)offsets, (int *)order, (int *)place, (int *)ws,
-              route_tokens(T), p ? *p : Scores{}};
+              (int *)ws + (int64_t)blocks * E, route_tokens(T), p ? *p : Scores{nullptr, 1., 1, 1, (int)E, 1, false, true}};
   const int herr = p ? launch_route_by<true>(element_of(dtype), a, blocks, (hipStream_t)stream) : launch_route_by<false>(element_of(dtype), a, blocks, (hipStream_t)stream);
   return herr == 0 ? SK_OK : SK_ERR_LAUNCH;
 }
@@ -762,7 +851,7 @@ static int check_scores(const sk_route_scores *s, int64_t E, int64_t k, Scores *
   if (reinterpret_cast<uintptr_t>(s->bias) & 3) return SK_ERR_ALIGN;
   // (all groups open: none is asked)
   const int groups = s->chosen_groups == s->groups ? 1 : s->groups;
-  *p = Scores{(const float *)s->bias, s->scale, groups, s->chosen_groups, s->scores == SK_SCORES_SIGMOID, s->renormalize != 0};
+  *p = Scores{(const float *)s->bias, s->scale, groups, s->chosen_groups, (int)(E / groups), 1, s->scores == SK_SCORES_SIGMOID, s->renormalize != 0};
   return SK_OK;
 }
 
