@@ -463,6 +463,7 @@ struct RouteExperts : torch::autograd::Function<RouteExperts> {
   static variable_list forward(AutogradContext *ctx, const Tensor &logits, int64_t k) {
     at::AutoDispatchBelowADInplaceOrView guard;
     static const auto route = OP(route_experts);
+    ctx->set_materialize_grads(false);
     const FiveTensors r = route.call(logits, k);
     ctx->save_for_backward({std::get<0>(r), std::get<1>(r)});
     ctx->saved_data["E"] = logits.size(1);
@@ -494,6 +495,7 @@ struct RouteScored : torch::autograd::Function<RouteScored> {
                                int64_t groups, int64_t chosen_groups, double scale) {
     at::AutoDispatchBelowADInplaceOrView guard;
     static const auto route = OP(route_scored);
+    ctx->set_materialize_grads(false);   // (of five results one has a gradient)
     const FiveTensors r = route.call(logits, k, bias, scores, renormalize, groups, chosen_groups, scale);
     ctx->save_for_backward({logits, std::get<1>(r)});
     ctx->saved_data["scores"] = scores;

@@ -438,6 +438,7 @@ class _RouteScored(torch.autograd.Function):
     def forward(ctx, logits, k, bias, *by):
         out = _ops.route_scored(logits, k, bias, *by)
         ctx.save_for_backward(logits, out[1])
+        ctx.set_materialize_grads(False)   # (of five results one has a gradient)
         ctx.by = by
         ctx.mark_non_differentiable(*out[1:])
         return tuple(out)
@@ -445,6 +446,8 @@ class _RouteScored(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dweights, *_):
+        if dweights is None:
+            return (None,) * 8
         return (_ops.route_scored_backward(*ctx.saved_tensors, dweights, *ctx.by), None, None, None, None, None, None, None)
 
 
