@@ -3,7 +3,8 @@
 // Value 2 i of a row is the low half of byte i.  A block with an infinity or a NaN has scale 255, the format's NaN, and codes 0.
 //
 // Both directions are one pass over memory, 16 bits and 17/32 of a byte a value, and what bounds them is that: a thread has eight values
-// (the conversions of this target take two at a time), four neighbours a block, whose maximum is two steps within a quad.
+// (the conversions of this target take two at a time), four neighbours a block, whose maximum is two steps within a quad.  28672 x 8192: 6.3
+// and 6.9 TB/s; of 32 bits 5.1 and 6.2 (a copy of 0.5 to 1 GB reaches 5.1 to 5.3).
 #include <hip/hip_runtime.h>
 
 #include "sk_device.h"
@@ -14,6 +15,9 @@ using namespace sk;
 
 namespace {
 
+// Arrays of values above half of the last cache's bytes (256 MB) pass it by, which leaves room for codes: 28672 x 8192 of 16 bits 104 us (5.7 TB/s),
+// so 94, back 105 and 86; 14336 rows 54 and 50, 51 and 45.  One that fits may be there: 4096 rows 16 us, past the caches 18.
+constexpr int64_t CACHED = (int64_t)128 << 20;
 constexpr int THREADS = 256, PIECES = 4;   // pieces of eight values that a thread has in flight
 enum { EL_F16 = 0, EL_BF16 = 1, EL_F32 = 2 };
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -79,7 +83,8 @@ __device__ __forceinline__ uint32_t encode(const Eight<EL> &v, uint32_t byte) {
 }
 
 // Rows of `pieces` pieces, `blocks` workgroups to a row.  (Rows without a gap between them are one row.)
-template <int EL, bool VEC>
+// VEC: 16-byte loads; PAST: past the caches
+template <int EL, bool VEC, bool PAST>
 __global__ __launch_bounds__(THREADS) void quantize_kernel(const char *X, int64_t rows, int64_t pieces, int64_t ldx_bytes, int64_t blocks, uint32_t *Q,
                                                            uint8_t *scales) {
   constexpr int BYTES = EL == EL_F32 ? 32 : 16;
@@ -93,7 +98,13 @@ __global__ __launch_bounds__(THREADS) void quantize_kernel(const char *X, int64_
     const int64_t p = first + i * THREADS;
     if (p >= pieces) continue;   // (a block's four threads all or none: pieces is a multiple of four)
     if constexpr (VEC) {
-      v[i] = *reinterpret_cast<const Eight<EL> *>(__builtin_assume_aligned(x + p * BYTES, 16));
+      const uint4v *from = reinterpret_cast<const uint4v *>(x + p * BYTES);
+#pragma unroll
+      for (int h = 0; h < BYTES / 16; ++h) {
+        const uint4v w = PAST ? __builtin_nontemporal_load(from + h) : from[h];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i].w[4 * h + e] = w[e];
+      }
     } else {
       typedef typename std::conditional<EL == EL_F32, uint32_t, uint16_t>::type Word;
       const Word *from = reinterpret_cast<const Word *>(x + p * BYTES);
@@ -112,21 +123,24 @@ __global__ __launch_bounds__(THREADS) void quantize_kernel(const char *X, int64_
   }
 }
 
-template <int EL>
-__global__ __launch_bounds__(THREADS) void dequantize_kernel(const uint32_t *Q, const uint8_t *scales, int64_t pieces, char *X, bool vec) {
-  const int64_t first = wide_block() * (THREADS * PIECES) + threadIdx.x;
-  uint32_t q[PIECES], byte[PIECES];
+// A thread has 16 bytes of values a piece: eight or, of 32 bits, four.
+template <int EL, bool VEC, bool PAST>
+__global__ __launch_bounds__(THREADS) void dequantize_kernel(const char *Q, const uint8_t *scales, int64_t pieces, char *X) {
+  constexpr int VALUES = EL == EL_F32 ? 4 : 8, MORE = PIECES * 8 / VALUES;
+  typedef typename std::conditional<EL == EL_F32, uint16_t, uint32_t>::type Codes;
+  const int64_t first = wide_block() * (THREADS * MORE) + threadIdx.x;
+  uint32_t q[MORE], byte[MORE];
 #pragma unroll
-  for (int i = 0; i < PIECES; ++i) {
+  for (int i = 0; i < MORE; ++i) {
     const int64_t p = first + i * THREADS;
     q[i] = byte[i] = 0;
     if (p < pieces) {
-      q[i] = Q[p];
-      byte[i] = scales[p >> 2];
+      q[i] = reinterpret_cast<const Codes *>(Q)[p];
+      byte[i] = scales[p / (32 / VALUES)];
     }
   }
 #pragma unroll
-  for (int i = 0; i < PIECES; ++i) {
+  for (int i = 0; i < MORE; ++i) {
     const int64_t p = first + i * THREADS;
     if (p >= pieces) continue;
     const float x = byte[i] == 255 ? __builtin_nanf("") : scale_value(byte[i]);
@@ -137,31 +151,25 @@ __global__ __launch_bounds__(THREADS) void dequantize_kernel(const uint32_t *Q, 
     };
     two(0, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i], 1.f, 0));
     two(2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i], 1.f, 1));
-    two(4, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i], 1.f, 2));
-    two(6, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i], 1.f, 3));
-    if constexpr (EL == EL_F32) {
-      float *to = reinterpret_cast<float *>(X) + 8 * p;
-      if (vec) {
-        *reinterpret_cast<floatx4 *>(to) = floatx4{f[0], f[1], f[2], f[3]};
-        *reinterpret_cast<floatx4 *>(to + 4) = floatx4{f[4], f[5], f[6], f[7]};
-      } else {
+    if constexpr (VALUES == 8) {
+      two(4, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i], 1.f, 2));
+      two(6, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i], 1.f, 3));
+    }
+    typedef typename std::conditional<EL == EL_F32, uint32_t, uint16_t>::type Word;
+    union { Word h[VALUES]; uint4v w; } o;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) to[e] = f[e];
-      }
+    for (int e = 0; e < VALUES; ++e) {
+      if constexpr (EL == EL_F32) o.h[e] = __builtin_bit_cast(uint32_t, f[e]);
+      else if constexpr (EL == EL_BF16) o.h[e] = __builtin_bit_cast(uint16_t, (__bf16)f[e]);
+      else o.h[e] = __builtin_bit_cast(uint16_t, (half_t)f[e]);
+    }
+    if constexpr (VEC) {
+      uint4v *to = reinterpret_cast<uint4v *>(X) + p;
+      if constexpr (PAST) __builtin_nontemporal_store(o.w, to);
+      else *to = o.w;
     } else {
-      union { uint16_t h[8]; uint4v w; } o;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if constexpr (EL == EL_BF16) o.h[e] = __builtin_bit_cast(uint16_t, (__bf16)f[e]);
-        else o.h[e] = __builtin_bit_cast(uint16_t, (half_t)f[e]);
-      }
-      uint16_t *to = reinterpret_cast<uint16_t *>(X) + 8 * p;
-      if (vec) {
-        *reinterpret_cast<uint4v *>(to) = o.w;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) to[e] = o.h[e];
-      }
+      for (int e = 0; e < VALUES; ++e) reinterpret_cast<Word *>(X)[VALUES * p + e] = o.h[e];
     }
   }
 }
@@ -226,19 +234,22 @@ extern "C" int sk_quantize_mxfp4(const void *X, int dtype, int64_t M, int64_t K,
     rows = 1;
   }
   const int64_t blocks = (pieces + THREADS * PIECES - 1) / (THREADS * PIECES);
-#define SK_QUANTIZE(EL, VEC)                                                                                                                       \
-  hipLaunchKernelGGL((quantize_kernel<EL, VEC>), wide_grid(rows * blocks), dim3(THREADS), 0, (hipStream_t)stream, (const char *)X, rows, pieces, \
+  const bool past = vec && M * K * size > CACHED;
+#define SK_QUANTIZE(EL, VEC, PAST)                                                                                                                \
+  hipLaunchKernelGGL((quantize_kernel<EL, VEC, PAST>), wide_grid(rows * blocks), dim3(THREADS), 0, (hipStream_t)stream, (const char *)X, rows, pieces, \
                      ldx * size, blocks, (uint32_t *)Q, (uint8_t *)scales)
+#define SK_QUANTIZE_OF(EL)                    \
+  if (past) SK_QUANTIZE(EL, true, true);      \
+  else if (vec) SK_QUANTIZE(EL, true, false); \
+  else SK_QUANTIZE(EL, false, false)
   if (el == EL_F16) {
-    if (vec) SK_QUANTIZE(EL_F16, true);
-    else SK_QUANTIZE(EL_F16, false);
+    SK_QUANTIZE_OF(EL_F16);
   } else if (el == EL_BF16) {
-    if (vec) SK_QUANTIZE(EL_BF16, true);
-    else SK_QUANTIZE(EL_BF16, false);
+    SK_QUANTIZE_OF(EL_BF16);
   } else {
-    if (vec) SK_QUANTIZE(EL_F32, true);
-    else SK_QUANTIZE(EL_F32, false);
+    SK_QUANTIZE_OF(EL_F32);
   }
+#undef SK_QUANTIZE_OF
 #undef SK_QUANTIZE
   return hipGetLastError() == hipSuccess ? SK_OK : SK_ERR_LAUNCH;
 }
@@ -249,15 +260,23 @@ extern "C" int sk_dequantize_mxfp4(const void *Q, const void *scales, int64_t M,
   if (!X || !Q || !scales) return SK_ERR_NULL;
   if (!fits(M, K)) return SK_ERR_SHAPE;
   if (K % 32 || misaligned(X, el == EL_F32 ? 3 : 1) || misaligned(Q, 3)) return SK_ERR_ALIGN;
-  const int64_t pieces = M * (K / 8);
-  const dim3 grid = wide_grid((pieces + THREADS * PIECES - 1) / (THREADS * PIECES));
-  const bool vec = !misaligned(X, 15);
-#define SK_DEQUANTIZE(EL)                                                                                                                     \
-  hipLaunchKernelGGL((dequantize_kernel<EL>), grid, dim3(THREADS), 0, (hipStream_t)stream, (const uint32_t *)Q, (const uint8_t *)scales, pieces, \
-                     (char *)X, vec)
-  if (el == EL_F16) SK_DEQUANTIZE(EL_F16);
-  else if (el == EL_BF16) SK_DEQUANTIZE(EL_BF16);
-  else SK_DEQUANTIZE(EL_F32);
+  const int64_t bytes = M * K * (el == EL_F32 ? 4 : 2), pieces = bytes / 16;
+  const dim3 grid = wide_grid((M * (K / 8) + THREADS * PIECES - 1) / (THREADS * PIECES));
+  const bool vec = !misaligned(X, 15), past = vec && bytes > CACHED;
+#define SK_DEQUANTIZE(EL, VEC, PAST) \
+  hipLaunchKernelGGL((dequantize_kernel<EL, VEC, PAST>), grid, dim3(THREADS), 0, (hipStream_t)stream, (const char *)Q, (const uint8_t *)scales, pieces, (char *)X)
+#define SK_DEQUANTIZE_OF(EL)                    \
+  if (past) SK_DEQUANTIZE(EL, true, true);      \
+  else if (vec) SK_DEQUANTIZE(EL, true, false); \
+  else SK_DEQUANTIZE(EL, false, false)
+  if (el == EL_F16) {
+    SK_DEQUANTIZE_OF(EL_F16);
+  } else if (el == EL_BF16) {
+    SK_DEQUANTIZE_OF(EL_BF16);
+  } else {
+    SK_DEQUANTIZE_OF(EL_F32);
+  }
+#undef SK_DEQUANTIZE_OF
 #undef SK_DEQUANTIZE
   return hipGetLastError() == hipSuccess ? SK_OK : SK_ERR_LAUNCH;
 }
