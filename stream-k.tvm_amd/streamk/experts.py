@@ -362,9 +362,8 @@ _SCORES = {"softmax": _lib.SK_SCORES_SOFTMAX, "sigmoid": _lib.SK_SCORES_SIGMOID}
 MAX_GROUPS = 64
 
 
-def _check_scored(logits, k, bias, scores, groups, chosen_groups, scale):
-    _on_device(logits, "logits", tuple(_LOGITS), 2)
-    E = logits.shape[1]
+def check_scores(E, k, scores, groups, chosen_groups, scale):
+    """Raises ValueError unless route_experts takes these with E experts."""
     if not 1 <= E <= MAX_EXPERTS or not 1 <= k <= min(E, MAX_CHOSEN):
         raise ValueError(f"1 to {MAX_EXPERTS} experts, of which 1 to {MAX_CHOSEN} are chosen: got {E} and k = {k}")
     if scores not in _SCORES:
@@ -375,6 +374,12 @@ def _check_scored(logits, k, bias, scores, groups, chosen_groups, scale):
         raise ValueError(f"{chosen_groups} groups of {E // groups} experts have no {k} to choose")
     if not math.isfinite(scale):
         raise ValueError(f"scale must be finite, got {scale}")
+
+
+def _check_scored(logits, k, bias, scores, groups, chosen_groups, scale):
+    _on_device(logits, "logits", tuple(_LOGITS), 2)
+    E = logits.shape[1]
+    check_scores(E, k, scores, groups, chosen_groups, scale)
     if bias is not None:
         _on_device(bias, "bias", (torch.float32,), 1)
         if bias.shape[0] != E or not bias.is_contiguous() or bias.device != logits.device:

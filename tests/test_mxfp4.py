@@ -123,6 +123,22 @@ def test_quantize_views(sk):
     assert torch.equal(sk.dequantize_mxfp4(q[5:], s[5:]).double().cpu(), values(q[5:], s[5:]).to(torch.bfloat16).double())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_arrays_larger_than_the_caches(sk, dtype):
+    # 16384 and more blocks of rows, and the same in parts that stay below
+    N, K = 8199, 8192
+    x = torch.randn(N, K, device="cuda", generator=torch.Generator("cuda").manual_seed(2)).to(TYPES[dtype])
+    x[8190:, 40] = math.inf
+    q, scale = sk.quantize_mxfp4(x)
+    back = sk.dequantize_mxfp4(q, scale, TYPES[dtype])
+    for lo in range(0, N, 1000):
+        part = slice(lo, lo + 1000)
+        pq, ps = sk.quantize_mxfp4(x[part])
+        assert torch.equal(q[part], pq) and torch.equal(scale[part], ps)
+        assert torch.equal(back[part].view(torch.uint8), sk.dequantize_mxfp4(pq, ps, TYPES[dtype]).view(torch.uint8))
+
+
 # ---- products ----
 def activate(x, name):
     return {None: lambda v: v, "relu": torch.relu, "silu": lambda v: v * torch.sigmoid(v),
