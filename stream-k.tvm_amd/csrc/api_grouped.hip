@@ -32,9 +32,7 @@ static int check_shape(const sk_grouped *g, GroupedShape *h) {
   if (g->lda / pairs * 2 * 256 >= (int64_t)1 << 31 || g->ldb / pairs * 2 * (nn ? g->K + 64 : 256) >= (int64_t)1 << 31 || g->ldc * 2 * 256 >= (int64_t)1 << 31)
     return SK_ERR_SHAPE;
   if (mx && !g->scales_tiled && g->K / 32 * 256 >= (int64_t)1 << 31) return SK_ERR_SHAPE;
-  if (mx && g->scales_tiled && (g->E * g->N > ((int64_t)1 << 27) - 256 || g->R > ((int64_t)1 << 27) - 256 ||
-                                (g->R > g->E * g->N ? g->R : g->E * g->N) * ((g->K + 511) / 512) >= (int64_t)1 << 27))
-    return SK_ERR_SHAPE;   // (offsets from a pair of chunks to another count in 32 bits)
+  if (mx && g->scales_tiled && !mx_tiled_fits(*h)) return SK_ERR_SHAPE;
   return SK_OK;
 }
 

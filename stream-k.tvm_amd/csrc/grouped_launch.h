@@ -36,6 +36,11 @@ struct MxOperands;
 int mx_variant(const GroupedShape &h);
 size_t mx_workspace(const GroupedShape &h);
 bool mx_needs_tiled(const GroupedShape &h);   // exponents (tile_mx.h)
+// tiled exponents of both operands are addressed with 32-bit offsets from a row's first
+static inline bool mx_tiled_fits(const GroupedShape &h) {
+  const int64_t b = h.E * h.N, most = (int64_t)1 << 27;
+  return b <= most - 256 && h.R <= most - 256 && (h.R > b ? h.R : b) * ((h.K + 511) / 512) < most;
+}
 size_t mx_asm_workspace(int cus);           // kernels_mx_asm.hip
 int launch_mx_asm(const MxOperands &g, const GroupedShape &h, bool bf16, const Workspace &ws, hipStream_t s);
 int launch_mx(const MxOperands &g, const GroupedShape &h, bool bf16, const Workspace &ws, hipStream_t s);

@@ -46,6 +46,8 @@ int64_t pitch(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1);
 bool is_ints(const Tensor &t, const Tensor &like, int64_t dim) {
   return t.scalar_type() == at::kInt && t.dim() == dim && t.is_contiguous() && t.device() == like.device();
 }
+// (of another device than the current one: the general implementations change to it)
+bool is_here(const Tensor &t) { return t.is_cuda() && t.get_device() == c10::hip::current_device(); }
 // a new tensor on the device of another one: the allocator's own entry, half a microsecond less than the dispatcher's
 Tensor fresh(const Tensor &like, at::IntArrayRef shape, at::ScalarType type) {
   return Tensor(at::detail::empty_cuda(shape, type, like.device(), std::nullopt));
@@ -129,7 +131,7 @@ bool grouped(const Tensor &rows, const Tensor &B, const Tensor &offsets, std::st
 std::tuple<Tensor, Tensor> quantize_mxfp4(const Tensor &x) {
   at::AutoDispatchBelowADInplaceOrView guard;
   const int dtype = dtype_of(x.scalar_type());
-  if (x.is_cuda() && dtype >= 0 && dtype != SK_I8 && x.dim() >= 1 && x.numel() > 0 && x.size(-1) % 32 == 0 && x.is_contiguous()) {
+  if (is_here(x) && dtype >= 0 && dtype != SK_I8 && x.dim() >= 1 && x.numel() > 0 && x.size(-1) % 32 == 0 && x.is_contiguous()) {
     const int64_t K = x.size(-1), M = x.numel() / K;
     c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
     shape.back() = K / 2;
@@ -143,7 +145,7 @@ std::tuple<Tensor, Tensor> quantize_mxfp4(const Tensor &x) {
 Tensor dequantize_mxfp4(const Tensor &q, const Tensor &scale, at::ScalarType dtype) {
   at::AutoDispatchBelowADInplaceOrView guard;
   const int to = dtype_of(dtype);
-  if (q.is_cuda() && q.scalar_type() == at::kByte && q.dim() >= 1 && q.numel() > 0 && q.size(-1) % 16 == 0 && q.is_contiguous() && aligned(q, 4) &&
+  if (is_here(q) && q.scalar_type() == at::kByte && q.dim() >= 1 && q.numel() > 0 && q.size(-1) % 16 == 0 && q.is_contiguous() && aligned(q, 4) &&
       scale.scalar_type() == at::kByte && scale.dim() == q.dim() && scale.is_contiguous() && scale.device() == q.device() && to >= 0 && to != SK_I8 &&
       scale.size(-1) * 16 == q.size(-1) && scale.sizes().slice(0, q.dim() - 1) == q.sizes().slice(0, q.dim() - 1)) {
     const int64_t K = 2 * q.size(-1);
@@ -158,7 +160,7 @@ Tensor dequantize_mxfp4(const Tensor &q, const Tensor &scale, at::ScalarType dty
 bool mx_product(const Tensor &A, const Tensor &B, const Tensor *offsets, MaybeType out_dtype, const Tensor *scale_a, const Tensor *scale_b, const Tensor *bias,
                 std::string_view activation, int64_t variant, Tensor &C) {
   const int64_t dims = offsets ? 3 : 2;
-  if (A.scalar_type() != at::kByte || B.scalar_type() != at::kByte || B.dim() != dims || B.device() != A.device() || !scale_a || !scale_b) return false;
+  if (!is_here(A) || A.scalar_type() != at::kByte || B.scalar_type() != at::kByte || B.dim() != dims || B.device() != A.device() || !scale_a || !scale_b) return false;
   if (!rows_in_place(A) && !one_row_in_place(A)) return false;
   const int64_t E = offsets ? B.size(0) : 1, N = B.size(-2), K = 2 * B.size(-1), R = A.size(0);
   if (E == 0 || N < 2 || K == 0 || K % 32 || 2 * A.size(1) != K || B.stride(-1) != 1) return false;
@@ -308,7 +310,7 @@ FiveTensors route_scored(const Tensor &logits, int64_t k, const MaybeTensor &bia
   at::AutoDispatchBelowADInplaceOrView guard;
   const int dtype = dtype_of(logits.scalar_type());
   sk_route_scores by;
-  if (logits.is_cuda() && dtype >= 0 && dtype != SK_I8 && logits.dim() == 2 && logits.size(0) > 0 && logits.is_contiguous() && k >= 1 && k <= logits.size(1) &&
+  if (is_here(logits) && dtype >= 0 && dtype != SK_I8 && logits.dim() == 2 && logits.size(0) > 0 && logits.is_contiguous() && k >= 1 && k <= logits.size(1) &&
       scores_of(scores, renormalize, groups, chosen_groups, scale, &by) &&
       (!bias.has_value() || (bias->scalar_type() == at::kFloat && bias->dim() == 1 && bias->size(0) == logits.size(1) && bias->is_contiguous() && bias->device() == logits.device()))) {
     const int64_t T = logits.size(0), E = logits.size(1);
@@ -329,7 +331,7 @@ Tensor route_scored_backward(const Tensor &logits, const Tensor &experts, const 
   at::AutoDispatchBelowADInplaceOrView guard;
   const int dtype = dtype_of(logits.scalar_type());
   sk_route_scores by;
-  if (logits.is_cuda() && dtype >= 0 && dtype != SK_I8 && logits.dim() == 2 && logits.size(0) > 0 && logits.is_contiguous() && is_ints(experts, logits, 2) &&
+  if (is_here(logits) && dtype >= 0 && dtype != SK_I8 && logits.dim() == 2 && logits.size(0) > 0 && logits.is_contiguous() && is_ints(experts, logits, 2) &&
       experts.size(0) == logits.size(0) && dweights.scalar_type() == at::kFloat && dweights.sizes() == experts.sizes() && dweights.is_contiguous() &&
       dweights.device() == logits.device() && scores_of(scores, renormalize, groups, chosen_groups, scale, &by)) {
     Tensor dlogits = fresh(logits, logits.sizes(), logits.scalar_type());

@@ -12,6 +12,7 @@ gradients, in native code (csrc/torch_ops_experts.cpp), which passes every other
 `<name>_general`; without the native library those and the autograd functions here stand in.
 """
 import ctypes
+import functools
 import math
 from typing import NamedTuple
 
@@ -32,6 +33,17 @@ def _operator(name, schema, run, fake):
         if suffix or not _NATIVE:
             ops._LIBRARY.impl(name + suffix, run, "CUDA")
     torch.library.register_fake(f"streamk::{name}", fake, lib=ops._LIBRARY)
+
+
+def _where_it_is(run):
+    """run, with the device of its first operand the current one."""
+    @functools.wraps(run)
+    def there(first, *args, **kwargs):
+        if not isinstance(first, torch.Tensor) or not first.is_cuda or first.device.index == torch.cuda.current_device():
+            return run(first, *args, **kwargs)
+        with torch.cuda.device(first.device):
+            return run(first, *args, **kwargs)
+    return there
 
 
 def _no_tangent(what, *operands):
@@ -90,6 +102,7 @@ def _exponents(t, name, shape, device):
     return t
 
 
+@_where_it_is
 def _mx_product(A, B, offsets, scale_a, scale_b, out_dtype, bias, activation, variant, out):
     """offsets None: one matrix, B [N, K / 2]."""
     _on_device(A, "A", (torch.uint8,), 2)
@@ -395,6 +408,7 @@ def _logit_rows(logits):
     return logits.contiguous() if logits.stride(1) != 1 and logits.shape[1] > 1 or logits.stride(0) < logits.shape[1] else logits
 
 
+@_where_it_is
 def _route_scored(logits, k, bias, scores, renormalize, groups, chosen_groups, scale):
     _check_scored(logits, k, bias, scores, groups, chosen_groups, scale)
     logits = _logit_rows(logits)
@@ -414,6 +428,7 @@ def _route_scored(logits, k, bias, scores, renormalize, groups, chosen_groups, s
     return weights, experts, offsets, order, place
 
 
+@_where_it_is
 def _route_scored_backward(logits, experts, dweights, scores, renormalize, groups, chosen_groups, scale):
     k = experts.shape[1]
     _check_scored(logits, k, None, scores, groups, chosen_groups, scale)

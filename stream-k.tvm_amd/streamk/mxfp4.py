@@ -12,6 +12,7 @@ from . import _lib, experts, ops
 _FLOATS = {torch.float16: _lib.SK_F16, torch.bfloat16: _lib.SK_BF16, torch.float32: _lib.SK_F32}
 
 
+@experts._where_it_is
 def _quantize(x):
     if not isinstance(x, torch.Tensor) or x.dtype not in _FLOATS:
         raise TypeError("x must be a float16, bfloat16 or float32 tensor")
@@ -33,6 +34,7 @@ def _quantize(x):
     return q, scale
 
 
+@experts._where_it_is
 def _dequantize(q, scale, dtype):
     if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dtype != torch.uint8:
         raise TypeError("q must be a CUDA/HIP tensor of bytes (uint8)")

@@ -366,6 +366,38 @@ def test_another_stream_and_a_graph(sk, M, N, K):
 
 
 @pytest.mark.gpu
+def test_beyond_four_gigabytes(sk):
+    # weights of 40 experts, 5.4e9 bytes, of which the first and the last have rows
+    E, N, K, g = 40, 16384, 16384, torch.Generator("cuda").manual_seed(3)
+    b = torch.empty(E, N, K // 2, dtype=torch.uint8, device="cuda").random_(generator=g)
+    sb = torch.randint(120, 127, (E, N, K // 32), dtype=torch.uint8, device="cuda", generator=g)
+    a, sa, va = operand(30, K, 9)
+    offsets = offsets_of([14] + [0] * (E - 2) + [16])
+    for variant in (0, 1, 2, 3, 5, 8):
+        C = sk.streamk_grouped(a, b, offsets, scale_a=sa, scale_b=sb, out_dtype=torch.bfloat16, variant=variant)
+        for e, r in ((0, slice(0, 14)), (E - 1, slice(14, 30))):
+            n = slice(N - 100, N)
+            vb = values(b[e, n], sb[e, n]).cuda()
+            assert_near(C[r, n], va[r] @ vb.T, K, va[r].abs() @ vb.abs().T)
+    del b, sb
+    # rows: 4.9e9 bytes of A, 4.9e9 values and more of x
+    M, K = 300000, 32768
+    a = torch.empty(M, K // 2, dtype=torch.uint8, device="cuda").random_(generator=g)
+    sa = torch.randint(120, 127, (M, K // 32), dtype=torch.uint8, device="cuda", generator=g)
+    b, sb, vb = operand(70, K, 10)
+    last = slice(M - 50, M)
+    va = values(a[last], sa[last]).cuda()
+    for variant in (0, 2, 5, 6):
+        C = sk.streamk_mxfp4(a, b, sa, sb, out_dtype=torch.bfloat16, variant=variant)
+        assert_near(C[last], va @ vb.T, K, va.abs() @ vb.abs().T)
+    x = sk.dequantize_mxfp4(a, sa)
+    assert torch.equal(x[last], sk.dequantize_mxfp4(a[last], sa[last]))
+    q, scale = sk.quantize_mxfp4(x)
+    want = sk.quantize_mxfp4(x[last])
+    assert torch.equal(q[last], want[0]) and torch.equal(scale[last], want[1])
+
+
+@pytest.mark.gpu
 def test_wrong_operands_are_refused(sk):
     a, sa, _ = operand(6, 64, 1)
     b, sb, _ = operand((3, 40), 64, 2)
