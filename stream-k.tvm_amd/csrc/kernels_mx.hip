@@ -35,41 +35,47 @@ static int launch(const MxOperands &operands, const GroupedShape &h, const Works
 }
 
 // (two tiles to a CU -- one stores or waits for its first rows while the other computes -- but for 64 x 64, whose registers fill it)
-template <bool BF16, int FM, int FN, int CTAS = 2>
-using MxWaveK = MxWithZero<TileWaveKMx<BF16, FM, FN, CTAS>>;
+template <bool BF16, int FM, int FN, bool WORDS, int CTAS = 2>
+using MxWaveK = MxWithZero<TileWaveKMx<BF16, FM, FN, CTAS, WORDS>>;
 
-// variant -> policy (BF16: C's type):  X(variant, policy)
-#define MX_TILES(X)                                        \
-  X(GV_MX16X16, MxWaveK<BF16, 1, 1>)                       \
-  X(GV_MX16X32, MxWaveK<BF16, 1, 2>)                       \
-  X(GV_WAVEK16, MxWaveK<BF16, 1, 4>)                       \
-  X(GV_WAVEK32, MxWaveK<BF16, 2, 4>)                       \
-  X(GV_WAVEK64, MxWaveK<BF16, 4, 4, 1>)                    \
-  X(GV_WAVEK64W, TileMxShared<BF16, 64, 128, 2, 2, 3, 2>)  \
-  X(GV_TILE128, TileMxShared<BF16, 128, 128, 2, 2, 4>)     \
+// variant -> policy (BF16: C's type; WORDS: tile_mx.h):  X(variant, policy)
+#define MX_ROWS(X)                                            \
+  X(GV_MX16X16, MxWaveK<BF16, 1, 1, WORDS>)                   \
+  X(GV_MX16X32, MxWaveK<BF16, 1, 2, WORDS>)                   \
+  X(GV_WAVEK16, MxWaveK<BF16, 1, 4, WORDS>)                   \
+  X(GV_WAVEK32, MxWaveK<BF16, 2, 4, WORDS>)                   \
+  X(GV_WAVEK64, MxWaveK<BF16, 4, 4, WORDS, 1>)
+#define MX_TILES(X)                                           \
+  X(GV_WAVEK64W, TileMxShared<BF16, 64, 128, 2, 2, 3, 2>)     \
+  X(GV_TILE128, TileMxShared<BF16, 128, 128, 2, 2, 4, 1>)     \
   X(GV_MX128_2, TileMxShared<BF16, 128, 128, 2, 2, 2, 2>)
 
+// (rows of exponents that are no words apart cannot be read where these tiles read them)
+static bool takes_tiled(int64_t K, int variant) {
+  return variant == GV_ASM256 || (K % 128 != 0 && (variant == GV_TILE128 || variant == GV_MX128_2 || variant == GV_WAVEK64W));
+}
 // The tile with the least estimated time, for rows that fall on the experts by chance.
-//     time = start + max(busy, memory) + hidden min(busy, memory), and where exponents are tiled 4 us and their bytes twice at 5 TB/s
+//     time = start + max(busy, memory) + hidden min(busy, memory), and where exponents are tiled 3.5 us and their bytes twice at 4 TB/s
 //   busy    iterations of `bk` values of the CU that has most -- whole rounds of tiles, and of those that are left their share and `cut`, or
-//           whole tiles where that is less (256 x 256: halves or quarters) -- each of `alone` or, of `per_cu` tiles at a time, `shared`;
+//           whole tiles where that is less (256 x 256: halves or quarters) -- each of `alone` or, of `per_cu` tiles at a time, `shared`, and more
+//           by `astray` where rows do not begin at 128 bytes (at 64: half of it), so that a chunk's are in two lines;
 //           `end` for a tile's beginning and end, `join` for a cut
 //   memory  the operands of the experts that have rows, and C, once at 6 TB/s
-// Fitted to 843 products (none to 256 experts, 1 to 16384 rows, N 20 to 28672, K 256 to 16384; mean |log error| 8 %, 256 x 256: 13 %).  On 1100
-// others its choice takes 1.016 of the fastest tile's time on average, 1.37 at worst, and more than 1.1 in 43.
+// Fitted to 993 products (none to 256 experts, 1 to 16384 rows, N 20 to 28672, K 256 to 16384, of which half no multiples of 128; mean
+// |log error| 7 to 13 %).  On 1350 others its choice takes 1.022 of the fastest tile's time on average, 1.7 at worst, and more than 1.1 in 73.
 struct MxCost {
   int variant, bm, bn, bk, per_cu, cut;
-  double start, alone, shared, end, join, hidden;   // us (hidden: a part)
+  double start, alone, shared, end, join, hidden, astray;   // us (hidden, astray: parts)
 };
-static const MxCost COSTS[9] = {{GV_MX16X16, 16, 16, 2048, 2, 3, 3.84, 0.22, 0.39, 1.16, 5.94, 0.25},
-                                {GV_MX16X32, 16, 32, 2048, 2, 3, 3.75, 0.57, 0.60, 1.14, 5.02, 0.30},
-                                {GV_WAVEK16, 16, 64, 2048, 2, 3, 3.72, 1.15, 1.03, 0.95, 3.90, 0.43},
-                                {GV_WAVEK32, 32, 64, 2048, 2, 3, 3.96, 1.50, 1.29, 1.04, 4.59, 0.40},
-                                {GV_WAVEK64, 64, 64, 2048, 1, 3, 2.99, 1.72, 0.00, 2.66, 4.73, 0.37},
-                                {GV_WAVEK64W, 64, 128, 512, 2, 8, 3.64, 0.64, 0.73, 1.68, 11.88, 0.42},
-                                {GV_MX128_2, 128, 128, 512, 2, 8, 5.09, 1.09, 1.06, 1.11, 18.08, 0.60},
-                                {GV_TILE128, 128, 128, 512, 1, 8, 3.54, 1.29, 0.00, 3.14, 13.70, 0.33},
-                                {GV_ASM256, 256, 256, 256, 1, 0, 5.28, 1.11, 0.00, 7.29, 19.39, 0.39}};
+static const MxCost COSTS[9] = {{GV_MX16X16, 16, 16, 2048, 2, 3, 4.11, 0.45, 0.26, 1.36, 6.50, 0.26, 1.59},
+                                {GV_MX16X32, 16, 32, 2048, 2, 3, 3.98, 0.55, 0.37, 1.30, 5.43, 0.35, 1.82},
+                                {GV_WAVEK16, 16, 64, 2048, 2, 3, 4.10, 0.91, 0.67, 1.09, 4.32, 0.55, 1.54},
+                                {GV_WAVEK32, 32, 64, 2048, 2, 3, 4.31, 1.20, 0.90, 1.21, 4.59, 0.49, 1.27},
+                                {GV_WAVEK64, 64, 64, 2048, 1, 3, 3.71, 1.40, 0.00, 2.83, 4.66, 0.33, 1.04},
+                                {GV_WAVEK64W, 64, 128, 512, 2, 8, 3.48, 0.72, 0.71, 1.79, 11.82, 0.41, 0.13},
+                                {GV_MX128_2, 128, 128, 512, 2, 8, 4.77, 1.14, 1.03, 1.34, 18.03, 0.56, 0.11},
+                                {GV_TILE128, 128, 128, 512, 1, 8, 3.45, 1.26, 0.00, 3.20, 13.28, 0.34, 0.05},
+                                {GV_ASM256, 256, 256, 256, 1, 0, 3.95, 1.08, 0.00, 7.70, 18.06, 0.45, 0.22}};
 static double estimate(const GroupedShape &h, double experts, const MxCost &c) {
   const double rows = h.R / experts, high = h.E == 1 ? (double)((h.R + c.bm - 1) / c.bm) : experts * fmax(1.0, 0.5 + rows / c.bm);
   const double tiles = ceil(high * (double)((h.N + c.bn - 1) / c.bn) - 1e-9), slots = (double)h.cus * c.per_cu;
@@ -86,10 +92,11 @@ static double estimate(const GroupedShape &h, double experts, const MxCost &c) {
     iters += joined ? run : ipt;
     if (joined) at_once = c.per_cu;
   }
-  const double busy = iters * fmax(c.alone, at_once * c.shared) + (whole + (rest > 0)) * c.end + (joined ? c.join : 0.0);
+  const double astray = 1.0 + (h.K % 256 == 0 ? 0.0 : (h.K % 128 == 0 ? 0.5 : 1.0)) * c.astray;
+  const double busy = iters * fmax(c.alone, at_once * c.shared) * astray + (whole + (rest > 0)) * c.end + (joined ? c.join : 0.0);
   const double memory = ((experts * h.N + h.R) * h.K * (17.0 / 32) + 2.0 * h.R * h.N) / 6e6;
-  const bool tiled = c.variant == GV_ASM256 || h.K % 128 != 0;
-  return c.start + fmax(busy, memory) + c.hidden * fmin(busy, memory) + (tiled ? 4.0 + (double)(h.E * h.N + h.R) * h.K / 32 * 2 / 5e6 : 0.0);
+  const bool tiled = takes_tiled(h.K, c.variant);
+  return c.start + fmax(busy, memory) + c.hidden * fmin(busy, memory) + (tiled ? 3.5 + (double)(h.E * h.N + h.R) * h.K / 32 * 2 / 4e6 : 0.0);
 }
 int mx_variant(const GroupedShape &h) {
   if (h.variant != GV_RULE) return h.variant;
@@ -107,24 +114,33 @@ int mx_variant(const GroupedShape &h) {
   return best;
 }
 size_t mx_workspace(const GroupedShape &h) {
-  constexpr bool BF16 = false;
+  constexpr bool BF16 = false, WORDS = false;
   const int v = mx_variant(h);
   if (v == GV_ASM256) return mx_asm_workspace(h.cus);
 #define X(V, ...) \
   if (v == V) return (size_t)WS_PART_OFF + (size_t)2 * h.cus * __VA_ARGS__::CTAS_PER_CU * __VA_ARGS__::TILE_ELEMS * 4;
+  MX_ROWS(X)
   MX_TILES(X)
 #undef X
   return 0;
 }
-// (rows of exponents that are no words apart cannot be read 16 bytes at a time)
-bool mx_needs_tiled(const GroupedShape &h) { return h.K % 128 != 0 || mx_variant(h) == GV_ASM256; }
+bool mx_needs_tiled(const GroupedShape &h) { return takes_tiled(h.K, mx_variant(h)); }
+template <bool BF16, bool DENSE, bool WORDS>
+static int launch_rows(const MxOperands &g, const GroupedShape &h, const Workspace &ws, hipStream_t s) {
+#define X(V, ...) \
+  if (h.variant == V) return launch<__VA_ARGS__, DENSE>(g, h, ws, s);
+  MX_ROWS(X)
+#undef X
+  return (int)hipErrorNotSupported;
+}
 template <bool BF16, bool DENSE>
 static int launch_by_variant(const MxOperands &g, const GroupedShape &h, const Workspace &ws, hipStream_t s) {
 #define X(V, ...) \
   if (h.variant == V) return launch<__VA_ARGS__, DENSE>(g, h, ws, s);
   MX_TILES(X)
 #undef X
-  return (int)hipErrorNotSupported;
+  const bool words = ((g.ea.pitch | g.eb.pitch) & 3) == 0;   // (the arrays begin at words)
+  return words ? launch_rows<BF16, DENSE, true>(g, h, ws, s) : launch_rows<BF16, DENSE, false>(g, h, ws, s);
 }
 int launch_mx(const MxOperands &g, const GroupedShape &h, bool bf16, const Workspace &ws, hipStream_t s) {
   if (h.variant == GV_ASM256) return launch_mx_asm(g, h, bf16, ws, s);

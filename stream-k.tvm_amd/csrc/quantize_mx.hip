@@ -181,29 +181,42 @@ struct TileScales {
   uint8_t *to;
   int64_t rows;
 };
-template <bool VEC>
+struct __attribute__((packed)) AnyBytes { uint4v w; };   // (the hardware takes 16 bytes at any address)
 __global__ __launch_bounds__(THREADS) void tile_scales_kernel(TileScales a, TileScales b, int64_t blocks_a, int blocks) {
+  constexpr int EACH = 64 * 16 / THREADS;
   __shared__ uint4v part[64][17];   // [row][16 bytes], a column of padding
   const bool second = (int64_t)blockIdx.x >= blocks_a;
   const TileScales &t = second ? b : a;
   const int64_t row0 = ((int64_t)blockIdx.x - (second ? blocks_a : 0)) * 64;
   const int pieces = (blocks + 15) / 16, p0 = (int)blockIdx.y * 16;
-  for (int i = threadIdx.x; i < 64 * 16; i += THREADS) {
-    const int64_t row = row0 + i / 16;
-    const int p = p0 + i % 16;
-    union { uint8_t c[16]; uint4v w; } o;
-    o.w = uint4v{0, 0, 0, 0};
-    if (row < t.rows && p < pieces) {
-      const uint8_t *from = t.from + row * blocks + 16 * p;
-      if constexpr (VEC) {
-        o.w = *reinterpret_cast<const uint4v *>(from);
-      } else {
+  uint4v w[EACH];
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (16 * p + e < blocks) o.c[e] = from[e];
-      }
+  for (int q = 0; q < EACH; ++q) {
+    const int i = threadIdx.x + q * THREADS, p = p0 + i % 16, n = blocks - 16 * p;   // (n: bytes from here to the row's end)
+    const int64_t row = row0 + i / 16;
+    w[q] = uint4v{0, 0, 0, 0};
+    if (row >= t.rows || n <= 0) continue;
+    const uint8_t *from = t.from + row * blocks + 16 * p;
+    if (n >= 16 || row + 16 < t.rows) {   // (a row has a byte at least)
+      w[q] = reinterpret_cast<const AnyBytes *>(from)->w;
+    } else {
+      union { uint8_t c[16]; uint4v w; } o;
+      o.w = w[q];
+#pragma unroll
+      for (int e = 0; e < 15; ++e)
+        if (e < n) o.c[e] = from[e];
+      w[q] = o.w;
     }
-    part[i / 16][i % 16] = o.w;
+  }
+#pragma unroll
+  for (int q = 0; q < EACH; ++q) {
+    const int i = threadIdx.x + q * THREADS, n = blocks - 16 * (p0 + i % 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {   // (what is behind the row)
+      const int left = n - 4 * e;
+      w[q][e] &= left >= 4 ? ~0u : (left <= 0 ? 0u : (1u << (8 * left)) - 1);
+    }
+    part[i / 16][i % 16] = w[q];
   }
   __syncthreads();
   for (int i = threadIdx.x; i < 64 * 16; i += THREADS) {
@@ -289,9 +302,6 @@ extern "C" int sk_tile_mx_scales(const void *a, int64_t rows_a, void *tiled_a, c
   const dim3 grid((unsigned)all, (unsigned)((blocks + 255) / 256));
   if (grid.y > 65535) return SK_ERR_SHAPE;
   const TileScales ta{(const uint8_t *)a, (uint8_t *)tiled_a, rows_a}, tb{(const uint8_t *)b, (uint8_t *)tiled_b, rows_b};
-  if (blocks % 16 == 0 && !misaligned(a, 15) && !misaligned(b, 15))
-    hipLaunchKernelGGL((tile_scales_kernel<true>), grid, dim3(THREADS), 0, (hipStream_t)stream, ta, tb, blocks_a, (int)blocks);
-  else
-    hipLaunchKernelGGL((tile_scales_kernel<false>), grid, dim3(THREADS), 0, (hipStream_t)stream, ta, tb, blocks_a, (int)blocks);
+  hipLaunchKernelGGL(tile_scales_kernel, grid, dim3(THREADS), 0, (hipStream_t)stream, ta, tb, blocks_a, (int)blocks);
   return hipGetLastError() == hipSuccess ? SK_OK : SK_ERR_LAUNCH;
 }

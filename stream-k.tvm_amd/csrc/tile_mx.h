@@ -20,10 +20,13 @@ struct MxExponents {
   const uint8_t *at, *end;
   int pitch, step;
   __device__ __forceinline__ MxExponents row(int64_t r) const { return MxExponents{at + r * pitch, end, pitch, step}; }
+  // from the word that it begins in to the word that the array ends in; loads take whole words
   __device__ __forceinline__ uint4v rsrc() const {
-    const int64_t n = end - at;
-    return make_rsrc_words(at, (uint32_t)(n > 0x7fffffff ? 0x7fffffff : n));
+    const uint8_t *from = at - shift();
+    const int64_t n = (end - from + 3) & ~(int64_t)3;
+    return make_rsrc_words(from, (uint32_t)(n > 0x7ffffffc ? 0x7ffffffc : n));
   }
+  __device__ __forceinline__ int shift() const { return (int)(reinterpret_cast<uintptr_t>(at) & 3); }
 };
 // The pair of a chunk's pieces that lane group l / 16 takes, 2 g and 2 g + 1.  The 16 lanes that the LDS serves together in a 16-byte read are
 // rows 0-3 and 12-15 of one group and rows 4-11 of the next; pieces of groups 0 and 1, and 2 and 3, that differ in two bits of their
@@ -33,7 +36,9 @@ struct MxArgs : WaveKArgs {      // (K, lda, ldb in pairs of bytes, four values)
   MxExponents ea, eb;            // of A's rows and of the weights'
 };
 
-template <bool BF16_, int FM_, int FN_, int CTAS_ = 1>
+// WORDS: rows of exponents begin at words (K a multiple of 128, or tiled).  Others are fetched from the word that they begin in, 16 bytes for each
+// chunk, and read at their bytes: 3 to 9 % slower than two chunks' in one load, and rows that are laid out anew first cost 7 us and more.
+template <bool BF16_, int FM_, int FN_, int CTAS_, bool WORDS>
 struct TileWaveKMx : WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> {
   typedef WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> Base;
   typedef MxArgs Args;
@@ -44,7 +49,7 @@ struct TileWaveKMx : WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> {
   static constexpr int FM = FM_, FN = FN_, BM = Base::BM, BN = Base::BN, WAVES = Base::WAVES, NT = Base::NT, NB = Base::NB;
   static constexpr int KV = 64, BK = 2 * KV * WAVES;  // pairs of bytes: of a chunk, of an iteration
   static constexpr int L = FM + FN;                   // blocks of a chunk, of two loads each
-  static constexpr int CHUNK = L * 2048, PAIR = 2 * 1024;   // bytes: of a chunk, of the exponents of two (64 rows of A and of the weights)
+  static constexpr int CHUNK = L * 2048, EXPS = 2 * 1024, PAIR = WORDS ? EXPS : 2 * EXPS;   // bytes: of a chunk, of exponents in one load and of two chunks (64 rows of A and of the weights)
   static constexpr int MOST = 40 * 1024 / CTAS_;      // a wave's share of the LDS
   static constexpr int S = (MOST - 2 * PAIR) / CHUNK >= 3 ? 3 : (MOST - 2 * PAIR) / CHUNK, PAIRS = 2;   // chunks, pairs in the ring
   static constexpr int EXPONENTS = S * CHUNK, RING = EXPONENTS + PAIRS * PAIR, LDS_BYTES = WAVES * RING, LDS_TOTAL = LDS_BYTES;
@@ -54,7 +59,7 @@ struct TileWaveKMx : WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> {
   static constexpr int H = NB, HR = H == 1 ? 1 : H - (H + 3) / 4;  // of a phase, of those that have fragments read beside them
 
   // loads of a chunk of this parity, and of the `behind` chunks that follow one of parity P
-  static constexpr int loads(int parity) { return 2 * L + (parity == 0 ? 2 : 0); }
+  static constexpr int loads(int parity) { return 2 * L + (parity == 0 ? (WORDS ? 2 : 4) : 0); }
   static constexpr int loads_behind(int P, int behind) { return behind == 0 ? 0 : loads_behind(P, behind - 1) + loads((P + behind) & 1); }
   // a chunk of parity P behind which `left` more chunks of the segment follow
   template <int P>
@@ -97,7 +102,10 @@ struct TileWaveKMx : WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> {
       off_a[e] = (uint32_t)(8 * e + row8) * lda_bytes + (uint32_t)kp[e] * 2;
       off_b[e] = (uint32_t)(8 * e + row8) * ldb_bytes + (uint32_t)kp[e] * 2;
     }
-    const uint32_t off_ea = lane < BM ? (uint32_t)(lane * a.ea.pitch) : OOB_OFFSET, off_eb = lane < BN ? (uint32_t)(lane * a.eb.pitch) : OOB_OFFSET;
+    // (from the word that they begin in)
+    const int shift_a = WORDS ? 0 : a.ea.row((int64_t)pm * BM).shift(), shift_b = WORDS ? 0 : a.eb.row((int64_t)pn * BN).shift();
+    const uint32_t off_ea = lane < BM ? (uint32_t)(shift_a + lane * a.ea.pitch) & (WORDS ? ~0u : ~3u) : OOB_OFFSET;
+    const uint32_t off_eb = lane < BN ? (uint32_t)(shift_b + lane * a.eb.pitch) & (WORDS ? ~0u : ~3u) : OOB_OFFSET;
     const uint32_t ring = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_address(smem) + wave * RING);
     // one row of tiles: see rotation_of.  Several: the CTAs of an XCD share A as well as the weights and stay on the same K
     const int rot = a.M <= BM ? rotation_of(pn, n) : Base::start_of(a, pn, n);
@@ -122,11 +130,15 @@ struct TileWaveKMx : WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> {
       wavek_dma_16<l * 2048>(A ? rsrc_a : rsrc_b, q.base, whole || kp[0] < q.left ? (A ? off_a : off_b)[0] : OOB_OFFSET, rows);
       wavek_dma_16<l * 2048 + 1024>(A ? rsrc_a : rsrc_b, q.base, whole || kp[1] < q.left ? (A ? off_a : off_b)[1] : OOB_OFFSET, rows);
     };
-    // (the exponents of a row's end and of what lies behind it arrive together; see read_exponents)
+    // (the exponents of a row's end and of what lies behind it arrive together; see read_exponents.  WORDS: of the pair that a chunk is in)
     auto issue_exponents = [&](const Chunk &q) {
-      const int at = __builtin_amdgcn_readfirstlane((int)q.kbytes / 256), to = __builtin_amdgcn_readfirstlane((int)q.pair);
-      wavek_dma_16<0>(rsrc_ea, (uint32_t)to, q.left > 0 ? off_ea : OOB_OFFSET, (uint32_t)(at * a.ea.step));
-      wavek_dma_16<1024>(rsrc_eb, (uint32_t)to, q.left > 0 ? off_eb : OOB_OFFSET, (uint32_t)(at * a.eb.step));
+      const int at = __builtin_amdgcn_readfirstlane((int)q.kbytes / (WORDS ? 256 : 128)), to = __builtin_amdgcn_readfirstlane((int)q.pair);
+      const int at_a = WORDS ? at * a.ea.step : at * 8, at_b = WORDS ? at * a.eb.step : at * 8;
+      wavek_dma_16<0>(rsrc_ea, (uint32_t)to, q.left > 0 ? off_ea : OOB_OFFSET, (uint32_t)at_a);
+      wavek_dma_16<1024>(rsrc_eb, (uint32_t)to, q.left > 0 ? off_eb : OOB_OFFSET, (uint32_t)at_b);
+      if constexpr (WORDS) return;
+      wavek_dma_16<EXPS>(rsrc_ea, (uint32_t)to, q.left > 0 ? off_ea : OOB_OFFSET, (uint32_t)(at_a + 8));
+      wavek_dma_16<EXPS + 1024>(rsrc_eb, (uint32_t)to, q.left > 0 ? off_eb : OOB_OFFSET, (uint32_t)(at_b + 8));
     };
 #pragma unroll
     for (int t = 0; t < S; ++t)
@@ -139,13 +151,15 @@ struct TileWaveKMx : WaveKTile<BF16_ ? WK_BF16 : WK_F16, FM_, FN_> {
     // fragments: lane (i, g) takes piece 2 g + s of its row for step s
     const char *mine = smem + wave * RING;
     const char *rd0 = mine + fi * 128 + ((2 * fg) ^ ((fi >> 1) & 7)) * 16, *rd1 = mine + fi * 128 + ((2 * fg + 1) ^ ((fi >> 1) & 7)) * 16;
-    const char *rd_e = mine + EXPONENTS + fi * 16 + 2 * fg;
+    struct __attribute__((packed, aligned(WORDS ? 2 : 1))) Two { uint16_t e; };
+    const char *rd_ea = mine + EXPONENTS + fi * 16 + 2 * fg + (WORDS ? 0 : (shift_a + fi * a.ea.pitch) & 3);   // (the same for row fi + 16, ..)
+    const char *rd_eb = mine + EXPONENTS + 1024 + fi * 16 + 2 * fg + (WORDS ? 0 : (shift_b + fi * a.eb.pitch) & 3);
     constexpr int READS = 3 * L;
     int slot = 0, pair = 0;   // of the chunk that is read next
     // read r of a chunk of parity P: the fragments of step 0 and the exponents, block by block, then the fragments of step 1
     auto read = [&](auto ri, auto parity, Frags &f) {
       constexpr int r = decltype(ri)::value, what = r < 2 * L ? r % 2 : 2, b = r < 2 * L ? r / 2 : r - 2 * L;
-      if constexpr (what == 1) f.e[b] = *reinterpret_cast<const uint16_t *>(rd_e + pair * PAIR + (b < FM ? b * 256 : 1024 + (b - FM) * 256) + 8 * decltype(parity)::value);
+      if constexpr (what == 1) f.e[b] = reinterpret_cast<const Two *>((b < FM ? rd_ea : rd_eb) + pair * PAIR + (b < FM ? b : b - FM) * 256 + (WORDS ? 8 : EXPS) * decltype(parity)::value)->e;
       else f.v[b][what / 2] = *reinterpret_cast<const intx4 *>((what ? rd1 : rd0) + slot * CHUNK + b * 2048);
     };
     // the last chunk of K: blocks behind K are zeros, and their exponents, which are another row's, have to be numbers

@@ -15,7 +15,7 @@
 
 namespace sk {
 
-template <bool BF16_, int BM_, int BN_, int WM_, int WN_, int STAGES_, int CTAS_ = 1>
+template <bool BF16_, int BM_, int BN_, int WM_, int WN_, int STAGES_, int CTAS_>
 struct TileMxShared {
   typedef MxArgs Args;
   typedef int intx4 __attribute__((ext_vector_type(4)));

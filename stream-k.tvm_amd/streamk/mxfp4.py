@@ -95,8 +95,8 @@ def dequantize_mxfp4(q, scale, dtype=torch.bfloat16):
 def streamk_mxfp4(A, B, scale_a, scale_b, *, out_dtype=torch.float16, out=None, bias=None, activation=None, variant=0):
     """C = activation(A @ B.T + bias) for microscaled 4-bit A [M, K / 2] and B [N, K / 2] (uint8) with scale_a [M, K / 32] and scale_b
     [N, K / 32] (uint8), as quantize_mxfp4 makes them; K a multiple of 32.  C is float16 or bfloat16 (`out_dtype`, which bias shares),
-    summed in fp32 and rounded once.  Where K is no multiple of 128, or the tiles are 256 x 256, scales are laid out anew on
-    the way (sk_tile_mx_scales in streamk.h).  variant: which tiles run (sk_grouped in streamk.h); 0 lets the sizes decide."""
+    summed in fp32 and rounded once.  With more than some dozen rows and a K that is no multiple of 128, or hundreds of
+    rows, scales are laid out anew on the way (sk_tile_mx_scales in streamk.h).  variant: which tiles run (sk_grouped in streamk.h); 0 lets the sizes decide."""
     A, B, scale_a, scale_b = (experts._bytes(t) for t in (A, B, scale_a, scale_b))
     if out is None:
         return _gemm_mxfp4(A, B, scale_a, scale_b, out_dtype, bias, activation or "none", variant)
