@@ -13,8 +13,9 @@
 
 namespace sk {
 
-// P: the policy; BF16: C's type; EPI: -1 nothing, else bias and the activation of this number
-template <class P, bool SCALED, bool BF16, int EPI>
+// P: the policy; BF16: C's type; EPI: -1 nothing, else bias and the activation of this number; PAST: C past the caches (4-bit operands,
+// 4096 x 8192 x 8192 with bias and SiLU 133.9 us, so 130.8)
+template <class P, bool SCALED, bool BF16, int EPI, bool PAST = false>
 struct AsmEnd {
   static constexpr int STRIDE = P::PATCH_STRIDE;
   static_assert(STRIDE == 64 * 4 + 16 && P::FN == 8 && P::WTN == 128, "16 rows of 64 values and a pad against bank conflicts");
@@ -93,7 +94,9 @@ struct AsmEnd {
           half_t *dst = C + (int64_t)row * ldc + c0;
           if (c0 + 8 <= N) {
             struct Eight { half4v h[2]; };
-            reinterpret_cast<AnyPiece *>(dst)->v = __builtin_bit_cast(uint4v, Eight{{h[0], h[1]}});
+            const uint4v piece = __builtin_bit_cast(uint4v, Eight{{h[0], h[1]}});
+            if constexpr (PAST) __builtin_nontemporal_store(piece, reinterpret_cast<AnyPiece *>(dst));
+            else *reinterpret_cast<AnyPiece *>(dst) = piece;
           } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)

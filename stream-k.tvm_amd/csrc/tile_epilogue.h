@@ -19,9 +19,7 @@ __device__ __forceinline__ half4v round4(floatx4 x) {
 }
 
 // 16 bytes anywhere in a row of C: the hardware takes them at any multiple of 2 bytes.
-struct __attribute__((packed, aligned(2))) AnyPiece {
-  uint4v v;
-};
+typedef uint4v AnyPiece __attribute__((aligned(2)));
 
 // Stores FM x FN blocks of a wave, the first of which stands at (row0, col0) of C, through a patch of LDS of the wave's own
 // (16 rows of FN * 32 + 16 bytes: the padding keeps the 8-byte writes and the 16-byte reads on different banks), one row of
@@ -55,7 +53,7 @@ struct BlockPatch {
         if (row < M && col < N) {
           half_t *dst = C + (int64_t)row * ldc + col;
           if (col + 8 <= N) {
-            reinterpret_cast<AnyPiece *>(dst)->v = v[s];
+            *reinterpret_cast<AnyPiece *>(dst) = v[s];
           } else {
             union { uint4v q; half_t h[8]; } u;
             u.q = v[s];

@@ -111,7 +111,7 @@ struct TileMxAsm : TileF16Asm<BF16 ? 6 : 5, false> {
     }
     const int wave = threadIdx.x >> 6, row0 = pm * P::BM + (wave >> 1) * P::WTM, col0 = pn * P::BN + (wave & 1) * P::WTN;
     by_epilogue(epi, [&](auto e) {
-      AsmEnd<TileMxAsm, false, BF16, decltype(e)::value>::store(a.C, a.ldc, a.M, a.N, row0, col0, nullptr, nullptr, epi_bias(epi), 0, P::FM);
+      AsmEnd<TileMxAsm, false, BF16, decltype(e)::value, true>::store(a.C, a.ldc, a.M, a.N, row0, col0, nullptr, nullptr, epi_bias(epi), 0, P::FM);
     });
   }
 };
