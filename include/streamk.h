@@ -481,7 +481,8 @@ int sk_grouped_wgrad(const void *A, const void *B, const void *offsets, void *C,
  * sk_gemm_grouped with dtype SK_MXFP4 multiplies them (SK_LAYOUT_NT): C[r] = activation(A[r] * B[e]^T + bias[e]), C in out_dtype, sums in
  * fp32, rounded once.  scale_a: [R] rows of K / 32 bytes, scale_b: [E, N] rows, 4-byte aligned; or, with scales_tiled, both tiled, 16-byte
  * aligned.  sk_mx_scales_tiled says whether a product (its shape and variant, on the current device) needs them tiled -- the tiles are
- * 256 x 256, or of variants 1, 6 and 7 with a K that is no multiple of 128 --; it refuses others with SK_ERR_CONFIG, and any product takes them.  offsets null and E = 1: all rows are the one expert's.  K, lda, ldb and expert_b are multiples of 32 values.
+ * 256 x 256, or of variants 1, 6 and 7 with a K that is no multiple of 128 --; it refuses others with SK_ERR_CONFIG, and any product takes
+ * them.  offsets null and E = 1: all rows are the one expert's.  K, lda, ldb and expert_b are multiples of 32 values.
  * The bytes of either array's scales tiled stay below 2 GiB.
  */
 int sk_quantize_mxfp4(const void *X, int dtype, int64_t M, int64_t K, int64_t ldx, void *Q, void *scales, void *stream);

@@ -168,7 +168,7 @@ VARIANTS = (0, 1, 2, 3, 4, 5, 6, 7, 8, 9)
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("variant", VARIANTS)
-@pytest.mark.parametrize("M,N,K", [(1, 2, 32), (1, 64, 256), (5, 77, 96), (16, 128, 1024), (17, 129, 1056), (33, 520, 2080), (64, 64, 4096), (100, 1000, 512),
+@pytest.mark.parametrize("M,N,K", [(1, 1, 32), (5, 1, 2080), (1, 2, 32), (1, 64, 256), (5, 77, 96), (16, 128, 1024), (17, 129, 1056), (33, 520, 2080), (64, 64, 4096), (100, 1000, 512),
                                    (1, 4096, 4096), (130, 257, 8224), (300, 515, 1312), (260, 300, 16448),
                                    (40, 200, 2944), (50, 72, 5024), (70, 130, 2560), (3, 300, 2848)])
 def test_product(sk, variant, M, N, K):

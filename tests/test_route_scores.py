@@ -96,7 +96,8 @@ def bias_of(E, seed):
 @pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("with_bias", [False, True])
 @pytest.mark.parametrize("T,E,k,groups,chosen_groups", [(1, 1, 1, 1, 1), (1, 8, 2, 1, 1), (5, 8, 2, 4, 2), (64, 256, 8, 8, 4), (65, 64, 6, 8, 3), (3, 6, 3, 6, 3),
-                                                         (130, 160, 6, 8, 1), (17, 1024, 64, 64, 32), (70, 300, 7, 3, 2), (9, 384, 8, 1, 1), (200, 36, 5, 4, 4)])
+                                                         (130, 160, 6, 8, 1), (17, 1024, 64, 64, 32), (70, 300, 7, 3, 2), (9, 384, 8, 1, 1), (200, 36, 5, 4, 4),
+                                                         (40, 250, 8, 10, 4), (40, 680, 12, 40, 9), (33, 60, 5, 20, 7), (300, 96, 5, 3, 2), (1500, 24, 3, 3, 2)])
 def test_route_by_scores(sk, scores, with_bias, T, E, k, groups, chosen_groups):
     z, bias = logits_of(T, E, 7 * T + E, closed=0.3), bias_of(E, E) if with_bias else None
     for renormalize, scale in ((True, 2.5), (False, 1.0)):
