@@ -456,8 +456,8 @@ typedef struct sk_grouped {
   int64_t variant;                                /* the tiles: 0 by size; 1: 128 x 128; 2: 256 x 256 (K a multiple of
                                                      64, int8: 128); 3 to 6: 16 x 64, 32 x 64, 64 x 64, 64 x 128,
                                                      whose waves stream K on their own (SK_LAYOUT_NN: only 64 x 64).
-                                                     SK_MXFP4: K any; 1: one to a CU, 7: two to a CU; 6: waves share
-                                                     the tile; 8, 9: 16 x 16, 16 x 32, whose waves stream K */
+                                                     SK_MXFP4: K any; 1, 6: waves share the tile, and 7: 128 x 256;
+                                                     8, 9: 16 x 16, 16 x 32, whose waves stream K */
   int64_t spin_limit;                             /* 0: 2^22 polls; negative: none (to test the way out) */
   int64_t scales_tiled;                           /* SK_MXFP4: not 0: scale_a and scale_b as sk_tile_mx_scales lays them out */
 } sk_grouped;

@@ -15,7 +15,7 @@ struct GroupedShape {
   int variant;   // GroupedVariant
 };
 // which tiles (0: by the rule in kernels_grouped.hip; launches know theirs)
-enum GroupedVariant { GV_RULE = 0, GV_TILE128 = 1, GV_ASM256 = 2, GV_WAVEK16 = 3, GV_WAVEK32 = 4, GV_WAVEK64 = 5, GV_WAVEK64W = 6, GV_MX128_2 = 7, GV_MX16X16 = 8, GV_MX16X32 = 9 };
+enum GroupedVariant { GV_RULE = 0, GV_TILE128 = 1, GV_ASM256 = 2, GV_WAVEK16 = 3, GV_WAVEK32 = 4, GV_WAVEK64 = 5, GV_WAVEK64W = 6, GV_MX128X256 = 7, GV_MX16X16 = 8, GV_MX16X32 = 9 };
 // the variant that a call takes (never GV_RULE; what a caller asked for, if anything), and the workspace it needs
 int grouped_variant(const GroupedShape &h);
 size_t grouped_workspace(const GroupedShape &h);

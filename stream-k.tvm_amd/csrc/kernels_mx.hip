@@ -47,12 +47,13 @@ using MxWaveK = MxWithZero<TileWaveKMx<BF16, FM, FN, CTAS, WORDS>>;
   X(GV_WAVEK64, MxWaveK<BF16, 4, 4, WORDS, 1>)
 #define MX_TILES(X)                                           \
   X(GV_WAVEK64W, TileMxShared<BF16, 64, 128, 2, 2, 3, 2>)     \
-  X(GV_TILE128, TileMxShared<BF16, 128, 128, 2, 2, 4, 1>)     \
-  X(GV_MX128_2, TileMxShared<BF16, 128, 128, 2, 2, 2, 2>)
+  X(GV_TILE128, TileMxShared<BF16, 128, 128, 2, 2, 2, 2>)     \
+  X(GV_MX128X256, TileMxShared<BF16, 128, 256, 2, 4, 3, 1>)
 
 // (rows of exponents that are no words apart cannot be read where these tiles read them)
 static bool takes_tiled(int64_t K, int variant) {
-  return variant == GV_ASM256 || (K % 128 != 0 && (variant == GV_TILE128 || variant == GV_MX128_2 || variant == GV_WAVEK64W));
+  const bool shared = variant == GV_WAVEK64W || variant == GV_TILE128 || variant == GV_MX128X256;
+  return variant == GV_ASM256 || (K % 128 != 0 && shared);
 }
 // The tile with the least estimated time, for rows that fall on the experts by chance.
 //     time = start + max(busy, memory) + hidden min(busy, memory), and where exponents are tiled 3.5 us and their bytes twice at 4 TB/s
@@ -62,20 +63,20 @@ static bool takes_tiled(int64_t K, int variant) {
 //           `end` for a tile's beginning and end, `join` for a cut
 //   memory  the operands of the experts that have rows, and C, once at 6 TB/s
 // Fitted to 993 products (none to 256 experts, 1 to 16384 rows, N 20 to 28672, K 256 to 16384, of which half no multiples of 128; mean
-// |log error| 7 to 13 %).  On 1350 others its choice takes 1.022 of the fastest tile's time on average, 1.7 at worst, and more than 1.1 in 73.
+// |log error| 7 to 13 %).  On 1450 others its choice takes 1.025 of the fastest tile's time on average, 1.8 at worst, and more than 1.1 in 85.
 struct MxCost {
   int variant, bm, bn, bk, per_cu, cut;
   double start, alone, shared, end, join, hidden, astray;   // us (hidden, astray: parts)
 };
-static const MxCost COSTS[9] = {{GV_MX16X16, 16, 16, 2048, 2, 3, 4.11, 0.45, 0.26, 1.36, 6.50, 0.26, 1.59},
-                                {GV_MX16X32, 16, 32, 2048, 2, 3, 3.98, 0.55, 0.37, 1.30, 5.43, 0.35, 1.82},
-                                {GV_WAVEK16, 16, 64, 2048, 2, 3, 4.10, 0.91, 0.67, 1.09, 4.32, 0.55, 1.54},
-                                {GV_WAVEK32, 32, 64, 2048, 2, 3, 4.31, 1.20, 0.90, 1.21, 4.59, 0.49, 1.27},
-                                {GV_WAVEK64, 64, 64, 2048, 1, 3, 3.71, 1.40, 0.00, 2.83, 4.66, 0.33, 1.04},
-                                {GV_WAVEK64W, 64, 128, 512, 2, 8, 3.48, 0.72, 0.71, 1.79, 11.82, 0.41, 0.13},
-                                {GV_MX128_2, 128, 128, 512, 2, 8, 4.77, 1.14, 1.03, 1.34, 18.03, 0.56, 0.11},
-                                {GV_TILE128, 128, 128, 512, 1, 8, 3.45, 1.26, 0.00, 3.20, 13.28, 0.34, 0.05},
-                                {GV_ASM256, 256, 256, 256, 1, 0, 3.95, 1.08, 0.00, 7.70, 18.06, 0.45, 0.22}};
+static const MxCost COSTS[9] = {{GV_MX16X16, 16, 16, 2048, 2, 3, 4.07, 0.44, 0.25, 1.36, 6.50, 0.27, 1.61},
+                                {GV_MX16X32, 16, 32, 2048, 2, 3, 3.95, 0.54, 0.36, 1.32, 5.42, 0.34, 1.84},
+                                {GV_WAVEK16, 16, 64, 2048, 2, 3, 4.04, 0.89, 0.65, 1.14, 4.35, 0.56, 1.58},
+                                {GV_WAVEK32, 32, 64, 2048, 2, 3, 4.27, 1.21, 0.89, 1.22, 4.62, 0.50, 1.27},
+                                {GV_WAVEK64, 64, 64, 2048, 1, 3, 3.73, 1.40, 0.00, 2.80, 4.69, 0.32, 1.03},
+                                {GV_WAVEK64W, 64, 128, 512, 2, 8, 3.49, 0.67, 0.71, 1.75, 11.85, 0.42, 0.10},
+                                {GV_TILE128, 128, 128, 512, 2, 8, 4.68, 1.16, 1.06, 1.31, 17.84, 0.54, 0.09},
+                                {GV_MX128X256, 128, 256, 512, 1, 8, 3.61, 1.94, 0.00, 2.87, 20.00, 0.48, 0.12},
+                                {GV_ASM256, 256, 256, 256, 1, 0, 1.00, 1.01, 0.00, 11.12, 18.83, 0.56, 0.25}};
 static double estimate(const GroupedShape &h, double experts, const MxCost &c) {
   const double rows = h.R / experts, high = h.E == 1 ? (double)((h.R + c.bm - 1) / c.bm) : experts * fmax(1.0, 0.5 + rows / c.bm);
   const double tiles = ceil(high * (double)((h.N + c.bn - 1) / c.bn) - 1e-9), slots = (double)h.cus * c.per_cu;

@@ -1,10 +1,13 @@
-// Microscaled 4-bit products (tile_mx.h) on tiles that a CTA's four waves share: WM x WN waves, each with its part of the tile, operands through
+// Microscaled 4-bit products (tile_mx.h) on tiles that a CTA's four or eight waves share: WM x WN waves, each with its part of the tile, operands through
 // a ring of LDS that all of them fill and read.
 //
-// A chunk is 256 values of K, 128 bytes a row; the exponents of two chunks come together, 16 bytes a row.  Each wave fetches a quarter of
-// a chunk's rows.  A chunk is multiplied in two steps of 128: beside the MFMAs of the first stand the reads of the second's fragments, then
+// A chunk is 256 values of K, 128 bytes a row; the exponents of two chunks come together, 16 bytes a row.  Each wave fetches its part
+// of a chunk's rows.  A chunk is multiplied in two steps of 128: beside the MFMAs of the first stand the reads of the second's fragments, then
 // one barrier -- everybody has read this chunk, and the next one has landed --, and beside those of the second the reads of the next
 // chunk's and the loads of the chunk that takes this one's place.  So STAGES - 1 chunks are on their way or waiting.
+//
+// Eight waves for 128 x 256: 1024 x 8192 x 8192 43 us where 128 x 128, two to a CU, take 55 and 256 x 256 47, 2048 x 4096 x 4096 24.5 and 25.3 (36).  One
+// 128 x 128 tile to a CU, in four stages: 58 us with four waves and 57 with eight.
 //
 // Against tile_mx.h's 64 x 64 tiles a 128 x 128 tile takes in half the bytes for each product, which is what bounds those with many
 // rows (a CU takes in 50 to 100 GB/s); against 256 x 256 tiles it fills the CUs from a quarter of the rows on.
@@ -22,14 +25,14 @@ struct TileMxShared {
   typedef int intx4 __attribute__((ext_vector_type(4)));
   typedef int intx8 __attribute__((ext_vector_type(8)));
   static constexpr bool COHERENT_PARTIALS = true, FIXUP_WORD_IN_LDS = true, BF16 = BF16_;
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = STAGES_, WAVES = 4, NT = 256;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = STAGES_, WAVES = WM_ * WN_, NT = 64 * WAVES;
   static constexpr int WTM = BM / WM, WTN = BN / WN, FM = WTM / 16, FN = WTN / 16, NB = FM * FN, TILE_ELEMS = BM * BN;
   static constexpr int KV = 64, BK = 2 * KV;                   // pairs of bytes: of a chunk, of an iteration
-  static constexpr int LW = (BM + BN) / 32;                    // a wave's loads of a chunk, 8 rows each
-  static constexpr int LE = (BM + BN + 255) / 256;             // and of two chunks' exponents, 64 rows each
-  static constexpr int CHUNK = (BM + BN) * 128, PAIR = LE * 256 * 16, PAIRS = (STAGES + 2) / 2;   // bytes; pairs of chunks whose exponents are kept
-  static constexpr int EXPONENTS = STAGES * CHUNK, LDS_BYTES = EXPONENTS + PAIRS * PAIR, CTAS_PER_CU = CTAS_, WAVES_PER_EU = CTAS_, CUT_COST = 8;
-  static_assert(WM * WN == WAVES && BM % 64 == 0 && BN % 64 == 0 && CTAS_ * LDS_BYTES <= 160 * 1024, "see above");
+  static constexpr int LW = (BM + BN) / (8 * WAVES);           // a wave's loads of a chunk, 8 rows each
+  static constexpr int LE = (BM + BN + NT - 1) / NT;           // and of two chunks' exponents, 64 rows each
+  static constexpr int CHUNK = (BM + BN) * 128, PAIR = (BM + BN) * 16, PAIRS = (STAGES + 2) / 2;   // bytes; pairs of chunks whose exponents are kept
+  static constexpr int EXPONENTS = STAGES * CHUNK, LDS_BYTES = EXPONENTS + PAIRS * PAIR, CTAS_PER_CU = CTAS_, WAVES_PER_EU = CTAS_ * WAVES / 4, CUT_COST = 8;
+  static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0 && CTAS_ * LDS_BYTES <= 160 * 1024, "see above");
   typedef BlockPatch<FM, FN> Patch;
   static_assert(WAVES * Patch::BYTES <= LDS_BYTES, "the patches fit the ring");
 
@@ -65,7 +68,7 @@ struct TileMxShared {
     const uint4v rsrc_a = uniform_rsrc(make_rsrc_words(a.A + (int64_t)pm * BM * a.lda, (uint32_t)rows_a * lda_bytes));
     const uint4v rsrc_b = uniform_rsrc(make_rsrc_words(a.B + (int64_t)pn * BN * a.ldb, (uint32_t)rows_b * ldb_bytes));
     const uint4v rsrc_ea = uniform_rsrc(a.ea.row((int64_t)pm * BM).rsrc()), rsrc_eb = uniform_rsrc(a.eb.row((int64_t)pn * BN).rsrc());
-    // load x of a chunk: rows 8 (wave + 4 x) .. + 7 of A's and then the weights', lane's row lane / 8; piece p (16 bytes, 32 values) of row r stands
+    // load x of a chunk: rows 8 (wave + WAVES x) .. + 7 of A's and then the weights', lane's row lane / 8; piece p (16 bytes, 32 values) of row r stands
     // at position p ^ ((r >> 1) & 7)
     const int row8 = lane >> 3, fi = lane & 15, fg = mx_group(lane), kp = ((lane & 7) ^ (4 * (wave & 1) + (row8 >> 1))) * 8;
     const uint32_t off_a = (uint32_t)row8 * lda_bytes + (uint32_t)kp * 2, off_b = (uint32_t)row8 * ldb_bytes + (uint32_t)kp * 2;
@@ -80,24 +83,24 @@ struct TileMxShared {
     auto chunk = [&](int t, int slot, int pair) {
       const int left = left_of(t);
       const uint32_t kbytes = (uint32_t)__builtin_amdgcn_readfirstlane(left > 0 ? (a.K - left) * 2 : 0);
-      return Chunk{kbytes, ring + (uint32_t)slot * CHUNK, ring + EXPONENTS + (uint32_t)pair * PAIR, left};
+      return Chunk{kbytes, ring + (uint32_t)slot * CHUNK, ring - (uint32_t)wave * 1024 + EXPONENTS + (uint32_t)pair * PAIR, left};
     };
     auto issue = [&](auto xi, const Chunk &q) {
       constexpr int x = decltype(xi)::value;
-      constexpr bool A = x < BM / 32;
-      const uint32_t rows = q.kbytes + (uint32_t)(8 * wave + 32 * (A ? x : x - BM / 32)) * (A ? lda_bytes : ldb_bytes);
-      wavek_dma_16<x * 4096>(A ? rsrc_a : rsrc_b, q.base, kp < q.left ? (A ? off_a : off_b) : OOB_OFFSET, rows);
+      constexpr bool A = x < BM / (8 * WAVES);
+      const uint32_t rows = q.kbytes + (uint32_t)(8 * (wave + WAVES * (A ? x : x - BM / (8 * WAVES)))) * (A ? lda_bytes : ldb_bytes);
+      wavek_dma_16<x * WAVES * 1024>(A ? rsrc_a : rsrc_b, q.base, kp < q.left ? (A ? off_a : off_b) : OOB_OFFSET, rows);
     };
-    // (rows 64 (wave + 4 y) ..; the exponents of a row's end and of what lies behind it arrive together, see mask_exponents)
+    // (rows 64 (wave + WAVES y) ..; the exponents of a row's end and of what lies behind it arrive together, see mask_exponents)
     auto issue_exponents = [&](const Chunk &q) {
       static_for<0, LE>([&](auto yi) {
         constexpr int y = decltype(yi)::value;
-        const int first = 64 * (wave + 4 * y);
-        const bool of_a = first < BM, any = first < BM + BN && q.left > 0;
+        const int first = min(64 * (wave + WAVES * y), BM + BN - 64);   // (waves behind the last rows fetch these again)
+        const bool of_a = first < BM, any = q.left > 0;
         const int at = (int)q.kbytes / 256;
         const uint32_t rows = (uint32_t)(any ? (of_a ? at * a.ea.step + first * a.ea.pitch : at * a.eb.step + (first - BM) * a.eb.pitch) : 0);
-        wavek_dma_16<y * 4096>(uniform_rsrc(of_a ? rsrc_ea : rsrc_eb), q.pair, any ? (of_a ? off_ea : off_eb) : OOB_OFFSET,
-                               (uint32_t)__builtin_amdgcn_readfirstlane((int)rows));
+        wavek_dma_16<0>(uniform_rsrc(of_a ? rsrc_ea : rsrc_eb), q.pair + (uint32_t)first * 16, any ? (of_a ? off_ea : off_eb) : OOB_OFFSET,
+                        (uint32_t)__builtin_amdgcn_readfirstlane((int)rows));
       });
     };
     static_for<0, STAGES>([&](auto t) {
