@@ -63,7 +63,7 @@ Low tiles (SK_TILE_ASM_*_LOW, _LOW_NN): at most 128 rows of A, 64 to a wave, who
 stand where blocks 0-3 of a full tile's waves do, so A has EARLY row groups only, and these are 32 consecutive rows of A each.  A
 block of the loop is 32 MFMAs with four loads (block 0) and eight (block 1); the loop's state rides with the reads at the top.  NN: B's row groups are split by K-step, as in the TN layout.
 
-Microscaled 4-bit operands (tile_mx_asm_gen.h, written with the argument `mx`; SK_TILE_ASM_LOOP_MX): the bytes travel as the 16-bit loop's, so that
+Microscaled 4-bit operands (tile_mx_asm_gen.h, written with the argument `mx`; SK_TILE_ASM_LOOP_MX, _LOW): the bytes travel as the 16-bit loop's, so that
 an iteration is 256 values of K and a block one v_mfma_scale_f32_16x16x128_f8f6f4 of 128 for each pair of fragments -- as many cycles as the
 16-bit MFMA of 32.  (With 32 x 32 x 64 instead, which a wave alone on its SIMD issues more easily, an iteration takes 1.69 us and not 1.57
 on random operands, where the power drawn sets the clock, and 1.00 and not 1.06 on zeros.)  Lane group g takes the 16-byte chunks 2 g (block 0) and 2 g + 1 (block 1) of a row, 32 values each, whose exponents
@@ -372,14 +372,17 @@ MX_RA1, MX_RB1, MX_RDA, MX_RDB, MX_TAIL = 124, 125, 126, 127, 122
 S_EL, S_EKA, S_EKB = 88, 89, 90
 
 
-def loop_text_mx():
+def loop_text_mx(low=False):
     """The 16-bit NT loop on microscaled 4-bit operands; see above.  %[tail]: 0x80000000 in the lanes whose chunk lies behind K in the
     last iteration, else 0; %[rea], %[reb], %[ve], %[eka], %[ekb], %[esa], %[esb], %[el]: descriptors, lane offset, offsets and LDS address (the
-    wave's 64 rows) of the exponents behind the first pair's, and the steps from pair to pair; %[rda], %[rdb]: where the lane reads the first ones."""
+    wave's 64 rows) of the exponents behind the first pair's, and the steps from pair to pair; %[rda], %[rdb]: where the lane reads the first ones.
+    low: of a tile of at most 128 rows, as in the 16-bit loop; %[vea]: the lane offset of A's exponents, the second wave row's from row 64 on."""
     L = []
     e = L.append
-    order = mfma_order()
-    early, late = early_groups(False), late_groups(False)
+    order = mfma_order(low)
+    early, late = early_groups(False, low), late_groups(False, low)
+    top, last, ld_last, rd_last = (4, 31, 30, 29) if low else (TOP, 63, LD_LAST, RD_LAST)
+    rows_a = 4 if low else 8           # 16-row blocks of A
 
     def exponents(p):
         return 88 if p == 0 else 104
@@ -397,22 +400,25 @@ def loop_text_mx():
 
     def read_exponents(p, which):      # for an iteration of parity p
         x = exponents(p) + (0 if which == "A" else 8)
-        return [([("E", which, i)], [f'"ds_read_u16 v{x + i}, v{MX_RDA if which == "A" else MX_RDB} offset:{i * 256 + 8 * p}']) for i in range(8)]
+        return [([("E", which, i)], [f'"ds_read_u16 v{x + i}, v{MX_RDA if which == "A" else MX_RDB} offset:{i * 256 + 8 * p}']) for i in range(rows_a if which == "A" else 8)]
 
     def early_reads(kk):
         return [read("A", 0, kk)] + [read("B", j, kk) for j in range(4)] + [read("A", i, kk) for i in range(1, 4)]
 
     def late_reads(kk):
-        return [read("B", j, kk) for j in range(4, 8)] + [read("A", i, kk) for i in range(4, 8)]
+        return [read("B", j, kk) for j in range(4, 8)] + [read("A", i, kk) for i in range(4, rows_a)]
 
     def load_groups(xs):
         groups = []
-        for pre, m0, ld in load_sequence(xs, False, f"v{VOA}", f"v{VOB}", None, f"s{S_LDS}", f"s{S_KA}", f"s{S_KB}"):
+        for pre, m0, ld in load_sequence(xs, False, f"v{VOA}", f"v{VOB}", None, f"s{S_LDS}", f"s{S_KA}", f"s{S_KB}", low=low):
             groups += [(None, pre + [m0]), (None, [ld])]
+        if low:     # (a load shares its gap with the address of the next one)
+            texts = [t for _, t in groups]
+            groups = [(None, texts[0])] + [(None, a + b) for a, b in zip(texts[1::2], texts[2::2])] + [(None, texts[-1])]
         return groups
 
     def load_exponents():              # of the next pair
-        return [(None, [f'"s_mov_b32 m0, s{S_EL}']), (None, [f'"buffer_load_dwordx4 %[ve], %[rea], s{S_EKA} offen lds', f'"s_add_u32 s{S_EKA}, s{S_EKA}, %[esa]']),
+        return [(None, [f'"s_mov_b32 m0, s{S_EL}']), (None, [f'"buffer_load_dwordx4 {"%[vea]" if low else "%[ve]"}, %[rea], s{S_EKA} offen lds', f'"s_add_u32 s{S_EKA}, s{S_EKA}, %[esa]']),
                 (None, [f'"s_add_u32 m0, s{S_EL}, 4096', f'"s_xor_b32 s{S_EL}, s{S_EL}, 0x2000']),
                 (None, [f'"buffer_load_dwordx4 %[ve], %[reb], s{S_EKB} offen lds', f'"s_add_u32 s{S_EKB}, s{S_EKB}, %[esb]'])]
 
@@ -434,11 +440,11 @@ def loop_text_mx():
             L.extend(texts)
             for t in tags or []:
                 tr.issue(t)
-        assert all(0 <= g <= 63 for g in plan), sorted(plan)
+        assert all(0 <= g <= last for g in plan), sorted(plan)
         L.extend(closing)
 
     # ---- entry, as in the 16-bit loop
-    zero_accumulators(L)
+    zero_accumulators(L, low)
     e(f'"s_mov_b32 s{S_IT}, 0')
     e(f'"s_xor_b32 s{S_LDS}, %[lds], 0x10000')
     e(f'"s_add_u32 s{S_KA}, %[ga0], 128')
@@ -463,26 +469,34 @@ def loop_text_mx():
     def body(p):
         # ---- block 0 (the exponents' address moves on with the pair)
         plan = dict(enumerate(late_reads(0)))
-        first = TOP
+        first = top
         if p == 1:
             plan[first] = (None, flip(f"v{MX_RDA}", "0x2000")[1] + flip(f"v{MX_RDB}", "0x2000")[1])
             first += 1
-        spread(plan, load_groups(late) + (load_exponents() if p == 0 else []), first, LD_LAST)
-        spread(plan, early_reads(1), first, RD_LAST)
-        spread(plan, read_exponents(1 - p, "A"), first, RD_LAST)
-        spread(plan, [flip("%[ra0]"), flip("%[rb0]")], first, 63)
+        spread(plan, load_groups(late) + (load_exponents() if p == 0 else []), first, ld_last)
+        spread(plan, early_reads(1), first, rd_last)
+        spread(plan, read_exponents(1 - p, "A"), first, rd_last)
+        spread(plan, [flip("%[ra0]"), flip("%[rb0]")], first, last)
         block(0, p, LdsTracker(at_top if p == 0 else ()), plan, [f'"s_waitcnt vmcnt({len(late) + (2 if p == 0 else 0)}) lgkmcnt(0)', '"s_barrier'])
         # ---- block 1
         plan = dict(enumerate(late_reads(1)))
         state = [[f'"s_add_u32 s{S_KA}, s{S_KA}, 128', f'"s_add_u32 s{S_KB}, s{S_KB}, 128', f'"s_xor_b32 s{S_LDS}, s{S_LDS}, 0x10000']] + offsets(2)
-        for g, texts in enumerate(state):
-            plan[TOP + g] = (None, texts)
-        after = TOP + len(state)
-        plan[63] = (None, [f'"s_add_u32 s{S_IT}, s{S_IT}, 1'])
-        spread(plan, load_groups(early), after, LD_LAST)
-        spread(plan, early_reads(0), after, RD_LAST)
-        spread(plan, read_exponents(1 - p, "B"), after, RD_LAST)
-        spread(plan, [flip(f"v{MX_RA1}"), flip(f"v{MX_RB1}")], after, 62)
+        exponents_b = read_exponents(1 - p, "B")
+        if low:     # (beside the reads at the top, and what is left in a gap behind them; exponents two to a gap)
+            for g, texts in enumerate(state[:top]):
+                plan[g] = (plan[g][0], plan[g][1] + texts)
+            plan[top] = (None, [t for texts in state[top:] for t in texts])
+            after = top + 1
+            exponents_b = [(a[0] + b[0], a[1] + b[1]) for a, b in zip(exponents_b[::2], exponents_b[1::2])]
+        else:
+            for g, texts in enumerate(state):
+                plan[top + g] = (None, texts)
+            after = top + len(state)
+        plan[last] = (None, [f'"s_add_u32 s{S_IT}, s{S_IT}, 1'])
+        spread(plan, load_groups(early), after, ld_last)
+        spread(plan, early_reads(0), after, rd_last)
+        spread(plan, exponents_b, after, rd_last)
+        spread(plan, [flip(f"v{MX_RA1}"), flip(f"v{MX_RB1}")], after, last - 1)
         block(1, p, LdsTracker(), plan, [f'"s_waitcnt vmcnt({len(early)}) lgkmcnt(0)', '"s_barrier', f'"s_cmp_lt_u32 s{S_IT}, %[n]',
                                          '"s_cbranch_scc0 L_sk_end%=' if p == 0 else '"s_cbranch_scc1 L_sk_loop%='])
 
@@ -675,6 +689,7 @@ def main_mx():
     print("// Generated by gen_tile_asm.py mx -- do not edit; see that file for the register plan and the schedule.")
     print("#pragma once")
     emit_macro("SK_TILE_ASM_LOOP_MX", "", loop_text_mx())
+    emit_macro("SK_TILE_ASM_LOOP_MX_LOW", "", loop_text_mx(True))
     clob = [f'"a{r}"' for r in range(256)] + [f'"v{r}"' for r in range(88, 256)] + [f'"s{r}"' for r in range(80, 91)]
     print("#define SK_TILE_ASM_CLOBBERS_MX \\")
     for k in range(0, len(clob), 16):

@@ -63,22 +63,27 @@ static bool takes_tiled(int64_t K, int variant) {
 //           `end` for a tile's beginning and end, `join` for a cut
 //   memory  the operands of the experts that have rows, and C, once at 6 TB/s
 // Fitted to 993 products (none to 256 experts, 1 to 16384 rows, N 20 to 28672, K 256 to 16384, of which half no multiples of 128; mean
-// |log error| 7 to 13 %).  On 1450 others its choice takes 1.025 of the fastest tile's time on average, 1.8 at worst, and more than 1.1 in 85.
+// |log error| 7 to 13 %).  On 750 others its choice takes 1.020 of the fastest tile's time on average, 1.7 at worst, and more than 1.1 in 40.
 struct MxCost {
   int variant, bm, bn, bk, per_cu, cut;
   double start, alone, shared, end, join, hidden, astray;   // us (hidden, astray: parts)
 };
-static const MxCost COSTS[9] = {{GV_MX16X16, 16, 16, 2048, 2, 3, 4.07, 0.44, 0.25, 1.36, 6.50, 0.27, 1.61},
-                                {GV_MX16X32, 16, 32, 2048, 2, 3, 3.95, 0.54, 0.36, 1.32, 5.42, 0.34, 1.84},
-                                {GV_WAVEK16, 16, 64, 2048, 2, 3, 4.04, 0.89, 0.65, 1.14, 4.35, 0.56, 1.58},
-                                {GV_WAVEK32, 32, 64, 2048, 2, 3, 4.27, 1.21, 0.89, 1.22, 4.62, 0.50, 1.27},
-                                {GV_WAVEK64, 64, 64, 2048, 1, 3, 3.73, 1.40, 0.00, 2.80, 4.69, 0.32, 1.03},
-                                {GV_WAVEK64W, 64, 128, 512, 2, 8, 3.49, 0.67, 0.71, 1.75, 11.85, 0.42, 0.10},
-                                {GV_TILE128, 128, 128, 512, 2, 8, 4.68, 1.16, 1.06, 1.31, 17.84, 0.54, 0.09},
-                                {GV_MX128X256, 128, 256, 512, 1, 8, 3.61, 1.94, 0.00, 2.87, 20.00, 0.48, 0.12},
-                                {GV_ASM256, 256, 256, 256, 1, 0, 1.00, 1.01, 0.00, 11.12, 18.83, 0.56, 0.25}};
+static const MxCost COSTS[9] = {{GV_MX16X16, 16, 16, 2048, 2, 3, 4.11, 0.44, 0.26, 1.37, 6.57, 0.25, 1.62},
+                                {GV_MX16X32, 16, 32, 2048, 2, 3, 3.95, 0.56, 0.37, 1.32, 5.48, 0.34, 1.79},
+                                {GV_WAVEK16, 16, 64, 2048, 2, 3, 4.12, 0.92, 0.67, 1.06, 4.34, 0.55, 1.51},
+                                {GV_WAVEK32, 32, 64, 2048, 2, 3, 4.27, 1.19, 0.87, 1.26, 4.70, 0.50, 1.30},
+                                {GV_WAVEK64, 64, 64, 2048, 1, 3, 3.76, 1.39, 0.00, 2.80, 4.69, 0.33, 1.03},
+                                {GV_WAVEK64W, 64, 128, 512, 2, 8, 3.51, 0.71, 0.71, 1.76, 11.85, 0.42, 0.11},
+                                {GV_TILE128, 128, 128, 512, 2, 8, 4.80, 1.14, 1.04, 1.25, 19.16, 0.54, 0.10},
+                                {GV_MX128X256, 128, 256, 512, 1, 8, 3.65, 1.89, 0.00, 2.90, 20.00, 0.48, 0.14},
+                                {GV_ASM256, 256, 256, 256, 1, 0, 1.00, 0.88, 0.00, 11.22, 18.72, 0.69, 0.26}};
 static double estimate(const GroupedShape &h, double experts, const MxCost &c) {
-  const double rows = h.R / experts, high = h.E == 1 ? (double)((h.R + c.bm - 1) / c.bm) : experts * fmax(1.0, 0.5 + rows / c.bm);
+  const double rows = h.R / experts;
+  double high = h.E == 1 ? (double)((h.R + c.bm - 1) / c.bm) : experts * fmax(1.0, 0.5 + rows / c.bm);
+  if (c.variant == GV_ASM256) {   // (a last tile of up to 128 rows counts 0.6)
+    const int64_t rest = h.R % 256;
+    high = h.E == 1 ? (double)(h.R / 256) + (rest == 0 ? 0.0 : (rest <= 128 ? 0.6 : 1.0)) : experts * fmax(0.6, 0.3 + rows / 256);
+  }
   const double tiles = ceil(high * (double)((h.N + c.bn - 1) / c.bn) - 1e-9), slots = (double)h.cus * c.per_cu;
   const double ipt = (double)((h.K + c.bk - 1) / c.bk), whole = floor(tiles / slots), rest = tiles - whole * slots;
   double iters = whole * ipt, at_once = whole > 0 ? c.per_cu : ceil(rest / h.cus);

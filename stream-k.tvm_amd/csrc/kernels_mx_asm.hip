@@ -1,5 +1,6 @@
 // The four-wave 256 x 256 tiles on microscaled 4-bit operands (tile_mx_asm.h), by expert or of one matrix.  The first loads of a CTA's next tile
-// go out before this one is stored.
+// go out before this one is stored.  A row tile of at most 128 rows is a low one, as in kernels_grouped_asm.hip: half the MFMAs, three quarters of
+// the loads; 2100 x 8192 x 8192 94 us, so 83, 100 x 28672 x 8192 51 and 44, 8 experts of 11008 x 4096, 8192 rows 221 and 218.
 #include "grouped_cut.h"
 #include "grouped_launch.h"
 #include "grouped_mx.h"
@@ -19,7 +20,7 @@ __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_mx_asm_kernel(MxGro
   struct Segment {
     GroupTile t;
     int cut, part, k0, n;   // (cut: number among the cut tiles, or -1)
-    bool last;
+    bool last, low;
   };
   const int items = cuts.whole + (tiles - cuts.whole) * cuts.parts, pairs = (ipt + 1) >> 1;
   auto segment = [&](int item, Segment &s) {
@@ -38,6 +39,7 @@ __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_mx_asm_kernel(MxGro
     s.n = min(2 * end, ipt) - s.k0;
     s.last = s.k0 + s.n == ipt;
     walk.find(tile, s.t);
+    s.low = s.t.rows - s.t.pm * P::BM <= P::BM / 2;
     return true;
   };
   typename P::Acc acc;
@@ -47,11 +49,19 @@ __global__ __launch_bounds__(P::NT, P::WAVES_PER_EU) void sk_mx_asm_kernel(MxGro
   while (have) {
     const typename P::Args a = expert_args<P>(g, s.t);
     const void *epi = expert_epilogue(g, s.t);
-    P::mac(a, s.t.pm, s.t.pn, s.k0, s.n, s.last, requested);
+    if (s.low) P::template mac<true>(a, s.t.pm, s.t.pn, s.k0, s.n, s.last, requested);
+    else P::template mac<false>(a, s.t.pm, s.t.pn, s.k0, s.n, s.last, requested);
     item += g.grid;
     have = requested = segment(item, next);
-    if (have) P::prefetch_first_stage(expert_args<P>(g, next.t), next.t.pm, next.t.pn, next.k0, next.n, next.last);
-    if (s.cut < 0 || join_parts<P>(acc, s.cut, s.part, cuts.parts, g.grid, g.spin_limit, ws, false)) P::store_c(a, s.t.pm, s.t.pn, epi);
+    if (have) {
+      const typename P::Args b = expert_args<P>(g, next.t);
+      if (next.low) P::template prefetch_first_stage<true>(b, next.t.pm, next.t.pn, next.k0, next.n, next.last);
+      else P::template prefetch_first_stage<false>(b, next.t.pm, next.t.pn, next.k0, next.n, next.last);
+    }
+    if (s.cut < 0 || join_parts<P>(acc, s.cut, s.part, cuts.parts, g.grid, g.spin_limit, ws, s.low)) {
+      if (s.low) P::template store_c<true>(a, s.t.pm, s.t.pn, epi);
+      else P::template store_c<false>(a, s.t.pm, s.t.pn, epi);
+    }
     s = next;
   }
 }

@@ -282,7 +282,8 @@ struct TileF16Asm {
   }
   template <int HALF>
   static __device__ __forceinline__ void store_c_direct(const Args &a, int pm, int pn) {
-    const int lane = threadIdx.x & 63;
+    // (MX, with two instances of this: no address is held through the loops)
+    const int lane = (MX ? pin_here((int)threadIdx.x) : (int)threadIdx.x) & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int wm = wave >> 1, wn = wave & 1;
     const int row0 = pm * BM + wm * WTM, col0 = pn * BN + wn * WTN;

@@ -24,11 +24,13 @@ struct TileMxAsm : TileF16Asm<BF16 ? 6 : 5, false> {
 
   struct Ctx {
     uint4v rsrc_a, rsrc_b, rsrc_ea, rsrc_eb;
-    uint32_t voff_a, voff_b, voff_e, tail;
+    uint32_t voff_a, voff_b, voff_ea, voff_e, tail;
     uint32_t goff_a, goff_b, goff_ea, goff_eb, gstep_a, gstep_b, step_ea, step_eb;
     uint32_t lds_wave, lds_e;
     uint32_t ra0, rb0, rda, rdb;   // where the lane reads fragments and exponents
   };
+  // LOW: at most 128 rows, 64 to a wave (TileF16Asm::LOW_TILE): the second wave row's 64 stand where a whole tile has rows 128 ..
+  template <bool LOW>
   static __device__ __forceinline__ Ctx make_ctx(const Args &a, int pm, int pn, int k0) {
     Ctx c;
     // (pinned: no address is held through the loop, which leaves the compiler 88 registers)
@@ -49,6 +51,7 @@ struct TileMxAsm : TileF16Asm<BF16 ? 6 : 5, false> {
     c.gstep_a = (uint32_t)(64 * a.lda);
     c.gstep_b = (uint32_t)(64 * a.ldb);
     c.voff_e = (uint32_t)((wave * 64 + lane) * 16);
+    c.voff_ea = c.voff_e - (LOW && wave >= 2 ? 64 * 16 : 0);
     c.goff_ea = (uint32_t)(k0 >> 1) * (uint32_t)a.ea.step;
     c.goff_eb = (uint32_t)(k0 >> 1) * (uint32_t)a.eb.step;
     c.step_ea = (uint32_t)a.ea.step;
@@ -66,7 +69,7 @@ struct TileMxAsm : TileF16Asm<BF16 ? 6 : 5, false> {
     c.rdb = base + EXPONENTS_AT + P::BM * 16 + (uint32_t)(wn * P::WTN + (lane & 15)) * 16 + 2 * g;
     return c;
   }
-  template <bool EARLY_ONLY>
+  template <bool LOW, bool EARLY_ONLY>
   static __device__ __forceinline__ void stage_loads(const Ctx &c, int stage, int n, bool last) {
     const uint32_t oob = stage < n ? 0u : OOB_OFFSET, tail = last && stage == n - 1 ? c.tail : 0u;
     const uint32_t voa = c.voff_a | oob | tail, vob = c.voff_b | oob | tail;
@@ -76,42 +79,59 @@ struct TileMxAsm : TileF16Asm<BF16 ? 6 : 5, false> {
       [gas] "s"(c.gstep_a), [gas2] "s"(2 * c.gstep_a), [gas3] "s"(3 * c.gstep_a), [gbs] "s"(c.gstep_b),                   \
       [gbs2] "s"(2 * c.gstep_b), [gbs3] "s"(3 * c.gstep_b), [lds] "s"(lds_stage)                                          \
   : "memory", "m0", "scc", "s83"
-    if constexpr (EARLY_ONLY) asm volatile(SK_TILE_ASM_LOADS_EARLY SK_MX_LOAD_OPERANDS);
+    if constexpr (LOW && EARLY_ONLY) asm volatile(SK_TILE_ASM_LOADS_EARLY_LOW SK_MX_LOAD_OPERANDS);
+    else if constexpr (LOW) asm volatile(SK_TILE_ASM_LOADS_LOW SK_MX_LOAD_OPERANDS);
+    else if constexpr (EARLY_ONLY) asm volatile(SK_TILE_ASM_LOADS_EARLY SK_MX_LOAD_OPERANDS);
     else asm volatile(SK_TILE_ASM_LOADS SK_MX_LOAD_OPERANDS);
 #undef SK_MX_LOAD_OPERANDS
   }
+  template <bool LOW>
   static __device__ __forceinline__ void first_loads(const Ctx &c, int n, bool last) {
-    dma_load_16(c.rsrc_ea, c.lds_e, c.voff_e, c.goff_ea);
+    dma_load_16(c.rsrc_ea, c.lds_e, c.voff_ea, c.goff_ea);
     dma_load_16(c.rsrc_eb, c.lds_e + P::BM * 16, c.voff_e, c.goff_eb);
-    stage_loads<false>(c, 0, n, last);
+    stage_loads<LOW, false>(c, 0, n, last);
   }
   // last: the segment ends with K
-  static __device__ __forceinline__ void prefetch_first_stage(const Args &a, int pm, int pn, int k0, int n, bool last) { first_loads(make_ctx(a, pm, pn, k0), n, last); }
+  template <bool LOW>
+  static __device__ __forceinline__ void prefetch_first_stage(const Args &a, int pm, int pn, int k0, int n, bool last) {
+    first_loads<LOW>(make_ctx<LOW>(a, pm, pn, k0), n, last);
+  }
+  template <bool LOW>
   static __device__ __forceinline__ void mac(const Args &a, int pm, int pn, int k0, int n, bool last, bool first_stage_requested) {
-    Ctx c = make_ctx(a, pm, pn, k0);
-    if (!first_stage_requested) first_loads(c, n, last);
+    Ctx c = make_ctx<LOW>(a, pm, pn, k0);
+    if (!first_stage_requested) first_loads<LOW>(c, n, last);
     // (directly ahead of the loop, whose first wait counts on these being the youngest operations)
-    stage_loads<true>(c, 1, n, last);
-    asm volatile(SK_TILE_ASM_LOOP_MX
-                 : [ra0] "+v"(c.ra0), [rb0] "+v"(c.rb0)
-                 : [rsa] "s"(c.rsrc_a), [rsb] "s"(c.rsrc_b), [rea] "s"(c.rsrc_ea), [reb] "s"(c.rsrc_eb), [voa] "v"(c.voff_a), [vob] "v"(c.voff_b),
-                   [ve] "v"(c.voff_e), [tail] "v"(last ? c.tail : 0u), [rda] "v"(c.rda), [rdb] "v"(c.rdb), [ga0] "s"(c.goff_a),
-                   [gb0] "s"(c.goff_b), [gas] "s"(c.gstep_a), [gas2] "s"(2 * c.gstep_a), [gas3] "s"(3 * c.gstep_a), [gbs] "s"(c.gstep_b),
-                   [gbs2] "s"(2 * c.gstep_b), [gbs3] "s"(3 * c.gstep_b), [n] "s"((uint32_t)n), [lds] "s"(c.lds_wave), [eka] "s"(c.goff_ea + c.step_ea),
-                   [ekb] "s"(c.goff_eb + c.step_eb), [esa] "s"(c.step_ea), [esb] "s"(c.step_eb),
-                   [el] "s"(c.lds_e + PAIR_BYTES)
-                 : "memory", "m0", "scc", SK_TILE_ASM_CLOBBERS_MX);
+    stage_loads<LOW, true>(c, 1, n, last);
+#define SK_MX_LOOP_OPERANDS(...) \
+  : [ra0] "+v"(c.ra0), [rb0] "+v"(c.rb0) \
+  : [rsa] "s"(c.rsrc_a), [rsb] "s"(c.rsrc_b), [rea] "s"(c.rsrc_ea), [reb] "s"(c.rsrc_eb), [voa] "v"(c.voff_a), [vob] "v"(c.voff_b), \
+  [ve] "v"(c.voff_e), __VA_ARGS__ [tail] "v"(last ? c.tail : 0u), [rda] "v"(c.rda), [rdb] "v"(c.rdb), [ga0] "s"(c.goff_a), \
+  [gb0] "s"(c.goff_b), [gas] "s"(c.gstep_a), [gas2] "s"(2 * c.gstep_a), [gas3] "s"(3 * c.gstep_a), [gbs] "s"(c.gstep_b), \
+  [gbs2] "s"(2 * c.gstep_b), [gbs3] "s"(3 * c.gstep_b), [n] "s"((uint32_t)n), [lds] "s"(c.lds_wave), [eka] "s"(c.goff_ea + c.step_ea), \
+  [ekb] "s"(c.goff_eb + c.step_eb), [esa] "s"(c.step_ea), [esb] "s"(c.step_eb), \
+  [el] "s"(c.lds_e + PAIR_BYTES) \
+  : "memory", "m0", "scc", SK_TILE_ASM_CLOBBERS_MX
+    if constexpr (LOW) asm volatile(SK_TILE_ASM_LOOP_MX_LOW SK_MX_LOOP_OPERANDS([vea] "v"(c.voff_ea),));
+    else asm volatile(SK_TILE_ASM_LOOP_MX SK_MX_LOOP_OPERANDS());
+#undef SK_MX_LOOP_OPERANDS
     // every wave has left the loop and its own loads have landed: the stages are free
     __syncthreads();
   }
-  static __device__ __forceinline__ void store_c(const Args &a, int pm, int pn, const void *epi) {
+  // LOW: the lower half of each wave's 128 rows; the second wave row's are the tile's rows 64 .., not 128 ..: C moved back by 64
+  template <bool LOW>
+  static __device__ __forceinline__ void store_c(Args a, int pm, int pn, const void *epi) {
+    if constexpr (LOW) {
+      const int back = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 7) * (P::WTM / 2);
+      a.C -= (int64_t)back * a.ldc;
+      a.M += back;
+    }
     if (P::direct_store_ok(a, pn, epi)) {
-      P::template store_c_direct<-1>(a, pm, pn);
+      P::template store_c_direct<LOW ? 0 : -1>(a, pm, pn);
       return;
     }
     const int wave = threadIdx.x >> 6, row0 = pm * P::BM + (wave >> 1) * P::WTM, col0 = pn * P::BN + (wave & 1) * P::WTN;
     by_epilogue(epi, [&](auto e) {
-      AsmEnd<TileMxAsm, false, BF16, decltype(e)::value, true>::store(a.C, a.ldc, a.M, a.N, row0, col0, nullptr, nullptr, epi_bias(epi), 0, P::FM);
+      AsmEnd<TileMxAsm, false, BF16, decltype(e)::value, true>::store(a.C, a.ldc, a.M, a.N, row0, col0, nullptr, nullptr, epi_bias(epi), 0, LOW ? P::FM / 2 : P::FM);
     });
   }
 };

@@ -853,6 +853,535 @@
   "s_nop 7\n\t" \
   "s_nop 7\n\t" \
   ""
+#define SK_TILE_ASM_LOOP_MX_LOW \
+  "v_accvgpr_write_b32 a0, 0\n\t" \
+  "v_accvgpr_write_b32 a1, 0\n\t" \
+  "v_accvgpr_write_b32 a2, 0\n\t" \
+  "v_accvgpr_write_b32 a3, 0\n\t" \
+  "v_accvgpr_write_b32 a4, 0\n\t" \
+  "v_accvgpr_write_b32 a5, 0\n\t" \
+  "v_accvgpr_write_b32 a6, 0\n\t" \
+  "v_accvgpr_write_b32 a7, 0\n\t" \
+  "v_accvgpr_write_b32 a8, 0\n\t" \
+  "v_accvgpr_write_b32 a9, 0\n\t" \
+  "v_accvgpr_write_b32 a10, 0\n\t" \
+  "v_accvgpr_write_b32 a11, 0\n\t" \
+  "v_accvgpr_write_b32 a12, 0\n\t" \
+  "v_accvgpr_write_b32 a13, 0\n\t" \
+  "v_accvgpr_write_b32 a14, 0\n\t" \
+  "v_accvgpr_write_b32 a15, 0\n\t" \
+  "v_accvgpr_write_b32 a16, 0\n\t" \
+  "v_accvgpr_write_b32 a17, 0\n\t" \
+  "v_accvgpr_write_b32 a18, 0\n\t" \
+  "v_accvgpr_write_b32 a19, 0\n\t" \
+  "v_accvgpr_write_b32 a20, 0\n\t" \
+  "v_accvgpr_write_b32 a21, 0\n\t" \
+  "v_accvgpr_write_b32 a22, 0\n\t" \
+  "v_accvgpr_write_b32 a23, 0\n\t" \
+  "v_accvgpr_write_b32 a24, 0\n\t" \
+  "v_accvgpr_write_b32 a25, 0\n\t" \
+  "v_accvgpr_write_b32 a26, 0\n\t" \
+  "v_accvgpr_write_b32 a27, 0\n\t" \
+  "v_accvgpr_write_b32 a28, 0\n\t" \
+  "v_accvgpr_write_b32 a29, 0\n\t" \
+  "v_accvgpr_write_b32 a30, 0\n\t" \
+  "v_accvgpr_write_b32 a31, 0\n\t" \
+  "v_accvgpr_write_b32 a32, 0\n\t" \
+  "v_accvgpr_write_b32 a33, 0\n\t" \
+  "v_accvgpr_write_b32 a34, 0\n\t" \
+  "v_accvgpr_write_b32 a35, 0\n\t" \
+  "v_accvgpr_write_b32 a36, 0\n\t" \
+  "v_accvgpr_write_b32 a37, 0\n\t" \
+  "v_accvgpr_write_b32 a38, 0\n\t" \
+  "v_accvgpr_write_b32 a39, 0\n\t" \
+  "v_accvgpr_write_b32 a40, 0\n\t" \
+  "v_accvgpr_write_b32 a41, 0\n\t" \
+  "v_accvgpr_write_b32 a42, 0\n\t" \
+  "v_accvgpr_write_b32 a43, 0\n\t" \
+  "v_accvgpr_write_b32 a44, 0\n\t" \
+  "v_accvgpr_write_b32 a45, 0\n\t" \
+  "v_accvgpr_write_b32 a46, 0\n\t" \
+  "v_accvgpr_write_b32 a47, 0\n\t" \
+  "v_accvgpr_write_b32 a48, 0\n\t" \
+  "v_accvgpr_write_b32 a49, 0\n\t" \
+  "v_accvgpr_write_b32 a50, 0\n\t" \
+  "v_accvgpr_write_b32 a51, 0\n\t" \
+  "v_accvgpr_write_b32 a52, 0\n\t" \
+  "v_accvgpr_write_b32 a53, 0\n\t" \
+  "v_accvgpr_write_b32 a54, 0\n\t" \
+  "v_accvgpr_write_b32 a55, 0\n\t" \
+  "v_accvgpr_write_b32 a56, 0\n\t" \
+  "v_accvgpr_write_b32 a57, 0\n\t" \
+  "v_accvgpr_write_b32 a58, 0\n\t" \
+  "v_accvgpr_write_b32 a59, 0\n\t" \
+  "v_accvgpr_write_b32 a60, 0\n\t" \
+  "v_accvgpr_write_b32 a61, 0\n\t" \
+  "v_accvgpr_write_b32 a62, 0\n\t" \
+  "v_accvgpr_write_b32 a63, 0\n\t" \
+  "v_accvgpr_write_b32 a64, 0\n\t" \
+  "v_accvgpr_write_b32 a65, 0\n\t" \
+  "v_accvgpr_write_b32 a66, 0\n\t" \
+  "v_accvgpr_write_b32 a67, 0\n\t" \
+  "v_accvgpr_write_b32 a68, 0\n\t" \
+  "v_accvgpr_write_b32 a69, 0\n\t" \
+  "v_accvgpr_write_b32 a70, 0\n\t" \
+  "v_accvgpr_write_b32 a71, 0\n\t" \
+  "v_accvgpr_write_b32 a72, 0\n\t" \
+  "v_accvgpr_write_b32 a73, 0\n\t" \
+  "v_accvgpr_write_b32 a74, 0\n\t" \
+  "v_accvgpr_write_b32 a75, 0\n\t" \
+  "v_accvgpr_write_b32 a76, 0\n\t" \
+  "v_accvgpr_write_b32 a77, 0\n\t" \
+  "v_accvgpr_write_b32 a78, 0\n\t" \
+  "v_accvgpr_write_b32 a79, 0\n\t" \
+  "v_accvgpr_write_b32 a80, 0\n\t" \
+  "v_accvgpr_write_b32 a81, 0\n\t" \
+  "v_accvgpr_write_b32 a82, 0\n\t" \
+  "v_accvgpr_write_b32 a83, 0\n\t" \
+  "v_accvgpr_write_b32 a84, 0\n\t" \
+  "v_accvgpr_write_b32 a85, 0\n\t" \
+  "v_accvgpr_write_b32 a86, 0\n\t" \
+  "v_accvgpr_write_b32 a87, 0\n\t" \
+  "v_accvgpr_write_b32 a88, 0\n\t" \
+  "v_accvgpr_write_b32 a89, 0\n\t" \
+  "v_accvgpr_write_b32 a90, 0\n\t" \
+  "v_accvgpr_write_b32 a91, 0\n\t" \
+  "v_accvgpr_write_b32 a92, 0\n\t" \
+  "v_accvgpr_write_b32 a93, 0\n\t" \
+  "v_accvgpr_write_b32 a94, 0\n\t" \
+  "v_accvgpr_write_b32 a95, 0\n\t" \
+  "v_accvgpr_write_b32 a96, 0\n\t" \
+  "v_accvgpr_write_b32 a97, 0\n\t" \
+  "v_accvgpr_write_b32 a98, 0\n\t" \
+  "v_accvgpr_write_b32 a99, 0\n\t" \
+  "v_accvgpr_write_b32 a100, 0\n\t" \
+  "v_accvgpr_write_b32 a101, 0\n\t" \
+  "v_accvgpr_write_b32 a102, 0\n\t" \
+  "v_accvgpr_write_b32 a103, 0\n\t" \
+  "v_accvgpr_write_b32 a104, 0\n\t" \
+  "v_accvgpr_write_b32 a105, 0\n\t" \
+  "v_accvgpr_write_b32 a106, 0\n\t" \
+  "v_accvgpr_write_b32 a107, 0\n\t" \
+  "v_accvgpr_write_b32 a108, 0\n\t" \
+  "v_accvgpr_write_b32 a109, 0\n\t" \
+  "v_accvgpr_write_b32 a110, 0\n\t" \
+  "v_accvgpr_write_b32 a111, 0\n\t" \
+  "v_accvgpr_write_b32 a112, 0\n\t" \
+  "v_accvgpr_write_b32 a113, 0\n\t" \
+  "v_accvgpr_write_b32 a114, 0\n\t" \
+  "v_accvgpr_write_b32 a115, 0\n\t" \
+  "v_accvgpr_write_b32 a116, 0\n\t" \
+  "v_accvgpr_write_b32 a117, 0\n\t" \
+  "v_accvgpr_write_b32 a118, 0\n\t" \
+  "v_accvgpr_write_b32 a119, 0\n\t" \
+  "v_accvgpr_write_b32 a120, 0\n\t" \
+  "v_accvgpr_write_b32 a121, 0\n\t" \
+  "v_accvgpr_write_b32 a122, 0\n\t" \
+  "v_accvgpr_write_b32 a123, 0\n\t" \
+  "v_accvgpr_write_b32 a124, 0\n\t" \
+  "v_accvgpr_write_b32 a125, 0\n\t" \
+  "v_accvgpr_write_b32 a126, 0\n\t" \
+  "v_accvgpr_write_b32 a127, 0\n\t" \
+  "s_mov_b32 s80, 0\n\t" \
+  "s_xor_b32 s86, %[lds], 0x10000\n\t" \
+  "s_add_u32 s81, %[ga0], 128\n\t" \
+  "s_add_u32 s82, %[gb0], 128\n\t" \
+  "s_mov_b32 s88, %[el]\n\t" \
+  "s_mov_b32 s89, %[eka]\n\t" \
+  "s_mov_b32 s90, %[ekb]\n\t" \
+  "v_xor_b32 v124, 16, %[ra0]\n\t" \
+  "v_xor_b32 v125, 16, %[rb0]\n\t" \
+  "v_mov_b32 v126, %[rda]\n\t" \
+  "v_mov_b32 v127, %[rdb]\n\t" \
+  "s_add_u32 s87, s80, 1\n\t" \
+  "s_cmp_lt_u32 s87, %[n]\n\t" \
+  "s_cselect_b32 s84, 0, 0x80000000\n\t" \
+  "s_add_u32 s87, s87, 1\n\t" \
+  "s_cmp_eq_u32 s87, %[n]\n\t" \
+  "s_cselect_b32 s85, 0x80000000, 0\n\t" \
+  "v_and_b32 v122, s85, %[tail]\n\t" \
+  "v_or3_b32 v120, s84, %[voa], v122\n\t" \
+  "v_or3_b32 v121, s84, %[vob], v122\n\t" \
+  "s_waitcnt vmcnt(8)\n\t" \
+  "s_barrier\n\t" \
+  "ds_read_u16 v88, v126 offset:0\n\t" \
+  "ds_read_u16 v89, v126 offset:256\n\t" \
+  "ds_read_u16 v90, v126 offset:512\n\t" \
+  "ds_read_u16 v91, v126 offset:768\n\t" \
+  "ds_read_u16 v96, v127 offset:0\n\t" \
+  "ds_read_u16 v97, v127 offset:256\n\t" \
+  "ds_read_u16 v98, v127 offset:512\n\t" \
+  "ds_read_u16 v99, v127 offset:768\n\t" \
+  "ds_read_u16 v100, v127 offset:1024\n\t" \
+  "ds_read_u16 v101, v127 offset:1280\n\t" \
+  "ds_read_u16 v102, v127 offset:1536\n\t" \
+  "ds_read_u16 v103, v127 offset:1792\n\t" \
+  "ds_read_b128 v[128:131], %[ra0] offset:0\n\t" \
+  "ds_read_b128 v[160:163], %[rb0] offset:0\n\t" \
+  "ds_read_b128 v[164:167], %[rb0] offset:2048\n\t" \
+  "ds_read_b128 v[168:171], %[rb0] offset:4096\n\t" \
+  "ds_read_b128 v[172:175], %[rb0] offset:6144\n\t" \
+  "ds_read_b128 v[132:135], %[ra0] offset:2048\n\t" \
+  "ds_read_b128 v[136:139], %[ra0] offset:4096\n\t" \
+  "ds_read_b128 v[140:143], %[ra0] offset:6144\n\t" \
+  "s_nop 7\n\t" \
+  "L_sk_loop%=:\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[0:3], v[160:163], v[128:131], a[0:3], v96, v88 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[176:179], %[rb0] offset:8192\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[4:7], v[164:167], v[128:131], a[4:7], v97, v88 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[180:183], %[rb0] offset:10240\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[8:11], v[168:171], v[128:131], a[8:11], v98, v88 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[184:187], %[rb0] offset:12288\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[12:15], v[172:175], v[128:131], a[12:15], v99, v88 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[188:191], %[rb0] offset:14336\n\t" \
+  "s_waitcnt lgkmcnt(6)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[44:47], v[172:175], v[132:135], a[44:47], v99, v89 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "s_add_u32 s83, s82, %[gbs2]\n\t" \
+  "s_add_u32 m0, s86, 40960\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[40:43], v[168:171], v[132:135], a[40:43], v98, v89 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[192:195], v124 offset:0\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[36:39], v[164:167], v[132:135], a[36:39], v97, v89 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_u16 v104, v126 offset:8\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[32:35], v[160:163], v[132:135], a[32:35], v96, v89 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 45056\n\t" \
+  "s_waitcnt lgkmcnt(7)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[64:67], v[160:163], v[136:139], a[64:67], v96, v90 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[224:227], v125 offset:0\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[68:71], v[164:167], v[136:139], a[68:71], v97, v90 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_xor_b32 %[ra0], 0x10000, %[ra0]\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[72:75], v[168:171], v[136:139], a[72:75], v98, v90 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs3]\n\t" \
+  "s_add_u32 m0, s86, 57344\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[76:79], v[172:175], v[136:139], a[76:79], v99, v90 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[228:231], v125 offset:2048\n\t" \
+  "s_waitcnt lgkmcnt(8)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[108:111], v[172:175], v[140:143], a[108:111], v99, v91 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_u16 v105, v126 offset:264\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[104:107], v[168:171], v[140:143], a[104:107], v98, v91 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 61440\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[100:103], v[164:167], v[140:143], a[100:103], v97, v91 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[232:235], v125 offset:4096\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[96:99], v[160:163], v[140:143], a[96:99], v96, v91 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "s_waitcnt lgkmcnt(9)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[112:115], v[176:179], v[140:143], a[112:115], v100, v91 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  "s_waitcnt lgkmcnt(8)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[116:119], v[180:183], v[140:143], a[116:119], v101, v91 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[236:239], v125 offset:6144\n\t" \
+  "s_waitcnt lgkmcnt(8)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[120:123], v[184:187], v[140:143], a[120:123], v102, v91 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_u16 v106, v126 offset:520\n\t" \
+  "s_waitcnt lgkmcnt(8)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[124:127], v[188:191], v[140:143], a[124:127], v103, v91 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "s_mov_b32 m0, s88\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[92:95], v[188:191], v[136:139], a[92:95], v103, v90 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[196:199], v124 offset:2048\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[88:91], v[184:187], v[136:139], a[88:91], v102, v90 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[84:87], v[180:183], v[136:139], a[84:87], v101, v90 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 %[vea], %[rea], s89 offen lds\n\t" \
+  "s_add_u32 s89, s89, %[esa]\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[80:83], v[176:179], v[136:139], a[80:83], v100, v90 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[200:203], v124 offset:4096\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[48:51], v[176:179], v[132:135], a[48:51], v100, v89 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_u16 v107, v126 offset:776\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[52:55], v[180:183], v[132:135], a[52:55], v101, v89 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "s_add_u32 m0, s88, 4096\n\t" \
+  "s_xor_b32 s88, s88, 0x2000\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[56:59], v[184:187], v[132:135], a[56:59], v102, v89 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[204:207], v124 offset:6144\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[60:63], v[188:191], v[132:135], a[60:63], v103, v89 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_xor_b32 %[rb0], 0x10000, %[rb0]\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[28:31], v[188:191], v[128:131], a[28:31], v103, v88 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 %[ve], %[reb], s90 offen lds\n\t" \
+  "s_add_u32 s90, s90, %[esb]\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[24:27], v[184:187], v[128:131], a[24:27], v102, v88 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[20:23], v[180:183], v[128:131], a[20:23], v101, v88 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[16:19], v[176:179], v[128:131], a[16:19], v100, v88 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "s_waitcnt vmcnt(6) lgkmcnt(0)\n\t" \
+  "s_barrier\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[0:3], v[224:227], v[192:195], a[0:3], v96, v88 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[240:243], v125 offset:8192\n\t" \
+  "s_add_u32 s81, s81, 128\n\t" \
+  "s_add_u32 s82, s82, 128\n\t" \
+  "s_xor_b32 s86, s86, 0x10000\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[4:7], v[228:231], v[192:195], a[4:7], v97, v88 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[244:247], v125 offset:10240\n\t" \
+  "s_add_u32 s87, s80, 2\n\t" \
+  "s_cmp_lt_u32 s87, %[n]\n\t" \
+  "s_cselect_b32 s84, 0, 0x80000000\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[8:11], v[232:235], v[192:195], a[8:11], v98, v88 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[248:251], v125 offset:12288\n\t" \
+  "s_add_u32 s87, s87, 1\n\t" \
+  "s_cmp_eq_u32 s87, %[n]\n\t" \
+  "s_cselect_b32 s85, 0x80000000, 0\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[12:15], v[236:239], v[192:195], a[12:15], v99, v88 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[252:255], v125 offset:14336\n\t" \
+  "v_and_b32 v122, s85, %[tail]\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[44:47], v[236:239], v[196:199], a[44:47], v99, v89 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_or3_b32 v120, s84, %[voa], v122\n\t" \
+  "v_or3_b32 v121, s84, %[vob], v122\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[40:43], v[232:235], v[196:199], a[40:43], v98, v89 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "s_mov_b32 s83, s81\n\t" \
+  "s_add_u32 m0, s86, 0\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[36:39], v[228:231], v[196:199], a[36:39], v97, v89 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[128:131], %[ra0] offset:0\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[32:35], v[224:227], v[196:199], a[32:35], v96, v89 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, s86, 4096\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[64:67], v[224:227], v[200:203], a[64:67], v96, v90 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_u16 v112, v127 offset:8\n\t" \
+  "ds_read_u16 v113, v127 offset:264\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[68:71], v[228:231], v[200:203], a[68:71], v97, v90 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[160:163], %[rb0] offset:0\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[72:75], v[232:235], v[200:203], a[72:75], v98, v90 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, s86, 16384\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[76:79], v[236:239], v[200:203], a[76:79], v99, v90 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_xor_b32 v124, 0x10000, v124\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[108:111], v[236:239], v[204:207], a[108:111], v99, v91 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[164:167], %[rb0] offset:2048\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[104:107], v[232:235], v[204:207], a[104:107], v98, v91 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, s86, 20480\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[100:103], v[228:231], v[204:207], a[100:103], v97, v91 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_u16 v114, v127 offset:520\n\t" \
+  "ds_read_u16 v115, v127 offset:776\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[96:99], v[224:227], v[204:207], a[96:99], v96, v91 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[168:171], %[rb0] offset:4096\n\t" \
+  "s_waitcnt lgkmcnt(11)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[112:115], v[240:243], v[204:207], a[112:115], v100, v91 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  "s_mov_b32 s83, s82\n\t" \
+  "s_add_u32 m0, s86, 32768\n\t" \
+  "s_waitcnt lgkmcnt(10)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[116:119], v[244:247], v[204:207], a[116:119], v101, v91 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "s_waitcnt lgkmcnt(9)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[120:123], v[248:251], v[204:207], a[120:123], v102, v91 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[172:175], %[rb0] offset:6144\n\t" \
+  "s_waitcnt lgkmcnt(9)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[124:127], v[252:255], v[204:207], a[124:127], v103, v91 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 36864\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[92:95], v[252:255], v[200:203], a[92:95], v103, v90 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_u16 v116, v127 offset:1032\n\t" \
+  "ds_read_u16 v117, v127 offset:1288\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[88:91], v[248:251], v[200:203], a[88:91], v102, v90 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[132:135], %[ra0] offset:2048\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[84:87], v[244:247], v[200:203], a[84:87], v101, v90 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs3]\n\t" \
+  "s_add_u32 m0, s86, 49152\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[80:83], v[240:243], v[200:203], a[80:83], v100, v90 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_xor_b32 v125, 0x10000, v125\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[48:51], v[240:243], v[196:199], a[48:51], v100, v89 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[136:139], %[ra0] offset:4096\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[52:55], v[244:247], v[196:199], a[52:55], v101, v89 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 53248\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[56:59], v[248:251], v[196:199], a[56:59], v102, v89 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_u16 v118, v127 offset:1544\n\t" \
+  "ds_read_u16 v119, v127 offset:1800\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[60:63], v[252:255], v[196:199], a[60:63], v103, v89 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[140:143], %[ra0] offset:6144\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[28:31], v[252:255], v[192:195], a[28:31], v103, v88 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[24:27], v[248:251], v[192:195], a[24:27], v102, v88 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[20:23], v[244:247], v[192:195], a[20:23], v101, v88 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[16:19], v[240:243], v[192:195], a[16:19], v100, v88 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "s_add_u32 s80, s80, 1\n\t" \
+  "s_waitcnt vmcnt(8) lgkmcnt(0)\n\t" \
+  "s_barrier\n\t" \
+  "s_cmp_lt_u32 s80, %[n]\n\t" \
+  "s_cbranch_scc0 L_sk_end%=\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[0:3], v[160:163], v[128:131], a[0:3], v112, v104 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[176:179], %[rb0] offset:8192\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[4:7], v[164:167], v[128:131], a[4:7], v113, v104 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[180:183], %[rb0] offset:10240\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[8:11], v[168:171], v[128:131], a[8:11], v114, v104 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[184:187], %[rb0] offset:12288\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[12:15], v[172:175], v[128:131], a[12:15], v115, v104 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[188:191], %[rb0] offset:14336\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[44:47], v[172:175], v[132:135], a[44:47], v115, v105 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_xor_b32 v126, 0x2000, v126\n\t" \
+  "v_xor_b32 v127, 0x2000, v127\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[40:43], v[168:171], v[132:135], a[40:43], v114, v105 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "s_add_u32 s83, s82, %[gbs2]\n\t" \
+  "s_add_u32 m0, s86, 40960\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[36:39], v[164:167], v[132:135], a[36:39], v113, v105 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[192:195], v124 offset:0\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[32:35], v[160:163], v[132:135], a[32:35], v112, v105 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_u16 v88, v126 offset:0\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[64:67], v[160:163], v[136:139], a[64:67], v112, v106 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[224:227], v125 offset:0\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[68:71], v[164:167], v[136:139], a[68:71], v113, v106 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_xor_b32 %[ra0], 0x10000, %[ra0]\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[72:75], v[168:171], v[136:139], a[72:75], v114, v106 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 45056\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[76:79], v[172:175], v[136:139], a[76:79], v115, v106 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[108:111], v[172:175], v[140:143], a[108:111], v115, v107 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[228:231], v125 offset:2048\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[104:107], v[168:171], v[140:143], a[104:107], v114, v107 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_u16 v89, v126 offset:256\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[100:103], v[164:167], v[140:143], a[100:103], v113, v107 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[232:235], v125 offset:4096\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[96:99], v[160:163], v[140:143], a[96:99], v112, v107 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs3]\n\t" \
+  "s_add_u32 m0, s86, 57344\n\t" \
+  "s_waitcnt lgkmcnt(9)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[112:115], v[176:179], v[140:143], a[112:115], v116, v107 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "s_waitcnt lgkmcnt(8)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[116:119], v[180:183], v[140:143], a[116:119], v117, v107 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "s_waitcnt lgkmcnt(7)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[120:123], v[184:187], v[140:143], a[120:123], v118, v107 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[236:239], v125 offset:6144\n\t" \
+  "s_waitcnt lgkmcnt(7)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[124:127], v[188:191], v[140:143], a[124:127], v119, v107 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_u16 v90, v126 offset:512\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[92:95], v[188:191], v[136:139], a[92:95], v119, v106 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 61440\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[88:91], v[184:187], v[136:139], a[88:91], v118, v106 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[196:199], v124 offset:2048\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[84:87], v[180:183], v[136:139], a[84:87], v117, v106 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[80:83], v[176:179], v[136:139], a[80:83], v116, v106 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_xor_b32 %[rb0], 0x10000, %[rb0]\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[48:51], v[176:179], v[132:135], a[48:51], v116, v105 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[200:203], v124 offset:4096\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[52:55], v[180:183], v[132:135], a[52:55], v117, v105 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[56:59], v[184:187], v[132:135], a[56:59], v118, v105 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_u16 v91, v126 offset:768\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[60:63], v[188:191], v[132:135], a[60:63], v119, v105 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[204:207], v124 offset:6144\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[28:31], v[188:191], v[128:131], a[28:31], v119, v104 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[24:27], v[184:187], v[128:131], a[24:27], v118, v104 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[20:23], v[180:183], v[128:131], a[20:23], v117, v104 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[16:19], v[176:179], v[128:131], a[16:19], v116, v104 op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "s_waitcnt vmcnt(4) lgkmcnt(0)\n\t" \
+  "s_barrier\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[0:3], v[224:227], v[192:195], a[0:3], v112, v104 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[240:243], v125 offset:8192\n\t" \
+  "s_add_u32 s81, s81, 128\n\t" \
+  "s_add_u32 s82, s82, 128\n\t" \
+  "s_xor_b32 s86, s86, 0x10000\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[4:7], v[228:231], v[192:195], a[4:7], v113, v104 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[244:247], v125 offset:10240\n\t" \
+  "s_add_u32 s87, s80, 2\n\t" \
+  "s_cmp_lt_u32 s87, %[n]\n\t" \
+  "s_cselect_b32 s84, 0, 0x80000000\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[8:11], v[232:235], v[192:195], a[8:11], v114, v104 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[248:251], v125 offset:12288\n\t" \
+  "s_add_u32 s87, s87, 1\n\t" \
+  "s_cmp_eq_u32 s87, %[n]\n\t" \
+  "s_cselect_b32 s85, 0x80000000, 0\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[12:15], v[236:239], v[192:195], a[12:15], v115, v104 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[252:255], v125 offset:14336\n\t" \
+  "v_and_b32 v122, s85, %[tail]\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[44:47], v[236:239], v[196:199], a[44:47], v115, v105 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_or3_b32 v120, s84, %[voa], v122\n\t" \
+  "v_or3_b32 v121, s84, %[vob], v122\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[40:43], v[232:235], v[196:199], a[40:43], v114, v105 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "s_mov_b32 s83, s81\n\t" \
+  "s_add_u32 m0, s86, 0\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[36:39], v[228:231], v[196:199], a[36:39], v113, v105 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[128:131], %[ra0] offset:0\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[32:35], v[224:227], v[196:199], a[32:35], v112, v105 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, s86, 4096\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[64:67], v[224:227], v[200:203], a[64:67], v112, v106 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_u16 v96, v127 offset:0\n\t" \
+  "ds_read_u16 v97, v127 offset:256\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[68:71], v[228:231], v[200:203], a[68:71], v113, v106 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[160:163], %[rb0] offset:0\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[72:75], v[232:235], v[200:203], a[72:75], v114, v106 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, s86, 16384\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[76:79], v[236:239], v[200:203], a[76:79], v115, v106 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_xor_b32 v124, 0x10000, v124\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[108:111], v[236:239], v[204:207], a[108:111], v115, v107 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[164:167], %[rb0] offset:2048\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[104:107], v[232:235], v[204:207], a[104:107], v114, v107 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gas]\n\t" \
+  "s_add_u32 m0, s86, 20480\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[100:103], v[228:231], v[204:207], a[100:103], v113, v107 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_u16 v98, v127 offset:512\n\t" \
+  "ds_read_u16 v99, v127 offset:768\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[96:99], v[224:227], v[204:207], a[96:99], v112, v107 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[168:171], %[rb0] offset:4096\n\t" \
+  "s_waitcnt lgkmcnt(11)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[112:115], v[240:243], v[204:207], a[112:115], v116, v107 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v120, %[rsa], s83 offen lds\n\t" \
+  "s_mov_b32 s83, s82\n\t" \
+  "s_add_u32 m0, s86, 32768\n\t" \
+  "s_waitcnt lgkmcnt(10)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[116:119], v[244:247], v[204:207], a[116:119], v117, v107 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "s_waitcnt lgkmcnt(9)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[120:123], v[248:251], v[204:207], a[120:123], v118, v107 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[172:175], %[rb0] offset:6144\n\t" \
+  "s_waitcnt lgkmcnt(9)\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[124:127], v[252:255], v[204:207], a[124:127], v119, v107 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 36864\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[92:95], v[252:255], v[200:203], a[92:95], v119, v106 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_u16 v100, v127 offset:1024\n\t" \
+  "ds_read_u16 v101, v127 offset:1280\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[88:91], v[248:251], v[200:203], a[88:91], v118, v106 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[132:135], %[ra0] offset:2048\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[84:87], v[244:247], v[200:203], a[84:87], v117, v106 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs3]\n\t" \
+  "s_add_u32 m0, s86, 49152\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[80:83], v[240:243], v[200:203], a[80:83], v116, v106 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_xor_b32 v125, 0x10000, v125\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[48:51], v[240:243], v[196:199], a[48:51], v116, v105 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[136:139], %[ra0] offset:4096\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[52:55], v[244:247], v[196:199], a[52:55], v117, v105 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  "s_add_u32 s83, s83, %[gbs]\n\t" \
+  "s_add_u32 m0, s86, 53248\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[56:59], v[248:251], v[196:199], a[56:59], v118, v105 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_u16 v102, v127 offset:1536\n\t" \
+  "ds_read_u16 v103, v127 offset:1792\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[60:63], v[252:255], v[196:199], a[60:63], v119, v105 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "ds_read_b128 v[140:143], %[ra0] offset:6144\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[28:31], v[252:255], v[192:195], a[28:31], v119, v104 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "buffer_load_dwordx4 v121, %[rsb], s83 offen lds\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[24:27], v[248:251], v[192:195], a[24:27], v118, v104 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[20:23], v[244:247], v[192:195], a[20:23], v117, v104 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "v_mfma_scale_f32_16x16x128_f8f6f4 a[16:19], v[240:243], v[192:195], a[16:19], v116, v104 op_sel:[1,1,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4\n\t" \
+  "s_add_u32 s80, s80, 1\n\t" \
+  "s_waitcnt vmcnt(8) lgkmcnt(0)\n\t" \
+  "s_barrier\n\t" \
+  "s_cmp_lt_u32 s80, %[n]\n\t" \
+  "s_cbranch_scc1 L_sk_loop%=\n\t" \
+  "L_sk_end%=:\n\t" \
+  "s_waitcnt vmcnt(0) lgkmcnt(0)\n\t" \
+  "s_nop 7\n\t" \
+  "s_nop 7\n\t" \
+  "s_nop 7\n\t" \
+  ""
 #define SK_TILE_ASM_CLOBBERS_MX \
   "a0", "a1", "a2", "a3", "a4", "a5", "a6", "a7", "a8", "a9", "a10", "a11", "a12", "a13", "a14", "a15", \
   "a16", "a17", "a18", "a19", "a20", "a21", "a22", "a23", "a24", "a25", "a26", "a27", "a28", "a29", "a30", "a31", \
