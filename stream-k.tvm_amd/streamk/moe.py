@@ -85,7 +85,8 @@ class StreamKMoE(torch.nn.Module):
         has NaN logits, which are never chosen: it goes to no expert and comes back as zeros."""
         T = x.shape[0]
         everyone = torch.arange(0, 2 * T, T, dtype=torch.int32, device=x.device)
-        return route_experts(streamk_grouped(x, self.router[None], everyone), self.chosen, bias=self.router_bias, **self.routing)
+        bias = self.router_bias.float() if self.router_bias is not None else None   # (the layer may have been cast)
+        return route_experts(streamk_grouped(x, self.router[None], everyone), self.chosen, bias=bias, **self.routing)
 
     def forward(self, x):
         if x.dtype != self.dtype or x.shape[-1] != self.hidden:

@@ -166,6 +166,9 @@ def test_routing_by_scores_trains(sk, dtype):
     assert ((out.double() - want).norm() / want.norm()).item() <= 8 * u
     for a, b in ((x, X), (layer.router, R), (layer.up, U), (layer.down, D)):
         assert ((a.grad.double() - b.grad).norm() / b.grad.norm()).item() <= 16 * u
+    # a layer that is cast: the bias has been rounded, and is used
+    with torch.no_grad():
+        assert layer.to(TYPES[dtype]).route(x).experts.shape == (T, chosen) and layer.router_bias.dtype == TYPES[dtype]
     # a closed expert is not chosen
     layer.router_bias[3] = -math.inf
     with torch.no_grad():
