@@ -367,6 +367,28 @@ def test_another_stream_and_a_graph(sk, M, N, K):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("variant", VARIANTS)
+def test_rows_of_a_wider_result(sk, variant):
+    # columns 3 .. of rows of an odd pitch, in a product and by expert, with and without an end; what lies beside them stays
+    M, N, K = 300, 267, 640
+    a, sa, va = operand(M, K, 1)
+    b, sb, vb = operand((2, N), K, 2)
+    offsets = offsets_of([140, 160])
+    want, magnitudes = torch.cat([va[:140] @ vb[0].T, va[140:] @ vb[1].T]), torch.cat([va[:140].abs() @ vb[0].abs().T, va[140:].abs() @ vb[1].abs().T])
+    for out in ROUNDING:
+        wide = torch.full((M, N + 10), 7.0, dtype=out, device="cuda")
+        bias = torch.randn(2, N, generator=torch.Generator().manual_seed(3)).to(out).cuda()
+        sk.streamk_mxfp4(a, b[0], sa, sb[0], out=wide[:, 3:3 + N], variant=variant)
+        assert_near(wide[:140, 3:3 + N], want[:140], K, magnitudes[:140])
+        sk.streamk_grouped(a, b, offsets, scale_a=sa, scale_b=sb, out=wide[:, 3:3 + N], variant=variant)
+        assert_near(wide[:, 3:3 + N], want, K, magnitudes)
+        sk.streamk_grouped(a, b, offsets, scale_a=sa, scale_b=sb, out=wide[:, 3:3 + N], bias=bias, activation="relu", variant=variant)
+        pre = want + torch.cat([bias[0].double().expand(140, N), bias[1].double().expand(160, N)])
+        assert_near(wide[:, 3:3 + N], pre.clamp(min=0), K, magnitudes, pre)
+        assert (wide[:, :3] == 7).all() and (wide[:, 3 + N:] == 7).all()
+
+
+@pytest.mark.gpu
 def test_beyond_four_gigabytes(sk):
     # weights of 40 experts, 5.4e9 bytes, of which the first and the last have rows
     E, N, K, g = 40, 16384, 16384, torch.Generator("cuda").manual_seed(3)
