@@ -366,7 +366,17 @@ __device__ __forceinline__ int scan_experts(int *total, int E, int *word) {
 
 // One workgroup does it all.  A second launch takes 1 to 2 us more, more tokens than waves take turns: 16 tokens, 6 of 64 experts 5.5 us in
 // one and 7.3 in two, 64 tokens 10 and 7.8; by scores and groups, 8 of 256 experts, 12 tokens 11.5 and 11.7, 32 tokens 21 and 11.6.
-constexpr int FEW_TOKENS = 32, FEW_TOKENS_SCORED = 16, FEW_EXPERTS = 256, FEW_WAVES = 16;
+constexpr int MAX_SPAN = 32, FEW_TOKENS = 32, FEW_TOKENS_SCORED = 16, FEW_EXPERTS = 256, FEW_WAVES = 16;
+// the most experts that a lane has where the groups' lanes, whole ones, are no more than a wave's (launch_route_of) and experts are up to `most`
+constexpr int span_of(int most) {
+  int span = 1;
+  for (int groups = 1; groups <= MAX_GROUPS; ++groups)
+    for (int size = 1; groups * size <= most; ++size)
+      while (groups * ((size + span - 1) / span) > 64) span *= 2;
+  return span;
+}
+constexpr int FEW_SPAN = span_of(FEW_EXPERTS);   // (3 groups of 85 experts: 8 to a lane, where 256 experts without groups are 4)
+static_assert(FEW_SPAN == 8 && span_of(MAX_EXPERTS) <= MAX_SPAN, "instances of launch_route_of");
 
 template <int EL, int S, bool SCORED>
 __global__ __launch_bounds__(64 * FEW_WAVES) void route_few_kernel(RouteArgs a) {
@@ -515,7 +525,7 @@ int route_blocks(int64_t T, int64_t E, bool scored) {
 template <int EL, int S, bool SCORED>
 int launch_route(RouteArgs a, int blocks, hipStream_t s) {
   a.scores.lanes = (a.scores.size + S - 1) / S;
-  if constexpr (S <= FEW_EXPERTS / 64) {
+  if constexpr (S <= FEW_SPAN) {
     if (blocks == 0) {
       const size_t lds = sizeof(int) * (FEW_TOKENS * a.k + (FEW_WAVES + 1) * a.E + 1);
       hipLaunchKernelGGL((route_few_kernel<EL, S, SCORED>), dim3(1), dim3(64 * FEW_WAVES), lds, s, a);
@@ -535,7 +545,7 @@ int launch_route(RouteArgs a, int blocks, hipStream_t s) {
   hipLaunchKernelGGL(route_place_kernel<true>, dim3(blocks), dim3(64 * WAVES), lds, s, a);
   return (int)hipGetLastError();
 }
-// experts to a lane so that the groups' lanes, whole ones, are no more than a wave's (32 always do, for up to 64 groups and 1024 experts)
+// experts to a lane so that the groups' lanes, whole ones, are no more than a wave's (MAX_SPAN always do)
 bool fits_wave(const Scores &p, int S) { return p.groups * ((p.size + S - 1) / S) <= 64; }
 template <int EL, bool SCORED>
 int launch_route_of(const RouteArgs &a, int blocks, hipStream_t s) {
@@ -544,7 +554,7 @@ int launch_route_of(const RouteArgs &a, int blocks, hipStream_t s) {
     if (fits_wave(a.scores, 2)) return launch_route<EL, 2, true>(a, blocks, s);
     if (fits_wave(a.scores, 4)) return launch_route<EL, 4, true>(a, blocks, s);
     if (fits_wave(a.scores, 8)) return launch_route<EL, 8, true>(a, blocks, s);
-    return fits_wave(a.scores, 16) ? launch_route<EL, 16, true>(a, blocks, s) : launch_route<EL, 32, true>(a, blocks, s);
+    return fits_wave(a.scores, 16) ? launch_route<EL, 16, true>(a, blocks, s) : launch_route<EL, MAX_SPAN, true>(a, blocks, s);
   } else {
     if (a.E <= 64) return launch_route<EL, 1, false>(a, blocks, s);
     if (a.E <= 128) return launch_route<EL, 2, false>(a, blocks, s);

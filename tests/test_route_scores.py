@@ -106,6 +106,27 @@ def test_route_by_scores(sk, scores, with_bias, T, E, k, groups, chosen_groups):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("T", [1, 7, 16])
+@pytest.mark.parametrize("E,groups", [(250, 10), (240, 40), (252, 12), (255, 3)])
+def test_few_tokens_in_groups_that_leave_lanes_unused(sk, E, groups, T, scores):
+    z, bias = logits_of(T, E, 7 * T + E, closed=0.3), bias_of(E, E)
+    for how in (dict(bias=None, renormalize=False), dict(bias=bias, renormalize=True, scale=2.5)):
+        how.update(scores=scores, groups=groups, chosen_groups=groups // 2)
+        assert_route(sk.route_experts(z, 5, **how), plain_route(z, 5, **how))
+
+
+@pytest.mark.gpu
+def test_few_tokens_in_groups_of_any_size(sk):
+    """Every pair of groups and experts that one workgroup routes with more experts to a lane than 256 without groups have."""
+    pairs = [(groups * size, groups) for groups in range(2, 65) for size in range(1, 256 // groups + 1) if groups * -(-size // 4) > 64]
+    assert len(pairs) == 69
+    for E, groups in pairs:
+        z, how = logits_of(2, E, E + groups), dict(scores="sigmoid", bias=bias_of(E, groups), groups=groups, chosen_groups=groups - 1, scale=2.5)
+        assert_route(sk.route_experts(z, 6, **how), plain_route(z, 6, **how))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
 def test_equal_scores_go_by_number(sk, dtype, scores):
