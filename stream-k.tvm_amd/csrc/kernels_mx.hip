@@ -110,7 +110,7 @@ int mx_variant(const GroupedShape &h) {
   int best = 0;
   double least = 0;
   for (const MxCost &c : COSTS) {
-    if (c.variant == GV_ASM256 && !mx_tiled_fits(h)) continue;
+    if (takes_tiled(h.K, c.variant) && !mx_tiled_fits(h)) continue;   // (64 x 64 and smaller tiles take any size)
     const double t = estimate(h, experts, c);
     if (best == 0 || t < least) {
       least = t;

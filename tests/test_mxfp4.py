@@ -421,6 +421,31 @@ def test_beyond_four_gigabytes(sk):
 
 
 @pytest.mark.gpu
+def test_the_tiles_that_the_sizes_ask_for_take_them(sk):
+    """Exponents that would be beyond 2 GiB as some tiles want them: others run."""
+    from streamk import _lib
+    L, asked = _lib.lib(), 0
+    for E, N, K, R in itertools.product((1, 8, 256), (64, 16384, 1 << 21), (32, 160, 4096, 4128, 16384, 16416), (1, 100, 3000, 100000, 1 << 24)):
+        if E * N * K > 1 << 38 or R * K > 1 << 38 or R * N > 1 << 36:
+            continue
+        g = _lib.SkGrouped(dtype=_lib.SK_MXFP4, layout=_lib.LAYOUT_NT, out_dtype=_lib.SK_F16, activation=0, E=E, R=R, N=N, K=K, lda=K, ldb=K, ldc=N,
+                           expert_b=N * K if E > 1 else 0)
+        assert L.sk_grouped_workspace_bytes(ctypes.byref(g)) > 0, (E, N, K, R)
+        g.scales_tiled = L.sk_mx_scales_tiled(ctypes.byref(g))
+        asked += g.scales_tiled
+        assert L.sk_grouped_workspace_bytes(ctypes.byref(g)) > 0, (E, N, K, R)
+    assert asked > 10
+    E, N, K, gen = 8, 15 << 17, 4128, torch.Generator("cuda").manual_seed(4)
+    b = torch.empty(E, N, K // 2, dtype=torch.uint8, device="cuda").random_(generator=gen)
+    sb = torch.randint(120, 127, (E, N, K // 32), dtype=torch.uint8, device="cuda", generator=gen)
+    a, sa, va = operand(200 * E, K, 11)
+    C = sk.streamk_grouped(a, b, offsets_of([200] * E), scale_a=sa, scale_b=sb, out_dtype=torch.bfloat16)
+    for e, n in ((0, slice(0, 50)), (E - 1, slice(N - 50, N))):
+        r, vb = slice(200 * e, 200 * e + 200), values(b[e, n], sb[e, n]).cuda()
+        assert_near(C[r, n], va[r] @ vb.T, K, va[r].abs() @ vb.abs().T)
+
+
+@pytest.mark.gpu
 def test_wrong_operands_are_refused(sk):
     a, sa, _ = operand(6, 64, 1)
     b, sb, _ = operand((3, 40), 64, 2)
