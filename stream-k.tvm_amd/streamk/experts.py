@@ -142,12 +142,15 @@ def _mx_product(A, B, offsets, scale_a, scale_b, out_dtype, bias, activation, va
                        K=K, A=A.data_ptr(), B=B.data_ptr(), offsets=offsets.data_ptr() if not dense else None, C=C.data_ptr(), lda=2 * _pitch(A),
                        ldb=2 * (B.stride(-2) if N > 1 else K // 2), ldc=max(C.stride(0), N), expert_b=2 * B.stride(0) if E > 1 else 0,
                        bias=bias.data_ptr() if bias is not None else None, scale_a=scale_a.data_ptr(), scale_b=scale_b.data_ptr(), variant=variant)
-    if _lib.lib().sk_mx_scales_tiled(ctypes.byref(g)) or scale_a.data_ptr() % 4 or scale_b.data_ptr() % 4:
+    if _lib.lib().sk_mx_scales_tiled(ctypes.byref(g)):
         width = (K + 511) // 512 * 16
         tiled_a, tiled_b = (torch.empty(t.numel() // (K // 32) * width, dtype=torch.uint8, device=A.device) for t in (scale_a, scale_b))
         _lib.check(_lib.lib().sk_tile_mx_scales(scale_a.data_ptr(), R, tiled_a.data_ptr(), scale_b.data_ptr(), E * N, tiled_b.data_ptr(), K // 32, ops._stream_ptr()),
                    "sk_tile_mx_scales")
         g.scale_a, g.scale_b, g.scales_tiled = tiled_a.data_ptr(), tiled_b.data_ptr(), 1
+    else:   # (views that begin inside a word)
+        scale_a, scale_b = (t.clone() if t.data_ptr() % 4 else t for t in (scale_a, scale_b))
+        g.scale_a, g.scale_b = scale_a.data_ptr(), scale_b.data_ptr()
     ws = ops._workspace(_lib.lib().sk_grouped_workspace_bytes(ctypes.byref(g)), A.device)
     _lib.check(_lib.lib().sk_gemm_grouped(ctypes.byref(g), ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
                                           ops._stream_ptr()), "sk_gemm_grouped")

@@ -446,6 +446,20 @@ def test_the_tiles_that_the_sizes_ask_for_take_them(sk):
 
 
 @pytest.mark.gpu
+def test_exponents_that_begin_inside_a_word(sk):
+    for M, N, K in ((5, 40, 96), (300, 520, 4128), (600, 2000, 2048), ((1 << 27) + 3, 8, 32)):   # (the last: more rows than exponents are laid out anew for)
+        gen = torch.Generator("cuda").manual_seed(M)
+        a = torch.empty(M, K // 2, dtype=torch.uint8, device="cuda").random_(generator=gen)
+        b, sb, vb = operand(N, K, 13)
+        sa = torch.randint(120, 127, (M * (K // 32) + 1,), dtype=torch.uint8, device="cuda", generator=gen)[1:].view(M, K // 32)
+        assert sa.data_ptr() % 4 == 1
+        C = sk.streamk_mxfp4(a, b, sa, sb, out_dtype=torch.bfloat16)
+        for r in (slice(0, 5), slice(M - 5, M)):
+            va = values(a[r], sa[r]).cuda()
+            assert_near(C[r], va @ vb.T, K, va.abs() @ vb.abs().T)
+
+
+@pytest.mark.gpu
 def test_wrong_operands_are_refused(sk):
     a, sa, _ = operand(6, 64, 1)
     b, sb, _ = operand((3, 40), 64, 2)
