@@ -12,10 +12,15 @@ struct Cuts {
   int whole, parts;
   __device__ __forceinline__ Cuts(int tiles, int grid, int ipt) {
     const int rest = (int)((unsigned)tiles % (unsigned)grid);
-    parts = ipt < CUT_LEAST || rest == 0 ? 1 : (rest * 4 <= grid ? 4 : (rest * 2 <= grid ? 2 : 1));
+    parts = parts_of(rest, grid, ipt);
     whole = parts > 1 ? tiles - rest : tiles;
   }
   static constexpr int CUT_LEAST = 32;   // iterations of a tile from which the exchange, some 20 us, pays
+  // (the rule of kernels_mx.hip counts on the same parts)
+  template <class Int>
+  static __host__ __device__ __forceinline__ constexpr int parts_of(Int rest, int grid, Int ipt) {
+    return ipt < CUT_LEAST || rest == 0 ? 1 : (rest * 4 <= grid ? 4 : (rest * 2 <= grid ? 2 : 1));
+  }
 };
 
 // The end of a part of a cut tile.  Each CTA of the tile takes a ticket; all but the last put their sums into the workspace and raise a

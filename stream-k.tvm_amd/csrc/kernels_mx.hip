@@ -2,6 +2,7 @@
 // or of one matrix.
 #include <cmath>
 
+#include "grouped_cut.h"
 #include "grouped_launch.h"
 #include "grouped_mx.h"
 #include "kernel_table.h"
@@ -58,7 +59,7 @@ static bool takes_tiled(int64_t K, int variant) {
 // The tile with the least estimated time, for rows that fall on the experts by chance.
 //     time = start + max(busy, memory) + hidden min(busy, memory), and where exponents are tiled 3.5 us and their bytes twice at 4 TB/s
 //   busy    iterations of `bk` values of the CU that has most -- whole rounds of tiles, and of those that are left their share and `cut`, or
-//           whole tiles where that is less (256 x 256: halves or quarters) -- each of `alone` or, of `per_cu` tiles at a time, `shared`, and more
+//           whole tiles where that is less (256 x 256: what Cuts takes) -- each of `alone` or, of `per_cu` tiles at a time, `shared`, and more
 //           by `astray` where rows do not begin at 128 bytes (at 64: half of it), so that a chunk's are in two lines;
 //           `end` for a tile's beginning and end, `join` for a cut
 //   memory  the operands of the experts that have rows, and C, once at 6 TB/s
@@ -89,7 +90,7 @@ static double estimate(const GroupedShape &h, double experts, const MxCost &c) {
   double iters = whole * ipt, at_once = whole > 0 ? c.per_cu : ceil(rest / h.cus);
   bool joined = false;
   if (rest > 0 && c.variant == GV_ASM256) {
-    const int parts = ipt < 64 ? 1 : (4 * rest <= h.cus ? 4 : (2 * rest <= h.cus ? 2 : 1));
+    const int parts = Cuts::parts_of((int64_t)rest, h.cus, (int64_t)ipt);
     joined = parts > 1;
     iters += ipt / parts;
   } else if (rest > 0) {

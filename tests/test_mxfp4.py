@@ -446,6 +446,22 @@ def test_the_tiles_that_the_sizes_ask_for_take_them(sk):
 
 
 @pytest.mark.gpu
+def test_the_choice_of_tiles_counts_on_the_cuts_that_are_made(sk):
+    """256 x 256 tiles that whole rounds leave are cut along K from 8192 on: 6 x 14 tiles in two, which take less time than tiles of 128 x 256
+    (68 and 71 to 76 us), where whole ones would take more.  With a K that is a multiple of 128 they alone want exponents tiled, which says
+    that they are chosen."""
+    from streamk import _lib
+    if torch.cuda.get_device_properties(0).multi_processor_count != 256:
+        pytest.skip("tiles of 256 CUs")
+    R, N, K = 1431, 3492, 14080
+    asks = []
+    for variant in (0, 2, 7):
+        g = _lib.SkGrouped(dtype=_lib.SK_MXFP4, layout=_lib.LAYOUT_NT, out_dtype=_lib.SK_F16, activation=0, E=1, R=R, N=N, K=K, lda=K, ldb=K, ldc=N, variant=variant)
+        asks.append(_lib.lib().sk_mx_scales_tiled(ctypes.byref(g)))
+    assert asks == [1, 1, 0]
+
+
+@pytest.mark.gpu
 def test_exponents_that_begin_inside_a_word(sk):
     for M, N, K in ((5, 40, 96), (300, 520, 4128), (600, 2000, 2048), ((1 << 27) + 3, 8, 32)):   # (the last: more rows than exponents are laid out anew for)
         gen = torch.Generator("cuda").manual_seed(M)
