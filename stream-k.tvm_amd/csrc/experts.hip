@@ -364,9 +364,10 @@ __device__ __forceinline__ int scan_experts(int *total, int E, int *word) {
   return *word;
 }
 
-// One workgroup does it all.  A second launch takes 1 to 2 us more, more tokens than waves take turns: 16 tokens, 6 of 64 experts 5.5 us in
-// one and 7.3 in two, 64 tokens 10 and 7.8; by scores and groups, 8 of 256 experts, 12 tokens 11.5 and 11.7, 32 tokens 21 and 11.6.
-constexpr int MAX_SPAN = 32, FEW_TOKENS = 32, FEW_TOKENS_SCORED = 16, FEW_EXPERTS = 256, FEW_WAVES = 16;
+// One workgroup does it all.  A second launch takes 1 to 2 us more, more tokens than waves take turns of k reductions each: 56 tokens, 2 of 8
+// experts 6.1 us in one and 6.3 in two, 64 tokens 6.7 and 6.5, 32 tokens, 6 of 64, 6.6 and 7.0, 40 tokens 7.2 and 6.8, 8 of 64, 24 tokens 6.6 and
+// 7.0, 32 tokens 7.0 and 6.6; by scores and groups, 8 of 256 experts, 12 tokens 11.5 and 11.7, 32 tokens 21 and 11.6.
+constexpr int MAX_SPAN = 32, FEW_TOKENS = 64, FEW_EXPERTS = 256, FEW_WAVES = 16;
 // the most experts that a lane has where the groups' lanes, whole ones, are no more than a wave's (launch_route_of) and experts are up to `most`
 constexpr int span_of(int most) {
   int span = 1;
@@ -473,6 +474,10 @@ __global__ __launch_bounds__(64 * SCAN_EXPERTS) void route_scan_kernel(int *coun
     before += c[j];
   }
 }
+// threads to an expert where a block adds up the counts of all blocks by itself, and the blocks up to which that is less than the scan: 512
+// tokens, 2 of 8 experts 6.5 us, with it 8.5, 8 of 64 experts 8.2 and 9.9; by scores, 8 of 256 experts, 256 tokens in 64 blocks 13.9 and 14.3
+constexpr int shares_of(int E) { return E < 64 * WAVES ? 64 * WAVES / E : 1; }
+constexpr int unscanned_blocks(int E) { return shares_of(E) > 2 ? 32 * shares_of(E) : 64; }
 // SCANNED: the kernel above has run; of a few blocks every block adds up the counts by itself
 template <bool SCANNED>
 __global__ __launch_bounds__(64 * WAVES) void route_place_kernel(RouteArgs a) {
@@ -480,21 +485,39 @@ __global__ __launch_bounds__(64 * WAVES) void route_place_kernel(RouteArgs a) {
   int *have = lds, *total = have + WAVES * a.E, *front = total + a.E, *word = front + a.E;
   const int t0 = blockIdx.x * a.tokens, t1 = min(a.T, t0 + a.tokens), slot0 = t0 * a.k, n = (t1 - t0) * a.k;
   const int *experts = a.experts + slot0;
-  for (int e = threadIdx.x; e < a.E; e += 64 * WAVES) {
-    int sum = 0, before = 0;
-    if constexpr (SCANNED) {
-      sum = a.totals[e];
-      before = a.counts[(int64_t)blockIdx.x * a.E + e];
-    } else {
-#pragma unroll 8
-      for (int b = 0; b < (int)gridDim.x; ++b) {
-        const int c = a.counts[(int64_t)b * a.E + e];
-        sum += c;
-        before += b < (int)blockIdx.x ? c : 0;
+  // (eight counts are on their way together)
+  const int blocks = (int)gridDim.x, shares = SCANNED || blocks <= 8 ? 1 : shares_of(a.E), step = 8 * shares;
+  if (SCANNED || shares > 1)
+    for (int e = threadIdx.x; e < a.E; e += 64 * WAVES) {
+      total[e] = SCANNED ? a.totals[e] : 0;
+      front[e] = SCANNED ? a.counts[(int64_t)blockIdx.x * a.E + e] : 0;
+    }
+  if constexpr (!SCANNED) {
+    if (shares > 1) __syncthreads();   // (uniform)
+    for (int i = threadIdx.x; i < shares * a.E; i += 64 * WAVES) {
+      const int share = (int)((unsigned)i / (unsigned)a.E), e = i - share * a.E;
+      int sum = 0, before = 0;
+      auto eight = [&](auto all, int b0) {
+        int c[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) c[j] = decltype(all)::value || b0 + j * shares < blocks ? a.counts[(b0 + j * shares) * a.E + e] : 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          sum += c[j];
+          before += b0 + j * shares < (int)blockIdx.x ? c[j] : 0;
+        }
+      };
+      int b0 = share;
+      for (; b0 + 7 * shares < blocks; b0 += step) eight(std::true_type{}, b0);
+      if (b0 < blocks) eight(std::false_type{}, b0);
+      if (shares == 1) {
+        total[e] = sum;
+        front[e] = before;
+      } else {   // (sums of whole numbers, whose order does not matter)
+        atomicAdd(&total[e], sum);
+        atomicAdd(&front[e], before);
       }
     }
-    total[e] = sum;
-    front[e] = before;
   }
   count_parts<WAVES>(experts, n, a.E, have);
   const int used = scan_experts(total, a.E, word);
@@ -513,13 +536,16 @@ __global__ __launch_bounds__(64 * WAVES) void route_place_kernel(RouteArgs a) {
   place_slots<WAVES>(a, experts, slot0, n, have);
 }
 
-constexpr int UNSCANNED_BLOCKS = 64;   // (8 of 256 experts, 128 tokens in 32 blocks: 10.7 us, with the scan 12.3; 256 tokens in 64: 12.1 and 12.4)
-int route_tokens(int64_t T) {
-  const int64_t tokens = (T + MOST_BLOCKS - 1) / MOST_BLOCKS;
-  return tokens < 4 ? 4 : (int)tokens;
+// tokens of a block (256 tokens, 8 of 64 experts, four to a block 8.1 us, eight 7.5; by scores, 128 tokens, 8 of 256, 12.5 and 13.0)
+int route_tokens(int64_t T, bool scored) {
+  const int64_t tokens = (T + MOST_BLOCKS - 1) / MOST_BLOCKS, least = scored ? 4 : 8;
+  return (int)(tokens < least ? least : tokens);
 }
-int route_blocks(int64_t T, int64_t E, bool scored) {
-  return T <= (scored ? FEW_TOKENS_SCORED : FEW_TOKENS) && E <= FEW_EXPERTS ? 0 : (int)((T + route_tokens(T) - 1) / route_tokens(T));
+bool few_tokens(int64_t T, int64_t E, int64_t k, bool scored) {
+  return E <= FEW_EXPERTS && (T <= FEW_WAVES || (!scored && T <= FEW_TOKENS && T * (k + 2) <= 256));
+}
+int route_blocks(int64_t T, int64_t E, int64_t k, bool scored) {
+  return few_tokens(T, E, k, scored) ? 0 : (int)((T + route_tokens(T, scored) - 1) / route_tokens(T, scored));
 }
 
 template <int EL, int S, bool SCORED>
@@ -536,7 +562,7 @@ int launch_route(RouteArgs a, int blocks, hipStream_t s) {
   hipLaunchKernelGGL((route_choose_kernel<EL, S, SCORED>), dim3(blocks), dim3(64 * waves), sizeof(int) * a.E, s, a);
   if (hipGetLastError() != hipSuccess) return 1;
   const size_t lds = sizeof(int) * ((WAVES + 2) * a.E + 1);
-  if (blocks <= UNSCANNED_BLOCKS) {
+  if (blocks <= unscanned_blocks(a.E)) {
     hipLaunchKernelGGL(route_place_kernel<false>, dim3(blocks), dim3(64 * WAVES), lds, s, a);
     return (int)hipGetLastError();
   }
@@ -833,7 +859,7 @@ int launched() { return hipGetLastError() == hipSuccess ? SK_OK : SK_ERR_LAUNCH;
 
 extern "C" size_t sk_route_workspace_bytes(int64_t T, int64_t E, int64_t k) {
   if (check_route_shape(T, E, k) != SK_OK) return 0;
-  const int blocks = route_blocks(T, E, true);   // (whichever takes more)
+  const int blocks = route_blocks(T, E, k, true);   // (whichever takes more)
   return blocks > 0 ? sizeof(int) * (size_t)(blocks + 1) * (size_t)E : 0;
 }
 
@@ -844,11 +870,11 @@ static int route(const void *logits, int dtype, int64_t T, int64_t E, int64_t k,
   if (int rc = check_route_shape(T, E, k)) return rc;
   if (!logits || !weights || !experts || !offsets || !order || !place) return SK_ERR_NULL;
   if (ld < E) return SK_ERR_SHAPE;
-  const int blocks = route_blocks(T, E, p != nullptr);
+  const int blocks = route_blocks(T, E, k, p != nullptr);
   if (ws_bytes < sk_route_workspace_bytes(T, E, k) || (blocks > 0 && !ws)) return SK_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(ws) & 3) return SK_ERR_ALIGN;
   RouteArgs a{logits, ld, (int)T, (int)E, (int)k, (float *)weights, (int *)experts, (int *)offsets, (int *)order, (int *)place, (int *)ws,
-              (int *)ws + (int64_t)blocks * E, route_tokens(T), p ? *p : Scores{nullptr, 1., 1, 1, (int)E, 1, false, true}};
+              (int *)ws + (int64_t)blocks * E, route_tokens(T, p != nullptr), p ? *p : Scores{nullptr, 1., 1, 1, (int)E, 1, false, true}};
   const int herr = p ? launch_route_by<true>(element_of(dtype), a, blocks, (hipStream_t)stream) : launch_route_by<false>(element_of(dtype), a, blocks, (hipStream_t)stream);
   return herr == 0 ? SK_OK : SK_ERR_LAUNCH;
 }

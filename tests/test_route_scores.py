@@ -127,6 +127,19 @@ def test_few_tokens_in_groups_of_any_size(sk):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("scores", [None, "sigmoid"])
+@pytest.mark.parametrize("E,k,sizes", [(1, 1, (64, 65, 300, 2051)), (3, 2, (33, 64, 65, 700, 2049)), (8, 2, (56, 65, 511, 2050, 4100)), (60, 3, (51, 52, 520, 1030, 2056)),
+                                       (100, 5, (37, 513, 520)), (129, 6, (33, 257, 520)), (256, 8, (25, 26, 259, 600)), (300, 4, (1, 9, 520))])
+def test_counts_of_every_number_of_blocks(sk, E, k, sizes, scores):
+    for T in sizes:
+        z = logits_of(T, E, T + E, closed=0.2)
+        how = dict() if scores is None else dict(scores=scores, bias=bias_of(E, T))
+        got, want = sk.route_experts(z, k, **how), plain_route(z, k, **how)
+        for a, b in zip(got[1:], want[1:]):   # (the weights do not come from counts)
+            assert torch.equal(a.cpu().long(), b)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
 def test_equal_scores_go_by_number(sk, dtype, scores):
