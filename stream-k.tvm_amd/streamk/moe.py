@@ -10,6 +10,7 @@ records applies it as an operation of its own.  int8 weights have a scale for ea
 quantised before they are laid out (a token's row and scales once, not once for each of its experts) and the hidden rows after the activation.
 """
 import math
+import warnings
 
 import torch
 
@@ -27,7 +28,9 @@ class StreamKMoE(torch.nn.Module):
     `dtype` (float16 or bfloat16; weight_format 'float16' and 'bfloat16' say it themselves, 'int8' and 'mxfp4' take float16 by default).
 
     scores, groups, chosen_groups, renormalize, scale: as route_experts takes them.  balance: the layer has a buffer `router_bias` (float32
-    [experts], zeros at first) that experts are chosen by beside their scores; who balances their load sets it."""
+    [experts], zeros at first) that experts are chosen by beside their scores; who balances their load sets it.  A cast of the layer rounds
+    it as it does any buffer, with a warning: in bfloat16 steps of a thousandth vanish from a half on.  The rule's own float32 sum, copied
+    into the buffer after each step, loses none; `layer.router_bias = layer.router_bias.float()` makes the buffer float32 again."""
 
     def __init__(self, hidden, intermediate, experts, chosen, *, activation="silu", weight_format="bfloat16", dtype=None, device=None, scores="softmax",
                  balance=False, groups=1, chosen_groups=1, renormalize=True, scale=1.0):
@@ -77,6 +80,13 @@ class StreamKMoE(torch.nn.Module):
             getattr(m, name).copy_(q)
             getattr(m, name + "_scale").copy_(scale)
         return m
+
+    def _apply(self, fn, *args, **kwargs):
+        before = self.router_bias
+        super()._apply(fn, *args, **kwargs)
+        if before is not None and self.router_bias.dtype != before.dtype and self.router_bias.dtype in (torch.float16, torch.bfloat16):
+            warnings.warn(f"StreamKMoE: router_bias has been rounded to {self.router_bias.dtype}; small steps added to it there are lost", stacklevel=3)
+        return self
 
     def route(self, x):
         """The route of x [T, hidden].  The router's product is one group of all rows.  Its logits come in x's type, as those of a linear

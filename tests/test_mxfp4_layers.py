@@ -202,3 +202,35 @@ def test_refusals(sk):
     with pytest.raises(ValueError):
         sk.StreamKMoE.quantized(sk.StreamKMoE(64, 64, 4, 2, weight_format="int8"), "mxfp4")
     assert "scores=sigmoid" in repr(sk.StreamKMoE(64, 64, 4, 2, scores="sigmoid"))
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_the_balance_bias_of_a_layer_that_is_cast(sk, dtype):
+    """A cast that rounds the bias says so; the rule in float32 arrives, to a unit roundoff, where steps added in 16 bits would not."""
+    import warnings
+    layer = sk.StreamKMoE(64, 64, 8, 2, weight_format=dtype, **ROUTED)
+    bias = torch.linspace(-1, 1, 8)
+    layer.router_bias.copy_(bias)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        layer.to("cpu")
+        layer.float()
+    assert torch.equal(layer.router_bias, bias)
+    with pytest.warns(UserWarning, match="router_bias"):
+        torch.nn.Sequential(layer).to(TYPES[dtype])
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        layer.to(TYPES[dtype])
+        sk.StreamKMoE(64, 64, 8, 2, weight_format=dtype).to(TYPES[dtype])   # (none to lose)
+    alone = layer.router_bias.clone()
+    for _ in range(1000):
+        bias += 0.001
+        alone += 0.001
+        layer.router_bias.copy_(bias)
+    want = torch.linspace(-1, 1, 8) + 1
+    # (1000 float32 sums, and 0.001 in float32)
+    assert ((layer.router_bias.double() - want.double()).abs() <= ROUNDOFF[TYPES[dtype]] * want.double() * 1.001 + 1000 * 2.0 ** -23).all()
+    if dtype == "bfloat16":
+        assert alone[-1] == 1   # 0.001 is less than half of the 2^-7 from 1 on
+    layer.router_bias = layer.router_bias.float()
+    assert layer.router_bias.dtype == torch.float32 and "router_bias" in layer.state_dict()
